@@ -259,6 +259,113 @@ int ts_lora_delta_batch(ts_ctx* ctx, const ts_sk* sk, const ts_lora* lora, const
 int ts_dp_noise(ts_ctx* ctx, double* h, uint32_t n, uint32_t d, double clip, double sigma, const uint64_t* seeds,
                 int on_device);
 
+/* ------------------------------------------------------------ decode step, plaintext
+ * Operators of the surrounding decode step on device tensors that belong to
+ * the host's framework: low-rank adapters of many requests beside a shared
+ * projection (the plaintext branch of _he_lora_delta,
+ * inference_engine.py:1234-1242, at every projection and for any number of
+ * requests), their gradients, and the rules applied to next-token logits.
+ *
+ * They need no context.  Every pointer is device memory on `device`; the
+ * work is queued on `stream` (a cudaStream_t of that device; NULL is the
+ * legacy default stream) and the call returns without waiting, allocating or
+ * touching state of its own, so that it can be captured in a CUDA graph.  The
+ * calling thread's current device is left as it was.  Strides count
+ * elements between rows; a row's elements are contiguous.  Nothing that the
+ * call writes may overlap what it reads, `base` excepted, which may be `out`
+ * itself.  Calls that may run at the same time need workspaces of their own. */
+#define TS_DTYPE_F32 0
+#define TS_DTYPE_BF16 1
+#define TS_DTYPE_F16 2
+
+#define TS_ADAPTER_MAX_RANK 256
+
+typedef struct ts_adapter_args {
+    int32_t dtype;           /* of x, weight, bias, base, lora_a, lora_b, grad and every result */
+    int32_t device;
+    void* stream;
+    uint64_t n;              /* tokens */
+    uint64_t tokens_per_id;  /* token m uses adapter[m / tokens_per_id] */
+    uint32_t d_in, d_out;
+    uint32_t r;              /* rank, 1 .. TS_ADAPTER_MAX_RANK */
+    uint32_t adapters;       /* 1 .. 65535 */
+    const void* x;           /* [n][d_in] */
+    int64_t x_stride;
+    const void* weight;      /* [d_out][d_in], or NULL: no shared projection */
+    int64_t weight_stride;
+    const void* bias;        /* [d_out], or NULL (forward only) */
+    const void* base;        /* [n][d_out], or NULL (forward only) */
+    int64_t base_stride;
+    const void* lora_a;      /* [adapters][r][d_in] */
+    const void* lora_b;      /* [adapters][d_out][r] */
+    const int32_t* adapter;  /* [ceil(n / tokens_per_id)]; outside [0, adapters): the token has none */
+    const float* scale;      /* [adapters], or NULL: 1 */
+    const void* grad;        /* [n][d_out]: gradient of out (backward only) */
+    int64_t grad_stride;
+    void* out;               /* forward [n][d_out]; backward [n][d_in]: gradient of x, or NULL */
+    int64_t out_stride;
+    void* grad_a;            /* [adapters][r][d_in] and [adapters][d_out][r] (backward only; both or neither) */
+    void* grad_b;
+    void* workspace;         /* ts_adapter_workspace bytes, 256-byte aligned; contents need not be kept */
+    uint64_t workspace_bytes;
+} ts_adapter_args;
+
+/* Bytes of workspace that the call below (backward: 0 or 1) needs with these
+ * sizes, strides and pointers (workspace itself need not be set). */
+int ts_adapter_workspace(const ts_adapter_args* args, int backward, uint64_t* bytes);
+/* out[m] = base[m] + x[m] weight^T + bias + scale_e (x[m] lora_a_e^T) lora_b_e^T,
+ * e = the token's adapter.  Sums are held in 32 bits; out is rounded once. */
+int ts_adapter_project(const ts_adapter_args* args);
+/* Gradients of the above for a gradient `grad` of out, weight, bias and scale
+ * held fixed: out[m] = grad[m] weight + u[m] lora_a_e with u[m] = scale_e
+ * grad[m] lora_b_e; grad_a_e = sum of u[m]^T x[m] and grad_b_e = scale_e sum
+ * of grad[m]^T (x[m] lora_a_e^T) over the adapter's tokens (zero without
+ * any), in an order fixed by the sizes alone.  The gradient of base is grad. */
+int ts_adapter_project_backward(const ts_adapter_args* args);
+
+#define TS_RULES_MAX_HISTORY 1048575
+#define TS_RULES_MAX_BIASES 4095
+
+typedef struct ts_rules_args {
+    int32_t dtype;               /* of logits */
+    int32_t out_dtype;           /* of out: dtype or TS_DTYPE_F32 */
+    int32_t device;
+    int32_t ids64;               /* tokens (bit 0) / bias_ids (bit 1) are int64, else int32 */
+    void* stream;
+    uint64_t n;                  /* rows */
+    uint32_t vocab;
+    uint32_t token_cols;         /* at most TS_RULES_MAX_HISTORY */
+    uint32_t bias_cols;          /* at most TS_RULES_MAX_BIASES */
+    uint32_t reserved;           /* 0 */
+    const void* logits;          /* [n][vocab] */
+    int64_t logits_stride;
+    const void* tokens;          /* [n][token_cols] history of ids (NULL: empty); ids outside [0, vocab) are skipped */
+    int64_t tokens_stride;
+    const int32_t* lengths;      /* [n] entries used, or NULL: token_cols */
+    const int32_t* prompt_lengths; /* [n] leading entries that are the prompt, or NULL: 0 */
+    const float* repetition;     /* [n], each NULL: no such penalty */
+    const float* frequency;
+    const float* presence;
+    const void* bias_ids;        /* [n][bias_cols], or NULL; ids outside [0, vocab) are skipped */
+    int64_t bias_ids_stride;     /* 0: one list for all rows */
+    const float* bias_values;    /* [n][bias_cols] */
+    int64_t bias_values_stride;
+    const int32_t* mask;         /* [n][ceil(vocab / 32)], bit v % 32 of word v / 32 set where v is allowed, or NULL */
+    int64_t mask_stride;         /* 0: one mask for all rows */
+    void* out;                   /* [n][vocab], may be logits itself (same type and stride), or NULL */
+    int64_t out_stride;
+    int64_t* pick;               /* [n], or NULL */
+} ts_rules_args;
+
+/* Per row, in 32 bits and in this order: tokens of the history have their
+ * logit divided by `repetition` where it is positive and multiplied by it
+ * elsewhere; tokens that occur c > 0 times behind the prompt part lose
+ * frequency * c, then presence; biases are added (of an id listed twice the
+ * last entry); masked tokens become -inf, whatever they were.  out gets the
+ * result rounded to its type, pick the lowest id of the greatest unrounded
+ * value (a NaN counts as greatest), or -1 where every value is -inf. */
+int ts_logit_rules(const ts_rules_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,11 @@ SIGNATURES = {
     "ts_lora_info": (cint, [vp, P(u32), P(u32), P(u32), P(u32), P(u32)]),
     "ts_lora_delta_batch": (cint, [vp, vp, vp, vp, u32, P(i32), P(i32), P(u64), vp, vp, cint]),
     "ts_dp_noise": (cint, [vp, vp, u32, u32, f64, f64, P(u64), cint]),
+    # argument blocks (ts_adapter_args, ts_rules_args) packed by struct.pack
+    "ts_adapter_workspace": (cint, [C.c_char_p, cint, P(u64)]),
+    "ts_adapter_project": (cint, [C.c_char_p]),
+    "ts_adapter_project_backward": (cint, [C.c_char_p]),
+    "ts_logit_rules": (cint, [C.c_char_p]),
 }
 
 

@@ -1,0 +1,278 @@
+// decode_ops.cu -- C entry points of the plaintext decode-step operators:
+// checks of the arguments, the layout of the workspace, the device, and the
+// launches.  Nothing here keeps state between calls.
+#include <cstring>
+
+#include "../../include/tsgpu.h"
+#include "lowrank.cuh"
+
+using namespace tsg;
+
+namespace tsg_host {
+int noalloc_fail(int code, const char* msg);  // tsgpu.cu: sets the thread's last error
+}
+
+namespace {
+
+int bad(const char* msg) { return tsg_host::noalloc_fail(TS_ERR_ARG, msg); }
+
+// Makes `device` current for a scope.
+struct OnDevice {
+    int before = -1;
+    cudaError_t status;
+    explicit OnDevice(int device) {
+        status = cudaGetDevice(&before);
+        if (status != cudaSuccess) return;
+        if (before == device)
+            before = -1;
+        else
+            status = cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+int cuda_status(cudaError_t e) {
+    if (e == cudaSuccess) return TS_OK;
+    const int code = e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? TS_ERR_NODEVICE : TS_ERR_CUDA;
+    cudaGetLastError();
+    return tsg_host::noalloc_fail(code, cudaGetErrorString(e));
+}
+
+// A matrix of `rows` rows of `row` bytes, `stride` bytes apart.
+struct Region {
+    uintptr_t p;
+    uint64_t rows, row, stride;
+    uint64_t bytes() const { return rows && p ? (rows - 1) * stride + row : 0; }
+};
+
+Region region(const void* p, uint64_t rows, uint64_t cols, int64_t stride, size_t size) {
+    return {reinterpret_cast<uintptr_t>(p), rows, cols * size, (uint64_t)stride * size};
+}
+
+bool overlap(const Region& a, const Region& b) {
+    if (!a.bytes() || !b.bytes() || a.p + a.bytes() <= b.p || b.p + b.bytes() <= a.p) return false;
+    if (a.stride != b.stride || !a.stride) return true;
+    // column ranges of one wider matrix
+    const uint64_t off = a.p <= b.p ? (b.p - a.p) % a.stride : (a.stride - (a.p - b.p) % a.stride) % a.stride;
+    return !(off >= a.row && off + b.row <= a.stride);
+}
+
+bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+constexpr uint64_t kMaxDim = 1u << 20, kMaxTokens = 1ull << 30, kMaxStride = 1ull << 40;
+
+bool stride_ok(int64_t s) { return s >= 0 && (uint64_t)s <= kMaxStride; }
+
+int check_adapter(const ts_adapter_args* a, int backward) {
+    if (!a) return bad("adapter arguments are NULL");
+    if (a->dtype < TS_DTYPE_F32 || a->dtype > TS_DTYPE_F16) return bad("unknown dtype");
+    if (a->d_in == 0 || a->d_in > kMaxDim || a->d_out == 0 || a->d_out > kMaxDim)
+        return bad("d_in and d_out must be in 1 .. 2^20");
+    if (a->r == 0 || a->r > TS_ADAPTER_MAX_RANK) return bad("the rank must be in 1 .. 256");
+    if (a->adapters == 0 || a->adapters > 65535) return bad("the number of adapters must be in 1 .. 65535");
+    if (a->n > kMaxTokens) return bad("at most 2^30 tokens in a call");
+    if (a->tokens_per_id == 0) return bad("tokens_per_id is 0");
+    const size_t size = dtype_size(a->dtype);
+    if (!stride_ok(a->x_stride) || !stride_ok(a->out_stride) || (a->weight && !stride_ok(a->weight_stride)) ||
+        (!backward && a->base && !stride_ok(a->base_stride)) || (backward && !stride_ok(a->grad_stride)))
+        return bad("a stride is negative or above 2^40");
+    if (backward) {
+        if (a->n && !a->out && !a->grad_a) return bad("no gradient is asked for");
+        if (!a->grad_a != !a->grad_b) return bad("grad_a and grad_b come together");
+        if (a->bias || a->base) return bad("bias and base have no place in the backward call");
+    } else if (a->grad || a->grad_a || a->grad_b) {
+        return bad("grad, grad_a and grad_b have no place in the forward call");
+    }
+    if (a->n && (!a->x || !a->lora_a || !a->lora_b || !a->adapter || (backward ? !a->grad : !a->out)))
+        return bad("a required pointer is NULL");
+    for (const void* p : {a->x, a->weight, a->bias, a->base, a->lora_a, a->lora_b, a->grad, (const void*)a->out,
+                          (const void*)a->grad_a, (const void*)a->grad_b})
+        if (!aligned_to(p, size)) return bad("a pointer is not aligned to its type");
+    if (!aligned_to(a->adapter, 4) || !aligned_to(a->scale, 4)) return bad("a pointer is not aligned to its type");
+    const uint64_t ids = a->n ? (a->n - 1) / a->tokens_per_id + 1 : 0;
+    const uint64_t wide = backward ? a->d_in : a->d_out;
+    if (a->out && a->n > 1 && (uint64_t)a->out_stride < wide) return bad("rows of out overlap");
+    const Region writes[] = {region(a->out, a->n, wide, a->out_stride, size),
+                             region(a->grad_a, 1, (uint64_t)a->adapters * a->r * a->d_in, 0, size),
+                             region(a->grad_b, 1, (uint64_t)a->adapters * a->r * a->d_out, 0, size),
+                             region(a->workspace, 1, a->workspace_bytes, 0, 1)};
+    const Region base = region(backward ? nullptr : a->base, a->n, a->d_out, a->base_stride, size);
+    const Region reads[] = {region(a->x, a->n, a->d_in, a->x_stride, size),
+                            region(a->weight, a->d_out, a->d_in, a->weight_stride, size),
+                            region(a->bias, 1, a->d_out, 0, size),
+                            region(a->lora_a, 1, (uint64_t)a->adapters * a->r * a->d_in, 0, size),
+                            region(a->lora_b, 1, (uint64_t)a->adapters * a->r * a->d_out, 0, size),
+                            region(a->grad, a->n, a->d_out, a->grad_stride, size),
+                            region(a->adapter, 1, ids, 0, 4), region(a->scale, 1, a->adapters, 0, 4), base};
+    for (const Region& w : writes) {
+        for (const Region& r : reads) {
+            const bool in_place = &w == writes && base.p && r.p == base.p && w.p == base.p && r.stride == w.stride && r.row == w.row &&
+                                  &r == reads + sizeof(reads) / sizeof(reads[0]) - 1;
+            if (!in_place && overlap(w, r)) return bad("what the call writes overlaps what it reads");
+        }
+        for (const Region& v : writes)
+            if (&v != &w && overlap(w, v)) return bad("two results, or a result and the workspace, overlap");
+    }
+    return TS_OK;
+}
+
+uint64_t up(uint64_t b) { return (b + 255) & ~255ull; }
+
+// Workspace: low [n][r] f32, and for the backward call u [n][r] f32.
+uint64_t adapter_bytes(const ts_adapter_args* a, int backward) { return up(a->n * a->r * 4) * (backward ? 2 : 1); }
+
+AdapterIds ids_of(const ts_adapter_args* a) { return {a->adapter, (long long)a->tokens_per_id, (int)a->adapters}; }
+
+int check_workspace(const ts_adapter_args* a, int backward) {
+    const uint64_t need = adapter_bytes(a, backward);
+    if (need && (!a->workspace || !aligned_to(a->workspace, 256) || a->workspace_bytes < need))
+        return bad("the workspace is missing, not 256-byte aligned or smaller than ts_adapter_workspace says");
+    return TS_OK;
+}
+
+int adapter_workspace(const ts_adapter_args* a, int backward, uint64_t* bytes) {
+    if (!bytes) return bad("bytes is NULL");
+    if (!a) return bad("adapter arguments are NULL");
+    ts_adapter_args b = *a;
+    b.workspace = nullptr;
+    b.workspace_bytes = 0;
+    const int rc = check_adapter(&b, backward);
+    if (rc) return rc;
+    *bytes = adapter_bytes(a, backward);
+    return TS_OK;
+}
+
+int adapter_project(const ts_adapter_args* a) {
+    int rc = check_adapter(a, 0);
+    if (rc || a->n == 0) return rc;
+    if ((rc = check_workspace(a, 0))) return rc;
+    OnDevice dev(a->device);
+    if (dev.status != cudaSuccess) return cuda_status(dev.status);
+    cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+    float* low = static_cast<float*>(a->workspace);
+    const long long ra = (long long)a->r * a->d_in, rb = (long long)a->r * a->d_out;
+    const LowArgs l{a->x, a->x_stride, (long long)a->n, (int)a->d_in, (int)a->r, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->scale, low};
+    cudaError_t e = launch_low(l, a->dtype, s);
+    if (e != cudaSuccess) return cuda_status(e);
+    const ProjectArgs p{a->x, a->x_stride, (long long)a->n, (int)a->d_in, (int)a->d_out, (int)a->r, a->weight, a->weight_stride, 1,
+                        a->bias, a->base, a->base_stride, low, {a->lora_b, rb, 1, a->r}, ids_of(a), a->out, a->out_stride};
+    return cuda_status(launch_project(p, a->dtype, s));
+}
+
+int adapter_project_backward(const ts_adapter_args* a) {
+    int rc = check_adapter(a, 1);
+    if (rc) return rc;
+    if ((rc = check_workspace(a, 1))) return rc;
+    OnDevice dev(a->device);
+    if (dev.status != cudaSuccess) return cuda_status(dev.status);
+    cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+    const long long n = (long long)a->n, ra = (long long)a->r * a->d_in, rb = (long long)a->r * a->d_out;
+    const size_t size = dtype_size(a->dtype);
+    if (n == 0) {
+        if (!a->grad_a) return TS_OK;
+        cudaError_t e = cudaMemsetAsync(a->grad_a, 0, (size_t)a->adapters * ra * size, s);
+        if (e == cudaSuccess) e = cudaMemsetAsync(a->grad_b, 0, (size_t)a->adapters * rb * size, s);
+        return cuda_status(e);
+    }
+    float* u = static_cast<float*>(a->workspace);
+    float* low = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + up(a->n * a->r * 4));
+    const LowArgs lu{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->r, {a->lora_b, rb, 1, a->r}, ids_of(a), a->scale, u};
+    cudaError_t e = launch_low(lu, a->dtype, s);
+    if (e == cudaSuccess && a->out) {
+        const ProjectArgs p{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->d_in, (int)a->r, a->weight, 1, a->weight_stride,
+                            nullptr, nullptr, 0, u, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->out, a->out_stride};
+        e = launch_project(p, a->dtype, s);
+    }
+    if (e == cudaSuccess && a->grad_a) {
+        const GradArgs ga{a->x, a->x_stride, n, (int)a->d_in, (int)a->r, u, ids_of(a), a->grad_a, ra, a->d_in, 1};
+        e = launch_grad(ga, a->dtype, s);
+        const LowArgs ll{a->x, a->x_stride, n, (int)a->d_in, (int)a->r, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->scale, low};
+        if (e == cudaSuccess) e = launch_low(ll, a->dtype, s);
+        const GradArgs gb{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->r, low, ids_of(a), a->grad_b, rb, 1, a->r};
+        if (e == cudaSuccess) e = launch_grad(gb, a->dtype, s);
+    }
+    return cuda_status(e);
+}
+
+int logit_rules(const ts_rules_args* a) {
+    if (!a) return bad("rules arguments are NULL");
+    if (a->dtype < TS_DTYPE_F32 || a->dtype > TS_DTYPE_F16) return bad("unknown dtype");
+    if (a->out && a->out_dtype != a->dtype && a->out_dtype != TS_DTYPE_F32) return bad("out_dtype must be dtype or f32");
+    if (a->reserved) return bad("reserved must be 0");
+    if (a->vocab == 0 || a->vocab > (1u << 30)) return bad("vocab must be in 1 .. 2^30");
+    if (a->n > 1u << 27) return bad("at most 2^27 rows in a call");
+    if (a->tokens && a->token_cols > TS_RULES_MAX_HISTORY) return bad("the history is longer than 1048575");
+    if (a->bias_ids && a->bias_cols > TS_RULES_MAX_BIASES) return bad("more than 4095 biases in a row");
+    if (!a->bias_ids != !a->bias_values) return bad("bias_ids and bias_values come together");
+    if (!a->tokens && a->token_cols) return bad("the history is NULL");
+    if (!stride_ok(a->logits_stride) || (a->out && !stride_ok(a->out_stride)) || (a->tokens && !stride_ok(a->tokens_stride)) ||
+        (a->bias_ids && (!stride_ok(a->bias_ids_stride) || !stride_ok(a->bias_values_stride))) ||
+        (a->mask && !stride_ok(a->mask_stride)))
+        return bad("a stride is negative or above 2^40");
+    if (a->n == 0) return TS_OK;
+    if (!a->out && !a->pick) return bad("neither out nor pick is asked for");
+    if (!a->logits) return bad("logits is NULL");
+    const size_t size = dtype_size(a->dtype), osize = dtype_size(a->out_dtype);
+    const size_t tsize = a->ids64 & 1 ? 8 : 4, bsize = a->ids64 & 2 ? 8 : 4;
+    if (!aligned_to(a->logits, size) || !aligned_to(a->out, osize) || !aligned_to(a->tokens, tsize) || !aligned_to(a->bias_ids, bsize) ||
+        !aligned_to(a->pick, 8))
+        return bad("a pointer is not aligned to its type");
+    for (const void* p : {(const void*)a->lengths, (const void*)a->prompt_lengths, (const void*)a->repetition, (const void*)a->frequency,
+                          (const void*)a->presence, (const void*)a->bias_values, (const void*)a->mask})
+        if (!aligned_to(p, 4)) return bad("a pointer is not aligned to its type");
+    if (a->out && a->n > 1 && (uint64_t)a->out_stride < a->vocab) return bad("rows of out overlap");
+    const Region logits = region(a->logits, a->n, a->vocab, a->logits_stride, size);
+    const Region out = region(a->out, a->n, a->vocab, a->out_stride, osize), pick = region(a->pick, 1, a->n, 0, 8);
+    const bool in_place = a->out == a->logits && a->dtype == a->out_dtype && a->out_stride == a->logits_stride;
+    const Region reads[] = {region(a->tokens, a->n, a->token_cols, a->tokens_stride, tsize),
+                            region(a->lengths, 1, a->n, 0, 4),
+                            region(a->prompt_lengths, 1, a->n, 0, 4),
+                            region(a->repetition, 1, a->n, 0, 4),
+                            region(a->frequency, 1, a->n, 0, 4),
+                            region(a->presence, 1, a->n, 0, 4),
+                            region(a->bias_ids, a->n, a->bias_cols, a->bias_ids_stride, bsize),
+                            region(a->bias_values, a->n, a->bias_cols, a->bias_values_stride, 4),
+                            region(a->mask, a->n, (a->vocab + 31) / 32, a->mask_stride, 4)};
+    for (const Region& r : reads)
+        if (overlap(out, r) || overlap(pick, r)) return bad("what the call writes overlaps what it reads");
+    if ((!in_place && overlap(out, logits)) || overlap(pick, logits) || overlap(out, pick))
+        return bad("what the call writes overlaps what it reads");
+    OnDevice dev(a->device);
+    if (dev.status != cudaSuccess) return cuda_status(dev.status);
+    const bool tokens = a->tokens && a->token_cols, biases = a->bias_ids && a->bias_cols;
+    const RulesArgs k{a->logits, a->logits_stride, (long long)a->n, a->vocab,
+                      tokens ? a->tokens : nullptr, a->tokens_stride, a->token_cols, a->ids64 & 1,
+                      a->lengths, a->prompt_lengths, a->repetition, a->frequency, a->presence,
+                      biases ? a->bias_ids : nullptr, a->bias_values, a->bias_ids_stride, a->bias_values_stride, a->bias_cols,
+                      a->ids64 >> 1 & 1, reinterpret_cast<const uint32_t*>(a->mask), a->mask_stride, a->out, a->out_stride,
+                      reinterpret_cast<long long*>(a->pick)};
+    return cuda_status(launch_rules(k, a->dtype, a->out ? a->out_dtype : a->dtype, static_cast<cudaStream_t>(a->stream)));
+}
+
+// No exception leaves a C entry point (the launch bookkeeping may fail to
+// allocate on the host).
+template <class F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (...) {
+        return TS_ERR_OOM;
+    }
+}
+
+}  // namespace
+
+extern "C" int ts_adapter_workspace(const ts_adapter_args* args, int backward, uint64_t* bytes) {
+    return guarded([&] { return adapter_workspace(args, backward, bytes); });
+}
+extern "C" int ts_adapter_project(const ts_adapter_args* args) {
+    return guarded([&] { return adapter_project(args); });
+}
+extern "C" int ts_adapter_project_backward(const ts_adapter_args* args) {
+    return guarded([&] { return adapter_project_backward(args); });
+}
+extern "C" int ts_logit_rules(const ts_rules_args* args) {
+    return guarded([&] { return logit_rules(args); });
+}
