@@ -98,6 +98,7 @@ SIGNATURES = {
     "ts_adapter_workspace": (cint, [C.c_char_p, cint, P(u64)]),
     "ts_adapter_project": (cint, [C.c_char_p]),
     "ts_adapter_project_backward": (cint, [C.c_char_p]),
+    "ts_expired_waits": (cint, [cint, P(u64)]),
     "ts_logit_rules": (cint, [C.c_char_p]),
 }
 

@@ -19,8 +19,9 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtsgpu.so")
 SOURCES = ["kernels.cu", "k_ntt.cu", "k_encode.cu", "k_encrypt.cu", "k_decrypt.cu", "tsgpu.cu", "noalloc.cu",
-           "k_lowrank.cu", "k_rules.cu", "decode_ops.cu"]
-HEADERS = ["common.cuh", "ntt.cuh", "fft.cuh", "kernels.cuh", "launch.cuh", "lowrank.cuh"]
+           "k_lowrank.cu", "k_project.cu", "k_rules.cu", "decode_ops.cu"]
+HEADERS = ["common.cuh", "ntt.cuh", "fft.cuh", "kernels.cuh", "launch.cuh", "lowrank.cuh",
+           "sm100.cuh"]
 
 
 def nvcc_path() -> str:

@@ -120,13 +120,71 @@ int check_adapter(const ts_adapter_args* a, int backward) {
 
 uint64_t up(uint64_t b) { return (b + 255) & ~255ull; }
 
-// Workspace: low [n][r] f32, and for the backward call u [n][r] f32.
-uint64_t adapter_bytes(const ts_adapter_args* a, int backward) { return up(a->n * a->r * 4) * (backward ? 2 : 1); }
+int up8(uint32_t d) { return (int)((d + 7) & ~7u); }
+
+// Rows of 16-bit elements that 16-byte loads and TMA take as they are: on
+// 16-byte boundaries, and one behind the other.
+bool rows_ok(const void* p, uint64_t rows, uint32_t cols, int64_t stride) {
+    return aligned_to(p, 16) && (rows < 2 || (stride % 8 == 0 && stride >= cols && stride < (1ll << 38)));
+}
+
+// What a call does with its sizes and pointers, and where it puts it.
+// Workspace: low (and for the backward call u) in f32; 16-bit operands whose
+// rows are not on 16-byte boundaries are copied there first, as is the
+// factor B of the backward call, transposed, so that its contraction axis is
+// contiguous.
+struct Plan {
+    bool f32, small, low_vec;
+    bool pack_x, pack_w, pack_a, pack_grad, pack_b;
+    uint64_t low, u, x, w, a, grad, b, bytes;
+};
+
+Plan plan_of(const ts_adapter_args* a, int backward) {
+    Plan p{};
+    p.f32 = a->dtype == TS_DTYPE_F32;
+    const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride);
+    const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in);
+    p.small = !p.f32 && !backward && a->n <= (uint64_t)kSmallTokens && (!a->weight || (x_ok && w_ok));
+    const bool whole_low = a->n > (uint64_t)kTokenLow;  // low by matrix instructions: aligned operands only
+    if (p.f32) {
+        const auto ok = [](const void* q, uint32_t cols, int64_t stride, uint64_t rows) {
+            return aligned_to(q, 16) && (rows < 2 || (stride % 4 == 0 && stride >= cols));
+        };
+        p.low_vec = !backward && ok(a->x, a->d_in, a->x_stride, a->n) && ok(a->lora_a, a->d_in, a->d_in, 2);
+    } else if (!backward) {
+        p.pack_x = !x_ok && ((a->weight && !p.small) || whole_low);
+        p.pack_w = a->weight && !p.small && !w_ok;
+        p.pack_a = !a_ok && whole_low;
+        p.low_vec = (x_ok || p.pack_x) && (a_ok || p.pack_a);
+    } else {
+        p.pack_x = !x_ok && a->grad_a;
+        p.pack_a = !a_ok && a->grad_a;
+        p.pack_w = a->weight && a->out && !w_ok;
+        p.pack_grad = !rows_ok(a->grad, a->n, a->d_out, a->grad_stride);
+        p.pack_b = true;
+        p.low_vec = true;
+    }
+    uint64_t at = 0;
+    const auto take = [&](bool want, uint64_t bytes) {
+        const uint64_t here = at;
+        if (want) at += up(bytes);
+        return here;
+    };
+    const uint64_t low = a->n * low_stride((int)a->r) * 4;
+    p.low = take(true, low);
+    p.u = take(backward, low);
+    p.x = take(p.pack_x, a->n * up8(a->d_in) * 2);
+    p.w = take(p.pack_w, (uint64_t)a->d_out * up8(a->d_in) * 2);
+    p.a = take(p.pack_a, (uint64_t)a->adapters * a->r * up8(a->d_in) * 2);
+    p.grad = take(p.pack_grad, a->n * up8(a->d_out) * 2);
+    p.b = take(p.pack_b, (uint64_t)a->adapters * a->r * up8(a->d_out) * 2);
+    p.bytes = a->n ? at : 0;
+    return p;
+}
 
 AdapterIds ids_of(const ts_adapter_args* a) { return {a->adapter, (long long)a->tokens_per_id, (int)a->adapters}; }
 
-int check_workspace(const ts_adapter_args* a, int backward) {
-    const uint64_t need = adapter_bytes(a, backward);
+int check_workspace(const ts_adapter_args* a, uint64_t need) {
     if (need && (!a->workspace || !aligned_to(a->workspace, 256) || a->workspace_bytes < need))
         return bad("the workspace is missing, not 256-byte aligned or smaller than ts_adapter_workspace says");
     return TS_OK;
@@ -140,60 +198,95 @@ int adapter_workspace(const ts_adapter_args* a, int backward, uint64_t* bytes) {
     b.workspace_bytes = 0;
     const int rc = check_adapter(&b, backward);
     if (rc) return rc;
-    *bytes = adapter_bytes(a, backward);
+    *bytes = plan_of(a, backward).bytes;
     return TS_OK;
 }
+
+// Rows of a matrix or factor as the kernels take them, copied to the
+// workspace first where `pack` is set.
+struct Rows {
+    const void* p;
+    long long stride;
+};
+
+struct Work {
+    const ts_adapter_args* a;
+    cudaStream_t s;
+    cudaError_t e = cudaSuccess;
+    void* at(uint64_t off) const { return static_cast<char*>(a->workspace) + off; }
+    Rows rows(bool pack, const void* p, uint64_t rows, uint32_t cols, long long stride, uint64_t off) {
+        if (!pack) return {p, rows < 2 ? up8(cols) : stride};
+        if (e == cudaSuccess) e = launch_pack({p, 0, stride, 1, (long long)rows, 1, (int)cols, up8(cols), at(off)}, s);
+        return {at(off), up8(cols)};
+    }
+};
 
 int adapter_project(const ts_adapter_args* a) {
     int rc = check_adapter(a, 0);
     if (rc || a->n == 0) return rc;
-    if ((rc = check_workspace(a, 0))) return rc;
+    const Plan p = plan_of(a, 0);
+    if ((rc = check_workspace(a, p.bytes))) return rc;
     OnDevice dev(a->device);
     if (dev.status != cudaSuccess) return cuda_status(dev.status);
-    cudaStream_t s = static_cast<cudaStream_t>(a->stream);
-    float* low = static_cast<float*>(a->workspace);
-    const long long ra = (long long)a->r * a->d_in, rb = (long long)a->r * a->d_out;
-    const LowArgs l{a->x, a->x_stride, (long long)a->n, (int)a->d_in, (int)a->r, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->scale, low};
-    cudaError_t e = launch_low(l, a->dtype, s);
-    if (e != cudaSuccess) return cuda_status(e);
-    const ProjectArgs p{a->x, a->x_stride, (long long)a->n, (int)a->d_in, (int)a->d_out, (int)a->r, a->weight, a->weight_stride, 1,
-                        a->bias, a->base, a->base_stride, low, {a->lora_b, rb, 1, a->r}, ids_of(a), a->out, a->out_stride};
-    return cuda_status(launch_project(p, a->dtype, s));
+    Work w{a, static_cast<cudaStream_t>(a->stream)};
+    const long long n = (long long)a->n, rb = (long long)a->r * a->d_out;
+    const int r = (int)a->r;
+    float* low = static_cast<float*>(w.at(p.low));
+    const Rows x = p.f32 ? Rows{a->x, a->x_stride} : w.rows(p.pack_x, a->x, a->n, a->d_in, a->x_stride, p.x);
+    const Rows wt = p.f32 ? Rows{a->weight, a->weight_stride} : w.rows(p.pack_w, a->weight, a->d_out, a->d_in, a->weight_stride, p.w);
+    Rows fa{a->lora_a, a->d_in};
+    if (p.pack_a) fa = w.rows(true, a->lora_a, (uint64_t)a->adapters * a->r, a->d_in, a->d_in, p.a);
+    const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low};
+    if (w.e == cudaSuccess) w.e = launch_low(&l, 1, a->dtype, p.low_vec, w.s);
+    const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, (int)a->d_out, r, wt.p, wt.stride, 0,
+                        a->bias, a->base, a->base_stride, low, {a->lora_b, rb, 1, r}, ids_of(a), a->out, a->out_stride};
+    if (w.e == cudaSuccess)
+        w.e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
+    return cuda_status(w.e);
 }
 
 int adapter_project_backward(const ts_adapter_args* a) {
     int rc = check_adapter(a, 1);
     if (rc) return rc;
-    if ((rc = check_workspace(a, 1))) return rc;
+    const Plan p = plan_of(a, 1);
+    if ((rc = check_workspace(a, p.bytes))) return rc;
     OnDevice dev(a->device);
     if (dev.status != cudaSuccess) return cuda_status(dev.status);
-    cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+    Work w{a, static_cast<cudaStream_t>(a->stream)};
     const long long n = (long long)a->n, ra = (long long)a->r * a->d_in, rb = (long long)a->r * a->d_out;
-    const size_t size = dtype_size(a->dtype);
+    const int r = (int)a->r, di = (int)a->d_in, d_o = (int)a->d_out;
     if (n == 0) {
         if (!a->grad_a) return TS_OK;
-        cudaError_t e = cudaMemsetAsync(a->grad_a, 0, (size_t)a->adapters * ra * size, s);
-        if (e == cudaSuccess) e = cudaMemsetAsync(a->grad_b, 0, (size_t)a->adapters * rb * size, s);
+        const size_t size = dtype_size(a->dtype);
+        cudaError_t e = cudaMemsetAsync(a->grad_a, 0, (size_t)a->adapters * ra * size, w.s);
+        if (e == cudaSuccess) e = cudaMemsetAsync(a->grad_b, 0, (size_t)a->adapters * rb * size, w.s);
         return cuda_status(e);
     }
-    float* u = static_cast<float*>(a->workspace);
-    float* low = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + up(a->n * a->r * 4));
-    const LowArgs lu{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->r, {a->lora_b, rb, 1, a->r}, ids_of(a), a->scale, u};
-    cudaError_t e = launch_low(lu, a->dtype, s);
-    if (e == cudaSuccess && a->out) {
-        const ProjectArgs p{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->d_in, (int)a->r, a->weight, 1, a->weight_stride,
-                            nullptr, nullptr, 0, u, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->out, a->out_stride};
-        e = launch_project(p, a->dtype, s);
+    float *low = static_cast<float*>(w.at(p.low)), *u = static_cast<float*>(w.at(p.u));
+    Rows x{a->x, a->x_stride}, wt{a->weight, a->weight_stride}, grad{a->grad, a->grad_stride}, fa{a->lora_a, di};
+    Factor fb{a->lora_b, rb, 1, r};
+    if (!p.f32) {
+        x = w.rows(p.pack_x, a->x, a->n, a->d_in, a->x_stride, p.x);
+        wt = w.rows(p.pack_w, a->weight, a->d_out, a->d_in, a->weight_stride, p.w);
+        grad = w.rows(p.pack_grad, a->grad, a->n, a->d_out, a->grad_stride, p.grad);
+        if (p.pack_a) fa = w.rows(true, a->lora_a, (uint64_t)a->adapters * a->r, a->d_in, a->d_in, p.a);
+        if (w.e == cudaSuccess) w.e = launch_pack({a->lora_b, rb, 1, r, r, (int)a->adapters, d_o, up8(a->d_out), w.at(p.b)}, w.s);
+        fb = {w.at(p.b), (long long)r * up8(a->d_out), up8(a->d_out), 1};
     }
-    if (e == cudaSuccess && a->grad_a) {
-        const GradArgs ga{a->x, a->x_stride, n, (int)a->d_in, (int)a->r, u, ids_of(a), a->grad_a, ra, a->d_in, 1};
-        e = launch_grad(ga, a->dtype, s);
-        const LowArgs ll{a->x, a->x_stride, n, (int)a->d_in, (int)a->r, {a->lora_a, ra, a->d_in, 1}, ids_of(a), a->scale, low};
-        if (e == cudaSuccess) e = launch_low(ll, a->dtype, s);
-        const GradArgs gb{a->grad, a->grad_stride, n, (int)a->d_out, (int)a->r, low, ids_of(a), a->grad_b, rb, 1, a->r};
-        if (e == cudaSuccess) e = launch_grad(gb, a->dtype, s);
+    const LowArgs l[2] = {{grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, u},
+                          {x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low}};
+    if (w.e == cudaSuccess) w.e = launch_low(l, a->grad_a ? 2 : 1, a->dtype, p.low_vec, w.s);
+    if (w.e == cudaSuccess && a->out) {
+        const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1,
+                            nullptr, nullptr, 0, u, {a->lora_a, ra, di, 1}, ids_of(a), a->out, a->out_stride};
+        w.e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }
-    return cuda_status(e);
+    if (w.e == cudaSuccess && a->grad_a) {
+        const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}}, n, r, ids_of(a)};
+        const bool vec = !p.f32 || (aligned_to(x.p, 16) && x.stride % 4 == 0 && aligned_to(grad.p, 16) && grad.stride % 4 == 0);
+        w.e = launch_grads(g, a->dtype, vec, w.s);
+    }
+    return cuda_status(w.e);
 }
 
 int logit_rules(const ts_rules_args* a) {
@@ -272,6 +365,16 @@ extern "C" int ts_adapter_project(const ts_adapter_args* args) {
 }
 extern "C" int ts_adapter_project_backward(const ts_adapter_args* args) {
     return guarded([&] { return adapter_project_backward(args); });
+}
+extern "C" int ts_expired_waits(int device, uint64_t* out) {
+    if (!out) return bad("out is NULL");
+    return guarded([&] {
+        OnDevice dev(device);
+        unsigned long long v = 0;
+        const int rc = cuda_status(dev.status != cudaSuccess ? dev.status : expired_waits(&v));
+        *out = v;
+        return rc;
+    });
 }
 extern "C" int ts_logit_rules(const ts_rules_args* args) {
     return guarded([&] { return logit_rules(args); });

@@ -1,5 +1,6 @@
 // k_lowrank.cu -- kernels of the low-rank adapters beside a shared
-// projection, and of their gradients.
+// projection, and of their gradients, but for the tensor-core projection of
+// many tokens (k_project.cu).
 //
 // For token m with adapter e (or none):
 //   low[m]  = s_e x[m] A_e^T                              (r values, f32)
@@ -9,11 +10,14 @@
 //   dx[m]   = dy[m] W + u[m] A_e
 //   dA_e    = sum over e's tokens of u[m]^T x[m]
 //   dB_e    = sum over e's tokens of dy[m]^T low[m]
-// The three kernels below are these lines; a factor's strides turn the
-// forward form into the backward one.  Sums are held in f32 and each result
-// is rounded to its type once.
+// The kernels below are these lines; a factor's strides turn the forward
+// form into the backward one.  Sums are held in f32 and each result is
+// rounded to its type once.
 #include "launch.cuh"
 #include "lowrank.cuh"
+#include "sm100.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace tsg {
 
@@ -37,32 +41,221 @@ __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat
 template <>
 __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 
-// One CTA per token, one warp per rank index in turn.
+// Two 16-bit elements as floats.
 template <class T>
-__global__ void __launch_bounds__(256) k_low(const LowArgs a) {
-    const long long m = blockIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int e = a.id.of(m);
-    float* low = a.low + m * a.r;
-    if (e < 0) {
-        for (int j = threadIdx.x; j < a.r; j += blockDim.x) low[j] = 0.f;
-        return;
+__device__ __forceinline__ float2 pair_f(uint32_t v) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Elements [k, k + 16 / sizeof(T)) of a row of `n`, zeros behind it.
+template <class T>
+__device__ __forceinline__ uint4 load16(const T* row, int k, int n) {
+    constexpr int V = 16 / sizeof(T);
+    if (k + V <= n) return *reinterpret_cast<const uint4*>(row + k);
+    T v[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = k + i < n ? row[k + i] : from_f<T>(0.f);
+    uint4 r;
+    memcpy(&r, v, 16);
+    return r;
+}
+
+template <class T>
+__device__ __forceinline__ float dot16(uint4 a, uint4 b, float v) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            v = fmaf(__uint_as_float(x[i]), __uint_as_float(y[i]), v);
+        } else {
+            const float2 p = pair_f<T>(x[i]), q = pair_f<T>(y[i]);
+            v = fmaf(p.y, q.y, fmaf(p.x, q.x, v));
+        }
     }
-    const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
-    const T* f = static_cast<const T*>(a.f.p) + e * a.f.se;
-    const float s = a.scale ? a.scale[e] : 1.f;
-    for (int j = warp; j < a.r; j += 8) {
-        float v = 0.f;
-        for (int k = lane; k < a.k; k += 32) v = fmaf(to_f(x[k]), to_f(f[j * a.f.sj + k * a.f.sk]), v);
+    return v;
+}
+
+// D = A B + C on 16 x 8 x 16 of a 16-bit type, f32 sums.
+template <class T>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma8_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---------------------------------------------------------------- packing
+
+// Copies rows to 16-byte boundaries, or transposes a factor: 32 x 32 tiles
+// through shared memory, read along whichever axis of src is contiguous.
+__global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
+    __shared__ uint16_t tile[32][33];
+    const uint16_t* src = static_cast<const uint16_t*>(a.src) + blockIdx.z * a.se;
+    uint16_t* dst = static_cast<uint16_t*>(a.dst) + (long long)blockIdx.z * a.rows * a.dst_cols;
+    const long long j0 = (long long)blockIdx.x * 32;
+    const int k0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = ty; i < 32; i += 8) {
+        const long long j = j0 + (a.sk == 1 ? i : tx);
+        const int k = k0 + (a.sk == 1 ? tx : i);
+        tile[(int)(j - j0)][k - k0] = j < a.rows && k < a.cols ? src[j * a.sj + k * a.sk] : (uint16_t)0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = ty; i < 32; i += 8)
+        if (j0 + i < a.rows && k0 + tx < a.dst_cols) dst[(j0 + i) * a.dst_cols + k0 + tx] = tile[i][tx];
+}
+
+// ---------------------------------------------------------------- low
+
+struct LowPair {
+    LowArgs a[2];
+};
+
+// Token by token: WPJ warps share one rank index of one token.  Bound: reading
+// each token's own factor (r k elements), from L2 where tokens share it.
+template <class T, bool VEC, int WPJ>
+__global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
+    release_dependents();
+    const LowArgs a = both.a[blockIdx.z];
+    const long long m = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPJ;
+    const int j = blockIdx.y * (8 / WPJ) + warp / WPJ;
+    const int rs = low_stride(a.r);
+    const int e = a.id.of(m);
+    float v = 0.f;
+    if (e >= 0 && j < a.r) {
+        const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
+        const T* f = static_cast<const T*>(a.f.p) + e * a.f.se + j * a.f.sj;
+        if constexpr (VEC) {
+            constexpr int V = 16 / sizeof(T);
+#pragma unroll 4
+            for (int k = (part * 32 + lane) * V; k < a.k; k += 32 * V * WPJ) v = dot16<T>(load16(x, k, a.k), load16(f, k, a.k), v);
+        } else {
+#pragma unroll 4
+            for (int k = part * 32 + lane; k < a.k; k += 32 * WPJ) v = fmaf(to_f(x[k]), to_f(f[k * a.f.sk]), v);
+        }
 #pragma unroll
         for (int q = 16; q; q >>= 1) v += __shfl_xor_sync(0xffffffffu, v, q);
-        if (lane == 0) low[j] = s * v;
+    }
+    if constexpr (WPJ > 1) {
+        __shared__ float part_sum[8];
+        if (lane == 0) part_sum[warp] = v;
+        __syncthreads();
+        if (part == 0) {
+            v = 0.f;
+#pragma unroll
+            for (int q = 0; q < WPJ; q++) v += part_sum[warp + q];
+        }
+    }
+    if (part == 0 && lane == 0 && j < rs) a.low[m * rs + j] = e >= 0 && j < a.r ? (a.scale ? a.scale[e] * v : v) : 0.f;
+}
+
+// 32 tokens per cluster of S CTAs, 8 S warps sharing the contraction in
+// 32-wide blocks.  Operands go from global memory to the matrix
+// instructions' registers: a thread's 16 bytes of a row are the k indexes
+// of two instructions, in the same (permuted) order for x and the factor.
+// For each distinct adapter among the 32 tokens all rows are multiplied and
+// the adapter's own are kept, so that another adapter's NaN stays out.
+template <class T>
+__global__ void __launch_bounds__(256) k_low_mma(const LowPair both) {
+    release_dependents();
+    const LowArgs a = both.a[blockIdx.z];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const long long m0 = (long long)(blockIdx.x / S) * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rs = low_stride(a.r);
+    __shared__ float red[8][32][33];
+    __shared__ float sum[32][33];
+    const int id = m0 + lane < a.n ? a.id.of(m0 + lane) : -1;
+    const unsigned in = (unsigned)min(32ll, a.n - m0);
+    const T* xr[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const long long m = m0 + g + 8 * i;  // rows behind the last token repeat it; they are not stored
+        xr[i] = static_cast<const T*>(a.x) + (m < a.n ? m : a.n - 1) * a.x_stride;
+    }
+    unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
+    // tokens without an adapter
+    if (rank == 0)
+        for (int i = threadIdx.x; i < 32 * rs; i += 256) {
+            const int row = i / rs;
+            if ((unsigned)row < in && !(todo >> row & 1)) a.low[(m0 + row) * rs + i % rs] = 0.f;
+        }
+    while (todo) {
+        const int e = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+        const unsigned mine = __ballot_sync(0xffffffffu, id == e);
+        todo &= ~mine;
+        const T* f = static_cast<const T*>(a.f.p) + e * a.f.se;
+        const float scale = a.scale ? a.scale[e] : 1.f;
+        for (int j0 = 0; j0 < a.r; j0 += 32) {
+            float acc[2][4][4] = {};
+            const T* fr[4];
+#pragma unroll
+            for (int nb = 0; nb < 4; nb++) fr[nb] = f + (long long)min(j0 + nb * 8 + g, a.r - 1) * a.f.sj;
+#pragma unroll 2
+            for (int k = (rank * 8 + warp) * 32 + 8 * t; k - 8 * t < a.k; k += 256 * S) {
+                uint4 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = load16(xr[i], k, a.k);
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++) {
+                    if (j0 + nb * 8 >= a.r) break;
+                    const uint4 b = load16(fr[nb], k, a.k);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        mma16<T>(acc[h][nb], x[2 * h].x, x[2 * h + 1].x, x[2 * h].y, x[2 * h + 1].y, b.x, b.y);
+                        mma16<T>(acc[h][nb], x[2 * h].z, x[2 * h + 1].z, x[2 * h].w, x[2 * h + 1].w, b.z, b.w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) red[warp][h * 16 + g + (c >> 1) * 8][nb * 8 + 2 * t + (c & 1)] = acc[h][nb][c];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 1024; i += 256) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < 8; w++) v += red[w][i >> 5][i & 31];
+                sum[i >> 5][i & 31] = v;
+            }
+            if (S > 1) cluster.sync();
+            else __syncthreads();
+            // each CTA finishes 32 / S of the rows
+            for (int i = threadIdx.x; i < 1024 / S; i += 256) {
+                const int row = rank * (32 / S) + (i >> 5), j = j0 + (i & 31);
+                if (mine >> row & 1 && j < rs) {
+                    float v = 0.f;
+                    for (int q = 0; q < S; q++) v += S > 1 ? *cluster.map_shared_rank(&sum[row][i & 31], q) : sum[row][i & 31];
+                    a.low[(m0 + row) * rs + j] = j < a.r ? scale * v : 0.f;
+                }
+            }
+            if (S > 1) cluster.sync();
+            else __syncthreads();
+        }
     }
 }
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 16 of the contraction at a time.
-template <class T>
-__global__ void __launch_bounds__(256) k_project(const ProjectArgs a) {
+// ---------------------------------------------------------------- projection
+
+// f32: 64 x 64 outputs per CTA, 4 x 4 per thread, 16 of the contraction at a
+// time.
+__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a) {
     constexpr int BM = 64, BN = 64, BK = 16;
     __shared__ float xs[BK][BM + 1], ws[BK][BN + 1];
     const long long m0 = (long long)blockIdx.x * BM;
@@ -70,17 +263,18 @@ __global__ void __launch_bounds__(256) k_project(const ProjectArgs a) {
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     float acc[4][4] = {};
     if (a.w) {
-        const T* x = static_cast<const T*>(a.x);
-        const T* w = static_cast<const T*>(a.w);
+        const float* x = static_cast<const float*>(a.x);
+        const float* w = static_cast<const float*>(a.w);
+        const long long w_so = a.w_t ? 1 : a.w_stride, w_sk = a.w_t ? a.w_stride : 1;
         for (int k0 = 0; k0 < a.k; k0 += BK) {
             for (int i = threadIdx.x; i < BM * BK; i += 256) {
                 const int k = i % BK, m = i / BK;
-                xs[k][m] = m0 + m < a.n && k0 + k < a.k ? to_f(x[(m0 + m) * a.x_stride + k0 + k]) : 0.f;
+                xs[k][m] = m0 + m < a.n && k0 + k < a.k ? x[(m0 + m) * a.x_stride + k0 + k] : 0.f;
             }
             for (int i = threadIdx.x; i < BN * BK; i += 256) {
                 // consecutive threads along whichever axis of W is contiguous
-                const int k = a.w_sk == 1 ? i % BK : i / BN, o = a.w_sk == 1 ? i / BK : i % BN;
-                ws[k][o] = o0 + o < a.o && k0 + k < a.k ? to_f(w[(o0 + o) * a.w_so + (k0 + k) * a.w_sk]) : 0.f;
+                const int k = a.w_t ? i / BN : i % BK, o = a.w_t ? i % BN : i / BK;
+                ws[k][o] = o0 + o < a.o && k0 + k < a.k ? w[(o0 + o) * w_so + (k0 + k) * w_sk] : 0.f;
             }
             __syncthreads();
 #pragma unroll
@@ -96,38 +290,359 @@ __global__ void __launch_bounds__(256) k_project(const ProjectArgs a) {
             __syncthreads();
         }
     }
+    const int rs = low_stride(a.r);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const long long m = m0 + ty + 16 * i;
         if (m >= a.n) continue;
         const int e = a.id.of(m);
-        const float* low = a.low + m * a.r;
-        const T* g = static_cast<const T*>(a.g.p) + (e < 0 ? 0 : e) * a.g.se;
+        const float* low = a.low + m * rs;
+        const float* g = static_cast<const float*>(a.g.p) + (e < 0 ? 0 : e) * a.g.se;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int o = o0 + tx + 16 * j;
             if (o >= a.o) continue;
             float v = acc[i][j];
-            if (a.bias) v += to_f(static_cast<const T*>(a.bias)[o]);
+            if (a.bias) v += static_cast<const float*>(a.bias)[o];
             if (e >= 0)
-                for (int q = 0; q < a.r; q++) v = fmaf(low[q], to_f(g[q * a.g.sj + o * a.g.sk]), v);
-            if (a.base) v += to_f(static_cast<const T*>(a.base)[m * a.base_stride + o]);
-            static_cast<T*>(a.out)[m * a.out_stride + o] = from_f<T>(v);
+                for (int q = 0; q < a.r; q++) v = fmaf(low[q], g[q * a.g.sj + o * a.g.sk], v);
+            if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
+            static_cast<float*>(a.out)[m * a.out_stride + o] = v;
         }
     }
 }
 
-// One thread per element of the gradient, all tokens in order.
-template <class T>
-__global__ void __launch_bounds__(256) k_grad(const GradArgs a) {
-    const int k = blockIdx.x * 256 + threadIdx.x;
-    const int j = blockIdx.y, e = blockIdx.z;
-    if (k >= a.k) return;
+// Few tokens: a CTA streams 16 rows of W once past all tokens, its warps
+// sharing the contraction in 32-wide blocks (operands as in k_low_mma, W as
+// the 16-row operand).  Bound: reading W; the stream starts before low is
+// there, and waits for it only to add the adapters' terms.
+template <class T, int NB, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) k_project_small(const ProjectArgs a) {
+    const int o0 = blockIdx.x * 16;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    extern __shared__ float red[];  // [WARPS][16][NB * 8 + 1]
+    constexpr int RS = NB * 8 + 1;
+    if (a.w) {
+        float acc[NB][4] = {};
+        const T* w = static_cast<const T*>(a.w);
+        const T* w0 = w + (long long)min(o0 + g, a.o - 1) * a.w_stride;
+        const T* w1 = w + (long long)min(o0 + g + 8, a.o - 1) * a.w_stride;
+        const T* xr[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min((long long)(nb * 8 + g), a.n - 1) * a.x_stride;
+#pragma unroll 4
+        for (int k = warp * 32 + 8 * t; k - 8 * t < a.k; k += WARPS * 32) {
+            const uint4 p = load16(w0, k, a.k), q = load16(w1, k, a.k);
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                const uint4 x = load16(xr[nb], k, a.k);
+                mma16<T>(acc[nb], p.x, q.x, p.y, q.y, x.x, x.y);
+                mma16<T>(acc[nb], p.z, q.z, p.w, q.w, x.z, x.w);
+            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) red[(warp * 16 + g + (c >> 1) * 8) * RS + nb * 8 + 2 * t + (c & 1)] = acc[nb][c];
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    const int rs = low_stride(a.r);
+    for (int i = threadIdx.x; i < 16 * NB * 8; i += WARPS * 32) {
+        const int o = o0 + (i & 15), m = i >> 4;
+        if (o >= a.o || m >= a.n) continue;
+        float v = a.bias ? to_f(static_cast<const T*>(a.bias)[o]) : 0.f;
+        if (a.w)
+#pragma unroll
+            for (int q = 0; q < WARPS; q++) v += red[(q * 16 + (i & 15)) * RS + m];
+        if (a.base) v += to_f(static_cast<const T*>(a.base)[m * a.base_stride + o]);
+        const int e = a.id.of(m);
+        if (e >= 0) {
+            const T* b = static_cast<const T*>(a.g.p) + e * a.g.se + o * a.g.sk;
+            const float* low = a.low + m * rs;
+#pragma unroll 8
+            for (int j = 0; j < a.r; j++) v = fmaf(low[j], to_f(b[j * a.g.sj]), v);
+        }
+        static_cast<T*>(a.out)[m * a.out_stride + o] = from_f<T>(v);
+    }
+}
+
+// ---------------------------------------------------------------- gradients of the factors
+
+constexpr int kGradScan = 2048;  // ids looked through at a time
+constexpr int kGradStages = 4;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <class T, int RB>
+struct GradTile {
+    static constexpr int kRow = sizeof(T) == 4 ? 136 * 4 : 288;  // 128 features; rows 8 banks apart
+    static constexpr int kURow = RB * 8 + 8;                     // floats
+    static constexpr int kX = 32 * kRow, kU = 32 * kURow * 4;
+    static constexpr int kSmem = kGradStages * (kX + kU);
+};
+
+// One adapter, 128 features and RB * 8 rank indexes per cluster of S CTAs.
+// Every CTA looks through the adapter indexes, keeps the positions of its
+// share of the adapter's tokens (every S-th group of 32, in order), gathers
+// their rows and sums low^T x with 16 x 8 x 8 TF32 products: features are
+// the 16-row axis, tokens the contraction.  16-bit x is exact in TF32; low
+// is rounded to 11 significant bits; for f32 inputs both are split into two
+// TF32 parts, which leaves 2^-22.  The partial sums of the cluster meet in
+// shared memory in a fixed order.  Bound: reading x once per 64 rank indexes.
+template <class T, int RB>
+__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int vec) {
+    using L = GradTile<T, RB>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int list[kGradScan + 64];
+    __shared__ int warp_count[8];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tile = blockIdx.x / S;
+    const GradArgs a = both.g[tile >= tiles0];
+    const int k0 = (tile >= tiles0 ? tile - tiles0 : tile) * 128, j0 = blockIdx.y * RB * 8, e = blockIdx.z;
+    const int rs = low_stride(both.r);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int wf = warp & 3, wt = warp >> 2;
     const T* x = static_cast<const T*>(a.x);
-    float v = 0.f;
-    for (long long m = 0; m < a.n; m++)
-        if (a.id.of(m) == e) v = fmaf(a.low[m * a.r + j], to_f(x[m * a.x_stride + k]), v);
-    static_cast<T*>(a.out)[e * a.se + j * a.sj + k * a.sk] = from_f<T>(v);
+    const uint32_t base = smem_u32(smem);
+    float acc[2][RB][4] = {};
+
+    long long found = 0;  // tokens of the adapter before this round
+    for (long long m0 = 0; m0 < both.n; m0 += kGradScan) {
+        for (int i = threadIdx.x; i < kGradScan + 64; i += 256) list[i] = -1;
+        unsigned hits = 0;
+        const long long at = m0 + threadIdx.x * 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (at + i < both.n && both.id.of(at + i) == e) hits |= 1u << i;
+        const int cnt = __popc(hits);
+        int before = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        if (lane == 31) warp_count[warp] = before;
+        __syncthreads();
+        int total = 0;
+        before -= cnt;
+#pragma unroll
+        for (int w = 0; w < 8; w++) before += w < warp ? warp_count[w] : 0, total += warp_count[w];
+        const auto own_before = [&](long long group) { return group / S + (group % S > rank); };  // own groups below `group`
+        const long long first = own_before(found >> 5);
+        while (hits) {
+            const int i = __ffs(hits) - 1;
+            hits &= hits - 1;
+            const long long pos = found + before++;
+            if ((pos >> 5) % S == rank) list[(int)(own_before(pos >> 5) - first) * 32 + (int)(pos & 31)] = (int)(at - m0) + i;
+        }
+        const int groups = total ? (int)(own_before(((found + total - 1) >> 5) + 1) - first) : 0;
+        found += total;
+        __syncthreads();
+
+        const auto fetch = [&](int q) {
+            if (q < groups) {
+                const uint32_t sx = base + (q % kGradStages) * (L::kX + L::kU), su = sx + L::kX;
+                constexpr int V = 16 / sizeof(T), C = 128 / V;
+                if (sizeof(T) == 4 && !vec) {
+                    for (int i = threadIdx.x; i < 32 * 128; i += 256) {
+                        const int row = i >> 7, c = i & 127, m = list[q * 32 + row];
+                        const bool in = m >= 0 && k0 + c < a.k;
+                        cp_async4(sx + row * L::kRow + c * 4, in ? x + (m0 + m) * a.x_stride + k0 + c : x, in ? 4 : 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = threadIdx.x; i < 32 * C; i += 256) {
+                        const int row = i / C, c = i % C * V, m = list[q * 32 + row];
+                        const int left = m >= 0 ? min(V, max(0, a.k - k0 - c)) : 0;
+                        cp_async16(sx + row * L::kRow + c * (int)sizeof(T), left ? x + (m0 + m) * a.x_stride + k0 + c : x, left * (int)sizeof(T));
+                    }
+                }
+#pragma unroll
+                for (int i = threadIdx.x; i < 32 * RB * 2; i += 256) {
+                    const int row = i / (RB * 2), c = i % (RB * 2) * 4, m = list[q * 32 + row];
+                    const bool in = m >= 0 && j0 + c < rs;
+                    cp_async16(su + (row * L::kURow + c) * 4, in ? a.low + (m0 + m) * rs + j0 + c : a.low, in ? 16 : 0);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int q = 0; q < kGradStages - 1; q++) fetch(q);
+        for (int q = 0; q < groups; q++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+            __syncthreads();
+            fetch(q + kGradStages - 1);
+            const uint8_t* sx = smem + (q % kGradStages) * (L::kX + L::kU);
+            const float* su = reinterpret_cast<const float*>(sx + L::kX);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int tok = (wt * 2 + h) * 8 + t;
+                // four features of two tokens per thread: rows g and g + 8 of two products
+                float f[2][4];
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const uint8_t* p = sx + (tok + 4 * z) * L::kRow + (wf * 32 + 4 * g) * sizeof(T);
+                    if constexpr (sizeof(T) == 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(p);
+                        f[z][0] = v.x, f[z][1] = v.y, f[z][2] = v.z, f[z][3] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(p);
+                        const float2 lo = pair_f<T>(v.x), hi = pair_f<T>(v.y);
+                        f[z][0] = lo.x, f[z][1] = lo.y, f[z][2] = hi.x, f[z][3] = hi.y;
+                    }
+                }
+                uint32_t am[2][4], al[2][4];
+#pragma unroll
+                for (int q2 = 0; q2 < 2; q2++)
+#pragma unroll
+                    for (int z = 0; z < 4; z++) {
+                        const float v = f[z >> 1][q2 * 2 + (z & 1)];
+                        if constexpr (sizeof(T) == 4) {
+                            am[q2][z] = to_tf32(v);
+                            al[q2][z] = to_tf32(v - __uint_as_float(am[q2][z]));
+                        } else {
+                            am[q2][z] = __float_as_uint(v);
+                        }
+                    }
+#pragma unroll
+                for (int nb = 0; nb < RB; nb++) {
+                    const float b0 = su[tok * L::kURow + nb * 8 + g], b1 = su[(tok + 4) * L::kURow + nb * 8 + g];
+                    const uint32_t m0b = to_tf32(b0), m1b = to_tf32(b1);
+#pragma unroll
+                    for (int q2 = 0; q2 < 2; q2++) {
+                        if constexpr (sizeof(T) == 4) {
+                            const uint32_t l0 = to_tf32(b0 - __uint_as_float(m0b)), l1 = to_tf32(b1 - __uint_as_float(m1b));
+                            mma8_tf32(acc[q2][nb], al[q2], m0b, m1b);
+                            mma8_tf32(acc[q2][nb], am[q2], l0, l1);
+                        }
+                        mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+    }
+
+    // the two token halves, then the cluster's CTAs: sum[rank index][feature]
+    float* sum = reinterpret_cast<float*>(smem);
+    constexpr int SR = 129;
+    static_assert(RB * 8 * SR * 4 <= L::kSmem, "the sums fit where the tiles were");
+#pragma unroll
+    for (int half = 1; half >= 0; half--) {
+        if (wt == half)
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+                for (int nb = 0; nb < RB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float* p = sum + (nb * 8 + 2 * t + (c & 1)) * SR + wf * 32 + 4 * g + 2 * q + (c >> 1);
+                        *p = half ? acc[q][nb][c] : *p + acc[q][nb][c];
+                    }
+        __syncthreads();
+    }
+    if (S > 1) cluster.sync();
+    const int per = RB * 8 * 128 / S;
+    for (int i = threadIdx.x; i < per; i += 256) {
+        const int q = rank * per + i;
+        // consecutive threads along whichever axis of the result is contiguous
+        const int j = a.sk == 1 ? q >> 7 : q % (RB * 8), k = a.sk == 1 ? q & 127 : q / (RB * 8);
+        float v = 0.f;
+        for (int c = 0; c < S; c++) v += S > 1 ? *cluster.map_shared_rank(sum + j * SR + k, c) : sum[j * SR + k];
+        if (j0 + j < both.r && k0 + k < a.k)
+            static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(v);
+    }
+    if (S > 1) cluster.sync();
+}
+
+int sm_count() {
+    int dev = 0, sms = 1;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+template <class T>
+cudaError_t low_launch(const LowArgs* a, int count, bool vec, cudaStream_t s) {
+    const LowPair both{{a[0], a[count - 1]}};
+    const long long n = a[0].n;
+    const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
+    KScope ks("adapter_low", s);
+    if constexpr (sizeof(T) == 2) {
+        if (n > kTokenLow) {
+            // as many CTAs share a contraction as it takes to give every SM
+            // one, while each still has four blocks for a warp
+            const long long tiles = (n + 31) / 32;
+            int S = 1;
+            while (S < 8 && tiles * S * count < sm_count() && kmax / (S * 2) >= 512) S *= 2;
+            return launch_cl(S, k_low_mma<T>, dim3((unsigned)(tiles * S), 1, count), 256, 0, s, both);
+        }
+    }
+    // long contractions over more warps, to have more loads in flight
+    const int rs = low_stride(a[0].r);
+    if (kmax * sizeof(T) > 4096) {
+        const dim3 grid((unsigned)n, (rs + 1) / 2, count);
+        if (vec) k_low_token<T, true, 4><<<grid, 256, 0, s>>>(both);
+        else k_low_token<T, false, 4><<<grid, 256, 0, s>>>(both);
+    } else {
+        const dim3 grid((unsigned)n, (rs + 7) / 8, count);
+        if (vec) k_low_token<T, true, 1><<<grid, 256, 0, s>>>(both);
+        else k_low_token<T, false, 1><<<grid, 256, 0, s>>>(both);
+    }
+    return cudaGetLastError();
+}
+
+template <class T, int NB>
+cudaError_t small_launch(const ProjectArgs& a, cudaStream_t s) {
+    // 16 warps where the contraction is long: an SM then has enough loads in
+    // flight for its share of the bandwidth
+    const int warps = a.k >= 4096 ? 16 : 8;
+    const size_t smem = (size_t)warps * 16 * (NB * 8 + 1) * 4;
+    const dim3 grid((a.o + 15) / 16);
+    KScope ks("adapter_project", s);
+    if (warps == 16) {
+        const cudaError_t e = ensure_smem(k_project_small<T, NB, 16>, smem);
+        return e != cudaSuccess ? e : launch_dependent(k_project_small<T, NB, 16>, grid, 512, smem, s, a);
+    }
+    return launch_dependent(k_project_small<T, NB, 8>, grid, 256, smem, s, a);
+}
+
+template <class T>
+cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
+    if (a.n <= 8) return small_launch<T, 1>(a, s);
+    if (a.n <= 16) return small_launch<T, 2>(a, s);
+    if (a.n <= 32) return small_launch<T, 4>(a, s);
+    return small_launch<T, 8>(a, s);
+}
+
+template <class T, int RB>
+cudaError_t grad_launch(const GradPair& a, bool vec, cudaStream_t s) {
+    using L = GradTile<T, RB>;
+    const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
+    // CTAs that share an adapter's tokens: until there are two for each SM,
+    // while each has two groups of tokens on average
+    const long long ctas = (long long)(t0 + t1) * passes * a.id.count;
+    int S = 1;
+    while (S < 8 && ctas * S < 2 * sm_count() && a.n / a.id.count >= 128 * S) S *= 2;
+    // the list is beside it: raise the limit even where the tiles alone fit the default
+    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 16);
+    if (e != cudaSuccess) return e;
+    KScope ks("adapter_grad", s);
+    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.id.count), 256, L::kSmem, s, a, t0, (int)vec);
+}
+
+template <class T>
+cudaError_t grad_width(const GradPair& a, bool vec, cudaStream_t s) {
+    if (a.r <= 16) return grad_launch<T, 2>(a, vec, s);
+    if (a.r <= 32) return grad_launch<T, 4>(a, vec, s);
+    return grad_launch<T, 8>(a, vec, s);
 }
 
 }  // namespace
@@ -137,27 +652,31 @@ __global__ void __launch_bounds__(256) k_grad(const GradArgs a) {
         case DT_F32: { using T = float; __VA_ARGS__; } break;          \
         case DT_BF16: { using T = __nv_bfloat16; __VA_ARGS__; } break; \
         case DT_F16: { using T = __half; __VA_ARGS__; } break;         \
-        default: return cudaErrorInvalidValue;                         \
-    }
+    }                                                                  \
+    return cudaErrorInvalidValue;
 
-cudaError_t launch_low(const LowArgs& a, int dtype, cudaStream_t s) {
-    KScope ks("adapter_low", s);
-    TSG_DTYPE_SWITCH(dtype, k_low<T><<<(unsigned)a.n, 256, 0, s>>>(a));
+cudaError_t launch_pack(const PackArgs& a, cudaStream_t s) {
+    KScope ks("adapter_pack", s);
+    k_pack<<<dim3((unsigned)((a.rows + 31) / 32), (a.dst_cols + 31) / 32, a.count), 256, 0, s>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t launch_project(const ProjectArgs& a, int dtype, cudaStream_t s) {
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return low_launch<T>(a, count, vec, s));
+}
+
+cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
     KScope ks("adapter_project", s);
-    const dim3 grid((unsigned)((a.n + 63) / 64), (a.o + 63) / 64);
-    TSG_DTYPE_SWITCH(dtype, k_project<T><<<grid, 256, 0, s>>>(a));
+    k_project_f32<<<dim3((unsigned)((a.n + 63) / 64), (a.o + 63) / 64), 256, 0, s>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t launch_grad(const GradArgs& a, int dtype, cudaStream_t s) {
-    KScope ks("adapter_grad", s);
-    const dim3 grid((a.k + 255) / 256, a.r, a.id.count);
-    TSG_DTYPE_SWITCH(dtype, k_grad<T><<<grid, 256, 0, s>>>(a));
-    return cudaGetLastError();
+cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s) {
+    return dtype == DT_BF16 ? small_width<__nv_bfloat16>(a, s) : small_width<__half>(a, s);
+}
+
+cudaError_t launch_grads(const GradPair& a, int dtype, bool vec, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, vec, s));
 }
 
 }  // namespace tsg

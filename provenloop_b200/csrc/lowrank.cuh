@@ -35,8 +35,14 @@ struct Factor {
     long long se, sj, sk;
 };
 
-// low[m][j] = scale_e * sum_k x[m][k] F[e][j][k] (f32 [n][r]; zero rows where
-// a token has no adapter).
+// Rows of low are padded to a multiple of four, zero behind r.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int low_stride(int r) { return (r + 3) & ~3; }
+
+// low[m][j] = scale_e * sum_k x[m][k] F[e][j][k] (f32 [n][low_stride(r)];
+// zero rows where a token has no adapter).
 struct LowArgs {
     const void* x;
     long long x_stride;
@@ -49,15 +55,16 @@ struct LowArgs {
 };
 
 // out[m][o] = base[m][o] + sum_k x[m][k] W(o, k) + bias[o]
-//           + sum_j low[m][j] G[e][j][o];  W(o, k) at w + o * w_so + k * w_sk,
-// each term but the last optional.
+//           + sum_j low[m][j] G[e][j][o], each term but the last optional.
+// W(o, k) is w[o][k], or w[k][o] where w_t is set (the backward call).
 struct ProjectArgs {
     const void* x;
     long long x_stride;
     long long n;
     int k, o, r;
     const void* w;
-    long long w_so, w_sk;
+    long long w_stride;
+    int w_t;
     const void* bias;
     const void* base;
     long long base_stride;
@@ -73,17 +80,47 @@ struct ProjectArgs {
 struct GradArgs {
     const void* x;
     long long x_stride;
-    long long n;
-    int k, r;
+    int k;
     const float* low;
-    AdapterIds id;
     void* out;
     long long se, sj, sk;
 };
+struct GradPair {
+    GradArgs g[2];
+    long long n;
+    int r;
+    AdapterIds id;
+};
 
-cudaError_t launch_low(const LowArgs& a, int dtype, cudaStream_t s);
-cudaError_t launch_project(const ProjectArgs& a, int dtype, cudaStream_t s);
-cudaError_t launch_grad(const GradArgs& a, int dtype, cudaStream_t s);
+// dst[e][j][k] (rows of `dst_cols` 16-bit elements, zeros behind `cols`) =
+// src[e * se + j * sj + k * sk].
+struct PackArgs {
+    const void* src;
+    long long se, sj, sk;
+    long long rows;
+    int count, cols, dst_cols;
+    void* dst;
+};
+
+// The kernels that a call takes go by its sizes; decode_ops.cu lays out the
+// workspace with the same rules.
+constexpr int kTokenLow = 128;    // up to here, and for f32, low is computed token by token
+constexpr int kSmallTokens = 64;  // up to here W is streamed once past all tokens
+
+cudaError_t launch_pack(const PackArgs& a, cudaStream_t s);
+// one or two of them (the same n, r and id) in one launch; `vec`: rows of x
+// and f start on 16-byte boundaries and f.sk is 1
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, cudaStream_t s);
+// f32, any strides
+cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s);
+// 16-bit types, at most kSmallTokens tokens; x and w (not transposed) on 16-byte boundaries
+cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s);
+// 16-bit types; x and w rows on 16-byte boundaries (k_project.cu)
+cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
+// rows of x on 16-byte boundaries, but for f32 (`vec`: they are)
+cudaError_t launch_grads(const GradPair& a, int dtype, bool vec, cudaStream_t s);
+// waits of k_project.cu that ran out on the current device so far
+cudaError_t expired_waits(unsigned long long* out);
 
 struct RulesArgs {
     const void* logits;
