@@ -48,7 +48,11 @@ __device__ __forceinline__ float2 pair_f(uint32_t v) {
     else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
-// Elements [k, k + 16 / sizeof(T)) of a row of `n`, zeros behind it.
+template <class T>
+__device__ __forceinline__ uint4 whole16(const T* row, int k) { return *reinterpret_cast<const uint4*>(row + k); }
+
+// Elements [k, k + 16 / sizeof(T)) of a row of `n`, zeros behind it.  Loops
+// take whole16 while they can: loads under a condition do not overlap.
 template <class T>
 __device__ __forceinline__ uint4 load16(const T* row, int k, int n) {
     constexpr int V = 16 / sizeof(T);
@@ -140,8 +144,10 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
         const T* f = static_cast<const T*>(a.f.p) + e * a.f.se + j * a.f.sj;
         if constexpr (VEC) {
             constexpr int V = 16 / sizeof(T);
+            int k = (part * 32 + lane) * V;
 #pragma unroll 4
-            for (int k = (part * 32 + lane) * V; k < a.k; k += 32 * V * WPJ) v = dot16<T>(load16(x, k, a.k), load16(f, k, a.k), v);
+            for (; k + V <= a.k; k += 32 * V * WPJ) v = dot16<T>(whole16(x, k), whole16(f, k), v);
+            if (k < a.k) v = dot16<T>(load16(x, k, a.k), load16(f, k, a.k), v);
         } else {
 #pragma unroll 4
             for (int k = part * 32 + lane; k < a.k; k += 32 * WPJ) v = fmaf(to_f(x[k]), to_f(f[k * a.f.sk]), v);
@@ -205,22 +211,24 @@ __global__ void __launch_bounds__(256) k_low_mma(const LowPair both) {
             const T* fr[4];
 #pragma unroll
             for (int nb = 0; nb < 4; nb++) fr[nb] = f + (long long)min(j0 + nb * 8 + g, a.r - 1) * a.f.sj;
-#pragma unroll 2
-            for (int k = (rank * 8 + warp) * 32 + 8 * t; k - 8 * t < a.k; k += 256 * S) {
-                uint4 x[4];
+const auto block = [&](auto load, int k) {
+                uint4 x[4], b[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = load16(xr[i], k, a.k);
+                for (int i = 0; i < 4; i++) x[i] = load(xr[i], k);
 #pragma unroll
-                for (int nb = 0; nb < 4; nb++) {
-                    if (j0 + nb * 8 >= a.r) break;
-                    const uint4 b = load16(fr[nb], k, a.k);
+                for (int nb = 0; nb < 4; nb++) b[nb] = load(fr[nb], k);
+#pragma unroll
+                for (int nb = 0; nb < 4; nb++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        mma16<T>(acc[h][nb], x[2 * h].x, x[2 * h + 1].x, x[2 * h].y, x[2 * h + 1].y, b.x, b.y);
-                        mma16<T>(acc[h][nb], x[2 * h].z, x[2 * h + 1].z, x[2 * h].w, x[2 * h + 1].w, b.z, b.w);
+                        mma16<T>(acc[h][nb], x[2 * h].x, x[2 * h + 1].x, x[2 * h].y, x[2 * h + 1].y, b[nb].x, b[nb].y);
+                        mma16<T>(acc[h][nb], x[2 * h].z, x[2 * h + 1].z, x[2 * h].w, x[2 * h + 1].w, b[nb].z, b[nb].w);
                     }
-                }
-            }
+            };
+            int k = (rank * 8 + warp) * 32;
+#pragma unroll 2
+            for (; k + 32 <= a.k; k += 256 * S) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
+            if (k < a.k) block([&](const T* row, int at) { return load16(row, at, a.k); }, k + 8 * t);
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -330,16 +338,21 @@ __global__ void __launch_bounds__(WARPS * 32) k_project_small(const ProjectArgs 
         const T* xr[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min((long long)(nb * 8 + g), a.n - 1) * a.x_stride;
-#pragma unroll 4
-        for (int k = warp * 32 + 8 * t; k - 8 * t < a.k; k += WARPS * 32) {
-            const uint4 p = load16(w0, k, a.k), q = load16(w1, k, a.k);
+const auto block = [&](auto load, int k) {
+            const uint4 p = load(w0, k), q = load(w1, k);
+            uint4 x[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) x[nb] = load(xr[nb], k);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
-                const uint4 x = load16(xr[nb], k, a.k);
-                mma16<T>(acc[nb], p.x, q.x, p.y, q.y, x.x, x.y);
-                mma16<T>(acc[nb], p.z, q.z, p.w, q.w, x.z, x.w);
+                mma16<T>(acc[nb], p.x, q.x, p.y, q.y, x[nb].x, x[nb].y);
+                mma16<T>(acc[nb], p.z, q.z, p.w, q.w, x[nb].z, x[nb].w);
             }
-        }
+        };
+        int k = warp * 32;
+#pragma unroll 4
+        for (; k + 32 <= a.k; k += WARPS * 32) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
+        if (k < a.k) block([&](const T* row, int at) { return load16(row, at, a.k); }, k + 8 * t);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -609,9 +622,9 @@ cudaError_t small_launch(const ProjectArgs& a, cudaStream_t s) {
     KScope ks("adapter_project", s);
     if (warps == 16) {
         const cudaError_t e = ensure_smem(k_project_small<T, NB, 16>, smem);
-        return e != cudaSuccess ? e : launch_dependent(k_project_small<T, NB, 16>, grid, 512, smem, s, a);
+        return e != cudaSuccess ? e : launch_dependent(1, k_project_small<T, NB, 16>, grid, 512, smem, s, a);
     }
-    return launch_dependent(k_project_small<T, NB, 8>, grid, 256, smem, s, a);
+    return launch_dependent(1, k_project_small<T, NB, 8>, grid, 256, smem, s, a);
 }
 
 template <class T>

@@ -1,7 +1,7 @@
 // sm100.cuh -- the asynchronous copies, barriers, tensor-core instructions
 // and launch attributes of sm_100a that the decode-step kernels use.
 //
-// Every wait ends: after kWaitNs the waiting thread counts the event in
+// Every wait ends: after kWaitCycles the waiting thread counts the event in
 // g_expired_waits, marks its CTA (`dead`) so that the CTA's other waits end
 // too, and the kernel returns without the results of that CTA.
 #pragma once
@@ -18,7 +18,7 @@ cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p
 
 namespace {
 
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr long long kWaitCycles = 4000000000ll;  // 2 s and more
 
 __device__ unsigned long long g_expired_waits;
 
@@ -37,45 +37,52 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* b) {
 __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
         : "r"(smem_u32(b)), "r"(parity)
         : "memory");
     return ok;
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
 // Waits for the phase `parity` of b to end; false when it did not in time.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, uint32_t* dead) {
     if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = now_ns();
+    const long long t0 = clock64();
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 64; i++)
             if (mbar_try(b, parity)) return true;
         if (*reinterpret_cast<volatile uint32_t*>(dead)) return false;
-        if (now_ns() - t0 > kWaitNs) {
+        if (clock64() - t0 > kWaitCycles) {
             atomicAdd(&g_expired_waits, 1ull);
             atomicExch(dead, 1u);
             return false;
         }
     }
 }
-// After an expired wait: gives what is in flight towards b a bounded time.
-__device__ __forceinline__ void settle(uint64_t* b) {
-    const unsigned long long t0 = now_ns();
-    const uint32_t s = smem_u32(b);
-    while (now_ns() - t0 < 1000000ull) {
-        uint32_t ok;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(ok)
-            : "r"(s), "r"(0u)
-            : "memory");
-    }
+// After an expired wait: a bounded time for what is in flight.
+__device__ __forceinline__ void settle() {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000) __nanosleep(1000);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address of the same shared-memory variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 
 // Position in a ring of barriers and the parity of its current phase.
@@ -88,19 +95,50 @@ struct Ring {
     }
 };
 
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* b) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(b))
-        : "memory");
+// One box of a tensor map to this CTA's shared memory; `bar` (a cluster
+// address) may be the other CTA's of a pair (CG = 2).
+template <int CG>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+            : "memory");
 }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// The other way: one box from this CTA's shared memory, as a bulk group of
+// the calling thread.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+                 "r"(y), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// Until the stores have read their shared memory, but for the last N groups.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+}
+template <int CG>
 __device__ __forceinline__ void tmem_free(uint32_t t, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols));
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -127,20 +165,37 @@ __device__ __forceinline__ uint64_t desc_k128(uint32_t addr) { return desc_of(ad
 __device__ __forceinline__ uint64_t desc_k64(uint32_t addr) { return desc_of(addr, 16, 512, 4); }
 __device__ __forceinline__ uint64_t desc_mn128(uint32_t addr, uint32_t mn) { return desc_of(addr, mn, 1024, 2); }
 
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-        "l"(b), "r"(idesc), "r"(add)
-        : "memory");
+    if constexpr (CG == 2)
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(add)
+                     : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(add)
+                     : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void mma_tf32(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-        "l"(b), "r"(idesc), "r"(add)
-        : "memory");
+    if constexpr (CG == 2)
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(add)
+                     : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(add)
+                     : "memory");
 }
+// Arrives at b (in both CTAs of a pair) when the instructions so far are done.
+template <int CG>
 __device__ __forceinline__ void mma_commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(b)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
 }
 // 32 columns of this warp's 32 lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
@@ -168,6 +223,12 @@ __device__ __forceinline__ void st_shared4(uint32_t at, uint32_t a, uint32_t b, 
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ uint4 ld_shared4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // Programmatic dependent launch: the dependent kernel may start once every
 // CTA of the one before it has called release_dependents, and sees that
 // kernel's results after grid_dependency_wait.
@@ -175,17 +236,21 @@ __device__ __forceinline__ void release_dependents() { asm volatile("griddepcont
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <class... KArgs, class... Args>
-cudaError_t launch_dependent(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
+cudaError_t launch_dependent(int cluster, void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(block, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
