@@ -129,19 +129,21 @@ bool rows_ok(const void* p, uint64_t rows, uint32_t cols, int64_t stride) {
 }
 
 // What a call does with its sizes and pointers, and where it puts it.
-// Workspace: low (and for the backward call u) in f32; 16-bit operands whose
-// rows are not on 16-byte boundaries are copied there first, as is the
-// factor B of the backward call, transposed, so that its contraction axis is
-// contiguous.
+// Workspace: low (and for the backward call u); 16-bit operands whose rows are
+// not on 16-byte boundaries are copied there first, as is the factor B of the
+// backward call, transposed, so that its contraction axis is contiguous; the
+// factor of the tensor-core projection in f32 with its flags; the tokens of
+// each adapter.
 struct Plan {
-    bool f32, small, low_vec;
-    bool pack_x, pack_w, pack_a, pack_grad, pack_b;
-    uint64_t low, u, x, w, a, grad, b, bytes;
+    bool f32, small, low_vec, out;
+    bool pack_x, pack_w, pack_a, pack_grad, pack_b, g32, lists;
+    uint64_t low, u, x, w, a, grad, b, g, bad, list, bytes;
 };
 
 Plan plan_of(const ts_adapter_args* a, int backward) {
     Plan p{};
     p.f32 = a->dtype == TS_DTYPE_F32;
+    p.out = !backward || a->out;
     const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride);
     const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in);
     p.small = !p.f32 && !backward && a->n <= (uint64_t)kSmallTokens && (!a->weight || (x_ok && w_ok));
@@ -156,6 +158,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_w = a->weight && !p.small && !w_ok;
         p.pack_a = !a_ok && whole_low;
         p.low_vec = (x_ok || p.pack_x) && (a_ok || p.pack_a);
+        p.g32 = !p.small;
     } else {
         p.pack_x = !x_ok && a->grad_a;
         p.pack_a = !a_ok && a->grad_a;
@@ -163,21 +166,26 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_grad = !rows_ok(a->grad, a->n, a->d_out, a->grad_stride);
         p.pack_b = true;
         p.low_vec = true;
+        p.g32 = a->out;
     }
+    p.lists = backward && a->grad_a;
     uint64_t at = 0;
     const auto take = [&](bool want, uint64_t bytes) {
         const uint64_t here = at;
         if (want) at += up(bytes);
         return here;
     };
-    const uint64_t low = a->n * low_stride((int)a->r) * 4;
-    p.low = take(true, low);
+    const uint64_t rs = low_stride((int)a->r), low = a->n * rs * 4, o = backward ? a->d_in : a->d_out;
+    p.low = take(!backward || a->grad_a, low);
     p.u = take(backward, low);
     p.x = take(p.pack_x, a->n * up8(a->d_in) * 2);
     p.w = take(p.pack_w, (uint64_t)a->d_out * up8(a->d_in) * 2);
     p.a = take(p.pack_a, (uint64_t)a->adapters * a->r * up8(a->d_in) * 2);
     p.grad = take(p.pack_grad, a->n * up8(a->d_out) * 2);
     p.b = take(p.pack_b, (uint64_t)a->adapters * a->r * up8(a->d_out) * 2);
+    p.g = take(p.g32, a->adapters * o * rs * 4);
+    p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * 4);
+    p.list = take(p.lists, (a->adapters + 1 + a->n) * 4);
     p.bytes = a->n ? at : 0;
     return p;
 }
@@ -202,7 +210,7 @@ int adapter_workspace(const ts_adapter_args* a, int backward, uint64_t* bytes) {
     return TS_OK;
 }
 
-// Rows of a matrix or factor as the kernels take them, copied to the
+// Rows of a matrix or factor as the kernels take them: copied to the
 // workspace first where `pack` is set.
 struct Rows {
     const void* p;
@@ -212,12 +220,20 @@ struct Rows {
 struct Work {
     const ts_adapter_args* a;
     cudaStream_t s;
-    cudaError_t e = cudaSuccess;
+    PackJobs jobs{};
+    int after_pack = 0;  // 2: what is packed is used by the next launch
     void* at(uint64_t off) const { return static_cast<char*>(a->workspace) + off; }
     Rows rows(bool pack, const void* p, uint64_t rows, uint32_t cols, long long stride, uint64_t off) {
         if (!pack) return {p, rows < 2 ? up8(cols) : stride};
-        if (e == cudaSuccess) e = launch_pack({p, 0, stride, 1, (long long)rows, 1, (int)cols, up8(cols), at(off)}, s);
+        jobs.add({PackJob::COPY, p, 0, stride, 1, (long long)rows, 1, (int)cols, up8(cols), at(off)});
+        after_pack = 2;
         return {at(off), up8(cols)};
+    }
+    cudaError_t pack() {
+        if (!jobs.jobs) return cudaSuccess;
+        if (!after_pack) after_pack = 1;
+        jobs.dtype = a->dtype;
+        return launch_pack(jobs, s);
     }
 };
 
@@ -230,19 +246,22 @@ int adapter_project(const ts_adapter_args* a) {
     if (dev.status != cudaSuccess) return cuda_status(dev.status);
     Work w{a, static_cast<cudaStream_t>(a->stream)};
     const long long n = (long long)a->n, rb = (long long)a->r * a->d_out;
-    const int r = (int)a->r;
+    const int r = (int)a->r, d_o = (int)a->d_out;
     float* low = static_cast<float*>(w.at(p.low));
     const Rows x = p.f32 ? Rows{a->x, a->x_stride} : w.rows(p.pack_x, a->x, a->n, a->d_in, a->x_stride, p.x);
     const Rows wt = p.f32 ? Rows{a->weight, a->weight_stride} : w.rows(p.pack_w, a->weight, a->d_out, a->d_in, a->weight_stride, p.w);
     Rows fa{a->lora_a, a->d_in};
     if (p.pack_a) fa = w.rows(true, a->lora_a, (uint64_t)a->adapters * a->r, a->d_in, a->d_in, p.a);
+    if (p.g32)
+        w.jobs.add({PackJob::TO_F32, a->lora_b, rb, r, 1, d_o, (int)a->adapters, r, low_stride(r), w.at(p.g), static_cast<uint32_t*>(w.at(p.bad))});
+    cudaError_t e = w.pack();
     const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low};
-    if (w.e == cudaSuccess) w.e = launch_low(&l, 1, a->dtype, p.low_vec, w.s);
-    const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, (int)a->d_out, r, wt.p, wt.stride, 0,
-                        a->bias, a->base, a->base_stride, low, {a->lora_b, rb, 1, r}, ids_of(a), a->out, a->out_stride};
-    if (w.e == cudaSuccess)
-        w.e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
-    return cuda_status(w.e);
+    if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, w.after_pack, w.s);
+    const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low,
+                        {a->lora_b, rb, 1, r}, static_cast<float*>(w.at(p.g)), static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+    if (e == cudaSuccess)
+        e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
+    return cuda_status(e);
 }
 
 int adapter_project_backward(const ts_adapter_args* a) {
@@ -270,23 +289,34 @@ int adapter_project_backward(const ts_adapter_args* a) {
         wt = w.rows(p.pack_w, a->weight, a->d_out, a->d_in, a->weight_stride, p.w);
         grad = w.rows(p.pack_grad, a->grad, a->n, a->d_out, a->grad_stride, p.grad);
         if (p.pack_a) fa = w.rows(true, a->lora_a, (uint64_t)a->adapters * a->r, a->d_in, a->d_in, p.a);
-        if (w.e == cudaSuccess) w.e = launch_pack({a->lora_b, rb, 1, r, r, (int)a->adapters, d_o, up8(a->d_out), w.at(p.b)}, w.s);
+        w.jobs.add({PackJob::COPY, a->lora_b, rb, 1, r, r, (int)a->adapters, d_o, up8(a->d_out), w.at(p.b)});
+        w.after_pack = 2;
         fb = {w.at(p.b), (long long)r * up8(a->d_out), up8(a->d_out), 1};
     }
+    if (p.g32)
+        w.jobs.add({PackJob::TO_F32, a->lora_a, ra, 1, di, di, (int)a->adapters, r, low_stride(r), w.at(p.g), static_cast<uint32_t*>(w.at(p.bad))});
+    int* first = static_cast<int*>(w.at(p.list));
+    if (p.lists) {
+        PackJob j{PackJob::LISTS};
+        j.rows = n, j.count = (int)a->adapters, j.dst = first, j.id = ids_of(a);
+        w.jobs.add(j);
+    }
+    cudaError_t e = w.pack();
     const LowArgs l[2] = {{grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, u},
                           {x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low}};
-    if (w.e == cudaSuccess) w.e = launch_low(l, a->grad_a ? 2 : 1, a->dtype, p.low_vec, w.s);
-    if (w.e == cudaSuccess && a->out) {
-        const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1,
-                            nullptr, nullptr, 0, u, {a->lora_a, ra, di, 1}, ids_of(a), a->out, a->out_stride};
-        w.e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
+    if (e == cudaSuccess) e = launch_low(l, a->grad_a ? 2 : 1, a->dtype, p.low_vec, w.after_pack, w.s);
+    if (e == cudaSuccess && a->out) {
+        const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u,
+                            {a->lora_a, ra, di, 1}, static_cast<float*>(w.at(p.g)), static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+        e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }
-    if (w.e == cudaSuccess && a->grad_a) {
-        const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}}, n, r, ids_of(a)};
+    if (e == cudaSuccess && a->grad_a) {
+        const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}},
+                         r, (int)a->adapters, first, first + a->adapters + 1};
         const bool vec = !p.f32 || (aligned_to(x.p, 16) && x.stride % 4 == 0 && aligned_to(grad.p, 16) && grad.stride % 4 == 0);
-        w.e = launch_grads(g, a->dtype, vec, w.s);
+        e = launch_grads(g, n, a->dtype, vec, w.s);
     }
-    return cuda_status(w.e);
+    return cuda_status(e);
 }
 
 int logit_rules(const ts_rules_args* a) {

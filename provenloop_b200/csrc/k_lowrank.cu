@@ -13,6 +13,8 @@
 // The kernels below are these lines; a factor's strides turn the forward
 // form into the backward one.  Sums are held in f32 and each result is
 // rounded to its type once.
+#include <climits>
+
 #include "launch.cuh"
 #include "lowrank.cuh"
 #include "sm100.cuh"
@@ -101,14 +103,11 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const uint32_t (&a)[4],
 
 // ---------------------------------------------------------------- packing
 
-// Copies rows to 16-byte boundaries, or transposes a factor: 32 x 32 tiles
-// through shared memory, read along whichever axis of src is contiguous.
-__global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
-    __shared__ uint16_t tile[32][33];
-    const uint16_t* src = static_cast<const uint16_t*>(a.src) + blockIdx.z * a.se;
-    uint16_t* dst = static_cast<uint16_t*>(a.dst) + (long long)blockIdx.z * a.rows * a.dst_cols;
-    const long long j0 = (long long)blockIdx.x * 32;
-    const int k0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+// 32 x 32 elements of a job through shared memory, read along whichever axis
+// of src is contiguous and handed over along k.
+template <class F>
+__device__ __forceinline__ void pack_tile(const PackJob& a, const uint16_t* src, long long j0, int k0, uint16_t (&tile)[32][33], F put) {
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
     for (int i = ty; i < 32; i += 8) {
         const long long j = j0 + (a.sk == 1 ? i : tx);
@@ -118,20 +117,110 @@ __global__ void __launch_bounds__(256) k_pack(const PackArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = ty; i < 32; i += 8)
-        if (j0 + i < a.rows && k0 + tx < a.dst_cols) dst[(j0 + i) * a.dst_cols + k0 + tx] = tile[i][tx];
+        if (j0 + i < a.rows && k0 + tx < a.dst_cols) put(j0 + i, k0 + tx, tile[i][tx]);
+    __syncthreads();
+}
+
+// Adapter e's tokens in order, and the number of tokens of lower adapters:
+// each block looks through all indexes.
+__device__ void pack_lists(const PackJob& a, int e) {
+    __shared__ int warp_own[8], warp_less[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* first = static_cast<int*>(a.dst);
+    int* list = first + a.count + 1;
+    int less = 0, own = 0;  // tokens of lower adapters, of this one
+    const auto scan = [&](auto see) {
+        // 256 tokens in a step, each step taken by every thread
+        long long m = 0;
+        for (; m + 2048 <= a.rows; m += 2048) {
+            int id[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) id[q] = a.id.of(m + q * 256 + threadIdx.x);
+#pragma unroll
+            for (int q = 0; q < 8; q++) see(id[q], m + q * 256 + threadIdx.x);
+        }
+        for (; m < a.rows; m += 256) see(m + threadIdx.x < a.rows ? a.id.of(m + threadIdx.x) : -1, m + threadIdx.x);
+    };
+    scan([&](int id, long long) { less += id >= 0 && id < e, own += id == e; });
+#pragma unroll
+    for (int q = 16; q; q >>= 1) less += __shfl_xor_sync(0xffffffffu, less, q), own += __shfl_xor_sync(0xffffffffu, own, q);
+    if (lane == 0) warp_less[warp] = less, warp_own[warp] = own;
+    __syncthreads();
+    less = own = 0;
+#pragma unroll
+    for (int w = 0; w < 8; w++) less += warp_less[w], own += warp_own[w];
+    if (threadIdx.x == 0) {
+        first[e] = less;
+        if (e + 1 == a.count) first[a.count] = less + own;
+    }
+    if (!own) return;
+    __syncthreads();
+    int at = less;
+    scan([&](int id, long long m) {
+        const bool mine = id == e;
+        const unsigned ball = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) warp_own[warp] = __popc(ball);
+        __syncthreads();
+        int before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) before += w < warp ? warp_own[w] : 0, total += warp_own[w];
+        if (mine) list[at + before + __popc(ball & ((1u << lane) - 1))] = (int)m;
+        at += total;
+        __syncthreads();
+    });
+}
+
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs jobs) {
+    release_dependents();
+    __shared__ uint16_t tile[32][33];
+    long long b = blockIdx.x;
+    int q = 0;
+    while (b >= jobs.job[q].blocks) b -= jobs.job[q++].blocks;
+    const PackJob& a = jobs.job[q];
+    if (a.kind == PackJob::LISTS) {
+        pack_lists(a, (int)b);
+    } else if (a.kind == PackJob::COPY) {
+        const long long tr = (a.rows + 31) / 32, tc = (a.dst_cols + 31) / 32;
+        const long long e = b / (tr * tc), in = b % (tr * tc);
+        uint16_t* dst = static_cast<uint16_t*>(a.dst) + e * a.rows * a.dst_cols;
+        pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, in % tr * 32, (int)(in / tr) * 32, tile,
+                  [&](long long j, int k, uint16_t v) { dst[j * a.dst_cols + k] = v; });
+    } else {
+        const long long tr = (a.rows + 127) / 128, e = b / tr, j0 = b % tr * 128;
+        float* dst = static_cast<float*>(a.dst) + e * a.rows * a.dst_cols;
+        bool bad = false;
+        for (long long j = j0; j < min(j0 + 128, a.rows); j += 32)
+            for (int k = 0; k < a.dst_cols; k += 32)
+                pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, j, k, tile, [&](long long jj, int kk, uint16_t v) {
+                    const float f = jobs.dtype == DT_BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+                    const bool ok = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
+                    bad |= !ok;
+                    dst[jj * a.dst_cols + kk] = ok ? f : 0.f;
+                });
+        bad = __syncthreads_or(bad);
+        if (threadIdx.x == 0) a.bad[e * tr + b % tr] = bad;
+    }
 }
 
 // ---------------------------------------------------------------- low
 
 struct LowPair {
     LowArgs a[2];
+    int after_pack;
 };
+
+// What is stored of a sum: see LowArgs.
+template <class T>
+__device__ __forceinline__ float low_value(float v) {
+    return sizeof(T) == 4 ? v : __uint_as_float(to_tf32(v));
+}
 
 // Token by token: WPJ warps share one rank index of one token.  Bound: reading
 // each token's own factor (r k elements), from L2 where tokens share it.
 template <class T, bool VEC, int WPJ>
 __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
     release_dependents();
+    if (both.after_pack == 2) grid_dependency_wait();
     const LowArgs a = both.a[blockIdx.z];
     const long long m = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPJ;
@@ -165,7 +254,9 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
             for (int q = 0; q < WPJ; q++) v += part_sum[warp + q];
         }
     }
-    if (part == 0 && lane == 0 && j < rs) a.low[m * rs + j] = e >= 0 && j < a.r ? (a.scale ? a.scale[e] * v : v) : 0.f;
+    if (part == 0 && lane == 0 && j < rs) a.low[m * rs + j] = e >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e] * v : v) : 0.f;
+    // the next launch waits for this one, and with it for the packing
+    if (both.after_pack == 1) grid_dependency_wait();
 }
 
 // 32 tokens per cluster of S CTAs, 8 S warps sharing the contraction in
@@ -177,6 +268,7 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
 template <class T>
 __global__ void __launch_bounds__(256) k_low_mma(const LowPair both) {
     release_dependents();
+    if (both.after_pack == 2) grid_dependency_wait();
     const LowArgs a = both.a[blockIdx.z];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -250,13 +342,14 @@ const auto block = [&](auto load, int k) {
                 if (mine >> row & 1 && j < rs) {
                     float v = 0.f;
                     for (int q = 0; q < S; q++) v += S > 1 ? *cluster.map_shared_rank(&sum[row][i & 31], q) : sum[row][i & 31];
-                    a.low[(m0 + row) * rs + j] = j < a.r ? scale * v : 0.f;
+                    a.low[(m0 + row) * rs + j] = j < a.r ? low_value<T>(scale * v) : 0.f;
                 }
             }
             if (S > 1) cluster.sync();
             else __syncthreads();
         }
     }
+    if (both.after_pack == 1) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------- projection
@@ -382,7 +475,6 @@ const auto block = [&](auto load, int k) {
 
 // ---------------------------------------------------------------- gradients of the factors
 
-constexpr int kGradScan = 2048;  // ids looked through at a time
 constexpr int kGradStages = 4;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -401,19 +493,16 @@ struct GradTile {
 };
 
 // One adapter, 128 features and RB * 8 rank indexes per cluster of S CTAs.
-// Every CTA looks through the adapter indexes, keeps the positions of its
-// share of the adapter's tokens (every S-th group of 32, in order), gathers
+// Every CTA takes every S-th group of 32 of the adapter's tokens, gathers
 // their rows and sums low^T x with 16 x 8 x 8 TF32 products: features are
-// the 16-row axis, tokens the contraction.  16-bit x is exact in TF32; low
-// is rounded to 11 significant bits; for f32 inputs both are split into two
-// TF32 parts, which leaves 2^-22.  The partial sums of the cluster meet in
-// shared memory in a fixed order.  Bound: reading x once per 64 rank indexes.
+// the 16-row axis, tokens the contraction.  16-bit x is exact in TF32, and
+// low has been rounded to it; for f32 inputs both are split into two TF32
+// parts, which leaves 2^-22.  The partial sums of the cluster meet in shared
+// memory in a fixed order.  Bound: reading x once per 64 rank indexes.
 template <class T, int RB>
 __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int vec) {
     using L = GradTile<T, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int list[kGradScan + 64];
-    __shared__ int warp_count[8];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tile = blockIdx.x / S;
@@ -426,62 +515,40 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
     const uint32_t base = smem_u32(smem);
     float acc[2][RB][4] = {};
 
-    long long found = 0;  // tokens of the adapter before this round
-    for (long long m0 = 0; m0 < both.n; m0 += kGradScan) {
-        for (int i = threadIdx.x; i < kGradScan + 64; i += 256) list[i] = -1;
-        unsigned hits = 0;
-        const long long at = m0 + threadIdx.x * 8;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (at + i < both.n && both.id.of(at + i) == e) hits |= 1u << i;
-        const int cnt = __popc(hits);
-        int before = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += y;
-        }
-        if (lane == 31) warp_count[warp] = before;
-        __syncthreads();
-        int total = 0;
-        before -= cnt;
-#pragma unroll
-        for (int w = 0; w < 8; w++) before += w < warp ? warp_count[w] : 0, total += warp_count[w];
-        const auto own_before = [&](long long group) { return group / S + (group % S > rank); };  // own groups below `group`
-        const long long first = own_before(found >> 5);
-        while (hits) {
-            const int i = __ffs(hits) - 1;
-            hits &= hits - 1;
-            const long long pos = found + before++;
-            if ((pos >> 5) % S == rank) list[(int)(own_before(pos >> 5) - first) * 32 + (int)(pos & 31)] = (int)(at - m0) + i;
-        }
-        const int groups = total ? (int)(own_before(((found + total - 1) >> 5) + 1) - first) : 0;
-        found += total;
-        __syncthreads();
-
+    const int begin = both.first[e], tokens = both.first[e + 1] - begin;
+    const int* list = both.list + begin;
+    const int all = (tokens + 31) / 32, groups = all / S + (all % S > rank);
+    {
+        const auto token = [&](int q, int row) {
+            const int at = (q * S + rank) * 32 + row;
+            return at < tokens ? list[at] : -1;
+        };
         const auto fetch = [&](int q) {
             if (q < groups) {
                 const uint32_t sx = base + (q % kGradStages) * (L::kX + L::kU), su = sx + L::kX;
                 constexpr int V = 16 / sizeof(T), C = 128 / V;
                 if (sizeof(T) == 4 && !vec) {
                     for (int i = threadIdx.x; i < 32 * 128; i += 256) {
-                        const int row = i >> 7, c = i & 127, m = list[q * 32 + row];
+                        const int row = i >> 7, c = i & 127;
+                        const long long m = token(q, row);
                         const bool in = m >= 0 && k0 + c < a.k;
-                        cp_async4(sx + row * L::kRow + c * 4, in ? x + (m0 + m) * a.x_stride + k0 + c : x, in ? 4 : 0);
+                        cp_async4(sx + row * L::kRow + c * 4, in ? x + m * a.x_stride + k0 + c : x, in ? 4 : 0);
                     }
                 } else {
 #pragma unroll
                     for (int i = threadIdx.x; i < 32 * C; i += 256) {
-                        const int row = i / C, c = i % C * V, m = list[q * 32 + row];
+                        const int row = i / C, c = i % C * V;
+                        const long long m = token(q, row);
                         const int left = m >= 0 ? min(V, max(0, a.k - k0 - c)) : 0;
-                        cp_async16(sx + row * L::kRow + c * (int)sizeof(T), left ? x + (m0 + m) * a.x_stride + k0 + c : x, left * (int)sizeof(T));
+                        cp_async16(sx + row * L::kRow + c * (int)sizeof(T), left ? x + m * a.x_stride + k0 + c : x, left * (int)sizeof(T));
                     }
                 }
 #pragma unroll
                 for (int i = threadIdx.x; i < 32 * RB * 2; i += 256) {
-                    const int row = i / (RB * 2), c = i % (RB * 2) * 4, m = list[q * 32 + row];
+                    const int row = i / (RB * 2), c = i % (RB * 2) * 4;
+                    const long long m = token(q, row);
                     const bool in = m >= 0 && j0 + c < rs;
-                    cp_async16(su + (row * L::kURow + c) * 4, in ? a.low + (m0 + m) * rs + j0 + c : a.low, in ? 16 : 0);
+                    cp_async16(su + (row * L::kURow + c) * 4, in ? a.low + m * rs + j0 + c : a.low, in ? 16 : 0);
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -527,7 +594,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
 #pragma unroll
                 for (int nb = 0; nb < RB; nb++) {
                     const float b0 = su[tok * L::kURow + nb * 8 + g], b1 = su[(tok + 4) * L::kURow + nb * 8 + g];
-                    const uint32_t m0b = to_tf32(b0), m1b = to_tf32(b1);
+                    const uint32_t m0b = sizeof(T) == 4 ? to_tf32(b0) : __float_as_uint(b0), m1b = sizeof(T) == 4 ? to_tf32(b1) : __float_as_uint(b1);
 #pragma unroll
                     for (int q2 = 0; q2 < 2; q2++) {
                         if constexpr (sizeof(T) == 4) {
@@ -583,8 +650,8 @@ int sm_count() {
 }
 
 template <class T>
-cudaError_t low_launch(const LowArgs* a, int count, bool vec, cudaStream_t s) {
-    const LowPair both{{a[0], a[count - 1]}};
+cudaError_t low_launch(const LowArgs* a, int count, bool vec, int after_pack, cudaStream_t s) {
+    const LowPair both{{a[0], a[count - 1]}, after_pack};
     const long long n = a[0].n;
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     KScope ks("adapter_low", s);
@@ -595,21 +662,18 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, cudaStream_t s) {
             const long long tiles = (n + 31) / 32;
             int S = 1;
             while (S < 8 && tiles * S * count < sm_count() && kmax / (S * 2) >= 512) S *= 2;
-            return launch_cl(S, k_low_mma<T>, dim3((unsigned)(tiles * S), 1, count), 256, 0, s, both);
+            const dim3 grid((unsigned)(tiles * S), 1, count);
+            return after_pack ? launch_dependent(S, k_low_mma<T>, grid, 256, 0, s, both) : launch_cl(S, k_low_mma<T>, grid, 256, 0, s, both);
         }
     }
     // long contractions over more warps, to have more loads in flight
     const int rs = low_stride(a[0].r);
-    if (kmax * sizeof(T) > 4096) {
-        const dim3 grid((unsigned)n, (rs + 1) / 2, count);
-        if (vec) k_low_token<T, true, 4><<<grid, 256, 0, s>>>(both);
-        else k_low_token<T, false, 4><<<grid, 256, 0, s>>>(both);
-    } else {
-        const dim3 grid((unsigned)n, (rs + 7) / 8, count);
-        if (vec) k_low_token<T, true, 1><<<grid, 256, 0, s>>>(both);
-        else k_low_token<T, false, 1><<<grid, 256, 0, s>>>(both);
-    }
-    return cudaGetLastError();
+    const auto go = [&](auto kern, int ranks) {
+        const dim3 grid((unsigned)n, (rs + ranks - 1) / ranks, count);
+        return after_pack ? launch_dependent(1, kern, grid, 256, 0, s, both) : launch_cl(1, kern, grid, 256, 0, s, both);
+    };
+    if (kmax * sizeof(T) > 4096) return vec ? go(k_low_token<T, true, 4>, 2) : go(k_low_token<T, false, 4>, 2);
+    return vec ? go(k_low_token<T, true, 1>, 8) : go(k_low_token<T, false, 1>, 8);
 }
 
 template <class T, int NB>
@@ -636,26 +700,25 @@ cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
 }
 
 template <class T, int RB>
-cudaError_t grad_launch(const GradPair& a, bool vec, cudaStream_t s) {
+cudaError_t grad_launch(const GradPair& a, long long n, bool vec, cudaStream_t s) {
     using L = GradTile<T, RB>;
     const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
     // CTAs that share an adapter's tokens: until there are two for each SM,
     // while each has two groups of tokens on average
-    const long long ctas = (long long)(t0 + t1) * passes * a.id.count;
+    const long long ctas = (long long)(t0 + t1) * passes * a.adapters;
     int S = 1;
-    while (S < 8 && ctas * S < 2 * sm_count() && a.n / a.id.count >= 128 * S) S *= 2;
-    // the list is beside it: raise the limit even where the tiles alone fit the default
-    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 16);
+    while (S < 8 && ctas * S < 2 * sm_count() && n / a.adapters >= 128 * S) S *= 2;
+    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem);
     if (e != cudaSuccess) return e;
     KScope ks("adapter_grad", s);
-    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.id.count), 256, L::kSmem, s, a, t0, (int)vec);
+    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.adapters), 256, L::kSmem, s, a, t0, (int)vec);
 }
 
 template <class T>
-cudaError_t grad_width(const GradPair& a, bool vec, cudaStream_t s) {
-    if (a.r <= 16) return grad_launch<T, 2>(a, vec, s);
-    if (a.r <= 32) return grad_launch<T, 4>(a, vec, s);
-    return grad_launch<T, 8>(a, vec, s);
+cudaError_t grad_width(const GradPair& a, long long n, bool vec, cudaStream_t s) {
+    if (a.r <= 16) return grad_launch<T, 2>(a, n, vec, s);
+    if (a.r <= 32) return grad_launch<T, 4>(a, n, vec, s);
+    return grad_launch<T, 8>(a, n, vec, s);
 }
 
 }  // namespace
@@ -668,14 +731,17 @@ cudaError_t grad_width(const GradPair& a, bool vec, cudaStream_t s) {
     }                                                                  \
     return cudaErrorInvalidValue;
 
-cudaError_t launch_pack(const PackArgs& a, cudaStream_t s) {
+cudaError_t launch_pack(const PackJobs& a, cudaStream_t s) {
+    long long blocks = 0;
+    for (int q = 0; q < a.jobs; q++) blocks += a.job[q].blocks;
+    if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
     KScope ks("adapter_pack", s);
-    k_pack<<<dim3((unsigned)((a.rows + 31) / 32), (a.dst_cols + 31) / 32, a.count), 256, 0, s>>>(a);
+    k_pack<<<(unsigned)blocks, 256, 0, s>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, cudaStream_t s) {
-    TSG_DTYPE_SWITCH(dtype, return low_launch<T>(a, count, vec, s));
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int after_pack, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return low_launch<T>(a, count, vec, after_pack, s));
 }
 
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
@@ -688,8 +754,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
     return dtype == DT_BF16 ? small_width<__nv_bfloat16>(a, s) : small_width<__half>(a, s);
 }
 
-cudaError_t launch_grads(const GradPair& a, int dtype, bool vec, cudaStream_t s) {
-    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, vec, s));
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, vec, s));
 }
 
 }  // namespace tsg

@@ -13,19 +13,19 @@
 // the 48 KiB that a 128 x 256 tile of its own would need.  What bounds large
 // n is these slices' way from L2 more than the tensor cores.
 //
-// The low-rank term is a few more steps of the same contraction.  Its axis
-// lists the rank indexes of the tile's distinct adapters one adapter after the
-// other; four builder warps write 16 of them at a time as TF32 operands: rows
-// of low, zero except in the token's own adapter's columns, and the
-// factor's columns.  So a tile whose tokens share an adapter (prefill,
-// training) pays r / 16 steps and a mixed one D r / 16 for D distinct
-// adapters, without sorting tokens or a second pass over out.  TF32 holds
-// bf16 and fp16 factors exactly and rounds low to 11 significant bits with
-// the range of f32, so that an fp16 low above 65504 does not overflow.
+// The low-rank term is a few more steps of the same contraction, 16 rank
+// indexes of one adapter at a time, for each distinct adapter of the tile:
+// four builder warps write the tokens' rows of low, zero for other
+// adapters' tokens, and TMA brings the factor's rows, both as TF32.  So a tile
+// whose tokens share an adapter (prefill, training) pays r / 16 steps and a
+// mixed one D r / 16 for D distinct adapters, without sorting tokens or a
+// second pass over out.  TF32 holds bf16 and fp16 factors exactly and low to
+// 11 significant bits with the range of f32, so that an fp16 low above
+// 65504 does not overflow.  The factors are converted once per call (k_pack).
 //
 // A zero times an adapter's NaN or infinity would spread to the other
-// tokens of the tile: the builders replace such elements by 0, flag the tile,
-// and the epilogue adds those terms to the adapter's own tokens only.
+// tokens of the tile: k_pack replaces such elements by 0 and flags them, and
+// the epilogue adds their terms to the adapter's own tokens only.
 #include <cuda.h>
 
 #include "launch.cuh"
@@ -36,32 +36,32 @@ namespace tsg {
 
 namespace {
 
-constexpr int kThreads = 320;  // warps 0-3 epilogue, 4-7 builders, 8 TMA, 9 matrix instructions
-constexpr int kXK = 16;        // low-rank columns per step
+constexpr int kThreads = 448;  // warps 0-7 epilogue, 8-11 builders, 12 TMA, 13 matrix instructions
+constexpr int kXK = 16;        // rank indexes per step
 
 template <int CG, int BN>
 struct Tile {
     static constexpr int kRows = BN / CG;                       // of W or the factor in a CTA
     static constexpr int kStage = 128 * 128 + kRows * 128;      // bytes: 64 16-bit elements of each row
     static constexpr int kXStage = (128 + kRows) * kXK * 4;     // TF32 operands
-    static constexpr int kXBufs = 2;
+    static constexpr int kXBufs = 3;
     static constexpr int kStages = 4;
-    static constexpr int kOut = 4 * 2 * 4096;                   // per epilogue warp two boxes of 32 rows x 64 outputs
+    static constexpr int kOut = 8 * 2 * 2048;                   // per epilogue warp two boxes of 32 rows x 32 outputs
     static constexpr int kSmem = kStages * kStage + kXBufs * kXStage + kOut + 1024 /* alignment */;
 };
 
 struct TcArgs {
     ProjectArgs p;
     int tiles_m, tiles_n, kblocks;
-    int vec_bias, vec_g;  // 16-byte loads are aligned
+    int vec_bias;         // 16-byte loads are aligned
     int tma_out;          // out, and base if there is one, take TMA boxes
 };
 
 // Everything beside the operand rings.
 struct Shared {
-    uint64_t full[8], empty[8], xfull[2], xempty[2], acc_full[2], acc_empty[2], drained, base_full[4][2];
+    uint64_t full[8], empty[8], xfull[4], xempty[4], acc_full[2], acc_empty[2], drained, base_full[8][2];
     uint32_t tmem, dead;
-    uint32_t xlast[2];
+    uint32_t xlast[4];
     uint32_t bad[8];  // by tile: an element of a factor is not finite
     alignas(16) int ids[256];
     int list[256], pos[256], warp_new[8];
@@ -98,7 +98,7 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
 template <class T, int CG, int BN, bool W_MN>
 __global__ void __launch_bounds__(kThreads, 1)
 k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
-             const __grid_constant__ CUtensorMap mout, const __grid_constant__ CUtensorMap mbase) {
+             const __grid_constant__ CUtensorMap mg, const __grid_constant__ CUtensorMap mout, const __grid_constant__ CUtensorMap mbase) {
     using L = Tile<CG, BN>;
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
@@ -110,17 +110,15 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.xfull[i], CG), mbar_init(&sh.xempty[i], 1);
-            mbar_init(&sh.acc_full[i], 1), mbar_init(&sh.acc_empty[i], 128 * CG);
-        }
+        for (int i = 0; i < L::kXBufs; i++) mbar_init(&sh.xfull[i], CG), mbar_init(&sh.xempty[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&sh.acc_full[i], 1), mbar_init(&sh.acc_empty[i], 256 * CG);
         mbar_init(&sh.drained, 1);
-        for (int i = 0; i < 8; i++) mbar_init(&sh.base_full[i >> 1][i & 1], 1);
+        for (int i = 0; i < 16; i++) mbar_init(&sh.base_full[i >> 1][i & 1], 1);
         sh.dead = 0;
         for (int i = 0; i < 8; i++) sh.bad[i] = 0;
         mbar_init_fence();
     }
-    if (warp == 9) tmem_alloc<CG>(&sh.tmem, 2 * BN);
+    if (warp == 13) tmem_alloc<CG>(&sh.tmem, 2 * BN);
     tc_fence_before();
     if constexpr (CG == 2) cluster_sync_all();
     else __syncthreads();
@@ -129,7 +127,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
     const int tiles = a.tiles_m * a.tiles_n, step = gridDim.x / CG;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;  // rank 0 issues the pair's instructions
 
-    if (warp == 8) {
+    if (warp == 12) {
         if (lane == 0) {
             Ring r(L::kStages, 1);
             for (int t = blockIdx.x / CG; t < tiles; t += step) {
@@ -150,7 +148,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             }
         tma_done:;
         }
-    } else if (warp == 9) {
+    } else if (warp == 13) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
             constexpr uint32_t shape = 1u << 4 | (uint32_t)(BN >> 3) << 17 | (128u * CG >> 4) << 24;
@@ -195,12 +193,13 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             }
         mma_done:;
         }
-    } else if (warp >= 4) {
-        // builders: thread i has row i of the CTA's tokens and kRows / 128
-        // rows of the factor; both CTAs of a pair list the adapters of all
-        // 128 CG tokens, in the order of their first tokens
-        const int i = threadIdx.x - 128, w = warp - 4;
-        grid_dependency_wait();  // low is written by the launch before this one
+    } else if (warp >= 8) {
+        // builders: thread i has row i of the CTA's tokens; both CTAs of a
+        // pair list the adapters of all 128 CG tokens, in the order of their
+        // first tokens
+        const int i = threadIdx.x - 256, w = warp - 8;
+        const int rs = low_stride(p.r), blocks = (p.o + 127) / 128;
+        grid_dependency_wait();  // low and the converted factors are written by the launches before
         Ring x(L::kXBufs, 1);
         int serial = 0;
         for (int t = blockIdx.x / CG; t < tiles; t += step, serial++) {
@@ -214,9 +213,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 e[h] = m0 + h * 128 + i < p.n ? p.id.of(m0 + h * 128 + i) : -1;
                 sh.ids[h * 128 + i] = e[h];
             }
-            // two tiles ahead: a pair's other CTA may have flagged the next tile
-            // already, and the epilogue is at most five behind
-            if (i == 0) sh.bad[(serial + 2) & 7] = 0;
+            if (i == 0) sh.bad[serial & 7] = 0;  // the epilogue is less than eight tiles behind
             bar_sync(1, 128);
 #pragma unroll
             for (int h = 0; h < CG; h++) {
@@ -249,115 +246,37 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 }
             bar_sync(1, 128);
             const int mine = CG == 2 && rank ? e[CG - 1] : e[0], mine_first = CG == 2 && rank ? first[CG - 1] : first[0];
-            const int own = mine >= 0 ? sh.pos[mine_first] * p.r : 1 << 30;  // this row's first column
-            const int cols = distinct * p.r;
-            const float* low = p.low + (m < p.n ? m : 0) * low_stride(p.r);
-            bool bad = false;
-            // kAhead steps of loads are in flight in registers: every load is
-            // made, from a clamped place, and selected where it is used
-            constexpr int H = (L::kRows + 127) / 128, kAhead = 3;
-            struct Step {
-                float a[kXK];
-                uint32_t b[H][kXK / 2];
-            } ahead[kAhead];
-            const auto load = [&](int c0, Step& st) {
-                if (p.r % 4 == 0) {
+            const int own = mine >= 0 ? sh.pos[mine_first] : -1;  // this row's adapter in the list
+            const float4* low = reinterpret_cast<const float4*>(p.low + (m < p.n ? m : 0) * rs);
+            const int tile_o = t / a.tiles_m * BN, blk = tile_o / 128;
+            for (int d = i; d < distinct; d += 128) {
+                const uint32_t* f = p.bad + (long long)sh.list[d] * blocks + blk;
+                if (f[0] || (BN == 256 && blk + 1 < blocks && f[1])) sh.bad[serial & 7] = 1;
+            }
+            const int steps = max(1, distinct);
+            for (int j = 0; j < rs; j += kXK) {
+                float4 f[4];
 #pragma unroll
-                    for (int q = 0; q < kXK; q += 4) {
-                        const int j = c0 + q - own;
-                        const float4 f = *reinterpret_cast<const float4*>(low + (j >= 0 && j < p.r ? j : 0));
-                        st.a[q] = f.x, st.a[q + 1] = f.y, st.a[q + 2] = f.z, st.a[q + 3] = f.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < kXK; q++) {
-                        const int j = c0 + q - own;
-                        st.a[q] = low[j >= 0 && j < p.r ? j : 0];
-                    }
-                }
-                if (a.vec_g) {
-#pragma unroll
-                    for (int q = 0; q < kXK; q += 8) {
-                        const int d = (c0 + q) / p.r, j = c0 + q - d * p.r;
-                        const T* g = static_cast<const T*>(p.g.p) + (d < distinct ? sh.list[d] * p.g.se + j : 0);
-#pragma unroll
-                        for (int h = 0; h < H; h++) {
-                            const int o = o0 + i + h * 128;
-                            const uint4 f = *reinterpret_cast<const uint4*>(g + (o < p.o ? o * p.g.sk : 0));
-                            st.b[h][q / 2] = f.x, st.b[h][q / 2 + 1] = f.y, st.b[h][q / 2 + 2] = f.z, st.b[h][q / 2 + 3] = f.w;
-                        }
-                    }
-                } else {
-                    int d = c0 / p.r, j = c0 - d * p.r;
-                    uint16_t v[H][kXK];
-#pragma unroll
-                    for (int q = 0; q < kXK; q++) {
-                        const uint16_t* g = static_cast<const uint16_t*>(p.g.p) + (d < distinct ? sh.list[d] * p.g.se + j * p.g.sj : 0);
-#pragma unroll
-                        for (int h = 0; h < H; h++) {
-                            const int o = o0 + i + h * 128;
-                            v[h][q] = g[o < p.o ? o * p.g.sk : 0];
-                        }
-                        if (++j == p.r) j = 0, d++;
-                    }
-#pragma unroll
-                    for (int h = 0; h < H; h++)
-#pragma unroll
-                        for (int q = 0; q < kXK / 2; q++) st.b[h][q] = v[h][2 * q] | (uint32_t)v[h][2 * q + 1] << 16;
-                }
-            };
-            const int steps = max(1, (cols + kXK - 1) / kXK);
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-                if (u < steps) load(u * kXK, ahead[u]);
-            for (int c = 0; c < steps; c += kAhead) {
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) {
-                    if (c + u >= steps) break;
-                    Step& st = ahead[u];
-                    const int c0 = (c + u) * kXK;
+                for (int q = 0; q < 4; q++) f[q] = low[j / 4 + q];
+                for (int d = 0; d < steps; d++, x.next()) {
                     const bool late = !mbar_wait(&sh.xempty[x.i], x.phase, &sh.dead);
                     const uint32_t s = xring + x.i * L::kXStage;
-                    uint32_t v[kXK];
-#pragma unroll
-                    for (int q = 0; q < kXK; q++) {
-                        const int j = c0 + q - own;
-                        v[q] = j >= 0 && j < p.r ? to_tf32(st.a[q]) : 0u;
+                    if (i == 0) {
+                        const uint32_t bar = CG == 2 ? map_rank(&sh.xfull[x.i], 0) : smem_u32(&sh.xfull[x.i]);
+                        tma_3d<CG>(s + 128 * kXK * 4, &mg, j, o0, distinct ? sh.list[d] : 0, bar);
+                        sh.xlast[x.i] = j + kXK >= rs && d + 1 == steps;
                     }
+                    const bool in = d == own;
 #pragma unroll
-                    for (int q = 0; q < kXK / 4; q++)
-                        st_shared4(s + i * 64 + ((q ^ (i >> 1 & 3)) << 4), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-#pragma unroll
-                    for (int h = 0; h < H; h++) {
-                        if (L::kRows < 128 && i >= L::kRows) break;
-                        const int row = i + h * 128;
-#pragma unroll
-                        for (int q = 0; q < kXK / 2; q++) {
-                            const float2 f = unpack2<T>(st.b[h][q]);
-                            const bool in0 = c0 + 2 * q < cols && o0 + row < p.o, in1 = c0 + 2 * q + 1 < cols && o0 + row < p.o;
-                            const bool ok0 = is_finite(f.x), ok1 = is_finite(f.y);
-                            v[2 * q] = in0 && ok0 ? __float_as_uint(f.x) : 0u;
-                            v[2 * q + 1] = in1 && ok1 ? __float_as_uint(f.y) : 0u;
-                            bad |= (in0 && !ok0) || (in1 && !ok1);
-                        }
-#pragma unroll
-                        for (int q = 0; q < kXK / 4; q++)
-                            st_shared4(s + 128 * kXK * 4 + row * 64 + ((q ^ (row >> 1 & 3)) << 4), v[4 * q], v[4 * q + 1], v[4 * q + 2],
-                                       v[4 * q + 3]);
-                    }
-                    if (bad) {
-                        sh.bad[serial & 7] = 1;
-                        if constexpr (CG == 2) st_cluster(map_rank(&sh.bad[serial & 7], rank ^ 1), 1);
-                    }
-                    if (i == 0) sh.xlast[x.i] = c + u + 1 == steps;
+                    for (int q = 0; q < 4; q++)
+                        st_shared4(s + i * 64 + ((q ^ (i >> 1 & 3)) << 4), in ? __float_as_uint(f[q].x) : 0u, in ? __float_as_uint(f[q].y) : 0u,
+                                   in ? __float_as_uint(f[q].z) : 0u, in ? __float_as_uint(f[q].w) : 0u);
                     fence_async_shared();
                     if (bar_or(1, 128, late)) goto build_done;  // all 128 threads or none
                     if (i == 0) {
-                        if constexpr (CG == 2) mbar_arrive_at(map_rank(&sh.xfull[x.i], 0));
-                        else mbar_arrive(&sh.xfull[x.i]);
+                        if (rank == 0) mbar_expect(&sh.xfull[x.i], CG * L::kRows * kXK * 4);
+                        else mbar_arrive_at(map_rank(&sh.xfull[x.i], 0));
                     }
-                    x.next();
-                    if (c + u + kAhead < steps) load(c0 + kAhead * kXK, st);
                 }
             }
         }
@@ -366,7 +285,8 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
         Ring acc(2, 0);
         int serial = 0;
         uint32_t base_phase = 0;  // bit: the phase of base_full[warp][buffer]
-        const uint32_t boxes = out_boxes + warp * 8192;
+        const uint32_t boxes = out_boxes + warp * 4096;
+        const int quarter = warp & 3, half = warp >> 2;  // of the accumulator's lanes, of its columns
         // This row's terms of elements of the factor that are not finite
         const auto add_bad = [&](long long m, int e, int o, float (&v)[32]) {
             for (int q = 0; q < 32 && o + q < p.o; q++)
@@ -400,14 +320,14 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             }
         };
         for (int t = blockIdx.x / CG; t < tiles; t += step, acc.next(), serial++) {
-            const int m0 = (t % a.tiles_m * CG + (int)rank) * 128 + warp * 32;  // this warp's first token
+            const int m0 = (t % a.tiles_m * CG + (int)rank) * 128 + quarter * 32;  // this warp's first token
             const long long m = (long long)m0 + lane;
-            const int o0 = t / a.tiles_m * BN;
-            const int groups = m0 < p.n ? (min(BN, p.o - o0) + 63) / 64 : 0;  // of 64 outputs
+            const int o0 = t / a.tiles_m * BN + half * (BN / 2);
+            const int groups = m0 < p.n ? (max(0, min(BN / 2, p.o - o0)) + 31) / 32 : 0;  // of 32 outputs
             const bool tma_base = a.tma_out && p.base;
             const auto fetch_base = [&](int g) {  // one lane; its buffer's last store has been read
-                mbar_expect(&sh.base_full[warp][g & 1], 4096);
-                tma_2d<1>(boxes + (g & 1) * 4096, &mbase, o0 + g * 64, m0, smem_u32(&sh.base_full[warp][g & 1]));
+                mbar_expect(&sh.base_full[warp][g & 1], 2048);
+                tma_2d<1>(boxes + (g & 1) * 2048, &mbase, o0 + g * 32, m0, smem_u32(&sh.base_full[warp][g & 1]));
             };
             if (tma_base && groups && lane == 0) {
                 tma_store_wait_read<0>();
@@ -416,7 +336,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             __syncwarp();
             if (!__all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc.i], acc.phase, &sh.dead))) break;
             tc_fence_after();
-            const uint32_t d = tmem + acc.i * BN + ((uint32_t)warp << 21);  // lane 32 * warp
+            const uint32_t d = tmem + acc.i * BN + half * (BN / 2) + ((uint32_t)quarter << 21);  // lane 32 * quarter
             const bool row = m < p.n;
             const bool bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[serial & 7]);
             const int e = bad && row ? p.id.of(m) : -1;
@@ -424,7 +344,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 // through shared memory, so that rows leave as whole boxes; base
                 // comes the same way into the box that takes the result
                 for (int g = 0; g < groups; g++) {
-                    const uint32_t box = boxes + (g & 1) * 4096;
+                    const uint32_t box = boxes + (g & 1) * 2048;
                     if (lane == 0) {
                         if (tma_base) {
                             tma_store_wait_read<0>();
@@ -433,46 +353,41 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                             tma_store_wait_read<1>();
                         }
                     }
+                    float v[32];
                     __syncwarp();
+                    tmem_ld32(d + g * 32, v);
+                    if (p.bias) add_bias(o0 + g * 32, v);
+                    if (e >= 0) add_bad(m, e, o0 + g * 32, v);
                     if (tma_base) {
                         mbar_wait(&sh.base_full[warp][g & 1], base_phase >> (g & 1) & 1, &sh.dead);
                         base_phase ^= 1u << (g & 1);
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int c = g * 64 + h * 32;
-                        float v[32];
-                        __syncwarp();
-                        tmem_ld32(d + c, v);
-                        if (p.bias) add_bias(o0 + c, v);
-                        if (e >= 0) add_bad(m, e, o0 + c, v);
+                    for (int q = 0; q < 4; q++) {
+                        const uint32_t at = box + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4);
+                        uint32_t u[4];
+                        if (tma_base) {
+                            const uint4 b = ld_shared4(at);
+                            u[0] = b.x, u[1] = b.y, u[2] = b.z, u[3] = b.w;
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t at = box + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4);
-                            uint32_t u[4];
-                            if (tma_base) {
-                                const uint4 b = ld_shared4(at);
-                                u[0] = b.x, u[1] = b.y, u[2] = b.z, u[3] = b.w;
-#pragma unroll
-                                for (int z = 0; z < 4; z++) {
-                                    const float2 f = unpack2<T>(u[z]);
-                                    v[q * 8 + 2 * z] += f.x, v[q * 8 + 2 * z + 1] += f.y;
-                                }
+                            for (int z = 0; z < 4; z++) {
+                                const float2 f = unpack2<T>(u[z]);
+                                v[q * 8 + 2 * z] += f.x, v[q * 8 + 2 * z + 1] += f.y;
                             }
-#pragma unroll
-                            for (int z = 0; z < 4; z++) u[z] = pack2<T>(v[q * 8 + 2 * z], v[q * 8 + 2 * z + 1]);
-                            st_shared4(at, u[0], u[1], u[2], u[3]);
                         }
+#pragma unroll
+                        for (int z = 0; z < 4; z++) u[z] = pack2<T>(v[q * 8 + 2 * z], v[q * 8 + 2 * z + 1]);
+                        st_shared4(at, u[0], u[1], u[2], u[3]);
                     }
                     fence_async_shared();
                     __syncwarp();
-                    if (lane == 0) tma_store_2d(&mout, o0 + g * 64, m0, box);
+                    if (lane == 0) tma_store_2d(&mout, o0 + g * 32, m0, box);
                 }
             } else {
                 // rows that are not on 16-byte boundaries
                 T* out = static_cast<T*>(p.out) + m * p.out_stride;
                 const T* base = static_cast<const T*>(p.base) + m * p.base_stride;
-                for (int c = 0; c < groups * 64 && o0 + c < p.o; c += 32) {
+                for (int c = 0; c < groups * 32; c += 32) {
                     float v[32];
                     __syncwarp();
                     tmem_ld32(d + c, v);
@@ -506,7 +421,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
     if (sh.dead && threadIdx.x == 0) settle();
     if constexpr (CG == 2) cluster_sync_all();
     else __syncthreads();
-    if (warp == 9) tmem_free<CG>(tmem, 2 * BN);
+    if (warp == 13) tmem_free<CG>(tmem, 2 * BN);
 }
 
 template <class T, int CG, int BN, bool W_MN>
@@ -520,13 +435,17 @@ cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
     const auto rows = [&](const void* q, long long stride) { return vec(q, p.n < 2 ? 0 : stride) && (p.n < 2 || (stride >= p.o && stride < (1ll << 38))); };
     a.tma_out = rows(p.out, p.out_stride) && (!p.base || rows(p.base, p.base_stride));
     a.vec_bias = vec(p.bias, 0);
-    a.vec_g = p.g.sj == 1 && vec(p.g.p, p.r);
-    CUtensorMap mx{}, mw{}, mout{}, mbase{};
+    CUtensorMap mx{}, mw{}, mg{}, mout{}, mbase{};
     const CUtensorMapDataType ty = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (a.tma_out) {
         const auto pitch = [&](long long stride) { return (uint64_t)(p.n < 2 ? (p.o + 7) / 8 * 8 : stride) * 2; };
-        cudaError_t e = tensor_map(&mout, ty, p.out, (uint64_t)p.o, (uint64_t)p.n, pitch(p.out_stride), 64, 32);
-        if (e == cudaSuccess && p.base) e = tensor_map(&mbase, ty, p.base, (uint64_t)p.o, (uint64_t)p.n, pitch(p.base_stride), 64, 32);
+        cudaError_t e = tensor_map(&mout, ty, p.out, (uint64_t)p.o, (uint64_t)p.n, pitch(p.out_stride), 32, 32);
+        if (e == cudaSuccess && p.base) e = tensor_map(&mbase, ty, p.base, (uint64_t)p.o, (uint64_t)p.n, pitch(p.base_stride), 32, 32);
+        if (e != cudaSuccess) return e;
+    }
+    {
+        const int rs = low_stride(p.r);
+        const cudaError_t e = tensor_map(&mg, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, p.g32, rs, p.o, (uint64_t)rs * 4, kXK, L::kRows, p.id.count);
         if (e != cudaSuccess) return e;
     }
     if (p.w) {
@@ -541,7 +460,7 @@ cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     KScope ks("adapter_project", s);
     const long long tiles = (long long)a.tiles_m * a.tiles_n, slots = sms / CG;
-    return launch_dependent(CG, kern, dim3((unsigned)(tiles < slots ? tiles : slots) * CG), kThreads, L::kSmem, s, a, mx, mw, mout, mbase);
+    return launch_dependent(CG, kern, dim3((unsigned)(tiles < slots ? tiles : slots) * CG), kThreads, L::kSmem, s, a, mx, mw, mg, mout, mbase);
 }
 
 template <class T, bool W_MN>
@@ -561,7 +480,7 @@ cudaError_t launch_width(const ProjectArgs& p, int sms, cudaStream_t s) {
 }  // namespace
 
 cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p, uint64_t cols, uint64_t rows, uint64_t row_bytes,
-                       uint32_t box_cols, uint32_t box_rows) {
+                       uint32_t box_cols, uint32_t box_rows, uint64_t count) {
     using Encode = decltype(&cuTensorMapEncodeTiled);
     static const Encode encode = [] {
         void* f = nullptr;
@@ -570,10 +489,12 @@ cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p
         return reinterpret_cast<Encode>(f);
     }();
     if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
-    const CUresult r = encode(out, type, 2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const uint32_t box_bytes = box_cols * (type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2);
+    const cuuint64_t dims[3] = {cols, rows, count}, strides[2] = {row_bytes, row_bytes * rows};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1}, step[3] = {1, 1, 1};
+    const CUresult r = encode(out, type, count ? 3 : 2, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 

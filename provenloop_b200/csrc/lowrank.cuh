@@ -35,14 +35,16 @@ struct Factor {
     long long se, sj, sk;
 };
 
-// Rows of low are padded to a multiple of four, zero behind r.
+// Rows of low are padded to a multiple of 16, zero behind r.
 #ifdef __CUDACC__
 __host__ __device__
 #endif
-inline int low_stride(int r) { return (r + 3) & ~3; }
+inline int low_stride(int r) { return (r + 15) & ~15; }
 
 // low[m][j] = scale_e * sum_k x[m][k] F[e][j][k] (f32 [n][low_stride(r)];
-// zero rows where a token has no adapter).
+// zero rows where a token has no adapter).  For 16-bit inputs the values are
+// rounded to TF32 (11 significant bits, the range of f32): what multiplies
+// them are matrix instructions on TF32, and their factors have fewer bits.
 struct LowArgs {
     const void* x;
     long long x_stride;
@@ -70,6 +72,8 @@ struct ProjectArgs {
     long long base_stride;
     const float* low;
     Factor g;  // sk here is the stride of o
+    const float* g32;     // g as f32 [e][o][low_stride(r)], elements that are not finite replaced by 0 (k_project.cu only)
+    const uint32_t* bad;  // [e][ceil(o / 128)]: some of them are
     AdapterIds id;
     void* out;
     long long out_stride;
@@ -87,19 +91,33 @@ struct GradArgs {
 };
 struct GradPair {
     GradArgs g[2];
-    long long n;
-    int r;
-    AdapterIds id;
+    int r, adapters;
+    const int* first;  // [adapters + 1]: adapter e's tokens, in order, are list[first[e] .. first[e + 1])
+    const int* list;
 };
 
-// dst[e][j][k] (rows of `dst_cols` 16-bit elements, zeros behind `cols`) =
-// src[e * se + j * sj + k * sk].
-struct PackArgs {
-    const void* src;
+// What a call lays out in its workspace first, in one launch: copies of
+// operands whose rows are not on 16-byte boundaries (or factors transposed),
+// factors as f32, the tokens of each adapter.
+struct PackJob {
+    enum Kind : int { COPY, TO_F32, LISTS } kind;
+    const void* src;  // COPY, TO_F32: element (e, j, k) at e * se + j * sj + k * sk
     long long se, sj, sk;
-    long long rows;
+    long long rows;  // j
     int count, cols, dst_cols;
-    void* dst;
+    void* dst;      // [count][rows][dst_cols], zeros behind cols: 16-bit elements / f32
+    uint32_t* bad;  // TO_F32: [count][ceil(rows / 128)]
+    AdapterIds id;  // LISTS: dst is first [count + 1], then the list [rows]
+    long long blocks;
+};
+constexpr int kMaxPack = 7;
+struct PackJobs {
+    PackJob job[kMaxPack];
+    int jobs, dtype;
+    void add(PackJob j) {
+        j.blocks = j.kind == PackJob::LISTS ? j.count : j.kind == PackJob::TO_F32 ? (j.rows + 127) / 128 * j.count : ((j.rows + 31) / 32) * ((j.dst_cols + 31) / 32) * j.count;
+        job[jobs++] = j;
+    }
 };
 
 // The kernels that a call takes go by its sizes; decode_ops.cu lays out the
@@ -107,10 +125,12 @@ struct PackArgs {
 constexpr int kTokenLow = 128;    // up to here, and for f32, low is computed token by token
 constexpr int kSmallTokens = 64;  // up to here W is streamed once past all tokens
 
-cudaError_t launch_pack(const PackArgs& a, cudaStream_t s);
+cudaError_t launch_pack(const PackJobs& a, cudaStream_t s);
 // one or two of them (the same n, r and id) in one launch; `vec`: rows of x
-// and f start on 16-byte boundaries and f.sk is 1
-cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, cudaStream_t s);
+// and f start on 16-byte boundaries and f.sk is 1; `after_pack`: launch_pack
+// was queued directly before, and its results are used here (2) or by the
+// next launch only (1), else 0
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int after_pack, cudaStream_t s);
 // f32, any strides
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s);
 // 16-bit types, at most kSmallTokens tokens; x and w (not transposed) on 16-byte boundaries
@@ -118,7 +138,7 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
 // 16-bit types; x and w rows on 16-byte boundaries (k_project.cu)
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
 // rows of x on 16-byte boundaries, but for f32 (`vec`: they are)
-cudaError_t launch_grads(const GradPair& a, int dtype, bool vec, cudaStream_t s);
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s);
 // waits of k_project.cu that ran out on the current device so far
 cudaError_t expired_waits(unsigned long long* out);
 

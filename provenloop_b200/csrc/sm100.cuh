@@ -11,10 +11,11 @@
 
 namespace tsg {
 
-// tensor map of a row-major matrix [rows][cols] of 16-bit elements in boxes
-// of box_cols x box_rows with 128-byte swizzle (k_project.cu)
+// Tensor map of a row-major matrix [rows][cols], or of `count` of them one
+// behind the other, in boxes of box_cols x box_rows; boxes 64 bytes wide have
+// the 64-byte swizzle, others (128 bytes) the 128-byte one (k_project.cu).
 cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p, uint64_t cols, uint64_t rows, uint64_t row_bytes,
-                       uint32_t box_cols, uint32_t box_rows);
+                       uint32_t box_cols, uint32_t box_rows, uint64_t count = 0);
 
 namespace {
 
@@ -111,6 +112,20 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
             : "memory");
 }
 
+template <int CG>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+}
 // The other way: one box from this CTA's shared memory, as a bulk group of
 // the calling thread.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
