@@ -147,7 +147,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride);
     const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in);
     p.small = !p.f32 && !backward && a->n <= (uint64_t)kSmallTokens && (!a->weight || (x_ok && w_ok));
-    const bool whole_low = a->n > (uint64_t)kTokenLow;  // low by matrix instructions: aligned operands only
+    const bool whole_low = !low_by_token((long long)a->n, a->d_in, a->d_in, a->r);  // by matrix instructions: aligned operands only
     if (p.f32) {
         const auto ok = [](const void* q, uint32_t cols, int64_t stride, uint64_t rows) {
             return aligned_to(q, 16) && (rows < 2 || (stride % 4 == 0 && stride >= cols));
@@ -158,7 +158,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_w = a->weight && !p.small && !w_ok;
         p.pack_a = !a_ok && whole_low;
         p.low_vec = (x_ok || p.pack_x) && (a_ok || p.pack_a);
-        p.g32 = !p.small;
+        p.g32 = !p.small && !factor_by_token((long long)a->n, a->d_out, a->r);
     } else {
         p.pack_x = !x_ok && a->grad_a;
         p.pack_a = !a_ok && a->grad_a;
@@ -166,7 +166,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_grad = !rows_ok(a->grad, a->n, a->d_out, a->grad_stride);
         p.pack_b = true;
         p.low_vec = true;
-        p.g32 = a->out;
+        p.g32 = a->out && !factor_by_token((long long)a->n, a->d_in, a->r);
     }
     p.lists = backward && a->grad_a;
     uint64_t at = 0;
@@ -184,7 +184,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     p.grad = take(p.pack_grad, a->n * up8(a->d_out) * 2);
     p.b = take(p.pack_b, (uint64_t)a->adapters * a->r * up8(a->d_out) * 2);
     p.g = take(p.g32, a->adapters * o * rs * 4);
-    p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * 4);
+    p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * (rs / 16) * 4);
     p.list = take(p.lists, (a->adapters + 1 + a->n) * 4);
     p.bytes = a->n ? at : 0;
     return p;
@@ -258,7 +258,7 @@ int adapter_project(const ts_adapter_args* a) {
     const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low};
     if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, w.after_pack, w.s);
     const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low,
-                        {a->lora_b, rb, 1, r}, static_cast<float*>(w.at(p.g)), static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+                        {a->lora_b, rb, 1, r}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
     if (e == cudaSuccess)
         e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
     return cuda_status(e);
@@ -307,7 +307,7 @@ int adapter_project_backward(const ts_adapter_args* a) {
     if (e == cudaSuccess) e = launch_low(l, a->grad_a ? 2 : 1, a->dtype, p.low_vec, w.after_pack, w.s);
     if (e == cudaSuccess && a->out) {
         const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u,
-                            {a->lora_a, ra, di, 1}, static_cast<float*>(w.at(p.g)), static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+                            {a->lora_a, ra, di, 1}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
         e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }
     if (e == cudaSuccess && a->grad_a) {

@@ -104,21 +104,56 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const uint32_t (&a)[4],
 // ---------------------------------------------------------------- packing
 
 // 32 x 32 elements of a job through shared memory, read along whichever axis
-// of src is contiguous and handed over along k.
-template <class F>
-__device__ __forceinline__ void pack_tile(const PackJob& a, const uint16_t* src, long long j0, int k0, uint16_t (&tile)[32][33], F put) {
+// of src is contiguous, written along k.
+__device__ __forceinline__ void pack_tile(const PackJob& a, const uint16_t* src, uint16_t* dst, long long j0, int k0) {
+    __shared__ uint16_t tile[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    uint16_t v[4];
 #pragma unroll
-    for (int i = ty; i < 32; i += 8) {
-        const long long j = j0 + (a.sk == 1 ? i : tx);
-        const int k = k0 + (a.sk == 1 ? tx : i);
-        tile[(int)(j - j0)][k - k0] = j < a.rows && k < a.cols ? src[j * a.sj + k * a.sk] : (uint16_t)0;
+    for (int i = 0; i < 4; i++) {  // loads from clamped places overlap, loads under a condition do not
+        const long long j = min(j0 + (a.sk == 1 ? ty + 8 * i : tx), a.rows - 1);
+        const int k = min(k0 + (a.sk == 1 ? tx : ty + 8 * i), a.cols - 1);
+        v[i] = src[j * a.sj + k * a.sk];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int j = a.sk == 1 ? ty + 8 * i : tx, k = a.sk == 1 ? tx : ty + 8 * i;
+        tile[j][k] = k0 + k < a.cols ? v[i] : (uint16_t)0;
     }
     __syncthreads();
 #pragma unroll
     for (int i = ty; i < 32; i += 8)
-        if (j0 + i < a.rows && k0 + tx < a.dst_cols) put(j0 + i, k0 + tx, tile[i][tx]);
+        if (j0 + i < a.rows && k0 + tx < a.dst_cols) dst[(j0 + i) * a.dst_cols + k0 + tx] = tile[i][tx];
+}
+
+// 128 rows x 16 columns of a factor as f32.
+__device__ __forceinline__ bool pack_f32(const PackJob& a, const uint16_t* src, float* dst, long long j0, int k0, int dtype) {
+    __shared__ float tile[128][17];
+    uint16_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int q = threadIdx.x + 256 * i;
+        const long long j = min(j0 + (a.sk == 1 ? q >> 4 : q & 127), a.rows - 1);
+        const int k = min(k0 + (a.sk == 1 ? q & 15 : q >> 7), a.cols - 1);
+        v[i] = src[j * a.sj + k * a.sk];
+    }
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int q = threadIdx.x + 256 * i;
+        const int j = a.sk == 1 ? q >> 4 : q & 127, k = a.sk == 1 ? q & 15 : q >> 7;
+        const float f = dtype == DT_BF16 ? __uint_as_float((uint32_t)v[i] << 16) : __half2float(__ushort_as_half(v[i]));
+        const bool in = j0 + j < a.rows && k0 + k < a.cols, ok = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
+        bad |= in && !ok;
+        tile[j][k] = in && ok ? f : 0.f;
+    }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int q = threadIdx.x + 256 * i;
+        if (j0 + (q >> 4) < a.rows) dst[(j0 + (q >> 4)) * a.dst_cols + k0 + (q & 15)] = tile[q >> 4][q & 15];
+    }
+    return bad;
 }
 
 // Adapter e's tokens in order, and the number of tokens of lower adapters:
@@ -172,7 +207,6 @@ __device__ void pack_lists(const PackJob& a, int e) {
 
 __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs jobs) {
     release_dependents();
-    __shared__ uint16_t tile[32][33];
     long long b = blockIdx.x;
     int q = 0;
     while (b >= jobs.job[q].blocks) b -= jobs.job[q++].blocks;
@@ -180,25 +214,16 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs j
     if (a.kind == PackJob::LISTS) {
         pack_lists(a, (int)b);
     } else if (a.kind == PackJob::COPY) {
-        const long long tr = (a.rows + 31) / 32, tc = (a.dst_cols + 31) / 32;
-        const long long e = b / (tr * tc), in = b % (tr * tc);
-        uint16_t* dst = static_cast<uint16_t*>(a.dst) + e * a.rows * a.dst_cols;
-        pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, in % tr * 32, (int)(in / tr) * 32, tile,
-                  [&](long long j, int k, uint16_t v) { dst[j * a.dst_cols + k] = v; });
+        const long long tr = (a.rows + 31) / 32, tc = (a.dst_cols + 31) / 32, e = b / (tr * tc), in = b % (tr * tc);
+        pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, static_cast<uint16_t*>(a.dst) + e * a.rows * a.dst_cols, in % tr * 32,
+                  (int)(in / tr) * 32);
     } else {
-        const long long tr = (a.rows + 127) / 128, e = b / tr, j0 = b % tr * 128;
-        float* dst = static_cast<float*>(a.dst) + e * a.rows * a.dst_cols;
-        bool bad = false;
-        for (long long j = j0; j < min(j0 + 128, a.rows); j += 32)
-            for (int k = 0; k < a.dst_cols; k += 32)
-                pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, j, k, tile, [&](long long jj, int kk, uint16_t v) {
-                    const float f = jobs.dtype == DT_BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-                    const bool ok = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
-                    bad |= !ok;
-                    dst[jj * a.dst_cols + kk] = ok ? f : 0.f;
-                });
-        bad = __syncthreads_or(bad);
-        if (threadIdx.x == 0) a.bad[e * tr + b % tr] = bad;
+        const int tc = a.dst_cols / 16;
+        const long long tr = (a.rows + 127) / 128, e = b / (tr * tc);
+        const bool bad = pack_f32(a, static_cast<const uint16_t*>(a.src) + e * a.se, static_cast<float*>(a.dst) + e * a.rows * a.dst_cols,
+                                  b / tc % tr * 128, (int)(b % tc) * 16, jobs.dtype);
+        const int any = __syncthreads_or(bad);
+        if (threadIdx.x == 0) a.bad[b] = any;
     }
 }
 
@@ -413,69 +438,118 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a) {
     }
 }
 
-// Few tokens: a CTA streams 16 rows of W once past all tokens, its warps
-// sharing the contraction in 32-wide blocks (operands as in k_low_mma, W as
-// the 16-row operand).  Bound: reading W; the stream starts before low is
-// there, and waits for it only to add the adapters' terms.
-template <class T, int NB, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) k_project_small(const ProjectArgs a) {
-    const int o0 = blockIdx.x * 16;
+// sum_j low[j] b[j] for a row of a factor; 16 bytes at a time where r and the
+// row allow, else 4, else 2.
+template <class T>
+__device__ __forceinline__ float dot_low(const float* low, const T* b, long long sj, int r, float v) {
+    if (sj == 1 && (r & 7) == 0 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+#pragma unroll 4
+        for (int j = 0; j < r; j += 8) {
+            const uint4 u = *reinterpret_cast<const uint4*>(b + j);
+            const float4 p = *reinterpret_cast<const float4*>(low + j), q = *reinterpret_cast<const float4*>(low + j + 4);
+            const float2 f0 = pair_f<T>(u.x), f1 = pair_f<T>(u.y), f2 = pair_f<T>(u.z), f3 = pair_f<T>(u.w);
+            v = fmaf(p.x, f0.x, v), v = fmaf(p.y, f0.y, v), v = fmaf(p.z, f1.x, v), v = fmaf(p.w, f1.y, v);
+            v = fmaf(q.x, f2.x, v), v = fmaf(q.y, f2.y, v), v = fmaf(q.z, f3.x, v), v = fmaf(q.w, f3.y, v);
+        }
+    } else if (sj == 1 && (r & 1) == 0 && (reinterpret_cast<uintptr_t>(b) & 3) == 0) {
+#pragma unroll 16
+        for (int j = 0; j < r; j += 2) {
+            const float2 f = pair_f<T>(*reinterpret_cast<const uint32_t*>(b + j));
+            v = fmaf(low[j], f.x, v), v = fmaf(low[j + 1], f.y, v);
+        }
+    } else {
+#pragma unroll 16
+        for (int j = 0; j < r; j++) v = fmaf(low[j], to_f(b[j * sj]), v);
+    }
+    return v;
+}
+
+// Few tokens: a cluster of S CTAs streams 16 MT rows of W once past NB * 8
+// tokens, its 8 S warps sharing the contraction in 32-wide blocks (operands
+// as in k_low_mma, W as the 16-row operand).  Bound: reading W, and with many
+// tokens the re-reads of x, which MT = 2 halves; the stream starts before low
+// is there, and waits for it only to add the adapters' terms.
+template <class T, int NB, int MT>
+__global__ void __launch_bounds__(256) k_project_small(const ProjectArgs a) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int o0 = (blockIdx.x / S) * 16 * MT;
+    const long long m0 = (long long)blockIdx.y * NB * 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    extern __shared__ float red[];  // [WARPS][16][NB * 8 + 1]
+    extern __shared__ float red[];  // [8][16 MT][RS], the sums over the warps in the first
     constexpr int RS = NB * 8 + 1;
     if (a.w) {
-        float acc[NB][4] = {};
-        const T* w = static_cast<const T*>(a.w);
-        const T* w0 = w + (long long)min(o0 + g, a.o - 1) * a.w_stride;
-        const T* w1 = w + (long long)min(o0 + g + 8, a.o - 1) * a.w_stride;
+        float acc[MT][NB][4] = {};
+        const T* wr[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; i++) wr[i] = static_cast<const T*>(a.w) + (long long)min(o0 + g + 8 * i, a.o - 1) * a.w_stride;
         const T* xr[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min((long long)(nb * 8 + g), a.n - 1) * a.x_stride;
-const auto block = [&](auto load, int k) {
-            const uint4 p = load(w0, k), q = load(w1, k);
-            uint4 x[NB];
+        for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min(m0 + nb * 8 + g, a.n - 1) * a.x_stride;
+        const auto block = [&](auto load, int k) {
+            uint4 w[2 * MT], x[NB];
+#pragma unroll
+            for (int i = 0; i < 2 * MT; i++) w[i] = load(wr[i], k);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) x[nb] = load(xr[nb], k);
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                mma16<T>(acc[nb], p.x, q.x, p.y, q.y, x[nb].x, x[nb].y);
-                mma16<T>(acc[nb], p.z, q.z, p.w, q.w, x[nb].z, x[nb].w);
-            }
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    mma16<T>(acc[i][nb], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, x[nb].x, x[nb].y);
+                    mma16<T>(acc[i][nb], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, x[nb].z, x[nb].w);
+                }
         };
-        int k = warp * 32;
-#pragma unroll 4
-        for (; k + 32 <= a.k; k += WARPS * 32) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
+        int k = (rank * 8 + warp) * 32;
+        constexpr int kUnroll = NB * MT >= 8 ? 2 : 4;
+#pragma unroll kUnroll
+        for (; k + 32 <= a.k; k += S * 256) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
         if (k < a.k) block([&](const T* row, int at) { return load16(row, at, a.k); }, k + 8 * t);
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) red[(warp * 16 + g + (c >> 1) * 8) * RS + nb * 8 + 2 * t + (c & 1)] = acc[nb][c];
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    red[(warp * 16 * MT + i * 16 + g + (c >> 1) * 8) * RS + nb * 8 + 2 * t + (c & 1)] = acc[i][nb][c];
+        __syncthreads();
+        if (S > 1) {
+            for (int i = threadIdx.x; i < 16 * MT * NB * 8; i += 256) {
+                float* p = red + (i / (NB * 8)) * RS + i % (NB * 8);
+                float v = 0.f;
+#pragma unroll
+                for (int q = 0; q < 8; q++) v += p[q * 16 * MT * RS];
+                *p = v;
+            }
+            cluster.sync();
+        }
     }
-    __syncthreads();
     grid_dependency_wait();
-    const int rs = low_stride(a.r);
-    for (int i = threadIdx.x; i < 16 * NB * 8; i += WARPS * 32) {
-        const int o = o0 + (i & 15), m = i >> 4;
+    const int rs = low_stride(a.r), per = 16 * MT * NB * 8 / S;
+    for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += 256) {
+        const int row = i % (16 * MT), col = i / (16 * MT), o = o0 + row;
+        const long long m = m0 + col;
         if (o >= a.o || m >= a.n) continue;
         float v = a.bias ? to_f(static_cast<const T*>(a.bias)[o]) : 0.f;
-        if (a.w)
-#pragma unroll
-            for (int q = 0; q < WARPS; q++) v += red[(q * 16 + (i & 15)) * RS + m];
         if (a.base) v += to_f(static_cast<const T*>(a.base)[m * a.base_stride + o]);
         const int e = a.id.of(m);
-        if (e >= 0) {
-            const T* b = static_cast<const T*>(a.g.p) + e * a.g.se + o * a.g.sk;
-            const float* low = a.low + m * rs;
-#pragma unroll 8
-            for (int j = 0; j < a.r; j++) v = fmaf(low[j], to_f(b[j * a.g.sj]), v);
+        if (e >= 0) v = dot_low(a.low + m * rs, static_cast<const T*>(a.g.p) + e * a.g.se + o * a.g.sk, a.g.sj, a.r, v);
+        if (a.w) {
+            float* p = red + row * RS + col;
+            if (S > 1)
+                for (int q = 0; q < S; q++) v += *cluster.map_shared_rank(p, q);
+            else
+#pragma unroll
+                for (int q = 0; q < 8; q++) v += p[q * 16 * MT * RS];
         }
         static_cast<T*>(a.out)[m * a.out_stride + o] = from_f<T>(v);
     }
+    if (S > 1) cluster.sync();
 }
 
 // ---------------------------------------------------------------- gradients of the factors
 
-constexpr int kGradStages = 4;
+constexpr int kGradChunk = 64;  // groups whose tokens are listed in shared memory at a time
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -489,7 +563,8 @@ struct GradTile {
     static constexpr int kRow = sizeof(T) == 4 ? 136 * 4 : 288;  // 128 features; rows 8 banks apart
     static constexpr int kURow = RB * 8 + 8;                     // floats
     static constexpr int kX = 32 * kRow, kU = 32 * kURow * 4;
-    static constexpr int kSmem = kGradStages * (kX + kU);
+    static constexpr int kStages = kX + kU > 16384 ? 4 : 6;
+    static constexpr int kSmem = kStages * (kX + kU);
 };
 
 // One adapter, 128 features and RB * 8 rank indexes per cluster of S CTAs.
@@ -503,6 +578,7 @@ template <class T, int RB>
 __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int vec) {
     using L = GradTile<T, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int own[kGradChunk * 32];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tile = blockIdx.x / S;
@@ -517,20 +593,22 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
 
     const int begin = both.first[e], tokens = both.first[e + 1] - begin;
     const int* list = both.list + begin;
-    const int all = (tokens + 31) / 32, groups = all / S + (all % S > rank);
-    {
-        const auto token = [&](int q, int row) {
-            const int at = (q * S + rank) * 32 + row;
-            return at < tokens ? list[at] : -1;
-        };
+    const int all = (tokens + 31) / 32, mine = all / S + (all % S > rank);  // groups of 32, and this CTA's
+    for (int q0 = 0; q0 < mine; q0 += kGradChunk) {
+        const int groups = min(kGradChunk, mine - q0);
+        for (int i = threadIdx.x; i < groups * 32; i += 256) {
+            const int at = ((q0 + (i >> 5)) * S + rank) * 32 + (i & 31);
+            own[i] = at < tokens ? list[at] : -1;
+        }
+        __syncthreads();
         const auto fetch = [&](int q) {
             if (q < groups) {
-                const uint32_t sx = base + (q % kGradStages) * (L::kX + L::kU), su = sx + L::kX;
+                const uint32_t sx = base + (q % L::kStages) * (L::kX + L::kU), su = sx + L::kX;
                 constexpr int V = 16 / sizeof(T), C = 128 / V;
                 if (sizeof(T) == 4 && !vec) {
                     for (int i = threadIdx.x; i < 32 * 128; i += 256) {
                         const int row = i >> 7, c = i & 127;
-                        const long long m = token(q, row);
+                        const long long m = own[q * 32 + row];
                         const bool in = m >= 0 && k0 + c < a.k;
                         cp_async4(sx + row * L::kRow + c * 4, in ? x + m * a.x_stride + k0 + c : x, in ? 4 : 0);
                     }
@@ -538,7 +616,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
 #pragma unroll
                     for (int i = threadIdx.x; i < 32 * C; i += 256) {
                         const int row = i / C, c = i % C * V;
-                        const long long m = token(q, row);
+                        const long long m = own[q * 32 + row];
                         const int left = m >= 0 ? min(V, max(0, a.k - k0 - c)) : 0;
                         cp_async16(sx + row * L::kRow + c * (int)sizeof(T), left ? x + m * a.x_stride + k0 + c : x, left * (int)sizeof(T));
                     }
@@ -546,7 +624,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
 #pragma unroll
                 for (int i = threadIdx.x; i < 32 * RB * 2; i += 256) {
                     const int row = i / (RB * 2), c = i % (RB * 2) * 4;
-                    const long long m = token(q, row);
+                    const long long m = own[q * 32 + row];
                     const bool in = m >= 0 && j0 + c < rs;
                     cp_async16(su + (row * L::kURow + c) * 4, in ? a.low + m * rs + j0 + c : a.low, in ? 16 : 0);
                 }
@@ -554,12 +632,12 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int q = 0; q < kGradStages - 1; q++) fetch(q);
+        for (int q = 0; q < L::kStages - 1; q++) fetch(q);
         for (int q = 0; q < groups; q++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
             __syncthreads();
-            fetch(q + kGradStages - 1);
-            const uint8_t* sx = smem + (q % kGradStages) * (L::kX + L::kU);
+            fetch(q + L::kStages - 1);
+            const uint8_t* sx = smem + (q % L::kStages) * (L::kX + L::kU);
             const float* su = reinterpret_cast<const float*>(sx + L::kX);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -656,7 +734,7 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, int after_pack, cu
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     KScope ks("adapter_low", s);
     if constexpr (sizeof(T) == 2) {
-        if (n > kTokenLow) {
+        if (!low_by_token(n, a[0].k, a[count - 1].k, a[0].r)) {
             // as many CTAs share a contraction as it takes to give every SM
             // one, while each still has four blocks for a warp
             const long long tiles = (n + 31) / 32;
@@ -676,27 +754,26 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, int after_pack, cu
     return vec ? go(k_low_token<T, true, 1>, 8) : go(k_low_token<T, false, 1>, 8);
 }
 
-template <class T, int NB>
+template <class T, int NB, int MT>
 cudaError_t small_launch(const ProjectArgs& a, cudaStream_t s) {
-    // 16 warps where the contraction is long: an SM then has enough loads in
-    // flight for its share of the bandwidth
-    const int warps = a.k >= 4096 ? 16 : 8;
-    const size_t smem = (size_t)warps * 16 * (NB * 8 + 1) * 4;
-    const dim3 grid((a.o + 15) / 16);
+    // as many CTAs share a contraction as it takes to give every SM one,
+    // while each of their warps has four blocks
+    const long long tiles = (long long)((a.o + 16 * MT - 1) / (16 * MT)) * ((a.n + NB * 8 - 1) / (NB * 8));
+    int S = 1;
+    while (S < 8 && a.w && tiles * S < sm_count() && a.k >= S * 2048) S *= 2;
+    const size_t smem = (size_t)8 * 16 * MT * (NB * 8 + 1) * 4;
+    const dim3 grid((unsigned)((a.o + 16 * MT - 1) / (16 * MT) * S), (unsigned)((a.n + NB * 8 - 1) / (NB * 8)));
     KScope ks("adapter_project", s);
-    if (warps == 16) {
-        const cudaError_t e = ensure_smem(k_project_small<T, NB, 16>, smem);
-        return e != cudaSuccess ? e : launch_dependent(1, k_project_small<T, NB, 16>, grid, 512, smem, s, a);
-    }
-    return launch_dependent(1, k_project_small<T, NB, 8>, grid, 256, smem, s, a);
+    const cudaError_t e = ensure_smem(k_project_small<T, NB, MT>, smem);
+    return e != cudaSuccess ? e : launch_dependent(S, k_project_small<T, NB, MT>, grid, 256, smem, s, a);
 }
 
 template <class T>
 cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
-    if (a.n <= 8) return small_launch<T, 1>(a, s);
-    if (a.n <= 16) return small_launch<T, 2>(a, s);
-    if (a.n <= 32) return small_launch<T, 4>(a, s);
-    return small_launch<T, 8>(a, s);
+    if (a.n <= 8) return small_launch<T, 1, 1>(a, s);
+    if (a.n <= 16) return small_launch<T, 2, 1>(a, s);
+    if (a.n <= 32) return small_launch<T, 4, 1>(a, s);
+    return small_launch<T, 8, 2>(a, s);
 }
 
 template <class T, int RB>
@@ -708,7 +785,8 @@ cudaError_t grad_launch(const GradPair& a, long long n, bool vec, cudaStream_t s
     const long long ctas = (long long)(t0 + t1) * passes * a.adapters;
     int S = 1;
     while (S < 8 && ctas * S < 2 * sm_count() && n / a.adapters >= 128 * S) S *= 2;
-    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem);
+    // own[] is beside it: raise the limit even where the tiles alone fit the default
+    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 16);
     if (e != cudaSuccess) return e;
     KScope ks("adapter_grad", s);
     return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.adapters), 256, L::kSmem, s, a, t0, (int)vec);

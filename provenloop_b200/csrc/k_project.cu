@@ -53,6 +53,7 @@ struct Tile {
 struct TcArgs {
     ProjectArgs p;
     int tiles_m, tiles_n, kblocks;
+    int split, x_rows;    // k_project_split
     int vec_bias;         // 16-byte loads are aligned
     int tma_out;          // out, and base if there is one, take TMA boxes
 };
@@ -248,11 +249,10 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             const int mine = CG == 2 && rank ? e[CG - 1] : e[0], mine_first = CG == 2 && rank ? first[CG - 1] : first[0];
             const int own = mine >= 0 ? sh.pos[mine_first] : -1;  // this row's adapter in the list
             const float4* low = reinterpret_cast<const float4*>(p.low + (m < p.n ? m : 0) * rs);
-            const int tile_o = t / a.tiles_m * BN, blk = tile_o / 128;
-            for (int d = i; d < distinct; d += 128) {
-                const uint32_t* f = p.bad + (long long)sh.list[d] * blocks + blk;
-                if (f[0] || (BN == 256 && blk + 1 < blocks && f[1])) sh.bad[serial & 7] = 1;
-            }
+            // the factor's flags for the tile's outputs
+            const int tile_o = t / a.tiles_m * BN, per = rs / kXK, flags = min((BN + 127) / 128, blocks - tile_o / 128) * per;
+            for (int d = i; d < distinct * flags; d += 128)
+                if (p.bad[((long long)sh.list[d / flags] * blocks + tile_o / 128) * per + d % flags]) sh.bad[serial & 7] = 1;
             const int steps = max(1, distinct);
             for (int j = 0; j < rs; j += kXK) {
                 float4 f[4];
@@ -424,6 +424,15 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
     if (warp == 13) tmem_free<CG>(tmem, 2 * BN);
 }
 
+template <class T, bool W_MN>
+cudaError_t operand_maps(const ProjectArgs& p, int x_rows, int w_rows, CUtensorMap* mx, CUtensorMap* mw) {
+    const CUtensorMapDataType ty = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cudaError_t e = tensor_map(mx, ty, p.x, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.x_stride * 2, 64, x_rows);
+    if (e != cudaSuccess) return e;
+    return W_MN ? tensor_map(mw, ty, p.w, (uint64_t)p.o, (uint64_t)p.k, (uint64_t)p.w_stride * 2, 64, 64)
+                : tensor_map(mw, ty, p.w, (uint64_t)p.k, (uint64_t)p.o, (uint64_t)p.w_stride * 2, 64, w_rows);
+}
+
 template <class T, int CG, int BN, bool W_MN>
 cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
     using L = Tile<CG, BN>;
@@ -449,10 +458,7 @@ cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     if (p.w) {
-        cudaError_t e = tensor_map(&mx, ty, p.x, (uint64_t)p.k, (uint64_t)p.n, (uint64_t)p.x_stride * 2, 64, 128);
-        if (e == cudaSuccess)
-            e = W_MN ? tensor_map(&mw, ty, p.w, (uint64_t)p.o, (uint64_t)p.k, (uint64_t)p.w_stride * 2, 64, 64)
-                     : tensor_map(&mw, ty, p.w, (uint64_t)p.k, (uint64_t)p.o, (uint64_t)p.w_stride * 2, 64, L::kRows);
+        const cudaError_t e = operand_maps<T, W_MN>(p, 128, L::kRows, &mx, &mw);
         if (e != cudaSuccess) return e;
     }
     auto kern = k_project_tc<T, CG, BN, W_MN>;
@@ -463,8 +469,248 @@ cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
     return launch_dependent(CG, kern, dim3((unsigned)(tiles < slots ? tiles : slots) * CG), kThreads, L::kSmem, s, a, mx, mw, mg, mout, mbase);
 }
 
+// v[z] += sum_j low[j] G(j, o + z) for eight neighbouring outputs: the
+// factor's 16 bytes along whichever axis is contiguous, else its elements.
+template <class T>
+__device__ __forceinline__ void add_low(const ProjectArgs& p, const float* low, const T* g, int o, float (&v)[8]) {
+    const bool whole = o + 8 <= p.o;
+    const T* at = g + o * p.g.sk;
+    if (p.g.sk == 1 && whole && (p.g.sj & 7) == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+#pragma unroll 8
+        for (int j = 0; j < p.r; j++) {
+            const uint4 q = *reinterpret_cast<const uint4*>(at + j * p.g.sj);
+            const float l = low[j];
+            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                const float2 f = unpack2<T>(u[z]);
+                v[2 * z] = fmaf(l, f.x, v[2 * z]), v[2 * z + 1] = fmaf(l, f.y, v[2 * z + 1]);
+            }
+        }
+    } else if (p.g.sj == 1 && (p.r & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+#pragma unroll 2
+        for (int j = 0; j < p.r; j += 8) {
+            const float4 l0 = *reinterpret_cast<const float4*>(low + j), l1 = *reinterpret_cast<const float4*>(low + j + 4);
+            uint4 q[8];
+#pragma unroll
+            for (int z = 0; z < 8; z++) q[z] = *reinterpret_cast<const uint4*>(g + min(o + z, p.o - 1) * p.g.sk + j);
+#pragma unroll
+            for (int z = 0; z < 8; z++) {
+                const float2 f0 = unpack2<T>(q[z].x), f1 = unpack2<T>(q[z].y), f2 = unpack2<T>(q[z].z), f3 = unpack2<T>(q[z].w);
+                v[z] = fmaf(l0.x, f0.x, v[z]), v[z] = fmaf(l0.y, f0.y, v[z]), v[z] = fmaf(l0.z, f1.x, v[z]), v[z] = fmaf(l0.w, f1.y, v[z]);
+                v[z] = fmaf(l1.x, f2.x, v[z]), v[z] = fmaf(l1.y, f2.y, v[z]), v[z] = fmaf(l1.z, f3.x, v[z]), v[z] = fmaf(l1.w, f3.y, v[z]);
+            }
+        }
+    } else if (p.g.sj == 1 && (p.r & 1) == 0 && (reinterpret_cast<uintptr_t>(g) & 3) == 0) {
+#pragma unroll 4
+        for (int j = 0; j < p.r; j += 2) {
+            const float2 l = *reinterpret_cast<const float2*>(low + j);
+            uint32_t q[8];
+#pragma unroll
+            for (int z = 0; z < 8; z++) q[z] = *reinterpret_cast<const uint32_t*>(g + min(o + z, p.o - 1) * p.g.sk + j);
+#pragma unroll
+            for (int z = 0; z < 8; z++) {
+                const float2 f = unpack2<T>(q[z]);
+                v[z] = fmaf(l.x, f.x, v[z]), v[z] = fmaf(l.y, f.y, v[z]);
+            }
+        }
+    } else {
+#pragma unroll 4
+        for (int j = 0; j < p.r; j++) {
+            float f[8];
+#pragma unroll
+            for (int z = 0; z < 8; z++) f[z] = elem<T>(g, j * p.g.sj + min(o + z, p.o - 1) * p.g.sk);
+#pragma unroll
+            for (int z = 0; z < 8; z++) v[z] = fmaf(low[j], f[z], v[z]);
+        }
+    }
+}
+
+// Not enough tiles for all SMs: a cluster of S CTAs shares the contraction of
+// a 128 x BN tile, each with a ring of its own, and the partial sums meet in
+// shared memory, where each CTA finishes BN / S of the outputs.  Each token
+// takes its own adapter's factor straight from L2 (n o r elements in all), so
+// that nothing is converted first.  Bound: reading W once by all SMs together,
+// and the launches' latency.  Without W only the last part runs.
+template <int BN>
+struct SplitTile {
+    static constexpr int kStages = BN == 64 ? 4 : 3;
+    static constexpr int kStage = 128 * 128 + BN * 128;
+    static constexpr int kRow = BN + 4;  // floats: rows of the partial sums four banks apart
+    static constexpr int kSmem = kStages * kStage + 1024;
+    static_assert(128 * kRow * 4 <= kStages * kStage, "the sums fit where the ring was");
+};
+
+template <class T, int BN, bool W_MN>
+__global__ void __launch_bounds__(256)
+k_project_split(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw) {
+    using L = SplitTile<BN>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
+    __shared__ uint32_t tmem_at, dead;
+    const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
+    float* sums = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));  // [128][kRow], when the ring is done with
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const ProjectArgs& p = a.p;
+    const int S = a.split, rank = (int)cluster_rank();
+    const int m0 = blockIdx.y * 128, o0 = blockIdx.x / S * BN;
+    if (a.kblocks) {
+        const int kb0 = a.kblocks * rank / S, kb1 = a.kblocks * (rank + 1) / S;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < L::kStages; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+            mbar_init(&done, 1);
+            dead = 0;
+            mbar_init_fence();
+        }
+        if (warp == 1) tmem_alloc<1>(&tmem_at, BN);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        const uint32_t tmem = tmem_at;
+        if (warp == 0) {
+            if (lane == 0) {
+                Ring r(L::kStages, 1);
+                for (int kb = kb0; kb < kb1; kb++, r.next()) {
+                    if (!mbar_wait(&empty[r.i], r.phase, &dead)) break;
+                    const uint32_t s = ring + r.i * L::kStage, bar = smem_u32(&full[r.i]);
+                    mbar_expect(&full[r.i], a.x_rows * 128 + BN * 128);
+                    tma_2d<1>(s, &mx, kb * 64, m0, bar);
+                    if constexpr (W_MN) {
+#pragma unroll
+                        for (int q = 0; q < BN / 64; q++) tma_2d<1>(s + 16384 + q * 8192, &mw, o0 + q * 64, kb * 64, bar);
+                    } else {
+                        tma_2d<1>(s + 16384, &mw, kb * 64, o0, bar);
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+                constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (W_MN ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | 8u << 24;
+                Ring r(L::kStages, 0);
+                for (int kb = kb0; kb < kb1; kb++, r.next()) {
+                    if (!mbar_wait(&full[r.i], r.phase, &dead)) break;
+                    tc_fence_after();
+                    const uint32_t s = ring + r.i * L::kStage;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint64_t db = W_MN ? desc_mn128(s + 16384 + k * 2048, 8192) : desc_k128(s + 16384 + k * 32);
+                        mma_f16<1>(tmem, desc_k128(s + k * 32), db, idesc, (kb - kb0) | k);
+                    }
+                    mma_commit<1>(&empty[r.i]);
+                }
+                mma_commit<1>(&done);
+            }
+        }
+        __syncwarp();
+        mbar_wait(&done, 0, &dead);
+        tc_fence_after();
+        const int row = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int c = (warp >> 2) * (BN / 2); c < (warp >> 2) * (BN / 2) + BN / 2; c += 32) {
+            float v[32];
+            __syncwarp();
+            tmem_ld32(tmem + c + ((uint32_t)(warp & 3) << 21), v);
+#pragma unroll
+            for (int q = 0; q < 32; q += 4)
+                *reinterpret_cast<float4*>(sums + row * L::kRow + c + q) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+        }
+        tc_fence_before();
+    }
+    if (S > 1) cluster_sync_all();
+    else __syncthreads();
+    grid_dependency_wait();  // low is written by the launch before this one
+    const int per = BN / S, rs = low_stride(p.r);
+    for (int i = threadIdx.x; i < 128 * (per / 8); i += 256) {
+        const int row = i & 127, col = rank * per + (i >> 7) * 8, o = o0 + col;
+        const long long m = m0 + row;
+        if (m >= p.n || o >= p.o) continue;
+        float v[8] = {};
+        if (a.kblocks)
+            for (int q = 0; q < S; q++) {
+                const float* f = sums + row * L::kRow + col;
+                float4 f0, f1;
+                if (S > 1) {
+                    const uint32_t at = map_rank(f, q);
+                    f0 = ld_cluster4(at), f1 = ld_cluster4(at + 16);
+                } else {
+                    f0 = *reinterpret_cast<const float4*>(f), f1 = *reinterpret_cast<const float4*>(f + 4);
+                }
+                v[0] += f0.x, v[1] += f0.y, v[2] += f0.z, v[3] += f0.w, v[4] += f1.x, v[5] += f1.y, v[6] += f1.z, v[7] += f1.w;
+            }
+        const int e = p.id.of(m);
+        const bool whole = o + 8 <= p.o;
+        T* out = static_cast<T*>(p.out) + m * p.out_stride + o;
+        const T* base = static_cast<const T*>(p.base) + m * p.base_stride + o;
+        if (p.bias) {
+#pragma unroll
+            for (int z = 0; z < 8; z++) v[z] += elem<T>(p.bias, min(o + z, p.o - 1));
+        }
+        if (p.base) {
+            if (whole && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
+                const uint4 q = *reinterpret_cast<const uint4*>(base);
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int z = 0; z < 4; z++) {
+                    const float2 f = unpack2<T>(u[z]);
+                    v[2 * z] += f.x, v[2 * z + 1] += f.y;
+                }
+            } else {
+#pragma unroll
+                for (int z = 0; z < 8; z++) v[z] += elem<T>(base, min(z, p.o - 1 - o));
+            }
+        }
+        if (e >= 0) add_low<T>(p, p.low + m * rs, static_cast<const T*>(p.g.p) + e * p.g.se, o, v);
+        uint32_t u[4];
+#pragma unroll
+        for (int z = 0; z < 4; z++) u[z] = pack2<T>(v[2 * z], v[2 * z + 1]);
+        if (whole && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+            *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+        } else {
+            const T* h = reinterpret_cast<const T*>(u);
+#pragma unroll
+            for (int z = 0; z < 8; z++)
+                if (o + z < p.o) out[z] = h[z];
+        }
+    }
+    if (a.kblocks && dead && threadIdx.x == 0) settle();
+    if (S > 1) cluster_sync_all();
+    else __syncthreads();
+    if (a.kblocks && warp == 1) tmem_free<1>(tmem_at, BN);
+}
+
+template <class T, int BN, bool W_MN>
+cudaError_t launch_split(const ProjectArgs& p, int sms, cudaStream_t s) {
+    using L = SplitTile<BN>;
+    TcArgs a{p};
+    a.tiles_m = (int)((p.n + 127) / 128);
+    a.tiles_n = (p.o + BN - 1) / BN;
+    a.kblocks = p.w ? (p.k + 63) / 64 : 0;
+    // as many CTAs share a tile as it takes to give every SM one, while each
+    // has two slices of the contraction and eight outputs of a row
+    a.split = 1;
+    while (a.split < 8 && (long long)a.tiles_m * a.tiles_n * a.split < sms && a.kblocks >= 4 * a.split) a.split *= 2;
+    a.x_rows = p.n < 128 ? (int)(p.n + 7) / 8 * 8 : 128;  // rows behind stay whatever they are: their sums are not used
+    CUtensorMap mx{}, mw{};
+    if (p.w) {
+        const cudaError_t e = operand_maps<T, W_MN>(p, a.x_rows, BN, &mx, &mw);
+        if (e != cudaSuccess) return e;
+    }
+    auto kern = k_project_split<T, BN, W_MN>;
+    const size_t smem = p.w ? L::kSmem : 0;
+    const cudaError_t e = ensure_smem(kern, smem);
+    if (e != cudaSuccess) return e;
+    KScope ks("adapter_project", s);
+    return launch_dependent(a.split, kern, dim3((unsigned)(a.tiles_n * a.split), a.tiles_m), 256, smem, s, a, mx, mw);
+}
+
 template <class T, bool W_MN>
 cudaError_t launch_width(const ProjectArgs& p, int sms, cudaStream_t s) {
+    if (!p.g32) {
+        // 64-wide tiles as long as they do not fill the SMs twice
+        const long long tiles = ((p.n + 127) / 128) * ((p.o + 63) / 64);
+        return tiles <= 2 * sms ? launch_split<T, 64, W_MN>(p, sms, s) : launch_split<T, 128, W_MN>(p, sms, s);
+    }
     // The tile with the least (rounds over the SMs) x (time of a tile): in
     // units of the slices' bytes, which is what a tile waits for.
     const auto cost = [&](int cg, int bn) {

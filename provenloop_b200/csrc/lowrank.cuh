@@ -73,7 +73,7 @@ struct ProjectArgs {
     const float* low;
     Factor g;  // sk here is the stride of o
     const float* g32;     // g as f32 [e][o][low_stride(r)], elements that are not finite replaced by 0 (k_project.cu only)
-    const uint32_t* bad;  // [e][ceil(o / 128)]: some of them are
+    const uint32_t* bad;  // [e][ceil(o / 128)][low_stride(r) / 16]: some of them are
     AdapterIds id;
     void* out;
     long long out_stride;
@@ -106,7 +106,7 @@ struct PackJob {
     long long rows;  // j
     int count, cols, dst_cols;
     void* dst;      // [count][rows][dst_cols], zeros behind cols: 16-bit elements / f32
-    uint32_t* bad;  // TO_F32: [count][ceil(rows / 128)]
+    uint32_t* bad;  // TO_F32: [count][ceil(rows / 128)][dst_cols / 16]
     AdapterIds id;  // LISTS: dst is first [count + 1], then the list [rows]
     long long blocks;
 };
@@ -115,15 +115,22 @@ struct PackJobs {
     PackJob job[kMaxPack];
     int jobs, dtype;
     void add(PackJob j) {
-        j.blocks = j.kind == PackJob::LISTS ? j.count : j.kind == PackJob::TO_F32 ? (j.rows + 127) / 128 * j.count : ((j.rows + 31) / 32) * ((j.dst_cols + 31) / 32) * j.count;
+        j.blocks = j.kind == PackJob::LISTS ? j.count : j.kind == PackJob::TO_F32 ? (j.rows + 127) / 128 * (j.dst_cols / 16) * j.count : ((j.rows + 31) / 32) * ((j.dst_cols + 31) / 32) * j.count;
         job[jobs++] = j;
     }
 };
 
 // The kernels that a call takes go by its sizes; decode_ops.cu lays out the
 // workspace with the same rules.
-constexpr int kTokenLow = 128;    // up to here, and for f32, low is computed token by token
-constexpr int kSmallTokens = 64;  // up to here W is streamed once past all tokens
+// Low token by token reads each token's factor (from L2 where tokens share
+// it): for f32 always, else up to 48 MiB of such reads, where it is faster than
+// matrix instructions if every token has an adapter of its own.
+inline bool low_by_token(long long n, long long k0, long long k1, long long r) { return n * r * (k0 > k1 ? k0 : k1) * 2 <= 48ll << 20; }
+constexpr int kSmallTokens = 16;  // up to here W is streamed once past all tokens
+// The projection takes each token's factor from where it is, n o r elements
+// in all, up to 32 MiB of them; above that the factors are converted first
+// and shared by the tokens of a tile.
+inline bool factor_by_token(long long n, long long o, long long r) { return n * o * r * 2 <= 32ll << 20; }
 
 cudaError_t launch_pack(const PackJobs& a, cudaStream_t s);
 // one or two of them (the same n, r and id) in one launch; `vec`: rows of x
@@ -135,7 +142,8 @@ cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int aft
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s);
 // 16-bit types, at most kSmallTokens tokens; x and w (not transposed) on 16-byte boundaries
 cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s);
-// 16-bit types; x and w rows on 16-byte boundaries (k_project.cu)
+// 16-bit types; x and w rows on 16-byte boundaries (k_project.cu); a.g32 is
+// null where factor_by_token
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
 // rows of x on 16-byte boundaries, but for f32 (`vec`: they are)
 cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s);
