@@ -323,7 +323,7 @@ int ts_adapter_project(const ts_adapter_args* args);
  * any), in an order fixed by the sizes alone.  The gradient of base is grad. */
 int ts_adapter_project_backward(const ts_adapter_args* args);
 
-/* Waits between the warps of a ts_adapter_* kernel that ran out (two seconds) on
+/* Waits within a kernel of ts_adapter_* or ts_logit_rules that ran out (two seconds) on
  * `device` since the library was loaded: 0, unless a kernel or the device is
  * broken; the results of such a call are not complete.  Waits for the device. */
 int ts_expired_waits(int device, uint64_t* out);

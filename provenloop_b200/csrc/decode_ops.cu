@@ -400,10 +400,12 @@ extern "C" int ts_expired_waits(int device, uint64_t* out) {
     if (!out) return bad("out is NULL");
     return guarded([&] {
         OnDevice dev(device);
-        unsigned long long v = 0;
-        const int rc = cuda_status(dev.status != cudaSuccess ? dev.status : expired_waits(&v));
-        *out = v;
-        return rc;
+        unsigned long long v = 0, w = 0;
+        cudaError_t e = dev.status;
+        if (e == cudaSuccess) e = expired_waits_project(&v);
+        if (e == cudaSuccess) e = expired_waits_rules(&w);
+        *out = v + w;
+        return cuda_status(e);
     });
 }
 extern "C" int ts_logit_rules(const ts_rules_args* args) {

@@ -744,9 +744,7 @@ cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t expired_waits(unsigned long long* out) {
-    return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out));
-}
+cudaError_t expired_waits_project(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
 
 cudaError_t launch_project_tc(const ProjectArgs& p, int dtype, cudaStream_t s) {
     int dev = 0, sms = 0;

@@ -15,16 +15,18 @@
 // row is split over a cluster of CTAs so that one row alone already uses
 // several SMs, and the pick is reduced through distributed shared memory: no
 // workspace, no atomics on global memory, hence nothing that two calls or
-// two captured graphs could share.
+// two captured graphs could share.  A CTA starts the asynchronous copy of its
+// segment of the row first and goes through the lists while it arrives.
 //
-// What the history and the biases say is kept per token of the CTA's
-// segment in shared memory: two bitmaps (history, history or bias) read with
-// every vector of logits, and one word (bias entry + 1 << 20 | count) that is
-// cleared, written and read only for the tokens that the lists name.
+// What the history and the biases say of the segment's tokens is kept in
+// shared memory: two bitmaps (history, history or bias) read with every vector
+// of logits, and for the tokens that the lists name one word each (bias entry
+// + 1 << 20 | count), found by counting the bits before the token's.
 #include <climits>
 
 #include "launch.cuh"
 #include "lowrank.cuh"
+#include "sm100.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -32,9 +34,10 @@ namespace tsg {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;  // and 64 registers: two CTAs per SM, one's lists beside the other's stream
 constexpr int kCluster = 8;
-constexpr uint32_t kSegment = 19456;  // tokens per segment: 76 KiB of words, two CTAs per SM
+constexpr uint32_t kSegment = 19456;  // tokens per segment: an eighth of a vocabulary of 150 thousand in one go
+constexpr uint32_t kWords = kSegment / 32;
 constexpr uint32_t kBiasShift = 20;   // count below, bias entry + 1 above
 
 struct Best {
@@ -78,14 +81,42 @@ __device__ __forceinline__ long long list_at(const void* p, int is64, long long 
     return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int32_t*>(p)[i];
 }
 
+// Entries [from, to) of a list of token ids whose token lies in the segment:
+// f(position in the segment, entry).
+template <class F>
+__device__ __forceinline__ void each_in(const void* list, int is64, long long at, uint32_t from, uint32_t to, uint32_t vocab, uint32_t shift,
+                                        uint32_t size, F f) {
+    uint32_t i = from + threadIdx.x;
+    for (; i + 3 * kThreads < to; i += 4 * kThreads) {
+        long long v[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = list_at(list, is64, at + i + q * kThreads);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t p = (uint32_t)v[q] + shift;
+            if ((unsigned long long)v[q] < vocab && p < size) f(p, i + q * kThreads);
+        }
+    }
+    for (; i < to; i += kThreads) {
+        const long long v = list_at(list, is64, at + i);
+        const uint32_t p = (uint32_t)v + shift;
+        if ((unsigned long long)v < vocab && p < size) f(p, i);
+    }
+}
+
+__host__ __device__ constexpr size_t head_bytes() { return (3 * kWords + 4) * 4; }
+
 // T: logits, O: output (written where a.out is not null).  The segment's
 // tokens are addressed by p = v + head, where head is the row's offset from
 // a 16-byte boundary in elements, so that vectors, bitmaps and words line up
-// in rows of any alignment.
+// in rows of any alignment.  Dynamic shared memory: the bitmaps and the bit
+// counts before their words, the named tokens' words, the segment's logits.
 template <class T, class O>
-__global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, uint32_t named) {
     constexpr int VEC = 16 / sizeof(T);
-    extern __shared__ uint32_t smem[];
+    extern __shared__ __align__(128) uint32_t smem[];
+    __shared__ uint64_t arrived;
+    __shared__ uint32_t dead;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), cl = (int)cluster.num_blocks();
     const long long row = blockIdx.x / cl;
@@ -95,6 +126,28 @@ __global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
     const uint32_t end = head + a.vocab;
     // whole vectors of output where the output row has the same phase
     const bool out_vec = out && reinterpret_cast<uintptr_t>(out) % 16 == head * sizeof(O) % 16;
+    const uint32_t span = ((end + cl - 1) / cl + 127) / 128 * 128;
+    const uint32_t first = min(end, rank * span), last = min(end, first + span);
+
+    uint32_t* seen = smem;
+    uint32_t* touched = seen + kWords;
+    uint32_t* before = touched + kWords;  // kWords + 4
+    uint32_t* word = before + kWords + 4;
+    T* buf = reinterpret_cast<T*>(word + named);
+    if (threadIdx.x == 0) {
+        mbar_init(&arrived, 1);
+        dead = 0;
+        fence_async_shared();
+    }
+    __syncthreads();
+    // the whole vectors of [lo, hi) to buf, by one thread
+    const auto fetch = [&](uint32_t lo, uint32_t hi) {
+        const uint32_t from = lo == 0 && head ? VEC : lo, to = hi / VEC * VEC;
+        const uint32_t bytes = to > from ? (to - from) * (uint32_t)sizeof(T) : 0;
+        mbar_expect(&arrived, bytes);
+        if (bytes) bulk_copy(smem_u32(buf + (from - lo)), x + from - head, bytes, &arrived);
+    };
+    if (threadIdx.x == 0 && first < last) fetch(first, min(last, first + kSegment));
 
     const uint32_t hist = a.tokens ? (uint32_t)max(0, min(a.lengths ? a.lengths[row] : INT_MAX, (int)a.token_cols)) : 0u;
     const uint32_t prompt = a.prompt_lengths ? (uint32_t)max(0, a.prompt_lengths[row]) : 0u;
@@ -107,88 +160,103 @@ __global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
     const uint32_t words = (a.vocab + 31) / 32;
     const bool lists = hist || biases;
 
-    uint32_t* seen = smem;                          // kSegment / 32
-    uint32_t* touched = seen + kSegment / 32;       // kSegment / 32
-    uint32_t* word = touched + kSegment / 32;       // kSegment
-
-    const uint32_t span = ((end + cl - 1) / cl + 127) / 128 * 128;
-    const uint32_t first = min(end, rank * span), last = min(end, first + span);
     Best best{-INFINITY, UINT_MAX};
-    for (uint32_t lo = first; lo < last; lo += kSegment) {
-        const uint32_t hi = min(last, lo + kSegment);
+    uint32_t phase = 0;
+    for (uint32_t lo = first; lo < last; lo += kSegment, phase ^= 1) {
+        const uint32_t hi = min(last, lo + kSegment), size = hi - lo, shift = head - lo;
+        if (lo != first) {
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                fence_async_shared();
+                fetch(lo, hi);
+            }
+        }
         if (lists) {
-            for (uint32_t i = threadIdx.x; i < kSegment / 16; i += kThreads) smem[i] = 0u;
+            for (uint32_t i = threadIdx.x; i < 2 * kWords; i += kThreads) smem[i] = 0u;
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < biases; i += kThreads) {
-                const long long v = list_at(a.bias_ids, a.bias64, bid0 + i);
-                const uint32_t p = (uint32_t)v + head - lo;
-                if ((unsigned long long)v < a.vocab && p < hi - lo) word[p] = 0u, atomicOr(touched + p / 32, 1u << p % 32);
-            }
-            for (uint32_t i = threadIdx.x; i < hist; i += kThreads) {
-                const long long v = list_at(a.tokens, a.tokens64, tok0 + i);
-                const uint32_t p = (uint32_t)v + head - lo;
-                if ((unsigned long long)v < a.vocab && p < hi - lo) {
-                    word[p] = 0u;
-                    atomicOr(touched + p / 32, 1u << p % 32);
-                    atomicOr(seen + p / 32, 1u << p % 32);
+            each_in(a.bias_ids, a.bias64, bid0, 0, biases, a.vocab, shift, size, [&](uint32_t p, uint32_t) { atomicOr(touched + p / 32, 1u << p % 32); });
+            each_in(a.tokens, a.tokens64, tok0, 0, hist, a.vocab, shift, size, [&](uint32_t p, uint32_t) {
+                atomicOr(touched + p / 32, 1u << p % 32);
+                atomicOr(seen + p / 32, 1u << p % 32);
+            });
+            const uint32_t most = min(named, size);
+            for (uint32_t i = threadIdx.x; i < most; i += kThreads) word[i] = 0u;
+            __syncthreads();
+            if (threadIdx.x < 32) {
+                // bits before each word: 19 words a lane
+                constexpr uint32_t kEach = kWords / 32;
+                static_assert(kWords % 32 == 0, "a lane has whole words");
+                uint32_t sum = 0;
+                for (uint32_t i = 0; i < kEach; i++) {
+                    before[threadIdx.x * kEach + i] = sum;
+                    sum += __popc(touched[threadIdx.x * kEach + i]);
                 }
-            }
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < biases; i += kThreads) {
-                const long long v = list_at(a.bias_ids, a.bias64, bid0 + i);
-                const uint32_t p = (uint32_t)v + head - lo;
-                if ((unsigned long long)v < a.vocab && p < hi - lo) atomicMax(word + p, (i + 1) << kBiasShift);
-            }
-            __syncthreads();
-            for (uint32_t i = prompt + threadIdx.x; i < hist; i += kThreads) {
-                const long long v = list_at(a.tokens, a.tokens64, tok0 + i);
-                const uint32_t p = (uint32_t)v + head - lo;
-                if ((unsigned long long)v < a.vocab && p < hi - lo) atomicAdd(word + p, 1u);
+                uint32_t incl = sum;
+#pragma unroll
+                for (int q = 1; q < 32; q <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, q);
+                    if (threadIdx.x >= q) incl += y;
+                }
+                for (uint32_t i = 0; i < kEach; i++) before[threadIdx.x * kEach + i] += incl - sum;
             }
             __syncthreads();
         }
+        const auto slot = [&](uint32_t p) { return before[p / 32] + __popc(touched[p / 32] & ((1u << p % 32) - 1)); };
+        if (lists) {
+            each_in(a.bias_ids, a.bias64, bid0, 0, biases, a.vocab, shift, size,
+                    [&](uint32_t p, uint32_t i) { atomicMax(word + slot(p), (i + 1) << kBiasShift); });
+            __syncthreads();
+            each_in(a.tokens, a.tokens64, tok0, prompt, hist, a.vocab, shift, size, [&](uint32_t p, uint32_t) { atomicAdd(word + slot(p), 1u); });
+            __syncthreads();
+        }
+        mbar_wait(&arrived, phase, &dead);
         for (uint32_t p0 = lo + threadIdx.x * VEC; p0 < hi; p0 += kThreads * VEC) {
             const bool whole = p0 >= head && p0 + VEC <= hi;
             Pack<T, VEC> in;
             if (whole) {
-                in = *reinterpret_cast<const Pack<T, VEC>*>(x + (p0 - head));
+                in = *reinterpret_cast<const Pack<T, VEC>*>(buf + (p0 - lo));
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; i++)
                     if (p0 + i >= head && p0 + i < hi) in.v[i] = x[p0 + i - head];
             }
             // the vector's bits; a group of VEC <= 8 lies in one word, since lo is a multiple of 128
-            uint32_t tb = 0, sb = 0, mb = UINT_MAX;
-            if (lists) {
-                const uint32_t q = p0 - lo;
-                tb = touched[q / 32] >> q % 32;
-                sb = seen[q / 32] >> q % 32;
-            }
+            const uint32_t q = p0 - lo;
+            uint32_t tb = 0, mb = UINT_MAX;
+            if (lists) tb = touched[q / 32] >> q % 32;
             if (mask) {
                 // token v0 of the vector's first element; v0 < 0 in a row's first vector
                 const long long v0 = (long long)p0 - head;
                 const long long w = v0 >> 5;
                 const uint32_t m0 = w >= 0 ? mask[w] : 0u;
-                const uint32_t m1 = w + 1 < words ? mask[w + 1] : 0u;
+                const uint32_t m1 = head && w + 1 < words ? mask[w + 1] : 0u;
                 mb = __funnelshift_r(m0, m1, (uint32_t)(v0 & 31));
             }
-            Pack<O, VEC> res;
+            float z[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; i++) z[i] = load_f(in.v[i]);
+            constexpr uint32_t kAll = (1u << VEC) - 1;
+            if (tb & kAll) {
+                const uint32_t sb = seen[q / 32] >> q % 32;
+#pragma unroll
+                for (int i = 0; i < VEC; i++)
+                    if (tb >> i & 1) {
+                        const uint32_t c = word[slot(q + i)];
+                        const uint32_t n = c & ((1u << kBiasShift) - 1), b = c >> kBiasShift;
+                        if (sb >> i & 1) z[i] = z[i] > 0.f ? __fdiv_rn(z[i], rho) : __fmul_rn(z[i], rho);
+                        if (n) z[i] = __fsub_rn(__fsub_rn(z[i], __fmul_rn(freq, (float)n)), pres);
+                        if (b) z[i] = __fadd_rn(z[i], a.bias_values[bval0 + b - 1]);
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                if (!whole && !(p0 + i >= head && p0 + i < hi)) continue;
-                float z = load_f(in.v[i]);
-                if (tb >> i & 1) {
-                    const uint32_t c = word[p0 + i - lo];
-                    const uint32_t n = c & ((1u << kBiasShift) - 1), b = c >> kBiasShift;
-                    if (sb >> i & 1) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-                    if (n) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)n)), pres);
-                    if (b) z = __fadd_rn(z, a.bias_values[bval0 + b - 1]);
-                }
-                if (!(mb >> i & 1)) z = -INFINITY;
-                take(best, z, p0 + i - head);
-                store_f(&res.v[i], z);
+                if (!(mb >> i & 1)) z[i] = -INFINITY;
+                if (whole || (p0 + i >= head && p0 + i < hi)) take(best, z[i], p0 + i - head);
             }
             if (out) {
+                Pack<O, VEC> res;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) store_f(&res.v[i], z[i]);
                 if (whole && out_vec) {
                     if constexpr (sizeof(O) * VEC > 16) {
                         const Pack<O, VEC / 2>* r2 = reinterpret_cast<const Pack<O, VEC / 2>*>(&res);
@@ -204,7 +272,6 @@ __global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
                 }
             }
         }
-        if (lists) __syncthreads();
     }
 
     unsigned long long key = key_of(best);
@@ -214,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
     if ((threadIdx.x & 31) == 0) warp_key[threadIdx.x >> 5] = key;
     __syncthreads();
     if (threadIdx.x < 32) {
-        key = warp_key[threadIdx.x];
+        key = threadIdx.x < kThreads / 32 ? warp_key[threadIdx.x] : 0ull;
 #pragma unroll
         for (int q = 16; q; q >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, q));
         if (threadIdx.x == 0) *cluster.map_shared_rank(&cta_key[rank], 0) = key;
@@ -228,14 +295,20 @@ __global__ void __launch_bounds__(kThreads) k_rules(const RulesArgs a) {
 
 template <class T, class O>
 cudaError_t launch_one(const RulesArgs& a, cudaStream_t s) {
-    const size_t smem = a.tokens || a.bias_ids ? (size_t)(kSegment / 16 + kSegment) * 4 : 0;
-    const cudaError_t e = ensure_smem(k_rules<T, O>, smem);
+    // words for as many tokens as the lists can name in a segment
+    const uint64_t most = (uint64_t)(a.tokens ? a.token_cols : 0) + (a.bias_ids ? a.bias_cols : 0);
+    const uint32_t span = ((a.vocab + 16 + kCluster - 1) / kCluster + 127) / 128 * 128, segment = span < kSegment ? span : kSegment;
+    const uint32_t named = (uint32_t)((most < segment ? most : segment) + 31) / 32 * 32;
+    const size_t smem = head_bytes() + (size_t)named * 4 + (size_t)segment * sizeof(T);
+    const cudaError_t e = ensure_smem(k_rules<T, O>, smem > 48 * 1024 ? smem : smem + 48 * 1024);
     if (e != cudaSuccess) return e;
     KScope ks("logit_rules", s);
-    return launch_cl(kCluster, k_rules<T, O>, dim3((unsigned)(a.n * kCluster)), kThreads, smem, s, a);
+    return launch_cl(kCluster, k_rules<T, O>, dim3((unsigned)(a.n * kCluster)), kThreads, smem, s, a, named);
 }
 
 }  // namespace
+
+cudaError_t expired_waits_rules(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
 
 cudaError_t launch_rules(const RulesArgs& a, int dtype, int out_dtype, cudaStream_t s) {
     if (dtype == DT_F32) return launch_one<float, float>(a, s);

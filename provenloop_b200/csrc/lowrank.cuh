@@ -147,8 +147,9 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
 // rows of x on 16-byte boundaries, but for f32 (`vec`: they are)
 cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s);
-// waits of k_project.cu that ran out on the current device so far
-cudaError_t expired_waits(unsigned long long* out);
+// waits of k_project.cu / k_rules.cu that ran out on the current device so far
+cudaError_t expired_waits_project(unsigned long long* out);
+cudaError_t expired_waits_rules(unsigned long long* out);
 
 struct RulesArgs {
     const void* logits;

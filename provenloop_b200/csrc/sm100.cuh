@@ -98,6 +98,13 @@ struct Ring {
     }
 };
 
+// `bytes` from global to this CTA's shared memory, both on 16-byte boundaries
+// and bytes a multiple of 16.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
 // One box of a tensor map to this CTA's shared memory; `bar` (a cluster
 // address) may be the other CTA's of a pair (CG = 2).
 template <int CG>

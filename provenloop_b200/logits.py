@@ -12,7 +12,7 @@ from __future__ import annotations
 import struct
 
 from ._lib import check, lib
-from .adapters import _dtype_code, _ptr
+from .adapters import _current_stream, _dtype_code, _load, _ptr
 
 _ARGS = struct.Struct("@4iPQ4IPqPq5PPqPqPqPqP")  # ts_rules_args
 
@@ -20,7 +20,9 @@ MAX_HISTORY, MAX_BIASES = 1048575, 4095
 
 
 def _per_row(t, name, dtype, n, device):
-    if t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if t.dtype is dtype and t.shape == (n,) and t.device == device and t.is_contiguous():
+        return
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape ({n},)")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, logits on {device}")
@@ -28,6 +30,11 @@ def _per_row(t, name, dtype, n, device):
 
 def _table(t, name, dtypes, n, device, cols=None):
     """Stride between rows of t [n, cols], or 0 for one row [cols] for all."""
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == n and t.dtype in dtypes and t.device == device and cols in (None, shape[1]):
+        row, col = t.stride()
+        if col == 1:
+            return row
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
     if t.dim() not in (1, 2) or (t.dim() == 2 and t.shape[0] != n) or (cols is not None and t.shape[-1] != cols):
@@ -65,7 +72,7 @@ def apply_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetiti
     The pick is the lowest id of the greatest unrounded value (a NaN counts as
     the greatest, as in ``torch.argmax``), -1 for a row that is -inf
     throughout.  At most 1048575 tokens and 4095 biases a row."""
-    import torch
+    torch = _load()
     code, device = _dtype_code(logits.dtype), logits.device
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [n, vocab] with contiguous rows")
@@ -119,9 +126,11 @@ def apply_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetiti
         out, o_stride = logits.new_empty((n, vocab)), vocab
     picks = torch.empty(n, dtype=torch.int64, device=device) if pick else None
     index = device.index
-    check(lib().ts_logit_rules(_ARGS.pack(
-        code, out_code, index, ids64, torch.cuda.current_stream(index).cuda_stream, n, vocab, cols, b_cols, 0, logits.data_ptr(),
+    rc = lib().ts_logit_rules(_ARGS.pack(
+        code, out_code, index, ids64, _current_stream(index), n, vocab, cols, b_cols, 0, logits.data_ptr(),
         logits.stride(0), _ptr(tokens), t_stride, _ptr(lengths), _ptr(prompt_lengths), _ptr(repetition), _ptr(frequency),
         _ptr(presence), _ptr(bias_ids), bi_stride, _ptr(bias_values), bv_stride, _ptr(mask), m_stride, _ptr(out), o_stride,
-        _ptr(picks))), "ts_logit_rules")
+        _ptr(picks)))
+    if rc:
+        check(rc, "ts_logit_rules")
     return out, picks

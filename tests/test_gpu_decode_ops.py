@@ -539,3 +539,12 @@ def test_rules_captured(R):
         want, picks, _ = _rules_ref(x.float().cpu().numpy(), **ref, dtype=np.float32)
         for _, (z, pick), _ in graphs:
             assert torch.equal(z.cpu(), torch.from_numpy(want).to(z.dtype)) and np.array_equal(pick.cpu().numpy(), picks)
+
+
+def test_no_wait_ran_out():
+    """Collected last: none of the calls above gave up a wait in a kernel."""
+    import ctypes as C
+    from provenloop_b200._lib import check, lib
+    v = C.c_uint64(1)
+    check(lib().ts_expired_waits(0, C.byref(v)))
+    assert v.value == 0
