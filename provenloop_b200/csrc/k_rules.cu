@@ -12,16 +12,20 @@
 //   torch.argmax); -1 where every z is -inf.
 //
 // The bound is the logits' traffic: each is read once and written once.  A
-// row is split over a cluster of CTAs so that one row alone already uses
-// several SMs, and the pick is reduced through distributed shared memory: no
+// row is split over a cluster of one to eight CTAs, so that a few rows already
+// use every SM, and the pick is reduced through distributed shared memory: no
 // workspace, no atomics on global memory, hence nothing that two calls or
-// two captured graphs could share.  A CTA starts the asynchronous copy of its
-// segment of the row first and goes through the lists while it arrives.
+// two captured graphs could share.  A CTA takes its part of the row in
+// segments, whose asynchronous copies run two ahead of it, and goes through
+// the lists (held in registers) while they arrive.
 //
-// What the history and the biases say of the segment's tokens is kept in
-// shared memory: two bitmaps (history, history or bias) read with every vector
-// of logits, and for the tokens that the lists name one word each (bias entry
-// + 1 << 20 | count), found by counting the bits before the token's.
+// What the lists say is kept in shared memory: a bitmap of the tokens that
+// they name, and for those one word each, found by counting the bits before
+// the token's.  The named tokens are computed first, from the lists' side; the
+// stream over the segments takes them, like masked tokens, as -inf, and they
+// are written over it in the end.  The stream selects by a table of the 256
+// masks of eight elements and works on pairs of 16-bit values: instructions,
+// not bytes, were its bound with one select and one comparison per logit.
 #include <climits>
 
 #include "launch.cuh"
@@ -36,19 +40,25 @@ namespace {
 
 constexpr int kThreads = 512;  // and 64 registers: two CTAs per SM, one's lists beside the other's stream
 constexpr int kCluster = 8;
-constexpr uint32_t kSegment = 19456;  // tokens per segment: an eighth of a vocabulary of 150 thousand in one go
-constexpr uint32_t kWords = kSegment / 32;
-constexpr uint32_t kBiasShift = 20;   // count below, bias entry + 1 above
+// Tokens per segment: 32 KiB of logits, of which two CTAs on an SM hold two
+// each.
+template <class T>
+constexpr uint32_t kSegment = 32768 / sizeof(T);
+// Tokens whose lists are held at a time, or, for lists that name more tokens
+// than fit beside them, half a segment.
+constexpr uint32_t kBlock = 262144;
+constexpr uint32_t kMaxSmem = 226 * 1024;
+constexpr uint32_t kSeen = 1u << 31;  // of a named token's word: it is in the history; the count below
 
 struct Best {
     float z;
     uint32_t v;
 };
 
-// Ascending v only, so an equal z never replaces an earlier one; -inf is
-// never taken.
-__device__ __forceinline__ void take(Best& b, float z, uint32_t v) {
-    if (z > b.z || (z != z && b.z == b.z)) b.z = z, b.v = v;
+// The greater of b and (z, v), of equal ones the lower v; -inf is never taken.
+__device__ __forceinline__ void take_any(Best& b, float z, uint32_t v) {
+    const bool nz = z != z, nb = b.z != b.z;
+    if (nz ? (!nb || v < b.v) : (!nb && (z > b.z || (z == b.z && v < b.v && z != -INFINITY)))) b.z = z, b.v = v;
 }
 
 // Orders (z, lowest v) as an integer; 0 below everything.
@@ -72,51 +82,91 @@ __device__ __forceinline__ void store_f(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
 
-template <class T, int N>
-struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
-    T v[N];
-};
+constexpr uint32_t kNone = UINT_MAX;
 
 __device__ __forceinline__ long long list_at(const void* p, int is64, long long i) {
     return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int32_t*>(p)[i];
 }
 
-// Entries [from, to) of a list of token ids whose token lies in the segment:
-// f(position in the segment, entry).
-template <class F>
-__device__ __forceinline__ void each_in(const void* list, int is64, long long at, uint32_t from, uint32_t to, uint32_t vocab, uint32_t shift,
-                                        uint32_t size, F f) {
-    uint32_t i = from + threadIdx.x;
-    for (; i + 3 * kThreads < to; i += 4 * kThreads) {
-        long long v[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) v[q] = list_at(list, is64, at + i + q * kThreads);
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t p = (uint32_t)v[q] + shift;
-            if ((unsigned long long)v[q] < vocab && p < size) f(p, i + q * kThreads);
-        }
-    }
-    for (; i < to; i += kThreads) {
-        const long long v = list_at(list, is64, at + i);
-        const uint32_t p = (uint32_t)v + shift;
-        if ((unsigned long long)v < vocab && p < size) f(p, i);
-    }
+// A token id, kNone outside the vocabulary.
+__device__ __forceinline__ uint32_t place(long long v, uint32_t vocab) { return (unsigned long long)v < vocab ? (uint32_t)v : kNone; }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-__host__ __device__ constexpr size_t head_bytes() { return (3 * kWords + 4) * 4; }
+// Eight 16-bit or four 32-bit logits: selection, maximum, one element.
+template <class T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static __device__ __forceinline__ void select(uint4& x, uint32_t ok, const uint4*) {
+        constexpr uint32_t low = 0xff800000u;
+        x.x = ok & 1 ? x.x : low, x.y = ok & 2 ? x.y : low, x.z = ok & 4 ? x.z : low, x.w = ok & 8 ? x.w : low;
+    }
+    static __device__ __forceinline__ float top(const uint4& x) {
+        return max_nan(max_nan(__uint_as_float(x.x), __uint_as_float(x.y)), max_nan(__uint_as_float(x.z), __uint_as_float(x.w)));
+    }
+};
+template <class T>
+struct Vec16 {
+    static constexpr uint32_t kLow = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    static __device__ __forceinline__ void select(uint4& x, uint32_t ok, const uint4* table) {
+        const uint4 m = table[ok & 255];
+        x.x = (x.x & m.x) | (kLow & ~m.x), x.y = (x.y & m.y) | (kLow & ~m.y);
+        x.z = (x.z & m.z) | (kLow & ~m.z), x.w = (x.w & m.w) | (kLow & ~m.w);
+    }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float top(const uint4& x) {
+        const uint32_t m = max2(max2(x.x, x.y), max2(x.z, x.w));
+        const T* h = reinterpret_cast<const T*>(&m);
+        return max_nan(load_f(h[0]), load_f(h[1]));
+    }
+};
+template <>
+struct Vec<__half> : Vec16<__half> {};
+template <>
+struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
 
-// T: logits, O: output (written where a.out is not null).  The segment's
-// tokens are addressed by p = v + head, where head is the row's offset from
-// a 16-byte boundary in elements, so that vectors, bitmaps and words line up
-// in rows of any alignment.  Dynamic shared memory: the bitmaps and the bit
-// counts before their words, the named tokens' words, the segment's logits.
+// Where a kernel's dynamic shared memory has what, in 32-bit words.
+struct RulesLayout {
+    uint32_t segment, block, buffers, bits, before, count, bias, pos, ok, buf, bytes;
+    // span: tokens of a CTA's part of the row; most: entries of its lists
+    RulesLayout(uint32_t span, uint32_t block_, uint64_t most, bool biases, uint32_t segment_, uint32_t size, uint32_t buffers_) {
+        segment = segment_, block = span < block_ ? span : block_, buffers = buffers_;
+        const uint32_t groups = (block + 127) / 128, named = (uint32_t)((most < block ? most : block) + 31) / 32 * 32;
+        uint32_t at = 1024;  // the table of masks
+        bits = at, at += named ? groups * 4 : 0;  // groups of 128 tokens
+        before = at, at += named ? groups : 0;
+        count = at, at += named;
+        bias = at, at += biases ? named : 0;
+        pos = at, at += named;
+        const uint32_t held = span < segment ? span : segment;  // a multiple of 128
+        ok = at, at += held / 32;
+        buf = at = (at + 31) / 32 * 32;
+        bytes = at * 4 + held * size * buffers;
+    }
+};
+
+// T: logits, O: output (written where a.out is not null).  The row's tokens
+// are addressed by p = v + head, where head is the row's offset from a 16-byte
+// boundary in elements, so that vectors and bitmaps line up in rows of any
+// alignment.  A CTA's part of the row goes in blocks of at most kBlock tokens,
+// and these in segments.
 template <class T, class O>
-__global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, uint32_t named) {
-    constexpr int VEC = 16 / sizeof(T);
+__global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const RulesLayout l) {
+    constexpr uint32_t VEC = 16 / sizeof(T), kPer = (kSegment<T> / 32 + kThreads - 1) / kThreads;
+    constexpr int kHeld = 8;  // entries of the history that a thread keeps in registers
     extern __shared__ __align__(128) uint32_t smem[];
-    __shared__ uint64_t arrived;
-    __shared__ uint32_t dead;
+    __shared__ uint64_t arrived[2];
+    __shared__ uint32_t dead, warp_bits[kThreads / 32];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), cl = (int)cluster.num_blocks();
     const long long row = blockIdx.x / cl;
@@ -128,26 +178,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, uint32
     const bool out_vec = out && reinterpret_cast<uintptr_t>(out) % 16 == head * sizeof(O) % 16;
     const uint32_t span = ((end + cl - 1) / cl + 127) / 128 * 128;
     const uint32_t first = min(end, rank * span), last = min(end, first + span);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    uint32_t* seen = smem;
-    uint32_t* touched = seen + kWords;
-    uint32_t* before = touched + kWords;  // kWords + 4
-    uint32_t* word = before + kWords + 4;
-    T* buf = reinterpret_cast<T*>(word + named);
+    const uint4* table = reinterpret_cast<const uint4*>(smem);
+    uint32_t *bits = smem + l.bits, *before = smem + l.before, *count = smem + l.count, *bias = smem + l.bias, *pos = smem + l.pos,
+             *okw = smem + l.ok;
+    T* bufs = reinterpret_cast<T*>(smem + l.buf);
+    // segment s's whole vectors to one of the two buffers, by one thread
+    const auto fetch = [&](uint32_t s) {
+        const uint32_t lo = first + s * l.segment;
+        if (lo >= last) return;
+        const uint32_t hi = min(last, lo + l.segment), from = lo == 0 && head ? VEC : lo, to = hi / VEC * VEC;
+        const uint32_t bytes = to > from ? (to - from) * (uint32_t)sizeof(T) : 0;
+        const uint32_t at = s & (l.buffers - 1);
+        mbar_expect(&arrived[at], bytes);
+        if (bytes) bulk_copy(smem_u32(bufs + at * l.segment + (from - lo)), x + from - head, bytes, &arrived[at]);
+    };
     if (threadIdx.x == 0) {
-        mbar_init(&arrived, 1);
+        mbar_init(&arrived[0], 1);
+        mbar_init(&arrived[1], 1);
         dead = 0;
         fence_async_shared();
+        fetch(0);
+        if (l.buffers == 2) fetch(1);
     }
-    __syncthreads();
-    // the whole vectors of [lo, hi) to buf, by one thread
-    const auto fetch = [&](uint32_t lo, uint32_t hi) {
-        const uint32_t from = lo == 0 && head ? VEC : lo, to = hi / VEC * VEC;
-        const uint32_t bytes = to > from ? (to - from) * (uint32_t)sizeof(T) : 0;
-        mbar_expect(&arrived, bytes);
-        if (bytes) bulk_copy(smem_u32(buf + (from - lo)), x + from - head, bytes, &arrived);
-    };
-    if (threadIdx.x == 0 && first < last) fetch(first, min(last, first + kSegment));
 
     const uint32_t hist = a.tokens ? (uint32_t)max(0, min(a.lengths ? a.lengths[row] : INT_MAX, (int)a.token_cols)) : 0u;
     const uint32_t prompt = a.prompt_lengths ? (uint32_t)max(0, a.prompt_lengths[row]) : 0u;
@@ -158,123 +212,206 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, uint32
     const float pres = a.presence ? a.presence[row] : 0.f;
     const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
     const uint32_t words = (a.vocab + 31) / 32;
-    const bool lists = hist || biases;
+    const bool lists = hist || biases, plain = !lists && !mask;
+    // the mask's bits of the 32 tokens from p on, a multiple of 32; others 0
+    const auto mask_at = [&](uint32_t p) {
+        const long long v0 = (long long)p - head, w = v0 >> 5;  // v0 < 0 in a misaligned row's first word
+        const uint32_t m0 = w >= 0 && w < words ? mask[w] : 0u, m1 = head && w + 1 < words ? mask[w + 1] : 0u;
+        return __funnelshift_r(m0, m1, (uint32_t)(v0 & 31));
+    };
 
-    Best best{-INFINITY, UINT_MAX};
-    uint32_t phase = 0;
-    for (uint32_t lo = first; lo < last; lo += kSegment, phase ^= 1) {
-        const uint32_t hi = min(last, lo + kSegment), size = hi - lo, shift = head - lo;
-        if (lo != first) {
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                fence_async_shared();
-                fetch(lo, hi);
-            }
-        }
+    // the first entries of the lists, and the mask's words of the next segment
+    uint32_t held[kHeld], held_bias = kNone, next_mask[kPer];
+#pragma unroll
+    for (int q = 0; q < kHeld; q++) held[q] = kNone;
+    if (mask) {
+#pragma unroll
+        for (uint32_t q = 0; q < kPer; q++) next_mask[q] = mask_at(first + (threadIdx.x + q * kThreads) * 32);
+    }
+    if (hist) {
+        long long v[kHeld];
+#pragma unroll
+        for (int q = 0; q < kHeld; q++) v[q] = list_at(a.tokens, a.tokens64, tok0 + min(threadIdx.x + q * kThreads, hist - 1));
+#pragma unroll
+        for (int q = 0; q < kHeld; q++)
+            if (threadIdx.x + q * kThreads < hist) held[q] = place(v[q], a.vocab);
+    }
+    if (threadIdx.x < biases) held_bias = place(list_at(a.bias_ids, a.bias64, bid0 + threadIdx.x), a.vocab);
+    if (sizeof(T) == 2 && !plain && threadIdx.x < 256) {
+        const uint32_t b = threadIdx.x;
+        const auto pair = [&](int i) { return (b >> i & 1 ? 0xffffu : 0u) | (b >> (i + 1) & 1 ? 0xffff0000u : 0u); };
+        reinterpret_cast<uint4*>(smem)[b] = make_uint4(pair(0), pair(2), pair(4), pair(6));
+    }
+
+    Best named{-INFINITY, UINT_MAX}, best{-INFINITY, UINT_MAX};
+    uint32_t s = 0;  // segment
+    for (uint32_t blk = first; blk < last; blk += l.block) {
+        const uint32_t blk_end = min(last, blk + l.block), size = blk_end - blk, groups = (size + 127) / 128;
+        uint32_t total = 0;  // named tokens
         if (lists) {
-            for (uint32_t i = threadIdx.x; i < 2 * kWords; i += kThreads) smem[i] = 0u;
+            // f(position in the block, entry) for the block's entries of a list
+            const auto each_token = [&](auto f) {
+                if (!hist) return;
+#pragma unroll
+                for (int q = 0; q < kHeld; q++)
+                    if (held[q] != kNone && held[q] + head - blk < size) f(held[q] + head - blk, threadIdx.x + q * kThreads);
+                for (uint32_t i = threadIdx.x + kHeld * kThreads; i < hist; i += kThreads) {
+                    const uint32_t v = place(list_at(a.tokens, a.tokens64, tok0 + i), a.vocab);
+                    if (v != kNone && v + head - blk < size) f(v + head - blk, i);
+                }
+            };
+            const auto each_bias = [&](auto f) {
+                if (held_bias != kNone && held_bias + head - blk < size) f(held_bias + head - blk, threadIdx.x);
+                for (uint32_t i = threadIdx.x + kThreads; i < biases; i += kThreads) {
+                    const uint32_t v = place(list_at(a.bias_ids, a.bias64, bid0 + i), a.vocab);
+                    if (v != kNone && v + head - blk < size) f(v + head - blk, i);
+                }
+            };
+            const auto slot = [&](uint32_t p) {
+                const uint4 w = reinterpret_cast<const uint4*>(bits)[p / 128];
+                const uint32_t q = p / 32 % 4, own = q == 0 ? w.x : q == 1 ? w.y : q == 2 ? w.z : w.w;
+                return before[p / 128] + (q > 0 ? __popc(w.x) : 0) + (q > 1 ? __popc(w.y) : 0) + (q > 2 ? __popc(w.z) : 0) +
+                       __popc(own & ((1u << p % 32) - 1));
+            };
+            if (blk != first) __syncthreads();
+            for (uint32_t i = threadIdx.x; i < groups; i += kThreads) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (uint32_t i = threadIdx.x; i < l.bias - l.count; i += kThreads) count[i] = 0u;
+            if (biases)
+                for (uint32_t i = threadIdx.x; i < l.pos - l.bias; i += kThreads) bias[i] = 0u;
             __syncthreads();
-            each_in(a.bias_ids, a.bias64, bid0, 0, biases, a.vocab, shift, size, [&](uint32_t p, uint32_t) { atomicOr(touched + p / 32, 1u << p % 32); });
-            each_in(a.tokens, a.tokens64, tok0, 0, hist, a.vocab, shift, size, [&](uint32_t p, uint32_t) {
-                atomicOr(touched + p / 32, 1u << p % 32);
-                atomicOr(seen + p / 32, 1u << p % 32);
-            });
-            const uint32_t most = min(named, size);
-            for (uint32_t i = threadIdx.x; i < most; i += kThreads) word[i] = 0u;
+            each_bias([&](uint32_t p, uint32_t) { atomicOr(bits + p / 32, 1u << p % 32); });
+            each_token([&](uint32_t p, uint32_t) { atomicOr(bits + p / 32, 1u << p % 32); });
             __syncthreads();
-            if (threadIdx.x < 32) {
-                // bits before each word: 19 words a lane
-                constexpr uint32_t kEach = kWords / 32;
-                static_assert(kWords % 32 == 0, "a lane has whole words");
+            // bits before each group, 512 groups at a time
+            uint32_t base = 0;
+            for (uint32_t g0 = 0; g0 < groups; g0 += kThreads) {
+                const uint32_t g = g0 + threadIdx.x;
                 uint32_t sum = 0;
-                for (uint32_t i = 0; i < kEach; i++) {
-                    before[threadIdx.x * kEach + i] = sum;
-                    sum += __popc(touched[threadIdx.x * kEach + i]);
+                if (g < groups) {
+                    const uint4 w = reinterpret_cast<const uint4*>(bits)[g];
+                    sum = __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w);
                 }
                 uint32_t incl = sum;
 #pragma unroll
                 for (int q = 1; q < 32; q <<= 1) {
                     const uint32_t y = __shfl_up_sync(0xffffffffu, incl, q);
-                    if (threadIdx.x >= q) incl += y;
+                    if (lane >= q) incl += y;
                 }
-                for (uint32_t i = 0; i < kEach; i++) before[threadIdx.x * kEach + i] += incl - sum;
+                if (lane == 31) warp_bits[warp] = incl;
+                __syncthreads();
+                uint32_t at = base + incl - sum;
+#pragma unroll
+                for (int q = 0; q < kThreads / 32; q++) at += q < warp ? warp_bits[q] : 0u, base += warp_bits[q];
+                if (g < groups) before[g] = at;
+                __syncthreads();
             }
+            total = base;
+            each_bias([&](uint32_t p, uint32_t i) {
+                const uint32_t at = slot(p);
+                pos[at] = p;
+                atomicMax(bias + at, i + 1);
+            });
+            each_token([&](uint32_t p, uint32_t i) {
+                const uint32_t at = slot(p);
+                pos[at] = p;
+                atomicOr(count + at, kSeen);
+                if (i >= prompt) atomicAdd(count + at, 1u);
+            });
             __syncthreads();
+            // the named tokens' results, kept as bits in place of their counts
+            for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
+                const uint32_t p = blk + pos[i], v = p - head;
+                float z = load_f(x[v]);
+                const uint32_t c = count[i], n = c & ~kSeen, b = biases ? bias[i] : 0u;
+                const uint32_t m = mask ? mask[v / 32] >> v % 32 : 1u;
+                const float add = b ? a.bias_values[bval0 + b - 1] : 0.f;
+                if (c & kSeen) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+                if (n) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)n)), pres);
+                if (b) z = __fadd_rn(z, add);
+                if (!(m & 1)) z = -INFINITY;
+                take_any(named, z, v);
+                count[i] = __float_as_uint(z);
+            }
+            __syncthreads();  // every named logit has been read: out may be logits itself
         }
-        const auto slot = [&](uint32_t p) { return before[p / 32] + __popc(touched[p / 32] & ((1u << p % 32) - 1)); };
-        if (lists) {
-            each_in(a.bias_ids, a.bias64, bid0, 0, biases, a.vocab, shift, size,
-                    [&](uint32_t p, uint32_t i) { atomicMax(word + slot(p), (i + 1) << kBiasShift); });
+        for (uint32_t lo = blk; lo < blk_end; lo += l.segment, s++) {
+            const uint32_t hi = min(blk_end, lo + l.segment), used = (hi - lo + 31) / 32;
+            const uint32_t at = s & (l.buffers - 1);
+            const T* buf = bufs + at * l.segment;
+            if (!plain) {
+#pragma unroll
+                for (uint32_t q = 0; q < kPer; q++) {
+                    const uint32_t i = threadIdx.x + q * kThreads;
+                    if (i < used) okw[i] = (mask ? next_mask[q] : UINT_MAX) & ~(lists ? bits[(lo - blk) / 32 + i] : 0u);
+                }
+                if (mask && hi < last) {
+#pragma unroll
+                    for (uint32_t q = 0; q < kPer; q++) next_mask[q] = mask_at(hi + (threadIdx.x + q * kThreads) * 32);
+                }
+            }
             __syncthreads();
-            each_in(a.tokens, a.tokens64, tok0, prompt, hist, a.vocab, shift, size, [&](uint32_t p, uint32_t) { atomicAdd(word + slot(p), 1u); });
-            __syncthreads();
-        }
-        mbar_wait(&arrived, phase, &dead);
-        for (uint32_t p0 = lo + threadIdx.x * VEC; p0 < hi; p0 += kThreads * VEC) {
-            const bool whole = p0 >= head && p0 + VEC <= hi;
-            Pack<T, VEC> in;
-            if (whole) {
-                in = *reinterpret_cast<const Pack<T, VEC>*>(buf + (p0 - lo));
-            } else {
+            mbar_wait(&arrived[at], s / l.buffers & 1, &dead);
+            // this thread's greatest vector of the segment; its element is found afterwards
+            float top = -INFINITY;
+            uint32_t top_at = kNone;
+            for (uint32_t q = threadIdx.x * VEC; q < hi - lo; q += kThreads * VEC) {
+                const uint32_t p0 = lo + q;
+                // the vector's bits: VEC <= 8 of them lie in one word
+                const uint32_t ok = plain ? UINT_MAX : okw[q / 32] >> q % 32;
+                if (p0 >= head && p0 + VEC <= hi) {
+                    uint4 z = *reinterpret_cast<const uint4*>(buf + q);
+                    if (!plain) Vec<T>::select(z, ok, table);
+                    const float m = Vec<T>::top(z);
+                    if (!(m <= top) && top == top) top = m, top_at = q;  // a NaN, once there, stays
+                    const T* e = reinterpret_cast<const T*>(&z);
+                    if (out) {
+                        O* to = out + (p0 - head);
+                        if constexpr (std::is_same<T, O>::value) {
+                            if (out_vec) {
+                                *reinterpret_cast<uint4*>(to) = z;
+                                continue;
+                            }
+                        } else if (out_vec) {
+                            float4 f[VEC / 4];
 #pragma unroll
-                for (int i = 0; i < VEC; i++)
-                    if (p0 + i >= head && p0 + i < hi) in.v[i] = x[p0 + i - head];
-            }
-            // the vector's bits; a group of VEC <= 8 lies in one word, since lo is a multiple of 128
-            const uint32_t q = p0 - lo;
-            uint32_t tb = 0, mb = UINT_MAX;
-            if (lists) tb = touched[q / 32] >> q % 32;
-            if (mask) {
-                // token v0 of the vector's first element; v0 < 0 in a row's first vector
-                const long long v0 = (long long)p0 - head;
-                const long long w = v0 >> 5;
-                const uint32_t m0 = w >= 0 ? mask[w] : 0u;
-                const uint32_t m1 = head && w + 1 < words ? mask[w + 1] : 0u;
-                mb = __funnelshift_r(m0, m1, (uint32_t)(v0 & 31));
-            }
-            float z[VEC];
+                            for (uint32_t i = 0; i < VEC / 4; i++)
+                                f[i] = make_float4(load_f(e[4 * i]), load_f(e[4 * i + 1]), load_f(e[4 * i + 2]), load_f(e[4 * i + 3]));
 #pragma unroll
-            for (int i = 0; i < VEC; i++) z[i] = load_f(in.v[i]);
-            constexpr uint32_t kAll = (1u << VEC) - 1;
-            if (tb & kAll) {
-                const uint32_t sb = seen[q / 32] >> q % 32;
+                            for (uint32_t i = 0; i < VEC / 4; i++) reinterpret_cast<float4*>(to)[i] = f[i];
+                            continue;
+                        }
 #pragma unroll
-                for (int i = 0; i < VEC; i++)
-                    if (tb >> i & 1) {
-                        const uint32_t c = word[slot(q + i)];
-                        const uint32_t n = c & ((1u << kBiasShift) - 1), b = c >> kBiasShift;
-                        if (sb >> i & 1) z[i] = z[i] > 0.f ? __fdiv_rn(z[i], rho) : __fmul_rn(z[i], rho);
-                        if (n) z[i] = __fsub_rn(__fsub_rn(z[i], __fmul_rn(freq, (float)n)), pres);
-                        if (b) z[i] = __fadd_rn(z[i], a.bias_values[bval0 + b - 1]);
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                if (!(mb >> i & 1)) z[i] = -INFINITY;
-                if (whole || (p0 + i >= head && p0 + i < hi)) take(best, z[i], p0 + i - head);
-            }
-            if (out) {
-                Pack<O, VEC> res;
-#pragma unroll
-                for (int i = 0; i < VEC; i++) store_f(&res.v[i], z[i]);
-                if (whole && out_vec) {
-                    if constexpr (sizeof(O) * VEC > 16) {
-                        const Pack<O, VEC / 2>* r2 = reinterpret_cast<const Pack<O, VEC / 2>*>(&res);
-                        Pack<O, VEC / 2>* o2 = reinterpret_cast<Pack<O, VEC / 2>*>(out + (p0 - head));
-                        o2[0] = r2[0], o2[1] = r2[1];
-                    } else {
-                        *reinterpret_cast<Pack<O, VEC>*>(out + (p0 - head)) = res;
+                        for (uint32_t i = 0; i < VEC; i++) store_f(to + i, load_f(e[i]));
                     }
                 } else {
-#pragma unroll
-                    for (int i = 0; i < VEC; i++)
-                        if (p0 + i >= head && p0 + i < hi) out[p0 + i - head] = res.v[i];
+                    // the row's ends, which did not come with the copy
+#pragma unroll 1
+                    for (uint32_t i = 0; i < VEC; i++) {
+                        if (p0 + i < head || p0 + i >= hi) continue;
+                        const uint32_t v = p0 + i - head;
+                        const float z = ok >> i & 1 ? load_f(x[v]) : -INFINITY;
+                        take_any(best, z, v);
+                        if (out) store_f(out + v, z);
+                    }
                 }
             }
+            if (top_at != kNone && !(top <= best.z)) {
+                const uint32_t ok = plain ? UINT_MAX : okw[top_at / 32] >> top_at % 32;
+#pragma unroll
+                for (uint32_t i = 0; i < VEC; i++)
+                    if (ok >> i & 1) take_any(best, load_f(buf[top_at + i]), lo + top_at + i - head);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                fence_async_shared();  // what was read from the buffer, before the next copy into it
+                fetch(s + l.buffers);
+            }
         }
+        if (out)
+            for (uint32_t i = threadIdx.x; i < total; i += kThreads) store_f(out + (blk + pos[i] - head), __uint_as_float(count[i]));
     }
 
-    unsigned long long key = key_of(best);
+    unsigned long long key = max(key_of(best), key_of(named));
 #pragma unroll
     for (int q = 16; q; q >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, q));
     __shared__ unsigned long long warp_key[kThreads / 32], cta_key[kCluster];
@@ -295,15 +432,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, uint32
 
 template <class T, class O>
 cudaError_t launch_one(const RulesArgs& a, cudaStream_t s) {
-    // words for as many tokens as the lists can name in a segment
+    // CTAs to a row: the fewest rounds of two CTAs per SM, each with its share of
+    // the row and a twentieth of a row for starting and for the pick
+    int dev = 0, sms = 1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    int cl = 1;
+    double least = 0;
+    for (int c = 1; c <= kCluster; c *= 2) {
+        const double cost = (double)((a.n * c + 2 * sms - 1) / (2 * sms)) * (1.0 / c + 0.05);
+        if (c == 1 || cost < least) cl = c, least = cost;
+    }
     const uint64_t most = (uint64_t)(a.tokens ? a.token_cols : 0) + (a.bias_ids ? a.bias_cols : 0);
-    const uint32_t span = ((a.vocab + 16 + kCluster - 1) / kCluster + 127) / 128 * 128, segment = span < kSegment ? span : kSegment;
-    const uint32_t named = (uint32_t)((most < segment ? most : segment) + 31) / 32 * 32;
-    const size_t smem = head_bytes() + (size_t)named * 4 + (size_t)segment * sizeof(T);
-    const cudaError_t e = ensure_smem(k_rules<T, O>, smem > 48 * 1024 ? smem : smem + 48 * 1024);
+    const uint32_t span = ((a.vocab + 16 + cl - 1) / cl + 127) / 128 * 128;
+    RulesLayout l(span, kBlock, most, a.bias_ids != nullptr, kSegment<T>, sizeof(T), span > kSegment<T> ? 2 : 1);
+    if (l.bytes > kMaxSmem) l = RulesLayout(span, kSegment<T> / 2, most, a.bias_ids != nullptr, kSegment<T> / 2, sizeof(T), 1);
+    e = ensure_smem(k_rules<T, O>, l.bytes + 1024);  // the pick's shared memory is beside it
     if (e != cudaSuccess) return e;
     KScope ks("logit_rules", s);
-    return launch_cl(kCluster, k_rules<T, O>, dim3((unsigned)(a.n * kCluster)), kThreads, smem, s, a, named);
+    return launch_cl(cl, k_rules<T, O>, dim3((unsigned)(a.n * cl)), kThreads, l.bytes, s, a, l);
 }
 
 }  // namespace

@@ -484,6 +484,52 @@ def test_rules_shared_rows_out_and_strides(R):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("n,v,hist,biases,dt", [(300, 40000, 30, 3, "bf16"), (40, 300007, 700, 33, "fp16"), (150, 60000, 20, 0, "fp32"),
+                                                (2, 300007, 60000, 4095, "bf16"), (160, 50001, 40000, 60, "fp32"),
+                                                (160, 50001, 40000, 60, "bf16"), (1, 2100001, 9, 3, "bf16")])
+def test_rules_splits(R, n, v, hist, biases, dt):
+    """Few and many rows (each row on one to eight CTAs, one or more segments
+    and blocks of the vocabulary), short and very long lists."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n + v)
+
+    def ints(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=g, device="cuda", dtype=torch.int64)
+
+    x = (torch.randn((n, v), generator=g, device="cuda") * 3).to(TYPES[dt])
+    kw = dict(tokens=ints(-1, v, n, hist), lengths=ints(0, hist + 1, n).int(), prompt_lengths=ints(0, hist + 1, n).int(),
+              repetition=1 + torch.rand(n, generator=g, device="cuda"), frequency=torch.rand(n, generator=g, device="cuda"),
+              presence=torch.rand(n, generator=g, device="cuda"))
+    if biases:
+        kw.update(bias_ids=ints(0, v, n, biases), bias_values=torch.randn((n, biases), generator=g, device="cuda") * 4)
+    mask = ints(-2 ** 31, 2 ** 31, n, (v + 31) // 32).int()
+    z, pick = R.apply_rules(x, **kw, mask=mask, out=torch.empty((n, v), device="cuda"))
+    # the same steps over whole rows, in 32 bits
+    col = torch.arange(hist, device="cuda")
+    tok = kw["tokens"]
+    used = (col < kw["lengths"][:, None]) & (tok >= 0)
+    spare = torch.where(used, tok, v)
+    seen = torch.zeros((n, v + 1), dtype=torch.int32, device="cuda").scatter_add_(1, spare, used.int())[:, :v] > 0
+    said = used & (col >= kw["prompt_lengths"][:, None])
+    count = torch.zeros((n, v + 1), dtype=torch.int32, device="cuda").scatter_add_(1, torch.where(said, tok, v), said.int())[:, :v]
+    rho, f, p = (kw[k][:, None] for k in ("repetition", "frequency", "presence"))
+    w = x.float()
+    w = torch.where(seen, torch.where(w > 0, w / rho, w * rho), w)
+    w = torch.where(count > 0, w - f * count - p, w)
+    if biases:
+        last = torch.full((n, v), -1, device="cuda", dtype=torch.int64)
+        last.scatter_reduce_(1, kw["bias_ids"], torch.arange(biases, device="cuda").expand(n, biases), "amax")
+        w = torch.where(last >= 0, w + kw["bias_values"].gather(1, last.clamp_min(0)), w)
+    at = torch.arange(v, device="cuda")
+    w = torch.where((mask[:, at // 32] >> (at % 32)) & 1 != 0, w, float("-inf"))
+    assert torch.equal(z, w)
+    best = w.amax(1, keepdim=True)
+    assert torch.equal(pick, torch.where(w == best, at, v).amin(1))
+    inplace = x.clone()
+    same, pick2 = R.apply_rules(inplace, **kw, mask=mask, out=inplace)
+    assert torch.equal(same, w.to(x.dtype)) and torch.equal(pick2, pick)
+
+
 def test_rules_ties_and_special_values(R):
     inf, nan = float("inf"), float("nan")
     rows = torch.zeros((7, 300), device="cuda")
