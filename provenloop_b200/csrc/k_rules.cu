@@ -48,7 +48,7 @@ constexpr uint32_t kSegment = 32768 / sizeof(T);
 // than fit beside them, half a segment.
 constexpr uint32_t kBlock = 262144;
 constexpr uint32_t kMaxSmem = 226 * 1024;
-constexpr uint32_t kSeen = 1u << 31;  // of a named token's word: it is in the history; the count below
+constexpr uint32_t kPrompt = 1u << 31;  // of a named token's word: it is in the prompt; the count behind it below
 
 struct Best {
     float z;
@@ -144,7 +144,7 @@ struct RulesLayout {
         const uint32_t groups = (block + 127) / 128, named = (uint32_t)((most < block ? most : block) + 31) / 32 * 32;
         uint32_t at = 1024;  // the table of masks
         bits = at, at += named ? groups * 4 : 0;  // groups of 128 tokens
-        before = at, at += named ? groups : 0;
+        before = at, at += named ? (groups + 3) / 4 * 4 : 0;
         count = at, at += named;
         bias = at, at += biases ? named : 0;
         pos = at, at += named;
@@ -228,10 +228,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
 #pragma unroll
         for (uint32_t q = 0; q < kPer; q++) next_mask[q] = mask_at(first + (threadIdx.x + q * kThreads) * 32);
     }
-    if (hist) {
+    if (a.tokens) {  // without waiting for the length
         long long v[kHeld];
 #pragma unroll
-        for (int q = 0; q < kHeld; q++) v[q] = list_at(a.tokens, a.tokens64, tok0 + min(threadIdx.x + q * kThreads, hist - 1));
+        for (int q = 0; q < kHeld; q++) v[q] = list_at(a.tokens, a.tokens64, tok0 + min(threadIdx.x + q * kThreads, a.token_cols - 1));
 #pragma unroll
         for (int q = 0; q < kHeld; q++)
             if (threadIdx.x + q * kThreads < hist) held[q] = place(v[q], a.vocab);
@@ -244,7 +244,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
     }
 
     Best named{-INFINITY, UINT_MAX}, best{-INFINITY, UINT_MAX};
-    uint32_t s = 0;  // segment
+    // this thread's first vector with the greatest element; which it is is found in the end
+    float top = -INFINITY;
+    uint32_t top_at = kNone, s = 0;  // s: segment
+    uint4 top_z = make_uint4(0, 0, 0, 0);
     for (uint32_t blk = first; blk < last; blk += l.block) {
         const uint32_t blk_end = min(last, blk + l.block), size = blk_end - blk, groups = (size + 127) / 128;
         uint32_t total = 0;  // named tokens
@@ -274,38 +277,33 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
                        __popc(own & ((1u << p % 32) - 1));
             };
             if (blk != first) __syncthreads();
-            for (uint32_t i = threadIdx.x; i < groups; i += kThreads) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
-            for (uint32_t i = threadIdx.x; i < l.bias - l.count; i += kThreads) count[i] = 0u;
-            if (biases)
-                for (uint32_t i = threadIdx.x; i < l.pos - l.bias; i += kThreads) bias[i] = 0u;
+            // bits, before, count and bias lie one behind the other
+            for (uint32_t i = threadIdx.x; i < (l.pos - l.bits) / 4; i += kThreads) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
             each_bias([&](uint32_t p, uint32_t) { atomicOr(bits + p / 32, 1u << p % 32); });
             each_token([&](uint32_t p, uint32_t) { atomicOr(bits + p / 32, 1u << p % 32); });
             __syncthreads();
-            // bits before each group, 512 groups at a time
-            uint32_t base = 0;
-            for (uint32_t g0 = 0; g0 < groups; g0 += kThreads) {
-                const uint32_t g = g0 + threadIdx.x;
-                uint32_t sum = 0;
-                if (g < groups) {
-                    const uint4 w = reinterpret_cast<const uint4*>(bits)[g];
-                    sum = __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w);
-                }
-                uint32_t incl = sum;
-#pragma unroll
-                for (int q = 1; q < 32; q <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, q);
-                    if (lane >= q) incl += y;
-                }
-                if (lane == 31) warp_bits[warp] = incl;
-                __syncthreads();
-                uint32_t at = base + incl - sum;
-#pragma unroll
-                for (int q = 0; q < kThreads / 32; q++) at += q < warp ? warp_bits[q] : 0u, base += warp_bits[q];
-                if (g < groups) before[g] = at;
-                __syncthreads();
+            // bits before each group; a thread has neighbouring ones
+            const uint32_t each = (groups + kThreads - 1) / kThreads, g0 = threadIdx.x * each, g1 = min(groups, g0 + each);
+            uint32_t sum = 0;
+            for (uint32_t g = g0; g < g1; g++) {
+                const uint4 w = reinterpret_cast<const uint4*>(bits)[g];
+                before[g] = sum;
+                sum += __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w);
             }
-            total = base;
+            uint32_t incl = sum;
+#pragma unroll
+            for (int q = 1; q < 32; q <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, incl, q);
+                if (lane >= q) incl += y;
+            }
+            if (lane == 31) warp_bits[warp] = incl;
+            __syncthreads();
+            uint32_t below = incl - sum;
+#pragma unroll
+            for (int q = 0; q < kThreads / 32; q++) below += q < warp ? warp_bits[q] : 0u, total += warp_bits[q];
+            for (uint32_t g = g0; g < g1; g++) before[g] += below;
+            __syncthreads();
             each_bias([&](uint32_t p, uint32_t i) {
                 const uint32_t at = slot(p);
                 pos[at] = p;
@@ -314,18 +312,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
             each_token([&](uint32_t p, uint32_t i) {
                 const uint32_t at = slot(p);
                 pos[at] = p;
-                atomicOr(count + at, kSeen);
-                if (i >= prompt) atomicAdd(count + at, 1u);
+                if (i < prompt) atomicOr(count + at, kPrompt);
+                else atomicAdd(count + at, 1u);
             });
             __syncthreads();
             // the named tokens' results, kept as bits in place of their counts
             for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
                 const uint32_t p = blk + pos[i], v = p - head;
                 float z = load_f(x[v]);
-                const uint32_t c = count[i], n = c & ~kSeen, b = biases ? bias[i] : 0u;
+                const uint32_t c = count[i], n = c & ~kPrompt, b = biases ? bias[i] : 0u;
                 const uint32_t m = mask ? mask[v / 32] >> v % 32 : 1u;
                 const float add = b ? a.bias_values[bval0 + b - 1] : 0.f;
-                if (c & kSeen) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+                if (c) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
                 if (n) z = __fsub_rn(__fsub_rn(z, __fmul_rn(freq, (float)n)), pres);
                 if (b) z = __fadd_rn(z, add);
                 if (!(m & 1)) z = -INFINITY;
@@ -351,9 +349,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
             }
             __syncthreads();
             mbar_wait(&arrived[at], s / l.buffers & 1, &dead);
-            // this thread's greatest vector of the segment; its element is found afterwards
-            float top = -INFINITY;
-            uint32_t top_at = kNone;
             for (uint32_t q = threadIdx.x * VEC; q < hi - lo; q += kThreads * VEC) {
                 const uint32_t p0 = lo + q;
                 // the vector's bits: VEC <= 8 of them lie in one word
@@ -362,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
                     uint4 z = *reinterpret_cast<const uint4*>(buf + q);
                     if (!plain) Vec<T>::select(z, ok, table);
                     const float m = Vec<T>::top(z);
-                    if (!(m <= top) && top == top) top = m, top_at = q;  // a NaN, once there, stays
+                    if (!(m <= top) && top == top) top = m, top_at = p0 - head, top_z = z;  // a NaN, once there, stays
                     const T* e = reinterpret_cast<const T*>(&z);
                     if (out) {
                         O* to = out + (p0 - head);
@@ -395,12 +390,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
                     }
                 }
             }
-            if (top_at != kNone && !(top <= best.z)) {
-                const uint32_t ok = plain ? UINT_MAX : okw[top_at / 32] >> top_at % 32;
-#pragma unroll
-                for (uint32_t i = 0; i < VEC; i++)
-                    if (ok >> i & 1) take_any(best, load_f(buf[top_at + i]), lo + top_at + i - head);
-            }
             __syncthreads();
             if (threadIdx.x == 0) {
                 fence_async_shared();  // what was read from the buffer, before the next copy into it
@@ -411,6 +400,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
             for (uint32_t i = threadIdx.x; i < total; i += kThreads) store_f(out + (blk + pos[i] - head), __uint_as_float(count[i]));
     }
 
+    if (top_at != kNone) {
+        const T* e = reinterpret_cast<const T*>(&top_z);
+#pragma unroll
+        for (uint32_t i = 0; i < VEC; i++) take_any(best, load_f(e[i]), top_at + i);
+    }
     unsigned long long key = max(key_of(best), key_of(named));
 #pragma unroll
     for (int q = 16; q; q >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, q));
