@@ -120,12 +120,14 @@ int check_adapter(const ts_adapter_args* a, int backward) {
 
 uint64_t up(uint64_t b) { return (b + 255) & ~255ull; }
 
-int up8(uint32_t d) { return (int)((d + 7) & ~7u); }
+// A row of `d` elements up to the next 16 bytes.
+int up16(uint32_t d, size_t size) { return (int)((d * size + 15) / 16 * (16 / size)); }
+int up8(uint32_t d) { return up16(d, 2); }
 
-// Rows of 16-bit elements that 16-byte loads and TMA take as they are: on
-// 16-byte boundaries, and one behind the other.
-bool rows_ok(const void* p, uint64_t rows, uint32_t cols, int64_t stride) {
-    return aligned_to(p, 16) && (rows < 2 || (stride % 8 == 0 && stride >= cols && stride < (1ll << 38)));
+// Rows that 16-byte loads, bulk copies and TMA take as they are: on 16-byte
+// boundaries, and one behind the other.
+bool rows_ok(const void* p, uint64_t rows, uint32_t cols, int64_t stride, size_t size) {
+    return aligned_to(p, 16) && (rows < 2 || (stride * size % 16 == 0 && stride >= cols && stride < (1ll << 38)));
 }
 
 // What a call does with its sizes and pointers, and where it puts it.
@@ -144,15 +146,15 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     Plan p{};
     p.f32 = a->dtype == TS_DTYPE_F32;
     p.out = !backward || a->out;
-    const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride);
-    const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in);
+    const size_t size = dtype_size(a->dtype);
+    const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride, size), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride, size);
+    const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in, size), g_ok = rows_ok(a->grad, a->n, a->d_out, a->grad_stride, size);
     p.small = !p.f32 && !backward && a->n <= (uint64_t)kSmallTokens && (!a->weight || (x_ok && w_ok));
     const bool whole_low = !low_by_token((long long)a->n, a->d_in, a->d_in, a->r);  // by matrix instructions: aligned operands only
     if (p.f32) {
-        const auto ok = [](const void* q, uint32_t cols, int64_t stride, uint64_t rows) {
-            return aligned_to(q, 16) && (rows < 2 || (stride % 4 == 0 && stride >= cols));
-        };
-        p.low_vec = !backward && ok(a->x, a->d_in, a->x_stride, a->n) && ok(a->lora_a, a->d_in, a->d_in, 2);
+        p.low_vec = !backward && x_ok && a_ok;
+        p.pack_x = backward && a->grad_a && !x_ok;
+        p.pack_grad = backward && a->grad_a && !g_ok;
     } else if (!backward) {
         p.pack_x = !x_ok && ((a->weight && !p.small) || whole_low);
         p.pack_w = a->weight && !p.small && !w_ok;
@@ -163,7 +165,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_x = !x_ok && a->grad_a;
         p.pack_a = !a_ok && a->grad_a;
         p.pack_w = a->weight && a->out && !w_ok;
-        p.pack_grad = !rows_ok(a->grad, a->n, a->d_out, a->grad_stride);
+        p.pack_grad = !g_ok;
         p.pack_b = true;
         p.low_vec = true;
         p.g32 = a->out && !factor_by_token((long long)a->n, a->d_in, a->r);
@@ -178,10 +180,10 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     const uint64_t rs = low_stride((int)a->r), low = a->n * rs * 4, o = backward ? a->d_in : a->d_out;
     p.low = take(!backward || a->grad_a, low);
     p.u = take(backward, low);
-    p.x = take(p.pack_x, a->n * up8(a->d_in) * 2);
+    p.x = take(p.pack_x, a->n * up16(a->d_in, size) * size);
     p.w = take(p.pack_w, (uint64_t)a->d_out * up8(a->d_in) * 2);
     p.a = take(p.pack_a, (uint64_t)a->adapters * a->r * up8(a->d_in) * 2);
-    p.grad = take(p.pack_grad, a->n * up8(a->d_out) * 2);
+    p.grad = take(p.pack_grad, a->n * up16(a->d_out, size) * size);
     p.b = take(p.pack_b, (uint64_t)a->adapters * a->r * up8(a->d_out) * 2);
     p.g = take(p.g32, a->adapters * o * rs * 4);
     p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * (rs / 16) * 4);
@@ -224,10 +226,12 @@ struct Work {
     int after_pack = 0;  // 2: what is packed is used by the next launch
     void* at(uint64_t off) const { return static_cast<char*>(a->workspace) + off; }
     Rows rows(bool pack, const void* p, uint64_t rows, uint32_t cols, long long stride, uint64_t off) {
-        if (!pack) return {p, rows < 2 ? up8(cols) : stride};
-        jobs.add({PackJob::COPY, p, 0, stride, 1, (long long)rows, 1, (int)cols, up8(cols), at(off)});
+        const size_t size = dtype_size(a->dtype);
+        const int pitch = up16(cols, size), halves = (int)size / 2;  // elements are copied as 16-bit ones
+        if (!pack) return {p, rows < 2 ? pitch : stride};
+        jobs.add({PackJob::COPY, p, 0, stride * halves, 1, (long long)rows, 1, (int)cols * halves, pitch * halves, at(off)});
         after_pack = 2;
-        return {at(off), up8(cols)};
+        return {at(off), pitch};
     }
     cudaError_t pack() {
         if (!jobs.jobs) return cudaSuccess;
@@ -284,7 +288,10 @@ int adapter_project_backward(const ts_adapter_args* a) {
     float *low = static_cast<float*>(w.at(p.low)), *u = static_cast<float*>(w.at(p.u));
     Rows x{a->x, a->x_stride}, wt{a->weight, a->weight_stride}, grad{a->grad, a->grad_stride}, fa{a->lora_a, di};
     Factor fb{a->lora_b, rb, 1, r};
-    if (!p.f32) {
+    if (p.f32) {
+        if (p.pack_x) x = w.rows(true, a->x, a->n, a->d_in, a->x_stride, p.x);
+        if (p.pack_grad) grad = w.rows(true, a->grad, a->n, a->d_out, a->grad_stride, p.grad);
+    } else {
         x = w.rows(p.pack_x, a->x, a->n, a->d_in, a->x_stride, p.x);
         wt = w.rows(p.pack_w, a->weight, a->d_out, a->d_in, a->weight_stride, p.w);
         grad = w.rows(p.pack_grad, a->grad, a->n, a->d_out, a->grad_stride, p.grad);
@@ -313,8 +320,7 @@ int adapter_project_backward(const ts_adapter_args* a) {
     if (e == cudaSuccess && a->grad_a) {
         const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}},
                          r, (int)a->adapters, first, first + a->adapters + 1};
-        const bool vec = !p.f32 || (aligned_to(x.p, 16) && x.stride % 4 == 0 && aligned_to(grad.p, 16) && grad.stride % 4 == 0);
-        e = launch_grads(g, n, a->dtype, vec, w.s);
+        e = launch_grads(g, n, a->dtype, w.s);
     }
     return cuda_status(e);
 }

@@ -229,11 +229,6 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs j
 
 // ---------------------------------------------------------------- low
 
-struct LowPair {
-    LowArgs a[2];
-    int after_pack;
-};
-
 // What is stored of a sum: see LowArgs.
 template <class T>
 __device__ __forceinline__ float low_value(float v) {
@@ -281,99 +276,6 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
     }
     if (part == 0 && lane == 0 && j < rs) a.low[m * rs + j] = e >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e] * v : v) : 0.f;
     // the next launch waits for this one, and with it for the packing
-    if (both.after_pack == 1) grid_dependency_wait();
-}
-
-// 32 tokens per cluster of S CTAs, 8 S warps sharing the contraction in
-// 32-wide blocks.  Operands go from global memory to the matrix
-// instructions' registers: a thread's 16 bytes of a row are the k indexes
-// of two instructions, in the same (permuted) order for x and the factor.
-// For each distinct adapter among the 32 tokens all rows are multiplied and
-// the adapter's own are kept, so that another adapter's NaN stays out.
-template <class T>
-__global__ void __launch_bounds__(256) k_low_mma(const LowPair both) {
-    release_dependents();
-    if (both.after_pack == 2) grid_dependency_wait();
-    const LowArgs a = both.a[blockIdx.z];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const long long m0 = (long long)(blockIdx.x / S) * 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int rs = low_stride(a.r);
-    __shared__ float red[8][32][33];
-    __shared__ float sum[32][33];
-    const int id = m0 + lane < a.n ? a.id.of(m0 + lane) : -1;
-    const unsigned in = (unsigned)min(32ll, a.n - m0);
-    const T* xr[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const long long m = m0 + g + 8 * i;  // rows behind the last token repeat it; they are not stored
-        xr[i] = static_cast<const T*>(a.x) + (m < a.n ? m : a.n - 1) * a.x_stride;
-    }
-    unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
-    // tokens without an adapter
-    if (rank == 0)
-        for (int i = threadIdx.x; i < 32 * rs; i += 256) {
-            const int row = i / rs;
-            if ((unsigned)row < in && !(todo >> row & 1)) a.low[(m0 + row) * rs + i % rs] = 0.f;
-        }
-    while (todo) {
-        const int e = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
-        const unsigned mine = __ballot_sync(0xffffffffu, id == e);
-        todo &= ~mine;
-        const T* f = static_cast<const T*>(a.f.p) + e * a.f.se;
-        const float scale = a.scale ? a.scale[e] : 1.f;
-        for (int j0 = 0; j0 < a.r; j0 += 32) {
-            float acc[2][4][4] = {};
-            const T* fr[4];
-#pragma unroll
-            for (int nb = 0; nb < 4; nb++) fr[nb] = f + (long long)min(j0 + nb * 8 + g, a.r - 1) * a.f.sj;
-const auto block = [&](auto load, int k) {
-                uint4 x[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = load(xr[i], k);
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++) b[nb] = load(fr[nb], k);
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        mma16<T>(acc[h][nb], x[2 * h].x, x[2 * h + 1].x, x[2 * h].y, x[2 * h + 1].y, b[nb].x, b[nb].y);
-                        mma16<T>(acc[h][nb], x[2 * h].z, x[2 * h + 1].z, x[2 * h].w, x[2 * h + 1].w, b[nb].z, b[nb].w);
-                    }
-            };
-            int k = (rank * 8 + warp) * 32;
-#pragma unroll 2
-            for (; k + 32 <= a.k; k += 256 * S) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
-            if (k < a.k) block([&](const T* row, int at) { return load16(row, at, a.k); }, k + 8 * t);
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int nb = 0; nb < 4; nb++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) red[warp][h * 16 + g + (c >> 1) * 8][nb * 8 + 2 * t + (c & 1)] = acc[h][nb][c];
-            __syncthreads();
-            for (int i = threadIdx.x; i < 1024; i += 256) {
-                float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < 8; w++) v += red[w][i >> 5][i & 31];
-                sum[i >> 5][i & 31] = v;
-            }
-            if (S > 1) cluster.sync();
-            else __syncthreads();
-            // each CTA finishes 32 / S of the rows
-            for (int i = threadIdx.x; i < 1024 / S; i += 256) {
-                const int row = rank * (32 / S) + (i >> 5), j = j0 + (i & 31);
-                if (mine >> row & 1 && j < rs) {
-                    float v = 0.f;
-                    for (int q = 0; q < S; q++) v += S > 1 ? *cluster.map_shared_rank(&sum[row][i & 31], q) : sum[row][i & 31];
-                    a.low[(m0 + row) * rs + j] = j < a.r ? low_value<T>(scale * v) : 0.f;
-                }
-            }
-            if (S > 1) cluster.sync();
-            else __syncthreads();
-        }
-    }
     if (both.after_pack == 1) grid_dependency_wait();
 }
 
@@ -465,8 +367,10 @@ __device__ __forceinline__ float dot_low(const float* low, const T* b, long long
 }
 
 // Few tokens: a cluster of S CTAs streams 16 MT rows of W once past NB * 8
-// tokens, its 8 S warps sharing the contraction in 32-wide blocks (operands
-// as in k_low_mma, W as the 16-row operand).  Bound: reading W, and with many
+// tokens, its 8 S warps sharing the contraction in 32-wide blocks.  Operands go
+// from global memory to the matrix instructions' registers: a thread's 16
+// bytes of a row are the k indexes of two instructions, in the same (permuted)
+// order for W and x.  Bound: reading W, and with many
 // tokens the re-reads of x, which MT = 2 halves; the stream starts before low
 // is there, and waits for it only to add the adapters' terms.
 template <class T, int NB, int MT>
@@ -549,13 +453,11 @@ __global__ void __launch_bounds__(256) k_project_small(const ProjectArgs a) {
 
 // ---------------------------------------------------------------- gradients of the factors
 
+
 constexpr int kGradChunk = 64;  // groups whose tokens are listed in shared memory at a time
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 template <class T, int RB>
@@ -573,9 +475,11 @@ struct GradTile {
 // the 16-row axis, tokens the contraction.  16-bit x is exact in TF32, and
 // low has been rounded to it; for f32 inputs both are split into two TF32
 // parts, which leaves 2^-22.  The partial sums of the cluster meet in shared
-// memory in a fixed order.  Bound: reading x once per 64 rank indexes.
+// memory in a fixed order.  Bound: reading x once per 64 rank indexes; the
+// copies' addresses were its instructions until a thread's column and its
+// part of a row were fixed for all groups.
 template <class T, int RB>
-__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int vec) {
+__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0) {
     using L = GradTile<T, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int own[kGradChunk * 32];
@@ -587,12 +491,20 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
     const int rs = low_stride(both.r);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int wf = warp & 3, wt = warp >> 2;
-    const T* x = static_cast<const T*>(a.x);
-    const uint32_t base = smem_u32(smem);
-    float acc[2][RB][4] = {};
-
     const int begin = both.first[e], tokens = both.first[e + 1] - begin;
     const int* list = both.list + begin;
+    float acc[2][RB][4] = {};
+
+    // this thread's part of every group: 16 bytes at one place of some rows
+    constexpr int C = 128 * (int)sizeof(T) / 16, kRows = 256 / C, kXParts = 32 / kRows;  // of x
+    constexpr int CU = RB * 2, kURows = 256 / CU < 32 ? 256 / CU : 32, kUParts = 32 / kURows;  // of low
+    const int xc = threadIdx.x % C, xrow = threadIdx.x / C, uc = threadIdx.x % CU, urow = threadIdx.x / CU;
+    const int xbytes = min(16, max(0, (a.k - k0) * (int)sizeof(T) - xc * 16)), ubytes = j0 + uc * 4 < rs && urow < 32 ? 16 : 0;
+    const char* xfrom = static_cast<const char*>(a.x) + (xbytes ? (size_t)k0 * sizeof(T) + xc * 16 : 0);
+    const char* ufrom = reinterpret_cast<const char*>(a.low) + (ubytes ? (size_t)j0 * 4 + uc * 16 : 0);
+    const long long xpitch = a.x_stride * (long long)sizeof(T);
+    const uint32_t base = smem_u32(smem), xto = base + xrow * L::kRow + xc * 16, uto = base + L::kX + urow * L::kURow * 4 + uc * 16;
+
     const int all = (tokens + 31) / 32, mine = all / S + (all % S > rank);  // groups of 32, and this CTA's
     for (int q0 = 0; q0 < mine; q0 += kGradChunk) {
         const int groups = min(kGradChunk, mine - q0);
@@ -601,43 +513,32 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, i
             own[i] = at < tokens ? list[at] : -1;
         }
         __syncthreads();
+        uint32_t put = 0, take = 0;  // stages' offsets
+        const auto next = [](uint32_t at) { return at + (L::kX + L::kU) == L::kSmem ? 0u : at + (L::kX + L::kU); };
         const auto fetch = [&](int q) {
             if (q < groups) {
-                const uint32_t sx = base + (q % L::kStages) * (L::kX + L::kU), su = sx + L::kX;
-                constexpr int V = 16 / sizeof(T), C = 128 / V;
-                if (sizeof(T) == 4 && !vec) {
-                    for (int i = threadIdx.x; i < 32 * 128; i += 256) {
-                        const int row = i >> 7, c = i & 127;
-                        const long long m = own[q * 32 + row];
-                        const bool in = m >= 0 && k0 + c < a.k;
-                        cp_async4(sx + row * L::kRow + c * 4, in ? x + m * a.x_stride + k0 + c : x, in ? 4 : 0);
-                    }
-                } else {
 #pragma unroll
-                    for (int i = threadIdx.x; i < 32 * C; i += 256) {
-                        const int row = i / C, c = i % C * V;
-                        const long long m = own[q * 32 + row];
-                        const int left = m >= 0 ? min(V, max(0, a.k - k0 - c)) : 0;
-                        cp_async16(sx + row * L::kRow + c * (int)sizeof(T), left ? x + m * a.x_stride + k0 + c : x, left * (int)sizeof(T));
-                    }
+                for (int i = 0; i < kXParts; i++) {
+                    const int m = own[q * 32 + xrow + i * kRows];
+                    cp_async16(xto + put + i * kRows * L::kRow, xfrom + max(m, 0) * xpitch, m >= 0 ? xbytes : 0);
                 }
+                if (urow < 32)
 #pragma unroll
-                for (int i = threadIdx.x; i < 32 * RB * 2; i += 256) {
-                    const int row = i / (RB * 2), c = i % (RB * 2) * 4;
-                    const long long m = own[q * 32 + row];
-                    const bool in = m >= 0 && j0 + c < rs;
-                    cp_async16(su + (row * L::kURow + c) * 4, in ? a.low + m * rs + j0 + c : a.low, in ? 16 : 0);
-                }
+                    for (int i = 0; i < kUParts; i++) {
+                        const int m = own[q * 32 + urow + i * kURows];
+                        cp_async16(uto + put + i * kURows * L::kURow * 4, ufrom + max(m, 0) * (long long)(rs * 4), m >= 0 ? ubytes : 0);
+                    }
             }
+            put = next(put);
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int q = 0; q < L::kStages - 1; q++) fetch(q);
-        for (int q = 0; q < groups; q++) {
+        for (int q = 0; q < groups; q++, take = next(take)) {
             asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
             __syncthreads();
             fetch(q + L::kStages - 1);
-            const uint8_t* sx = smem + (q % L::kStages) * (L::kX + L::kU);
+            const uint8_t* sx = smem + take;
             const float* su = reinterpret_cast<const float*>(sx + L::kX);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -729,21 +630,12 @@ int sm_count() {
 
 template <class T>
 cudaError_t low_launch(const LowArgs* a, int count, bool vec, int after_pack, cudaStream_t s) {
-    const LowPair both{{a[0], a[count - 1]}, after_pack};
     const long long n = a[0].n;
+    if (sizeof(T) == 2 && !low_by_token(n, a[0].k, a[count - 1].k, a[0].r))
+        return launch_low_tc(a, count, std::is_same<T, __half>::value ? DT_F16 : DT_BF16, after_pack, s);
+    const LowPair both{{a[0], a[count - 1]}, after_pack};
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     KScope ks("adapter_low", s);
-    if constexpr (sizeof(T) == 2) {
-        if (!low_by_token(n, a[0].k, a[count - 1].k, a[0].r)) {
-            // as many CTAs share a contraction as it takes to give every SM
-            // one, while each still has four blocks for a warp
-            const long long tiles = (n + 31) / 32;
-            int S = 1;
-            while (S < 8 && tiles * S * count < sm_count() && kmax / (S * 2) >= 512) S *= 2;
-            const dim3 grid((unsigned)(tiles * S), 1, count);
-            return after_pack ? launch_dependent(S, k_low_mma<T>, grid, 256, 0, s, both) : launch_cl(S, k_low_mma<T>, grid, 256, 0, s, both);
-        }
-    }
     // long contractions over more warps, to have more loads in flight
     const int rs = low_stride(a[0].r);
     const auto go = [&](auto kern, int ranks) {
@@ -777,26 +669,25 @@ cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
 }
 
 template <class T, int RB>
-cudaError_t grad_launch(const GradPair& a, long long n, bool vec, cudaStream_t s) {
+cudaError_t grad_launch(const GradPair& a, long long n, cudaStream_t s) {
     using L = GradTile<T, RB>;
     const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
-    // CTAs that share an adapter's tokens: until there are two for each SM,
-    // while each has two groups of tokens on average
+    // CTAs that share an adapter's tokens: until there are four for each SM,
+    // while each has four groups of tokens on average
     const long long ctas = (long long)(t0 + t1) * passes * a.adapters;
     int S = 1;
-    while (S < 8 && ctas * S < 2 * sm_count() && n / a.adapters >= 128 * S) S *= 2;
-    // own[] is beside it: raise the limit even where the tiles alone fit the default
-    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 16);
+    while (S < 8 && ctas * S < 4 * sm_count() && n / a.adapters >= 256 * S) S *= 2;
+    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 1024);  // own[] is beside the tiles
     if (e != cudaSuccess) return e;
     KScope ks("adapter_grad", s);
-    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.adapters), 256, L::kSmem, s, a, t0, (int)vec);
+    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.adapters), 256, L::kSmem, s, a, t0);
 }
 
 template <class T>
-cudaError_t grad_width(const GradPair& a, long long n, bool vec, cudaStream_t s) {
-    if (a.r <= 16) return grad_launch<T, 2>(a, n, vec, s);
-    if (a.r <= 32) return grad_launch<T, 4>(a, n, vec, s);
-    return grad_launch<T, 8>(a, n, vec, s);
+cudaError_t grad_width(const GradPair& a, long long n, cudaStream_t s) {
+    if (a.r <= 16) return grad_launch<T, 2>(a, n, s);
+    if (a.r <= 32) return grad_launch<T, 4>(a, n, s);
+    return grad_launch<T, 8>(a, n, s);
 }
 
 }  // namespace
@@ -832,8 +723,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
     return dtype == DT_BF16 ? small_width<__nv_bfloat16>(a, s) : small_width<__half>(a, s);
 }
 
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s) {
-    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, vec, s));
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, s));
 }
 
 }  // namespace tsg

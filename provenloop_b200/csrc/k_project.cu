@@ -704,6 +704,196 @@ cudaError_t launch_split(const ProjectArgs& p, int sms, cudaStream_t s) {
     return launch_dependent(a.split, kern, dim3((unsigned)(a.tiles_n * a.split), a.tiles_m), 256, smem, s, a, mx, mw);
 }
 
+// low of many tokens: a cluster of S CTAs shares the contraction of 128
+// tokens with the factors of the tile's distinct adapters, whose rank indexes,
+// 16 to a unit, lie side by side as the products' columns; a token keeps its
+// own adapter's.  Eight units at a time: a tile with more of them reads x
+// again.  Bound: reading x.
+struct LowTile {
+    static constexpr int kUnits = 8, kCols = 16 * kUnits;
+    static constexpr int kStages = 3;
+    static constexpr int kStage = 128 * 128 + kCols * 128;
+    static constexpr int kRow = kCols + 4;
+    static constexpr int kSmem = kStages * kStage + 1024;
+    static_assert(128 * kRow * 4 <= kStages * kStage, "the sums fit where the ring was");
+};
+
+struct LowMaps {
+    CUtensorMap x[2], f[2];
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid_constant__ LowMaps maps) {
+    using L = LowTile;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
+    __shared__ uint32_t tmem_at, dead;
+    __shared__ alignas(16) int ids[128];
+    __shared__ int list[128], pos[128], warp_new[4];
+    release_dependents();
+    const LowArgs& a = both.a[blockIdx.z];
+    const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
+    float* sums = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));  // [128][kRow], when the ring is done with
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = gridDim.y, rank = (int)cluster_rank();
+    const long long m0 = (long long)blockIdx.x * 128;
+    const int rs = low_stride(a.r), per = rs / 16, kblocks = (a.k + 63) / 64;
+    const int kb0 = kblocks * rank / S, kb1 = kblocks * (rank + 1) / S;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        mbar_init(&done, 1);
+        dead = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) tmem_alloc<1>(&tmem_at, L::kCols);
+    // the tile's adapters in the order of their first tokens
+    int first = 0, e = -1;
+    bool lead = false;
+    unsigned ball = 0;
+    if (warp < 4) {
+        e = m0 + threadIdx.x < a.n ? a.id.of(m0 + threadIdx.x) : -1;
+        ids[threadIdx.x] = e;
+        first = warp * 32 + __ffs(__match_any_sync(0xffffffffu, e)) - 1;
+    }
+    __syncthreads();
+    if (warp < 4) {
+        for (int j = warp * 8 - 1; j >= 0; j--) {
+            const int4 v = reinterpret_cast<const int4*>(ids)[j];
+            if (v.w == e) first = 4 * j + 3;
+            if (v.z == e) first = 4 * j + 2;
+            if (v.y == e) first = 4 * j + 1;
+            if (v.x == e) first = 4 * j;
+        }
+        lead = e >= 0 && first == (int)threadIdx.x;
+        ball = __ballot_sync(0xffffffffu, lead);
+        if (lane == 0) warp_new[warp] = __popc(ball);
+    }
+    __syncthreads();
+    int distinct = 0;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        if (q == warp && lead) {
+            const int at = distinct + __popc(ball & ((1u << lane) - 1));
+            list[at] = e;
+            pos[threadIdx.x] = at;
+        }
+        distinct += warp_new[q];
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int own = warp < 4 && e >= 0 ? pos[first] : -1;
+    const uint32_t tmem = tmem_at;
+    if (warp < 4) ids[threadIdx.x] = own;  // from here on: place in the list
+    if (both.after_pack == 2) grid_dependency_wait();
+    __syncthreads();
+
+    const int units = distinct * per;
+    Ring fill(L::kStages, 1), drain(L::kStages, 0);
+    uint32_t done_phase = 0;
+    for (int u0 = 0; u0 < units; u0 += L::kUnits, done_phase ^= 1) {
+        const int nu = min(L::kUnits, units - u0);
+        if (warp == 0) {
+            if (lane == 0)
+                for (int kb = kb0; kb < kb1; kb++, fill.next()) {
+                    if (!mbar_wait(&empty[fill.i], fill.phase, &dead)) break;
+                    const uint32_t s = ring + fill.i * L::kStage, bar = smem_u32(&full[fill.i]);
+                    mbar_expect(&full[fill.i], 16384 + nu * 2048);
+                    tma_2d<1>(s, &maps.x[blockIdx.z], kb * 64, (int)m0, bar);
+                    for (int u = 0; u < nu; u++)
+                        tma_3d<1>(s + 16384 + u * 2048, &maps.f[blockIdx.z], kb * 64, (u0 + u) % per * 16, list[(u0 + u) / per], bar);
+                }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+                const uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (uint32_t)(2 * nu) << 17 | 8u << 24;
+                for (int kb = kb0; kb < kb1; kb++, drain.next()) {
+                    if (!mbar_wait(&full[drain.i], drain.phase, &dead)) break;
+                    tc_fence_after();
+                    const uint32_t s = ring + drain.i * L::kStage;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) mma_f16<1>(tmem, desc_k128(s + k * 32), desc_k128(s + 16384 + k * 32), idesc, (kb - kb0) | k);
+                    mma_commit<1>(&empty[drain.i]);
+                }
+                mma_commit<1>(&done);
+            }
+        }
+        __syncwarp();
+        mbar_wait(&done, done_phase, &dead);
+        tc_fence_after();
+        const int row = (warp & 3) * 32 + lane;
+        for (int c = warp >> 2 << 5; c < nu * 16; c += 64) {
+            float v[32];
+            __syncwarp();
+            tmem_ld32(tmem + c + ((uint32_t)(warp & 3) << 21), v);
+            if (kb1 > kb0) {
+#pragma unroll
+                for (int q = 0; q < 32; q += 4)
+                    *reinterpret_cast<float4*>(sums + row * L::kRow + c + q) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(sums + row * L::kRow + c + q) = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+        tc_fence_before();
+        if (S > 1) cluster_sync_all();
+        else __syncthreads();
+        tc_fence_after();
+        // each CTA finishes 128 / S of the tokens, four rank indexes a thread
+        const int rows = 128 / S;
+        for (int i = threadIdx.x; i < rows * nu * 4; i += 256) {
+            const int r = rank * rows + i / (nu * 4), c = i % (nu * 4) * 4, u = u0 + c / 16;
+            if (ids[r] != u / per) continue;
+            const int at = list[u / per], j = u % per * 16 + c % 16;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < S; q++) {
+                const float* p = sums + r * L::kRow + c;
+                const float4 f = S > 1 ? ld_cluster4(map_rank(p, q)) : *reinterpret_cast<const float4*>(p);
+                v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+            }
+            const float scale = a.scale ? a.scale[at] : 1.f;
+            const auto put = [&](float f, int jj) { return jj < a.r ? __uint_as_float(to_tf32(scale * f)) : 0.f; };
+            *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + j) = make_float4(put(v.x, j), put(v.y, j + 1), put(v.z, j + 2), put(v.w, j + 3));
+        }
+        // the sums have been read before the ring's memory is filled again
+        fence_async_shared();
+        if (S > 1) cluster_sync_all();
+        else __syncthreads();
+    }
+    // tokens without an adapter
+    for (int i = rank * 256 + threadIdx.x; i < 128 * rs / 4; i += 256 * S) {
+        const int r = i / (rs / 4);
+        if (ids[r] < 0 && m0 + r < a.n) *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + i % (rs / 4) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (dead && threadIdx.x == 0) settle();
+    __syncthreads();
+    if (warp == 1) tmem_free<1>(tmem, L::kCols);
+    if (both.after_pack == 1) grid_dependency_wait();
+}
+
+template <class T>
+cudaError_t low_tc(const LowArgs* a, int count, int after_pack, int sms, cudaStream_t s) {
+    LowPair both{{a[0], a[count - 1]}, after_pack};
+    LowMaps maps{};
+    const CUtensorMapDataType ty = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < count; i++) {
+        cudaError_t e = tensor_map(&maps.x[i], ty, a[i].x, (uint64_t)a[i].k, (uint64_t)a[i].n, (uint64_t)a[i].x_stride * 2, 64, 128);
+        if (e == cudaSuccess)
+            e = tensor_map(&maps.f[i], ty, a[i].f.p, (uint64_t)a[i].k, (uint64_t)a[i].r, (uint64_t)a[i].f.sj * 2, 64, 16, (uint64_t)a[i].id.count);
+        if (e != cudaSuccess) return e;
+    }
+    // as many CTAs share a contraction as it takes to have two for each SM,
+    // while each has two slices
+    const long long tiles = (a[0].n + 127) / 128;
+    const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
+    int S = 1;
+    while (S < 8 && tiles * S * count < 2 * sms && kmax / 64 >= 4 * S) S *= 2;
+    const cudaError_t e = ensure_smem(k_low_tc<T>, LowTile::kSmem);
+    if (e != cudaSuccess) return e;
+    KScope ks("adapter_low", s);
+    return launch_split_y(S, after_pack != 0, k_low_tc<T>, dim3((unsigned)tiles, S, count), 256, LowTile::kSmem, s, both, maps);
+}
+
 template <class T, bool W_MN>
 cudaError_t launch_width(const ProjectArgs& p, int sms, cudaStream_t s) {
     if (!p.g32) {
@@ -745,6 +935,14 @@ cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p
 }
 
 cudaError_t expired_waits_project(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
+
+cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, int after_pack, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    return dtype == DT_BF16 ? low_tc<__nv_bfloat16>(a, count, after_pack, sms, s) : low_tc<__half>(a, count, after_pack, sms, s);
+}
 
 cudaError_t launch_project_tc(const ProjectArgs& p, int dtype, cudaStream_t s) {
     int dev = 0, sms = 0;

@@ -56,6 +56,11 @@ struct LowArgs {
     float* low;
 };
 
+struct LowPair {
+    LowArgs a[2];
+    int after_pack;  // launch_low
+};
+
 // out[m][o] = base[m][o] + sum_k x[m][k] W(o, k) + bias[o]
 //           + sum_j low[m][j] G[e][j][o], each term but the last optional.
 // W(o, k) is w[o][k], or w[k][o] where w_t is set (the backward call).
@@ -138,6 +143,8 @@ cudaError_t launch_pack(const PackJobs& a, cudaStream_t s);
 // was queued directly before, and its results are used here (2) or by the
 // next launch only (1), else 0
 cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int after_pack, cudaStream_t s);
+// 16-bit types, x and f on 16-byte boundaries, many tokens (k_project.cu)
+cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, int after_pack, cudaStream_t s);
 // f32, any strides
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s);
 // 16-bit types, at most kSmallTokens tokens; x and w (not transposed) on 16-byte boundaries
@@ -145,8 +152,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
 // 16-bit types; x and w rows on 16-byte boundaries (k_project.cu); a.g32 is
 // null where factor_by_token
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
-// rows of x on 16-byte boundaries, but for f32 (`vec`: they are)
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool vec, cudaStream_t s);
+// rows of x on 16-byte boundaries
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, cudaStream_t s);
 // waits of k_project.cu / k_rules.cu that ran out on the current device so far
 cudaError_t expired_waits_project(unsigned long long* out);
 cudaError_t expired_waits_rules(unsigned long long* out);

@@ -259,23 +259,41 @@ __device__ __forceinline__ uint4 ld_shared4(uint32_t at) {
 __device__ __forceinline__ void release_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+struct Launch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[2];
+    // cx x cy: cluster; dependent: programmatically dependent on the launch before
+    Launch(int cx, int cy, bool dependent, dim3 grid, unsigned block, size_t smem, cudaStream_t s) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(block, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = s;
+        cfg.attrs = at;
+        if (dependent) {
+            at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+        }
+        if (cx * cy > 1) {
+            at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+            at[cfg.numAttrs].val.clusterDim.x = (unsigned)cx;
+            at[cfg.numAttrs].val.clusterDim.y = (unsigned)cy;
+            at[cfg.numAttrs++].val.clusterDim.z = 1;
+        }
+    }
+};
+
 template <class... KArgs, class... Args>
 cudaError_t launch_dependent(int cluster, void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = (unsigned)cluster;
-    at[1].val.clusterDim.y = 1;
-    at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
+    const Launch l(cluster, 1, true, grid, block, smem, s);
+    return cudaLaunchKernelEx(&l.cfg, kern, args...);
+}
+
+// Clusters along y.
+template <class... KArgs, class... Args>
+cudaError_t launch_split_y(int cluster, bool dependent, void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t s,
+                           Args... args) {
+    const Launch l(1, cluster, dependent, grid, block, smem, s);
+    return cudaLaunchKernelEx(&l.cfg, kern, args...);
 }
 
 }  // namespace
