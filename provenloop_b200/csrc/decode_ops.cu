@@ -320,7 +320,7 @@ int adapter_project_backward(const ts_adapter_args* a) {
     if (e == cudaSuccess && a->grad_a) {
         const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}},
                          r, (int)a->adapters, first, first + a->adapters + 1};
-        e = launch_grads(g, n, a->dtype, w.s);
+        e = launch_grads(g, n, a->dtype, !p.f32 && a->out, w.s);
     }
     return cuda_status(e);
 }

@@ -157,51 +157,44 @@ __device__ __forceinline__ bool pack_f32(const PackJob& a, const uint16_t* src, 
 }
 
 // Adapter e's tokens in order, and the number of tokens of lower adapters:
-// each block looks through all indexes.
+// each block looks through all indexes, a warp through neighbouring ones.
 __device__ void pack_lists(const PackJob& a, int e) {
     __shared__ int warp_own[8], warp_less[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int* first = static_cast<int*>(a.dst);
     int* list = first + a.count + 1;
-    int less = 0, own = 0;  // tokens of lower adapters, of this one
-    const auto scan = [&](auto see) {
-        // 256 tokens in a step, each step taken by every thread
-        long long m = 0;
-        for (; m + 2048 <= a.rows; m += 2048) {
+    const long long each = (a.rows + 255) / 256 * 32, m0 = min(warp * each, a.rows), m1 = min(m0 + each, a.rows);
+    const auto scan = [&](auto see) {  // 32 tokens in a step, eight steps' loads together
+        long long m = m0;
+        for (; m + 256 <= m1; m += 256) {
             int id[8];
 #pragma unroll
-            for (int q = 0; q < 8; q++) id[q] = a.id.of(m + q * 256 + threadIdx.x);
+            for (int q = 0; q < 8; q++) id[q] = a.id.of(m + q * 32 + lane);
 #pragma unroll
-            for (int q = 0; q < 8; q++) see(id[q], m + q * 256 + threadIdx.x);
+            for (int q = 0; q < 8; q++) see(id[q], m + q * 32 + lane);
         }
-        for (; m < a.rows; m += 256) see(m + threadIdx.x < a.rows ? a.id.of(m + threadIdx.x) : -1, m + threadIdx.x);
+        for (; m < m1; m += 32) see(m + lane < m1 ? a.id.of(m + lane) : -1, m + lane);
     };
-    scan([&](int id, long long) { less += id >= 0 && id < e, own += id == e; });
-#pragma unroll
-    for (int q = 16; q; q >>= 1) less += __shfl_xor_sync(0xffffffffu, less, q), own += __shfl_xor_sync(0xffffffffu, own, q);
-    if (lane == 0) warp_less[warp] = less, warp_own[warp] = own;
+    int less = 0, own = 0;  // tokens of lower adapters, of this one
+    scan([&](int id, long long) {
+        less += __popc(__ballot_sync(0xffffffffu, id >= 0 && id < e));
+        own += __popc(__ballot_sync(0xffffffffu, id == e));
+    });
+    if (lane == 0) warp_own[warp] = own, warp_less[warp] = less;
     __syncthreads();
-    less = own = 0;
+    int at = 0, total = 0;
+    less = 0;
 #pragma unroll
-    for (int w = 0; w < 8; w++) less += warp_less[w], own += warp_own[w];
+    for (int w = 0; w < 8; w++) less += warp_less[w], at += w < warp ? warp_own[w] : 0, total += warp_own[w];
     if (threadIdx.x == 0) {
         first[e] = less;
-        if (e + 1 == a.count) first[a.count] = less + own;
+        if (e + 1 == a.count) first[a.count] = less + total;
     }
-    if (!own) return;
-    __syncthreads();
-    int at = less;
-    scan([&](int id, long long m) {
-        const bool mine = id == e;
-        const unsigned ball = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) warp_own[warp] = __popc(ball);
-        __syncthreads();
-        int before = 0, total = 0;
-#pragma unroll
-        for (int w = 0; w < 8; w++) before += w < warp ? warp_own[w] : 0, total += warp_own[w];
-        if (mine) list[at + before + __popc(ball & ((1u << lane) - 1))] = (int)m;
-        at += total;
-        __syncthreads();
+    at += less;
+    if (own) scan([&](int id, long long m) {
+        const unsigned ball = __ballot_sync(0xffffffffu, id == e);
+        if (id == e) list[at + __popc(ball & ((1u << lane) - 1))] = (int)m;
+        at += __popc(ball);
     });
 }
 
@@ -465,7 +458,7 @@ struct GradTile {
     static constexpr int kRow = sizeof(T) == 4 ? 136 * 4 : 288;  // 128 features; rows 8 banks apart
     static constexpr int kURow = RB * 8 + 8;                     // floats
     static constexpr int kX = 32 * kRow, kU = 32 * kURow * 4;
-    static constexpr int kStages = kX + kU > 16384 ? 4 : 6;
+    static constexpr int kStages = 4;
     static constexpr int kSmem = kStages * (kX + kU);
 };
 
@@ -479,7 +472,7 @@ struct GradTile {
 // copies' addresses were its instructions until a thread's column and its
 // part of a row were fixed for all groups.
 template <class T, int RB>
-__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0) {
+__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int dependent) {
     using L = GradTile<T, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int own[kGradChunk * 32];
@@ -491,7 +484,9 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0) {
     const int rs = low_stride(both.r);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int wf = warp & 3, wt = warp >> 2;
-    const int begin = both.first[e], tokens = both.first[e + 1] - begin;
+    // what is read here was complete before the launch before this one let it
+    // start (k_project.cu); that launch itself is waited for in the end
+    const int begin = __ldcg(both.first + e), tokens = __ldcg(both.first + e + 1) - begin;
     const int* list = both.list + begin;
     float acc[2][RB][4] = {};
 
@@ -510,7 +505,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0) {
         const int groups = min(kGradChunk, mine - q0);
         for (int i = threadIdx.x; i < groups * 32; i += 256) {
             const int at = ((q0 + (i >> 5)) * S + rank) * 32 + (i & 31);
-            own[i] = at < tokens ? list[at] : -1;
+            own[i] = at < tokens ? __ldcg(list + at) : -1;
         }
         __syncthreads();
         uint32_t put = 0, take = 0;  // stages' offsets
@@ -620,6 +615,7 @@ __global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0) {
             static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(v);
     }
     if (S > 1) cluster.sync();
+    if (dependent) grid_dependency_wait();
 }
 
 int sm_count() {
@@ -669,7 +665,7 @@ cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
 }
 
 template <class T, int RB>
-cudaError_t grad_launch(const GradPair& a, long long n, cudaStream_t s) {
+cudaError_t grad_launch(const GradPair& a, long long n, bool dependent, cudaStream_t s) {
     using L = GradTile<T, RB>;
     const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
     // CTAs that share an adapter's tokens: until there are four for each SM,
@@ -680,14 +676,15 @@ cudaError_t grad_launch(const GradPair& a, long long n, cudaStream_t s) {
     const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 1024);  // own[] is beside the tiles
     if (e != cudaSuccess) return e;
     KScope ks("adapter_grad", s);
-    return launch_cl(S, k_grad<T, RB>, dim3((unsigned)((t0 + t1) * S), passes, a.adapters), 256, L::kSmem, s, a, t0);
+    const dim3 grid((unsigned)((t0 + t1) * S), passes, a.adapters);
+    return dependent ? launch_dependent(S, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, 1) : launch_cl(S, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, 0);
 }
 
 template <class T>
-cudaError_t grad_width(const GradPair& a, long long n, cudaStream_t s) {
-    if (a.r <= 16) return grad_launch<T, 2>(a, n, s);
-    if (a.r <= 32) return grad_launch<T, 4>(a, n, s);
-    return grad_launch<T, 8>(a, n, s);
+cudaError_t grad_width(const GradPair& a, long long n, bool dependent, cudaStream_t s) {
+    if (a.r <= 16) return grad_launch<T, 2>(a, n, dependent, s);
+    if (a.r <= 32) return grad_launch<T, 4>(a, n, dependent, s);
+    return grad_launch<T, 8>(a, n, dependent, s);
 }
 
 }  // namespace
@@ -723,8 +720,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
     return dtype == DT_BF16 ? small_width<__nv_bfloat16>(a, s) : small_width<__half>(a, s);
 }
 
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, cudaStream_t s) {
-    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, s));
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, dependent, s));
 }
 
 }  // namespace tsg

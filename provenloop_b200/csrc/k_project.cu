@@ -26,6 +26,7 @@
 // A zero times an adapter's NaN or infinity would spread to the other
 // tokens of the tile: k_pack replaces such elements by 0 and flags them, and
 // the epilogue adds their terms to the adapter's own tokens only.
+#include <climits>
 #include <cuda.h>
 
 #include "launch.cuh"
@@ -58,14 +59,54 @@ struct TcArgs {
     int tma_out;          // out, and base if there is one, take TMA boxes
 };
 
+// The distinct adapters of a tile of up to 256 tokens, in the order of their
+// first tokens.
+struct TileAdapters {
+    alignas(16) uint32_t next[2][4];
+    int list[256];
+};
+
+// `e`: the adapters of this thread's tokens i, i + 128, ... (four warps, w this
+// one).  Returns the number of distinct ones; place: each token's in the list
+// (complete after the caller's next barrier), -1 without an adapter.  One
+// round for each: few, mostly, and code that runs once a tile is paid by
+// the instruction.
+template <int W>
+__device__ __forceinline__ int tile_adapters(TileAdapters& s, int w, const int (&e)[W], int (&place)[W]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < W; h++) place[h] = -1;
+#pragma unroll 1
+    for (int d = 0;; d++) {
+        // the first token without a place: its number and adapter
+        uint32_t key = UINT_MAX;
+#pragma unroll
+        for (int h = W - 1; h >= 0; h--) {
+            const unsigned left = __ballot_sync(0xffffffffu, place[h] < 0 && e[h] >= 0);
+            const int at = left ? __ffs(left) - 1 : 0;
+            const int first = __shfl_sync(0xffffffffu, e[h], at);
+            if (left) key = (uint32_t)(h * 128 + w * 32 + at) << 16 | (uint32_t)first;
+        }
+        if (lane == 0) s.next[d & 1][w] = key;
+        bar_sync(1, 128);
+        const uint4 all = *reinterpret_cast<const uint4*>(s.next[d & 1]);
+        key = min(min(all.x, all.y), min(all.z, all.w));
+        if (key == UINT_MAX) return d;
+        const int found = (int)(key & 0xffffu);
+#pragma unroll
+        for (int h = 0; h < W; h++)
+            if (e[h] == found) place[h] = d;
+        if (w == 0 && lane == 0) s.list[d] = found;
+    }
+}
+
 // Everything beside the operand rings.
 struct Shared {
     uint64_t full[8], empty[8], xfull[4], xempty[4], acc_full[2], acc_empty[2], drained, base_full[8][2];
     uint32_t tmem, dead;
-    uint32_t xlast[4];
     uint32_t bad[8];  // by tile: an element of a factor is not finite
-    alignas(16) int ids[256];
-    int list[256], pos[256], warp_new[8];
+    uint32_t steps[4];  // by tile: low-rank steps
+    TileAdapters adapters;
 };
 
 template <class T>
@@ -157,38 +198,58 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             constexpr uint32_t xdesc = shape | 2u << 7 | 2u << 10;
             Ring r(L::kStages, 0), x(L::kXBufs, 0), acc(2, 1);
             uint32_t drain_phase = 0;
-            for (int t = blockIdx.x / CG; t < tiles; t += step, acc.next()) {
+            // The two kinds of instruction are ordered by waiting: a few hundred
+            // of some ten thousand cycles.
+            const auto drained = [&] {
+                mma_commit<CG>(&sh.drained);
+                const bool ok = mbar_wait(&sh.drained, drain_phase, &sh.dead);
+                drain_phase ^= 1;
+                return ok;
+            };
+            int serial = 0;
+            for (int t = blockIdx.x / CG; t < tiles; t += step, acc.next(), serial++) {
                 if (!mbar_wait(&sh.acc_empty[acc.i], acc.phase, &sh.dead)) goto mma_done;
                 tc_fence_after();
                 const uint32_t d = tmem + acc.i * BN;
+                uint32_t add = 0;
+                int steps = 1, at = 0;
+                const auto low_step = [&] {
+                    if (!mbar_wait(&sh.xfull[x.i], x.phase, &sh.dead)) return false;
+                    tc_fence_after();
+                    if (at++ == 0) steps = *reinterpret_cast<volatile uint32_t*>(&sh.steps[serial & 3]);
+                    const uint32_t s = xring + x.i * L::kXStage;
+#pragma unroll
+                    for (int k = 0; k < kXK / 8; k++, add = 1)
+                        mma_tf32<CG>(d, desc_k64(s + k * 32), desc_k64(s + 128 * kXK * 4 + k * 32), xdesc, add);
+                    mma_commit<CG>(&sh.xempty[x.i]);
+                    x.next();
+                    return true;
+                };
+                // Two low-rank steps, which were filled during the tile before, come
+                // first, but for the first tile, whose low may still be computed;
+                // the rest, filled in the meantime, after the shared projection.
+                // The order of the sums goes by sizes and indexes alone.
+                if (serial && a.kblocks) {
+                    while (at < steps && at < 2)
+                        if (!low_step()) goto mma_done;
+                    if (!drained()) goto mma_done;
+                }
                 for (int kb = 0; kb < a.kblocks; kb++, r.next()) {
                     if (!mbar_wait(&sh.full[r.i], r.phase, &sh.dead)) goto mma_done;
                     tc_fence_after();
                     const uint32_t s = ring + r.i * L::kStage;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
+                    for (int k = 0; k < 4; k++, add = 1) {
                         const uint64_t da = desc_k128(s + k * 32);
                         const uint64_t db = W_MN ? desc_mn128(s + 16384 + k * 2048, 8192) : desc_k128(s + 16384 + k * 32);
-                        mma_f16<CG>(d, da, db, idesc, kb | k);
+                        mma_f16<CG>(d, da, db, idesc, add);
                     }
                     mma_commit<CG>(&sh.empty[r.i]);
                 }
-                if (a.kblocks) {
-                    // the two kinds of instruction are ordered by waiting: once
-                    // per tile, a few hundred of some ten thousand cycles
-                    mma_commit<CG>(&sh.drained);
-                    if (!mbar_wait(&sh.drained, drain_phase, &sh.dead)) goto mma_done;
-                    drain_phase ^= 1;
-                }
-                for (bool first = a.kblocks == 0, last = false; !last; first = false, x.next()) {
-                    if (!mbar_wait(&sh.xfull[x.i], x.phase, &sh.dead)) goto mma_done;
-                    tc_fence_after();
-                    last = *reinterpret_cast<volatile uint32_t*>(&sh.xlast[x.i]);
-                    const uint32_t s = xring + x.i * L::kXStage;
-#pragma unroll
-                    for (int k = 0; k < kXK / 8; k++)
-                        mma_tf32<CG>(d, desc_k64(s + k * 32), desc_k64(s + 128 * kXK * 4 + k * 32), xdesc, !first || k);
-                    mma_commit<CG>(&sh.xempty[x.i]);
+                if (at < steps) {
+                    if (a.kblocks && !drained()) goto mma_done;
+                    while (at < steps)
+                        if (!low_step()) goto mma_done;
                 }
                 mma_commit<CG>(&sh.acc_full[acc.i]);
             }
@@ -201,70 +262,45 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
         const int i = threadIdx.x - 256, w = warp - 8;
         const int rs = low_stride(p.r), blocks = (p.o + 127) / 128;
         grid_dependency_wait();  // low and the converted factors are written by the launches before
+        release_dependents();    // what the next launch (the gradients) reads is there
+        const auto load_ids = [&](int t, int (&e)[CG]) {
+#pragma unroll
+            for (int h = 0; h < CG; h++) {
+                const long long m = ((long long)(t % a.tiles_m) * CG + h) * 128 + i;
+                e[h] = t < tiles && m < p.n ? p.id.of(m) : -1;
+            }
+        };
         Ring x(L::kXBufs, 1);
-        int serial = 0;
+        int serial = 0, e[CG];
+        load_ids(blockIdx.x / CG, e);
         for (int t = blockIdx.x / CG; t < tiles; t += step, serial++) {
             const long long m0 = (long long)(t % a.tiles_m) * 128 * CG, m = m0 + rank * 128 + i;
             const int o0 = t / a.tiles_m * BN + (int)rank * L::kRows;
-            int e[CG], first[CG];
-            bool lead[CG];
-            unsigned ball[CG];
-#pragma unroll
-            for (int h = 0; h < CG; h++) {
-                e[h] = m0 + h * 128 + i < p.n ? p.id.of(m0 + h * 128 + i) : -1;
-                sh.ids[h * 128 + i] = e[h];
-            }
+            int pos[CG];
             if (i == 0) sh.bad[serial & 7] = 0;  // the epilogue is less than eight tiles behind
-            bar_sync(1, 128);
-#pragma unroll
-            for (int h = 0; h < CG; h++) {
-                // the first token with the same adapter
-                first[h] = h * 128 + (w << 5) + __ffs(__match_any_sync(0xffffffffu, e[h])) - 1;
-#pragma unroll 4
-                for (int j = h * 32 + w * 8 - 1; j >= 0; j--) {
-                    const int4 v = reinterpret_cast<const int4*>(sh.ids)[j];
-                    if (v.w == e[h]) first[h] = 4 * j + 3;
-                    if (v.z == e[h]) first[h] = 4 * j + 2;
-                    if (v.y == e[h]) first[h] = 4 * j + 1;
-                    if (v.x == e[h]) first[h] = 4 * j;
-                }
-                lead[h] = e[h] >= 0 && first[h] == h * 128 + i;
-                ball[h] = __ballot_sync(0xffffffffu, lead[h]);
-                if (lane == 0) sh.warp_new[h * 4 + w] = __popc(ball[h]);
-            }
-            bar_sync(1, 128);
-            int distinct = 0;
-#pragma unroll
-            for (int h = 0; h < CG; h++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (q == w && lead[h]) {
-                        const int at = distinct + __popc(ball[h] & ((1u << lane) - 1));
-                        sh.list[at] = e[h];
-                        sh.pos[h * 128 + i] = at;
-                    }
-                    distinct += sh.warp_new[h * 4 + q];
-                }
-            bar_sync(1, 128);
-            const int mine = CG == 2 && rank ? e[CG - 1] : e[0], mine_first = CG == 2 && rank ? first[CG - 1] : first[0];
-            const int own = mine >= 0 ? sh.pos[mine_first] : -1;  // this row's adapter in the list
+            const int distinct = tile_adapters(sh.adapters, w, e, pos);
+            const int own = CG == 2 && rank ? pos[CG - 1] : pos[0];
+            // the next tile's
+            load_ids(t + step, e);
             const float4* low = reinterpret_cast<const float4*>(p.low + (m < p.n ? m : 0) * rs);
-            // the factor's flags for the tile's outputs
+            // the factor's flags for the tile's outputs; the first of them are looked at with low
             const int tile_o = t / a.tiles_m * BN, per = rs / kXK, flags = min((BN + 127) / 128, blocks - tile_o / 128) * per;
-            for (int d = i; d < distinct * flags; d += 128)
-                if (p.bad[((long long)sh.list[d / flags] * blocks + tile_o / 128) * per + d % flags]) sh.bad[serial & 7] = 1;
+            const auto flag = [&](int d) { return p.bad[((long long)sh.adapters.list[d / flags] * blocks + tile_o / 128) * per + d % flags]; };
+            uint32_t bad = i < distinct * flags ? flag(i) : 0u;
+            for (int d = i + 128; d < distinct * flags; d += 128) bad |= flag(d);
             const int steps = max(1, distinct);
+            if (i == 0) sh.steps[serial & 3] = steps * per;
             for (int j = 0; j < rs; j += kXK) {
                 float4 f[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) f[q] = low[j / 4 + q];
+                if (bad) sh.bad[serial & 7] = 1;
                 for (int d = 0; d < steps; d++, x.next()) {
                     const bool late = !mbar_wait(&sh.xempty[x.i], x.phase, &sh.dead);
                     const uint32_t s = xring + x.i * L::kXStage;
                     if (i == 0) {
                         const uint32_t bar = CG == 2 ? map_rank(&sh.xfull[x.i], 0) : smem_u32(&sh.xfull[x.i]);
-                        tma_3d<CG>(s + 128 * kXK * 4, &mg, j, o0, distinct ? sh.list[d] : 0, bar);
-                        sh.xlast[x.i] = j + kXK >= rs && d + 1 == steps;
+                        tma_3d<CG>(s + 128 * kXK * 4, &mg, j, o0, distinct ? sh.adapters.list[d] : 0, bar);
                     }
                     const bool in = d == own;
 #pragma unroll
@@ -620,6 +656,7 @@ k_project_split(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __
     if (S > 1) cluster_sync_all();
     else __syncthreads();
     grid_dependency_wait();  // low is written by the launch before this one
+    release_dependents();
     const int per = BN / S, rs = low_stride(p.r);
     for (int i = threadIdx.x; i < 128 * (per / 8); i += 256) {
         const int row = i & 127, col = rank * per + (i >> 7) * 8, o = o0 + col;
@@ -728,8 +765,8 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[L::kStages], empty[L::kStages], done;
     __shared__ uint32_t tmem_at, dead;
-    __shared__ alignas(16) int ids[128];
-    __shared__ int list[128], pos[128], warp_new[4];
+    __shared__ TileAdapters adapters;
+    __shared__ int place[128], found;  // each token's place in the list, its length
     release_dependents();
     const LowArgs& a = both.a[blockIdx.z];
     const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
@@ -746,47 +783,20 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
         mbar_init_fence();
     }
     if (warp == 1) tmem_alloc<1>(&tmem_at, L::kCols);
-    // the tile's adapters in the order of their first tokens
-    int first = 0, e = -1;
-    bool lead = false;
-    unsigned ball = 0;
+    int e[1] = {-1}, own[1] = {-1}, distinct = 0;
     if (warp < 4) {
-        e = m0 + threadIdx.x < a.n ? a.id.of(m0 + threadIdx.x) : -1;
-        ids[threadIdx.x] = e;
-        first = warp * 32 + __ffs(__match_any_sync(0xffffffffu, e)) - 1;
-    }
-    __syncthreads();
-    if (warp < 4) {
-        for (int j = warp * 8 - 1; j >= 0; j--) {
-            const int4 v = reinterpret_cast<const int4*>(ids)[j];
-            if (v.w == e) first = 4 * j + 3;
-            if (v.z == e) first = 4 * j + 2;
-            if (v.y == e) first = 4 * j + 1;
-            if (v.x == e) first = 4 * j;
-        }
-        lead = e >= 0 && first == (int)threadIdx.x;
-        ball = __ballot_sync(0xffffffffu, lead);
-        if (lane == 0) warp_new[warp] = __popc(ball);
-    }
-    __syncthreads();
-    int distinct = 0;
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        if (q == warp && lead) {
-            const int at = distinct + __popc(ball & ((1u << lane) - 1));
-            list[at] = e;
-            pos[threadIdx.x] = at;
-        }
-        distinct += warp_new[q];
+        if (m0 + threadIdx.x < a.n) e[0] = a.id.of(m0 + threadIdx.x);
+        distinct = tile_adapters(adapters, warp, e, own);
+        place[threadIdx.x] = own[0];
+        if (threadIdx.x == 0) found = distinct;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int own = warp < 4 && e >= 0 ? pos[first] : -1;
+    distinct = found;
     const uint32_t tmem = tmem_at;
-    if (warp < 4) ids[threadIdx.x] = own;  // from here on: place in the list
+    const int* list = adapters.list;
     if (both.after_pack == 2) grid_dependency_wait();
-    __syncthreads();
 
     const int units = distinct * per;
     Ring fill(L::kStages, 1), drain(L::kStages, 0);
@@ -843,7 +853,7 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
         const int rows = 128 / S;
         for (int i = threadIdx.x; i < rows * nu * 4; i += 256) {
             const int r = rank * rows + i / (nu * 4), c = i % (nu * 4) * 4, u = u0 + c / 16;
-            if (ids[r] != u / per) continue;
+            if (place[r] != u / per) continue;
             const int at = list[u / per], j = u % per * 16 + c % 16;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int q = 0; q < S; q++) {
@@ -863,7 +873,7 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
     // tokens without an adapter
     for (int i = rank * 256 + threadIdx.x; i < 128 * rs / 4; i += 256 * S) {
         const int r = i / (rs / 4);
-        if (ids[r] < 0 && m0 + r < a.n) *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + i % (rs / 4) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (place[r] < 0 && m0 + r < a.n) *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + i % (rs / 4) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (dead && threadIdx.x == 0) settle();
     __syncthreads();
@@ -882,12 +892,12 @@ cudaError_t low_tc(const LowArgs* a, int count, int after_pack, int sms, cudaStr
             e = tensor_map(&maps.f[i], ty, a[i].f.p, (uint64_t)a[i].k, (uint64_t)a[i].r, (uint64_t)a[i].f.sj * 2, 64, 16, (uint64_t)a[i].id.count);
         if (e != cudaSuccess) return e;
     }
-    // as many CTAs share a contraction as it takes to have two for each SM,
+    // as many CTAs share a contraction as still run together, two on each SM,
     // while each has two slices
     const long long tiles = (a[0].n + 127) / 128;
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     int S = 1;
-    while (S < 8 && tiles * S * count < 2 * sms && kmax / 64 >= 4 * S) S *= 2;
+    while (S < 8 && tiles * S * count <= sms && kmax / 64 >= 4 * S) S *= 2;
     const cudaError_t e = ensure_smem(k_low_tc<T>, LowTile::kSmem);
     if (e != cudaSuccess) return e;
     KScope ks("adapter_low", s);

@@ -152,8 +152,9 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
 // 16-bit types; x and w rows on 16-byte boundaries (k_project.cu); a.g32 is
 // null where factor_by_token
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
-// rows of x on 16-byte boundaries
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, cudaStream_t s);
+// rows of x on 16-byte boundaries; `dependent`: launch_project_tc was queued
+// directly before, and behind it what is read here
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, cudaStream_t s);
 // waits of k_project.cu / k_rules.cu that ran out on the current device so far
 cudaError_t expired_waits_project(unsigned long long* out);
 cudaError_t expired_waits_rules(unsigned long long* out);
