@@ -126,32 +126,50 @@ __device__ __forceinline__ void pack_tile(const PackJob& a, const uint16_t* src,
         if (j0 + i < a.rows && k0 + tx < a.dst_cols) dst[(j0 + i) * a.dst_cols + k0 + tx] = tile[i][tx];
 }
 
-// 128 rows x 16 columns of a factor as f32.
+// 128 rows x 16 columns of a factor as f32; returns whether an element is not
+// finite.  A thread takes 8 neighbours along whichever axis of src is
+// contiguous, in one load where they are on a 16-byte boundary.
 __device__ __forceinline__ bool pack_f32(const PackJob& a, const uint16_t* src, float* dst, long long j0, int k0, int dtype) {
     __shared__ float tile[128][17];
+    const bool along = a.sk == 1;  // k is the contiguous axis
+    const int j = along ? threadIdx.x >> 1 : (threadIdx.x & 15) * 8, k = along ? (threadIdx.x & 1) * 8 : threadIdx.x >> 4;
+    const long long jj = j0 + j;
+    const int kk = k0 + k, left = along ? (jj < a.rows ? a.cols - kk : 0) : (kk < a.cols ? (int)min(8ll, a.rows - jj) : 0);
+    const uint16_t* from = src + (left > 0 ? jj * a.sj + kk * a.sk : 0);
     uint16_t v[8];
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+        const uint4 u = *reinterpret_cast<const uint4*>(from);
+        memcpy(v, &u, 16);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int q = threadIdx.x + 256 * i;
-        const long long j = min(j0 + (a.sk == 1 ? q >> 4 : q & 127), a.rows - 1);
-        const int k = min(k0 + (a.sk == 1 ? q & 15 : q >> 7), a.cols - 1);
-        v[i] = src[j * a.sj + k * a.sk];
+        for (int i = 0; i < 8; i++) v[i] = from[i < left ? i : 0];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= left) v[i] = 0;
     }
     bool bad = false;
+    float f[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const int q = threadIdx.x + 256 * i;
-        const int j = a.sk == 1 ? q >> 4 : q & 127, k = a.sk == 1 ? q & 15 : q >> 7;
-        const float f = dtype == DT_BF16 ? __uint_as_float((uint32_t)v[i] << 16) : __half2float(__ushort_as_half(v[i]));
-        const bool in = j0 + j < a.rows && k0 + k < a.cols, ok = (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
-        bad |= in && !ok;
-        tile[j][k] = in && ok ? f : 0.f;
+        f[i] = dtype == DT_BF16 ? __uint_as_float((uint32_t)v[i] << 16) : __half2float(__ushort_as_half(v[i]));
+        if ((__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u) f[i] = 0.f, bad = true;
     }
-    __syncthreads();
+    if (along) {
+        if (jj < a.rows) {
+            float4* to = reinterpret_cast<float4*>(dst + jj * a.dst_cols + kk);
+            to[0] = make_float4(f[0], f[1], f[2], f[3]), to[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int q = threadIdx.x + 256 * i;
-        if (j0 + (q >> 4) < a.rows) dst[(j0 + (q >> 4)) * a.dst_cols + k0 + (q & 15)] = tile[q >> 4][q & 15];
+        for (int i = 0; i < 8; i++) tile[j + i][k] = f[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int row = (threadIdx.x >> 2) + 64 * i, col = (threadIdx.x & 3) * 4;
+            if (j0 + row < a.rows)
+                *reinterpret_cast<float4*>(dst + (j0 + row) * a.dst_cols + k0 + col) =
+                    make_float4(tile[row][col], tile[row][col + 1], tile[row][col + 2], tile[row][col + 3]);
+        }
     }
     return bad;
 }

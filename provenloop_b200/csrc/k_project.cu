@@ -13,12 +13,13 @@
 // the 48 KiB that a 128 x 256 tile of its own would need.  What bounds large
 // n is these slices' way from L2 more than the tensor cores.
 //
-// The low-rank term is a few more steps of the same contraction, 16 rank
-// indexes of one adapter at a time, for each distinct adapter of the tile:
-// four builder warps write the tokens' rows of low, zero for other
-// adapters' tokens, and TMA brings the factor's rows, both as TF32.  So a tile
-// whose tokens share an adapter (prefill, training) pays r / 16 steps and a
-// mixed one D r / 16 for D distinct adapters, without sorting tokens or a
+// The low-rank term is a few more slices of the same contraction, behind the
+// shared ones in the same ring: units of 16 rank indexes of one adapter, two
+// to a slice, for each distinct adapter of the tile.  Four builder warps write
+// the tokens' rows of low, zero for other adapters' tokens, and TMA brings
+// the factor's rows, both as TF32.  So a tile whose tokens share an adapter
+// (prefill, training) pays r / 16 units and a mixed one D r / 16 for D distinct
+// adapters, without sorting tokens or a
 // second pass over out.  TF32 holds bf16 and fp16 factors exactly and low to
 // 11 significant bits with the range of f32, so that an fp16 low above
 // 65504 does not overflow.  The factors are converted once per call (k_pack).
@@ -38,17 +39,16 @@ namespace tsg {
 namespace {
 
 constexpr int kThreads = 448;  // warps 0-7 epilogue, 8-11 builders, 12 TMA, 13 matrix instructions
-constexpr int kXK = 16;        // rank indexes per step
+constexpr int kXK = 16;        // rank indexes per unit
 
 template <int CG, int BN>
 struct Tile {
     static constexpr int kRows = BN / CG;                       // of W or the factor in a CTA
     static constexpr int kStage = 128 * 128 + kRows * 128;      // bytes: 64 16-bit elements of each row
-    static constexpr int kXStage = (128 + kRows) * kXK * 4;     // TF32 operands
-    static constexpr int kXBufs = 3;
-    static constexpr int kStages = 4;
+    static constexpr int kUnit = kStage / 2;                    // kXK TF32 values of each row
+    static constexpr int kStages = 6;
     static constexpr int kOut = 8 * 2 * 2048;                   // per epilogue warp two boxes of 32 rows x 32 outputs
-    static constexpr int kSmem = kStages * kStage + kXBufs * kXStage + kOut + 1024 /* alignment */;
+    static constexpr int kSmem = kStages * kStage + kOut + 1024 /* alignment */;
 };
 
 struct TcArgs {
@@ -102,10 +102,10 @@ __device__ __forceinline__ int tile_adapters(TileAdapters& s, int w, const int (
 
 // Everything beside the operand rings.
 struct Shared {
-    uint64_t full[8], empty[8], xfull[4], xempty[4], acc_full[2], acc_empty[2], drained, base_full[8][2];
+    uint64_t full[8], empty[8], counted[8], turn[2], acc_full[2], acc_empty[2], drained, base_full[8][2];
     uint32_t tmem, dead;
-    uint32_t bad[8];  // by tile: an element of a factor is not finite
-    uint32_t steps[4];  // by tile: low-rank steps
+    uint32_t bad[16]; // by tile: an element of a factor is not finite
+    int units[8];     // by tile: low-rank units, there when counted
     TileAdapters adapters;
 };
 
@@ -145,19 +145,19 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
     const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t xring = ring + L::kStages * L::kStage;
-    const uint32_t out_boxes = xring + L::kXBufs * L::kXStage;
+    const uint32_t out_boxes = ring + L::kStages * L::kStage;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ProjectArgs& p = a.p;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
-        for (int i = 0; i < L::kXBufs; i++) mbar_init(&sh.xfull[i], CG), mbar_init(&sh.xempty[i], 1);
-        for (int i = 0; i < 2; i++) mbar_init(&sh.acc_full[i], 1), mbar_init(&sh.acc_empty[i], 256 * CG);
+        for (int i = 0; i < L::kStages; i++) mbar_init(&sh.full[i], CG), mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < 8; i++) mbar_init(&sh.counted[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&sh.turn[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&sh.acc_full[i], 1), mbar_init(&sh.acc_empty[i], 8 * CG);
         mbar_init(&sh.drained, 1);
         for (int i = 0; i < 16; i++) mbar_init(&sh.base_full[i >> 1][i & 1], 1);
         sh.dead = 0;
-        for (int i = 0; i < 8; i++) sh.bad[i] = 0;
+        for (int i = 0; i < 16; i++) sh.bad[i] = 0;
         mbar_init_fence();
     }
     if (warp == 13) tmem_alloc<CG>(&sh.tmem, 2 * BN);
@@ -168,17 +168,26 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
     const uint32_t tmem = sh.tmem;
     const int tiles = a.tiles_m * a.tiles_n, step = gridDim.x / CG;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;  // rank 0 issues the pair's instructions
+    // The TMA warp and the builders fill the ring in turns, tile by tile: a
+    // barrier's parity tells a slice's use from the one before only to whom
+    // comes next.  turn[0]: the shared slices of a tile have their places, the
+    // builders may go on; turn[1]: so have the builders' (half as many as the
+    // tile has units).  counted: the units of a tile are known; the ring is
+    // less than eight tiles long.
+    const bool shared_part = a.kblocks > 0;
 
     if (warp == 12) {
         if (lane == 0) {
             Ring r(L::kStages, 1);
-            for (int t = blockIdx.x / CG; t < tiles; t += step) {
+            int serial = 0;
+            for (int t = blockIdx.x / CG; t < tiles && shared_part; t += step, serial++) {
                 const int m0 = (t % a.tiles_m * CG + (int)rank) * 128, o0 = t / a.tiles_m * BN + (int)rank * L::kRows;
                 for (int kb = 0; kb < a.kblocks; kb++, r.next()) {
                     if (!mbar_wait(&sh.empty[r.i], r.phase, &sh.dead)) goto tma_done;
                     const uint32_t s = ring + r.i * L::kStage;
                     const uint32_t bar = CG == 2 ? map_rank(&sh.full[r.i], 0) : smem_u32(&sh.full[r.i]);
                     if (rank == 0) mbar_expect(&sh.full[r.i], CG * L::kStage);
+                    else mbar_arrive_relaxed_at(bar);
                     tma_2d<CG>(s, &mx, kb * 64, m0, bar);
                     if constexpr (W_MN) {
 #pragma unroll
@@ -187,6 +196,9 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                         tma_2d<CG>(s + 16384, &mw, kb * 64, o0, bar);
                     }
                 }
+                mbar_arrive(&sh.turn[0]);
+                if (!mbar_wait(&sh.turn[1], serial & 1, &sh.dead)) break;
+                r.skip((*reinterpret_cast<volatile int*>(&sh.units[serial & 7]) + 1) / 2);
             }
         tma_done:;
         }
@@ -196,44 +208,14 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             constexpr uint32_t shape = 1u << 4 | (uint32_t)(BN >> 3) << 17 | (128u * CG >> 4) << 24;
             constexpr uint32_t idesc = shape | fmt << 7 | fmt << 10 | (W_MN ? 1u << 16 : 0u);
             constexpr uint32_t xdesc = shape | 2u << 7 | 2u << 10;
-            Ring r(L::kStages, 0), x(L::kXBufs, 0), acc(2, 1);
+            Ring r(L::kStages, 0), acc(2, 1);
             uint32_t drain_phase = 0;
-            // The two kinds of instruction are ordered by waiting: a few hundred
-            // of some ten thousand cycles.
-            const auto drained = [&] {
-                mma_commit<CG>(&sh.drained);
-                const bool ok = mbar_wait(&sh.drained, drain_phase, &sh.dead);
-                drain_phase ^= 1;
-                return ok;
-            };
-            int serial = 0;
+            int serial = 0, units;
             for (int t = blockIdx.x / CG; t < tiles; t += step, acc.next(), serial++) {
                 if (!mbar_wait(&sh.acc_empty[acc.i], acc.phase, &sh.dead)) goto mma_done;
                 tc_fence_after();
                 const uint32_t d = tmem + acc.i * BN;
                 uint32_t add = 0;
-                int steps = 1, at = 0;
-                const auto low_step = [&] {
-                    if (!mbar_wait(&sh.xfull[x.i], x.phase, &sh.dead)) return false;
-                    tc_fence_after();
-                    if (at++ == 0) steps = *reinterpret_cast<volatile uint32_t*>(&sh.steps[serial & 3]);
-                    const uint32_t s = xring + x.i * L::kXStage;
-#pragma unroll
-                    for (int k = 0; k < kXK / 8; k++, add = 1)
-                        mma_tf32<CG>(d, desc_k64(s + k * 32), desc_k64(s + 128 * kXK * 4 + k * 32), xdesc, add);
-                    mma_commit<CG>(&sh.xempty[x.i]);
-                    x.next();
-                    return true;
-                };
-                // Two low-rank steps, which were filled during the tile before, come
-                // first, but for the first tile, whose low may still be computed;
-                // the rest, filled in the meantime, after the shared projection.
-                // The order of the sums goes by sizes and indexes alone.
-                if (serial && a.kblocks) {
-                    while (at < steps && at < 2)
-                        if (!low_step()) goto mma_done;
-                    if (!drained()) goto mma_done;
-                }
                 for (int kb = 0; kb < a.kblocks; kb++, r.next()) {
                     if (!mbar_wait(&sh.full[r.i], r.phase, &sh.dead)) goto mma_done;
                     tc_fence_after();
@@ -246,10 +228,25 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                     }
                     mma_commit<CG>(&sh.empty[r.i]);
                 }
-                if (at < steps) {
-                    if (a.kblocks && !drained()) goto mma_done;
-                    while (at < steps)
-                        if (!low_step()) goto mma_done;
+                if (!mbar_wait(&sh.counted[serial & 7], serial >> 3 & 1, &sh.dead)) goto mma_done;
+                units = *reinterpret_cast<volatile int*>(&sh.units[serial & 7]);
+                if (a.kblocks && units) {
+                    // the two kinds of instruction are ordered by waiting: a few
+                    // hundred of some ten thousand cycles
+                    mma_commit<CG>(&sh.drained);
+                    if (!mbar_wait(&sh.drained, drain_phase, &sh.dead)) goto mma_done;
+                    drain_phase ^= 1;
+                }
+                for (int u = 0; u < units; u += 2, r.next()) {
+                    if (!mbar_wait(&sh.full[r.i], r.phase, &sh.dead)) goto mma_done;
+                    tc_fence_after();
+                    for (int h = 0; h < 2 && u + h < units; h++) {
+                        const uint32_t s = ring + r.i * L::kStage + h * L::kUnit;
+#pragma unroll
+                        for (int k = 0; k < kXK / 8; k++, add = 1)
+                            mma_tf32<CG>(d, desc_k64(s + k * 32), desc_k64(s + 128 * kXK * 4 + k * 32), xdesc, add);
+                    }
+                    mma_commit<CG>(&sh.empty[r.i]);
                 }
                 mma_commit<CG>(&sh.acc_full[acc.i]);
             }
@@ -270,14 +267,14 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 e[h] = t < tiles && m < p.n ? p.id.of(m) : -1;
             }
         };
-        Ring x(L::kXBufs, 1);
+        Ring r(L::kStages, 1);
         int serial = 0, e[CG];
         load_ids(blockIdx.x / CG, e);
         for (int t = blockIdx.x / CG; t < tiles; t += step, serial++) {
             const long long m0 = (long long)(t % a.tiles_m) * 128 * CG, m = m0 + rank * 128 + i;
             const int o0 = t / a.tiles_m * BN + (int)rank * L::kRows;
             int pos[CG];
-            if (i == 0) sh.bad[serial & 7] = 0;  // the epilogue is less than eight tiles behind
+            if (i == 0) sh.bad[serial & 15] = 0;  // the ring and the accumulators are less than sixteen tiles
             const int distinct = tile_adapters(sh.adapters, w, e, pos);
             const int own = CG == 2 && rank ? pos[CG - 1] : pos[0];
             // the next tile's
@@ -288,18 +285,29 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             const auto flag = [&](int d) { return p.bad[((long long)sh.adapters.list[d / flags] * blocks + tile_o / 128) * per + d % flags]; };
             uint32_t bad = i < distinct * flags ? flag(i) : 0u;
             for (int d = i + 128; d < distinct * flags; d += 128) bad |= flag(d);
-            const int steps = max(1, distinct);
-            if (i == 0) sh.steps[serial & 3] = steps * per;
+            // without a shared product something has to clear the accumulator
+            const int count = a.kblocks ? distinct : max(1, distinct), units = count * per;
+            if (i == 0) {
+                sh.units[serial & 7] = units;
+                mbar_arrive(&sh.counted[serial & 7]);
+            }
+            r.skip(a.kblocks);
+            bool late = shared_part && !mbar_wait(&sh.turn[0], serial & 1, &sh.dead);
+            if (!units) {
+                if (bar_or(1, 128, late)) goto build_done;
+                if (i == 0) mbar_arrive(&sh.turn[1]);
+            }
+            int u = 0;
+            float4 f[4];
             for (int j = 0; j < rs; j += kXK) {
-                float4 f[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) f[q] = low[j / 4 + q];
-                if (bad) sh.bad[serial & 7] = 1;
-                for (int d = 0; d < steps; d++, x.next()) {
-                    const bool late = !mbar_wait(&sh.xempty[x.i], x.phase, &sh.dead);
-                    const uint32_t s = xring + x.i * L::kXStage;
+                if (bad) sh.bad[serial & 15] = 1;
+                for (int d = 0; d < count; d++, u++) {
+                    const uint32_t s = ring + r.i * L::kStage + (u & 1) * L::kUnit;
+                    if (!(u & 1)) late |= !mbar_wait(&sh.empty[r.i], r.phase, &sh.dead);
                     if (i == 0) {
-                        const uint32_t bar = CG == 2 ? map_rank(&sh.xfull[x.i], 0) : smem_u32(&sh.xfull[x.i]);
+                        const uint32_t bar = CG == 2 ? map_rank(&sh.full[r.i], 0) : smem_u32(&sh.full[r.i]);
                         tma_3d<CG>(s + 128 * kXK * 4, &mg, j, o0, distinct ? sh.adapters.list[d] : 0, bar);
                     }
                     const bool in = d == own;
@@ -309,9 +317,13 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                                    in ? __float_as_uint(f[q].z) : 0u, in ? __float_as_uint(f[q].w) : 0u);
                     fence_async_shared();
                     if (bar_or(1, 128, late)) goto build_done;  // all 128 threads or none
-                    if (i == 0) {
-                        if (rank == 0) mbar_expect(&sh.xfull[x.i], CG * L::kRows * kXK * 4);
-                        else mbar_arrive_at(map_rank(&sh.xfull[x.i], 0));
+                    if ((u & 1) || u + 1 == units) {
+                        if (i == 0) {
+                            if (rank == 0) mbar_expect(&sh.full[r.i], CG * (1 + (u & 1)) * L::kRows * kXK * 4);
+                            else mbar_arrive_at(map_rank(&sh.full[r.i], 0));
+                            if (u + 1 == units && shared_part) mbar_arrive(&sh.turn[1]);
+                        }
+                        r.next();
                     }
                 }
             }
@@ -374,7 +386,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             tc_fence_after();
             const uint32_t d = tmem + acc.i * BN + half * (BN / 2) + ((uint32_t)quarter << 21);  // lane 32 * quarter
             const bool row = m < p.n;
-            const bool bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[serial & 7]);
+            const bool bad = *reinterpret_cast<volatile uint32_t*>(&sh.bad[serial & 15]);
             const int e = bad && row ? p.id.of(m) : -1;
             if (a.tma_out) {
                 // through shared memory, so that rows leave as whole boxes; base
@@ -445,8 +457,11 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 }
             }
             tc_fence_before();
-            if constexpr (CG == 2) mbar_arrive_at(map_rank(&sh.acc_empty[acc.i], 0));
-            else mbar_arrive(&sh.acc_empty[acc.i]);
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) mbar_arrive_at(map_rank(&sh.acc_empty[acc.i], 0));
+                else mbar_arrive(&sh.acc_empty[acc.i]);
+            }
         }
         if (lane == 0) tma_store_wait_read<0>();
     }

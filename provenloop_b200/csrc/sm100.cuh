@@ -82,6 +82,11 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// Without ordering what came before: a release to the cluster costs some
+// hundred cycles, which a thread that only starts copies need not pay.
+__device__ __forceinline__ void mbar_arrive_relaxed_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
@@ -95,6 +100,11 @@ struct Ring {
     __device__ __forceinline__ Ring(int n_, uint32_t phase_) : n(n_), phase(phase_) {}
     __device__ __forceinline__ void next() {
         if (++i == n) i = 0, phase ^= 1;
+    }
+    __device__ __forceinline__ void skip(int by) {
+        i += by;
+        phase ^= (uint32_t)(i / n) & 1;
+        i %= n;
     }
 };
 

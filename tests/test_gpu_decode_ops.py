@@ -158,6 +158,10 @@ SHAPES = [  # n, d_in, d_out, r, adapters, layout
     (300, 8960, 256, 64, 5, "ragged"),
     (513, 1001, 770, 7, 3, "ragged"),
     (1100, 1536, 264, 16, 200, "mixed"),
+    (2300, 1536, 4104, 32, 5, "ragged"),
+    (1500, 4104, 4096, 16, 3, "none"),
+    (1300, 4104, 1000, 17, 40, "mixed"),
+    (4099, 200, 2056, 16, 2, "one"),
 ]
 
 
@@ -270,12 +274,12 @@ def test_no_tokens(A):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("n", [8, 40, 200])
+@pytest.mark.parametrize("n,i,o", [(8, 264, 200), (40, 264, 200), (200, 264, 200), (300, 264, 4000), (300, 4000, 264)])
 @pytest.mark.parametrize("weight", [True, False])
-def test_a_request_is_not_touched_by_the_others(A, n, weight, dt):
+def test_a_request_is_not_touched_by_the_others(A, n, i, o, weight, dt):
     """NaN and infinities in one adapter, or in one request's rows, stay with
     the tokens that use them, forward and backward."""
-    s = _inputs(n, 264, 200, 16, 3, dt, "mixed", seed=9)
+    s = _inputs(n, i, o, 16, 3, dt, "mixed", seed=9)
     s["ids"] = (torch.arange(n, device="cuda") % 4 - 1).to(torch.int32)
     kw = dict(weight=s["w"] if weight else None, scale=s["scale"])
     clean = A.adapter_project(s["x"], s["a"], s["b"], s["ids"], **kw)
