@@ -139,7 +139,7 @@ bool rows_ok(const void* p, uint64_t rows, uint32_t cols, int64_t stride, size_t
 struct Plan {
     bool f32, small, low_vec, out;
     bool pack_x, pack_w, pack_a, pack_grad, pack_b, g32, lists;
-    uint64_t low, u, x, w, a, grad, b, g, bad, list, bytes;
+    uint64_t low, u, usplit, x, w, a, grad, b, g, bad, list, partial, bytes;
 };
 
 Plan plan_of(const ts_adapter_args* a, int backward) {
@@ -180,6 +180,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     const uint64_t rs = low_stride((int)a->r), low = a->n * rs * 4, o = backward ? a->d_in : a->d_out;
     p.low = take(!backward || a->grad_a, low);
     p.u = take(backward, low);
+    p.usplit = take(p.lists && a->dtype == TS_DTYPE_BF16, low);  // low itself is split then
     p.x = take(p.pack_x, a->n * up16(a->d_in, size) * size);
     p.w = take(p.pack_w, (uint64_t)a->d_out * up8(a->d_in) * 2);
     p.a = take(p.pack_a, (uint64_t)a->adapters * a->r * up8(a->d_in) * 2);
@@ -188,6 +189,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     p.g = take(p.g32, a->adapters * o * rs * 4);
     p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * (rs / 16) * 4);
     p.list = take(p.lists, (a->adapters + 1 + a->n) * 4);
+    p.partial = take(p.lists && a->n, a->n ? grad_partial_bytes((long long)a->n, a->d_in, a->d_out, (int)a->r) : 0);
     p.bytes = a->n ? at : 0;
     return p;
 }
@@ -223,19 +225,16 @@ struct Work {
     const ts_adapter_args* a;
     cudaStream_t s;
     PackJobs jobs{};
-    int after_pack = 0;  // 2: what is packed is used by the next launch
     void* at(uint64_t off) const { return static_cast<char*>(a->workspace) + off; }
     Rows rows(bool pack, const void* p, uint64_t rows, uint32_t cols, long long stride, uint64_t off) {
         const size_t size = dtype_size(a->dtype);
         const int pitch = up16(cols, size), halves = (int)size / 2;  // elements are copied as 16-bit ones
         if (!pack) return {p, rows < 2 ? pitch : stride};
         jobs.add({PackJob::COPY, p, 0, stride * halves, 1, (long long)rows, 1, (int)cols * halves, pitch * halves, at(off)});
-        after_pack = 2;
         return {at(off), pitch};
     }
     cudaError_t pack() {
         if (!jobs.jobs) return cudaSuccess;
-        if (!after_pack) after_pack = 1;
         jobs.dtype = a->dtype;
         return launch_pack(jobs, s);
     }
@@ -259,8 +258,9 @@ int adapter_project(const ts_adapter_args* a) {
     if (p.g32)
         w.jobs.add({PackJob::TO_F32, a->lora_b, rb, r, 1, d_o, (int)a->adapters, r, low_stride(r), w.at(p.g), static_cast<uint32_t*>(w.at(p.bad))});
     cudaError_t e = w.pack();
-    const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low};
-    if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, w.after_pack, w.s);
+    const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low, nullptr};
+    const int after_pack = !w.jobs.jobs ? 0 : p.pack_x || p.pack_a ? 2 : 1;
+    if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, &after_pack, w.s);
     const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low,
                         {a->lora_b, rb, 1, r}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
     if (e == cudaSuccess)
@@ -297,7 +297,6 @@ int adapter_project_backward(const ts_adapter_args* a) {
         grad = w.rows(p.pack_grad, a->grad, a->n, a->d_out, a->grad_stride, p.grad);
         if (p.pack_a) fa = w.rows(true, a->lora_a, (uint64_t)a->adapters * a->r, a->d_in, a->d_in, p.a);
         w.jobs.add({PackJob::COPY, a->lora_b, rb, 1, r, r, (int)a->adapters, d_o, up8(a->d_out), w.at(p.b)});
-        w.after_pack = 2;
         fb = {w.at(p.b), (long long)r * up8(a->d_out), up8(a->d_out), 1};
     }
     if (p.g32)
@@ -309,18 +308,25 @@ int adapter_project_backward(const ts_adapter_args* a) {
         w.jobs.add(j);
     }
     cudaError_t e = w.pack();
-    const LowArgs l[2] = {{grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, u},
-                          {x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low}};
-    if (e == cudaSuccess) e = launch_low(l, a->grad_a ? 2 : 1, a->dtype, p.low_vec, w.after_pack, w.s);
+    // u last: it needs the packed factor, low mostly nothing of the packing
+    const bool split = a->dtype == TS_DTYPE_BF16 && a->grad_a;
+    uint16_t* const lsplit = split ? reinterpret_cast<uint16_t*>(low) : nullptr;
+    uint16_t* const usplit = split ? static_cast<uint16_t*>(w.at(p.usplit)) : nullptr;
+    const LowArgs l[2] = {{x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, split ? nullptr : low, lsplit},
+                          {grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, a->out || !split ? u : nullptr, usplit}};
+    const int after_pack[2] = {!w.jobs.jobs ? 0 : p.pack_x || p.pack_a ? 2 : 1, !w.jobs.jobs ? 0 : p.pack_b || p.pack_grad ? 2 : 1};
+    const int skip = a->grad_a ? 0 : 1;
+    if (e == cudaSuccess) e = launch_low(l + skip, 2 - skip, a->dtype, p.low_vec, after_pack + skip, w.s);
     if (e == cudaSuccess && a->out) {
         const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u,
                             {a->lora_a, ra, di, 1}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
         e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }
     if (e == cudaSuccess && a->grad_a) {
-        const GradPair g{{{x.p, x.stride, di, u, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, low, a->grad_b, rb, 1, r}},
+        const void *gu = split ? (const void*)usplit : u, *gl = split ? (const void*)lsplit : low;
+        const GradPair g{{{x.p, x.stride, di, gu, a->grad_a, ra, di, 1}, {grad.p, grad.stride, d_o, gl, a->grad_b, rb, 1, r}},
                          r, (int)a->adapters, first, first + a->adapters + 1};
-        e = launch_grads(g, n, a->dtype, !p.f32 && a->out, w.s);
+        e = launch_grads(g, n, a->dtype, !p.f32 && a->out, static_cast<float*>(w.at(p.partial)), w.s);
     }
     return cuda_status(e);
 }

@@ -181,23 +181,36 @@ __device__ void pack_lists(const PackJob& a, int e) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int* first = static_cast<int*>(a.dst);
     int* list = first + a.count + 1;
-    const long long each = (a.rows + 255) / 256 * 32, m0 = min(warp * each, a.rows), m1 = min(m0 + each, a.rows);
-    const auto scan = [&](auto see) {  // 32 tokens in a step, eight steps' loads together
-        long long m = m0;
-        for (; m + 256 <= m1; m += 256) {
-            int id[8];
+    // four neighbouring tokens a lane, in one load where the indexes allow
+    const long long each = (a.rows + 1023) / 1024 * 128, m0 = min(warp * each, a.rows), m1 = min(m0 + each, a.rows);
+    const bool quads = a.id.per == 1 && (reinterpret_cast<uintptr_t>(a.id.ids) & 15) == 0;
+    const auto scan = [&](auto see) {
+        const auto known = [&](int id) { return (unsigned)id < (unsigned)a.id.count ? id : -1; };
+        long long m = m0 + lane * 4;
+        if (quads)
+            for (; m - lane * 4 + 512 <= m1; m += 512) {
+                int4 id[4];
 #pragma unroll
-            for (int q = 0; q < 8; q++) id[q] = a.id.of(m + q * 32 + lane);
+                for (int q = 0; q < 4; q++) id[q] = *reinterpret_cast<const int4*>(a.id.ids + m + q * 128);
 #pragma unroll
-            for (int q = 0; q < 8; q++) see(id[q], m + q * 32 + lane);
+                for (int q = 0; q < 4; q++) {
+                    const int v[4] = {known(id[q].x), known(id[q].y), known(id[q].z), known(id[q].w)};
+                    see(v, m + q * 128);
+                }
+            }
+        for (; m - lane * 4 < m1; m += 128) {
+            int v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = m + i < m1 ? a.id.of(m + i) : -1;
+            see(v, m);
         }
-        for (; m < m1; m += 32) see(m + lane < m1 ? a.id.of(m + lane) : -1, m + lane);
     };
     int less = 0, own = 0;  // tokens of lower adapters, of this one
-    scan([&](int id, long long) {
-        less += __popc(__ballot_sync(0xffffffffu, id >= 0 && id < e));
-        own += __popc(__ballot_sync(0xffffffffu, id == e));
+    scan([&](const int (&id)[4], long long) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) less += id[i] >= 0 && id[i] < e, own += id[i] == e;
     });
+    less = __reduce_add_sync(0xffffffffu, less), own = __reduce_add_sync(0xffffffffu, own);
     if (lane == 0) warp_own[warp] = own, warp_less[warp] = less;
     __syncthreads();
     int at = 0, total = 0;
@@ -209,10 +222,17 @@ __device__ void pack_lists(const PackJob& a, int e) {
         if (e + 1 == a.count) first[a.count] = less + total;
     }
     at += less;
-    if (own) scan([&](int id, long long m) {
-        const unsigned ball = __ballot_sync(0xffffffffu, id == e);
-        if (id == e) list[at + __popc(ball & ((1u << lane) - 1))] = (int)m;
-        at += __popc(ball);
+    if (own) scan([&](const int (&id)[4], long long m) {
+        unsigned ball[4];
+        int before = at;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            ball[i] = __ballot_sync(0xffffffffu, id[i] == e);
+            before += __popc(ball[i] & ((1u << lane) - 1)), at += __popc(ball[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (id[i] == e) list[before++] = (int)m + i;
     });
 }
 
@@ -251,7 +271,7 @@ __device__ __forceinline__ float low_value(float v) {
 template <class T, bool VEC, int WPJ>
 __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
     release_dependents();
-    if (both.after_pack == 2) grid_dependency_wait();
+    if (both.after_pack[blockIdx.z] == 2) grid_dependency_wait();
     const LowArgs a = both.a[blockIdx.z];
     const long long m = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPJ;
@@ -285,9 +305,16 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
             for (int q = 0; q < WPJ; q++) v += part_sum[warp + q];
         }
     }
-    if (part == 0 && lane == 0 && j < rs) a.low[m * rs + j] = e >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e] * v : v) : 0.f;
+    if (part == 0 && lane == 0 && j < rs) {
+        const float low = e >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e] * v : v) : 0.f;
+        if (a.low) a.low[m * rs + j] = low;
+        if (a.split) {
+            const __nv_bfloat16 h = __float2bfloat16_rn(low), l = __float2bfloat16_rn(low - __bfloat162float(h));
+            a.split[m * 2 * rs + j] = __bfloat16_as_ushort(h), a.split[(m * 2 + 1) * rs + j] = __bfloat16_as_ushort(l);
+        }
+    }
     // the next launch waits for this one, and with it for the packing
-    if (both.after_pack == 1) grid_dependency_wait();
+    if (both.after_pack[blockIdx.z] == 1) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------- projection
@@ -465,7 +492,7 @@ __global__ void __launch_bounds__(256) k_project_small(const ProjectArgs a) {
 // ---------------------------------------------------------------- gradients of the factors
 
 
-constexpr int kGradChunk = 64;  // groups whose tokens are listed in shared memory at a time
+constexpr int kGradChunk = 32;  // groups whose tokens are listed in shared memory at a time
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -473,167 +500,244 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int by
 
 template <class T, int RB>
 struct GradTile {
-    static constexpr int kRow = sizeof(T) == 4 ? 136 * 4 : 288;  // 128 features; rows 8 banks apart
-    static constexpr int kURow = RB * 8 + 8;                     // floats
-    static constexpr int kX = 32 * kRow, kU = 32 * kURow * 4;
-    static constexpr int kStages = 4;
+    static constexpr bool kSplit = std::is_same<T, __nv_bfloat16>::value;  // low as two bf16 terms
+    // 128 features; rows four (split: 16 bytes; else 8 banks) apart from a multiple of all banks
+    static constexpr int kRow = kSplit ? 272 : sizeof(T) == 4 ? 136 * 4 : 288;
+    static constexpr int kURow = kSplit ? RB * 32 + 16 : RB * 32 + 32;  // bytes
+    static constexpr int kX = 32 * kRow, kU = 32 * kURow;
+    static constexpr int kStages = sizeof(T) == 4 || RB == 8 ? 4 : 5;
+    static constexpr int kPerSm = sizeof(T) == 4 || RB == 8 ? 2 : 3;  // CTAs
     static constexpr int kSmem = kStages * (kX + kU);
 };
 
-// One adapter, 128 features and RB * 8 rank indexes per cluster of S CTAs.
-// Every CTA takes every S-th group of 32 of the adapter's tokens, gathers
-// their rows and sums low^T x with 16 x 8 x 8 TF32 products: features are
-// the 16-row axis, tokens the contraction.  16-bit x is exact in TF32, and
-// low has been rounded to it; for f32 inputs both are split into two TF32
-// parts, which leaves 2^-22.  The partial sums of the cluster meet in shared
-// memory in a fixed order.  Bound: reading x once per 64 rank indexes; the
-// copies' addresses were its instructions until a thread's column and its
-// part of a row were fixed for all groups.
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// A window of W places of the tokens' list (adapter by adapter), 128 features
+// and RB * 8 rank indexes per CTA, so that CTAs have the same work however
+// the tokens are spread over the adapters.  For each adapter in the window, in
+// groups of 32 tokens, the rows are gathered and low^T x summed with matrix
+// instructions whose 16-row axis are the features and whose contraction the
+// tokens.  bf16: 16 x 8 x 16 products with low's two bf16 terms, which are its
+// 11 bits exactly, operands transposed on the way from shared memory.  Else
+// 16 x 8 x 8 TF32 products: fp16 x is exact in TF32, and low has been rounded
+// to it; for f32 inputs both are split into two TF32 parts, which leaves
+// 2^-22.  An adapter that lies in one window is written here; the others' sums
+// over a window go to the workspace, and k_grad_sum adds them in the
+// windows' order.  Bound: reading x once per 64 rank indexes.
 template <class T, int RB>
-__global__ void __launch_bounds__(256) k_grad(const GradPair both, int tiles0, int dependent) {
+__global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const GradPair both, int tiles0, int window, float* partial, int dependent) {
     using L = GradTile<T, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int own[kGradChunk * 32];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int tile = blockIdx.x / S;
+    __shared__ int own[kGradChunk * 32], start;
+    release_dependents();
+    const int tile = blockIdx.x;
     const GradArgs a = both.g[tile >= tiles0];
-    const int k0 = (tile >= tiles0 ? tile - tiles0 : tile) * 128, j0 = blockIdx.y * RB * 8, e = blockIdx.z;
+    const int k0 = (tile >= tiles0 ? tile - tiles0 : tile) * 128, j0 = blockIdx.y * RB * 8;
     const int rs = low_stride(both.r);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int wf = warp & 3, wt = warp >> 2;
     // what is read here was complete before the launch before this one let it
     // start (k_project.cu); that launch itself is waited for in the end
-    const int begin = __ldcg(both.first + e), tokens = __ldcg(both.first + e + 1) - begin;
-    const int* list = both.list + begin;
-    float acc[2][RB][4] = {};
+    const int* first = both.first;
+    const int pos0 = blockIdx.z * window, total = first[both.adapters], pos1 = min(pos0 + window, total);
+    for (int e = threadIdx.x; e < both.adapters; e += 256)
+        if (first[e] <= pos0 && pos0 < first[e + 1]) start = e;
+    __syncthreads();
 
     // this thread's part of every group: 16 bytes at one place of some rows
     constexpr int C = 128 * (int)sizeof(T) / 16, kRows = 256 / C, kXParts = 32 / kRows;  // of x
     constexpr int CU = RB * 2, kURows = 256 / CU < 32 ? 256 / CU : 32, kUParts = 32 / kURows;  // of low
     const int xc = threadIdx.x % C, xrow = threadIdx.x / C, uc = threadIdx.x % CU, urow = threadIdx.x / CU;
-    const int xbytes = min(16, max(0, (a.k - k0) * (int)sizeof(T) - xc * 16)), ubytes = j0 + uc * 4 < rs && urow < 32 ? 16 : 0;
+    const int xbytes = min(16, max(0, (a.k - k0) * (int)sizeof(T) - xc * 16));
+    // split: RB parts of the high terms, RB of the low ones
+    const int uj = L::kSplit ? j0 + uc % RB * 8 : j0 + uc * 4, ufirst = L::kSplit ? (uc / RB * rs + uj) * 2 : uj * 4;
+    const int ubytes = uj < rs && urow < 32 ? 16 : 0;
     const char* xfrom = static_cast<const char*>(a.x) + (xbytes ? (size_t)k0 * sizeof(T) + xc * 16 : 0);
-    const char* ufrom = reinterpret_cast<const char*>(a.low) + (ubytes ? (size_t)j0 * 4 + uc * 16 : 0);
+    const char* ufrom = static_cast<const char*>(a.low) + (ubytes ? ufirst : 0);
     const long long xpitch = a.x_stride * (long long)sizeof(T);
-    const uint32_t base = smem_u32(smem), xto = base + xrow * L::kRow + xc * 16, uto = base + L::kX + urow * L::kURow * 4 + uc * 16;
+    const uint32_t base = smem_u32(smem), xto = base + xrow * L::kRow + xc * 16, uto = base + L::kX + urow * L::kURow + uc * 16;
 
-    const int all = (tokens + 31) / 32, mine = all / S + (all % S > rank);  // groups of 32, and this CTA's
-    for (int q0 = 0; q0 < mine; q0 += kGradChunk) {
-        const int groups = min(kGradChunk, mine - q0);
-        for (int i = threadIdx.x; i < groups * 32; i += 256) {
-            const int at = ((q0 + (i >> 5)) * S + rank) * 32 + (i & 31);
-            own[i] = at < tokens ? __ldcg(list + at) : -1;
-        }
-        __syncthreads();
-        uint32_t put = 0, take = 0;  // stages' offsets
-        const auto next = [](uint32_t at) { return at + (L::kX + L::kU) == L::kSmem ? 0u : at + (L::kX + L::kU); };
-        const auto fetch = [&](int q) {
-            if (q < groups) {
-#pragma unroll
-                for (int i = 0; i < kXParts; i++) {
-                    const int m = own[q * 32 + xrow + i * kRows];
-                    cp_async16(xto + put + i * kRows * L::kRow, xfrom + max(m, 0) * xpitch, m >= 0 ? xbytes : 0);
-                }
-                if (urow < 32)
-#pragma unroll
-                    for (int i = 0; i < kUParts; i++) {
-                        const int m = own[q * 32 + urow + i * kURows];
-                        cp_async16(uto + put + i * kURows * L::kURow * 4, ufrom + max(m, 0) * (long long)(rs * 4), m >= 0 ? ubytes : 0);
-                    }
+    int e = start;
+    for (int pos = pos0; pos < pos1; e++) {
+        const int e0 = first[e], e1 = first[e + 1], end = min(e1, pos1);
+        if (e1 <= pos) continue;
+        float acc[2][RB][4] = {};
+        const int all = (end - pos + 31) / 32;
+        for (int q0 = 0; q0 < all; q0 += kGradChunk) {
+            const int groups = min(kGradChunk, all - q0);
+            for (int i = threadIdx.x; i < groups * 32; i += 256) {
+                const int at = pos + q0 * 32 + i;
+                own[i] = at < end ? both.list[at] : -1;
             }
-            put = next(put);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int q = 0; q < L::kStages - 1; q++) fetch(q);
-        for (int q = 0; q < groups; q++, take = next(take)) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
             __syncthreads();
-            fetch(q + L::kStages - 1);
-            const uint8_t* sx = smem + take;
-            const float* su = reinterpret_cast<const float*>(sx + L::kX);
+            uint32_t put = 0, take = 0;  // stages' offsets
+            const auto next = [](uint32_t at) { return at + (L::kX + L::kU) == L::kSmem ? 0u : at + (L::kX + L::kU); };
+            const auto fetch = [&](int q) {
+                if (q < groups) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int tok = (wt * 2 + h) * 8 + t;
-                // four features of two tokens per thread: rows g and g + 8 of two products
-                float f[2][4];
-#pragma unroll
-                for (int z = 0; z < 2; z++) {
-                    const uint8_t* p = sx + (tok + 4 * z) * L::kRow + (wf * 32 + 4 * g) * sizeof(T);
-                    if constexpr (sizeof(T) == 4) {
-                        const float4 v = *reinterpret_cast<const float4*>(p);
-                        f[z][0] = v.x, f[z][1] = v.y, f[z][2] = v.z, f[z][3] = v.w;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(p);
-                        const float2 lo = pair_f<T>(v.x), hi = pair_f<T>(v.y);
-                        f[z][0] = lo.x, f[z][1] = lo.y, f[z][2] = hi.x, f[z][3] = hi.y;
+                    for (int i = 0; i < kXParts; i++) {
+                        const int m = own[q * 32 + xrow + i * kRows];
+                        cp_async16(xto + put + i * kRows * L::kRow, xfrom + max(m, 0) * xpitch, m >= 0 ? xbytes : 0);
                     }
+                    if (urow < 32)
+#pragma unroll
+                        for (int i = 0; i < kUParts; i++) {
+                            const int m = own[q * 32 + urow + i * kURows];
+                            cp_async16(uto + put + i * kURows * L::kURow, ufrom + max(m, 0) * (long long)(rs * 4), m >= 0 ? ubytes : 0);
+                        }
                 }
-                uint32_t am[2][4], al[2][4];
+                put = next(put);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
 #pragma unroll
-                for (int q2 = 0; q2 < 2; q2++)
+            for (int q = 0; q < L::kStages - 1; q++) fetch(q);
+            for (int q = 0; q < groups; q++, take = next(take)) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+                __syncthreads();
+                fetch(q + L::kStages - 1);
+                const uint8_t* sx = smem + take;
+                if constexpr (L::kSplit) {
+                    // 16 tokens a warp; lanes address rows of 8 x 8 blocks: tokens down, features / rank indexes across
+                    const uint32_t xat = base + take + (wt * 16 + (lane >> 4) * 8 + (lane & 7)) * L::kRow + (wf * 32 + (lane >> 3 & 1) * 8) * 2;
+                    const uint32_t uat = base + take + L::kX + (wt * 16 + (lane & 15)) * L::kURow + (lane >> 4) * 16;
+                    uint32_t f[2][4];
+                    ldmatrix4_trans(f[0], xat);
+                    ldmatrix4_trans(f[1], xat + 32);
 #pragma unroll
-                    for (int z = 0; z < 4; z++) {
-                        const float v = f[z >> 1][q2 * 2 + (z & 1)];
+                    for (int term = 0; term < 2; term++)
+#pragma unroll
+                        for (int nb = 0; nb < RB; nb += 2) {
+                            uint32_t u[4];
+                            ldmatrix4_trans(u, uat + term * RB * 16 + nb * 16);
+#pragma unroll
+                            for (int q = 0; q < 2; q++) {
+                                mma16<T>(acc[q][nb], f[q][0], f[q][1], f[q][2], f[q][3], u[0], u[1]);
+                                mma16<T>(acc[q][nb + 1], f[q][0], f[q][1], f[q][2], f[q][3], u[2], u[3]);
+                            }
+                        }
+                    continue;
+                }
+                const float* su = reinterpret_cast<const float*>(sx + L::kX);
+                constexpr int UR = L::kURow / 4;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int tok = (wt * 2 + h) * 8 + t;
+                    // four features of two tokens per thread: rows g and g + 8 of two products
+                    float f[2][4];
+#pragma unroll
+                    for (int z = 0; z < 2; z++) {
+                        const uint8_t* p = sx + (tok + 4 * z) * L::kRow + (wf * 32 + 4 * g) * sizeof(T);
                         if constexpr (sizeof(T) == 4) {
-                            am[q2][z] = to_tf32(v);
-                            al[q2][z] = to_tf32(v - __uint_as_float(am[q2][z]));
+                            const float4 v = *reinterpret_cast<const float4*>(p);
+                            f[z][0] = v.x, f[z][1] = v.y, f[z][2] = v.z, f[z][3] = v.w;
                         } else {
-                            am[q2][z] = __float_as_uint(v);
+                            const uint2 v = *reinterpret_cast<const uint2*>(p);
+                            const float2 lo = pair_f<T>(v.x), hi = pair_f<T>(v.y);
+                            f[z][0] = lo.x, f[z][1] = lo.y, f[z][2] = hi.x, f[z][3] = hi.y;
                         }
                     }
+                    uint32_t am[2][4], al[2][4];
 #pragma unroll
-                for (int nb = 0; nb < RB; nb++) {
-                    const float b0 = su[tok * L::kURow + nb * 8 + g], b1 = su[(tok + 4) * L::kURow + nb * 8 + g];
-                    const uint32_t m0b = sizeof(T) == 4 ? to_tf32(b0) : __float_as_uint(b0), m1b = sizeof(T) == 4 ? to_tf32(b1) : __float_as_uint(b1);
+                    for (int q2 = 0; q2 < 2; q2++)
 #pragma unroll
-                    for (int q2 = 0; q2 < 2; q2++) {
-                        if constexpr (sizeof(T) == 4) {
-                            const uint32_t l0 = to_tf32(b0 - __uint_as_float(m0b)), l1 = to_tf32(b1 - __uint_as_float(m1b));
-                            mma8_tf32(acc[q2][nb], al[q2], m0b, m1b);
-                            mma8_tf32(acc[q2][nb], am[q2], l0, l1);
+                        for (int z = 0; z < 4; z++) {
+                            const float v = f[z >> 1][q2 * 2 + (z & 1)];
+                            if constexpr (sizeof(T) == 4) {
+                                am[q2][z] = to_tf32(v);
+                                al[q2][z] = to_tf32(v - __uint_as_float(am[q2][z]));
+                            } else {
+                                am[q2][z] = __float_as_uint(v);
+                            }
                         }
-                        mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
+#pragma unroll
+                    for (int nb = 0; nb < RB; nb++) {
+                        const float b0 = su[tok * UR + nb * 8 + g], b1 = su[(tok + 4) * UR + nb * 8 + g];
+                        const uint32_t m0b = sizeof(T) == 4 ? to_tf32(b0) : __float_as_uint(b0), m1b = sizeof(T) == 4 ? to_tf32(b1) : __float_as_uint(b1);
+#pragma unroll
+                        for (int q2 = 0; q2 < 2; q2++) {
+                            if constexpr (sizeof(T) == 4) {
+                                const uint32_t l0 = to_tf32(b0 - __uint_as_float(m0b)), l1 = to_tf32(b1 - __uint_as_float(m1b));
+                                mma8_tf32(acc[q2][nb], al[q2], m0b, m1b);
+                                mma8_tf32(acc[q2][nb], am[q2], l0, l1);
+                            }
+                            mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
+                        }
                     }
                 }
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();
-    }
 
-    // the two token halves, then the cluster's CTAs: sum[rank index][feature]
-    float* sum = reinterpret_cast<float*>(smem);
-    constexpr int SR = 129;
-    static_assert(RB * 8 * SR * 4 <= L::kSmem, "the sums fit where the tiles were");
+        // the two token halves: sum[rank index][feature]
+        float* sum = reinterpret_cast<float*>(smem);
+        constexpr int SR = 129;
+        static_assert(RB * 8 * SR * 4 <= L::kSmem, "the sums fit where the tiles were");
 #pragma unroll
-    for (int half = 1; half >= 0; half--) {
-        if (wt == half)
+        for (int half = 1; half >= 0; half--) {
+            if (wt == half)
 #pragma unroll
-            for (int q = 0; q < 2; q++)
+                for (int q = 0; q < 2; q++)
 #pragma unroll
-                for (int nb = 0; nb < RB; nb++)
+                    for (int nb = 0; nb < RB; nb++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float* p = sum + (nb * 8 + 2 * t + (c & 1)) * SR + wf * 32 + 4 * g + 2 * q + (c >> 1);
-                        *p = half ? acc[q][nb][c] : *p + acc[q][nb][c];
-                    }
+                        for (int c = 0; c < 4; c++) {
+                            const int feature = L::kSplit ? 16 * q + g + 8 * (c >> 1) : 4 * g + 2 * q + (c >> 1);
+                            float* p = sum + (nb * 8 + 2 * t + (c & 1)) * SR + wf * 32 + feature;
+                            *p = half ? acc[q][nb][c] : *p + acc[q][nb][c];
+                        }
+            __syncthreads();
+        }
+        const bool whole = e0 >= pos0 && e1 <= pos1;
+        float* to = partial + ((((long long)blockIdx.z * 2 + (e0 >= pos0)) * gridDim.y + blockIdx.y) * gridDim.x + tile) * (RB * 8 * 128);
+        for (int i = threadIdx.x; i < RB * 8 * 128; i += 256) {
+            // consecutive threads along whichever axis of the result is contiguous
+            const int j = a.sk == 1 ? i >> 7 : i % (RB * 8), k = a.sk == 1 ? i & 127 : i / (RB * 8);
+            const float v = sum[j * SR + k];
+            if (!whole) to[i] = v;
+            else if (j0 + j < both.r && k0 + k < a.k)
+                static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(v);
+        }
         __syncthreads();
+        pos = end;
     }
-    if (S > 1) cluster.sync();
-    const int per = RB * 8 * 128 / S;
-    for (int i = threadIdx.x; i < per; i += 256) {
-        const int q = rank * per + i;
-        // consecutive threads along whichever axis of the result is contiguous
-        const int j = a.sk == 1 ? q >> 7 : q % (RB * 8), k = a.sk == 1 ? q & 127 : q / (RB * 8);
-        float v = 0.f;
-        for (int c = 0; c < S; c++) v += S > 1 ? *cluster.map_shared_rank(sum + j * SR + k, c) : sum[j * SR + k];
-        if (j0 + j < both.r && k0 + k < a.k)
-            static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(v);
-    }
-    if (S > 1) cluster.sync();
     if (dependent) grid_dependency_wait();
+}
+
+// The gradients of adapters whose tokens lie in several windows, and zeros for
+// those without tokens.
+template <class T, int RB>
+__global__ void __launch_bounds__(256) k_grad_sum(const GradPair both, int tiles0, int window, const float* partial) {
+    grid_dependency_wait();
+    constexpr int kParts = RB * 8 * 128 / 1024;  // four neighbouring results a thread
+    const int tile = blockIdx.x, e = blockIdx.z, pass = blockIdx.y / kParts, i = (blockIdx.y % kParts * 256 + threadIdx.x) * 4;
+    const GradArgs a = both.g[tile >= tiles0];
+    const int k0 = (tile >= tiles0 ? tile - tiles0 : tile) * 128, j0 = pass * RB * 8;
+    const int e0 = both.first[e], e1 = both.first[e + 1], w0 = e0 / window, w1 = e1 > e0 ? (e1 - 1) / window : w0 - 1;
+    if (w0 == w1) return;
+    const long long each = (long long)(gridDim.y / kParts) * gridDim.x * (RB * 8 * 128);  // between a window's two sums
+    const float* from = partial + ((long long)pass * gridDim.x + tile) * (RB * 8 * 128) + i;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](float4 f) { v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w; };
+    // the adapter begins in its first window and goes on in the others
+    if (w1 > w0) add(*reinterpret_cast<const float4*>(from + (w0 * 2 + 1) * each));
+    int w = w0 + 1;
+    for (; w + 7 <= w1; w += 8) {
+        float4 f[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) f[q] = *reinterpret_cast<const float4*>(from + (w + q) * 2 * each);
+#pragma unroll
+        for (int q = 0; q < 8; q++) add(f[q]);
+    }
+    for (; w <= w1; w++) add(*reinterpret_cast<const float4*>(from + w * 2 * each));
+    const float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int j = a.sk == 1 ? i >> 7 : (i + q) % (RB * 8), k = a.sk == 1 ? (i + q) & 127 : i / (RB * 8);
+        if (j0 + j < both.r && k0 + k < a.k) static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(r[q]);
+    }
 }
 
 int sm_count() {
@@ -643,18 +747,18 @@ int sm_count() {
 }
 
 template <class T>
-cudaError_t low_launch(const LowArgs* a, int count, bool vec, int after_pack, cudaStream_t s) {
+cudaError_t low_launch(const LowArgs* a, int count, bool vec, const int* after_pack, cudaStream_t s) {
     const long long n = a[0].n;
     if (sizeof(T) == 2 && !low_by_token(n, a[0].k, a[count - 1].k, a[0].r))
         return launch_low_tc(a, count, std::is_same<T, __half>::value ? DT_F16 : DT_BF16, after_pack, s);
-    const LowPair both{{a[0], a[count - 1]}, after_pack};
+    const LowPair both{{a[0], a[count - 1]}, {after_pack[0], after_pack[count - 1]}};
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     KScope ks("adapter_low", s);
     // long contractions over more warps, to have more loads in flight
     const int rs = low_stride(a[0].r);
     const auto go = [&](auto kern, int ranks) {
         const dim3 grid((unsigned)n, (rs + ranks - 1) / ranks, count);
-        return after_pack ? launch_dependent(1, kern, grid, 256, 0, s, both) : launch_cl(1, kern, grid, 256, 0, s, both);
+        return after_pack[0] ? launch_dependent(1, kern, grid, 256, 0, s, both) : launch_cl(1, kern, grid, 256, 0, s, both);
     };
     if (kmax * sizeof(T) > 4096) return vec ? go(k_low_token<T, true, 4>, 2) : go(k_low_token<T, false, 4>, 2);
     return vec ? go(k_low_token<T, true, 1>, 8) : go(k_low_token<T, false, 1>, 8);
@@ -683,26 +787,24 @@ cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
 }
 
 template <class T, int RB>
-cudaError_t grad_launch(const GradPair& a, long long n, bool dependent, cudaStream_t s) {
+cudaError_t grad_launch(const GradPair& a, long long n, bool dependent, float* partial, cudaStream_t s) {
     using L = GradTile<T, RB>;
     const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
-    // CTAs that share an adapter's tokens: until there are four for each SM,
-    // while each has four groups of tokens on average
-    const long long ctas = (long long)(t0 + t1) * passes * a.adapters;
-    int S = 1;
-    while (S < 8 && ctas * S < 4 * sm_count() && n / a.adapters >= 256 * S) S *= 2;
-    const cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 1024);  // own[] is beside the tiles
+    const int window = grad_window(n, a.g[0].k, a.g[1].k, a.r);
+    cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 1024);  // own[] is beside the tiles
     if (e != cudaSuccess) return e;
-    KScope ks("adapter_grad", s);
-    const dim3 grid((unsigned)((t0 + t1) * S), passes, a.adapters);
-    return dependent ? launch_dependent(S, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, 1) : launch_cl(S, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, 0);
+    const dim3 grid((unsigned)(t0 + t1), passes, (unsigned)((n + window - 1) / window)), sums((unsigned)(t0 + t1), passes * (RB * 8 * 128 / 1024), a.adapters);
+    KScope ks("adapter_grad", s, 2);
+    e = dependent ? launch_dependent(1, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, window, partial, 1)
+                  : launch_cl(1, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, window, partial, 0);
+    return e != cudaSuccess ? e : launch_dependent(1, k_grad_sum<T, RB>, sums, 256, 0, s, a, t0, window, static_cast<const float*>(partial));
 }
 
 template <class T>
-cudaError_t grad_width(const GradPair& a, long long n, bool dependent, cudaStream_t s) {
-    if (a.r <= 16) return grad_launch<T, 2>(a, n, dependent, s);
-    if (a.r <= 32) return grad_launch<T, 4>(a, n, dependent, s);
-    return grad_launch<T, 8>(a, n, dependent, s);
+cudaError_t grad_width(const GradPair& a, long long n, bool dependent, float* partial, cudaStream_t s) {
+    if (a.r <= 16) return grad_launch<T, 2>(a, n, dependent, partial, s);
+    if (a.r <= 32) return grad_launch<T, 4>(a, n, dependent, partial, s);
+    return grad_launch<T, 8>(a, n, dependent, partial, s);
 }
 
 }  // namespace
@@ -724,7 +826,7 @@ cudaError_t launch_pack(const PackJobs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int after_pack, cudaStream_t s) {
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, const int* after_pack, cudaStream_t s) {
     TSG_DTYPE_SWITCH(dtype, return low_launch<T>(a, count, vec, after_pack, s));
 }
 
@@ -738,8 +840,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
     return dtype == DT_BF16 ? small_width<__nv_bfloat16>(a, s) : small_width<__half>(a, s);
 }
 
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, cudaStream_t s) {
-    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, dependent, s));
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, float* partial, cudaStream_t s) {
+    TSG_DTYPE_SWITCH(dtype, return grad_width<T>(a, n, dependent, partial, s));
 }
 
 }  // namespace tsg

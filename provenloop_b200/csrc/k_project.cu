@@ -315,9 +315,9 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                     for (int q = 0; q < 4; q++)
                         st_shared4(s + i * 64 + ((q ^ (i >> 1 & 3)) << 4), in ? __float_as_uint(f[q].x) : 0u, in ? __float_as_uint(f[q].y) : 0u,
                                    in ? __float_as_uint(f[q].z) : 0u, in ? __float_as_uint(f[q].w) : 0u);
-                    fence_async_shared();
-                    if (bar_or(1, 128, late)) goto build_done;  // all 128 threads or none
                     if ((u & 1) || u + 1 == units) {
+                        fence_async_shared();
+                        if (bar_or(1, 128, late)) goto build_done;  // all 128 threads or none
                         if (i == 0) {
                             if (rank == 0) mbar_expect(&sh.full[r.i], CG * (1 + (u & 1)) * L::kRows * kXK * 4);
                             else mbar_arrive_at(map_rank(&sh.full[r.i], 0));
@@ -774,6 +774,18 @@ struct LowMaps {
     CUtensorMap x[2], f[2];
 };
 
+// Four values of token m's low.
+__device__ __forceinline__ void put(const LowArgs& a, long long m, int rs, int j, float4 v) {
+    if (a.low) *reinterpret_cast<float4*>(a.low + m * rs + j) = v;
+    if (a.split) {
+        const uint32_t h0 = pack2<__nv_bfloat16>(v.x, v.y), h1 = pack2<__nv_bfloat16>(v.z, v.w);
+        const float2 f0 = unpack2<__nv_bfloat16>(h0), f1 = unpack2<__nv_bfloat16>(h1);
+        uint16_t* to = a.split + m * 2 * rs + j;
+        *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
+        *reinterpret_cast<uint2*>(to + rs) = make_uint2(pack2<__nv_bfloat16>(v.x - f0.x, v.y - f0.y), pack2<__nv_bfloat16>(v.z - f1.x, v.w - f1.y));
+    }
+}
+
 template <class T>
 __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid_constant__ LowMaps maps) {
     using L = LowTile;
@@ -811,7 +823,7 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
     distinct = found;
     const uint32_t tmem = tmem_at;
     const int* list = adapters.list;
-    if (both.after_pack == 2) grid_dependency_wait();
+    if (both.after_pack[blockIdx.z] == 2) grid_dependency_wait();
 
     const int units = distinct * per;
     Ring fill(L::kStages, 1), drain(L::kStages, 0);
@@ -877,8 +889,8 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
                 v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
             }
             const float scale = a.scale ? a.scale[at] : 1.f;
-            const auto put = [&](float f, int jj) { return jj < a.r ? __uint_as_float(to_tf32(scale * f)) : 0.f; };
-            *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + j) = make_float4(put(v.x, j), put(v.y, j + 1), put(v.z, j + 2), put(v.w, j + 3));
+            const auto value = [&](float f, int jj) { return jj < a.r ? __uint_as_float(to_tf32(scale * f)) : 0.f; };
+            put(a, m0 + r, rs, j, make_float4(value(v.x, j), value(v.y, j + 1), value(v.z, j + 2), value(v.w, j + 3)));
         }
         // the sums have been read before the ring's memory is filled again
         fence_async_shared();
@@ -888,17 +900,17 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
     // tokens without an adapter
     for (int i = rank * 256 + threadIdx.x; i < 128 * rs / 4; i += 256 * S) {
         const int r = i / (rs / 4);
-        if (place[r] < 0 && m0 + r < a.n) *reinterpret_cast<float4*>(a.low + (m0 + r) * rs + i % (rs / 4) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (place[r] < 0 && m0 + r < a.n) put(a, m0 + r, rs, i % (rs / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
     }
     if (dead && threadIdx.x == 0) settle();
     __syncthreads();
     if (warp == 1) tmem_free<1>(tmem, L::kCols);
-    if (both.after_pack == 1) grid_dependency_wait();
+    if (both.after_pack[blockIdx.z] == 1) grid_dependency_wait();
 }
 
 template <class T>
-cudaError_t low_tc(const LowArgs* a, int count, int after_pack, int sms, cudaStream_t s) {
-    LowPair both{{a[0], a[count - 1]}, after_pack};
+cudaError_t low_tc(const LowArgs* a, int count, const int* after_pack, int sms, cudaStream_t s) {
+    LowPair both{{a[0], a[count - 1]}, {after_pack[0], after_pack[count - 1]}};
     LowMaps maps{};
     const CUtensorMapDataType ty = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     for (int i = 0; i < count; i++) {
@@ -916,7 +928,7 @@ cudaError_t low_tc(const LowArgs* a, int count, int after_pack, int sms, cudaStr
     const cudaError_t e = ensure_smem(k_low_tc<T>, LowTile::kSmem);
     if (e != cudaSuccess) return e;
     KScope ks("adapter_low", s);
-    return launch_split_y(S, after_pack != 0, k_low_tc<T>, dim3((unsigned)tiles, S, count), 256, LowTile::kSmem, s, both, maps);
+    return launch_split_y(S, after_pack[0] != 0, k_low_tc<T>, dim3((unsigned)tiles, S, count), 256, LowTile::kSmem, s, both, maps);
 }
 
 template <class T, bool W_MN>
@@ -961,7 +973,7 @@ cudaError_t tensor_map(CUtensorMap* out, CUtensorMapDataType type, const void* p
 
 cudaError_t expired_waits_project(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
 
-cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, int after_pack, cudaStream_t s) {
+cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, const int* after_pack, cudaStream_t s) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -53,12 +53,13 @@ struct LowArgs {
     Factor f;
     AdapterIds id;
     const float* scale;
-    float* low;
+    float* low;      // or null
+    uint16_t* split; // or null; bf16 inputs: the same values as two bf16 terms, [n][2][low_stride(r)]
 };
 
 struct LowPair {
     LowArgs a[2];
-    int after_pack;  // launch_low
+    int after_pack[2];  // launch_low
 };
 
 // out[m][o] = base[m][o] + sum_k x[m][k] W(o, k) + bias[o]
@@ -90,7 +91,7 @@ struct GradArgs {
     const void* x;
     long long x_stride;
     int k;
-    const float* low;
+    const void* low;  // LowArgs' split for bf16 x, else its low: rows of 4 low_stride(r) bytes
     void* out;
     long long se, sj, sk;
 };
@@ -137,14 +138,32 @@ constexpr int kSmallTokens = 16;  // up to here W is streamed once past all toke
 // and shared by the tokens of a tile.
 inline bool factor_by_token(long long n, long long o, long long r) { return n * o * r * 2 <= 32ll << 20; }
 
+// Places of the tokens' list that a CTA of the gradients takes: three CTAs for
+// each SM over the tiles of 128 features and up to 64 rank indexes, at least
+// 128 places each.
+inline int grad_ranks(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : (r + 63) / 64 * 64; }  // padded
+inline long long grad_tiles(long long k0, long long k1) { return (k0 + 127) / 128 + (k1 + 127) / 128; }
+constexpr int kGradSms = 148;  // fixed, so that the sums' order is the same on every device
+inline int grad_window(long long n, long long k0, long long k1, int r) {
+    const int sms = kGradSms;
+    const long long ctas = grad_tiles(k0, k1) * (r <= 64 ? 1 : (r + 63) / 64);
+    long long windows = (3 * sms + ctas - 1) / ctas;
+    if (windows > (n + 127) / 128) windows = (n + 127) / 128;
+    return (int)((n + windows * 32 - 1) / (windows * 32) * 32);
+}
+inline uint64_t grad_partial_bytes(long long n, long long k0, long long k1, int r) {
+    const int w = grad_window(n, k0, k1, r);
+    return (uint64_t)((n + w - 1) / w) * 2 * grad_tiles(k0, k1) * 128 * grad_ranks(r) * 4;
+}
+
 cudaError_t launch_pack(const PackJobs& a, cudaStream_t s);
 // one or two of them (the same n, r and id) in one launch; `vec`: rows of x
-// and f start on 16-byte boundaries and f.sk is 1; `after_pack`: launch_pack
-// was queued directly before, and its results are used here (2) or by the
-// next launch only (1), else 0
-cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, int after_pack, cudaStream_t s);
+// and f start on 16-byte boundaries and f.sk is 1; `after_pack`, for each:
+// launch_pack was queued directly before, and its results are used here (2)
+// or by the next launch only (1), else 0
+cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, const int* after_pack, cudaStream_t s);
 // 16-bit types, x and f on 16-byte boundaries, many tokens (k_project.cu)
-cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, int after_pack, cudaStream_t s);
+cudaError_t launch_low_tc(const LowArgs* a, int count, int dtype, const int* after_pack, cudaStream_t s);
 // f32, any strides
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s);
 // 16-bit types, at most kSmallTokens tokens; x and w (not transposed) on 16-byte boundaries
@@ -153,8 +172,8 @@ cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s
 // null where factor_by_token
 cudaError_t launch_project_tc(const ProjectArgs& a, int dtype, cudaStream_t s);
 // rows of x on 16-byte boundaries; `dependent`: launch_project_tc was queued
-// directly before, and behind it what is read here
-cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, cudaStream_t s);
+// directly before, and behind it what is read here; partial: grad_partial_bytes
+cudaError_t launch_grads(const GradPair& a, long long n, int dtype, bool dependent, float* partial, cudaStream_t s);
 // waits of k_project.cu / k_rules.cu that ran out on the current device so far
 cudaError_t expired_waits_project(unsigned long long* out);
 cudaError_t expired_waits_rules(unsigned long long* out);
