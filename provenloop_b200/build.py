@@ -1,6 +1,7 @@
 """Build libtsgpu.so (the CUDA engine behind the C ABI in include/tsgpu.h).
 
-Compiles every CUDA source for sm_100a only, in-tree, with plain nvcc:
+Compiles every CUDA source for sm_100a only, in-tree, with plain nvcc, and
+beside it the checks of the torch entry points (_torch_ops.so, host code):
 
     python -m provenloop_b200.build           # or __graft_entry__.build()
 
@@ -18,6 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtsgpu.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")  # torch tensors to argument blocks (csrc/torch_ops.cpp)
 SOURCES = ["kernels.cu", "k_ntt.cu", "k_encode.cu", "k_encrypt.cu", "k_decrypt.cu", "tsgpu.cu", "noalloc.cu",
            "k_lowrank.cu", "k_project.cu", "k_rules.cu", "decode_ops.cu"]
 HEADERS = ["common.cuh", "ntt.cuh", "fft.cuh", "kernels.cuh", "launch.cuh", "lowrank.cuh",
@@ -43,11 +45,25 @@ def flags(verbose_ptxas: bool = False):
     return f
 
 
+def torch_ops_command(out: str):
+    import sysconfig
+
+    import torch
+    base = os.path.dirname(torch.__file__)
+    inc, libs = os.path.join(base, "include"), os.path.join(base, "lib")
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc,
+            "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
+            "-I", os.path.join(cuda, "include"), os.path.join(CSRC, "torch_ops.cpp"), "-o", out, "-L", libs, "-ltorch_python", "-ltorch",
+            "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_OPS):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, s) for s in SOURCES + HEADERS] + [os.path.join(ROOT, "include", "tsgpu.h")]
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_OPS))
+    deps = [os.path.join(CSRC, s) for s in SOURCES + HEADERS + ["torch_ops.cpp"]] + [os.path.join(ROOT, "include", "tsgpu.h")]
     return any(os.path.getmtime(p) > t for p in deps if os.path.exists(p))
 
 
@@ -65,10 +81,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [nvcc, "-c", os.path.join(CSRC, s), "-o", obj] + flags(verbose)
         procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
         objs.append(obj)
+    procs.append(("torch_ops.cpp", subprocess.Popen(torch_ops_command(TORCH_OPS + ".tmp"), stdout=subprocess.PIPE, stderr=subprocess.PIPE,
+                                                    text=True)))
     for s, p in procs:
         out, err = p.communicate()
         if p.returncode != 0:
-            raise RuntimeError(f"nvcc failed for {s}:\n{out}\n{err}")
+            raise RuntimeError(f"compiling {s} failed:\n{out}\n{err}")
         if verbose:
             sys.stdout.write(out + err)
     tmp = LIB + ".tmp"
@@ -77,6 +95,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
     for o in objs:
         os.remove(o)
     return LIB
