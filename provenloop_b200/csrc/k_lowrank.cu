@@ -266,51 +266,88 @@ __device__ __forceinline__ float low_value(float v) {
     return sizeof(T) == 4 ? v : __uint_as_float(to_tf32(v));
 }
 
-// Token by token: WPJ warps share one rank index of one token.  Bound: reading
+// Token by token: WPJ warps share one rank index of NT neighbouring tokens,
+// whose factor row is read once where they have one adapter.  Bound: reading
 // each token's own factor (r k elements), from L2 where tokens share it.
-template <class T, bool VEC, int WPJ>
+template <class T, bool VEC, int WPJ, int NT>
 __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
     release_dependents();
     if (both.after_pack[blockIdx.z] == 2) grid_dependency_wait();
     const LowArgs a = both.a[blockIdx.z];
-    const long long m = blockIdx.x;
+    const long long m0 = (long long)blockIdx.x * NT;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPJ;
-    const int j = blockIdx.y * (8 / WPJ) + warp / WPJ;
-    const int rs = low_stride(a.r);
-    const int e = a.id.of(m);
-    float v = 0.f;
-    if (e >= 0 && j < a.r) {
-        const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
-        const T* f = static_cast<const T*>(a.f.p) + e * a.f.se + j * a.f.sj;
+    const int j = blockIdx.y * (8 / WPJ) + warp / WPJ, rs = low_stride(a.r);
+    int e[NT];
+    bool one = true;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        e[i] = m0 + i < a.n ? a.id.of(m0 + i) : -1;
+        one &= e[i] == e[0];
+    }
+    float v[NT] = {};
+    const T* f[NT];
+    const T* x[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {  // clamped places: what they give is not kept
+        x[i] = static_cast<const T*>(a.x) + min(m0 + i, a.n - 1) * a.x_stride;
+        f[i] = static_cast<const T*>(a.f.p) + max(e[i], 0) * a.f.se + min(j, a.r - 1) * a.f.sj;
+    }
+    if (!(one && e[0] < 0)) {
         if constexpr (VEC) {
             constexpr int V = 16 / sizeof(T);
             int k = (part * 32 + lane) * V;
+            if (one) {
 #pragma unroll 4
-            for (; k + V <= a.k; k += 32 * V * WPJ) v = dot16<T>(whole16(x, k), whole16(f, k), v);
-            if (k < a.k) v = dot16<T>(load16(x, k, a.k), load16(f, k, a.k), v);
+                for (; k + V <= a.k; k += 32 * V * WPJ) {
+                    const uint4 fk = whole16(f[0], k);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) v[i] = dot16<T>(whole16(x[i], k), fk, v[i]);
+                }
+            } else {
+#pragma unroll 2
+                for (; k + V <= a.k; k += 32 * V * WPJ)
+#pragma unroll
+                    for (int i = 0; i < NT; i++) v[i] = dot16<T>(whole16(x[i], k), whole16(f[i], k), v[i]);
+            }
+            if (k < a.k)
+#pragma unroll
+                for (int i = 0; i < NT; i++) v[i] = dot16<T>(load16(x[i], k, a.k), load16(f[i], k, a.k), v[i]);
         } else {
 #pragma unroll 4
-            for (int k = part * 32 + lane; k < a.k; k += 32 * WPJ) v = fmaf(to_f(x[k]), to_f(f[k * a.f.sk]), v);
+            for (int k = part * 32 + lane; k < a.k; k += 32 * WPJ)
+#pragma unroll
+                for (int i = 0; i < NT; i++) v[i] = fmaf(to_f(x[i][k]), to_f(f[i][k * a.f.sk]), v[i]);
         }
 #pragma unroll
-        for (int q = 16; q; q >>= 1) v += __shfl_xor_sync(0xffffffffu, v, q);
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int q = 16; q; q >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], q);
     }
     if constexpr (WPJ > 1) {
-        __shared__ float part_sum[8];
-        if (lane == 0) part_sum[warp] = v;
-        __syncthreads();
-        if (part == 0) {
-            v = 0.f;
+        __shared__ float part_sum[8][NT];
+        if (lane == 0)
 #pragma unroll
-            for (int q = 0; q < WPJ; q++) v += part_sum[warp + q];
-        }
+            for (int i = 0; i < NT; i++) part_sum[warp][i] = v[i];
+        __syncthreads();
+        if (part == 0)
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                v[i] = 0.f;
+#pragma unroll
+                for (int q = 0; q < WPJ; q++) v[i] += part_sum[warp + q][i];
+            }
     }
     if (part == 0 && lane == 0 && j < rs) {
-        const float low = e >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e] * v : v) : 0.f;
-        if (a.low) a.low[m * rs + j] = low;
-        if (a.split) {
-            const __nv_bfloat16 h = __float2bfloat16_rn(low), l = __float2bfloat16_rn(low - __bfloat162float(h));
-            a.split[m * 2 * rs + j] = __bfloat16_as_ushort(h), a.split[(m * 2 + 1) * rs + j] = __bfloat16_as_ushort(l);
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const long long m = m0 + i;
+            if (m >= a.n) break;
+            const float low = e[i] >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e[i]] * v[i] : v[i]) : 0.f;
+            if (a.low) a.low[m * rs + j] = low;
+            if (a.split) {
+                const __nv_bfloat16 h = __float2bfloat16_rn(low), l = __float2bfloat16_rn(low - __bfloat162float(h));
+                a.split[m * 2 * rs + j] = __bfloat16_as_ushort(h), a.split[(m * 2 + 1) * rs + j] = __bfloat16_as_ushort(l);
+            }
         }
     }
     // the next launch waits for this one, and with it for the packing
@@ -319,62 +356,145 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
 
 // ---------------------------------------------------------------- projection
 
-// f32: 64 x 64 outputs per CTA, 4 x 4 per thread, 16 of the contraction at a
-// time.
-__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a) {
-    constexpr int BM = 64, BN = 64, BK = 16;
-    __shared__ float xs[BK][BM + 1], ws[BK][BN + 1];
-    const long long m0 = (long long)blockIdx.x * BM;
+// f32: BM x BN outputs per CTA, TM x TN per thread in two halves, 16 of the
+// contraction at a time, the next ones on their way in registers.  A cluster
+// of S CTAs shares the contraction where the tiles are few, and each finishes
+// BM / S of the rows.  On the FMA pipe: the tensor cores' TF32 would need
+// three products and rounds its sums towards zero.
+template <int BM, int BN, int TM, int TN>
+__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int vec_x, int vec_w) {
+    constexpr int BK = 16, LX = BM * BK / 1024, LW = BN * BK / 1024;  // float4 loads of a thread
+    static_assert((BM / TM) * (BN / TN) == 256, "one thread per TM x TN outputs");
+    __shared__ __align__(16) float xs[2][BK][BM + 4], ws[2][BK][BN + 4];
+    constexpr bool kShared = BM == 64;  // the contraction may be shared
+    __shared__ float part[kShared ? BM : 1][BN + 1];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const long long m0 = (long long)(blockIdx.x / S) * BM;
     const int o0 = blockIdx.y * BN;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
+    constexpr int TX = BN / TN;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    float acc[TM][TN] = {};
     if (a.w) {
         const float* x = static_cast<const float*>(a.x);
         const float* w = static_cast<const float*>(a.w);
-        const long long w_so = a.w_t ? 1 : a.w_stride, w_sk = a.w_t ? a.w_stride : 1;
-        for (int k0 = 0; k0 < a.k; k0 += BK) {
-            for (int i = threadIdx.x; i < BM * BK; i += 256) {
-                const int k = i % BK, m = i / BK;
-                xs[k][m] = m0 + m < a.n && k0 + k < a.k ? x[(m0 + m) * a.x_stride + k0 + k] : 0.f;
+        const int blocks = (a.k + BK - 1) / BK, b0 = blocks * rank / S, b1 = blocks * (rank + 1) / S;
+        float4 nx[LX], nw[LW];
+        // four neighbours of a row that ends at `n`, from a clamped place
+        const auto quad = [](const float* row, int at, int n, bool in, bool vec) {
+            if (vec && in && at + 4 <= n) return *reinterpret_cast<const float4*>(row + at);
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = row[min(at + i, n - 1)];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!in || at + i >= n) v[i] = 0.f;
+            return make_float4(v[0], v[1], v[2], v[3]);
+        };
+        const auto load = [&](int b) {
+            const int k0 = b * BK;
+#pragma unroll
+            for (int i = 0; i < LX; i++) {
+                const int q = threadIdx.x + 256 * i;
+                const long long m = m0 + q / 4;
+                nx[i] = quad(x + min(m, a.n - 1) * a.x_stride, k0 + q % 4 * 4, a.k, m < a.n, vec_x);
             }
-            for (int i = threadIdx.x; i < BN * BK; i += 256) {
-                // consecutive threads along whichever axis of W is contiguous
-                const int k = a.w_t ? i / BN : i % BK, o = a.w_t ? i % BN : i / BK;
-                ws[k][o] = o0 + o < a.o && k0 + k < a.k ? w[(o0 + o) * w_so + (k0 + k) * w_sk] : 0.f;
+#pragma unroll
+            for (int i = 0; i < LW; i++) {
+                const int q = threadIdx.x + 256 * i;
+                if (a.w_t) {
+                    const int k = k0 + q / (BN / 4);
+                    nw[i] = quad(w + (long long)min(k, a.k - 1) * a.w_stride, o0 + q % (BN / 4) * 4, a.o, k < a.k, vec_w);
+                } else {
+                    const int o = o0 + q / 4;
+                    nw[i] = quad(w + (long long)min(o, a.o - 1) * a.w_stride, k0 + q % 4 * 4, a.k, o < a.o, vec_w);
+                }
             }
+        };
+        const auto store = [&](int s) {
+#pragma unroll
+            for (int i = 0; i < LX; i++) {
+                const int q = threadIdx.x + 256 * i, m = q / 4, k = q % 4 * 4;
+                xs[s][k][m] = nx[i].x, xs[s][k + 1][m] = nx[i].y, xs[s][k + 2][m] = nx[i].z, xs[s][k + 3][m] = nx[i].w;
+            }
+#pragma unroll
+            for (int i = 0; i < LW; i++) {
+                const int q = threadIdx.x + 256 * i;
+                if (a.w_t) {
+                    *reinterpret_cast<float4*>(&ws[s][q / (BN / 4)][q % (BN / 4) * 4]) = nw[i];
+                } else {
+                    const int o = q / 4, k = q % 4 * 4;
+                    ws[s][k][o] = nw[i].x, ws[s][k + 1][o] = nw[i].y, ws[s][k + 2][o] = nw[i].z, ws[s][k + 3][o] = nw[i].w;
+                }
+            }
+        };
+        if (b0 < b1) {
+            load(b0);
+            store(0);
             __syncthreads();
+            for (int b = b0; b < b1; b++) {
+                const int s = (b - b0) & 1;
+                if (b + 1 < b1) load(b + 1);
 #pragma unroll
-            for (int k = 0; k < BK; k++) {
-                float xv[4], wv[4];
+                for (int k = 0; k < BK; k++) {
+                    float xv[TM], wv[TN];
 #pragma unroll
-                for (int i = 0; i < 4; i++) xv[i] = xs[k][ty + 16 * i], wv[i] = ws[k][tx + 16 * i];
+                    for (int i = 0; i < TM; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&xs[s][k][ty * 4 + i / 4 * (BM / (TM / 4))]);
+                        xv[i] = f.x, xv[i + 1] = f.y, xv[i + 2] = f.z, xv[i + 3] = f.w;
+                    }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < TN; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&ws[s][k][tx * 4 + i / 4 * (BN / (TN / 4))]);
+                        wv[i] = f.x, wv[i + 1] = f.y, wv[i + 2] = f.z, wv[i + 3] = f.w;
+                    }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+                    for (int i = 0; i < TM; i++)
+#pragma unroll
+                        for (int j = 0; j < TN; j++) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+                }
+                if (b + 1 < b1) store(s ^ 1);
+                __syncthreads();
             }
-            __syncthreads();
         }
     }
     const int rs = low_stride(a.r);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const long long m = m0 + ty + 16 * i;
-        if (m >= a.n) continue;
+    const auto finish = [&](long long m, int o, float v) {
+        if (a.bias) v += static_cast<const float*>(a.bias)[o];
+        if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
         const int e = a.id.of(m);
-        const float* low = a.low + m * rs;
-        const float* g = static_cast<const float*>(a.g.p) + (e < 0 ? 0 : e) * a.g.se;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int o = o0 + tx + 16 * j;
-            if (o >= a.o) continue;
-            float v = acc[i][j];
-            if (a.bias) v += static_cast<const float*>(a.bias)[o];
-            if (e >= 0)
-                for (int q = 0; q < a.r; q++) v = fmaf(low[q], g[q * a.g.sj + o * a.g.sk], v);
-            if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
-            static_cast<float*>(a.out)[m * a.out_stride + o] = v;
+        if (e >= 0) {
+            const float* low = a.low + m * rs;
+            const float* g = static_cast<const float*>(a.g.p) + e * a.g.se + o * a.g.sk;
+#pragma unroll 8
+            for (int j = 0; j < a.r; j++) v = fmaf(low[j], g[j * a.g.sj], v);
         }
+        static_cast<float*>(a.out)[m * a.out_stride + o] = v;
+    };
+    const auto row_of = [&](int i) { return ty * 4 + i / 4 * (BM / (TM / 4)) + i % 4; };
+    const auto col_of = [&](int j) { return tx * 4 + j / 4 * (BN / (TN / 4)) + j % 4; };
+    if constexpr (kShared) {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) part[row_of(i)][col_of(j)] = acc[i][j];
+        if (S > 1) cluster.sync();
+        else __syncthreads();
+        const int rows = BM / S;
+        for (int q = threadIdx.x; q < rows * BN; q += 256) {
+            const int row = rank * rows + q / BN, col = q % BN;
+            if (m0 + row >= a.n || o0 + col >= a.o) continue;
+            float v = 0.f;
+            for (int c = 0; c < S; c++) v += S > 1 ? *cluster.map_shared_rank(&part[row][col], c) : part[row][col];
+            finish(m0 + row, o0 + col, v);
+        }
+        if (S > 1) cluster.sync();
+    } else {
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+                if (m0 + row_of(i) < a.n && o0 + col_of(j) < a.o) finish(m0 + row_of(i), o0 + col_of(j), acc[i][j]);
     }
 }
 
@@ -756,12 +876,19 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, const int* after_p
     KScope ks("adapter_low", s);
     // long contractions over more warps, to have more loads in flight
     const int rs = low_stride(a[0].r);
-    const auto go = [&](auto kern, int ranks) {
-        const dim3 grid((unsigned)n, (rs + ranks - 1) / ranks, count);
+    const auto go = [&](auto kern, int ranks, int tokens) {
+        const dim3 grid((unsigned)((n + tokens - 1) / tokens), (rs + ranks - 1) / ranks, count);
         return after_pack[0] ? launch_dependent(1, kern, grid, 256, 0, s, both) : launch_cl(1, kern, grid, 256, 0, s, both);
     };
-    if (kmax * sizeof(T) > 4096) return vec ? go(k_low_token<T, true, 4>, 2) : go(k_low_token<T, false, 4>, 2);
-    return vec ? go(k_low_token<T, true, 1>, 8) : go(k_low_token<T, false, 1>, 8);
+    // four tokens a warp once that leaves eight CTAs for every SM (48 tokens with
+    // adapters of their own over 8960: 8 us one by one, 16 us by fours)
+    const bool longk = kmax * sizeof(T) > 4096;
+    if (n * rs / (longk ? 8 : 32) >= 8 * sm_count()) {
+        if (longk) return vec ? go(k_low_token<T, true, 4, 4>, 2, 4) : go(k_low_token<T, false, 4, 4>, 2, 4);
+        return vec ? go(k_low_token<T, true, 1, 4>, 8, 4) : go(k_low_token<T, false, 1, 4>, 8, 4);
+    }
+    if (longk) return vec ? go(k_low_token<T, true, 4, 1>, 2, 1) : go(k_low_token<T, false, 4, 1>, 2, 1);
+    return vec ? go(k_low_token<T, true, 1, 1>, 8, 1) : go(k_low_token<T, false, 1, 1>, 8, 1);
 }
 
 template <class T, int NB, int MT>
@@ -831,9 +958,16 @@ cudaError_t launch_low(const LowArgs* a, int count, int dtype, bool vec, const i
 }
 
 cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
+    const auto vec = [](const void* p, long long stride, long long rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows < 2 || stride % 4 == 0); };
+    const int vx = vec(a.x, a.x_stride, a.n), vw = vec(a.w, a.w_stride, a.w_t ? a.k : a.o);
     KScope ks("adapter_project", s);
-    k_project_f32<<<dim3((unsigned)((a.n + 63) / 64), (a.o + 63) / 64), 256, 0, s>>>(a);
-    return cudaGetLastError();
+    // large tiles where they fill the SMs, else small ones whose contraction
+    // is shared until they do, 64 of it for each CTA at least
+    const long long large = ((a.n + 127) / 128) * ((a.o + 127) / 128), small = ((a.n + 63) / 64) * ((a.o + 63) / 64);
+    if (large >= sm_count()) return launch_cl(1, k_project_f32<128, 128, 8, 8>, dim3((unsigned)((a.n + 127) / 128), (a.o + 127) / 128), 256, 0, s, a, vx, vw);
+    int S = 1;
+    while (S < 8 && a.w && small * S < 2 * sm_count() && a.k >= 128 * S) S *= 2;
+    return launch_cl(S, k_project_f32<64, 64, 4, 4>, dim3((unsigned)((a.n + 63) / 64 * S), (a.o + 63) / 64), 256, 0, s, a, vx, vw);
 }
 
 cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s) {
