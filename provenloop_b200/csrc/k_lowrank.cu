@@ -501,8 +501,8 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
 // sum_j low[j] b[j] for a row of a factor; 16 bytes at a time where r and the
 // row allow, else 4, else 2.
 template <class T>
-__device__ __forceinline__ float dot_low(const float* low, const T* b, long long sj, int r, float v) {
-    if (sj == 1 && (r & 7) == 0 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+__device__ __forceinline__ float dot_low(const float* low, const T* b, int r, float v) {
+    if ((r & 7) == 0 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll 4
         for (int j = 0; j < r; j += 8) {
             const uint4 u = *reinterpret_cast<const uint4*>(b + j);
@@ -511,98 +511,105 @@ __device__ __forceinline__ float dot_low(const float* low, const T* b, long long
             v = fmaf(p.x, f0.x, v), v = fmaf(p.y, f0.y, v), v = fmaf(p.z, f1.x, v), v = fmaf(p.w, f1.y, v);
             v = fmaf(q.x, f2.x, v), v = fmaf(q.y, f2.y, v), v = fmaf(q.z, f3.x, v), v = fmaf(q.w, f3.y, v);
         }
-    } else if (sj == 1 && (r & 1) == 0 && (reinterpret_cast<uintptr_t>(b) & 3) == 0) {
-#pragma unroll 16
-        for (int j = 0; j < r; j += 2) {
-            const float2 f = pair_f<T>(*reinterpret_cast<const uint32_t*>(b + j));
-            v = fmaf(low[j], f.x, v), v = fmaf(low[j + 1], f.y, v);
+    } else if ((r & 1) == 0 && (reinterpret_cast<uintptr_t>(b) & 3) == 0) {
+        // blocks of unconditional loads, from clamped places behind the last rank
+        for (int j = 0; j < r; j += 16) {
+            float2 l[8];
+            uint32_t q[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int at = min(j + 2 * i, r - 2);
+                q[i] = *reinterpret_cast<const uint32_t*>(b + at), l[i] = *reinterpret_cast<const float2*>(low + at);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float2 f = pair_f<T>(q[i]);
+                if (j + 2 * i < r) v = fmaf(l[i].x, f.x, v), v = fmaf(l[i].y, f.y, v);
+            }
         }
     } else {
-#pragma unroll 16
-        for (int j = 0; j < r; j++) v = fmaf(low[j], to_f(b[j * sj]), v);
+        for (int j = 0; j < r; j += 8) {
+            float l[8], f[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) l[i] = low[min(j + i, r - 1)], f[i] = to_f(b[min(j + i, r - 1)]);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (j + i < r) v = fmaf(l[i], f[i], v);
+        }
     }
     return v;
 }
 
-// Few tokens: a cluster of S CTAs streams 16 MT rows of W once past NB * 8
+// Few tokens: a cluster of S CTAs streams 16 rows of W once past NB * 8
 // tokens, its 8 S warps sharing the contraction in 32-wide blocks.  Operands go
 // from global memory to the matrix instructions' registers: a thread's 16
 // bytes of a row are the k indexes of two instructions, in the same (permuted)
-// order for W and x.  Bound: reading W, and with many
-// tokens the re-reads of x, which MT = 2 halves; the stream starts before low
-// is there, and waits for it only to add the adapters' terms.
-template <class T, int NB, int MT>
+// order for W and x.  Bound: reading W, and the launch's latency; the stream
+// starts before low is there, and waits for it only to add the adapters' terms.
+template <class T, int NB>
 __global__ void __launch_bounds__(256) k_project_small(const ProjectArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int o0 = (blockIdx.x / S) * 16 * MT;
-    const long long m0 = (long long)blockIdx.y * NB * 8;
+    const int o0 = (blockIdx.x / S) * 16;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    extern __shared__ float red[];  // [8][16 MT][RS], the sums over the warps in the first
+    extern __shared__ float red[];  // [8][16][RS], the sums over the warps in the first
     constexpr int RS = NB * 8 + 1;
     if (a.w) {
-        float acc[MT][NB][4] = {};
-        const T* wr[2 * MT];
+        float acc[NB][4] = {};
+        const T* wr[2];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; i++) wr[i] = static_cast<const T*>(a.w) + (long long)min(o0 + g + 8 * i, a.o - 1) * a.w_stride;
+        for (int i = 0; i < 2; i++) wr[i] = static_cast<const T*>(a.w) + (long long)min(o0 + g + 8 * i, a.o - 1) * a.w_stride;
         const T* xr[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min(m0 + nb * 8 + g, a.n - 1) * a.x_stride;
+        for (int nb = 0; nb < NB; nb++) xr[nb] = static_cast<const T*>(a.x) + min((long long)nb * 8 + g, a.n - 1) * a.x_stride;
         const auto block = [&](auto load, int k) {
-            uint4 w[2 * MT], x[NB];
+            uint4 w[2], x[NB];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; i++) w[i] = load(wr[i], k);
+            for (int i = 0; i < 2; i++) w[i] = load(wr[i], k);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) x[nb] = load(xr[nb], k);
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    mma16<T>(acc[i][nb], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, x[nb].x, x[nb].y);
-                    mma16<T>(acc[i][nb], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, x[nb].z, x[nb].w);
-                }
+            for (int nb = 0; nb < NB; nb++) {
+                mma16<T>(acc[nb], w[0].x, w[1].x, w[0].y, w[1].y, x[nb].x, x[nb].y);
+                mma16<T>(acc[nb], w[0].z, w[1].z, w[0].w, w[1].w, x[nb].z, x[nb].w);
+            }
         };
         int k = (rank * 8 + warp) * 32;
-        constexpr int kUnroll = NB * MT >= 8 ? 2 : 4;
-#pragma unroll kUnroll
+#pragma unroll 4
         for (; k + 32 <= a.k; k += S * 256) block([](const T* row, int at) { return whole16(row, at); }, k + 8 * t);
         if (k < a.k) block([&](const T* row, int at) { return load16(row, at, a.k); }, k + 8 * t);
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    red[(warp * 16 * MT + i * 16 + g + (c >> 1) * 8) * RS + nb * 8 + 2 * t + (c & 1)] = acc[i][nb][c];
+            for (int c = 0; c < 4; c++) red[(warp * 16 + g + (c >> 1) * 8) * RS + nb * 8 + 2 * t + (c & 1)] = acc[nb][c];
         __syncthreads();
         if (S > 1) {
-            for (int i = threadIdx.x; i < 16 * MT * NB * 8; i += 256) {
+            for (int i = threadIdx.x; i < 16 * NB * 8; i += 256) {
                 float* p = red + (i / (NB * 8)) * RS + i % (NB * 8);
                 float v = 0.f;
 #pragma unroll
-                for (int q = 0; q < 8; q++) v += p[q * 16 * MT * RS];
+                for (int q = 0; q < 8; q++) v += p[q * 16 * RS];
                 *p = v;
             }
             cluster.sync();
         }
     }
     grid_dependency_wait();
-    const int rs = low_stride(a.r), per = 16 * MT * NB * 8 / S;
+    const int rs = low_stride(a.r), per = 16 * NB * 8 / S;
     for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += 256) {
-        const int row = i % (16 * MT), col = i / (16 * MT), o = o0 + row;
-        const long long m = m0 + col;
+        const int row = i % 16, m = i / 16, o = o0 + row;
         if (o >= a.o || m >= a.n) continue;
         float v = a.bias ? to_f(static_cast<const T*>(a.bias)[o]) : 0.f;
         if (a.base) v += to_f(static_cast<const T*>(a.base)[m * a.base_stride + o]);
         const int e = a.id.of(m);
-        if (e >= 0) v = dot_low(a.low + m * rs, static_cast<const T*>(a.g.p) + e * a.g.se + o * a.g.sk, a.g.sj, a.r, v);
+        if (e >= 0) v = dot_low(a.low + m * rs, static_cast<const T*>(a.g.p) + e * a.g.se + o * a.g.sk, a.r, v);
         if (a.w) {
-            float* p = red + row * RS + col;
+            float* p = red + row * RS + m;
             if (S > 1)
                 for (int q = 0; q < S; q++) v += *cluster.map_shared_rank(p, q);
             else
 #pragma unroll
-                for (int q = 0; q < 8; q++) v += p[q * 16 * MT * RS];
+                for (int q = 0; q < 8; q++) v += p[q * 16 * RS];
         }
         static_cast<T*>(a.out)[m * a.out_stride + o] = from_f<T>(v);
     }
@@ -891,27 +898,21 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, const int* after_p
     return vec ? go(k_low_token<T, true, 1, 1>, 8, 1) : go(k_low_token<T, false, 1, 1>, 8, 1);
 }
 
-template <class T, int NB, int MT>
+template <class T, int NB>
 cudaError_t small_launch(const ProjectArgs& a, cudaStream_t s) {
     // as many CTAs share a contraction as it takes to give every SM one,
     // while each of their warps has four blocks
-    const long long tiles = (long long)((a.o + 16 * MT - 1) / (16 * MT)) * ((a.n + NB * 8 - 1) / (NB * 8));
+    const int tiles = (a.o + 15) / 16;
     int S = 1;
     while (S < 8 && a.w && tiles * S < sm_count() && a.k >= S * 2048) S *= 2;
-    const size_t smem = (size_t)8 * 16 * MT * (NB * 8 + 1) * 4;
-    const dim3 grid((unsigned)((a.o + 16 * MT - 1) / (16 * MT) * S), (unsigned)((a.n + NB * 8 - 1) / (NB * 8)));
+    const size_t smem = (size_t)8 * 16 * (NB * 8 + 1) * 4;
     KScope ks("adapter_project", s);
-    const cudaError_t e = ensure_smem(k_project_small<T, NB, MT>, smem);
-    return e != cudaSuccess ? e : launch_dependent(S, k_project_small<T, NB, MT>, grid, 256, smem, s, a);
+    const cudaError_t e = ensure_smem(k_project_small<T, NB>, smem);
+    return e != cudaSuccess ? e : launch_dependent(S, k_project_small<T, NB>, dim3((unsigned)(tiles * S)), 256, smem, s, a);
 }
 
 template <class T>
-cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) {
-    if (a.n <= 8) return small_launch<T, 1, 1>(a, s);
-    if (a.n <= 16) return small_launch<T, 2, 1>(a, s);
-    if (a.n <= 32) return small_launch<T, 4, 1>(a, s);
-    return small_launch<T, 8, 2>(a, s);
-}
+cudaError_t small_width(const ProjectArgs& a, cudaStream_t s) { return a.n <= 8 ? small_launch<T, 1>(a, s) : small_launch<T, 2>(a, s); }
 
 template <class T, int RB>
 cudaError_t grad_launch(const GradPair& a, long long n, bool dependent, float* partial, cudaStream_t s) {

@@ -520,20 +520,24 @@ cudaError_t launch_tile(const ProjectArgs& p, int sms, cudaStream_t s) {
     return launch_dependent(CG, kern, dim3((unsigned)(tiles < slots ? tiles : slots) * CG), kThreads, L::kSmem, s, a, mx, mw, mg, mout, mbase);
 }
 
-// v[z] += sum_j low[j] G(j, o + z) for eight neighbouring outputs: the
-// factor's 16 bytes along whichever axis is contiguous, else its elements.
-template <class T>
-__device__ __forceinline__ void add_low(const ProjectArgs& p, const float* low, const T* g, int o, float (&v)[8]) {
-    const bool whole = o + 8 <= p.o;
+// v[z] += sum_j low[j] G(j, o + z) for N neighbouring outputs: the factor's
+// widest loads along whichever axis is contiguous, else its elements.
+template <class T, int N>
+__device__ __forceinline__ void add_low(const ProjectArgs& p, const float* low, const T* g, int o, float (&v)[N]) {
     const T* at = g + o * p.g.sk;
-    if (p.g.sk == 1 && whole && (p.g.sj & 7) == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+    if (p.g.sk == 1 && o + N <= p.o && p.g.sj % N == 0 && reinterpret_cast<uintptr_t>(at) % (2 * N) == 0) {
 #pragma unroll 8
         for (int j = 0; j < p.r; j++) {
-            const uint4 q = *reinterpret_cast<const uint4*>(at + j * p.g.sj);
+            uint32_t u[N / 2];
+            if constexpr (N == 8) {
+                const uint4 q = *reinterpret_cast<const uint4*>(at + j * p.g.sj);
+                u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
+            } else {
+                u[0] = *reinterpret_cast<const uint32_t*>(at + j * p.g.sj);
+            }
             const float l = low[j];
-            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int z = 0; z < 4; z++) {
+            for (int z = 0; z < N / 2; z++) {
                 const float2 f = unpack2<T>(u[z]);
                 v[2 * z] = fmaf(l, f.x, v[2 * z]), v[2 * z + 1] = fmaf(l, f.y, v[2 * z + 1]);
             }
@@ -542,37 +546,54 @@ __device__ __forceinline__ void add_low(const ProjectArgs& p, const float* low, 
 #pragma unroll 2
         for (int j = 0; j < p.r; j += 8) {
             const float4 l0 = *reinterpret_cast<const float4*>(low + j), l1 = *reinterpret_cast<const float4*>(low + j + 4);
-            uint4 q[8];
+            uint4 q[N];
 #pragma unroll
-            for (int z = 0; z < 8; z++) q[z] = *reinterpret_cast<const uint4*>(g + min(o + z, p.o - 1) * p.g.sk + j);
+            for (int z = 0; z < N; z++) q[z] = *reinterpret_cast<const uint4*>(g + min(o + z, p.o - 1) * p.g.sk + j);
 #pragma unroll
-            for (int z = 0; z < 8; z++) {
+            for (int z = 0; z < N; z++) {
                 const float2 f0 = unpack2<T>(q[z].x), f1 = unpack2<T>(q[z].y), f2 = unpack2<T>(q[z].z), f3 = unpack2<T>(q[z].w);
                 v[z] = fmaf(l0.x, f0.x, v[z]), v[z] = fmaf(l0.y, f0.y, v[z]), v[z] = fmaf(l0.z, f1.x, v[z]), v[z] = fmaf(l0.w, f1.y, v[z]);
                 v[z] = fmaf(l1.x, f2.x, v[z]), v[z] = fmaf(l1.y, f2.y, v[z]), v[z] = fmaf(l1.z, f3.x, v[z]), v[z] = fmaf(l1.w, f3.y, v[z]);
             }
         }
     } else if (p.g.sj == 1 && (p.r & 1) == 0 && (reinterpret_cast<uintptr_t>(g) & 3) == 0) {
-#pragma unroll 4
-        for (int j = 0; j < p.r; j += 2) {
-            const float2 l = *reinterpret_cast<const float2*>(low + j);
-            uint32_t q[8];
+        // blocks of whole unconditional loads, from clamped places behind the last rank
+        constexpr int B = N == 8 ? 4 : 8;
+        for (int j = 0; j < p.r; j += 2 * B) {
+            float2 l[B];
+            uint32_t q[B][N];
 #pragma unroll
-            for (int z = 0; z < 8; z++) q[z] = *reinterpret_cast<const uint32_t*>(g + min(o + z, p.o - 1) * p.g.sk + j);
+            for (int b = 0; b < B; b++) {
+                const int at = min(j + 2 * b, p.r - 2);
+                l[b] = *reinterpret_cast<const float2*>(low + at);
 #pragma unroll
-            for (int z = 0; z < 8; z++) {
-                const float2 f = unpack2<T>(q[z]);
-                v[z] = fmaf(l.x, f.x, v[z]), v[z] = fmaf(l.y, f.y, v[z]);
+                for (int z = 0; z < N; z++) q[b][z] = *reinterpret_cast<const uint32_t*>(g + min(o + z, p.o - 1) * p.g.sk + at);
             }
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (j + 2 * b < p.r)
+#pragma unroll
+                    for (int z = 0; z < N; z++) {
+                        const float2 f = unpack2<T>(q[b][z]);
+                        v[z] = fmaf(l[b].x, f.x, v[z]), v[z] = fmaf(l[b].y, f.y, v[z]);
+                    }
         }
     } else {
-#pragma unroll 4
-        for (int j = 0; j < p.r; j++) {
-            float f[8];
+        constexpr int B = N == 8 ? 4 : 8;
+        for (int j = 0; j < p.r; j += B) {
+            float l[B], f[B][N];
 #pragma unroll
-            for (int z = 0; z < 8; z++) f[z] = elem<T>(g, j * p.g.sj + min(o + z, p.o - 1) * p.g.sk);
+            for (int b = 0; b < B; b++) {
+                const int at = min(j + b, p.r - 1);
+                l[b] = low[at];
 #pragma unroll
-            for (int z = 0; z < 8; z++) v[z] = fmaf(low[j], f[z], v[z]);
+                for (int z = 0; z < N; z++) f[b][z] = elem<T>(g, at * p.g.sj + min(o + z, p.o - 1) * p.g.sk);
+            }
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (j + b < p.r)
+#pragma unroll
+                    for (int z = 0; z < N; z++) v[z] = fmaf(l[b], f[b][z], v[z]);
         }
     }
 }
@@ -580,17 +601,86 @@ __device__ __forceinline__ void add_low(const ProjectArgs& p, const float* low, 
 // Not enough tiles for all SMs: a cluster of S CTAs shares the contraction of
 // a 128 x BN tile, each with a ring of its own, and the partial sums meet in
 // shared memory, where each CTA finishes BN / S of the outputs.  Each token
-// takes its own adapter's factor straight from L2 (n o r elements in all), so
-// that nothing is converted first.  Bound: reading W once by all SMs together,
-// and the launches' latency.  Without W only the last part runs.
+// takes its own adapter's factor straight from memory (n o r elements in all),
+// so that nothing is converted first.  Where a CTA's share is small, the six
+// warps that neither load nor multiply compute these terms meanwhile.  Bound:
+// reading W once by all SMs together, and the launches' latency.
 template <int BN>
 struct SplitTile {
     static constexpr int kStages = BN == 64 ? 4 : 3;
     static constexpr int kStage = 128 * 128 + BN * 128;
     static constexpr int kRow = BN + 4;  // floats: rows of the partial sums four banks apart
-    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kEarly = 2048;  // outputs of a CTA whose other terms are computed during the contraction
+    static constexpr int kSmem = kStages * kStage + kEarly * 4 + 1024;
     static_assert(128 * kRow * 4 <= kStages * kStage, "the sums fit where the ring was");
 };
+
+// Bias, base and the adapter's term of N neighbouring outputs of token m.
+template <class T, int N>
+__device__ __forceinline__ void other_terms(const ProjectArgs& p, long long m, int o, float (&v)[N]) {
+    const int e = p.id.of(m);
+    if (p.bias) {
+#pragma unroll
+        for (int z = 0; z < N; z++) v[z] += elem<T>(p.bias, min(o + z, p.o - 1));
+    }
+    if (p.base) {
+        const T* base = static_cast<const T*>(p.base) + m * p.base_stride + o;
+        if (o + N <= p.o && reinterpret_cast<uintptr_t>(base) % (2 * N) == 0) {
+            uint32_t u[N / 2];
+            if constexpr (N == 8) {
+                const uint4 q = *reinterpret_cast<const uint4*>(base);
+                u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
+            } else {
+                u[0] = *reinterpret_cast<const uint32_t*>(base);
+            }
+#pragma unroll
+            for (int z = 0; z < N / 2; z++) {
+                const float2 f = unpack2<T>(u[z]);
+                v[2 * z] += f.x, v[2 * z + 1] += f.y;
+            }
+        } else {
+#pragma unroll
+            for (int z = 0; z < N; z++) v[z] += elem<T>(base, min(z, p.o - 1 - o));
+        }
+    }
+    if (e >= 0) add_low<T, N>(p, p.low + m * low_stride(p.r), static_cast<const T*>(p.g.p) + e * p.g.se, o, v);
+}
+
+template <class T, int N>
+__device__ __forceinline__ void put_outputs(const ProjectArgs& p, long long m, int o, const float (&v)[N]) {
+    T* out = static_cast<T*>(p.out) + m * p.out_stride + o;
+    uint32_t u[N / 2];
+#pragma unroll
+    for (int z = 0; z < N / 2; z++) u[z] = pack2<T>(v[2 * z], v[2 * z + 1]);
+    if (o + N <= p.o && reinterpret_cast<uintptr_t>(out) % (2 * N) == 0) {
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+        else *reinterpret_cast<uint32_t*>(out) = u[0];
+    } else {
+        const T* h = reinterpret_cast<const T*>(u);
+#pragma unroll
+        for (int z = 0; z < N; z++)
+            if (o + z < p.o) out[z] = h[z];
+    }
+}
+
+// v[z] += the partial sums of all CTAs of the cluster.
+template <int N>
+__device__ __forceinline__ void add_sums(const float* f, int S, float (&v)[N]) {
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+        if (q >= S) break;
+        if constexpr (N == 2) {
+            const float2 w = ld_cluster2(map_rank(f, q));
+            v[0] += w.x, v[1] += w.y;
+        } else {
+#pragma unroll
+            for (int z = 0; z < N; z += 4) {
+                const float4 w = ld_cluster4(map_rank(f + z, q));
+                v[z] += w.x, v[z + 1] += w.y, v[z + 2] += w.z, v[z + 3] += w.w;
+            }
+        }
+    }
+}
 
 template <class T, int BN, bool W_MN>
 __global__ void __launch_bounds__(256)
@@ -601,159 +691,147 @@ k_project_split(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __
     __shared__ uint32_t tmem_at, dead;
     const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
     float* sums = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));  // [128][kRow], when the ring is done with
+    float* terms = sums + L::kStages * L::kStage / 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ProjectArgs& p = a.p;
     const int S = a.split, rank = (int)cluster_rank();
-    const int m0 = blockIdx.y * 128, o0 = blockIdx.x / S * BN;
-    if (a.kblocks) {
-        const int kb0 = a.kblocks * rank / S, kb1 = a.kblocks * (rank + 1) / S;
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < L::kStages; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-            mbar_init(&done, 1);
-            dead = 0;
-            mbar_init_fence();
-        }
-        if (warp == 1) tmem_alloc<1>(&tmem_at, BN);
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        const uint32_t tmem = tmem_at;
-        if (warp == 0) {
-            if (lane == 0) {
-                Ring r(L::kStages, 1);
-                for (int kb = kb0; kb < kb1; kb++, r.next()) {
-                    if (!mbar_wait(&empty[r.i], r.phase, &dead)) break;
-                    const uint32_t s = ring + r.i * L::kStage, bar = smem_u32(&full[r.i]);
-                    mbar_expect(&full[r.i], a.x_rows * 128 + BN * 128);
-                    tma_2d<1>(s, &mx, kb * 64, m0, bar);
-                    if constexpr (W_MN) {
-#pragma unroll
-                        for (int q = 0; q < BN / 64; q++) tma_2d<1>(s + 16384 + q * 8192, &mw, o0 + q * 64, kb * 64, bar);
-                    } else {
-                        tma_2d<1>(s + 16384, &mw, kb * 64, o0, bar);
-                    }
-                }
-            }
-        } else if (warp == 1) {
-            if (lane == 0) {
-                constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-                constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (W_MN ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | 8u << 24;
-                Ring r(L::kStages, 0);
-                for (int kb = kb0; kb < kb1; kb++, r.next()) {
-                    if (!mbar_wait(&full[r.i], r.phase, &dead)) break;
-                    tc_fence_after();
-                    const uint32_t s = ring + r.i * L::kStage;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint64_t db = W_MN ? desc_mn128(s + 16384 + k * 2048, 8192) : desc_k128(s + 16384 + k * 32);
-                        mma_f16<1>(tmem, desc_k128(s + k * 32), db, idesc, (kb - kb0) | k);
-                    }
-                    mma_commit<1>(&empty[r.i]);
-                }
-                mma_commit<1>(&done);
-            }
-        }
-        __syncwarp();
-        mbar_wait(&done, 0, &dead);
-        tc_fence_after();
-        const int row = (warp & 3) * 32 + lane;
-#pragma unroll
-        for (int c = (warp >> 2) * (BN / 2); c < (warp >> 2) * (BN / 2) + BN / 2; c += 32) {
-            float v[32];
-            __syncwarp();
-            tmem_ld32(tmem + c + ((uint32_t)(warp & 3) << 21), v);
-#pragma unroll
-            for (int q = 0; q < 32; q += 4)
-                *reinterpret_cast<float4*>(sums + row * L::kRow + c + q) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
-        }
-        tc_fence_before();
+    const long long m0 = (long long)(blockIdx.x / S) * 128;
+    const int o0 = blockIdx.y * BN, rows = (int)min(128LL, p.n - m0);
+    const int per = BN / S, col0 = rank * per;  // this CTA's outputs
+    const bool early = rows * per <= L::kEarly;
+    const int kb0 = a.kblocks * rank / S, kb1 = a.kblocks * (rank + 1) / S;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; i++) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        mbar_init(&done, 1);
+        dead = 0;
+        mbar_init_fence();
     }
-    if (S > 1) cluster_sync_all();
-    else __syncthreads();
-    grid_dependency_wait();  // low is written by the launch before this one
-    release_dependents();
-    const int per = BN / S, rs = low_stride(p.r);
-    for (int i = threadIdx.x; i < 128 * (per / 8); i += 256) {
-        const int row = i & 127, col = rank * per + (i >> 7) * 8, o = o0 + col;
-        const long long m = m0 + row;
-        if (m >= p.n || o >= p.o) continue;
-        float v[8] = {};
-        if (a.kblocks)
-            for (int q = 0; q < S; q++) {
-                const float* f = sums + row * L::kRow + col;
-                float4 f0, f1;
-                if (S > 1) {
-                    const uint32_t at = map_rank(f, q);
-                    f0 = ld_cluster4(at), f1 = ld_cluster4(at + 16);
+    if (warp == 1) tmem_alloc<1>(&tmem_at, BN);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring r(L::kStages, 1);
+            for (int kb = kb0; kb < kb1; kb++, r.next()) {
+                if (!mbar_wait(&empty[r.i], r.phase, &dead)) break;
+                const uint32_t s = ring + r.i * L::kStage, bar = smem_u32(&full[r.i]);
+                mbar_expect(&full[r.i], a.x_rows * 128 + BN * 128);
+                tma_2d<1>(s, &mx, kb * 64, (int)m0, bar);
+                if constexpr (W_MN) {
+#pragma unroll
+                    for (int q = 0; q < BN / 64; q++) tma_2d<1>(s + 16384 + q * 8192, &mw, o0 + q * 64, kb * 64, bar);
                 } else {
-                    f0 = *reinterpret_cast<const float4*>(f), f1 = *reinterpret_cast<const float4*>(f + 4);
+                    tma_2d<1>(s + 16384, &mw, kb * 64, o0, bar);
                 }
-                v[0] += f0.x, v[1] += f0.y, v[2] += f0.z, v[3] += f0.w, v[4] += f1.x, v[5] += f1.y, v[6] += f1.z, v[7] += f1.w;
-            }
-        const int e = p.id.of(m);
-        const bool whole = o + 8 <= p.o;
-        T* out = static_cast<T*>(p.out) + m * p.out_stride + o;
-        const T* base = static_cast<const T*>(p.base) + m * p.base_stride + o;
-        if (p.bias) {
-#pragma unroll
-            for (int z = 0; z < 8; z++) v[z] += elem<T>(p.bias, min(o + z, p.o - 1));
-        }
-        if (p.base) {
-            if (whole && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
-                const uint4 q = *reinterpret_cast<const uint4*>(base);
-                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int z = 0; z < 4; z++) {
-                    const float2 f = unpack2<T>(u[z]);
-                    v[2 * z] += f.x, v[2 * z + 1] += f.y;
-                }
-            } else {
-#pragma unroll
-                for (int z = 0; z < 8; z++) v[z] += elem<T>(base, min(z, p.o - 1 - o));
             }
         }
-        if (e >= 0) add_low<T>(p, p.low + m * rs, static_cast<const T*>(p.g.p) + e * p.g.se, o, v);
-        uint32_t u[4];
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+            constexpr uint32_t idesc = 1u << 4 | fmt << 7 | fmt << 10 | (W_MN ? 1u << 16 : 0u) | (uint32_t)(BN >> 3) << 17 | 8u << 24;
+            Ring r(L::kStages, 0);
+            for (int kb = kb0; kb < kb1; kb++, r.next()) {
+                if (!mbar_wait(&full[r.i], r.phase, &dead)) break;
+                tc_fence_after();
+                const uint32_t s = ring + r.i * L::kStage;
 #pragma unroll
-        for (int z = 0; z < 4; z++) u[z] = pack2<T>(v[2 * z], v[2 * z + 1]);
-        if (whole && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-            *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
-        } else {
-            const T* h = reinterpret_cast<const T*>(u);
-#pragma unroll
-            for (int z = 0; z < 8; z++)
-                if (o + z < p.o) out[z] = h[z];
+                for (int k = 0; k < 4; k++) {
+                    const uint64_t db = W_MN ? desc_mn128(s + 16384 + k * 2048, 8192) : desc_k128(s + 16384 + k * 32);
+                    mma_f16<1>(tmem, desc_k128(s + k * 32), db, idesc, (kb - kb0) | k);
+                }
+                mma_commit<1>(&empty[r.i]);
+            }
+            mma_commit<1>(&done);
+        }
+    } else if (early) {
+        grid_dependency_wait();  // low is written by the launch before this one
+        release_dependents();
+        for (int i = threadIdx.x - 64; i < rows * (per / 2); i += 192) {
+            const int row = i / (per / 2), o = o0 + col0 + i % (per / 2) * 2;
+            if (o >= p.o) continue;
+            float v[2] = {};
+            other_terms<T, 2>(p, m0 + row, o, v);
+            *reinterpret_cast<float2*>(terms + 2 * i) = make_float2(v[0], v[1]);
         }
     }
-    if (a.kblocks && dead && threadIdx.x == 0) settle();
+    __syncwarp();
+    mbar_wait(&done, 0, &dead);
+    tc_fence_after();
+    const int row = (warp & 3) * 32 + lane;
+#pragma unroll
+    for (int c = (warp >> 2) * (BN / 2); c < (warp >> 2) * (BN / 2) + BN / 2; c += 32) {
+        float v[32];
+        __syncwarp();
+        tmem_ld32(tmem + c + ((uint32_t)(warp & 3) << 21), v);
+#pragma unroll
+        for (int q = 0; q < 32; q += 4)
+            *reinterpret_cast<float4*>(sums + row * L::kRow + c + q) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+    }
+    tc_fence_before();
     if (S > 1) cluster_sync_all();
     else __syncthreads();
-    if (a.kblocks && warp == 1) tmem_free<1>(tmem_at, BN);
+    if (early) {
+        for (int i = threadIdx.x; i < rows * (per / 2); i += 256) {
+            const int row = i / (per / 2), col = col0 + i % (per / 2) * 2;
+            if (o0 + col >= p.o) continue;
+            const float2 t = *reinterpret_cast<const float2*>(terms + 2 * i);
+            float v[2] = {t.x, t.y};
+            add_sums<2>(sums + row * L::kRow + col, S, v);
+            put_outputs<T, 2>(p, m0 + row, o0 + col, v);
+        }
+    } else {
+        grid_dependency_wait();  // low is written by the launch before this one
+        release_dependents();
+        for (int i = threadIdx.x; i < rows * (per / 8); i += 256) {
+            const int row = i / (per / 8), col = col0 + i % (per / 8) * 8;
+            if (o0 + col >= p.o) continue;
+            float v[8] = {};
+            add_sums<8>(sums + row * L::kRow + col, S, v);
+            other_terms<T, 8>(p, m0 + row, o0 + col, v);
+            put_outputs<T, 8>(p, m0 + row, o0 + col, v);
+        }
+    }
+    if (dead && threadIdx.x == 0) settle();
+    if (S > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 1) tmem_free<1>(tmem_at, BN);
+}
+
+// The adapters' term beside a base and a bias, without a shared projection:
+// 32 tokens x 64 outputs a CTA.  Bound: latency, then reading base.
+template <class T>
+__global__ void __launch_bounds__(256, 2) k_add_low(const ProjectArgs p) {
+    const long long m = (long long)blockIdx.x * 32 + threadIdx.x / 8;
+    const int o = blockIdx.y * 64 + threadIdx.x % 8 * 8;
+    grid_dependency_wait();
+    release_dependents();
+    if (m >= p.n || o >= p.o) return;
+    float v[8] = {};
+    other_terms<T, 8>(p, m, o, v);
+    put_outputs<T, 8>(p, m, o, v);
 }
 
 template <class T, int BN, bool W_MN>
 cudaError_t launch_split(const ProjectArgs& p, int sms, cudaStream_t s) {
     using L = SplitTile<BN>;
     TcArgs a{p};
-    a.tiles_m = (int)((p.n + 127) / 128);
     a.tiles_n = (p.o + BN - 1) / BN;
-    a.kblocks = p.w ? (p.k + 63) / 64 : 0;
+    a.kblocks = (p.k + 63) / 64;
+    a.tiles_m = (int)((p.n + 127) / 128);
     // as many CTAs share a tile as it takes to give every SM one, while each
     // has two slices of the contraction and eight outputs of a row
     a.split = 1;
     while (a.split < 8 && (long long)a.tiles_m * a.tiles_n * a.split < sms && a.kblocks >= 4 * a.split) a.split *= 2;
     a.x_rows = p.n < 128 ? (int)(p.n + 7) / 8 * 8 : 128;  // rows behind stay whatever they are: their sums are not used
     CUtensorMap mx{}, mw{};
-    if (p.w) {
-        const cudaError_t e = operand_maps<T, W_MN>(p, a.x_rows, BN, &mx, &mw);
-        if (e != cudaSuccess) return e;
-    }
     auto kern = k_project_split<T, BN, W_MN>;
-    const size_t smem = p.w ? L::kSmem : 0;
-    const cudaError_t e = ensure_smem(kern, smem);
+    cudaError_t e = operand_maps<T, W_MN>(p, a.x_rows, BN, &mx, &mw);
+    if (e == cudaSuccess) e = ensure_smem(kern, L::kSmem);
     if (e != cudaSuccess) return e;
     KScope ks("adapter_project", s);
-    return launch_dependent(a.split, kern, dim3((unsigned)(a.tiles_n * a.split), a.tiles_m), 256, smem, s, a, mx, mw);
+    return launch_dependent(a.split, kern, dim3((unsigned)(a.tiles_m * a.split), a.tiles_n), 256, L::kSmem, s, a, mx, mw);
 }
 
 // low of many tokens: a cluster of S CTAs shares the contraction of 128
@@ -934,6 +1012,10 @@ cudaError_t low_tc(const LowArgs* a, int count, const int* after_pack, int sms, 
 template <class T, bool W_MN>
 cudaError_t launch_width(const ProjectArgs& p, int sms, cudaStream_t s) {
     if (!p.g32) {
+        if (!p.w) {
+            KScope ks("adapter_project", s);
+            return launch_dependent(1, k_add_low<T>, dim3((unsigned)((p.n + 31) / 32), (p.o + 63) / 64), 256, 0, s, p);
+        }
         // 64-wide tiles as long as they do not fill the SMs twice
         const long long tiles = ((p.n + 127) / 128) * ((p.o + 63) / 64);
         return tiles <= 2 * sms ? launch_split<T, 64, W_MN>(p, sms, s) : launch_split<T, 128, W_MN>(p, sms, s);
