@@ -23,6 +23,13 @@ Seeds, the routed expert and the DP seed are derived on the device from a
 token counter, so a decode step issues stream work only: ``capture`` records
 the whole step -- transformer, 28 HE-LoRA calls, DP noise, greedy pick -- as
 one CUDA graph that is replayed per token.
+
+``LoraBatch`` is the plaintext twin for requests that are not encrypted (the
+reference's plaintext branch, inference_engine.py:1234-1242): a batch of them
+at once, each with an adapter of its own, in the projections' own kernels.
+
+Both take ``rules`` for the pick, the keyword arguments of
+``logits.apply_rules`` other than the history, which is kept here.
 """
 from __future__ import annotations
 
@@ -32,7 +39,9 @@ import numpy as np
 
 from . import tensafe_he
 from ._lib import check, lib
+from .adapters import adapter_project
 from .backend import ZeroMoaiLora, dp_sigma, lora_delta_graphable
+from .logits import apply_rules
 
 QWEN25_15B = dict(hidden_size=1536, intermediate_size=8960, num_hidden_layers=28, num_attention_heads=12,
                   num_key_value_heads=2, vocab_size=151936, max_position_embeddings=32768, rope_theta=1000000.0,
@@ -56,6 +65,114 @@ def build_model(device="cuda", seed: int = 2, layers: int = 28):
 def encryption_seed(token: int, layer: int) -> int:
     """Seed of (token, layer)'s encryption (the device computes the same)."""
     return token * _SEED_TOKEN + layer * _SEED_LAYER + _SEED_BASE
+
+
+class GreedyPick:
+    """Greedy picks for the next tokens of a batch, under ``rules`` if given
+    (keyword arguments of ``logits.apply_rules``).  The requests' histories
+    lie on the device, so that a captured step extends its own.  A request
+    whose rules leave no token gets -1."""
+
+    def __init__(self, rules, requests: int, room: int, device):
+        import torch
+
+        self.rules = None if rules is None else dict(rules)
+        self.tokens = torch.zeros((requests, room), dtype=torch.int64, device=device)
+        self.lengths = torch.zeros((requests,), dtype=torch.int32, device=device)
+        self.prompts = torch.zeros((requests,), dtype=torch.int32, device=device)
+
+    def start(self, prompt):
+        """Histories that hold the prompts [requests, k] (or one token)."""
+        import torch
+
+        if self.rules is None:
+            return
+        k = prompt.shape[1] if isinstance(prompt, torch.Tensor) else 1
+        self.tokens[:, :k] = prompt
+        self.lengths.fill_(k)
+        self.prompts.fill_(k)
+
+    def __call__(self, logits):
+        """Picks [requests, 1] for logits [requests, vocab]."""
+        if self.rules is None:
+            return logits.argmax(dim=-1, keepdim=True)
+        picks = apply_rules(logits, self.tokens, self.lengths, self.prompts, write=False, **self.rules)[1].view(-1, 1)
+        self.tokens.scatter_(1, self.lengths.long().view(-1, 1), picks)
+        self.lengths.add_(1)
+        return picks
+
+
+def _generate(model, prompt_ids, tokens, rules, device, after=None):
+    """Greedy decode of prompts [requests, k], eager (DynamicCache)."""
+    import torch
+    from transformers import DynamicCache
+
+    ids = prompt_ids
+    pick = GreedyPick(rules, ids.shape[0], ids.shape[1] + tokens, device)
+    pick.start(ids)
+    cache = DynamicCache()
+    out_ids = []
+    with torch.no_grad():
+        for _ in range(tokens):
+            res = model(input_ids=ids, past_key_values=cache, use_cache=True)
+            out_ids.append(pick(res.logits[:, -1, :]))
+            ids = out_ids[-1] if rules is None else out_ids[-1].clamp_min(0)  # behind the end of a request: token 0
+            if after:
+                after()
+    return torch.cat(out_ids, dim=1)
+
+
+class LoraBatch:
+    """Plaintext LoRA (q_proj, v_proj) on every layer of ``model`` for batches
+    of requests, each with its own adapter or none.
+
+    weights: per layer (A_q, A_v [experts, r, d], B_q [experts, d, r], B_v
+    [experts, dv, r]), as ``HeLoraDecoder.weights`` holds them."""
+
+    def __init__(self, model, weights):
+        import torch
+
+        p = next(model.parameters())
+        self.model, self.dev = model, p.device
+        self._adapter = None  # int32 [requests], while ``generate`` runs
+        self._modules = []
+        if len(weights) != len(model.model.layers):
+            raise ValueError(f"{len(weights)} layers of adapters for {len(model.model.layers)} layers")
+        for layer, (aq, av, bq, bv) in zip(model.model.layers, weights):
+            for module, a, b in ((layer.self_attn.q_proj, aq, bq), (layer.self_attn.v_proj, av, bv)):
+                a, b = (torch.as_tensor(w).to(device=p.device, dtype=p.dtype).contiguous() for w in (a, b))
+                self._modules.append((module, module.__dict__.get("forward")))
+                module.forward = self._forward(module, module.forward, a, b)
+
+    def _forward(self, module, plain, a, b):
+        def forward(x):
+            if self._adapter is None:
+                return plain(x)
+            return adapter_project(x, a, b, self._adapter, weight=module.weight, bias=module.bias)
+        return forward
+
+    def generate(self, prompt_ids, adapter, tokens: int = 16, rules=None):
+        """Greedy decode of prompts [requests, k] with adapter[i] for request
+        i (-1 for none); rows of ``rules`` belong to the requests."""
+        import torch
+
+        ids = torch.as_tensor(prompt_ids, device=self.dev)
+        adapter = torch.as_tensor(adapter, dtype=torch.int32, device=self.dev)
+        if ids.dim() != 2 or adapter.shape != (ids.shape[0],):
+            raise ValueError("prompt_ids must be [requests, tokens] and adapter [requests]")
+        self._adapter = adapter
+        try:
+            return _generate(self.model, ids, tokens, rules, self.dev)
+        finally:
+            self._adapter = None
+
+    def remove(self):
+        for module, before in reversed(self._modules):
+            if before is None:
+                del module.forward
+            else:
+                module.forward = before
+        self._modules = []
 
 
 class HeLoraDecoder:
@@ -153,28 +270,23 @@ class HeLoraDecoder:
         s = stream if stream is not None else torch.cuda.current_stream(self.dev)
         check(lib().ts_ctx_set_stream(self.ctx.handle, s.cuda_stream), "ts_ctx_set_stream")
 
-    def generate(self, prompt_ids, tokens: int = 16):
-        """Greedy decode, eager (DynamicCache); every forward pass runs
-        HE-LoRA on all layers."""
+    def generate(self, prompt_ids, tokens: int = 16, rules=None):
+        """Greedy decode, eager (DynamicCache), under ``rules`` if given;
+        every forward pass runs HE-LoRA on all layers."""
         import torch
-        from transformers import DynamicCache
 
         self.bind_stream()
         ids = torch.as_tensor(prompt_ids, device=self.dev).view(1, -1)
-        cache = DynamicCache()
-        out_ids = []
-        with torch.no_grad():
-            for _ in range(tokens):
-                res = self.model(input_ids=ids, past_key_values=cache, use_cache=True)
-                ids = res.logits[:, -1, :].argmax(dim=-1, keepdim=True)
-                out_ids.append(ids)
-                self.token += 1
-        return torch.cat(out_ids, dim=1)
 
-    def capture(self, max_len: int = 64, warmup: int = 2):
+        def count():
+            self.token += 1
+        return _generate(self.model, ids, tokens, rules, self.dev, after=count)
+
+    def capture(self, max_len: int = 64, warmup: int = 2, rules=None):
         """Capture one decode step (static KV cache) as a CUDA graph on a
         side stream; returns run(prompt_id, n) that decodes n tokens from a
-        one-token prompt by replaying it."""
+        one-token prompt by replaying it, under ``rules`` if given (their
+        tensors are read at every replay)."""
         import torch
         from transformers import StaticCache
 
@@ -184,21 +296,23 @@ class HeLoraDecoder:
         ids = torch.zeros((1, 1), dtype=torch.long, device=self.dev)
         pos = torch.zeros((1,), dtype=torch.long, device=self.dev)
         outs = torch.zeros((1, max_len), dtype=torch.long, device=self.dev)
+        pick = GreedyPick(rules, 1, max_len + 1, self.dev)
+        pick.start(0)
         stream = torch.cuda.Stream(device=self.dev)
         self.bind_stream(stream)
 
         def step():
             r = self.model(input_ids=ids, cache_position=pos, position_ids=pos.view(1, 1), past_key_values=cache,
                            use_cache=True)
-            nxt = r.logits[:, -1, :].argmax(dim=-1, keepdim=True)
+            nxt = pick(r.logits[:, -1, :])
             outs.index_copy_(1, pos, nxt)
-            ids.copy_(nxt)
+            ids.copy_(nxt if rules is None else nxt.clamp_min(0))
             pos.add_(1)
             self.token.add_(1)
 
         stream.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.no_grad(), torch.cuda.stream(stream):
-            for _ in range(warmup):  # sizes the library's scratch, loads kernels
+            for _ in range(min(warmup, max_len)):  # sizes the library's scratch, loads kernels
                 step()
             stream.synchronize()
             graph = torch.cuda.CUDAGraph()
@@ -214,6 +328,7 @@ class HeLoraDecoder:
                 # (cumulative_length), which must restart with pos
                 cache.reset()
                 ids.fill_(int(prompt_id))
+                pick.start(int(prompt_id))
                 pos.zero_()
                 self.token.fill_(int(start_token))
                 for _ in range(n):

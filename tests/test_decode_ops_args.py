@@ -3,6 +3,7 @@ entry points on CPU tensors, and the C entry points' own checks, which come
 before any CUDA call."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -164,3 +165,22 @@ def _rules_args(**kw):
 def test_c_rules_refusals(change, match):
     assert _lib.lib().ts_logit_rules(_rules_args(**change)) == _lib.TS_ERR_ARG
     assert match in _lib.last_error()
+
+
+def test_lora_batch_refusals():
+    from types import SimpleNamespace as N
+    from provenloop_b200.decode_step import LoraBatch
+    linear = torch.nn.Linear(4, 4)
+    layers = [N(self_attn=N(q_proj=linear, v_proj=torch.nn.Linear(4, 2)))]
+    model = N(parameters=linear.parameters, model=N(layers=layers))
+    one = tuple(np.zeros(s, np.float32) for s in ((2, 3, 4), (2, 3, 4), (2, 4, 3), (2, 2, 3)))
+    with pytest.raises(ValueError, match="layers"):
+        LoraBatch(model, [one, one])
+    batch = LoraBatch(model, [one])
+    x = torch.ones(1, 4)
+    assert torch.equal(layers[0].self_attn.q_proj(x), torch.nn.functional.linear(x, linear.weight, linear.bias))  # outside of generate
+    for ids, adapter in (([1, 2], [0]), ([[1, 2]], [0, 1]), ([[1, 2]], 0)):
+        with pytest.raises(ValueError, match="requests"):
+            batch.generate(ids, adapter)
+    batch.remove()
+    assert "forward" not in linear.__dict__

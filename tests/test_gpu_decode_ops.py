@@ -591,6 +591,98 @@ def test_rules_captured(R):
             assert torch.equal(z.cpu(), torch.from_numpy(want).to(z.dtype)) and np.array_equal(pick.cpu().numpy(), picks)
 
 
+def test_training_step_of_two_layers(A, R):
+    """Forward through two projections, the rules' pick on the result, the
+    gradients back through both, an update, and forward again."""
+    first, second = _inputs(230, 520, 264, 16, 3, "bf16", "ragged", seed=21), _inputs(230, 264, 1000, 30, 3, "bf16", "ragged", seed=22)
+    second["ids"] = first["ids"]
+    for _ in range(2):
+        second["x"] = _check_project(A, first)
+        y = _check_project(A, second)
+        z, pick = R.apply_rules(y, mask=torch.full((32,), 0x5555_5555, dtype=torch.int32, device="cuda"))
+        want = y.clone()
+        want[:, 1::2] = -float("inf")
+        assert torch.equal(z, want) and torch.equal(pick, want.float().argmax(1))
+        first["dy"], da2, db2 = _check_backward(A, second)
+        _, da1, db1 = _check_backward(A, first)
+        for s, da, db in ((first, da1, db1), (second, da2, db2)):
+            s["a"], s["b"] = s["a"] - 1e-3 * da, s["b"] - 1e-3 * db
+
+
+def _model():
+    from provenloop_b200.decode_step import build_model
+    return build_model(layers=2)
+
+
+def _layers(model, rank, experts, seed):
+    rng, cfg = np.random.default_rng(seed), model.config
+    d, dv = cfg.hidden_size, cfg.num_key_value_heads * (cfg.hidden_size // cfg.num_attention_heads)
+    shapes = ((experts, rank, d), (experts, rank, d), (experts, d, rank), (experts, dv, rank))
+    return [tuple((0.05 * rng.standard_normal(s)).astype(np.float32) for s in shapes) for _ in range(cfg.num_hidden_layers)]
+
+
+def test_lora_batch_decodes_under_rules():
+    """A batch of requests, each with its own adapter: every projection of
+    every step and every pick against the 64-bit forms."""
+    from types import SimpleNamespace
+    from provenloop_b200.decode_step import LoraBatch
+    model, n, k, steps = _model(), 5, 7, 4
+    weights, v = _layers(model, 16, 3, 4), model.config.vocab_size
+    plain = model.model.layers[0].self_attn.q_proj.forward
+    batch = LoraBatch(model, weights)
+    seen, logits, hooks = [], [], []
+    for layer, (aq, av, bq, bv) in zip(model.model.layers, weights):
+        for module, a, b in ((layer.self_attn.q_proj, aq, bq), (layer.self_attn.v_proj, av, bv)):
+            a, b = (torch.from_numpy(w).cuda().bfloat16() for w in (a, b))
+            hooks.append(module.register_forward_hook(lambda m, i, o, a=a, b=b: seen.append((m, i[0].clone(), o.clone(), a, b))))
+    hooks.append(model.lm_head.register_forward_hook(lambda m, i, o: logits.append(o[:, -1].detach().clone())))
+    rng = np.random.default_rng(8)
+    prompt = rng.integers(0, v, (n, k))
+    adapter = [0, 2, -1, 1, 0]
+    ref = dict(rho=(1 + rng.random(n)).astype(np.float32), f=rng.random(n).astype(np.float32), p=rng.random(n).astype(np.float32),
+               bias_ids=rng.integers(0, v, (n, 3)), bias=rng.standard_normal((n, 3)).astype(np.float32),
+               mask=rng.integers(-2 ** 31, 2 ** 31, (n, (v + 31) // 32)).astype(np.int32))
+    ref["mask"][3] = 0  # this request ends at once
+    names = dict(rho="repetition", f="frequency", p="presence", bias="bias_values")
+    got = batch.generate(prompt, adapter, tokens=steps, rules={names.get(q, q): torch.from_numpy(t).cuda() for q, t in ref.items()}).cpu().numpy()
+    for h in hooks:
+        h.remove()
+    assert got.shape == (n, steps) and len(logits) == steps and len(seen) == steps * 4
+    history = prompt
+    for i in range(steps):
+        lengths = np.full(n, history.shape[1], np.int32)
+        picks = _rules_ref(logits[i].float().cpu().numpy(), tokens=history, lengths=lengths, prompt=np.full(n, k, np.int32), **ref,
+                           dtype=np.float32)[1]
+        assert np.array_equal(got[:, i], picks) and picks[3] == -1
+        history = np.concatenate([history, picks[:, None]], axis=1)
+    for module, x, y, a, b in seen:
+        ids = torch.tensor(adapter, dtype=torch.int32, device="cuda").repeat_interleave(x.shape[1])
+        s = dict(x=x.flatten(0, 1), a=a, b=b, ids=ids, w=module.weight.detach(), bias=module.bias.detach(), scale=torch.ones(3, device="cuda"))
+        _check_project(SimpleNamespace(adapter_project=lambda *_, **__: y.flatten(0, 1)), s, scale=False)
+    batch.remove()
+    assert model.model.layers[0].self_attn.q_proj.forward == plain
+
+
+def test_encrypted_decode_under_rules():
+    """Eager and captured: three biased tokens in the order of their biases
+    (a token once picked loses more than any bias), the rest within the mask."""
+    from provenloop_b200 import tensafe_he
+    from provenloop_b200.decode_step import HeLoraDecoder
+    model, ctx = _model(), tensafe_he.CkksContext(16384)
+    dec = HeLoraDecoder(model, ctx, ctx.keygen(0), rank=16, experts=3, seed=2)
+    mask = torch.full(((model.config.vocab_size + 31) // 32,), 0x0F0F_0F0F, dtype=torch.int32, device="cuda")
+    rules = dict(presence=torch.full((1,), 1000.0, device="cuda"), bias_ids=torch.tensor([3, 9, 11], device="cuda"),
+                 bias_values=torch.tensor([300.0, 200.0, 100.0], device="cuda"), mask=mask)
+    run = dec.capture(max_len=8, rules=rules)
+    for decode, n in ((lambda p, n: dec.generate([p], tokens=n, rules=rules), 5), (run, 5), (run, 8)):
+        out = decode(151643, n)
+        torch.cuda.synchronize()  # run works on a stream of its own
+        ids = out[0].tolist()
+        assert ids[:3] == [3, 9, 11] and len(set(ids)) == len(ids)
+        assert all(t >= 0 and t % 8 < 4 for t in ids)
+    dec.remove()
+
+
 def test_no_wait_ran_out():
     """Collected last: none of the calls above gave up a wait in a kernel."""
     import ctypes as C
