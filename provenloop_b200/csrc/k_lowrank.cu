@@ -103,27 +103,27 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], const uint32_t (&a)[4],
 
 // ---------------------------------------------------------------- packing
 
-// 32 x 32 elements of a job through shared memory, read along whichever axis
-// of src is contiguous, written along k.
+// 32 rows x 128 columns of a job through shared memory, read along whichever
+// axis of src is contiguous, written along k.
 __device__ __forceinline__ void pack_tile(const PackJob& a, const uint16_t* src, uint16_t* dst, long long j0, int k0) {
-    __shared__ uint16_t tile[32][33];
+    __shared__ __align__(4) uint16_t tile[32][130];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    uint16_t v[4];
+    const bool along = a.sk == 1;
+    const auto row = [&](int i) { return along ? ty + 8 * (i >> 2) : tx; };
+    const auto col = [&](int i) { return along ? tx + 32 * (i & 3) : ty + 8 * i; };
+    uint16_t v[16];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {  // loads from clamped places overlap, loads under a condition do not
-        const long long j = min(j0 + (a.sk == 1 ? ty + 8 * i : tx), a.rows - 1);
-        const int k = min(k0 + (a.sk == 1 ? tx : ty + 8 * i), a.cols - 1);
-        v[i] = src[j * a.sj + k * a.sk];
-    }
+    for (int i = 0; i < 16; i++)  // loads from clamped places overlap, loads under a condition do not
+        v[i] = src[min(j0 + row(i), a.rows - 1) * a.sj + min(k0 + col(i), a.cols - 1) * a.sk];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int j = a.sk == 1 ? ty + 8 * i : tx, k = a.sk == 1 ? tx : ty + 8 * i;
-        tile[j][k] = k0 + k < a.cols ? v[i] : (uint16_t)0;
-    }
+    for (int i = 0; i < 16; i++) tile[row(i)][col(i)] = k0 + col(i) < a.cols ? v[i] : (uint16_t)0;
     __syncthreads();
 #pragma unroll
-    for (int i = ty; i < 32; i += 8)
-        if (j0 + i < a.rows && k0 + tx < a.dst_cols) dst[(j0 + i) * a.dst_cols + k0 + tx] = tile[i][tx];
+    for (int i = 0; i < 8; i++) {
+        const int j = ty + 8 * (i >> 1), k = (tx + 32 * (i & 1)) * 2;
+        if (j0 + j < a.rows && k0 + k < a.dst_cols)
+            *reinterpret_cast<uint32_t*>(dst + (j0 + j) * a.dst_cols + k0 + k) = *reinterpret_cast<const uint32_t*>(&tile[j][k]);
+    }
 }
 
 // 128 rows x 16 columns of a factor as f32; returns whether an element is not
@@ -245,9 +245,9 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs j
     if (a.kind == PackJob::LISTS) {
         pack_lists(a, (int)b);
     } else if (a.kind == PackJob::COPY) {
-        const long long tr = (a.rows + 31) / 32, tc = (a.dst_cols + 31) / 32, e = b / (tr * tc), in = b % (tr * tc);
+        const long long tr = (a.rows + 31) / 32, tc = (a.dst_cols + 127) / 128, e = b / (tr * tc), in = b % (tr * tc);
         pack_tile(a, static_cast<const uint16_t*>(a.src) + e * a.se, static_cast<uint16_t*>(a.dst) + e * a.rows * a.dst_cols, in % tr * 32,
-                  (int)(in / tr) * 32);
+                  (int)(in / tr) * 128);
     } else {
         const int tc = a.dst_cols / 16;
         const long long tr = (a.rows + 127) / 128, e = b / (tr * tc);
@@ -357,15 +357,18 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
 // ---------------------------------------------------------------- projection
 
 // f32: BM x BN outputs per CTA, TM x TN per thread in two halves, 16 of the
-// contraction at a time, the next ones on their way in registers.  A cluster
-// of S CTAs shares the contraction where the tiles are few, and each finishes
+// contraction at a time, the next ones on their way in registers.  The
+// adapters' terms are more of the same contraction, one after the other for
+// the adapters of the tile, each added to its own tokens' sums only.  A
+// cluster of S CTAs shares both where the tiles are few, and each finishes
 // BM / S of the rows.  On the FMA pipe: the tensor cores' TF32 would need
 // three products and rounds its sums towards zero.
 template <int BM, int BN, int TM, int TN>
-__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int vec_x, int vec_w) {
+__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int vec_x, int vec_w, int vec_g) {
     constexpr int BK = 16, LX = BM * BK / 1024, LW = BN * BK / 1024;  // float4 loads of a thread
     static_assert((BM / TM) * (BN / TN) == 256, "one thread per TM x TN outputs");
     __shared__ __align__(16) float xs[2][BK][BM + 4], ws[2][BK][BN + 4];
+    __shared__ __align__(16) int ids[BM];
     constexpr bool kShared = BM == 64;  // the contraction may be shared
     __shared__ float part[kShared ? BM : 1][BN + 1];
     cg::cluster_group cluster = cg::this_cluster();
@@ -374,11 +377,14 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
     const int o0 = blockIdx.y * BN;
     constexpr int TX = BN / TN;
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    const auto row_of = [&](int i) { return ty * 4 + i / 4 * (BM / (TM / 4)) + i % 4; };
+    const auto col_of = [&](int j) { return tx * 4 + j / 4 * (BN / (TN / 4)) + j % 4; };
+    if (threadIdx.x < BM) ids[threadIdx.x] = m0 + threadIdx.x < a.n ? a.id.of(m0 + threadIdx.x) : -1;
     float acc[TM][TN] = {};
-    if (a.w) {
-        const float* x = static_cast<const float*>(a.x);
-        const float* w = static_cast<const float*>(a.w);
-        const int blocks = (a.k + BK - 1) / BK, b0 = blocks * rank / S, b1 = blocks * (rank + 1) / S;
+    // acc += rows x [n][k] times w [o][k], or [k][o] where `w_t`, over blocks
+    // [b0, b1) of k; of an adapter's factor for the rows in `mine` only
+    const auto contract = [&](const float* x, long long x_stride, bool vx, const float* w, long long w_stride, bool w_t, bool vw, int kk,
+                              int b0, int b1, auto one, unsigned mine) {
         float4 nx[LX], nw[LW];
         // four neighbours of a row that ends at `n`, from a clamped place
         const auto quad = [](const float* row, int at, int n, bool in, bool vec) {
@@ -397,17 +403,17 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
             for (int i = 0; i < LX; i++) {
                 const int q = threadIdx.x + 256 * i;
                 const long long m = m0 + q / 4;
-                nx[i] = quad(x + min(m, a.n - 1) * a.x_stride, k0 + q % 4 * 4, a.k, m < a.n, vec_x);
+                nx[i] = quad(x + min(m, a.n - 1) * x_stride, k0 + q % 4 * 4, kk, m < a.n, vx);
             }
 #pragma unroll
             for (int i = 0; i < LW; i++) {
                 const int q = threadIdx.x + 256 * i;
-                if (a.w_t) {
+                if (w_t) {
                     const int k = k0 + q / (BN / 4);
-                    nw[i] = quad(w + (long long)min(k, a.k - 1) * a.w_stride, o0 + q % (BN / 4) * 4, a.o, k < a.k, vec_w);
+                    nw[i] = quad(w + (long long)min(k, kk - 1) * w_stride, o0 + q % (BN / 4) * 4, a.o, k < kk, vw);
                 } else {
                     const int o = o0 + q / 4;
-                    nw[i] = quad(w + (long long)min(o, a.o - 1) * a.w_stride, k0 + q % 4 * 4, a.k, o < a.o, vec_w);
+                    nw[i] = quad(w + (long long)min(o, a.o - 1) * w_stride, k0 + q % 4 * 4, kk, o < a.o, vw);
                 }
             }
         };
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
 #pragma unroll
             for (int i = 0; i < LW; i++) {
                 const int q = threadIdx.x + 256 * i;
-                if (a.w_t) {
+                if (w_t) {
                     *reinterpret_cast<float4*>(&ws[s][q / (BN / 4)][q % (BN / 4) * 4]) = nw[i];
                 } else {
                     const int o = q / 4, k = q % 4 * 4;
@@ -428,51 +434,64 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
                 }
             }
         };
-        if (b0 < b1) {
-            load(b0);
-            store(0);
-            __syncthreads();
-            for (int b = b0; b < b1; b++) {
-                const int s = (b - b0) & 1;
-                if (b + 1 < b1) load(b + 1);
+        if (b0 >= b1) return;
+        load(b0);
+        store(0);
+        __syncthreads();
+        for (int b = b0; b < b1; b++) {
+            const int s = (b - b0) & 1;
+            if (b + 1 < b1) load(b + 1);
 #pragma unroll
-                for (int k = 0; k < BK; k++) {
-                    float xv[TM], wv[TN];
+            for (int k = 0; k < BK; k++) {
+                float xv[TM], wv[TN];
 #pragma unroll
-                    for (int i = 0; i < TM; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&xs[s][k][ty * 4 + i / 4 * (BM / (TM / 4))]);
-                        xv[i] = f.x, xv[i + 1] = f.y, xv[i + 2] = f.z, xv[i + 3] = f.w;
-                    }
+                for (int i = 0; i < TM; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&xs[s][k][ty * 4 + i / 4 * (BM / (TM / 4))]);
+                    xv[i] = f.x, xv[i + 1] = f.y, xv[i + 2] = f.z, xv[i + 3] = f.w;
+                }
 #pragma unroll
-                    for (int i = 0; i < TN; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&ws[s][k][tx * 4 + i / 4 * (BN / (TN / 4))]);
-                        wv[i] = f.x, wv[i + 1] = f.y, wv[i + 2] = f.z, wv[i + 3] = f.w;
-                    }
+                for (int i = 0; i < TN; i += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&ws[s][k][tx * 4 + i / 4 * (BN / (TN / 4))]);
+                    wv[i] = f.x, wv[i + 1] = f.y, wv[i + 2] = f.z, wv[i + 3] = f.w;
+                }
 #pragma unroll
-                    for (int i = 0; i < TM; i++)
+                for (int i = 0; i < TM; i++)
+                    if (!decltype(one)::value || (mine >> i & 1))
 #pragma unroll
                         for (int j = 0; j < TN; j++) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
-                }
-                if (b + 1 < b1) store(s ^ 1);
-                __syncthreads();
             }
+            if (b + 1 < b1) store(s ^ 1);
+            __syncthreads();
         }
+    };
+    if (a.w) {
+        const int blocks = (a.k + BK - 1) / BK;
+        contract(static_cast<const float*>(a.x), a.x_stride, vec_x, static_cast<const float*>(a.w), a.w_stride, a.w_t, vec_w, a.k,
+                 blocks * rank / S, blocks * (rank + 1) / S, std::false_type(), 0);
     }
-    const int rs = low_stride(a.r);
+    __syncthreads();
+    const bool g_t = a.g.sk == 1 && a.g.sj != 1;  // [r][o], else [o][r]
+    for (int e = -1, at = 0;; at++) {
+        int next = INT_MAX;  // the tile's adapters in ascending order; every thread looks for itself
+#pragma unroll 4
+        for (int i = 0; i < BM; i += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(ids + i);
+            next = min(min(next, q.x > e ? q.x : INT_MAX), min(q.y > e ? q.y : INT_MAX, min(q.z > e ? q.z : INT_MAX, q.w > e ? q.w : INT_MAX)));
+        }
+        if (next == INT_MAX) break;
+        e = next;
+        if (at % S != rank) continue;
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < TM; i++) mine |= (unsigned)(ids[row_of(i)] == e) << i;
+        contract(a.low, low_stride(a.r), true, static_cast<const float*>(a.g.p) + e * a.g.se, g_t ? a.g.sj : a.g.sk, g_t, vec_g, a.r, 0,
+                 (a.r + BK - 1) / BK, std::true_type(), mine);
+    }
     const auto finish = [&](long long m, int o, float v) {
         if (a.bias) v += static_cast<const float*>(a.bias)[o];
         if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
-        const int e = a.id.of(m);
-        if (e >= 0) {
-            const float* low = a.low + m * rs;
-            const float* g = static_cast<const float*>(a.g.p) + e * a.g.se + o * a.g.sk;
-#pragma unroll 8
-            for (int j = 0; j < a.r; j++) v = fmaf(low[j], g[j * a.g.sj], v);
-        }
         static_cast<float*>(a.out)[m * a.out_stride + o] = v;
     };
-    const auto row_of = [&](int i) { return ty * 4 + i / 4 * (BM / (TM / 4)) + i % 4; };
-    const auto col_of = [&](int j) { return tx * 4 + j / 4 * (BN / (TN / 4)) + j % 4; };
     if constexpr (kShared) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
@@ -962,13 +981,15 @@ cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
     const auto vec = [](const void* p, long long stride, long long rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows < 2 || stride % 4 == 0); };
     const int vx = vec(a.x, a.x_stride, a.n), vw = vec(a.w, a.w_stride, a.w_t ? a.k : a.o);
     KScope ks("adapter_project", s);
+    // a factor's rows: r rows of o elements, or o rows of r
+    const int vg = vec(a.g.p, a.g.sk == 1 && a.g.sj != 1 ? a.g.sj : a.g.sk, 2) && (a.id.count == 1 || a.g.se % 4 == 0);
     // large tiles where they fill the SMs, else small ones whose contraction
     // is shared until they do, 64 of it for each CTA at least
     const long long large = ((a.n + 127) / 128) * ((a.o + 127) / 128), small = ((a.n + 63) / 64) * ((a.o + 63) / 64);
-    if (large >= sm_count()) return launch_cl(1, k_project_f32<128, 128, 8, 8>, dim3((unsigned)((a.n + 127) / 128), (a.o + 127) / 128), 256, 0, s, a, vx, vw);
+    if (large >= sm_count()) return launch_cl(1, k_project_f32<128, 128, 8, 8>, dim3((unsigned)((a.n + 127) / 128), (a.o + 127) / 128), 256, 0, s, a, vx, vw, vg);
     int S = 1;
     while (S < 8 && a.w && small * S < 2 * sm_count() && a.k >= 128 * S) S *= 2;
-    return launch_cl(S, k_project_f32<64, 64, 4, 4>, dim3((unsigned)((a.n + 63) / 64 * S), (a.o + 63) / 64), 256, 0, s, a, vx, vw);
+    return launch_cl(S, k_project_f32<64, 64, 4, 4>, dim3((unsigned)((a.n + 63) / 64 * S), (a.o + 63) / 64), 256, 0, s, a, vx, vw, vg);
 }
 
 cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s) {

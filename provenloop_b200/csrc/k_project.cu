@@ -432,28 +432,44 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                     if (lane == 0) tma_store_2d(&mout, o0 + g * 32, m0, box);
                 }
             } else {
-                // rows that are not on 16-byte boundaries
-                T* out = static_cast<T*>(p.out) + m * p.out_stride;
-                const T* base = static_cast<const T*>(p.base) + m * p.base_stride;
-                for (int c = 0; c < groups * 32; c += 32) {
+                // rows that are not on 16-byte boundaries: through the box as
+                // well, and from there (to there) a row of 32 at a time
+                const uint16_t* base = static_cast<const uint16_t*>(p.base);
+                uint16_t* out = static_cast<uint16_t*>(p.out);
+                const int rows = (int)max(0LL, min(32LL, p.n - m0));
+                const auto at = [&](int i, int c) { return boxes + i * 64 + ((c >> 3 ^ (i >> 1 & 3)) << 4) + (c & 7) * 2; };
+                for (int g = 0; g < groups; g++) {
+                    const int o = o0 + g * 32 + lane, oc = min(o, p.o - 1);  // this lane's column
                     float v[32];
                     __syncwarp();
-                    tmem_ld32(d + c, v);
-                    if (p.bias) add_bias(o0 + c, v);
-                    if (e >= 0) add_bad(m, e, o0 + c, v);
-                    if (row) {
-                        if (p.base) {
-#pragma unroll
-                            for (int z = 0; z < 32; z++) v[z] += elem<T>(base, min(o0 + c + z, p.o - 1));
-                        }
-#pragma unroll
-                        for (int z = 0; z < 16; z++) {
-                            const uint32_t u = pack2<T>(v[2 * z], v[2 * z + 1]);
-                            const T* h = reinterpret_cast<const T*>(&u);
-                            if (o0 + c + 2 * z < p.o) out[o0 + c + 2 * z] = h[0];
-                            if (o0 + c + 2 * z + 1 < p.o) out[o0 + c + 2 * z + 1] = h[1];
-                        }
+                    if (p.base) {
+#pragma unroll 16
+                        for (int i = 0; i < 32; i++) st_shared2b(at(i, lane), base[(m0 + min(i, rows - 1)) * p.base_stride + oc]);
+                        __syncwarp();
                     }
+                    tmem_ld32(d + g * 32, v);
+                    if (p.bias) add_bias(o0 + g * 32, v);
+                    if (e >= 0) add_bad(m, e, o0 + g * 32, v);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t u[4];
+                        if (p.base) {
+                            const uint4 b = ld_shared4(at(lane, q * 8));
+                            u[0] = b.x, u[1] = b.y, u[2] = b.z, u[3] = b.w;
+#pragma unroll
+                            for (int z = 0; z < 4; z++) {
+                                const float2 f = unpack2<T>(u[z]);
+                                v[q * 8 + 2 * z] += f.x, v[q * 8 + 2 * z + 1] += f.y;
+                            }
+                        }
+#pragma unroll
+                        for (int z = 0; z < 4; z++) u[z] = pack2<T>(v[q * 8 + 2 * z], v[q * 8 + 2 * z + 1]);
+                        st_shared4(at(lane, q * 8), u[0], u[1], u[2], u[3]);
+                    }
+                    __syncwarp();
+#pragma unroll 16
+                    for (int i = 0; i < 32; i++)
+                        if (i < rows && o < p.o) out[(m0 + i) * p.out_stride + o] = ld_shared2b(at(i, lane));
                 }
             }
             tc_fence_before();

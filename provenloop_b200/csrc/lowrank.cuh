@@ -121,7 +121,7 @@ struct PackJobs {
     PackJob job[kMaxPack];
     int jobs, dtype;
     void add(PackJob j) {
-        j.blocks = j.kind == PackJob::LISTS ? j.count : j.kind == PackJob::TO_F32 ? (j.rows + 127) / 128 * (j.dst_cols / 16) * j.count : ((j.rows + 31) / 32) * ((j.dst_cols + 31) / 32) * j.count;
+        j.blocks = j.kind == PackJob::LISTS ? j.count : j.kind == PackJob::TO_F32 ? (j.rows + 127) / 128 * (j.dst_cols / 16) * j.count : ((j.rows + 31) / 32) * ((j.dst_cols + 127) / 128) * j.count;
         job[jobs++] = j;
     }
 };

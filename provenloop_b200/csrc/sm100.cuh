@@ -93,6 +93,13 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
     return v;
 }
 
+__device__ __forceinline__ void st_shared2b(uint32_t at, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory"); }
+__device__ __forceinline__ uint16_t ld_shared2b(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float2 ld_cluster2(uint32_t cluster_addr) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr) : "memory");
