@@ -189,7 +189,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     p.g = take(p.g32, a->adapters * o * rs * 4);
     p.bad = take(p.g32, a->adapters * ((o + 127) / 128) * (rs / 16) * 4);
     p.list = take(p.lists, (a->adapters + 1 + a->n) * 4);
-    p.partial = take(p.lists && a->n, a->n ? grad_partial_bytes((long long)a->n, a->d_in, a->d_out, (int)a->r) : 0);
+    p.partial = take(p.lists && a->n, a->n ? grad_partial_bytes((long long)a->n, a->d_in, a->d_out, (int)a->r, (int)a->adapters) : 0);
     p.bytes = a->n ? at : 0;
     return p;
 }

@@ -852,37 +852,57 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
     if (dependent) grid_dependency_wait();
 }
 
+// Four neighbouring results of one thread, 1024 of a CTA at a time.
+template <class T>
+__device__ __forceinline__ void put4(T* to, const float (&r)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(to) = make_float4(r[0], r[1], r[2], r[3]);
+    } else {
+        T h[4] = {from_f<T>(r[0]), from_f<T>(r[1]), from_f<T>(r[2]), from_f<T>(r[3])};
+        uint2 u;
+        memcpy(&u, h, 8);
+        *reinterpret_cast<uint2*>(to) = u;
+    }
+}
+
 // The gradients of adapters whose tokens lie in several windows, and zeros for
-// those without tokens.
+// those without tokens; `chunks` times 1024 results of a tile per CTA.
 template <class T, int RB>
-__global__ void __launch_bounds__(256) k_grad_sum(const GradPair both, int tiles0, int window, const float* partial) {
+__global__ void __launch_bounds__(256) k_grad_sum(const GradPair both, int tiles0, int window, int chunks, const float* partial) {
     grid_dependency_wait();
-    constexpr int kParts = RB * 8 * 128 / 1024;  // four neighbouring results a thread
-    const int tile = blockIdx.x, e = blockIdx.z, pass = blockIdx.y / kParts, i = (blockIdx.y % kParts * 256 + threadIdx.x) * 4;
+    constexpr int kChunks = RB * 8 * 128 / 1024;
+    const int tile = blockIdx.x, e = blockIdx.z, groups = kChunks / chunks, pass = blockIdx.y / groups;
     const GradArgs a = both.g[tile >= tiles0];
     const int k0 = (tile >= tiles0 ? tile - tiles0 : tile) * 128, j0 = pass * RB * 8;
     const int e0 = both.first[e], e1 = both.first[e + 1], w0 = e0 / window, w1 = e1 > e0 ? (e1 - 1) / window : w0 - 1;
     if (w0 == w1) return;
-    const long long each = (long long)(gridDim.y / kParts) * gridDim.x * (RB * 8 * 128);  // between a window's two sums
-    const float* from = partial + ((long long)pass * gridDim.x + tile) * (RB * 8 * 128) + i;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    const auto add = [&](float4 f) { v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w; };
-    // the adapter begins in its first window and goes on in the others
-    if (w1 > w0) add(*reinterpret_cast<const float4*>(from + (w0 * 2 + 1) * each));
-    int w = w0 + 1;
-    for (; w + 7 <= w1; w += 8) {
-        float4 f[8];
+    const long long each = (long long)(gridDim.y / groups) * gridDim.x * (RB * 8 * 128);  // between a window's two sums
+    for (int chunk = blockIdx.y % groups * chunks, last = chunk + chunks; chunk < last; chunk++) {
+        const int i = (chunk * 256 + threadIdx.x) * 4;
+        const float* from = partial + ((long long)pass * gridDim.x + tile) * (RB * 8 * 128) + i;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const auto add = [&](float4 f) { v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w; };
+        // the adapter begins in its first window and goes on in the others
+        if (w1 > w0) add(*reinterpret_cast<const float4*>(from + (w0 * 2 + 1) * each));
+        int w = w0 + 1;
+        for (; w + 7 <= w1; w += 8) {
+            float4 f[8];
 #pragma unroll
-        for (int q = 0; q < 8; q++) f[q] = *reinterpret_cast<const float4*>(from + (w + q) * 2 * each);
+            for (int q = 0; q < 8; q++) f[q] = *reinterpret_cast<const float4*>(from + (w + q) * 2 * each);
 #pragma unroll
-        for (int q = 0; q < 8; q++) add(f[q]);
-    }
-    for (; w <= w1; w++) add(*reinterpret_cast<const float4*>(from + w * 2 * each));
-    const float r[4] = {v.x, v.y, v.z, v.w};
+            for (int q = 0; q < 8; q++) add(f[q]);
+        }
+        for (; w <= w1; w++) add(*reinterpret_cast<const float4*>(from + w * 2 * each));
+        const float r[4] = {v.x, v.y, v.z, v.w};
+        // along whichever axis of the result is contiguous
+        const int j = a.sk == 1 ? i >> 7 : i % (RB * 8), k = a.sk == 1 ? i & 127 : i / (RB * 8), left = a.sk == 1 ? a.k - (k0 + k) : both.r - (j0 + j);
+        if (a.sk == 1 ? j0 + j >= both.r : k0 + k >= a.k) continue;
+        T* to = static_cast<T*>(a.out) + e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk;
+        if (left >= 4 && reinterpret_cast<uintptr_t>(to) % (4 * sizeof(T)) == 0) put4(to, r);
+        else
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        const int j = a.sk == 1 ? i >> 7 : (i + q) % (RB * 8), k = a.sk == 1 ? (i + q) & 127 : i / (RB * 8);
-        if (j0 + j < both.r && k0 + k < a.k) static_cast<T*>(a.out)[e * a.se + (j0 + j) * a.sj + (long long)(k0 + k) * a.sk] = from_f<T>(r[q]);
+            for (int q = 0; q < 4; q++)
+                if (q < left) to[q] = from_f<T>(r[q]);
     }
 }
 
@@ -937,14 +957,19 @@ template <class T, int RB>
 cudaError_t grad_launch(const GradPair& a, long long n, bool dependent, float* partial, cudaStream_t s) {
     using L = GradTile<T, RB>;
     const int t0 = (a.g[0].k + 127) / 128, t1 = (a.g[1].k + 127) / 128, passes = (a.r + RB * 8 - 1) / (RB * 8);
-    const int window = grad_window(n, a.g[0].k, a.g[1].k, a.r);
+    const int window = grad_window(n, a.g[0].k, a.g[1].k, a.r, a.adapters);
     cudaError_t e = ensure_smem(k_grad<T, RB>, L::kSmem + 1024);  // own[] is beside the tiles
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)(t0 + t1), passes, (unsigned)((n + window - 1) / window)), sums((unsigned)(t0 + t1), passes * (RB * 8 * 128 / 1024), a.adapters);
+    const dim3 grid((unsigned)(t0 + t1), passes, (unsigned)((n + window - 1) / window));
+    // larger parts of a tile per CTA as long as eight CTAs for every SM are left
+    constexpr int kChunks = RB * 8 * 128 / 1024;
+    int chunks = 1;
+    while (chunks < kChunks && (long long)(t0 + t1) * passes * a.adapters * kChunks / (2 * chunks) >= 8 * sm_count()) chunks *= 2;
+    const dim3 sums((unsigned)(t0 + t1), passes * (kChunks / chunks), a.adapters);
     KScope ks("adapter_grad", s, 2);
     e = dependent ? launch_dependent(1, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, window, partial, 1)
                   : launch_cl(1, k_grad<T, RB>, grid, 256, L::kSmem, s, a, t0, window, partial, 0);
-    return e != cudaSuccess ? e : launch_dependent(1, k_grad_sum<T, RB>, sums, 256, 0, s, a, t0, window, static_cast<const float*>(partial));
+    return e != cudaSuccess ? e : launch_dependent(1, k_grad_sum<T, RB>, sums, 256, 0, s, a, t0, window, chunks, static_cast<const float*>(partial));
 }
 
 template <class T>

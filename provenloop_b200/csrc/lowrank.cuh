@@ -139,20 +139,23 @@ constexpr int kSmallTokens = 16;  // up to here W is streamed once past all toke
 inline bool factor_by_token(long long n, long long o, long long r) { return n * o * r * 2 <= 32ll << 20; }
 
 // Places of the tokens' list that a CTA of the gradients takes: three CTAs for
-// each SM over the tiles of 128 features and up to 64 rank indexes, at least
-// 128 places each.
+// each SM over the tiles of 128 features and up to 64 rank indexes, and at least
+// 128 places each, or down to 32 while they hold two adapters or more (each
+// costs a CTA about 3 us however few its tokens: GRADFIG).
 inline int grad_ranks(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : (r + 63) / 64 * 64; }  // padded
 inline long long grad_tiles(long long k0, long long k1) { return (k0 + 127) / 128 + (k1 + 127) / 128; }
 constexpr int kGradSms = 148;  // fixed, so that the sums' order is the same on every device
-inline int grad_window(long long n, long long k0, long long k1, int r) {
+inline int grad_window(long long n, long long k0, long long k1, int r, int adapters) {
     const int sms = kGradSms;
     const long long ctas = grad_tiles(k0, k1) * (r <= 64 ? 1 : (r + 63) / 64);
     long long windows = (3 * sms + ctas - 1) / ctas;
-    if (windows > (n + 127) / 128) windows = (n + 127) / 128;
+    long long most = (n + 31) / 32 < adapters / 2 ? (n + 31) / 32 : adapters / 2;
+    if (most < (n + 127) / 128) most = (n + 127) / 128;
+    if (windows > most) windows = most;
     return (int)((n + windows * 32 - 1) / (windows * 32) * 32);
 }
-inline uint64_t grad_partial_bytes(long long n, long long k0, long long k1, int r) {
-    const int w = grad_window(n, k0, k1, r);
+inline uint64_t grad_partial_bytes(long long n, long long k0, long long k1, int r, int adapters) {
+    const int w = grad_window(n, k0, k1, r, adapters);
     return (uint64_t)((n + w - 1) / w) * 2 * grad_tiles(k0, k1) * 128 * grad_ranks(r) * 4;
 }
 
