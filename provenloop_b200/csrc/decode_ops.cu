@@ -160,7 +160,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_w = a->weight && !p.small && !w_ok;
         p.pack_a = !a_ok && whole_low;
         p.low_vec = (x_ok || p.pack_x) && (a_ok || p.pack_a);
-        p.g32 = !p.small && !factor_by_token((long long)a->n, a->d_out, a->r);
+        p.g32 = !p.small && !factor_by_token((long long)a->n, a->d_out, a->r, a->weight ? a->d_in : 0);
     } else {
         p.pack_x = !x_ok && a->grad_a;
         p.pack_a = !a_ok && a->grad_a;
@@ -168,7 +168,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
         p.pack_grad = !g_ok;
         p.pack_b = true;
         p.low_vec = true;
-        p.g32 = a->out && !factor_by_token((long long)a->n, a->d_in, a->r);
+        p.g32 = a->out && !factor_by_token((long long)a->n, a->d_in, a->r, a->weight ? a->d_out : 0);
     }
     p.lists = backward && a->grad_a;
     uint64_t at = 0;

@@ -14,6 +14,7 @@
 // form into the backward one.  Sums are held in f32 and each result is
 // rounded to its type once.
 #include <climits>
+#include <type_traits>
 
 #include "launch.cuh"
 #include "lowrank.cuh"
@@ -357,26 +358,34 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
 // ---------------------------------------------------------------- projection
 
 // f32: BM x BN outputs per CTA, TM x TN per thread in two halves, 16 of the
-// contraction at a time, the next ones on their way in registers.  The
+// contraction at a time, the next D times as many on their way in registers.  The
 // adapters' terms are more of the same contraction, one after the other for
 // the adapters of the tile, each added to its own tokens' sums only.  A
 // cluster of S CTAs shares both where the tiles are few, and each finishes
-// BM / S of the rows.  On the FMA pipe: the tensor cores' TF32 would need
+// some of the rows.  On the FMA pipe: the tensor cores' TF32 would need
 // three products and rounds its sums towards zero.
-template <int BM, int BN, int TM, int TN>
-__global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int vec_x, int vec_w, int vec_g) {
-    constexpr int BK = 16, LX = BM * BK / 1024, LW = BN * BK / 1024;  // float4 loads of a thread
+template <int BM, int BN>
+struct F32Tile {
+    static constexpr int BK = 16, kTiles = 2 * BK * (BM + 4 + BN + 4) * 4, kSums = BM * (BN + 1) * 4;
+    static constexpr int kSmem = kTiles > kSums ? kTiles : kSums;
+};
+
+template <int BM, int BN, int TM, int TN, int D>
+__global__ void __launch_bounds__(256, BM == 64 ? 2 : 1) k_project_f32(const ProjectArgs a, int vec_x, int vec_w, int vec_g) {
+    constexpr int BK = F32Tile<BM, BN>::BK, LX = BM * BK / 1024, LW = BN * BK / 1024;  // float4 loads of a thread
     static_assert((BM / TM) * (BN / TN) == 256, "one thread per TM x TN outputs");
-    __shared__ __align__(16) float xs[2][BK][BM + 4], ws[2][BK][BN + 4];
+    extern __shared__ __align__(16) float room[];
+    float (*const xs)[BK][BM + 4] = reinterpret_cast<float (*)[BK][BM + 4]>(room);
+    float (*const ws)[BK][BN + 4] = reinterpret_cast<float (*)[BK][BN + 4]>(room + 2 * BK * (BM + 4));
+    float (*const part)[BN + 1] = reinterpret_cast<float (*)[BN + 1]>(room);  // behind the contraction
     __shared__ __align__(16) int ids[BM];
-    constexpr bool kShared = BM == 64;  // the contraction may be shared
-    __shared__ float part[kShared ? BM : 1][BN + 1];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long m0 = (long long)(blockIdx.x / S) * BM;
     const int o0 = blockIdx.y * BN;
-    constexpr int TX = BN / TN;
-    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    static_assert(BN / TN == 16, "16 x 16 threads");
+    // a warp is 4 x 8 of them: its reads of w fill the banks once
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = (warp & 1) * 8 + (lane & 7), ty = (warp >> 1) * 4 + (lane >> 3);
     const auto row_of = [&](int i) { return ty * 4 + i / 4 * (BM / (TM / 4)) + i % 4; };
     const auto col_of = [&](int j) { return tx * 4 + j / 4 * (BN / (TN / 4)) + j % 4; };
     if (threadIdx.x < BM) ids[threadIdx.x] = m0 + threadIdx.x < a.n ? a.id.of(m0 + threadIdx.x) : -1;
@@ -385,83 +394,86 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
     // [b0, b1) of k; of an adapter's factor for the rows in `mine` only
     const auto contract = [&](const float* x, long long x_stride, bool vx, const float* w, long long w_stride, bool w_t, bool vw, int kk,
                               int b0, int b1, auto one, unsigned mine) {
-        float4 nx[LX], nw[LW];
-        // four neighbours of a row that ends at `n`, from a clamped place
-        const auto quad = [](const float* row, int at, int n, bool in, bool vec) {
-            if (vec && in && at + 4 <= n) return *reinterpret_cast<const float4*>(row + at);
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = row[min(at + i, n - 1)];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (!in || at + i >= n) v[i] = 0.f;
-            return make_float4(v[0], v[1], v[2], v[3]);
+        float4 nx[D][LX], nw[D][LW];
+        // four neighbours of a row that ends at `n`, from clamped places: what
+        // is behind the end is replaced by zeros on the way to shared memory,
+        // since a use of the values here would wait for them
+        const auto quad = [](const float* row, int at, int n, bool vec) {
+            if (vec && at + 4 <= n) return *reinterpret_cast<const float4*>(row + at);
+            return make_float4(row[min(at, n - 1)], row[min(at + 1, n - 1)], row[min(at + 2, n - 1)], row[min(at + 3, n - 1)]);
         };
-        const auto load = [&](int b) {
+        const auto load = [&](int b, float4 (&nx)[LX], float4 (&nw)[LW]) {
             const int k0 = b * BK;
 #pragma unroll
             for (int i = 0; i < LX; i++) {
                 const int q = threadIdx.x + 256 * i;
-                const long long m = m0 + q / 4;
-                nx[i] = quad(x + min(m, a.n - 1) * x_stride, k0 + q % 4 * 4, kk, m < a.n, vx);
+                nx[i] = quad(x + min(m0 + q / 4, a.n - 1) * x_stride, k0 + q % 4 * 4, kk, vx);
             }
 #pragma unroll
             for (int i = 0; i < LW; i++) {
                 const int q = threadIdx.x + 256 * i;
-                if (w_t) {
-                    const int k = k0 + q / (BN / 4);
-                    nw[i] = quad(w + (long long)min(k, kk - 1) * w_stride, o0 + q % (BN / 4) * 4, a.o, k < kk, vw);
-                } else {
-                    const int o = o0 + q / 4;
-                    nw[i] = quad(w + (long long)min(o, a.o - 1) * w_stride, k0 + q % 4 * 4, kk, o < a.o, vw);
-                }
+                if (w_t) nw[i] = quad(w + (long long)min(k0 + q / (BN / 4), kk - 1) * w_stride, o0 + q % (BN / 4) * 4, a.o, vw);
+                else nw[i] = quad(w + (long long)min(o0 + q / 4, a.o - 1) * w_stride, k0 + q % 4 * 4, kk, vw);
             }
         };
-        const auto store = [&](int s) {
+        const auto store = [&](int b, int s, float4 (&nx)[LX], float4 (&nw)[LW]) {
+            const int left = kk - b * BK;
+            const auto cut = [&](float4 v, int k) {
+                return make_float4(k < left ? v.x : 0.f, k + 1 < left ? v.y : 0.f, k + 2 < left ? v.z : 0.f, k + 3 < left ? v.w : 0.f);
+            };
 #pragma unroll
             for (int i = 0; i < LX; i++) {
                 const int q = threadIdx.x + 256 * i, m = q / 4, k = q % 4 * 4;
-                xs[s][k][m] = nx[i].x, xs[s][k + 1][m] = nx[i].y, xs[s][k + 2][m] = nx[i].z, xs[s][k + 3][m] = nx[i].w;
+                const float4 v = cut(nx[i], k);
+                xs[s][k][m] = v.x, xs[s][k + 1][m] = v.y, xs[s][k + 2][m] = v.z, xs[s][k + 3][m] = v.w;
             }
 #pragma unroll
             for (int i = 0; i < LW; i++) {
                 const int q = threadIdx.x + 256 * i;
                 if (w_t) {
-                    *reinterpret_cast<float4*>(&ws[s][q / (BN / 4)][q % (BN / 4) * 4]) = nw[i];
+                    const bool in = q / (BN / 4) < left;
+                    *reinterpret_cast<float4*>(&ws[s][q / (BN / 4)][q % (BN / 4) * 4]) = in ? nw[i] : make_float4(0.f, 0.f, 0.f, 0.f);
                 } else {
                     const int o = q / 4, k = q % 4 * 4;
-                    ws[s][k][o] = nw[i].x, ws[s][k + 1][o] = nw[i].y, ws[s][k + 2][o] = nw[i].z, ws[s][k + 3][o] = nw[i].w;
+                    const float4 v = cut(nw[i], k);
+                    ws[s][k][o] = v.x, ws[s][k + 1][o] = v.y, ws[s][k + 2][o] = v.z, ws[s][k + 3][o] = v.w;
                 }
             }
         };
         if (b0 >= b1) return;
-        load(b0);
-        store(0);
+#pragma unroll
+        for (int d = 0; d < D; d++)
+            if (b0 + d < b1) load(b0 + d, nx[d], nw[d]);
+        store(b0, 0, nx[0], nw[0]);
         __syncthreads();
-        for (int b = b0; b < b1; b++) {
-            const int s = (b - b0) & 1;
-            if (b + 1 < b1) load(b + 1);
+        for (int c = b0; c < b1; c += D) {
 #pragma unroll
-            for (int k = 0; k < BK; k++) {
-                float xv[TM], wv[TN];
+            for (int d = 0; d < D; d++) {
+                const int b = c + d, s = (b - b0) & 1;
+                if (b >= b1) break;
+                if (b + D < b1) load(b + D, nx[d], nw[d]);
+#pragma unroll(BM == 64 ? BK : BK / 2)
+                for (int k = 0; k < BK; k++) {  // 128: whole, it would take the registers of the loads under way
+                    float xv[TM], wv[TN];
 #pragma unroll
-                for (int i = 0; i < TM; i += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&xs[s][k][ty * 4 + i / 4 * (BM / (TM / 4))]);
-                    xv[i] = f.x, xv[i + 1] = f.y, xv[i + 2] = f.z, xv[i + 3] = f.w;
+                    for (int i = 0; i < TM; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&xs[s][k][ty * 4 + i / 4 * (BM / (TM / 4))]);
+                        xv[i] = f.x, xv[i + 1] = f.y, xv[i + 2] = f.z, xv[i + 3] = f.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < TN; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&ws[s][k][tx * 4 + i / 4 * (BN / (TN / 4))]);
+                        wv[i] = f.x, wv[i + 1] = f.y, wv[i + 2] = f.z, wv[i + 3] = f.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < TM; i++)
+                        if (!decltype(one)::value || (mine >> i & 1))
+#pragma unroll
+                            for (int j = 0; j < TN; j++) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
                 }
-#pragma unroll
-                for (int i = 0; i < TN; i += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&ws[s][k][tx * 4 + i / 4 * (BN / (TN / 4))]);
-                    wv[i] = f.x, wv[i + 1] = f.y, wv[i + 2] = f.z, wv[i + 3] = f.w;
-                }
-#pragma unroll
-                for (int i = 0; i < TM; i++)
-                    if (!decltype(one)::value || (mine >> i & 1))
-#pragma unroll
-                        for (int j = 0; j < TN; j++) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+                if (b + 1 < b1) store(b + 1, s ^ 1, nx[(d + 1) % D], nw[(d + 1) % D]);
+                __syncthreads();
             }
-            if (b + 1 < b1) store(s ^ 1);
-            __syncthreads();
         }
     };
     if (a.w) {
@@ -492,22 +504,21 @@ __global__ void __launch_bounds__(256) k_project_f32(const ProjectArgs a, int ve
         if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
         static_cast<float*>(a.out)[m * a.out_stride + o] = v;
     };
-    if constexpr (kShared) {
+    if (S > 1) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
 #pragma unroll
             for (int j = 0; j < TN; j++) part[row_of(i)][col_of(j)] = acc[i][j];
-        if (S > 1) cluster.sync();
-        else __syncthreads();
-        const int rows = BM / S;
+        cluster.sync();
+        const int row0 = BM * rank / S, rows = BM * (rank + 1) / S - row0;
         for (int q = threadIdx.x; q < rows * BN; q += 256) {
-            const int row = rank * rows + q / BN, col = q % BN;
+            const int row = row0 + q / BN, col = q % BN;
             if (m0 + row >= a.n || o0 + col >= a.o) continue;
             float v = 0.f;
-            for (int c = 0; c < S; c++) v += S > 1 ? *cluster.map_shared_rank(&part[row][col], c) : part[row][col];
+            for (int c = 0; c < S; c++) v += *cluster.map_shared_rank(&part[row][col], c);
             finish(m0 + row, o0 + col, v);
         }
-        if (S > 1) cluster.sync();
+        cluster.sync();
     } else {
 #pragma unroll
         for (int i = 0; i < TM; i++)
@@ -1008,13 +1019,25 @@ cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
     KScope ks("adapter_project", s);
     // a factor's rows: r rows of o elements, or o rows of r
     const int vg = vec(a.g.p, a.g.sk == 1 && a.g.sj != 1 ? a.g.sj : a.g.sk, 2) && (a.id.count == 1 || a.g.se % 4 == 0);
-    // large tiles where they fill the SMs, else small ones whose contraction
-    // is shared until they do, 64 of it for each CTA at least
-    const long long large = ((a.n + 127) / 128) * ((a.o + 127) / 128), small = ((a.n + 63) / 64) * ((a.o + 63) / 64);
-    if (large >= sm_count()) return launch_cl(1, k_project_f32<128, 128, 8, 8>, dim3((unsigned)((a.n + 127) / 128), (a.o + 127) / 128), 256, 0, s, a, vx, vw, vg);
-    int S = 1;
-    while (S < 8 && a.w && small * S < 2 * sm_count() && a.k >= 128 * S) S *= 2;
-    return launch_cl(S, k_project_f32<64, 64, 4, 4>, dim3((unsigned)((a.n + 63) / 64 * S), (a.o + 63) / 64), 256, 0, s, a, vx, vw, vg);
+    // The tile and the number of CTAs that share a contraction with the least
+    // time on the SM with the most CTAs: a 64 x 64 tile takes 0.35 of a
+    // 128 x 128 one, whose operands' way from shared memory costs half, and
+    // clusters of four and more leave some SMs of each group out.
+    int tile = 64, S = 1;
+    double least = 1e300;
+    for (int size = 64; size <= 128; size *= 2) {
+        const long long tiles = (a.n + size - 1) / size * ((a.o + size - 1) / size);
+        for (int c = 1; c <= 8 && (c == 1 || (a.w && a.k >= 64 * c)); c *= 2) {
+            const int sms = c < 4 ? sm_count() : sm_count() * 128 / 148;
+            const double cost = ((double)((tiles * c + sms - 1) / sms) / c + 0.005 * c) * (size == 64 ? 0.35 : 1);
+            if (cost < least) tile = size, S = c, least = cost;
+        }
+    }
+    const auto go = [&](auto kern, size_t smem) {
+        const cudaError_t e = ensure_smem(kern, smem);
+        return e != cudaSuccess ? e : launch_cl(S, kern, dim3((unsigned)((a.n + tile - 1) / tile * S), (a.o + tile - 1) / tile), 256, smem, s, a, vx, vw, vg);
+    };
+    return tile == 64 ? go(k_project_f32<64, 64, 4, 4, 4>, F32Tile<64, 64>::kSmem) : go(k_project_f32<128, 128, 8, 8, 1>, F32Tile<128, 128>::kSmem);
 }
 
 cudaError_t launch_project_small(const ProjectArgs& a, int dtype, cudaStream_t s) {

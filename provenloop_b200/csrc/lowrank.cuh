@@ -135,8 +135,12 @@ inline bool low_by_token(long long n, long long k0, long long k1, long long r) {
 constexpr int kSmallTokens = 16;  // up to here W is streamed once past all tokens
 // The projection takes each token's factor from where it is, n o r elements
 // in all, up to 32 MiB of them; above that the factors are converted first
-// and shared by the tokens of a tile.
-inline bool factor_by_token(long long n, long long o, long long r) { return n * o * r * 2 <= 32ll << 20; }
+// and shared by the tokens of a tile.  Tiles too few for half of the SMs with
+// a long contraction (k, 0 without a shared projection) take it all the same,
+// since only that way shares a contraction: FACTORFIG.
+inline bool factor_by_token(long long n, long long o, long long r, long long k) {
+    return n * o * r * 2 <= 32ll << 20 || (k >= 4096 && ((n + 127) / 128) * ((o + 63) / 64) < 74);
+}
 
 // Places of the tokens' list that a CTA of the gradients takes: three CTAs for
 // each SM over the tiles of 128 features and up to 64 rank indexes, and at least
