@@ -150,7 +150,7 @@ Plan plan_of(const ts_adapter_args* a, int backward) {
     const bool x_ok = rows_ok(a->x, a->n, a->d_in, a->x_stride, size), w_ok = rows_ok(a->weight, a->d_out, a->d_in, a->weight_stride, size);
     const bool a_ok = rows_ok(a->lora_a, 2, a->d_in, a->d_in, size), g_ok = rows_ok(a->grad, a->n, a->d_out, a->grad_stride, size);
     p.small = !p.f32 && !backward && a->n <= (uint64_t)kSmallTokens && (!a->weight || (x_ok && w_ok));
-    const bool whole_low = !low_by_token((long long)a->n, a->d_in, a->d_in, a->r);  // by matrix instructions: aligned operands only
+    const bool whole_low = !low_by_token((long long)a->n, a->d_in, a->d_in, a->r, a->adapters);  // by matrix instructions: aligned operands only
     if (p.f32) {
         p.low_vec = !backward && x_ok && a_ok;
         p.pack_x = backward && a->grad_a && !x_ok;

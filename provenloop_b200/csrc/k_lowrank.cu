@@ -360,10 +360,13 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
 // f32: BM x BN outputs per CTA, TM x TN per thread in two halves, 16 of the
 // contraction at a time, the next D times as many on their way in registers.  The
 // adapters' terms are more of the same contraction, one after the other for
-// the adapters of the tile, each added to its own tokens' sums only.  A
+// up to kF32Adapters adapters of the tile, each added to its own tokens' sums
+// only; with more of them each output takes its token's own.  A
 // cluster of S CTAs shares both where the tiles are few, and each finishes
 // some of the rows.  On the FMA pipe: the tensor cores' TF32 would need
 // three products and rounds its sums towards zero.
+constexpr int kF32Adapters = 8;
+
 template <int BM, int BN>
 struct F32Tile {
     static constexpr int BK = 16, kTiles = 2 * BK * (BM + 4 + BN + 4) * 4, kSums = BM * (BN + 1) * 4;
@@ -483,15 +486,19 @@ __global__ void __launch_bounds__(256, BM == 64 ? 2 : 1) k_project_f32(const Pro
     }
     __syncthreads();
     const bool g_t = a.g.sk == 1 && a.g.sj != 1;  // [r][o], else [o][r]
-    for (int e = -1, at = 0;; at++) {
-        int next = INT_MAX;  // the tile's adapters in ascending order; every thread looks for itself
+    int distinct = 0;
+    const auto above = [&](int e) {  // the tile's next adapter; every thread looks for itself
+        int next = INT_MAX;
 #pragma unroll 4
         for (int i = 0; i < BM; i += 4) {
             const int4 q = *reinterpret_cast<const int4*>(ids + i);
             next = min(min(next, q.x > e ? q.x : INT_MAX), min(q.y > e ? q.y : INT_MAX, min(q.z > e ? q.z : INT_MAX, q.w > e ? q.w : INT_MAX)));
         }
-        if (next == INT_MAX) break;
-        e = next;
+        return next;
+    };
+    for (int e = above(-1); e != INT_MAX && distinct <= kF32Adapters; e = above(e)) distinct++;
+    const bool each = distinct > kF32Adapters;
+    for (int e = above(-1), at = 0; !each && e != INT_MAX; e = above(e), at++) {
         if (at % S != rank) continue;
         unsigned mine = 0;
 #pragma unroll
@@ -502,14 +509,27 @@ __global__ void __launch_bounds__(256, BM == 64 ? 2 : 1) k_project_f32(const Pro
     const auto finish = [&](long long m, int o, float v) {
         if (a.bias) v += static_cast<const float*>(a.bias)[o];
         if (a.base) v += static_cast<const float*>(a.base)[m * a.base_stride + o];
+        if (each && ids[m - m0] >= 0) {
+            const float *low = a.low + m * low_stride(a.r), *g = static_cast<const float*>(a.g.p) + ids[m - m0] * a.g.se + o * a.g.sk;
+            constexpr int U = 8;  // blocks of loads from clamped places
+            for (int j = 0; j < a.r; j += U) {
+                float l[U], f[U];
+#pragma unroll
+                for (int i = 0; i < U; i++) l[i] = low[min(j + i, a.r - 1)], f[i] = g[min(j + i, a.r - 1) * a.g.sj];
+#pragma unroll
+                for (int i = 0; i < U; i++)
+                    if (j + i < a.r) v = fmaf(l[i], f[i], v);
+            }
+        }
         static_cast<float*>(a.out)[m * a.out_stride + o] = v;
     };
-    if (S > 1) {
+    if (S > 1 || each) {
 #pragma unroll
         for (int i = 0; i < TM; i++)
 #pragma unroll
             for (int j = 0; j < TN; j++) part[row_of(i)][col_of(j)] = acc[i][j];
-        cluster.sync();
+        if (S > 1) cluster.sync();
+        else __syncthreads();
         const int row0 = BM * rank / S, rows = BM * (rank + 1) / S - row0;
         for (int q = threadIdx.x; q < rows * BN; q += 256) {
             const int row = row0 + q / BN, col = q % BN;
@@ -518,7 +538,7 @@ __global__ void __launch_bounds__(256, BM == 64 ? 2 : 1) k_project_f32(const Pro
             for (int c = 0; c < S; c++) v += *cluster.map_shared_rank(&part[row][col], c);
             finish(m0 + row, o0 + col, v);
         }
-        cluster.sync();
+        if (S > 1) cluster.sync();
     } else {
 #pragma unroll
         for (int i = 0; i < TM; i++)
@@ -926,7 +946,7 @@ int sm_count() {
 template <class T>
 cudaError_t low_launch(const LowArgs* a, int count, bool vec, const int* after_pack, cudaStream_t s) {
     const long long n = a[0].n;
-    if (sizeof(T) == 2 && !low_by_token(n, a[0].k, a[count - 1].k, a[0].r))
+    if (sizeof(T) == 2 && !low_by_token(n, a[0].k, a[count - 1].k, a[0].r, a[0].id.count))
         return launch_low_tc(a, count, std::is_same<T, __half>::value ? DT_F16 : DT_BF16, after_pack, s);
     const LowPair both{{a[0], a[count - 1]}, {after_pack[0], after_pack[count - 1]}};
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;

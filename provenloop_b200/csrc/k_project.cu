@@ -54,7 +54,7 @@ struct Tile {
 struct TcArgs {
     ProjectArgs p;
     int tiles_m, tiles_n, kblocks;
-    int split, x_rows;    // k_project_split
+    int split, rows, x_rows;  // k_project_split
     int vec_bias;         // 16-byte loads are aligned
     int tma_out;          // out, and base if there is one, take TMA boxes
 };
@@ -711,8 +711,8 @@ k_project_split(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ProjectArgs& p = a.p;
     const int S = a.split, rank = (int)cluster_rank();
-    const long long m0 = (long long)(blockIdx.x / S) * 128;
-    const int o0 = blockIdx.y * BN, rows = (int)min(128LL, p.n - m0);
+    const long long m0 = (long long)(blockIdx.x / S) * a.rows;
+    const int o0 = blockIdx.y * BN, rows = (int)min((long long)a.rows, p.n - m0);
     const int per = BN / S, col0 = rank * per;  // this CTA's outputs
     const bool early = rows * per <= L::kEarly;
     const int kb0 = a.kblocks * rank / S, kb1 = a.kblocks * (rank + 1) / S;
@@ -840,7 +840,13 @@ cudaError_t launch_split(const ProjectArgs& p, int sms, cudaStream_t s) {
     // has two slices of the contraction and eight outputs of a row
     a.split = 1;
     while (a.split < 8 && (long long)a.tiles_m * a.tiles_n * a.split < sms && a.kblocks >= 4 * a.split) a.split *= 2;
-    a.x_rows = p.n < 128 ? (int)(p.n + 7) / 8 * 8 : 128;  // rows behind stay whatever they are: their sums are not used
+    // where that is not enough, tiles of fewer tokens, for the adapters' terms
+    a.rows = 128;
+    while (a.rows > 32 && p.n > a.rows / 2 && (long long)a.tiles_m * a.tiles_n * a.split < sms) {
+        a.rows /= 2;
+        a.tiles_m = (int)((p.n + a.rows - 1) / a.rows);
+    }
+    a.x_rows = p.n < a.rows ? (int)(p.n + 7) / 8 * 8 : a.rows;  // rows behind stay whatever they are: their sums are not used
     CUtensorMap mx{}, mw{};
     auto kern = k_project_split<T, BN, W_MN>;
     cudaError_t e = operand_maps<T, W_MN>(p, a.x_rows, BN, &mx, &mw);

@@ -129,23 +129,31 @@ struct PackJobs {
 // The kernels that a call takes go by its sizes; decode_ops.cu lays out the
 // workspace with the same rules.
 // Low token by token reads each token's factor (from L2 where tokens share
-// it): for f32 always, else up to 48 MiB of such reads, where it is faster than
-// matrix instructions if every token has an adapter of its own.
-inline bool low_by_token(long long n, long long k0, long long k1, long long r) { return n * r * (k0 > k1 ? k0 : k1) * 2 <= 48ll << 20; }
+// it): for f32 always, else up to 48 MiB of such reads, and up to 256 MiB where
+// a tile of the matrix form may have to go past x more than four times for its
+// tokens' adapters (739 tokens of 47 adapters of rank 64 over 1536: 26 us token
+// by token, 157 us as a matrix; 3453 tokens in 23 requests of rank 16: 31 and 10).
+inline bool low_by_token(long long n, long long k0, long long k1, long long r, long long adapters) {
+    const long long bytes = n * r * (k0 > k1 ? k0 : k1) * 2, tile = n < 128 ? n : 128;
+    const long long units = (adapters < tile ? adapters : tile) * (low_stride((int)r) / 16);
+    return bytes <= (units > 32 ? 256ll : 48ll) << 20;
+}
 constexpr int kSmallTokens = 16;  // up to here W is streamed once past all tokens
 // The projection takes each token's factor from where it is, n o r elements
 // in all, up to 32 MiB of them; above that the factors are converted first
 // and shared by the tokens of a tile.  Tiles too few for half of the SMs with
 // a long contraction (k, 0 without a shared projection) take it all the same,
-// since only that way shares a contraction: FACTORFIG.
+// since only that way shares a contraction (217 tokens, 8960 -> 1536, rank 64:
+// 80 us for the backward call, 85 with converted factors).
 inline bool factor_by_token(long long n, long long o, long long r, long long k) {
     return n * o * r * 2 <= 32ll << 20 || (k >= 4096 && ((n + 127) / 128) * ((o + 63) / 64) < 74);
 }
 
 // Places of the tokens' list that a CTA of the gradients takes: three CTAs for
 // each SM over the tiles of 128 features and up to 64 rank indexes, and at least
-// 128 places each, or down to 32 while they hold two adapters or more (each
-// costs a CTA about 3 us however few its tokens: GRADFIG).
+// 128 places each, or down to 8 while they hold two adapters or more (each
+// costs a CTA 3 to 10 us however few its tokens: 72 tokens of 42 adapters of
+// rank 64 over 1536 + 1536 take 57 us so and 147 us in windows of 32).
 inline int grad_ranks(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : (r + 63) / 64 * 64; }  // padded
 inline long long grad_tiles(long long k0, long long k1) { return (k0 + 127) / 128 + (k1 + 127) / 128; }
 constexpr int kGradSms = 148;  // fixed, so that the sums' order is the same on every device
@@ -153,9 +161,10 @@ inline int grad_window(long long n, long long k0, long long k1, int r, int adapt
     const int sms = kGradSms;
     const long long ctas = grad_tiles(k0, k1) * (r <= 64 ? 1 : (r + 63) / 64);
     long long windows = (3 * sms + ctas - 1) / ctas;
-    long long most = (n + 31) / 32 < adapters / 2 ? (n + 31) / 32 : adapters / 2;
+    long long most = (n + 7) / 8 < adapters / 2 ? (n + 7) / 8 : adapters / 2;
     if (most < (n + 127) / 128) most = (n + 127) / 128;
     if (windows > most) windows = most;
+    if (windows * 32 > n) return (int)((n + windows * 8 - 1) / (windows * 8) * 8);
     return (int)((n + windows * 32 - 1) / (windows * 32) * 32);
 }
 inline uint64_t grad_partial_bytes(long long n, long long k0, long long k1, int r, int adapters) {
