@@ -320,7 +320,7 @@ int ts_adapter_project(const ts_adapter_args* args);
  * held fixed: out[m] = grad[m] weight + u[m] lora_a_e with u[m] = scale_e
  * grad[m] lora_b_e; grad_a_e = sum of u[m]^T x[m] and grad_b_e = scale_e sum
  * of grad[m]^T (x[m] lora_a_e^T) over the adapter's tokens (zero without
- * any), in an order fixed by the sizes alone.  The gradient of base is grad. */
+ * any), in an order fixed by the sizes and indexes alone.  The gradient of base is grad. */
 int ts_adapter_project_backward(const ts_adapter_args* args);
 
 /* Waits within a kernel of ts_adapter_* or ts_logit_rules that ran out (two seconds) on

