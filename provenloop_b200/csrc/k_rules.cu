@@ -23,12 +23,16 @@
 // they name, and for those one word each, found by counting the bits before
 // the token's.  The named tokens are computed first, from the lists' side; the
 // stream over the segments takes them, like masked tokens, as -inf, and they
-// are written over it in the end.  The stream selects by a table of the 256
-// masks of eight elements and works on pairs of 16-bit values: instructions,
-// not bytes, were its bound with one select and one comparison per logit, and
-// still are: 64 rows of 151936 in f32 with every rule take 28 us (2.8 TB/s), 256
-// rows in bf16 of which only the picks are wanted 39 us (2.0 TB/s), one row with
-// 4096 tokens of history 12 us.
+// are written over it in the end.  The stream works on pairs of 16-bit values
+// and on four vectors a thread at a time, and compares them with the greatest
+// value that the CTA has seen, so that hardly a warp has to look closer.
+//
+// What bounds it now: the lists, which keep the stream waiting for a third of
+// the time (their loads queue behind the first segments), and half of the
+// issue slots.  64 rows of 151936 in f32 with every rule take 28 us (2.8 TB/s),
+// 256 rows in bf16 of which only the picks are wanted 36 us (2.2 TB/s; 39 us when
+// each thread compared with its own greatest), one row with 4096 tokens of
+// history 12 to 14 us.
 #include <climits>
 
 #include "launch.cuh"
@@ -64,12 +68,17 @@ __device__ __forceinline__ void take_any(Best& b, float z, uint32_t v) {
     if (nz ? (!nb || v < b.v) : (!nb && (z > b.z || (z == b.z && v < b.v && z != -INFINITY)))) b.z = z, b.v = v;
 }
 
+// Orders values as integers, NaN above all, and back.
+__device__ __forceinline__ uint32_t order_of(float z) {
+    const uint32_t u = __float_as_uint(z + 0.f);  // -0 counts as 0
+    return z != z ? UINT_MAX : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) && k != UINT_MAX ? k & 0x7fffffffu : k == UINT_MAX ? k : ~k); }
+
 // Orders (z, lowest v) as an integer; 0 below everything.
 __device__ __forceinline__ unsigned long long key_of(const Best& b) {
     if (b.v == UINT_MAX) return 0ull;
-    const uint32_t u = __float_as_uint(b.z + 0.f);  // -0 counts as 0
-    const uint32_t k = b.z != b.z ? UINT_MAX : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-    return (unsigned long long)k << 32 | (uint32_t)~b.v;
+    return (unsigned long long)order_of(b.z) << 32 | (uint32_t)~b.v;
 }
 
 template <class T>
@@ -105,21 +114,32 @@ template <class T>
 struct Vec;
 template <>
 struct Vec<float> {
-    static __device__ __forceinline__ void select(uint4& x, uint32_t ok, const uint4*) {
+    static __device__ __forceinline__ void select(uint4& x, uint32_t ok) {
         constexpr uint32_t low = 0xff800000u;
         x.x = ok & 1 ? x.x : low, x.y = ok & 2 ? x.y : low, x.z = ok & 4 ? x.z : low, x.w = ok & 8 ? x.w : low;
     }
     static __device__ __forceinline__ float top(const uint4& x) {
         return max_nan(max_nan(__uint_as_float(x.x), __uint_as_float(x.y)), max_nan(__uint_as_float(x.z), __uint_as_float(x.w)));
     }
+    static __device__ __forceinline__ float top4(const uint4 (&x)[4]) {
+        return max_nan(max_nan(top(x[0]), top(x[1])), max_nan(top(x[2]), top(x[3])));
+    }
 };
 template <class T>
 struct Vec16 {
     static constexpr uint32_t kLow = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-    static __device__ __forceinline__ void select(uint4& x, uint32_t ok, const uint4* table) {
-        const uint4 m = table[ok & 255];
-        x.x = (x.x & m.x) | (kLow & ~m.x), x.y = (x.y & m.y) | (kLow & ~m.y);
-        x.z = (x.z & m.z) | (kLow & ~m.z), x.w = (x.w & m.w) | (kLow & ~m.w);
+    // Four bits to the sign bits of a word's bytes, by one product without
+    // carries, and each sign over half a word.
+    static __device__ __forceinline__ void select(uint4& x, uint32_t ok) {
+        const uint32_t lo = (ok & 0x0f) * 0x10204080u, hi = (ok & 0xf0) * 0x01020408u;
+        const auto spread = [](uint32_t signs, uint32_t bytes) {
+            uint32_t m;
+            asm("prmt.b32 %0, %1, 0, %2;" : "=r"(m) : "r"(signs), "r"(bytes));
+            return m;
+        };
+        const uint32_t m0 = spread(lo, 0x9988u), m1 = spread(lo, 0xbbaau), m2 = spread(hi, 0x9988u), m3 = spread(hi, 0xbbaau);
+        x.x = (x.x & m0) | (kLow & ~m0), x.y = (x.y & m1) | (kLow & ~m1);
+        x.z = (x.z & m2) | (kLow & ~m2), x.w = (x.w & m3) | (kLow & ~m3);
     }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
@@ -127,10 +147,14 @@ struct Vec16 {
         else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
-    static __device__ __forceinline__ float top(const uint4& x) {
-        const uint32_t m = max2(max2(x.x, x.y), max2(x.z, x.w));
+    static __device__ __forceinline__ uint32_t pair(const uint4& x) { return max2(max2(x.x, x.y), max2(x.z, x.w)); }
+    static __device__ __forceinline__ float single(uint32_t m) {
         const T* h = reinterpret_cast<const T*>(&m);
         return max_nan(load_f(h[0]), load_f(h[1]));
+    }
+    static __device__ __forceinline__ float top(const uint4& x) { return single(pair(x)); }
+    static __device__ __forceinline__ float top4(const uint4 (&x)[4]) {
+        return single(max2(max2(pair(x[0]), pair(x[1])), max2(pair(x[2]), pair(x[3]))));
     }
 };
 template <>
@@ -140,19 +164,20 @@ struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
 
 // Where a kernel's dynamic shared memory has what, in 32-bit words.
 struct RulesLayout {
-    uint32_t segment, block, buffers, bits, before, count, bias, pos, ok, buf, bytes;
+    uint32_t segment, block, buffers, bits, before, count, bias, pos, ok, ok_words, buf, bytes;
     // span: tokens of a CTA's part of the row; most: entries of its lists
     RulesLayout(uint32_t span, uint32_t block_, uint64_t most, bool biases, uint32_t segment_, uint32_t size, uint32_t buffers_) {
         segment = segment_, block = span < block_ ? span : block_, buffers = buffers_;
         const uint32_t groups = (block + 127) / 128, named = (uint32_t)((most < block ? most : block) + 31) / 32 * 32;
-        uint32_t at = 1024;  // the table of masks
+        uint32_t at = 0;
         bits = at, at += named ? groups * 4 : 0;  // groups of 128 tokens
         before = at, at += named ? (groups + 3) / 4 * 4 : 0;
         count = at, at += named;
         bias = at, at += biases ? named : 0;
         pos = at, at += named;
         const uint32_t held = span < segment ? span : segment;  // a multiple of 128
-        ok = at, at += held / 32;
+        ok_words = held / 32;  // of one segment
+        ok = at, at += ok_words * 2;
         buf = at = (at + 31) / 32 * 32;
         bytes = at * 4 + held * size * buffers;
     }
@@ -169,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
     constexpr int kHeld = 8;  // entries of the history that a thread keeps in registers
     extern __shared__ __align__(128) uint32_t smem[];
     __shared__ uint64_t arrived[2];
-    __shared__ uint32_t dead, warp_bits[kThreads / 32];
+    __shared__ uint32_t dead, warp_bits[kThreads / 32], floor_of;  // the CTA's greatest before this segment
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), cl = (int)cluster.num_blocks();
     const long long row = blockIdx.x / cl;
@@ -183,7 +208,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
     const uint32_t first = min(end, rank * span), last = min(end, first + span);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const uint4* table = reinterpret_cast<const uint4*>(smem);
     uint32_t *bits = smem + l.bits, *before = smem + l.before, *count = smem + l.count, *bias = smem + l.bias, *pos = smem + l.pos,
              *okw = smem + l.ok;
     T* bufs = reinterpret_cast<T*>(smem + l.buf);
@@ -201,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
         mbar_init(&arrived[0], 1);
         mbar_init(&arrived[1], 1);
         dead = 0;
+        floor_of = order_of(-INFINITY);
         fence_async_shared();
         fetch(0);
         if (l.buffers == 2) fetch(1);
@@ -240,12 +265,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
             if (threadIdx.x + q * kThreads < hist) held[q] = place(v[q], a.vocab);
     }
     if (threadIdx.x < biases) held_bias = place(list_at(a.bias_ids, a.bias64, bid0 + threadIdx.x), a.vocab);
-    if (sizeof(T) == 2 && !plain && threadIdx.x < 256) {
-        const uint32_t b = threadIdx.x;
-        const auto pair = [&](int i) { return (b >> i & 1 ? 0xffffu : 0u) | (b >> (i + 1) & 1 ? 0xffff0000u : 0u); };
-        reinterpret_cast<uint4*>(smem)[b] = make_uint4(pair(0), pair(2), pair(4), pair(6));
-    }
-
     Best named{-INFINITY, UINT_MAX}, best{-INFINITY, UINT_MAX};
     // this thread's first vector with the greatest element; which it is is found in the end
     float top = -INFINITY;
@@ -333,54 +352,85 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
                 take_any(named, z, v);
                 count[i] = __float_as_uint(z);
             }
-            __syncthreads();  // every named logit has been read: out may be logits itself
         }
+        // which tokens of the segment from `lo` on the stream takes as they are,
+        // and the mask's words of the segment behind it
+        const auto prepare = [&](uint32_t lo, uint32_t* to) {
+            const uint32_t used = (min(blk_end, lo + l.segment) - lo + 31) / 32;
+#pragma unroll
+            for (uint32_t q = 0; q < kPer; q++) {
+                const uint32_t i = threadIdx.x + q * kThreads;
+                if (i < used) to[i] = (mask ? next_mask[q] : UINT_MAX) & ~(lists ? bits[(lo - blk) / 32 + i] : 0u);
+            }
+            if (mask && lo + l.segment < last) {
+#pragma unroll
+                for (uint32_t q = 0; q < kPer; q++) next_mask[q] = mask_at(lo + l.segment + (threadIdx.x + q * kThreads) * 32);
+            }
+        };
+        if (!plain) prepare(blk, okw + (s & 1) * l.ok_words);
+        __syncthreads();  // also, every named logit has been read: out may be logits itself
         for (uint32_t lo = blk; lo < blk_end; lo += l.segment, s++) {
-            const uint32_t hi = min(blk_end, lo + l.segment), used = (hi - lo + 31) / 32;
-            const uint32_t at = s & (l.buffers - 1);
+            const uint32_t hi = min(blk_end, lo + l.segment), at = s & (l.buffers - 1);
             const T* buf = bufs + at * l.segment;
-            if (!plain) {
+            const uint32_t* ok_bits = okw + (s & 1) * l.ok_words;
+            mbar_wait(&arrived[at], s / l.buffers & 1, &dead);
+            // what all threads have seen in earlier segments, at lower ids: once a
+            // few segments are through, hardly a warp finds a greater one
+            const float below = value_of(*const_cast<volatile uint32_t*>(&floor_of));
+            if (!(top >= below) && top == top) top = below, top_at = kNone;
+            const uint32_t top_was = top_at;
+            const auto see = [&](const uint4& z, uint32_t v) {
+                const float m = Vec<T>::top(z);
+                if (!(m <= top) && top == top) top = m, top_at = v, top_z = z;  // a NaN, once there, stays
+            };
+            const auto put = [&](const uint4& z, uint32_t v) {
+                const T* e = reinterpret_cast<const T*>(&z);
+                O* to = out + v;
+                if (!out_vec) {
 #pragma unroll
-                for (uint32_t q = 0; q < kPer; q++) {
-                    const uint32_t i = threadIdx.x + q * kThreads;
-                    if (i < used) okw[i] = (mask ? next_mask[q] : UINT_MAX) & ~(lists ? bits[(lo - blk) / 32 + i] : 0u);
+                    for (uint32_t i = 0; i < VEC; i++) store_f(to + i, load_f(e[i]));
+                } else if constexpr (std::is_same<T, O>::value) {
+                    *reinterpret_cast<uint4*>(to) = z;
+                } else {
+                    float4 f[VEC / 4];
+#pragma unroll
+                    for (uint32_t i = 0; i < VEC / 4; i++)
+                        f[i] = make_float4(load_f(e[4 * i]), load_f(e[4 * i + 1]), load_f(e[4 * i + 2]), load_f(e[4 * i + 3]));
+#pragma unroll
+                    for (uint32_t i = 0; i < VEC / 4; i++) reinterpret_cast<float4*>(to)[i] = f[i];
                 }
-                if (mask && hi < last) {
+            };
+            constexpr uint32_t kStep = kThreads * VEC;
+            uint32_t q = threadIdx.x * VEC;
+            // four vectors a thread at once where they lie in the segment: one
+            // comparison with the greatest so far, which seldom finds a greater
+            const uint32_t whole = lo >= head ? (hi - lo) / (4 * kStep) * (4 * kStep) : 0u;
+            for (; q < whole; q += 4 * kStep) {
+                uint4 z[4];
 #pragma unroll
-                    for (uint32_t q = 0; q < kPer; q++) next_mask[q] = mask_at(hi + (threadIdx.x + q * kThreads) * 32);
+                for (uint32_t j = 0; j < 4; j++) z[j] = *reinterpret_cast<const uint4*>(buf + q + j * kStep);
+                if (!plain) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) Vec<T>::select(z[j], ok_bits[q / 32 + j * (kStep / 32)] >> q % 32);
+                }
+                if (!(Vec<T>::top4(z) <= top) && top == top) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) see(z[j], lo + q + j * kStep - head);
+                }
+                if (out) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) put(z[j], lo + q + j * kStep - head);
                 }
             }
-            __syncthreads();
-            mbar_wait(&arrived[at], s / l.buffers & 1, &dead);
-            for (uint32_t q = threadIdx.x * VEC; q < hi - lo; q += kThreads * VEC) {
+            for (; q < hi - lo; q += kStep) {
                 const uint32_t p0 = lo + q;
                 // the vector's bits: VEC <= 8 of them lie in one word
-                const uint32_t ok = plain ? UINT_MAX : okw[q / 32] >> q % 32;
+                const uint32_t ok = plain ? UINT_MAX : ok_bits[q / 32] >> q % 32;
                 if (p0 >= head && p0 + VEC <= hi) {
                     uint4 z = *reinterpret_cast<const uint4*>(buf + q);
-                    if (!plain) Vec<T>::select(z, ok, table);
-                    const float m = Vec<T>::top(z);
-                    if (!(m <= top) && top == top) top = m, top_at = p0 - head, top_z = z;  // a NaN, once there, stays
-                    const T* e = reinterpret_cast<const T*>(&z);
-                    if (out) {
-                        O* to = out + (p0 - head);
-                        if constexpr (std::is_same<T, O>::value) {
-                            if (out_vec) {
-                                *reinterpret_cast<uint4*>(to) = z;
-                                continue;
-                            }
-                        } else if (out_vec) {
-                            float4 f[VEC / 4];
-#pragma unroll
-                            for (uint32_t i = 0; i < VEC / 4; i++)
-                                f[i] = make_float4(load_f(e[4 * i]), load_f(e[4 * i + 1]), load_f(e[4 * i + 2]), load_f(e[4 * i + 3]));
-#pragma unroll
-                            for (uint32_t i = 0; i < VEC / 4; i++) reinterpret_cast<float4*>(to)[i] = f[i];
-                            continue;
-                        }
-#pragma unroll
-                        for (uint32_t i = 0; i < VEC; i++) store_f(to + i, load_f(e[i]));
-                    }
+                    if (!plain) Vec<T>::select(z, ok);
+                    see(z, p0 - head);
+                    if (out) put(z, p0 - head);
                 } else {
                     // the row's ends, which did not come with the copy
 #pragma unroll 1
@@ -393,7 +443,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
                     }
                 }
             }
+            const uint32_t new_floor = top_at != top_was ? order_of(top) : 0u;
+            if (!plain && hi < blk_end) prepare(hi, okw + (~s & 1) * l.ok_words);
             __syncthreads();
+            if (new_floor) atomicMax(&floor_of, new_floor);
             if (threadIdx.x == 0) {
                 fence_async_shared();  // what was read from the buffer, before the next copy into it
                 fetch(s + l.buffers);
