@@ -29,10 +29,10 @@
 //
 // What bounds it now: the lists, which keep the stream waiting for a third of
 // the time (their loads queue behind the first segments), and half of the
-// issue slots.  64 rows of 151936 in f32 with every rule take 28 us (2.8 TB/s),
-// 256 rows in bf16 of which only the picks are wanted 36 us (2.2 TB/s; 39 us when
-// each thread compared with its own greatest), one row with 4096 tokens of
-// history 12 to 14 us.
+// issue slots.  64 rows of 151936 in f32 with every rule take 27 us (2.9 TB/s),
+// 256 rows in bf16 of which only the picks are wanted 35 us (2.2 TB/s; 2 us more
+// when each thread compared with its own greatest), one row with 4096 tokens
+// of history 12 to 14 us.
 #include <climits>
 
 #include "launch.cuh"
@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
         floor_of = order_of(-INFINITY);
         fence_async_shared();
         fetch(0);
-        if (l.buffers == 2) fetch(1);
     }
 
     const uint32_t hist = a.tokens ? (uint32_t)max(0, min(a.lengths ? a.lengths[row] : INT_MAX, (int)a.token_cols)) : 0u;
@@ -265,6 +264,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
             if (threadIdx.x + q * kThreads < hist) held[q] = place(v[q], a.vocab);
     }
     if (threadIdx.x < biases) held_bias = place(list_at(a.bias_ids, a.bias64, bid0 + threadIdx.x), a.vocab);
+    // the second segment's copy starts once the lists' loads are through, which
+    // would queue behind it (28.3 and 26.7 us for 64 rows with every rule)
+    if (threadIdx.x == 0 && l.buffers == 2) {
+        asm volatile("" ::"r"(held[0]));
+        fetch(1);
+    }
+
     Best named{-INFINITY, UINT_MAX}, best{-INFINITY, UINT_MAX};
     // this thread's first vector with the greatest element; which it is is found in the end
     float top = -INFINITY;
