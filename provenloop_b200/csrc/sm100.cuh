@@ -106,11 +106,6 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t cluster_addr) {
     return v;
 }
 
-// `bytes` (a multiple of 16) from a 16-byte boundary of global memory on to L2.
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(__cvta_generic_to_global(p)), "r"(bytes) : "memory");
-}
-
 // Position in a ring of barriers and the parity of its current phase.
 struct Ring {
     int i = 0, n;
