@@ -357,6 +357,73 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
     if (both.after_pack[blockIdx.z] == 1) grid_dependency_wait();
 }
 
+// f32 factors whose contiguous axis is the rank's (the backward call's B):
+// 32 rank indexes of four neighbouring tokens a CTA, a lane each, the
+// contraction over the warps.  Bound: reading the factor, from L2.  284 tokens,
+// rank 64 over 1536: 17 us, about 110 with lanes along the contraction, which
+// takes less below rank 32 (634 tokens, rank 13: 13 us, 43 so).
+__global__ void __launch_bounds__(1024) k_low_cols(const LowArgs a) {
+    constexpr int NT = 4, U = 4;  // U: rows of the factor under way
+    __shared__ float part[32][NT][32];
+    const long long m0 = (long long)blockIdx.x * NT;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.y * 32 + lane, rs = low_stride(a.r);
+    int e[NT];
+    const float *f[NT], *x[NT];
+    bool one = true;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {  // clamped places: what they give is not kept
+        e[i] = m0 + i < a.n ? a.id.of(m0 + i) : -1;
+        one &= e[i] == e[0];
+        x[i] = static_cast<const float*>(a.x) + min(m0 + i, a.n - 1) * a.x_stride;
+        f[i] = static_cast<const float*>(a.f.p) + max(e[i], 0) * a.f.se + min(j, a.r - 1) * a.f.sj;
+    }
+    float v[NT] = {};
+    if (!(one && e[0] < 0)) {
+        const int k0 = (int)((long long)a.k * warp / 32), k1 = (int)((long long)a.k * (warp + 1) / 32);
+        for (int k = k0; k < k1; k += U) {
+            float fk[U];
+            if (one) {
+                float xk[U][NT];
+#pragma unroll
+                for (int q = 0; q < U; q++) {
+                    const int at = min(k + q, k1 - 1);
+                    fk[q] = f[0][at * a.f.sk];
+#pragma unroll
+                    for (int i = 0; i < NT; i++) xk[q][i] = x[i][at];
+                }
+#pragma unroll
+                for (int q = 0; q < U; q++)
+                    if (k + q < k1)
+#pragma unroll
+                        for (int i = 0; i < NT; i++) v[i] = fmaf(xk[q][i], fk[q], v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    float xk[U];
+#pragma unroll
+                    for (int q = 0; q < U; q++) {
+                        const int at = min(k + q, k1 - 1);
+                        fk[q] = f[i][at * a.f.sk], xk[q] = x[i][at];
+                    }
+#pragma unroll
+                    for (int q = 0; q < U; q++)
+                        if (k + q < k1) v[i] = fmaf(xk[q], fk[q], v[i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++) part[warp][i][lane] = v[i];
+    __syncthreads();
+    const int i = threadIdx.x >> 5;  // the first four warps finish a token each
+    if (i >= NT || m0 + i >= a.n || j >= rs) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 32; w++) sum += part[w][i][lane];
+    const int own = a.id.of(m0 + i);
+    a.low[(m0 + i) * rs + j] = own >= 0 && j < a.r ? (a.scale ? a.scale[own] * sum : sum) : 0.f;
+}
+
 // ---------------------------------------------------------------- projection
 
 // f32: BM x BN outputs per CTA, TM x TN per thread in two halves, 16 of the
@@ -591,6 +658,63 @@ __device__ __forceinline__ float dot_low(const float* low, const T* b, int r, fl
         }
     }
     return v;
+}
+
+// f32, few tokens: a warp for each output of four tokens.  Bound: reading W,
+// and the launches' latency: one token of 1536 -> 1536 takes 6 us, 23 as a tile;
+// 31 of them take 37 us, 28 as tiles.
+__global__ void __launch_bounds__(256) k_project_f32_few(const ProjectArgs a, int vec) {
+    constexpr int NT = 4, U = 4;  // U: loads of a row under way
+    const int lane = threadIdx.x & 31, o = blockIdx.x * 8 + (threadIdx.x >> 5), m0 = blockIdx.y * NT;
+    float v[NT] = {};
+    if (a.w && o < a.o) {
+        const float* w = static_cast<const float*>(a.w) + o * a.w_stride;
+        const float* x[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++) x[i] = static_cast<const float*>(a.x) + min((long long)m0 + i, a.n - 1) * a.x_stride;
+        const int whole = vec ? a.k / 4 * 4 : 0;
+        for (int k = lane * 4; k < whole; k += 128 * U) {
+            float4 f[U];
+#pragma unroll
+            for (int q = 0; q < U; q++) f[q] = *reinterpret_cast<const float4*>(w + min(k + 128 * q, whole - 4));
+#pragma unroll
+            for (int q = 0; q < U; q++)
+                if (k + 128 * q < whole)
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const float4 g = *reinterpret_cast<const float4*>(x[i] + k + 128 * q);
+                        v[i] = fmaf(f[q].x, g.x, v[i]), v[i] = fmaf(f[q].y, g.y, v[i]), v[i] = fmaf(f[q].z, g.z, v[i]), v[i] = fmaf(f[q].w, g.w, v[i]);
+                    }
+        }
+        for (int k = whole + lane; k < a.k; k += 32 * 2 * U) {
+            float f[2 * U];
+#pragma unroll
+            for (int q = 0; q < 2 * U; q++) f[q] = w[min(k + 32 * q, a.k - 1)];
+#pragma unroll
+            for (int q = 0; q < 2 * U; q++)
+                if (k + 32 * q < a.k)
+#pragma unroll
+                    for (int i = 0; i < NT; i++) v[i] = fmaf(f[q], x[i][k + 32 * q], v[i]);
+        }
+    }
+    grid_dependency_wait();
+    if (o >= a.o) return;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const int m = m0 + i, e = m < a.n ? a.id.of(m) : -1;
+        if (e >= 0) {
+            const float *low = a.low + m * low_stride(a.r), *g = static_cast<const float*>(a.g.p) + e * a.g.se + o * a.g.sk;
+            for (int j = lane; j < a.r; j += 32) v[i] = fmaf(low[j], g[j], v[i]);
+        }
+#pragma unroll
+        for (int q = 16; q; q >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], q);
+        if (lane == i && m < a.n) {
+            float y = v[i];
+            if (a.bias) y += static_cast<const float*>(a.bias)[o];
+            if (a.base) y += static_cast<const float*>(a.base)[m * a.base_stride + o];
+            static_cast<float*>(a.out)[m * a.out_stride + o] = y;
+        }
+    }
 }
 
 // Few tokens: a cluster of S CTAs streams 16 rows of W once past NB * 8
@@ -955,6 +1079,13 @@ cudaError_t low_launch(const LowArgs* a, int count, bool vec, const int* after_p
     const long long n = a[0].n;
     if (sizeof(T) == 2 && !low_by_token(n, a[0].k, a[count - 1].k, a[0].r, a[0].id.count))
         return launch_low_tc(a, count, std::is_same<T, __half>::value ? DT_F16 : DT_BF16, after_pack, s);
+    if (sizeof(T) == 4 && a[count - 1].f.sk >= 32) {
+        const LowArgs& u = a[count - 1];
+        const cudaError_t e = count == 2 ? low_launch<T>(a, 1, vec, after_pack, s) : cudaSuccess;
+        if (e != cudaSuccess) return e;
+        KScope ks("adapter_low", s);
+        return launch_cl(1, k_low_cols, dim3((unsigned)((n + 3) / 4), (u.r + 31) / 32), 1024, 0, s, u);
+    }
     const LowPair both{{a[0], a[count - 1]}, {after_pack[0], after_pack[count - 1]}};
     const int kmax = a[0].k > a[count - 1].k ? a[0].k : a[count - 1].k;
     KScope ks("adapter_low", s);
@@ -1044,6 +1175,8 @@ cudaError_t launch_project_f32(const ProjectArgs& a, cudaStream_t s) {
     const auto vec = [](const void* p, long long stride, long long rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows < 2 || stride % 4 == 0); };
     const int vx = vec(a.x, a.x_stride, a.n), vw = vec(a.w, a.w_stride, a.w_t ? a.k : a.o);
     KScope ks("adapter_project", s);
+    if (a.n <= kSmallTokens && !a.w_t)
+        return launch_dependent(1, k_project_f32_few, dim3((a.o + 7) / 8, (unsigned)((a.n + 3) / 4)), 256, 0, s, a, vx && vw);
     // a factor's rows: r rows of o elements, or o rows of r
     const int vg = vec(a.g.p, a.g.sk == 1 && a.g.sj != 1 ? a.g.sj : a.g.sk, 2) && (a.id.count == 1 || a.g.se % 4 == 0);
     // The tile and the number of CTAs that share a contraction with the least
