@@ -52,11 +52,14 @@ def torch_ops_command(out: str):
     base = os.path.dirname(torch.__file__)
     inc, libs = os.path.join(base, "include"), os.path.join(base, "lib")
     cuda = os.path.dirname(os.path.dirname(nvcc_path()))
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden",
+    # the C++ library by its shared object: a compiler that finds only the static
+    # one would give the module a second copy beside torch's, and an exception
+    # that passes between them ends the process
+    return [shutil.which("g++") or os.environ.get("CXX", "c++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc,
             "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
             "-I", os.path.join(cuda, "include"), os.path.join(CSRC, "torch_ops.cpp"), "-o", out, "-L", libs, "-ltorch_python", "-ltorch",
-            "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+            "-ltorch_cpu", "-lc10", "-lc10_cuda", "-nostdlib++", "-l:libstdc++.so.6"]
 
 
 def needs_build() -> bool:
