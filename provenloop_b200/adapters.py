@@ -64,5 +64,5 @@ def adapter_project_backward(grad, x, lora_a, lora_b, adapter, weight=None, scal
     bias and scale held fixed: (d x [..., d_in], d lora_a, d lora_b), in the
     inputs' dtype, None where not needed.  An adapter without tokens gets
     zeros.  (The gradient of base is ``grad`` itself.)  The order of every sum
-    depends on the sizes and indexes alone."""
+    depends on the sizes, the indexes and the kind of GPU alone."""
     return (_ops or _load()).backward(grad, x, lora_a, lora_b, adapter, weight, scale, need_x, need_adapters)
