@@ -262,7 +262,7 @@ int adapter_project(const ts_adapter_args* a) {
     const int after_pack = !w.jobs.jobs ? 0 : p.pack_x || p.pack_a ? 2 : 1;
     if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, &after_pack, w.s);
     const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low,
-                        {a->lora_b, rb, 1, r}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+                        {a->lora_b, rb, 1, r}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride, p.pack_x || p.pack_w};
     if (e == cudaSuccess)
         e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
     return cuda_status(e);
@@ -319,7 +319,7 @@ int adapter_project_backward(const ts_adapter_args* a) {
     if (e == cudaSuccess) e = launch_low(l + skip, 2 - skip, a->dtype, p.low_vec, after_pack + skip, w.s);
     if (e == cudaSuccess && a->out) {
         const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u,
-                            {a->lora_a, ra, di, 1}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride};
+                            {a->lora_a, ra, di, 1}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride, p.pack_grad || p.pack_w};
         e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }
     if (e == cudaSuccess && a->grad_a) {

@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
             }
         }
     }
-    // the next launch waits for this one, and with it for the packing
+    // what the next launch reads behind its own wait for this one then comes
+    // behind the packing too
     if (both.after_pack[blockIdx.z] == 1) grid_dependency_wait();
 }
 

@@ -180,6 +180,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
 
     if (warp == 12) {
         if (lane == 0) {
+            if (p.packed) grid_dependency_wait();
             Ring r(L::kStages, 1);
             int serial = 0;
             for (int t = blockIdx.x / CG; t < tiles && shared_part; t += step, serial++) {
@@ -734,6 +735,7 @@ k_project_split(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __
     const uint32_t tmem = tmem_at;
     if (warp == 0) {
         if (lane == 0) {
+            if (p.packed) grid_dependency_wait();
             Ring r(L::kStages, 1);
             for (int kb = kb0; kb < kb1; kb++, r.next()) {
                 if (!mbar_wait(&empty[r.i], r.phase, &dead)) break;

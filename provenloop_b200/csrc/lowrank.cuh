@@ -83,6 +83,11 @@ struct ProjectArgs {
     AdapterIds id;
     void* out;
     long long out_stride;
+    // x or w lies in the workspace, written by launch_pack.  launch_low, which
+    // stands between the two, lets the projection start before the packing is
+    // over (it only waits for it before it ends), so what loads x and w has to
+    // wait for launch_low first; other operands' loads start at once.
+    int packed;
 };
 
 // Gradient of one factor: out[e][j][k] = sum over the tokens m of adapter e
