@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
     __shared__ uint64_t arrived[2];
     __shared__ uint32_t dead, warp_bits[kThreads / 32], floor_of;  // the CTA's greatest before this segment
     cg::cluster_group cluster = cg::this_cluster();
+    cluster_arrive();  // waited for before the first access to another CTA's shared memory
     const int rank = (int)cluster.block_rank(), cl = (int)cluster.num_blocks();
     const long long row = blockIdx.x / cl;
     const T* x = static_cast<const T*>(a.logits) + row * a.logits_stride;
@@ -473,6 +474,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rules(const RulesArgs a, const 
     __shared__ unsigned long long warp_key[kThreads / 32], cta_key[kCluster];
     if ((threadIdx.x & 31) == 0) warp_key[threadIdx.x >> 5] = key;
     __syncthreads();
+    cluster_wait();  // the other CTAs have started
     if (threadIdx.x < 32) {
         key = threadIdx.x < kThreads / 32 ? warp_key[threadIdx.x] : 0ull;
 #pragma unroll

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_gpu_decode_ops import _check_backward, _check_project, _inputs
+from tests.test_gpu_decode_ops import TYPES, _check_backward, _check_project, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -20,6 +20,12 @@ def _device():
 def A():
     from provenloop_b200 import adapters
     return adapters
+
+
+@pytest.fixture(scope="module")
+def R():
+    from provenloop_b200 import logits
+    return logits
 
 
 def _c_args(A, s, back, out, da=None, db=None, ws=None):
@@ -107,6 +113,27 @@ def test_rows_off_16_bytes_queued_one_behind_the_other(A, shapes, dt, back, capt
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(p, q) for p, q in zip(g, w))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("vocab", [1, 127, 130, 700, 1024])
+def test_rules_rows_shorter_than_their_cluster(R, vocab, dt):
+    """One row is split over eight CTAs, most of which get no token of a small
+    vocabulary and bring their (empty) pick at once: the pick is the row's
+    wherever it lies, also on a busy GPU."""
+    rows = torch.full((vocab, vocab), -1.0, dtype=TYPES[dt], device="cuda")
+    rows.fill_diagonal_(1.0)
+    mask = torch.full(((vocab + 31) // 32,), -1, dtype=torch.int32, device="cuda")
+    busy = torch.randn((2048, 2048), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+    at = list(range(vocab)) if vocab < 200 else list(range(0, vocab, 7)) + [vocab - 1]
+    picks = [R.apply_rules(rows[i:i + 1], mask=mask if i % 2 else None, write=False)[1] for i in at]
+    torch.cuda.synchronize()
+    assert torch.cat(picks).tolist() == at
 
 
 def test_no_wait_ran_out():
