@@ -154,7 +154,7 @@ __device__ __forceinline__ bool pack_f32(const PackJob& a, const uint16_t* src, 
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         f[i] = dtype == DT_BF16 ? __uint_as_float((uint32_t)v[i] << 16) : __half2float(__ushort_as_half(v[i]));
-        if ((__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u) f[i] = 0.f, bad = true;
+        if ((__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u) f[i] = copysignf(1.f, f[i]), bad = true;
     }
     if (along) {
         if (jj < a.rows) {
@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
             const float low = e[i] >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e[i]] * v[i] : v[i]) : 0.f;
             if (a.low) a.low[m * rs + j] = low;
             if (a.split) {
-                const __nv_bfloat16 h = __float2bfloat16_rn(low), l = __float2bfloat16_rn(low - __bfloat162float(h));
-                a.split[m * 2 * rs + j] = __bfloat16_as_ushort(h), a.split[(m * 2 + 1) * rs + j] = __bfloat16_as_ushort(l);
+                uint32_t h, l;
+                bf16_terms(low, h, l);
+                a.split[m * 2 * rs + j] = (uint16_t)h, a.split[(m * 2 + 1) * rs + j] = (uint16_t)l;
             }
         }
     }
@@ -829,7 +830,8 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
 // 11 bits exactly, operands transposed on the way from shared memory.  Else
 // 16 x 8 x 8 TF32 products: fp16 x is exact in TF32, and low has been rounded
 // to it; for f32 inputs both are split into two TF32 parts, which leaves
-// 2^-22.  An adapter that lies in one window is written here; the others' sums
+// 2^-22 (their products of infinities left apart cost 3 to 5 % of an f32 call:
+// 1024 tokens of 1536 -> 1536, rank 16: 261 us, 255 with NaNs for them).  An adapter that lies in one window is written here; the others' sums
 // over a window go to the workspace, and k_grad_sum adds them in the
 // windows' order.  Bound: reading x once per 64 rank indexes.  8192 tokens of
 // 1536 and 1536, rank 16, three adapters: 18 us, 2.8 TB/s; 2048 of 8960 and
@@ -947,30 +949,45 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
                         }
                     }
                     uint32_t am[2][4], al[2][4];
+                    bool special = false;
 #pragma unroll
                     for (int q2 = 0; q2 < 2; q2++)
 #pragma unroll
                         for (int z = 0; z < 4; z++) {
                             const float v = f[z >> 1][q2 * 2 + (z & 1)];
-                            if constexpr (sizeof(T) == 4) {
-                                am[q2][z] = to_tf32(v);
-                                al[q2][z] = to_tf32(v - __uint_as_float(am[q2][z]));
-                            } else {
-                                am[q2][z] = __float_as_uint(v);
-                            }
+                            if constexpr (sizeof(T) == 4) special |= tf32_terms(v, am[q2][z], al[q2][z]);
+                            else am[q2][z] = __float_as_uint(v);
                         }
+                    // an infinity of x times the lower term of low would be a NaN
+                    // where that is zero or of the other sign
+                    if constexpr (sizeof(T) == 4) special = __any_sync(0xffffffffu, special);
 #pragma unroll
                     for (int nb = 0; nb < RB; nb++) {
                         const float b0 = su[tok * UR + nb * 8 + g], b1 = su[(tok + 4) * UR + nb * 8 + g];
-                        const uint32_t m0b = sizeof(T) == 4 ? to_tf32(b0) : __float_as_uint(b0), m1b = sizeof(T) == 4 ? to_tf32(b1) : __float_as_uint(b1);
+                        uint32_t m0b = __float_as_uint(b0), m1b = __float_as_uint(b1), l0, l1;
+                        if constexpr (sizeof(T) == 4) {
+                            const bool s0 = tf32_terms(b0, m0b, l0), s1 = tf32_terms(b1, m1b, l1);
 #pragma unroll
-                        for (int q2 = 0; q2 < 2; q2++) {
-                            if constexpr (sizeof(T) == 4) {
-                                const uint32_t l0 = to_tf32(b0 - __uint_as_float(m0b)), l1 = to_tf32(b1 - __uint_as_float(m1b));
-                                mma8_tf32(acc[q2][nb], al[q2], m0b, m1b);
-                                mma8_tf32(acc[q2][nb], am[q2], l0, l1);
+                            for (int q2 = 0; q2 < 2; q2++) {
+                                mma8_tf32(acc[q2][nb], al[q2], s0 ? 0u : m0b, s1 ? 0u : m1b);
+                                if (!special) mma8_tf32(acc[q2][nb], am[q2], l0, l1);
                             }
-                            mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
+                        }
+#pragma unroll
+                        for (int q2 = 0; q2 < 2; q2++) mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
+                    }
+                    if (sizeof(T) == 4 && special) {
+#pragma unroll
+                        for (int q2 = 0; q2 < 2; q2++)
+#pragma unroll
+                            for (int z = 0; z < 4; z++)
+                                if ((am[q2][z] & 0x7f800000u) == 0x7f800000u) am[q2][z] = 0u;
+#pragma unroll
+                        for (int nb = 0; nb < RB; nb++) {
+                            uint32_t m0b, m1b, l0, l1;
+                            tf32_terms(su[tok * UR + nb * 8 + g], m0b, l0), tf32_terms(su[(tok + 4) * UR + nb * 8 + g], m1b, l1);
+#pragma unroll
+                            for (int q2 = 0; q2 < 2; q2++) mma8_tf32(acc[q2][nb], am[q2], l0, l1);
                         }
                     }
                 }

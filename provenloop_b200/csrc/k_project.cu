@@ -27,8 +27,9 @@
 // 65504 does not overflow.  The factors are converted once per call (k_pack).
 //
 // A zero times an adapter's NaN or infinity would spread to the other
-// tokens of the tile: k_pack replaces such elements by 0 and flags them, and
-// the epilogue adds their terms to the adapter's own tokens only.
+// tokens of the tile: k_pack replaces such elements by 1 of their sign (of which an infinite
+// low gives the right infinity) and flags them, and the epilogue adds their
+// terms to the adapter's own tokens only.
 #include <climits>
 #include <cuda.h>
 
@@ -888,11 +889,11 @@ struct LowMaps {
 __device__ __forceinline__ void put(const LowArgs& a, long long m, int rs, int j, float4 v) {
     if (a.low) *reinterpret_cast<float4*>(a.low + m * rs + j) = v;
     if (a.split) {
-        const uint32_t h0 = pack2<__nv_bfloat16>(v.x, v.y), h1 = pack2<__nv_bfloat16>(v.z, v.w);
-        const float2 f0 = unpack2<__nv_bfloat16>(h0), f1 = unpack2<__nv_bfloat16>(h1);
+        uint32_t h[4], l[4];
+        bf16_terms(v.x, h[0], l[0]), bf16_terms(v.y, h[1], l[1]), bf16_terms(v.z, h[2], l[2]), bf16_terms(v.w, h[3], l[3]);
         uint16_t* to = a.split + m * 2 * rs + j;
-        *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
-        *reinterpret_cast<uint2*>(to + rs) = make_uint2(pack2<__nv_bfloat16>(v.x - f0.x, v.y - f0.y), pack2<__nv_bfloat16>(v.z - f1.x, v.w - f1.y));
+        *reinterpret_cast<uint2*>(to) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+        *reinterpret_cast<uint2*>(to + rs) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
     }
 }
 

@@ -78,7 +78,7 @@ struct ProjectArgs {
     long long base_stride;
     const float* low;
     Factor g;  // sk here is the stride of o
-    const float* g32;     // g as f32 [e][o][low_stride(r)], elements that are not finite replaced by 0 (k_project.cu only)
+    const float* g32;     // g as f32 [e][o][low_stride(r)], elements that are not finite replaced by 1 of their sign (k_project.cu only)
     const uint32_t* bad;  // [e][ceil(o / 128)][low_stride(r) / 16]: some of them are
     AdapterIds id;
     void* out;

@@ -7,6 +7,7 @@
 #pragma once
 #include <cstdint>
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 namespace tsg {
@@ -269,6 +270,30 @@ __device__ __forceinline__ uint32_t to_tf32(float v) {
     uint32_t r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
     return r;
+}
+// v as two bf16 terms of one sign, neither of them zero: the upper one is one
+// step below v's first 8 bits, the lower one the rest, rounded, so that their
+// sum is within 2^-15 v.  An infinity times such a v has the sign of their
+// product and not the NaN of an infinity times zero or of two signs; values
+// that round to infinity in 8 bits stay finite.  Infinities and NaNs are both
+// terms.  (v below bf16's second least value, 2^-132, counts as zero there.)
+__device__ __forceinline__ void bf16_terms(float v, uint32_t& high, uint32_t& low) {
+    const uint32_t u = __float_as_uint(v), m = u >> 16 & 0x7fffu;
+    const bool special = m >= 0x7f80u;
+    high = special ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) : (u >> 16 & 0x8000u) | (m > 0u ? m - 1u : 0u);
+    low = special ? high : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v - __uint_as_float(high << 16)));
+}
+
+// v = high + low for TF32 instructions, low zero where v is not finite (the
+// upper term then is v): products with the lower terms have to leave out what
+// is not finite.  Returns whether v is not.  Values that would round to
+// infinity are cut instead.
+__device__ __forceinline__ bool tf32_terms(float v, uint32_t& high, uint32_t& low) {
+    const uint32_t u = __float_as_uint(v), m = u & 0x7fffffffu;
+    const bool special = m >= 0x7f800000u;
+    high = special ? (m > 0x7f800000u ? 0x7fffffffu : u) : (m >= 0x7f7ff000u ? u : u + 0x1000u) & 0xffffe000u;
+    low = special ? 0u : to_tf32(v - __uint_as_float(high));
+    return special;
 }
 __device__ __forceinline__ void st_shared4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");

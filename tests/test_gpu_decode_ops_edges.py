@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_gpu_decode_ops import TYPES, _check_backward, _check_project, _inputs
+from tests.test_gpu_decode_ops import TYPES, _check_backward, _check_project, _high64, _inputs, _low64
 
 pytestmark = pytest.mark.gpu
 
@@ -134,6 +134,76 @@ def test_rules_rows_shorter_than_their_cluster(R, vocab, dt):
     picks = [R.apply_rules(rows[i:i + 1], mask=mask if i % 2 else None, write=False)[1] for i in at]
     torch.cuda.synchronize()
     assert torch.cat(picks).tolist() == at
+
+
+def _special64(s, weight):
+    """y, dx, da and db in 64 bits, with the terms' absolute sums, of 16 or 32
+    bit inputs that hold infinities."""
+    x, dy, a, b, ids = s["x"].double(), s["dy"].double(), s["a"].double(), s["b"].double(), s["ids"]
+    low, lmag = _low64(x, a, s["scale"], ids)
+    u, umag = _low64(dy, b.transpose(1, 2), s["scale"], ids)
+    y, ymag = _high64(low, lmag, b.transpose(1, 2), ids)
+    dx, dxmag = _high64(u, umag, a, ids)
+    if weight:
+        w = s["w"].double()
+        y, ymag, dx, dxmag = y + x @ w.T, ymag + x.abs() @ w.T.abs(), dx + dy @ w, dxmag + dy.abs() @ w.abs()
+    own = [(ids == e).nonzero()[:, 0] for e in range(a.shape[0])]
+    da, damag = (torch.stack([p[r].T @ q[r] for r in own]) for p, q in ((u, x), (umag, x.abs())))
+    db, dbmag = (torch.stack([p[r].T @ q[r] for r in own]) for p, q in ((dy, low), (dy.abs(), lmag)))
+    return (y, dx, da, db), (ymag, dxmag, damag, dbmag)
+
+
+def _same_where_special(got, want, mag, terms):
+    """Infinities and NaNs where the 64-bit values have them, and the other
+    values near those: half a step of the type, the intermediate's 11 bits at
+    least, and sums of `terms` in 32 bits."""
+    t, got = got.dtype, got.double()
+    special = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[special].nan_to_num(0.0), want[special].nan_to_num(0.0))
+    tol = torch.finfo(t).eps / 2 * want.abs() + ((0 if t is torch.float32 else 2.0 ** -11) + (terms + 8) * 2.0 ** -23) * 1.01 * mag + 2.0 ** -25
+    assert ((got - want).abs() <= tol)[~special].all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("weight", [True, False])
+@pytest.mark.parametrize("n,i,o,r", [(9, 264, 200, 16), (70, 136, 328, 30), (300, 264, 136, 64), (700, 4104, 264, 16), (2400, 264, 7176, 1)])
+def test_infinities_stay_infinities(A, n, i, o, r, weight, dt):
+    """An infinity in an input makes those results infinite (or, where
+    infinities of both signs or a zero meet it, not a number) that it makes so in
+    64 bits, of the adapters' gradients too."""
+    s = _inputs(n, i, o, r, 3, dt, "mixed", seed=60)
+    s["ids"] = torch.where(torch.arange(n, device="cuda") == n // 2, 1, torch.arange(n, device="cuda") % 2 * 2).int()
+    m, inf = n // 2, float("inf")
+    puts = (("x", (m, 5), inf), ("dy", (m, 7), -inf), ("a", (1, r - 1, 3), inf), ("b", (1, 130, 0), -inf), ("scale", (1,), inf))
+    for names in (("x",), ("dy",), ("a",), ("b",), ("scale",), ("x", "b"), ("a", "dy")):
+        q = dict(s)
+        for name, at, value in puts:
+            if name in names:
+                q[name] = s[name].clone()
+                q[name][at] = value
+        y = A.adapter_project(q["x"], q["a"], q["b"], q["ids"], weight=q["w"] if weight else None, scale=q["scale"])
+        got = (y, *A.adapter_project_backward(q["dy"], q["x"], q["a"], q["b"], q["ids"], weight=q["w"] if weight else None, scale=q["scale"]))
+        want, mags = _special64(q, weight)
+        for g, w, mag, terms in zip(got, want, mags, (i + r, o + r, o + n, i + n)):
+            _same_where_special(g, w, mag, terms)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [1, 33, 200])
+def test_largest_values_stay_finite(A, n, dt):
+    """Gradients of the largest inputs and intermediates, which round to
+    infinity in fewer bits than they have, are finite where they are in 64 bits."""
+    s = _inputs(n, 72, 40, 16, 1, dt, "one", seed=61)
+    s["x"].zero_(), s["a"].zero_(), s["dy"].mul_(2.0 ** -8)
+    s["x"][:, 3] = torch.finfo(TYPES[dt]).max if n == 1 else 2.0 ** 120
+    s["a"][:, :, 3] = 1.0
+    s["scale"].fill_(1.003 if dt == "bf16" else 1.0)  # bf16: the intermediate is behind the type's largest value
+    got = A.adapter_project_backward(s["dy"], s["x"], s["a"], s["b"], s["ids"], scale=s["scale"])
+    want, mags = _special64(s, False)
+    for g, w, mag, terms in zip(got, want[1:], mags[1:], (56, 40 + n, 72 + n)):
+        assert torch.isfinite(g).all()
+        _same_where_special(g, w, mag, terms)
 
 
 def test_no_wait_ran_out():
