@@ -314,13 +314,20 @@ typedef struct ts_adapter_args {
  * sizes, strides and pointers (workspace itself need not be set). */
 int ts_adapter_workspace(const ts_adapter_args* args, int backward, uint64_t* bytes);
 /* out[m] = base[m] + x[m] weight^T + bias + scale_e (x[m] lora_a_e^T) lora_b_e^T,
- * e = the token's adapter.  Sums are held in 32 bits; out is rounded once. */
+ * e = the token's adapter.  Sums are held in 32 bits; out is rounded once.
+ * The intermediate scale_e x[m] lora_a_e^T keeps its 32 bits too, but for
+ * 16-bit types in calls where the tokens of a tile share factors (n d_out r
+ * above 2^24, mostly): there it is rounded to 11 significant bits, with the
+ * range of f32, as an operand of tensor-core products. */
 int ts_adapter_project(const ts_adapter_args* args);
 /* Gradients of the above for a gradient `grad` of out, weight, bias and scale
  * held fixed: out[m] = grad[m] weight + u[m] lora_a_e with u[m] = scale_e
  * grad[m] lora_b_e; grad_a_e = sum of u[m]^T x[m] and grad_b_e = scale_e sum
  * of grad[m]^T (x[m] lora_a_e^T) over the adapter's tokens (zero without
- * any), in an order fixed by the sizes and indexes alone.  The gradient of base is grad. */
+ * any), in an order fixed by the sizes and indexes alone.  The gradient of base is grad.
+ * out treats u as the forward call treats its intermediate (n d_in r).  The
+ * factors' gradients hold both intermediates to a relative 2^-22 (f32), 2^-20
+ * (f16) or 2^-15 (bf16). */
 int ts_adapter_project_backward(const ts_adapter_args* args);
 
 /* Waits within a kernel of ts_adapter_* or ts_logit_rules that ran out (two seconds) on

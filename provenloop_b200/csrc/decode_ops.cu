@@ -258,10 +258,10 @@ int adapter_project(const ts_adapter_args* a) {
     if (p.g32)
         w.jobs.add({PackJob::TO_F32, a->lora_b, rb, r, 1, d_o, (int)a->adapters, r, low_stride(r), w.at(p.g), static_cast<uint32_t*>(w.at(p.bad))});
     cudaError_t e = w.pack();
-    const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low, nullptr};
+    const LowArgs l{x.p, x.stride, n, (int)a->d_in, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, low, nullptr, p.g32};
     const int after_pack = !w.jobs.jobs ? 0 : p.pack_x || p.pack_a ? 2 : 1;
     if (e == cudaSuccess) e = launch_low(&l, 1, a->dtype, p.low_vec, &after_pack, w.s);
-    const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low,
+    const ProjectArgs q{x.p, x.stride, n, (int)a->d_in, d_o, r, wt.p, wt.stride, 0, a->bias, a->base, a->base_stride, low, p.g32,
                         {a->lora_b, rb, 1, r}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride, p.pack_x || p.pack_w};
     if (e == cudaSuccess)
         e = p.f32 ? launch_project_f32(q, w.s) : p.small ? launch_project_small(q, a->dtype, w.s) : launch_project_tc(q, a->dtype, w.s);
@@ -312,13 +312,14 @@ int adapter_project_backward(const ts_adapter_args* a) {
     const bool split = a->dtype == TS_DTYPE_BF16 && a->grad_a;
     uint16_t* const lsplit = split ? reinterpret_cast<uint16_t*>(low) : nullptr;
     uint16_t* const usplit = split ? static_cast<uint16_t*>(w.at(p.usplit)) : nullptr;
-    const LowArgs l[2] = {{x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, split ? nullptr : low, lsplit},
-                          {grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, a->out || !split ? u : nullptr, usplit}};
+    const int u_tf32 = p.g32 && (split || !a->grad_a);  // else the gradients read u too
+    const LowArgs l[2] = {{x.p, x.stride, n, di, r, {fa.p, r * fa.stride, fa.stride, 1}, ids_of(a), a->scale, split ? nullptr : low, lsplit, 0},
+                          {grad.p, grad.stride, n, d_o, r, fb, ids_of(a), a->scale, a->out || !split ? u : nullptr, usplit, u_tf32}};
     const int after_pack[2] = {!w.jobs.jobs ? 0 : p.pack_x || p.pack_a ? 2 : 1, !w.jobs.jobs ? 0 : p.pack_b || p.pack_grad ? 2 : 1};
     const int skip = a->grad_a ? 0 : 1;
     if (e == cudaSuccess) e = launch_low(l + skip, 2 - skip, a->dtype, p.low_vec, after_pack + skip, w.s);
     if (e == cudaSuccess && a->out) {
-        const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u,
+        const ProjectArgs q{grad.p, grad.stride, n, d_o, di, r, wt.p, wt.stride, 1, nullptr, nullptr, 0, u, u_tf32,
                             {a->lora_a, ra, di, 1}, p.g32 ? static_cast<float*>(w.at(p.g)) : nullptr, static_cast<uint32_t*>(w.at(p.bad)), ids_of(a), a->out, a->out_stride, p.pack_grad || p.pack_w};
         e = p.f32 ? launch_project_f32(q, w.s) : launch_project_tc(q, a->dtype, w.s);
     }

@@ -262,12 +262,6 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs j
 
 // ---------------------------------------------------------------- low
 
-// What is stored of a sum: see LowArgs.
-template <class T>
-__device__ __forceinline__ float low_value(float v) {
-    return sizeof(T) == 4 ? v : __uint_as_float(to_tf32(v));
-}
-
 // Token by token: WPJ warps share one rank index of NT neighbouring tokens,
 // whose factor row is read once where they have one adapter.  Bound: reading
 // each token's own factor (r k elements), from L2 where tokens share it.  48
@@ -345,8 +339,8 @@ __global__ void __launch_bounds__(256) k_low_token(const LowPair both) {
         for (int i = 0; i < NT; i++) {
             const long long m = m0 + i;
             if (m >= a.n) break;
-            const float low = e[i] >= 0 && j < a.r ? low_value<T>(a.scale ? a.scale[e[i]] * v[i] : v[i]) : 0.f;
-            if (a.low) a.low[m * rs + j] = low;
+            const float low = e[i] >= 0 && j < a.r ? (a.scale ? a.scale[e[i]] * v[i] : v[i]) : 0.f;
+            if (a.low) a.low[m * rs + j] = a.tf32 ? __uint_as_float(to_tf32(low)) : low;
             if (a.split) {
                 uint32_t h, l;
                 bf16_terms(low, h, l);
@@ -826,11 +820,11 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
 // the tokens are spread over the adapters.  For each adapter in the window, in
 // groups of 32 tokens, the rows are gathered and low^T x summed with matrix
 // instructions whose 16-row axis are the features and whose contraction the
-// tokens.  bf16: 16 x 8 x 16 products with low's two bf16 terms, which are its
-// 11 bits exactly, operands transposed on the way from shared memory.  Else
-// 16 x 8 x 8 TF32 products: fp16 x is exact in TF32, and low has been rounded
-// to it; for f32 inputs both are split into two TF32 parts, which leaves
-// 2^-22 (their products of infinities left apart cost 3 to 5 % of an f32 call:
+// tokens.  bf16: 16 x 8 x 16 products with low's two bf16 terms, which hold it
+// to 2^-15, operands transposed on the way from shared memory.  Else
+// 16 x 8 x 8 TF32 products: low is split into two TF32 parts, which leaves 2^-20 beside fp16 x, exact
+// in TF32 (65 us beside a base for 4096 tokens of 1536 and 1536, rank 64; 57 with
+// low in 11 bits alone), and 2^-22 beside f32 x, which is split as well (their products of infinities left apart cost 3 to 5 % of an f32 call:
 // 1024 tokens of 1536 -> 1536, rank 16: 261 us, 255 with NaNs for them).  An adapter that lies in one window is written here; the others' sums
 // over a window go to the workspace, and k_grad_sum adds them in the
 // windows' order.  Bound: reading x once per 64 rank indexes.  8192 tokens of
@@ -936,6 +930,7 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
                     const int tok = (wt * 2 + h) * 8 + t;
                     // four features of two tokens per thread: rows g and g + 8 of two products
                     float f[2][4];
+                    uint32_t odd = 0;  // fp16: signs of exponents that are full
 #pragma unroll
                     for (int z = 0; z < 2; z++) {
                         const uint8_t* p = sx + (tok + 4 * z) * L::kRow + (wf * 32 + 4 * g) * sizeof(T);
@@ -945,11 +940,12 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
                         } else {
                             const uint2 v = *reinterpret_cast<const uint2*>(p);
                             const float2 lo = pair_f<T>(v.x), hi = pair_f<T>(v.y);
+                            odd |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u);
                             f[z][0] = lo.x, f[z][1] = lo.y, f[z][2] = hi.x, f[z][3] = hi.y;
                         }
                     }
                     uint32_t am[2][4], al[2][4];
-                    bool special = false;
+                    bool special = odd & 0x80008000u;
 #pragma unroll
                     for (int q2 = 0; q2 < 2; q2++)
 #pragma unroll
@@ -960,23 +956,22 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
                         }
                     // an infinity of x times the lower term of low would be a NaN
                     // where that is zero or of the other sign
-                    if constexpr (sizeof(T) == 4) special = __any_sync(0xffffffffu, special);
+                    special = __any_sync(0xffffffffu, special);
 #pragma unroll
                     for (int nb = 0; nb < RB; nb++) {
                         const float b0 = su[tok * UR + nb * 8 + g], b1 = su[(tok + 4) * UR + nb * 8 + g];
-                        uint32_t m0b = __float_as_uint(b0), m1b = __float_as_uint(b1), l0, l1;
-                        if constexpr (sizeof(T) == 4) {
-                            const bool s0 = tf32_terms(b0, m0b, l0), s1 = tf32_terms(b1, m1b, l1);
+                        uint32_t m0b, m1b, l0, l1;
+                        bool s0 = false, s1 = false;
+                        if constexpr (sizeof(T) == 4) s0 = tf32_terms(b0, m0b, l0), s1 = tf32_terms(b1, m1b, l1);
+                        else m0b = __float_as_uint(b0), m1b = __float_as_uint(b1), l0 = tf32_rest(b0), l1 = tf32_rest(b1);
 #pragma unroll
-                            for (int q2 = 0; q2 < 2; q2++) {
-                                mma8_tf32(acc[q2][nb], al[q2], s0 ? 0u : m0b, s1 ? 0u : m1b);
-                                if (!special) mma8_tf32(acc[q2][nb], am[q2], l0, l1);
-                            }
+                        for (int q2 = 0; q2 < 2; q2++) {
+                            if constexpr (sizeof(T) == 4) mma8_tf32(acc[q2][nb], al[q2], s0 ? 0u : m0b, s1 ? 0u : m1b);
+                            if (!special) mma8_tf32(acc[q2][nb], am[q2], l0, l1);
+                            mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
                         }
-#pragma unroll
-                        for (int q2 = 0; q2 < 2; q2++) mma8_tf32(acc[q2][nb], am[q2], m0b, m1b);
                     }
-                    if (sizeof(T) == 4 && special) {
+                    if (special) {
 #pragma unroll
                         for (int q2 = 0; q2 < 2; q2++)
 #pragma unroll
@@ -984,8 +979,10 @@ __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const G
                                 if ((am[q2][z] & 0x7f800000u) == 0x7f800000u) am[q2][z] = 0u;
 #pragma unroll
                         for (int nb = 0; nb < RB; nb++) {
+                            const float b0 = su[tok * UR + nb * 8 + g], b1 = su[(tok + 4) * UR + nb * 8 + g];
                             uint32_t m0b, m1b, l0, l1;
-                            tf32_terms(su[tok * UR + nb * 8 + g], m0b, l0), tf32_terms(su[(tok + 4) * UR + nb * 8 + g], m1b, l1);
+                            if constexpr (sizeof(T) == 4) tf32_terms(b0, m0b, l0), tf32_terms(b1, m1b, l1);
+                            else l0 = tf32_rest(b0), l1 = tf32_rest(b1);
 #pragma unroll
                             for (int q2 = 0; q2 < 2; q2++) mma8_tf32(acc[q2][nb], am[q2], l0, l1);
                         }

@@ -24,7 +24,9 @@
 // (prefill, training) pays r / 16 units and a mixed one D r / 16 for D distinct
 // adapters, without sorting tokens or a second pass over out.  TF32 holds bf16 and fp16 factors exactly and low to
 // 11 significant bits with the range of f32, so that an fp16 low above
-// 65504 does not overflow.  The factors are converted once per call (k_pack).
+// 65504 does not overflow; a second term for its other bits would double the
+// units.  (Elsewhere in this file low is a factor of FMAs and keeps its 24
+// bits.)  The factors are converted once per call (k_pack).
 //
 // A zero times an adapter's NaN or infinity would spread to the other
 // tokens of the tile: k_pack replaces such elements by 1 of their sign (of which an infinite
@@ -283,7 +285,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
             const int own = CG == 2 && rank ? pos[CG - 1] : pos[0];
             // the next tile's
             load_ids(t + step, e);
-            const float4* low = reinterpret_cast<const float4*>(p.low + (m < p.n ? m : 0) * rs);
+            const uint4* low = reinterpret_cast<const uint4*>(p.low + (m < p.n ? m : 0) * rs);
             // the factor's flags for the tile's outputs; the first of them are looked at with low
             const int tile_o = t / a.tiles_m * BN, per = rs / kXK, flags = min((BN + 127) / 128, blocks - tile_o / 128) * per;
             const auto flag = [&](int d) { return p.bad[((long long)sh.adapters.list[d / flags] * blocks + tile_o / 128) * per + d % flags]; };
@@ -302,10 +304,16 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                 if (i == 0) mbar_arrive(&sh.turn[1]);
             }
             int u = 0;
-            float4 f[4];
+            uint4 f[4];
             for (int j = 0; j < rs; j += kXK) {
 #pragma unroll
                 for (int q = 0; q < 4; q++) f[q] = low[j / 4 + q];
+                if (!p.low_tf32) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        f[q] = make_uint4(to_tf32(__uint_as_float(f[q].x)), to_tf32(__uint_as_float(f[q].y)), to_tf32(__uint_as_float(f[q].z)),
+                                          to_tf32(__uint_as_float(f[q].w)));
+                }
                 if (bad) sh.bad[serial & 15] = 1;
                 for (int d = 0; d < count; d++, u++) {
                     const uint32_t s = ring + r.i * L::kStage + (u & 1) * L::kUnit;
@@ -317,8 +325,7 @@ k_project_tc(const TcArgs a, const __grid_constant__ CUtensorMap mx, const __gri
                     const bool in = d == own;
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        st_shared4(s + i * 64 + ((q ^ (i >> 1 & 3)) << 4), in ? __float_as_uint(f[q].x) : 0u, in ? __float_as_uint(f[q].y) : 0u,
-                                   in ? __float_as_uint(f[q].z) : 0u, in ? __float_as_uint(f[q].w) : 0u);
+                        st_shared4(s + i * 64 + ((q ^ (i >> 1 & 3)) << 4), in ? f[q].x : 0u, in ? f[q].y : 0u, in ? f[q].z : 0u, in ? f[q].w : 0u);
                     if ((u & 1) || u + 1 == units) {
                         fence_async_shared();
                         if (bar_or(1, 128, late)) goto build_done;  // all 128 threads or none
@@ -887,7 +894,13 @@ struct LowMaps {
 
 // Four values of token m's low.
 __device__ __forceinline__ void put(const LowArgs& a, long long m, int rs, int j, float4 v) {
-    if (a.low) *reinterpret_cast<float4*>(a.low + m * rs + j) = v;
+    if (a.low) {
+        float4* to = reinterpret_cast<float4*>(a.low + m * rs + j);
+        if (a.tf32)
+            *reinterpret_cast<uint4*>(to) = make_uint4(to_tf32(v.x), to_tf32(v.y), to_tf32(v.z), to_tf32(v.w));
+        else
+            *to = v;
+    }
     if (a.split) {
         uint32_t h[4], l[4];
         bf16_terms(v.x, h[0], l[0]), bf16_terms(v.y, h[1], l[1]), bf16_terms(v.z, h[2], l[2]), bf16_terms(v.w, h[3], l[3]);
@@ -1000,7 +1013,7 @@ __global__ void __launch_bounds__(256) k_low_tc(const LowPair both, const __grid
                 v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
             }
             const float scale = a.scale ? a.scale[at] : 1.f;
-            const auto value = [&](float f, int jj) { return jj < a.r ? __uint_as_float(to_tf32(scale * f)) : 0.f; };
+            const auto value = [&](float f, int jj) { return jj < a.r ? scale * f : 0.f; };
             put(a, m0 + r, rs, j, make_float4(value(v.x, j), value(v.y, j + 1), value(v.z, j + 2), value(v.w, j + 3)));
         }
         // the sums have been read before the ring's memory is filled again

@@ -42,9 +42,10 @@ __host__ __device__
 inline int low_stride(int r) { return (r + 15) & ~15; }
 
 // low[m][j] = scale_e * sum_k x[m][k] F[e][j][k] (f32 [n][low_stride(r)];
-// zero rows where a token has no adapter).  For 16-bit inputs the values are
-// rounded to TF32 (11 significant bits, the range of f32): what multiplies
-// them are matrix instructions on TF32, and their factors have fewer bits.
+// zero rows where a token has no adapter).  What multiplies them by FMA takes
+// them as they are; matrix instructions take them rounded to TF32 (k_project_tc:
+// 11 significant bits, the range of f32; nothing else may read them then), as two such terms (gradients of f32
+// and fp16 inputs) or as two bf16 terms (of bf16 inputs).
 struct LowArgs {
     const void* x;
     long long x_stride;
@@ -54,7 +55,8 @@ struct LowArgs {
     AdapterIds id;
     const float* scale;
     float* low;      // or null
-    uint16_t* split; // or null; bf16 inputs: the same values as two bf16 terms, [n][2][low_stride(r)]
+    uint16_t* split; // or null; bf16 inputs: the same values as bf16_terms, [n][2][low_stride(r)]
+    int tf32;        // low is rounded to TF32 when it is written (here that hides; in k_project_tc it costs 1 % of a prefill)
 };
 
 struct LowPair {
@@ -77,6 +79,7 @@ struct ProjectArgs {
     const void* base;
     long long base_stride;
     const float* low;
+    int low_tf32;  // as LowArgs' tf32
     Factor g;  // sk here is the stride of o
     const float* g32;     // g as f32 [e][o][low_stride(r)], elements that are not finite replaced by 1 of their sign (k_project.cu only)
     const uint32_t* bad;  // [e][ceil(o / 128)][low_stride(r) / 16]: some of them are

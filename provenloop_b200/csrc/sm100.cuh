@@ -284,6 +284,13 @@ __device__ __forceinline__ void bf16_terms(float v, uint32_t& high, uint32_t& lo
     low = special ? high : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v - __uint_as_float(high << 16)));
 }
 
+// What a TF32 instruction leaves out of v, which it cuts to 11 significant
+// bits; zero where v is not finite.
+__device__ __forceinline__ uint32_t tf32_rest(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x7f800000u) == 0x7f800000u ? 0u : __float_as_uint(v - __uint_as_float(u & 0xffffe000u));
+}
+
 // v = high + low for TF32 instructions, low zero where v is not finite (the
 // upper term then is v): products with the lower terms have to leave out what
 // is not finite.  Returns whether v is not.  Values that would round to

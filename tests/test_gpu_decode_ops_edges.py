@@ -206,6 +206,46 @@ def test_largest_values_stay_finite(A, n, dt):
         _same_where_special(g, w, mag, terms)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,i,o,r,weight", [(1, 16, 200, 1, True), (16, 8, 200, 3, False), (40, 16, 333, 2, True),
+                                            (300, 24, 1001, 1, False), (300, 16, 264, 3, True), (200, 9, 520, 2, True)])
+def test_intermediate_keeps_its_bits(A, n, i, o, r, weight, dt):
+    """Where the other terms cancel the adapter's but for a rounding, the
+    result shows the intermediate's last bits: sums of k terms in 32 bits are
+    off by less than (k + 8) 2^-23 of the terms' absolute sum, and nothing else is
+    rounded before the result."""
+    s = _inputs(n, i, o, r, 3, dt, "ragged", seed=70)
+    low, lmag = _low64(s["x"], s["a"], s["scale"], s["ids"])
+    y, mag = _high64(low, lmag, s["b"].transpose(1, 2), s["ids"])
+    if weight:
+        y, mag = y + s["x"].double() @ s["w"].double().T, mag + s["x"].double().abs() @ s["w"].double().abs().T
+    base = (-y).to(s["x"].dtype)
+    got = A.adapter_project(s["x"], s["a"], s["b"], s["ids"], weight=s["w"] if weight else None, base=base, scale=s["scale"])
+    want, mag = y + base.double(), mag + base.double().abs()
+    tol = torch.finfo(got.dtype).eps / 2 * want.abs() + (2 * i + r + 8) * 2.0 ** -23 * mag + 2.0 ** -25
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt,bits", [("bf16", 15), ("fp16", 20), ("fp32", 22)])
+@pytest.mark.parametrize("n,i,o,r", [(2, 72, 40, 3), (40, 264, 200, 16), (500, 264, 136, 64), (3000, 4104, 40, 16)])
+def test_gradients_keep_the_intermediates_bits(A, n, i, o, r, dt, bits):
+    """Pairs of tokens whose terms cancel but for a small difference of their
+    intermediates, which hold to a relative 2^-bits; sums of n terms in 32 bits."""
+    s = _inputs(n, i, o, r, 1, dt, "one", seed=71)
+    s["x"][1::2] = s["x"][::2]
+    s["x"][1::2, :3] += 2.0 ** -6
+    s["dy"][1::2] = -s["dy"][::2]
+    s["dy"][1::2, :3] += 2.0 ** -6
+    _, da, db = A.adapter_project_backward(s["dy"], s["x"], s["a"], s["b"], s["ids"], scale=s["scale"])
+    (_, _, wa, wb), (_, _, ma, mb) = _special64(s, False)
+    low = _low64(s["x"], s["a"], s["scale"], s["ids"])[0].abs()
+    u = _low64(s["dy"], s["b"].transpose(1, 2), s["scale"], s["ids"])[0].abs()
+    held = (u.T @ s["x"].double().abs(), s["dy"].double().abs().T @ low)  # of the products with the intermediates
+    for g, w, mag, h, k in zip((da, db), (wa, wb), (ma, mb), held, (o, i)):
+        tol = torch.finfo(g.dtype).eps / 2 * w.abs() + 2.0 ** -bits * h + (k + 8) * 2.0 ** -23 * mag + (n + 8) * 2.0 ** -23 * h + 2.0 ** -25
+        assert ((g.double() - w).abs() <= tol * 1.01).all()
+
+
 def test_no_wait_ran_out():
     """Collected last: none of the calls above gave up a wait in a kernel."""
     from provenloop_b200._lib import check, lib
