@@ -8,6 +8,7 @@
 // points' addresses come from the binding that loaded it (bind).
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAStream.h>
@@ -98,6 +99,13 @@ void no_history(const at::Tensor* t) {
     if (t && t->requires_grad() && at::GradMode::is_enabled())
         bad("an input requires a gradient, which this call does not record: call it under torch.no_grad() (adapter_project_backward "
             "gives the adapters' gradients)");
+    if (t && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined())
+        bad("an input has a forward-mode tangent, which this call would lose: call it on the primal (torch.autograd.forward_ad.unpack_dual)");
+}
+
+// `t` has been written: autograd finds out if it had saved it.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 void finish(int rc, const char* what) {
@@ -233,6 +241,7 @@ PyObject* project(PyObject*, PyObject* const* args, Py_ssize_t n) {
         q.out = out.mutable_data_ptr();
         run(q, false, x);
         if (given) {
+            written(*given);
             Py_INCREF(args[8]);
             return args[8];
         }
@@ -346,7 +355,7 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t count) {
             q.mask_stride = table(*v, "mask", v->scalar_type() == at::kInt, "int32", n, (vocab + 31) / 32, x);
             q.mask = static_cast<const int32_t*>(v->const_data_ptr());
         }
-        no_history(&x);
+        for (const at::Tensor* v : {&x, t[4], t[5], t[6], t[8]}) no_history(v);
         at::Tensor out;
         if (const at::Tensor* v = t[10]) {
             if (!write) bad("out is given, but write is false");
@@ -368,6 +377,7 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (picks.defined()) q.pick = static_cast<int64_t*>(picks.mutable_data_ptr());
         q.stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)q.device).stream();
         finish(g.rules(&q), "ts_logit_rules");
+        if (t[10]) written(*t[10]);
         PyObject* r = PyTuple_New(2);
         if (!r) throw PyFailed{};
         if (t[10]) {

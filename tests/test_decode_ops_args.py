@@ -75,6 +75,35 @@ def test_rules_refusals(change, match):
         logits.apply_rules(**{"logits": torch.zeros(2, 100), **change})
 
 
+_RULES = dict(tokens=torch.zeros(2, 5, dtype=torch.int64), repetition=torch.ones(2), frequency=torch.ones(2), presence=torch.ones(2),
+              bias_ids=torch.zeros(2, 3, dtype=torch.int64), bias_values=torch.zeros(2, 3))
+
+
+@pytest.mark.parametrize("name", ["repetition", "frequency", "presence", "bias_values"])
+def test_rules_refuse_parameters_that_want_gradients(name):
+    change = {name: _RULES[name].clone().requires_grad_()}
+    with pytest.raises(ValueError, match="no_grad"):
+        logits.apply_rules(**{"logits": torch.zeros(2, 100), **_RULES, **change})
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        logits.apply_rules(**{"logits": torch.zeros(2, 100), **_RULES, **change})
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    scale, bias, base = torch.ones(3), torch.zeros(24), torch.zeros(4, 24)
+    project = {**_tensors(), "scale": scale, "bias": bias, "base": base, "weight": torch.zeros(24, 16), "out": torch.zeros(4, 24)}
+    back = {**_tensors(), "grad": torch.zeros(4, 24), "scale": scale, "weight": torch.zeros(24, 16)}
+    rules = {"logits": torch.zeros(2, 100), **_RULES, "out": torch.zeros(2, 100)}
+    with fw.dual_level():
+        for call, args in ((adapters.adapter_project, project), (adapters.adapter_project_backward, back), (logits.apply_rules, rules)):
+            for name, t in args.items():
+                if t.is_floating_point():
+                    with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                        call(**{**args, name: fw.make_dual(t, torch.ones_like(t))})
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+                call(**args)
+
+
 # ---------------------------------------------------------------- C entry points
 
 _A = ("dtype device stream n per d_in d_out r adapters x x_stride weight w_stride bias base base_stride lora_a lora_b adapter scale "

@@ -246,6 +246,25 @@ def test_gradients_keep_the_intermediates_bits(A, n, i, o, r, dt, bits):
         assert ((g.double() - w).abs() <= tol * 1.01).all()
 
 
+def test_autograd_sees_what_is_overwritten(A, R):
+    """A tensor that autograd has saved and a call writes over makes the
+    backward pass an error, not a wrong gradient."""
+    s = _inputs(6, 64, 40, 8, 2, "fp32", "one")
+    w = torch.ones(40, device="cuda", requires_grad=True)
+    for write in (lambda t: A.adapter_project(s["x"], s["a"], s["b"], s["ids"], out=t),
+                  lambda t: A.adapter_project(s["x"], s["a"], s["b"], s["ids"], base=t, out=t),
+                  lambda t: R.apply_rules(t, out=t), lambda t: R.apply_rules(s["base"], out=t[:, :])):
+        saved = s["base"].clone()
+        loss = (saved * w).sum()
+        with torch.no_grad():
+            write(saved)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():  # tensors that count no versions
+        made = torch.zeros((6, 40), device="cuda")
+    assert A.adapter_project(s["x"], s["a"], s["b"], s["ids"], out=made) is made and made.any()
+
+
 def test_no_wait_ran_out():
     """Collected last: none of the calls above gave up a wait in a kernel."""
     from provenloop_b200._lib import check, lib
