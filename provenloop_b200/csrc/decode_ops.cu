@@ -415,6 +415,8 @@ extern "C" int ts_expired_waits(int device, uint64_t* out) {
         OnDevice dev(device);
         unsigned long long v = 0, w = 0;
         cudaError_t e = dev.status;
+        // the copies below wait for the legacy stream's work alone
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
         if (e == cudaSuccess) e = expired_waits_project(&v);
         if (e == cudaSuccess) e = expired_waits_rules(&w);
         *out = v + w;

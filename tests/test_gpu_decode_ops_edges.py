@@ -265,6 +265,22 @@ def test_autograd_sees_what_is_overwritten(A, R):
     assert A.adapter_project(s["x"], s["a"], s["b"], s["ids"], out=made) is made and made.any()
 
 
+def test_expired_waits_are_counted_behind_the_work():
+    """ts_expired_waits waits for streams that the legacy stream does not."""
+    from provenloop_b200._lib import check, lib
+    busy, v = torch.randn((8192, 8192), device="cuda"), C.c_uint64(1)
+    check(lib().ts_expired_waits(0, C.byref(v)))
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+        done.record()
+    assert not done.query()
+    check(lib().ts_expired_waits(0, C.byref(v)))
+    assert done.query() and v.value == 0
+
+
 def test_no_wait_ran_out():
     """Collected last: none of the calls above gave up a wait in a kernel."""
     from provenloop_b200._lib import check, lib
