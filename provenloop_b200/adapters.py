@@ -7,9 +7,10 @@ adapter or none, beside the projection that the adapters belong to:
 * ``adapter_project`` -- ``y = x W^T + bias + scale_e (x A_e^T) B_e^T``, or the
   same delta added to a projection that has been computed already;
 * ``adapter_project_backward`` -- the gradients for x and for the adapters
-  (the projection is frozen), with which adapters are trained.
+  (the projection is frozen), with which adapters are trained;
+* ``expired_waits`` -- whether a kernel has given up.
 
-Both take CUDA tensors, run on torch's current stream of their device and
+The first two take CUDA tensors, run on torch's current stream of their device and
 return without waiting; the workspace comes from torch's allocator, so calls
 may be captured in CUDA graphs and run on several streams.  They do not
 record autograd history and refuse inputs that ask for it: call them under
@@ -66,3 +67,18 @@ def adapter_project_backward(grad, x, lora_a, lora_b, adapter, weight=None, scal
     zeros.  (The gradient of base is ``grad`` itself.)  The order of every sum
     depends on the sizes, the indexes and the kind of GPU alone."""
     return (_ops or _load()).backward(grad, x, lora_a, lora_b, adapter, weight, scale, need_x, need_adapters)
+
+
+def expired_waits(device=None) -> int:
+    """How many waits inside kernels of this module and of ``logits`` have run
+    out (after two seconds) on ``device`` (default: the current one) since the
+    library was loaded.  Anything but 0 means that a kernel or the device is
+    broken and that some call's results are incomplete: the calls themselves do
+    not wait and cannot say so.  Waits for the device."""
+    import torch
+    d = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
+    if d.type != "cuda":
+        raise ValueError(f"{d} is not a CUDA device")
+    v = C.c_uint64()
+    check(lib().ts_expired_waits(torch.cuda.current_device() if d.index is None else d.index, C.byref(v)), "ts_expired_waits")
+    return v.value

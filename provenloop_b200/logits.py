@@ -6,6 +6,7 @@ requests, and the greedy pick.  It takes CUDA tensors, runs on torch's current
 stream of their device and returns without waiting.  The history, its lengths
 and all parameters are read on the device, so that a captured decode step
 that extends its own history replays with the new tokens.
+``adapters.expired_waits`` tells whether a kernel has given up a wait.
 """
 from __future__ import annotations
 

@@ -104,6 +104,23 @@ def test_forward_mode_tangents_are_refused():
                 call(**args)
 
 
+def test_expired_waits_reach_python(monkeypatch):
+    asked = []
+
+    class Fake:
+        @staticmethod
+        def ts_expired_waits(device, out):
+            asked.append(device)
+            C.cast(out, C.POINTER(C.c_uint64))[0] = 5 + device
+            return 0
+    monkeypatch.setattr(adapters, "lib", lambda: Fake)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    assert [adapters.expired_waits(d) for d in (None, 2, "cuda", "cuda:1", torch.device("cuda", 4))] == [8, 7, 8, 6, 9]
+    assert asked == [3, 2, 3, 1, 4]
+    with pytest.raises(ValueError, match="cpu"):
+        adapters.expired_waits("cpu")
+
+
 # ---------------------------------------------------------------- C entry points
 
 _A = ("dtype device stream n per d_in d_out r adapters x x_stride weight w_stride bias base base_stride lora_a lora_b adapter scale "
