@@ -34,6 +34,7 @@ Both take ``rules`` for the pick, the keyword arguments of
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 
@@ -124,7 +125,8 @@ def _generate(model, prompt_ids, tokens, rules, device, after=None):
 
 class LoraBatch:
     """Plaintext LoRA (q_proj, v_proj) on every layer of ``model`` for batches
-    of requests, each with its own adapter or none.
+    of requests, each with its own adapter or none.  Several threads may
+    ``generate`` at once.
 
     weights: per layer (A_q, A_v [experts, r, d], B_q [experts, d, r], B_v
     [experts, dv, r]), as ``HeLoraDecoder.weights`` holds them."""
@@ -134,7 +136,7 @@ class LoraBatch:
 
         p = next(model.parameters())
         self.model, self.dev = model, p.device
-        self._adapter = None  # int32 [requests], while ``generate`` runs
+        self._run = threading.local()  # .adapter, int32 [requests], while ``generate`` runs on a thread
         self._modules = []
         if len(weights) != len(model.model.layers):
             raise ValueError(f"{len(weights)} layers of adapters for {len(model.model.layers)} layers")
@@ -146,9 +148,10 @@ class LoraBatch:
 
     def _forward(self, module, plain, a, b):
         def forward(x):
-            if self._adapter is None:
+            adapter = getattr(self._run, "adapter", None)
+            if adapter is None:
                 return plain(x)
-            return adapter_project(x, a, b, self._adapter, weight=module.weight, bias=module.bias)
+            return adapter_project(x, a, b, adapter, weight=module.weight, bias=module.bias)
         return forward
 
     def generate(self, prompt_ids, adapter, tokens: int = 16, rules=None):
@@ -160,11 +163,11 @@ class LoraBatch:
         adapter = torch.as_tensor(adapter, dtype=torch.int32, device=self.dev)
         if ids.dim() != 2 or adapter.shape != (ids.shape[0],):
             raise ValueError("prompt_ids must be [requests, tokens] and adapter [requests]")
-        self._adapter = adapter
+        self._run.adapter = adapter
         try:
             return _generate(self.model, ids, tokens, rules, self.dev)
         finally:
-            self._adapter = None
+            self._run.adapter = None
 
     def remove(self):
         for module, before in reversed(self._modules):

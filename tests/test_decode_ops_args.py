@@ -230,3 +230,35 @@ def test_lora_batch_refusals():
             batch.generate(ids, adapter)
     batch.remove()
     assert "forward" not in linear.__dict__
+
+
+def test_lora_batch_on_two_threads(monkeypatch):
+    """The batch of one thread keeps its adapters when another one's ends."""
+    import threading
+    from types import SimpleNamespace as N
+    from provenloop_b200 import decode_step
+    linear = torch.nn.Linear(4, 4)
+    model = N(parameters=linear.parameters, model=N(layers=[N(self_attn=N(q_proj=linear, v_proj=torch.nn.Linear(4, 2)))]))
+    batch = decode_step.LoraBatch(model, [tuple(np.zeros(s, np.float32) for s in ((2, 3, 4), (2, 3, 4), (2, 4, 3), (2, 2, 3)))])
+    used, both, ended = {}, threading.Barrier(2, timeout=20), threading.Event()
+    monkeypatch.setattr(decode_step, "adapter_project", lambda x, a, b, adapter, **kw: used[len(adapter)].append(adapter.tolist()))
+
+    def decode(model, ids, *_):
+        n = ids.shape[0]
+        used[n] = []
+        both.wait()
+        if n == 2:
+            assert ended.wait(20)
+        linear(torch.zeros(n, 1, 4))
+
+    def first():
+        batch.generate([[1]], [1])
+        ended.set()
+
+    monkeypatch.setattr(decode_step, "_generate", decode)
+    thread = threading.Thread(target=first)
+    thread.start()
+    batch.generate([[1], [2]], [0, -1])
+    thread.join()
+    assert used == {1: [[1]], 2: [[0, -1]]}
+    batch.remove()
