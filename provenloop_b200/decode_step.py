@@ -289,7 +289,8 @@ class HeLoraDecoder:
         """Capture one decode step (static KV cache) as a CUDA graph on a
         side stream; returns run(prompt_id, n) that decodes n tokens from a
         one-token prompt by replaying it, under ``rules`` if given (their
-        tensors are read at every replay)."""
+        tensors are read at every replay, behind what the caller's current
+        stream holds).  The tokens are there when ``run.stream`` is done."""
         import torch
         from transformers import StaticCache
 
@@ -326,6 +327,7 @@ class HeLoraDecoder:
         def run(prompt_id: int, n: int, start_token: int = 0):
             if n > max_len:
                 raise ValueError(f"at most {max_len} tokens per capture")
+            stream.wait_stream(torch.cuda.current_stream(self.dev))  # it may hold new values of the rules
             with torch.cuda.stream(stream):
                 # the static cache keeps its own device write position
                 # (cumulative_length), which must restart with pos

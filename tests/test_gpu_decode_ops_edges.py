@@ -281,6 +281,28 @@ def test_expired_waits_are_counted_behind_the_work():
     assert done.query() and v.value == 0
 
 
+def test_captured_decode_sees_rules_changed_before_it():
+    """New values of the rules' tensors, queued on the current stream behind
+    other work, are the ones that the replay reads."""
+    from provenloop_b200 import tensafe_he
+    from provenloop_b200.decode_step import HeLoraDecoder, build_model
+    model, ctx = build_model(layers=1), tensafe_he.CkksContext(16384)
+    dec = HeLoraDecoder(model, ctx, ctx.keygen(0), rank=16, experts=3, seed=2)
+    mask = torch.zeros(((model.config.vocab_size + 31) // 32,), dtype=torch.int32, device="cuda")
+    run = dec.capture(max_len=4, rules=dict(mask=mask))
+    busy = torch.randn((8192, 8192), device="cuda")
+    torch.cuda.synchronize()
+    for allowed in (5, 77):
+        for _ in range(20):
+            busy @ busy
+        mask.zero_()
+        mask[allowed // 32:allowed // 32 + 1].fill_(1 << allowed % 32)
+        out = run(1, 3)
+        torch.cuda.synchronize()
+        assert out.tolist() == [[allowed] * 3]
+    dec.remove()
+
+
 def test_no_wait_ran_out():
     """Collected last: none of the calls above gave up a wait in a kernel."""
     from provenloop_b200._lib import check, lib
