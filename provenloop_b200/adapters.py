@@ -22,6 +22,7 @@ import ctypes as C
 import os
 import struct
 
+from . import build
 from ._lib import HERE, check, lib
 
 _ARGS = struct.Struct("@2iP2Q4IPqPqPPqPPPPPqPqPPPQ")  # ts_adapter_args, for callers of the C entry points
@@ -36,6 +37,8 @@ def _load():
         path = os.path.join(HERE, "_torch_ops.so")
         if not os.path.exists(path):
             raise ImportError(f"{path} not found; build it with `python -m provenloop_b200.build`")
+        if not build.torch_ops_fits():
+            raise ImportError(f"{path} was not built for {build.torch_tag()}; build it with `python -m provenloop_b200.build`")
         from . import _torch_ops
         L = lib()
         entries = (L.ts_adapter_workspace, L.ts_adapter_project, L.ts_adapter_project_backward, L.ts_logit_rules)

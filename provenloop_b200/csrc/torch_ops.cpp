@@ -414,4 +414,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods}
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_ops() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_ops() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", TSGPU_BUILT_FOR) < 0) Py_CLEAR(m);
+    return m;
+}
