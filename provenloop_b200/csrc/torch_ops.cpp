@@ -35,6 +35,12 @@ struct {
 // A Python error is set.
 struct PyFailed {};
 
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PyFailed{};
+    return v;
+}
+
 const at::Tensor* tensor(PyObject* o, const char* name, bool optional = false) {
     if (optional && o == Py_None) return nullptr;
     if (!THPVariable_Check(o)) bad(std::string(name) + " must be a tensor");
@@ -256,7 +262,7 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor &dy = *tensor(args[0], "grad"), &x = *tensor(args[1], "x"), &a = *tensor(args[2], "lora_a"), &b = *tensor(args[3], "lora_b"),
                          &ids = *tensor(args[4], "adapter");
         const at::Tensor *w = tensor(args[5], "weight", true), *scale = tensor(args[6], "scale", true);
-        const bool need_x = PyObject_IsTrue(args[7]) == 1, need_adapters = PyObject_IsTrue(args[8]) == 1;
+        const bool need_x = truth(args[7]), need_adapters = truth(args[8]);
         ts_adapter_args q{};
         common(q, x, a, b, ids, w, scale);
         c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
@@ -317,7 +323,7 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t count) {
                                             "bias_ids", "bias_values", "mask", "out"};
         const at::Tensor* t[11];
         for (int i = 1; i < 11; i++) t[i] = tensor(args[i], names[i], true);
-        const bool write = PyObject_IsTrue(args[11]) == 1, pick = PyObject_IsTrue(args[12]) == 1;
+        const bool write = truth(args[11]), pick = truth(args[12]);
         ts_rules_args q{};
         q.dtype = q.out_dtype = dtype_code(x.scalar_type());
         if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1)) bad("logits must be [n, vocab] with contiguous rows");

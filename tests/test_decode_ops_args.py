@@ -104,6 +104,16 @@ def test_forward_mode_tangents_are_refused():
                 call(**args)
 
 
+def test_flags_without_a_truth_value():
+    both = torch.ones(2, dtype=torch.bool)
+    for name in ("need_x", "need_adapters"):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            adapters.adapter_project_backward(grad=torch.zeros(4, 24), **_tensors(), **{name: both})
+    for name in ("write", "pick"):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            logits.apply_rules(torch.zeros(2, 100), **{name: both})
+
+
 def test_expired_waits_reach_python(monkeypatch):
     asked = []
 
