@@ -159,6 +159,8 @@ class LoraBatch:
         i (-1 for none); rows of ``rules`` belong to the requests."""
         import torch
 
+        if not self._modules:
+            raise RuntimeError("the adapters have been removed from the model")
         ids = torch.as_tensor(prompt_ids, device=self.dev)
         adapter = torch.as_tensor(adapter, dtype=torch.int32, device=self.dev)
         if ids.dim() != 2 or adapter.shape != (ids.shape[0],):

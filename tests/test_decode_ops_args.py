@@ -242,6 +242,22 @@ def test_lora_batch_refusals():
     assert "forward" not in linear.__dict__
 
 
+def _one_layer():
+    from types import SimpleNamespace as N
+    from provenloop_b200.decode_step import LoraBatch
+    linear = torch.nn.Linear(4, 4)
+    model = N(parameters=linear.parameters, model=N(layers=[N(self_attn=N(q_proj=linear, v_proj=torch.nn.Linear(4, 2)))]))
+    return linear, lambda: LoraBatch(model, [tuple(np.zeros(s, np.float32) for s in ((2, 3, 4), (2, 3, 4), (2, 4, 3), (2, 2, 3)))])
+
+
+def test_lora_batch_removed_does_not_decode():
+    _, make = _one_layer()
+    batch = make()
+    batch.remove()
+    with pytest.raises(RuntimeError, match="removed"):
+        batch.generate([[1]], [0])
+
+
 def test_lora_batch_on_two_threads(monkeypatch):
     """The batch of one thread keeps its adapters when another one's ends."""
     import threading
