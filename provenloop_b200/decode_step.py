@@ -143,8 +143,9 @@ class LoraBatch:
         for layer, (aq, av, bq, bv) in zip(model.model.layers, weights):
             for module, a, b in ((layer.self_attn.q_proj, aq, bq), (layer.self_attn.v_proj, av, bv)):
                 a, b = (torch.as_tensor(w).to(device=p.device, dtype=p.dtype).contiguous() for w in (a, b))
-                self._modules.append((module, module.__dict__.get("forward")))
-                module.forward = self._forward(module, module.forward, a, b)
+                before, own = module.__dict__.get("forward"), self._forward(module, module.forward, a, b)
+                self._modules.append((module, before, own))
+                module.forward = own
 
     def _forward(self, module, plain, a, b):
         def forward(x):
@@ -172,7 +173,10 @@ class LoraBatch:
             self._run.adapter = None
 
     def remove(self):
-        for module, before in reversed(self._modules):
+        """Leaves the model as it was; batches made later on it go first."""
+        if any(module.__dict__.get("forward") is not own for module, _, own in self._modules):
+            raise RuntimeError("another batch was made on this model later: remove that one first")
+        for module, before, _ in reversed(self._modules):
             if before is None:
                 del module.forward
             else:

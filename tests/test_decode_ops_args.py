@@ -258,6 +258,19 @@ def test_lora_batch_removed_does_not_decode():
         batch.generate([[1]], [0])
 
 
+def test_lora_batches_leave_a_model_in_turn():
+    linear, make = _one_layer()
+    first, second = make(), make()
+    over = linear.forward
+    with pytest.raises(RuntimeError, match="first"):
+        first.remove()
+    assert linear.forward is over  # the second one's adapters are still there
+    second.remove()
+    first.remove()
+    assert "forward" not in linear.__dict__
+    first.remove()
+
+
 def test_lora_batch_on_two_threads(monkeypatch):
     """The batch of one thread keeps its adapters when another one's ends."""
     import threading
