@@ -815,21 +815,21 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-// A window of W places of the tokens' list (adapter by adapter), 128 features
-// and RB * 8 rank indexes per CTA, so that CTAs have the same work however
-// the tokens are spread over the adapters.  For each adapter in the window, in
-// groups of 32 tokens, the rows are gathered and low^T x summed with matrix
-// instructions whose 16-row axis are the features and whose contraction the
-// tokens.  bf16: 16 x 8 x 16 products with low's two bf16 terms, which hold it
-// to 2^-15, operands transposed on the way from shared memory.  Else
-// 16 x 8 x 8 TF32 products: low is split into two TF32 parts, which leaves 2^-20 beside fp16 x, exact
-// in TF32 (65 us beside a base for 4096 tokens of 1536 and 1536, rank 64; 57 with
-// low in 11 bits alone), and 2^-22 beside f32 x, which is split as well (their products of infinities left apart cost 3 to 5 % of an f32 call:
-// 1024 tokens of 1536 -> 1536, rank 16: 261 us, 255 with NaNs for them).  An adapter that lies in one window is written here; the others' sums
-// over a window go to the workspace, and k_grad_sum adds them in the
-// windows' order.  Bound: reading x once per 64 rank indexes.  8192 tokens of
-// 1536 and 1536, rank 16, three adapters: 18 us, 2.8 TB/s; 2048 of 8960 and
-// 1536, rank 32: 26 us.
+// A window of W places of the tokens' list (adapter by adapter), 128 features and RB * 8
+// rank indexes per CTA, so that CTAs have the same work however the tokens are spread
+// over the adapters.  For each adapter in the window, in groups of 32 tokens, the rows
+// are gathered and low^T x summed with matrix instructions whose 16-row axis are the
+// features and whose contraction the tokens.  bf16: 16 x 8 x 16 products with low's two
+// bf16 terms, which hold it to 2^-15, operands transposed on the way from shared memory.
+// Else 16 x 8 x 8 TF32 products: low is split into two TF32 parts, which leaves 2^-20
+// beside fp16 x, exact in TF32 (65 us beside a base for 4096 tokens of 1536 and 1536,
+// rank 64; 57 with low in 11 bits alone), and 2^-22 beside f32 x, which is split as well
+// (their products of infinities left apart cost 3 to 5 % of an f32 call: 1024 tokens of
+// 1536 -> 1536, rank 16: 261 us, 255 with NaNs for them).  An adapter that lies in one
+// window is written here; the others' sums over a window go to the workspace, and
+// k_grad_sum adds them in the windows' order.  Bound: reading x once per 64 rank
+// indexes.  8192 tokens of 1536 and 1536, rank 16, three adapters: 18 us, 2.8 TB/s; 2048
+// of 8960 and 1536, rank 32: 26 us.
 template <class T, int RB>
 __global__ void __launch_bounds__(256, (GradTile<T, RB>::kPerSm)) k_grad(const GradPair both, int tiles0, int window, float* partial, int dependent) {
     using L = GradTile<T, RB>;

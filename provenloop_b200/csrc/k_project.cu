@@ -116,8 +116,7 @@ struct Shared {
 
 template <class T>
 __device__ __forceinline__ float elem(const void* p, long long i) {
-    if constexpr (sizeof(T) == 4) return static_cast<const float*>(p)[i];
-    else if constexpr (std::is_same<T, __half>::value) return __half2float(static_cast<const __half*>(p)[i]);
+    if constexpr (std::is_same<T, __half>::value) return __half2float(static_cast<const __half*>(p)[i]);
     else return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 

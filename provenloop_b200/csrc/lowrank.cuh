@@ -146,6 +146,7 @@ inline bool low_by_token(long long n, long long k0, long long k1, long long r, l
     const long long units = (adapters < tile ? adapters : tile) * (low_stride((int)r) / 16);
     return bytes <= (units > 32 ? 256ll : 48ll) << 20;
 }
+constexpr int kSms = 148;  // the workspace's rules and the gradients' order of sums go by a B200's, whatever device is current
 constexpr int kSmallTokens = 16;  // up to here W is streamed once past all tokens
 // The projection takes each token's factor from where it is, n o r elements
 // in all, up to 32 MiB of them; above that the factors are converted first
@@ -154,7 +155,7 @@ constexpr int kSmallTokens = 16;  // up to here W is streamed once past all toke
 // since only that way shares a contraction (217 tokens, 8960 -> 1536, rank 64:
 // 80 us for the backward call, 85 with converted factors).
 inline bool factor_by_token(long long n, long long o, long long r, long long k) {
-    return n * o * r * 2 <= 32ll << 20 || (k >= 4096 && ((n + 127) / 128) * ((o + 63) / 64) < 74);
+    return n * o * r * 2 <= 32ll << 20 || (k >= 4096 && ((n + 127) / 128) * ((o + 63) / 64) < kSms / 2);
 }
 
 // Places of the tokens' list that a CTA of the gradients takes: three CTAs for
@@ -164,11 +165,9 @@ inline bool factor_by_token(long long n, long long o, long long r, long long k) 
 // rank 64 over 1536 + 1536 take 57 us so and 147 us in windows of 32).
 inline int grad_ranks(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : (r + 63) / 64 * 64; }  // padded
 inline long long grad_tiles(long long k0, long long k1) { return (k0 + 127) / 128 + (k1 + 127) / 128; }
-constexpr int kGradSms = 148;  // fixed, so that the sums' order is the same on every device
 inline int grad_window(long long n, long long k0, long long k1, int r, int adapters) {
-    const int sms = kGradSms;
     const long long ctas = grad_tiles(k0, k1) * (r <= 64 ? 1 : (r + 63) / 64);
-    long long windows = (3 * sms + ctas - 1) / ctas;
+    long long windows = (3 * kSms + ctas - 1) / ctas;
     long long most = (n + 7) / 8 < adapters / 2 ? (n + 7) / 8 : adapters / 2;
     if (most < (n + 127) / 128) most = (n + 127) / 128;
     if (windows > most) windows = most;
