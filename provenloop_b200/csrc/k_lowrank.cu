@@ -824,8 +824,8 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
 // Else 16 x 8 x 8 TF32 products: low is split into two TF32 parts, which leaves 2^-20
 // beside fp16 x, exact in TF32 (65 us beside a base for 4096 tokens of 1536 and 1536,
 // rank 64; 57 with low in 11 bits alone), and 2^-22 beside f32 x, which is split as well
-// (their products of infinities left apart cost 3 to 5 % of an f32 call: 1024 tokens of
-// 1536 -> 1536, rank 16: 261 us, 255 with NaNs for them).  An adapter that lies in one
+// (their products of infinities left apart cost 1 to 3 % of an f32 call: 1024 tokens of
+// 1536 -> 1536, rank 16: 258 us, 255 with NaNs for them).  An adapter that lies in one
 // window is written here; the others' sums over a window go to the workspace, and
 // k_grad_sum adds them in the windows' order.  Bound: reading x once per 64 rank
 // indexes.  8192 tokens of 1536 and 1536, rank 16, three adapters: 18 us, 2.8 TB/s; 2048
