@@ -378,6 +378,108 @@ typedef struct ts_rules_args {
  * value (a NaN counts as greatest), or -1 where every value is -inf. */
 int ts_logit_rules(const ts_rules_args* args);
 
+/* ------------------------------------------------------------ training, plaintext
+ * What stands around ts_adapter_project_backward when adapters are trained:
+ * losses on next-token logits with their gradients, and the clipping of the
+ * adapters' gradients.  The conventions are those of the decode step above. */
+#define TS_LOSS_LOGPROBS 0          /* the calls, as ts_loss_workspace names them */
+#define TS_LOSS_LOGPROBS_BACKWARD 1
+#define TS_LOSS_POLICY 2
+#define TS_LOSS_PREFERENCE 3
+
+#define TS_REDUCE_TOKEN 0    /* kind of the policy loss: mean over the rows that count, */
+#define TS_REDUCE_SEQUENCE 1 /* mean over the sequences of each one's mean (0 where none counts), */
+#define TS_REDUCE_SUM 2      /* sum over the rows */
+
+#define TS_PREFER_SIGMOID 0 /* kind of the preference loss */
+#define TS_PREFER_HINGE 1
+#define TS_PREFER_SQUARED 2
+
+typedef struct ts_loss_args {
+    int32_t dtype;            /* of logits and grad */
+    int32_t device;
+    void* stream;
+    uint64_t n;               /* rows */
+    uint32_t vocab;
+    int32_t targets64;        /* targets are int64, else int32 */
+    const void* logits;       /* [n][vocab] */
+    int64_t logits_stride;
+    const void* targets;      /* [n]: the token whose log-probability is taken; outside [0, vocab): the row does not count */
+    const float* grad_logprobs; /* [n] (TS_LOSS_LOGPROBS_BACKWARD) */
+    uint32_t sequences;       /* of the two losses; a preference loss has the chosen ones first, then as many rejected ones */
+    int32_t kind;             /* TS_REDUCE_* or TS_PREFER_* */
+    const int32_t* starts;    /* [sequences + 1], ascending: sequence s has the rows starts[s] .. starts[s + 1]; rows in none do
+                                 not count.  NULL: n / sequences rows each */
+    const float* old_logprobs; /* [n], or NULL: the log-probabilities themselves (policy) */
+    const float* ref_logprobs; /* [n], or NULL: no KL term (policy), 0 (preference) */
+    const float* advantages;  /* [n] or [sequences] (policy) */
+    int32_t advantage_rows;   /* advantages has n entries */
+    int32_t average;          /* preference: a sequence's mean in place of its sum */
+    float clip_low, clip_high, kl; /* policy */
+    float beta, smoothing;    /* preference; smoothing of the sigmoid kind alone */
+    float reserved;           /* 0 */
+    const float* grad_scale;  /* one value that the losses' gradient is multiplied by, or NULL: 1 */
+    float* loss;              /* one value (the two losses) */
+    float* margins;           /* [sequences / 2], or NULL (preference) */
+    float* logprobs;          /* [n]; NULL where not wanted (the two losses) */
+    void* grad;               /* [n][vocab], may be logits itself (same stride); NULL where not wanted (the two losses) */
+    int64_t grad_stride;
+    void* workspace;          /* ts_loss_workspace bytes, 256-byte aligned; contents need not be kept */
+    uint64_t workspace_bytes;
+} ts_loss_args;
+
+/* Bytes of workspace that the call `op` (TS_LOSS_*) needs. */
+int ts_loss_workspace(const ts_loss_args* args, int op, uint64_t* bytes);
+/* logprobs[i] = log softmax(logits[i])[targets[i]]; 0 for rows that do not count. */
+int ts_token_logprobs(const ts_loss_args* args);
+/* grad[i][v] = grad_logprobs[i] ([v = targets[i]] - softmax(logits[i])[v]).  In
+ * this call and the next two, a row that does not count and one whose
+ * log-probability has the gradient 0 get zeros, whatever they hold; every row
+ * is written. */
+int ts_token_logprobs_backward(const ts_loss_args* args);
+/* With l the log-probability of a row that counts, rho = exp(l - old) and A its
+ * advantage: -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A)
+ * + kl (exp(ref - l) - (ref - l) - 1), reduced over the rows as `kind` says.  grad is
+ * grad_scale times the loss's gradient for the logits (old, ref and A held
+ * fixed; a ratio on a border counts as not clipped). */
+int ts_policy_loss(const ts_loss_args* args);
+/* Sequence p and sequence p + sequences / 2 are a pair.  With D the sum (or mean)
+ * of l - ref over the rows of the first that count less that over the second's, h = beta D:
+ * -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h), max(0, 1 - h), or
+ * (D - 1 / (2 beta))^2; loss is the mean over the pairs, margins the h.  grad as above. */
+int ts_preference_loss(const ts_loss_args* args);
+
+#define TS_CLIP_MAX_GROUPS 65535
+
+typedef struct ts_clip_tensor {
+    const void* grad;   /* elements one behind the other */
+    void* out;          /* may be grad itself (of the same type) */
+    uint64_t elements;  /* a multiple of the groups */
+    int32_t dtype;      /* of grad */
+    int32_t out_dtype;  /* dtype or TS_DTYPE_F32 */
+} ts_clip_tensor;
+
+typedef struct ts_clip_args {
+    int32_t device;
+    uint32_t groups;       /* 1, or the adapters of a stack: group e is the e-th of `groups` equal parts of every tensor */
+    void* stream;
+    uint64_t count;        /* tensors */
+    const ts_clip_tensor* tensors; /* in host memory, read before the call returns */
+    const float* max_norms; /* [groups] or one value in device memory, or NULL */
+    float max_norm;        /* where max_norms is NULL */
+    int32_t one_max;       /* max_norms has one value */
+    float* norms;          /* [groups] */
+    void* workspace;       /* ts_clip_workspace bytes, 256-byte aligned; contents need not be kept */
+    uint64_t workspace_bytes;
+} ts_clip_args;
+
+int ts_clip_workspace(const ts_clip_args* args, uint64_t* bytes);
+/* norms[e] = square root of the sum of the squares of group e's elements; out =
+ * grad min(1, max_norm / norm), rounded once.  A group whose norm is not
+ * finite is left as it is (copied to out): the norm says so.  The order of the
+ * sums depends on the sizes alone. */
+int ts_clip_gradients(const ts_clip_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,12 +94,19 @@ SIGNATURES = {
     "ts_lora_info": (cint, [vp, P(u32), P(u32), P(u32), P(u32), P(u32)]),
     "ts_lora_delta_batch": (cint, [vp, vp, vp, vp, u32, P(i32), P(i32), P(u64), vp, vp, cint]),
     "ts_dp_noise": (cint, [vp, vp, u32, u32, f64, f64, P(u64), cint]),
-    # argument blocks (ts_adapter_args, ts_rules_args) packed by struct.pack
+    # argument blocks (ts_adapter_args, ts_rules_args, ts_loss_args, ts_clip_args) packed by struct.pack
     "ts_adapter_workspace": (cint, [C.c_char_p, cint, P(u64)]),
     "ts_adapter_project": (cint, [C.c_char_p]),
     "ts_adapter_project_backward": (cint, [C.c_char_p]),
     "ts_expired_waits": (cint, [cint, P(u64)]),
     "ts_logit_rules": (cint, [C.c_char_p]),
+    "ts_loss_workspace": (cint, [C.c_char_p, cint, P(u64)]),
+    "ts_token_logprobs": (cint, [C.c_char_p]),
+    "ts_token_logprobs_backward": (cint, [C.c_char_p]),
+    "ts_policy_loss": (cint, [C.c_char_p]),
+    "ts_preference_loss": (cint, [C.c_char_p]),
+    "ts_clip_workspace": (cint, [C.c_char_p, P(u64)]),
+    "ts_clip_gradients": (cint, [C.c_char_p]),
 }
 
 

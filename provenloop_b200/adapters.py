@@ -8,9 +8,11 @@ adapter or none, beside the projection that the adapters belong to:
   same delta added to a projection that has been computed already;
 * ``adapter_project_backward`` -- the gradients for x and for the adapters
   (the projection is frozen), with which adapters are trained;
+* ``clip_gradients`` -- the norm of an adapter's gradients over all tensors,
+  for each adapter of a stack, and their clipping;
 * ``expired_waits`` -- whether a kernel has given up.
 
-The first two take CUDA tensors, run on torch's current stream of their device and
+The first three take CUDA tensors, run on torch's current stream of their device and
 return without waiting; the workspace comes from torch's allocator, so calls
 may be captured in CUDA graphs and run on several streams.  They do not
 record autograd history and refuse inputs that ask for it: call them under
@@ -26,6 +28,8 @@ from . import build
 from ._lib import HERE, check, lib
 
 _ARGS = struct.Struct("@2iP2Q4IPqPqPPqPPPPPqPqPPPQ")  # ts_adapter_args, for callers of the C entry points
+_CLIP_ARGS = struct.Struct("@iIPQPPfiPPQ")  # ts_clip_args
+_CLIP_TENSOR = struct.Struct("@PPQ2i")  # ts_clip_tensor
 _ops = None
 
 
@@ -41,7 +45,9 @@ def _load():
             raise ImportError(f"{path} was not built for {build.torch_tag()}; build it with `python -m provenloop_b200.build`")
         from . import _torch_ops
         L = lib()
-        entries = (L.ts_adapter_workspace, L.ts_adapter_project, L.ts_adapter_project_backward, L.ts_logit_rules)
+        entries = (L.ts_adapter_workspace, L.ts_adapter_project, L.ts_adapter_project_backward, L.ts_logit_rules, L.ts_loss_workspace,
+                   L.ts_token_logprobs, L.ts_token_logprobs_backward, L.ts_policy_loss, L.ts_preference_loss, L.ts_clip_workspace,
+                   L.ts_clip_gradients)
         _torch_ops.bind(*(C.cast(f, C.c_void_p).value for f in entries), check)
         _ops = _torch_ops
     return _ops
@@ -70,6 +76,26 @@ def adapter_project_backward(grad, x, lora_a, lora_b, adapter, weight=None, scal
     zeros.  (The gradient of base is ``grad`` itself.)  The order of every sum
     depends on the sizes, the indexes and the kind of GPU alone."""
     return (_ops or _load()).backward(grad, x, lora_a, lora_b, adapter, weight, scale, need_x, need_adapters)
+
+
+def clip_gradients(grads, max_norm, adapters=None, out=None):
+    """Scales gradients so that their norm is at most ``max_norm``, in place
+    or to ``out``; returns the norm from before.
+
+    grads: a list of CUDA tensors of any shapes (float32, bfloat16, float16, also
+    mixed; dense in memory), None entries are skipped.  The norm is the root of
+    the sum of all their squares: a 0-dim float32 tensor.  With ``adapters``
+    given, every tensor is a stack [adapters, ...] (contiguous), as
+    ``adapter_project_backward`` returns them, and each adapter has a norm over its part of
+    all tensors and is clipped by itself: float32 [adapters].  max_norm: a
+    number, or a float32 tensor with one value or one for each adapter, which is
+    read on the device.  out: a list of tensors like grads, each of its gradient's
+    dtype or float32; gradients that are only read may occur twice and then count twice.
+
+    Values are multiplied in 32 bits by min(1, max_norm / norm) and rounded
+    once.  What has a norm that is not finite is left as it is (or copied to ``out``): look
+    at the norm before the step.  The order of the sums depends on the sizes alone."""
+    return (_ops or _load()).clip(grads, max_norm, adapters, out)
 
 
 def expired_waits(device=None) -> int:

@@ -24,9 +24,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtsgpu.so")
 TORCH_OPS = os.path.join(HERE, "_torch_ops.so")  # torch tensors to argument blocks (csrc/torch_ops.cpp)
 SOURCES = ["kernels.cu", "k_ntt.cu", "k_encode.cu", "k_encrypt.cu", "k_decrypt.cu", "tsgpu.cu", "noalloc.cu",
-           "k_lowrank.cu", "k_project.cu", "k_rules.cu", "decode_ops.cu"]
+           "k_lowrank.cu", "k_project.cu", "k_rules.cu", "decode_ops.cu", "k_loss.cu", "k_clip.cu", "train_ops.cu"]
 HEADERS = ["common.cuh", "ntt.cuh", "fft.cuh", "kernels.cuh", "launch.cuh", "lowrank.cuh",
-           "sm100.cuh"]
+           "sm100.cuh", "entry.cuh", "train.cuh"]
 
 
 def nvcc_path() -> str:
@@ -143,7 +143,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         _finish("torch_ops.cpp", ops, verbose)
         os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
     elif not have_torch():
-        print("torch is not installed: _torch_ops.so (provenloop_b200.adapters and .logits) was not built", file=sys.stderr)
+        print("torch is not installed: _torch_ops.so (provenloop_b200.adapters, .logits and .losses) was not built", file=sys.stderr)
     return LIB
 
 

@@ -3,67 +3,14 @@
 // launches.  Nothing here keeps state between calls.
 #include <cstring>
 
-#include "../../include/tsgpu.h"
+#include "entry.cuh"
 #include "lowrank.cuh"
 
 using namespace tsg;
 
-namespace tsg_host {
-int noalloc_fail(int code, const char* msg);  // tsgpu.cu: sets the thread's last error
-}
-
 namespace {
 
-int bad(const char* msg) { return tsg_host::noalloc_fail(TS_ERR_ARG, msg); }
-
-// Makes `device` current for a scope.
-struct OnDevice {
-    int before = -1;
-    cudaError_t status;
-    explicit OnDevice(int device) {
-        status = cudaGetDevice(&before);
-        if (status != cudaSuccess) return;
-        if (before == device)
-            before = -1;
-        else
-            status = cudaSetDevice(device);
-    }
-    ~OnDevice() {
-        if (before >= 0) cudaSetDevice(before);
-    }
-};
-
-int cuda_status(cudaError_t e) {
-    if (e == cudaSuccess) return TS_OK;
-    const int code = e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? TS_ERR_NODEVICE : TS_ERR_CUDA;
-    cudaGetLastError();
-    return tsg_host::noalloc_fail(code, cudaGetErrorString(e));
-}
-
-// A matrix of `rows` rows of `row` bytes, `stride` bytes apart.
-struct Region {
-    uintptr_t p;
-    uint64_t rows, row, stride;
-    uint64_t bytes() const { return rows && p ? (rows - 1) * stride + row : 0; }
-};
-
-Region region(const void* p, uint64_t rows, uint64_t cols, int64_t stride, size_t size) {
-    return {reinterpret_cast<uintptr_t>(p), rows, cols * size, (uint64_t)stride * size};
-}
-
-bool overlap(const Region& a, const Region& b) {
-    if (!a.bytes() || !b.bytes() || a.p + a.bytes() <= b.p || b.p + b.bytes() <= a.p) return false;
-    if (a.stride != b.stride || !a.stride) return true;
-    // column ranges of one wider matrix
-    const uint64_t off = a.p <= b.p ? (b.p - a.p) % a.stride : (a.stride - (a.p - b.p) % a.stride) % a.stride;
-    return !(off >= a.row && off + b.row <= a.stride);
-}
-
-bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-
-constexpr uint64_t kMaxDim = 1u << 20, kMaxTokens = 1ull << 30, kMaxStride = 1ull << 40;
-
-bool stride_ok(int64_t s) { return s >= 0 && (uint64_t)s <= kMaxStride; }
+constexpr uint64_t kMaxDim = 1u << 20, kMaxTokens = 1ull << 30;
 
 int check_adapter(const ts_adapter_args* a, int backward) {
     if (!a) return bad("adapter arguments are NULL");
@@ -117,8 +64,6 @@ int check_adapter(const ts_adapter_args* a, int backward) {
     }
     return TS_OK;
 }
-
-uint64_t up(uint64_t b) { return (b + 255) & ~255ull; }
 
 // A row of `d` elements up to the next 16 bytes.
 int up16(uint32_t d, size_t size) { return (int)((d * size + 15) / 16 * (16 / size)); }
@@ -385,17 +330,6 @@ int logit_rules(const ts_rules_args* a) {
                       a->ids64 >> 1 & 1, reinterpret_cast<const uint32_t*>(a->mask), a->mask_stride, a->out, a->out_stride,
                       reinterpret_cast<long long*>(a->pick)};
     return cuda_status(launch_rules(k, a->dtype, a->out ? a->out_dtype : a->dtype, static_cast<cudaStream_t>(a->stream)));
-}
-
-// No exception leaves a C entry point (the launch bookkeeping may fail to
-// allocate on the host).
-template <class F>
-int guarded(F f) {
-    try {
-        return f();
-    } catch (...) {
-        return TS_ERR_OOM;
-    }
 }
 
 }  // namespace

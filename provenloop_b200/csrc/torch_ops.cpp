@@ -1,6 +1,6 @@
 // torch_ops.cpp -- torch tensors to the argument blocks of the plaintext
-// decode-step operators (include/tsgpu.h): the checks, the allocations and the
-// current stream of provenloop_b200.adapters and .logits.
+// operators (include/tsgpu.h): the checks, the allocations and the current
+// stream of provenloop_b200.adapters, .logits and .losses.
 //
 // A decode step makes these calls at every projection, and a call on one
 // token is shorter on the GPU than its checks were in Python: this module is
@@ -13,9 +13,12 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <climits>
+#include <memory>
 #include <sstream>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/tsgpu.h"
 
@@ -26,6 +29,10 @@ struct {
     decltype(&ts_adapter_project) project = nullptr;
     decltype(&ts_adapter_project_backward) backward = nullptr;
     decltype(&ts_logit_rules) rules = nullptr;
+    decltype(&ts_loss_workspace) loss_workspace = nullptr;
+    decltype(&ts_token_logprobs) losses[4] = {};  // by TS_LOSS_*
+    decltype(&ts_clip_workspace) clip_workspace = nullptr;
+    decltype(&ts_clip_gradients) clip = nullptr;
     PyObject* check = nullptr;  // _lib.check: raises for a status
 } g;
 
@@ -104,7 +111,7 @@ void whole(const at::Tensor& t, const char* name, at::ScalarType dtype, const at
 void no_history(const at::Tensor* t) {
     if (t && t->requires_grad() && at::GradMode::is_enabled())
         bad("an input requires a gradient, which this call does not record: call it under torch.no_grad() (adapter_project_backward "
-            "gives the adapters' gradients)");
+            "gives the adapters' gradients, the losses their logits')");
     if (t && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined())
         bad("an input has a forward-mode tangent, which this call would lose: call it on the primal (torch.autograd.forward_ad.unpack_dual)");
 }
@@ -397,15 +404,309 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
-// (addresses of ts_adapter_workspace, ts_adapter_project, ts_adapter_project_backward, ts_logit_rules, _lib.check)
+double number(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PyFailed{};
+    return v;
+}
+
+int whole_number(PyObject* o) {
+    const long v = PyLong_AsLong(o);
+    if (v == -1 && PyErr_Occurred()) throw PyFailed{};
+    if (v < INT_MIN || v > INT_MAX) bad("a number is too large");
+    return (int)v;
+}
+
+// f32 per row, of the targets' shape.
+const float* like_targets(const at::Tensor* t, const char* name, const at::Tensor& targets, const at::Tensor& x) {
+    if (!t) return nullptr;
+    whole(*t, name, at::kFloat, x, targets.sizes());
+    no_history(t);
+    return static_cast<const float*>(t->const_data_ptr());
+}
+
+const float* one_value(const at::Tensor* t, const char* name, const at::Tensor& x) {
+    if (!t) return nullptr;
+    if (t->scalar_type() != at::kFloat || t->numel() != 1) bad(std::string(name) + " must be one float32 value, not " + type_of(t->scalar_type()) + " " + shape_of(t->sizes()));
+    if (t->device() != x.device()) bad(std::string(name) + " is on " + t->device().str() + ", not on " + x.device().str());
+    no_history(t);
+    return static_cast<const float*>(t->const_data_ptr());
+}
+
+// Logits and targets of the losses and of the log-probabilities.
+void loss_rows(ts_loss_args& q, const at::Tensor& x, const at::Tensor& targets) {
+    q.dtype = dtype_code(x.scalar_type());
+    q.logits_stride = row_stride(x, "logits");
+    const auto size = x.sizes();
+    const int64_t vocab = size.back();
+    if (vocab == 0) bad("the vocabulary is empty");
+    if (vocab > 0x7fffffffll) bad("the vocabulary is too large");
+    if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt) bad("targets must be int32 or int64, not " + type_of(targets.scalar_type()));
+    whole(targets, "targets", targets.scalar_type(), x, size.slice(0, size.size() - 1));
+    no_history(&x);
+    q.targets64 = targets.scalar_type() == at::kLong;
+    q.n = (uint64_t)targets.numel(), q.vocab = (uint32_t)vocab;
+    q.logits = x.const_data_ptr(), q.targets = targets.const_data_ptr();
+}
+
+// The sequences that the rows of a loss form.
+void loss_sequences(ts_loss_args& q, const at::Tensor& x, const at::Tensor& targets, const at::Tensor* starts) {
+    if (starts) {
+        if (targets.dim() != 1) bad("with starts, logits must be [rows, vocab] and targets [rows]");
+        if (starts->dim() != 1 || starts->size(0) < 2) bad("starts must hold the sequences' first rows and the end of the last, not " + shape_of(starts->sizes()));
+        whole(*starts, "starts", at::kInt, x, {starts->size(0)});
+        if (starts->size(0) > 0x40000000ll) bad("too many sequences");
+        q.starts = static_cast<const int32_t*>(starts->const_data_ptr());
+        q.sequences = (uint32_t)(starts->size(0) - 1);
+    } else {
+        if (targets.dim() > 1 && targets.size(0) > 0x40000000ll) bad("too many sequences");
+        q.sequences = targets.dim() > 1 ? (uint32_t)targets.size(0) : 1;
+    }
+}
+
+// The gradient's tensor: `given`, or a new one, or none.  Everything else has
+// been checked; sets the device.
+at::Tensor loss_grad(ts_loss_args& q, const at::Tensor& x, const at::Tensor* given, bool need) {
+    at::Tensor grad;
+    if (given) {
+        if (!need) bad("out is given, but no gradient is asked for");
+        same(*given, "out", x.scalar_type(), x, x.sizes());
+        q.grad_stride = row_stride(*given, "out");
+        no_history(given);
+        grad = *given;
+    }
+    q.device = on_device(x, "the tensors");
+    if (!given && need) {
+        grad = at::empty(x.sizes(), x.options());
+        q.grad_stride = x.sizes().back();
+    }
+    if (grad.defined()) q.grad = grad.mutable_data_ptr();
+    return grad;
+}
+
+void run_loss(ts_loss_args& q, int op, const at::Tensor& x) {
+    static const char* const names[] = {"ts_token_logprobs", "ts_token_logprobs_backward", "ts_policy_loss", "ts_preference_loss"};
+    q.stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)q.device).stream();
+    uint64_t bytes = 0;
+    finish(g.loss_workspace(&q, op, &bytes), "ts_loss_workspace");
+    at::Tensor ws;
+    if (bytes) {
+        ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        q.workspace = ws.mutable_data_ptr();
+        q.workspace_bytes = bytes;
+    }
+    finish(g.losses[op](&q), names[op]);
+}
+
+PyObject* given_or(const at::Tensor* given, PyObject* object, const at::Tensor& t) {
+    if (!given) return none_or(t);
+    written(*given);
+    Py_INCREF(object);
+    return object;
+}
+
+// (logits, targets) -> logprobs
+PyObject* logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&] {
+        arity(n, 2);
+        const at::Tensor &x = *tensor(args[0], "logits"), &targets = *tensor(args[1], "targets");
+        ts_loss_args q{};
+        loss_rows(q, x, targets);
+        q.device = on_device(x, "the tensors");
+        at::Tensor out = at::empty(targets.sizes(), x.options().dtype(at::kFloat));
+        q.logprobs = static_cast<float*>(out.mutable_data_ptr());
+        run_loss(q, TS_LOSS_LOGPROBS, x);
+        return THPVariable_Wrap(out);
+    });
+}
+
+// (grad, logits, targets, out) -> gradient of logits
+PyObject* logprobs_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&] {
+        arity(n, 4);
+        const at::Tensor &dy = *tensor(args[0], "grad"), &x = *tensor(args[1], "logits"), &targets = *tensor(args[2], "targets");
+        const at::Tensor* given = tensor(args[3], "out", true);
+        ts_loss_args q{};
+        loss_rows(q, x, targets);
+        q.grad_logprobs = like_targets(&dy, "grad", targets, x);
+        const at::Tensor grad = loss_grad(q, x, given, true);
+        run_loss(q, TS_LOSS_LOGPROBS_BACKWARD, x);
+        return given_or(given, args[3], grad);
+    });
+}
+
+// (logits, targets, old, advantages, ref, starts, clip_low, clip_high, kl, kind, grad_scale, need_grad, out) -> (loss, logprobs, grad or None)
+PyObject* policy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        arity(n, 13);
+        const at::Tensor &x = *tensor(args[0], "logits"), &targets = *tensor(args[1], "targets"), &adv = *tensor(args[3], "advantages");
+        const at::Tensor *old = tensor(args[2], "old_logprobs", true), *ref = tensor(args[4], "ref_logprobs", true),
+                         *starts = tensor(args[5], "starts", true), *scale = tensor(args[10], "grad_scale", true), *given = tensor(args[12], "out", true);
+        ts_loss_args q{};
+        loss_rows(q, x, targets);
+        loss_sequences(q, x, targets, starts);
+        q.old_logprobs = like_targets(old, "old_logprobs", targets, x);
+        q.ref_logprobs = like_targets(ref, "ref_logprobs", targets, x);
+        if (adv.sizes() == targets.sizes()) {
+            q.advantages = like_targets(&adv, "advantages", targets, x);
+            q.advantage_rows = 1;
+        } else {
+            whole(adv, "advantages", at::kFloat, x, {(int64_t)q.sequences});
+            no_history(&adv);
+            q.advantages = static_cast<const float*>(adv.const_data_ptr());
+        }
+        q.clip_low = (float)number(args[6]), q.clip_high = (float)number(args[7]), q.kl = (float)number(args[8]);
+        q.kind = whole_number(args[9]);
+        q.grad_scale = one_value(scale, "grad_scale", x);
+        const bool need = truth(args[11]);
+        const at::Tensor grad = loss_grad(q, x, given, need);
+        at::Tensor loss = at::empty({}, x.options().dtype(at::kFloat)), lp = at::empty(targets.sizes(), x.options().dtype(at::kFloat));
+        q.loss = static_cast<float*>(loss.mutable_data_ptr()), q.logprobs = static_cast<float*>(lp.mutable_data_ptr());
+        run_loss(q, TS_LOSS_POLICY, x);
+        PyObject* r = PyTuple_New(3);
+        if (!r) throw PyFailed{};
+        PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(loss));
+        PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lp));
+        PyTuple_SET_ITEM(r, 2, given_or(given, args[12], grad));
+        return r;
+    });
+}
+
+// (logits, targets, ref, starts, beta, kind, smoothing, average, grad_scale, need_grad, out) -> (loss, margins, logprobs, grad or None)
+PyObject* preference(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        arity(n, 11);
+        const at::Tensor &x = *tensor(args[0], "logits"), &targets = *tensor(args[1], "targets");
+        const at::Tensor *ref = tensor(args[2], "ref_logprobs", true), *starts = tensor(args[3], "starts", true),
+                         *scale = tensor(args[8], "grad_scale", true), *given = tensor(args[10], "out", true);
+        ts_loss_args q{};
+        loss_rows(q, x, targets);
+        loss_sequences(q, x, targets, starts);
+        if (q.sequences % 2) bad("the sequences must be the chosen ones and as many rejected ones, not " + std::to_string(q.sequences));
+        q.ref_logprobs = like_targets(ref, "ref_logprobs", targets, x);
+        q.beta = (float)number(args[4]), q.kind = whole_number(args[5]), q.smoothing = (float)number(args[6]);
+        q.average = truth(args[7]);
+        q.grad_scale = one_value(scale, "grad_scale", x);
+        const bool need = truth(args[9]);
+        const at::Tensor grad = loss_grad(q, x, given, need);
+        const auto f32 = x.options().dtype(at::kFloat);
+        at::Tensor loss = at::empty({}, f32), margins = at::empty({(int64_t)(q.sequences / 2)}, f32), lp = at::empty(targets.sizes(), f32);
+        q.loss = static_cast<float*>(loss.mutable_data_ptr()), q.margins = static_cast<float*>(margins.mutable_data_ptr());
+        q.logprobs = static_cast<float*>(lp.mutable_data_ptr());
+        run_loss(q, TS_LOSS_PREFERENCE, x);
+        PyObject* r = PyTuple_New(4);
+        if (!r) throw PyFailed{};
+        PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(loss));
+        PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(margins));
+        PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(lp));
+        PyTuple_SET_ITEM(r, 3, given_or(given, args[10], grad));
+        return r;
+    });
+}
+
+// A list or tuple for a scope.
+struct Items {
+    PyObject* o;
+    Items(PyObject* list, const char* name) : o(PySequence_Check(list) && !THPVariable_Check(list) ? PySequence_Fast(list, "") : nullptr) {
+        if (!o) {
+            PyErr_Clear();
+            bad(std::string(name) + " must be a list of tensors");
+        }
+    }
+    ~Items() { Py_DECREF(o); }
+    Items(const Items&) = delete;
+    Items& operator=(const Items&) = delete;
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(o); }
+    PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(o, i); }
+};
+
+// (grads, max_norm, adapters or None, out or None) -> norms
+PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        arity(n, 4);
+        const Items grads(args[0], "grads");
+        const bool apart = args[3] != Py_None;
+        std::unique_ptr<Items> outs(apart ? new Items(args[3], "out") : nullptr);
+        if (apart && outs->size() != grads.size()) bad("out must have as many tensors as grads");
+        const bool each = args[2] != Py_None;
+        const int groups = each ? whole_number(args[2]) : 1;
+        if (groups < 1 || groups > TS_CLIP_MAX_GROUPS) bad("the number of adapters must be in 1 .. " + std::to_string(TS_CLIP_MAX_GROUPS));
+        std::vector<ts_clip_tensor> list;
+        list.reserve(grads.size());
+        const at::Tensor* like = nullptr;
+        for (Py_ssize_t i = 0; i < grads.size(); i++) {
+            if (grads[i] == Py_None) continue;
+            const at::Tensor& t = *tensor(grads[i], "every entry of grads");
+            if (!like) like = &t;
+            ts_clip_tensor c{};
+            c.dtype = c.out_dtype = dtype_code(t.scalar_type());
+            if (t.device() != like->device()) bad("a gradient is on " + t.device().str() + ", not on " + like->device().str());
+            if (each ? !t.is_contiguous() : !t.is_non_overlapping_and_dense())
+                bad(each ? "the gradients of stacked adapters must be contiguous" : "the gradients must be dense in memory");
+            if (each && (t.dim() < 1 || t.size(0) != groups))
+                bad("the gradients of " + std::to_string(groups) + " stacked adapters must have that leading dimension, not " + shape_of(t.sizes()));
+            no_history(&t);
+            c.elements = (uint64_t)t.numel();
+            if (apart) {
+                const at::Tensor& o = *tensor((*outs)[i], "every entry of out");
+                if (o.sizes() != t.sizes() || o.device() != t.device() || (o.scalar_type() != t.scalar_type() && o.scalar_type() != at::kFloat))
+                    bad("an entry of out must be " + shape_of(t.sizes()) + " on " + t.device().str() + ", " + type_of(t.scalar_type()) + " or torch.float32");
+                if (o.strides() != t.strides() && !(o.is_contiguous() && t.is_contiguous())) bad("an entry of out must have its gradient's layout in memory");
+                no_history(&o);
+                c.out_dtype = dtype_code(o.scalar_type());
+                c.out = o.mutable_data_ptr();
+                c.grad = t.const_data_ptr();
+            } else {
+                c.grad = c.out = t.mutable_data_ptr();
+            }
+            list.push_back(c);
+        }
+        if (!like) bad("grads has no tensors");
+        ts_clip_args q{};
+        q.groups = (uint32_t)groups, q.count = list.size(), q.tensors = list.data();
+        if (THPVariable_Check(args[1])) {
+            const at::Tensor& m = THPVariable_Unpack(args[1]);
+            q.one_max = m.numel() == 1;
+            if (m.scalar_type() != at::kFloat || !m.is_contiguous() || (!q.one_max && (!each || m.dim() != 1 || m.size(0) != groups)))
+                bad("max_norm must be a number, one float32 value or one for each adapter, not " + type_of(m.scalar_type()) + " " + shape_of(m.sizes()));
+            if (m.device() != like->device()) bad("max_norm is on " + m.device().str() + ", not on " + like->device().str());
+            no_history(&m);
+            q.max_norms = static_cast<const float*>(m.const_data_ptr());
+        } else {
+            q.max_norm = (float)number(args[1]);
+            if (!(q.max_norm >= 0.f)) bad("max_norm must not be negative");
+        }
+        q.device = on_device(*like, "the tensors");
+        at::Tensor norms = each ? at::empty({groups}, like->options().dtype(at::kFloat)) : at::empty({}, like->options().dtype(at::kFloat));
+        q.norms = static_cast<float*>(norms.mutable_data_ptr());
+        q.stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)q.device).stream();
+        uint64_t bytes = 0;
+        finish(g.clip_workspace(&q, &bytes), "ts_clip_workspace");
+        at::Tensor ws = at::empty({(int64_t)bytes}, like->options().dtype(at::kByte));
+        q.workspace = ws.mutable_data_ptr();
+        q.workspace_bytes = bytes;
+        finish(g.clip(&q), "ts_clip_gradients");
+        const Items& changed = apart ? *outs : grads;
+        for (Py_ssize_t i = 0; i < grads.size(); i++)
+            if (grads[i] != Py_None) written(THPVariable_Unpack(changed[i]));
+        return THPVariable_Wrap(norms);
+    });
+}
+
+// (addresses of ts_adapter_workspace, ts_adapter_project, ts_adapter_project_backward, ts_logit_rules, ts_loss_workspace,
+// ts_token_logprobs, ts_token_logprobs_backward, ts_policy_loss, ts_preference_loss, ts_clip_workspace, ts_clip_gradients, _lib.check)
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long a[4];
+    unsigned long long a[11];
     PyObject* check;
-    if (!PyArg_ParseTuple(args, "KKKKO", &a[0], &a[1], &a[2], &a[3], &check)) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10], &check)) return nullptr;
     g.workspace = reinterpret_cast<decltype(g.workspace)>(a[0]);
     g.project = reinterpret_cast<decltype(g.project)>(a[1]);
     g.backward = reinterpret_cast<decltype(g.backward)>(a[2]);
     g.rules = reinterpret_cast<decltype(g.rules)>(a[3]);
+    g.loss_workspace = reinterpret_cast<decltype(g.loss_workspace)>(a[4]);
+    for (int i = 0; i < 4; i++) g.losses[i] = reinterpret_cast<decltype(g.losses[i])>(a[5 + i]);
+    g.clip_workspace = reinterpret_cast<decltype(g.clip_workspace)>(a[9]);
+    g.clip = reinterpret_cast<decltype(g.clip)>(a[10]);
     Py_INCREF(check);
     Py_XSETREF(g.check, check);
     Py_RETURN_NONE;
@@ -415,6 +716,11 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"project", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(project)), METH_FASTCALL, nullptr},
                          {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(backward)), METH_FASTCALL, nullptr},
                          {"rules", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rules)), METH_FASTCALL, nullptr},
+                         {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(logprobs)), METH_FASTCALL, nullptr},
+                         {"logprobs_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(logprobs_backward)), METH_FASTCALL, nullptr},
+                         {"policy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(policy)), METH_FASTCALL, nullptr},
+                         {"preference", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(preference)), METH_FASTCALL, nullptr},
+                         {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods};
 

@@ -1,0 +1,99 @@
+// train.cuh -- internal interface between the C entry points of the training
+// operators (train_ops.cu) and their kernels (k_loss.cu, k_clip.cu).  Not part
+// of the public ABI.
+#pragma once
+#include "lowrank.cuh"
+
+namespace tsg {
+
+// Rows of logits, what of each counts, and where they lie.
+struct LossRows {
+    const void* logits;
+    long long stride;
+    long long n;
+    uint32_t vocab;
+    int targets64;
+    const void* targets;
+    uint32_t sequences;
+    const int32_t* starts;  // or null: `per` rows each
+    long long per;
+#ifdef __CUDACC__
+    // The row's target, or -1: it does not count.
+    __device__ __forceinline__ int target(long long row) const {
+        const long long y = targets64 ? static_cast<const long long*>(targets)[row] : (long long)static_cast<const int32_t*>(targets)[row];
+        return (unsigned long long)y < vocab ? (int)y : -1;
+    }
+    // The row's sequence, or -1: it is in none (with `starts` alone).
+    __device__ __forceinline__ int sequence(long long row) const {
+        if (!starts) return (int)(row / per);
+        if (row < starts[0] || row >= starts[sequences]) return -1;
+        uint32_t lo = 0, hi = sequences;  // starts[lo] <= row < starts[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (row < starts[mid]) hi = mid;
+            else lo = mid;
+        }
+        return (int)lo;
+    }
+#endif
+};
+
+// max of a row and the sum of exp(z - max).
+struct RowStats {
+    float max, sum;
+};
+
+struct PolicyTerms {
+    const float *old, *ref, *advantages;
+    int advantage_rows, kind;
+    float low, high, kl;  // 1 - clip_low, 1 + clip_high
+};
+
+struct PreferTerms {
+    const float* ref;
+    int kind, average;
+    float beta, smoothing;
+};
+
+// What a loss's launches hand to one another, in the workspace.
+struct LossWork {
+    int* sequence;    // [n]: of a row that counts, else -1 (policy)
+    int* counts;      // [sequences + 1]: rows that count, and all of them (policy)
+    RowStats* stats;  // [n] (preference)
+    float* slope;     // [sequences]: d loss / d log-probability (preference)
+    double* parts;    // [n] (policy), [pairs] (preference): the loss is their sum
+};
+
+struct LossOut {
+    float *loss, *margins, *logprobs;
+    void* grad;
+    long long grad_stride;
+    const float* grad_scale;
+};
+
+cudaError_t launch_logprobs(const LossRows& r, float* logprobs, int dtype, cudaStream_t s);
+cudaError_t launch_logprobs_backward(const LossRows& r, const float* g, const LossOut& o, int dtype, cudaStream_t s);
+cudaError_t launch_policy(const LossRows& r, const PolicyTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s);
+cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s);
+
+// One group's part of one tensor.
+struct ClipTensor {
+    const void* grad;
+    void* out;
+    uint64_t part;  // elements of a group
+    int dtype, out_dtype;
+};
+struct ClipArgs {
+    const ClipTensor* tensors;  // host memory
+    uint64_t count;
+    uint32_t groups;
+    const float* max_norms;
+    float max_norm;
+    int one_max;
+    float* norms;
+    double* partial;  // clip_partials(...) of them
+};
+uint64_t clip_partials(const ClipTensor* t, uint64_t count, uint32_t groups);
+cudaError_t launch_clip(const ClipArgs& a, cudaStream_t s);
+
+}  // namespace tsg
