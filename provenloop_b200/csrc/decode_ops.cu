@@ -5,6 +5,7 @@
 
 #include "entry.cuh"
 #include "lowrank.cuh"
+#include "train.cuh"
 
 using namespace tsg;
 
@@ -347,13 +348,14 @@ extern "C" int ts_expired_waits(int device, uint64_t* out) {
     if (!out) return bad("out is NULL");
     return guarded([&] {
         OnDevice dev(device);
-        unsigned long long v = 0, w = 0;
+        unsigned long long v = 0, w = 0, l = 0;
         cudaError_t e = dev.status;
         // the copies below wait for the legacy stream's work alone
         if (e == cudaSuccess) e = cudaDeviceSynchronize();
         if (e == cudaSuccess) e = expired_waits_project(&v);
         if (e == cudaSuccess) e = expired_waits_rules(&w);
-        *out = v + w;
+        if (e == cudaSuccess) e = expired_waits_loss(&l);
+        *out = v + w + l;
         return cuda_status(e);
     });
 }

@@ -6,9 +6,13 @@
 //   out = g min(1, max_e / norm_e), rounded once
 // A group whose norm is not finite is left as it is.
 //
-// The bound is the tensors' traffic.  Parts go in chunks; each chunk's sum of
-// squares is a 64-bit value of its own, and a group's are added in an order
-// that depends on the sizes alone.
+// The bound is the tensors' traffic: each element is read for the norm, and
+// read and written for the clipping.  Three launches: the sums of squares of chunks
+// of parts, the norms, and the scaling, which goes backwards over the chunks,
+// since the latest are still in L2.
+//
+// A chunk's sum of squares is a 64-bit value of its own, and a group's are
+// added in an order that depends on the sizes alone.
 #include "launch.cuh"
 #include "sm100.cuh"
 #include "train.cuh"
@@ -17,9 +21,9 @@ namespace tsg {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr uint32_t kChunk = 16384;  // elements of a part that a CTA takes
-constexpr int kTable = 128;         // tensors in a launch's arguments
+constexpr int kThreads = 512;
+constexpr uint32_t kChunkBytes = 32768;  // of a part that a CTA takes at a time
+constexpr int kMinTable = 16, kMaxTable = 448;  // tensors in a launch's arguments (14 KB of at most 32)
 
 struct ClipEntry {
     const void* grad;
@@ -28,27 +32,37 @@ struct ClipEntry {
     uint32_t chunk0;  // chunks of a group in the entries before
     int16_t dtype, out_dtype;
 };
+template <int N>
 struct ClipTable {
-    ClipEntry t[kTable];
+    ClipEntry t[N];
     int count;
-    uint32_t chunks;      // of a group in this launch
+    uint32_t chunks;            // of a group in this launch
     uint32_t group_chunks, at;  // of a group in all launches, and in those before
-    double* partial;      // [groups][group_chunks]
-    const float* factor;  // [groups]
+    double* partial;            // [groups][group_chunks]
+    float* factor;              // [groups]
 };
 
-__device__ __forceinline__ const ClipEntry& entry_of(const ClipTable& a, uint32_t chunk) {
+__host__ __device__ __forceinline__ uint32_t chunk_elements(int dtype) { return kChunkBytes / (dtype == DT_F32 ? 4 : 2); }
+
+// Elements of one chunk.
+struct Piece {
+    const ClipEntry* t;
+    uint64_t from;  // in the tensor
+    uint32_t n;
+};
+template <int N>
+__device__ __forceinline__ Piece piece_of(const ClipTable<N>& a, uint32_t group, uint32_t chunk) {
     int lo = 0, hi = a.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
         if (chunk < a.t[mid].chunk0) hi = mid;
         else lo = mid;
     }
-    return a.t[lo];
+    const ClipEntry& t = a.t[lo];
+    const uint32_t most = chunk_elements(t.dtype);
+    const uint64_t at = (uint64_t)(chunk - t.chunk0) * most, left = t.part - at;
+    return {&t, group * t.part + at, left < most ? (uint32_t)left : most};
 }
-
-template <class T>
-__device__ __forceinline__ float value(T v) { return (float)v; }
 
 template <int N>
 __device__ double block_total(double v) {
@@ -62,103 +76,167 @@ __device__ double block_total(double v) {
     return v;
 }
 
-// Sum of the squares of n elements.  Those of a vector are added in 32 bits,
-// and once more in 64 where that may overflow or lose what is small.
+template <class T>
+__device__ __forceinline__ float value(T v) { return (float)v; }
+
+// Sum of a vector's squares: in 32 bits, and once more in 64 where that may
+// overflow or lose what is small.
+template <class T>
+__device__ __forceinline__ double vector_squares(const uint4& z) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    const T* e = reinterpret_cast<const T*>(&z);
+    float s = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) s = fmaf(value(e[i]), value(e[i]), s);
+    if ((s > 1e-30f && s < 1e37f) || ((z.x | z.y | z.z | z.w) & 0x7fff7fffu) == 0) return s;
+    double d = 0.0;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) d += (double)value(e[i]) * value(e[i]);
+    return d;
+}
+
+// f(vector's place p, vector) and g(element's place) over n elements at x, whose
+// places count from head, x's offset from a 16-byte boundary: whole vectors, four at
+// a time, and the elements at the ends.
+template <class T, class F, class E>
+__device__ __forceinline__ void each(const T* x, uint32_t n, F vector, E element) {
+    constexpr uint32_t N = 16 / sizeof(T), STEP = kThreads * N;
+    const uint32_t head = (uint32_t)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), end = head + n;
+    const uint32_t lo = head ? N : 0, hi = end / N * N;  // places of whole vectors
+    for (uint32_t p = lo + threadIdx.x * N; p < hi; p += 4 * STEP) {
+        uint4 z[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (p + j * STEP < hi) z[j] = *reinterpret_cast<const uint4*>(x + (p + j * STEP) - head);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+            if (p + j * STEP < hi) vector(p + j * STEP - head, z[j]);
+    }
+    // at most N - 1 elements before and behind, or all of them where there is no whole vector
+    const uint32_t i = threadIdx.x, first = min(lo, end);
+    if (i >= head && i < first) element(i - head);
+    const uint32_t tail = max(hi, first);
+    if (tail + i < end) element(tail + i - head);
+}
+
 template <class T>
 __device__ double squares(const T* x, uint32_t n) {
-    constexpr uint32_t N = 16 / sizeof(T);
-    const uint32_t head = (uint32_t)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), end = head + n;
     double total = 0.0;
-    for (uint32_t p = threadIdx.x * N; p < end; p += kThreads * N) {
-        if (p >= head && p + N <= end) {
-            const uint4 z = *reinterpret_cast<const uint4*>(x + p - head);
-            const T* e = reinterpret_cast<const T*>(&z);
-            float s = 0.f;
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) s = fmaf(value(e[i]), value(e[i]), s);
-            if (s > 1e-30f && s < 1e37f) {
-                total += s;
-            } else {
-                for (uint32_t i = 0; i < N; i++) total += (double)value(e[i]) * value(e[i]);
-            }
-        } else {
-            for (uint32_t i = 0; i < N; i++)
-                if (p + i >= head && p + i < end) total += (double)value(x[p + i - head]) * value(x[p + i - head]);
-        }
-    }
+    each(x, n, [&](uint32_t, const uint4& z) { total += vector_squares<T>(z); },
+         [&](uint32_t i) { total += (double)value(x[i]) * value(x[i]); });
     return total;
 }
 
 template <class T, class O>
-__device__ void scaled(const T* x, O* out, uint32_t n, float by) {
-    constexpr uint32_t N = 16 / sizeof(T);
-    const uint32_t head = (uint32_t)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)), end = head + n;
-    const bool whole = (reinterpret_cast<uintptr_t>(out) - head * sizeof(O)) % 16 == 0;
-    for (uint32_t p = threadIdx.x * N; p < end; p += kThreads * N) {
-        if (whole && p >= head && p + N <= end) {
-            const uint4 z = *reinterpret_cast<const uint4*>(x + p - head);
-            const T* e = reinterpret_cast<const T*>(&z);
-            uint4 r[sizeof(O) / sizeof(T)];
-            O* o = reinterpret_cast<O*>(r);
+__device__ __forceinline__ void put(O* out, const uint4& z, float by) {
+    constexpr uint32_t N = 16 / sizeof(T), W = sizeof(O) / sizeof(T);
+    const T* e = reinterpret_cast<const T*>(&z);
+    uint4 r[W];
+    O* o = reinterpret_cast<O*>(r);
 #pragma unroll
-            for (uint32_t i = 0; i < N; i++) o[i] = (O)(value(e[i]) * by);
+    for (uint32_t i = 0; i < N; i++) o[i] = (O)(value(e[i]) * by);
+    if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof(O) / sizeof(T); i++) reinterpret_cast<uint4*>(out + p - head)[i] = r[i];
-        } else {
-            for (uint32_t i = 0; i < N; i++)
-                if (p + i >= head && p + i < end) out[p + i - head] = (O)(value(x[p + i - head]) * by);
-        }
+        for (uint32_t i = 0; i < W; i++) reinterpret_cast<uint4*>(out)[i] = r[i];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) out[i] = o[i];
     }
 }
 
-__global__ void __launch_bounds__(kThreads) k_squares(const __grid_constant__ ClipTable a) {
+template <class T, class O>
+__device__ void scaled(const T* x, O* out, uint32_t n, float by) {
+    each(x, n, [&](uint32_t i, const uint4& z) { put<T, O>(out + i, z, by); }, [&](uint32_t i) { out[i] = (O)(value(x[i]) * by); });
+}
+
+__device__ __forceinline__ double piece_squares(const Piece& p) {
+    if (p.t->dtype == DT_F32) return squares(static_cast<const float*>(p.t->grad) + p.from, p.n);
+    if (p.t->dtype == DT_BF16) return squares(static_cast<const __nv_bfloat16*>(p.t->grad) + p.from, p.n);
+    return squares(static_cast<const __half*>(p.t->grad) + p.from, p.n);
+}
+template <class T>
+__device__ __forceinline__ void piece_scaled(const Piece& p, float by) {
+    const T* x = static_cast<const T*>(p.t->grad) + p.from;
+    if (p.t->out_dtype == DT_F32) scaled(x, static_cast<float*>(p.t->out) + p.from, p.n, by);
+    else scaled(x, static_cast<T*>(p.t->out) + p.from, p.n, by);
+}
+
+// What a group is multiplied by, from its sum of squares.
+struct Limit {
+    const float* max_norms;
+    float max_norm;
+    int one_max;
+    __device__ __forceinline__ float factor(uint32_t group, double sum, float* norm) const {
+        const double root = sqrt(sum), most = max_norms ? max_norms[one_max ? 0 : group] : max_norm;
+        *norm = (float)root;
+        return isfinite(*norm) && root > most ? (float)(fmax(most, 0.0) / root) : 1.f;
+    }
+};
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) k_squares(const __grid_constant__ ClipTable<N> a) {
+    release_dependents();
     const uint32_t group = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const ClipEntry& t = entry_of(a, chunk);
-    const uint64_t at = (uint64_t)(chunk - t.chunk0) * kChunk, from = group * t.part + at;
-    const uint32_t n = (uint32_t)min((unsigned long long)kChunk, (unsigned long long)(t.part - at));
-    double v;
-    if (t.dtype == DT_F32) v = squares(static_cast<const float*>(t.grad) + from, n);
-    else if (t.dtype == DT_BF16) v = squares(static_cast<const __nv_bfloat16*>(t.grad) + from, n);
-    else v = squares(static_cast<const __half*>(t.grad) + from, n);
-    v = block_total<kThreads>(v);
+    const double v = block_total<kThreads>(piece_squares(piece_of(a, group, chunk)));
     if (threadIdx.x == 0) a.partial[(uint64_t)group * a.group_chunks + a.at + chunk] = v;
 }
 
 // A group's norm and factor.  One CTA for each group.
-__global__ void __launch_bounds__(1024) k_norms(const double* partial, uint32_t chunks, const float* max_norms, float max_norm, int one_max,
-                                                float* norms, float* factor) {
+__global__ void __launch_bounds__(1024) k_norms(const double* partial, uint32_t chunks, const Limit l, float* norms, float* factor) {
+    release_dependents();
     grid_dependency_wait();
     const double* p = partial + (uint64_t)blockIdx.x * chunks;
     double v = 0.0;
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < chunks; i += 1024) v += p[i];
     v = block_total<1024>(v);
-    if (threadIdx.x) return;
-    const double root = sqrt(v), most = max_norms ? max_norms[one_max ? 0 : blockIdx.x] : max_norm;
-    const float norm = (float)root;
-    norms[blockIdx.x] = norm;
-    factor[blockIdx.x] = isfinite(norm) && root > most ? (float)(fmax(most, 0.0) / root) : 1.f;
+    if (threadIdx.x == 0) factor[blockIdx.x] = l.factor(blockIdx.x, v, norms + blockIdx.x);
 }
 
-__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ ClipTable a) {
+template <int N>
+__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ ClipTable<N> a) {
+    const uint32_t last = gridDim.x - 1 - blockIdx.x, group = last / a.chunks, chunk = last % a.chunks;
+    const Piece p = piece_of(a, group, chunk);
     grid_dependency_wait();
-    const uint32_t group = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const ClipEntry& t = entry_of(a, chunk);
     const float by = a.factor[group];
-    if (by == 1.f && t.grad == t.out) return;
-    const uint64_t at = (uint64_t)(chunk - t.chunk0) * kChunk, from = group * t.part + at;
-    const uint32_t n = (uint32_t)min((unsigned long long)kChunk, (unsigned long long)(t.part - at));
-    if (t.dtype == DT_F32) scaled(static_cast<const float*>(t.grad) + from, static_cast<float*>(t.out) + from, n, by);
-    else if (t.dtype == DT_BF16 && t.out_dtype == DT_BF16)
-        scaled(static_cast<const __nv_bfloat16*>(t.grad) + from, static_cast<__nv_bfloat16*>(t.out) + from, n, by);
-    else if (t.dtype == DT_BF16) scaled(static_cast<const __nv_bfloat16*>(t.grad) + from, static_cast<float*>(t.out) + from, n, by);
-    else if (t.out_dtype == DT_F16) scaled(static_cast<const __half*>(t.grad) + from, static_cast<__half*>(t.out) + from, n, by);
-    else scaled(static_cast<const __half*>(t.grad) + from, static_cast<float*>(t.out) + from, n, by);
+    if (by == 1.f && p.t->grad == p.t->out) return;
+    if (p.t->dtype == DT_F32) piece_scaled<float>(p, by);
+    else if (p.t->dtype == DT_BF16) piece_scaled<__nv_bfloat16>(p, by);
+    else piece_scaled<__half>(p, by);
 }
 
 uint64_t chunks_of(const ClipTensor* t, uint64_t count) {
     uint64_t c = 0;
-    for (uint64_t i = 0; i < count; i++) c += (t[i].part + kChunk - 1) / kChunk;
+    for (uint64_t i = 0; i < count; i++) c += (t[i].part + chunk_elements(t[i].dtype) - 1) / chunk_elements(t[i].dtype);
     return c;
+}
+
+// The launches over the tensors, N to a launch: the squares, or the scaling.
+template <int N>
+cudaError_t passes(const ClipArgs& a, uint64_t chunks, float* factor, bool scale, KScope* ks, cudaStream_t s) {
+    uint64_t at = 0;
+    cudaError_t e = cudaSuccess;
+    for (uint64_t i = 0; i < a.count && e == cudaSuccess;) {
+        ClipTable<N> t;
+        t.count = 0, t.chunks = 0, t.group_chunks = (uint32_t)chunks, t.at = (uint32_t)at, t.partial = a.partial, t.factor = factor;
+        for (; i < a.count && t.count < N; i++) {
+            const ClipTensor& c = a.tensors[i];
+            if (!c.part) continue;
+            t.t[t.count++] = {c.grad, c.out, c.part, t.chunks, (int16_t)c.dtype, (int16_t)c.out_dtype};
+            t.chunks += (uint32_t)((c.part + chunk_elements(c.dtype) - 1) / chunk_elements(c.dtype));
+        }
+        if (!t.count) break;
+        at += t.chunks;
+        const dim3 grid(t.chunks * a.groups);
+        if (scale) {
+            e = launch_dependent(1, k_scale<N>, grid, kThreads, 0, s, t);
+        } else {
+            k_squares<N><<<grid, kThreads, 0, s>>>(t);
+            e = cudaGetLastError();
+        }
+        ks->kernels++;
+    }
+    return e;
 }
 
 }  // namespace
@@ -167,35 +245,14 @@ uint64_t clip_partials(const ClipTensor* t, uint64_t count, uint32_t groups) { r
 
 cudaError_t launch_clip(const ClipArgs& a, cudaStream_t s) {
     const uint64_t chunks = chunks_of(a.tensors, a.count);
-    float* factor = reinterpret_cast<float*>(a.partial + chunks * a.groups);
-    cudaError_t e = cudaSuccess;
+    float* const factor = reinterpret_cast<float*>(a.partial + chunks * a.groups);
+    const Limit l{a.max_norms, a.max_norm, a.one_max};
     KScope ks("clip_gradients", s, 1);
-    for (int pass = 0; pass < 2; pass++) {
-        uint64_t at = 0;
-        for (uint64_t i = 0; i < a.count && e == cudaSuccess;) {
-            ClipTable t{};
-            t.group_chunks = (uint32_t)chunks, t.at = (uint32_t)at, t.partial = a.partial, t.factor = factor;
-            for (; i < a.count && t.count < kTable; i++) {
-                const ClipTensor& c = a.tensors[i];
-                if (!c.part) continue;
-                t.t[t.count++] = {c.grad, c.out, c.part, t.chunks, (int16_t)c.dtype, (int16_t)c.out_dtype};
-                t.chunks += (uint32_t)((c.part + kChunk - 1) / kChunk);
-            }
-            if (!t.count) break;
-            at += t.chunks;
-            const dim3 grid(t.chunks * a.groups);
-            if (pass) {
-                e = launch_dependent(1, k_scale, grid, kThreads, 0, s, t);
-            } else {
-                k_squares<<<grid, kThreads, 0, s>>>(t);
-                e = cudaGetLastError();
-            }
-            ks.kernels++;
-        }
-        if (pass == 0 && e == cudaSuccess)
-            e = launch_dependent(1, k_norms, dim3(a.groups), 1024, 0, s, (const double*)a.partial, (uint32_t)chunks, a.max_norms, a.max_norm,
-                                 a.one_max, a.norms, factor);
-    }
+    const bool few = a.count <= (uint64_t)kMinTable;
+    cudaError_t e = few ? passes<kMinTable>(a, chunks, factor, false, &ks, s) : passes<kMaxTable>(a, chunks, factor, false, &ks, s);
+    if (e == cudaSuccess)
+        e = launch_dependent(1, k_norms, dim3(a.groups), 1024, 0, s, (const double*)a.partial, (uint32_t)chunks, l, a.norms, factor);
+    if (e == cudaSuccess) e = few ? passes<kMinTable>(a, chunks, factor, true, &ks, s) : passes<kMaxTable>(a, chunks, factor, true, &ks, s);
     return e;
 }
 

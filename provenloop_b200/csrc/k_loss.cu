@@ -10,31 +10,36 @@
 //
 // The bound is the logits' traffic: each is read once, and its gradient
 // written once.
+#include <atomic>
+#include <cfloat>
+
 #include "../../include/tsgpu.h"
 #include "launch.cuh"
 #include "sm100.cuh"
 #include "train.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace tsg {
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// What k_rows does with a row: its log-probability; the gradient for a given
-// g; the policy loss's g; the gradient for known statistics and a g by sequence.
-enum RowMode : int { LOGPROBS, GIVEN, POLICY, KNOWN };
+
+// What is done with a row that counts: its log-probability; the gradient for
+// a given g; the policy loss; the gradient for known statistics and a g by sequence.
+enum Mode : int { LOGPROBS, GIVEN, POLICY, KNOWN };
 
 struct RowArgs {
     LossRows r;
     PolicyTerms p;
     LossWork w;
     LossOut o;
-    const float* g;   // GIVEN: [n]
+    const float* g;  // GIVEN: [n]
+    int mode;
+    int backwards;   // the last rows first
+    int wait;        // the launch before this one has to be waited for
+    int units;       // clusters (k_ring) or rows (k_short)
 };
 
 __device__ __forceinline__ float exp2_fast(float v) {
@@ -118,41 +123,194 @@ struct Lane<__half> {
     static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// exp(a - b) for a <= b, 1 where they are the same infinity.
-__device__ __forceinline__ float weight(float a, float b) { return a == b ? 1.f : exp2_fast((a - b) * kLog2e); }
-
-// Statistics of two parts of a row as one.  A NaN is in the sum.
-__device__ __forceinline__ RowStats join(const RowStats& a, const RowStats& b) {
-    const float m = fmaxf(a.max, b.max);
-    return {m, a.sum * weight(a.max, m) + b.sum * weight(b.max, m)};
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+// exp(a - b) for a <= b, 1 where they are equal.
+__device__ __forceinline__ float weight(float a, float b) { return exp2_fast((a - b) * kLog2e); }
+__device__ __forceinline__ float2 weight2(float2 a, float2 less) {
+    const float2 d = mul2(add2(a, less), make_float2(kLog2e, kLog2e));
+    return make_float2(exp2_fast(d.x), exp2_fast(d.y));
 }
 
-// l = log-probability of a row's target with logit z, in 64 bits: the row's
-// one value that all of its gradient hangs on.
+// Of a warp's lanes, the same bits in all of them.
+__device__ __forceinline__ RowStats join_lanes(const RowStats& s) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(s.max));
+    float sum = s.sum * weight(s.max, m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return {m, sum};
+}
+// Of no elements, or of such as are -inf; differences of finite maxima are never NaN.
+__device__ __forceinline__ RowStats nothing() { return {-FLT_MAX, 0.f}; }
+
+// Adds four vectors to a thread's statistics.
+template <class T>
+__device__ __forceinline__ void see4(RowStats& t, const uint4 (&z)[4]) {
+    constexpr int N = Lane<T>::N;
+    const float m = fmaxf(t.max, fmaxf(fmaxf(Lane<T>::top(z[0]), Lane<T>::top(z[1])), fmaxf(Lane<T>::top(z[2]), Lane<T>::top(z[3]))));
+    const float2 less = make_float2(-m, -m);
+    float2 sum[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float f[N];
+        Lane<T>::open(z[j], f);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) sum[j] = add2(sum[j], weight2(make_float2(f[i], f[i + 1]), less));
+    }
+    const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+    t.sum = fmaf(t.sum, weight(t.max, m), all.x + all.y), t.max = m;
+}
+
+struct Coef {
+    float g, by, zy, max;
+};
+template <class T>
+__device__ __forceinline__ uint4 slope_of(const uint4& z, const Coef& c) {
+    constexpr int N = Lane<T>::N;
+    const float2 less = make_float2(-c.max, -c.max), by = make_float2(c.by, c.by);
+    float f[N];
+    Lane<T>::open(z, f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 p = mul2(weight2(make_float2(f[i], f[i + 1]), less), by);
+        f[i] = p.x, f[i + 1] = p.y;
+    }
+    return Lane<T>::close(f);
+}
+template <class T>
+__device__ __forceinline__ void fix_target(T* out, const Coef& c) {
+    *out = Lane<T>::put(fmaf(c.by, weight(c.zy, c.max), c.g));
+}
+
+// log s: the exponent's part in 64 bits, so that what is left has an error of 2^-24.
+__device__ __forceinline__ double log_of(float s) {
+    if (!(s >= 0.5f && s < INFINITY)) return log((double)s);
+    const uint32_t u = __float_as_uint(s), up = (u & 0x7fffffu) > 0x400000u;  // mantissa above 1.5: halved
+    return (double)((int)(u >> 23) - 127 + (int)up) * 0.69314718055994531 + (double)logf(__uint_as_float((u & 0x7fffffu) | (up ? 0x3f000000u : 0x3f800000u)));
+}
+
+// The log-probability of a row's target with logit z: the one value that all
+// of the row's gradient hangs on.
 __device__ __forceinline__ double logprob(float z, const RowStats& s) {
-    return z == -INFINITY ? (double)-INFINITY : ((double)z - (double)s.max) - log((double)s.sum);
+    return z == -INFINITY ? (double)-INFINITY : ((double)z - (double)s.max) - log_of(s.sum);
 }
 
-// The policy loss's term of a row and its derivative by l, without the row's weight.
-__device__ __forceinline__ double policy_term(const PolicyTerms& p, long long row, double l, double a, double* slope) {
-    const double rho = p.old ? exp(l - (double)p.old[row]) : l == l ? 1.0 : l, cut = rho < p.low ? (double)p.low : rho > p.high ? (double)p.high : rho;
-    const double whole = rho * a, held = cut * a;
+// What finishes a row, loaded before its statistics are there.
+struct RowInfo {
+    float zy, old, ref, a;  // a: advantage (POLICY), g (GIVEN, KNOWN)
+    RowStats s;             // KNOWN
+    double share, scaled;   // of the row in the policy loss, and in its gradient
+};
+
+__device__ __forceinline__ RowInfo row_info(const RowArgs& a, long long row, float zy) {
+    RowInfo i{zy, 0.f, 0.f, 0.f, {0.f, 1.f}, 0.0, 0.0};
+    if (a.mode == GIVEN) i.a = a.g[row];
+    if (a.mode == KNOWN) {
+        i.a = a.w.slope[a.r.sequence(row)];
+        i.s = a.w.stats[row];
+    }
+    if (a.mode == POLICY) {
+        const int q = a.r.sequence(row), kind = a.p.kind;
+        i.a = a.p.advantages[a.p.advantage_rows ? row : q];
+        if (a.p.old) i.old = a.p.old[row];
+        if (a.p.ref) i.ref = a.p.ref[row];
+        i.share = kind == TS_REDUCE_TOKEN ? 1.0 / a.w.counts[a.r.sequences] : kind == TS_REDUCE_SEQUENCE ? 1.0 / ((double)a.w.counts[q] * a.r.sequences) : 1.0;
+        i.scaled = i.share * (a.o.grad_scale ? (double)*a.o.grad_scale : 1.0);
+    }
+    return i;
+}
+
+// The policy loss's term of a row, and its derivative by l.
+__device__ __forceinline__ double policy_term(const PolicyTerms& p, const RowInfo& i, double l, double* slope) {
+    const double rho = p.old ? (double)expf((float)(l - (double)i.old)) : l == l ? 1.0 : l;
+    const double cut = rho < p.low ? (double)p.low : rho > p.high ? (double)p.high : rho, whole = rho * i.a, held = cut * i.a;
     const bool clipped = whole > held;  // not where one is a NaN
     double term = clipped ? -held : -whole, by = clipped ? 0.0 : -whole;
     if (p.ref && p.kl != 0.f) {
-        const double d = (double)p.ref[row] - l, e = expm1(d);
-        // exp(d) - 1 - d, by its series where that cancels (rest below 2^-50 of it)
-        const double k = fabs(d) < 1e-3 ? d * d * (0.5 + d * (1.0 / 6 + d * (1.0 / 24 + d * (1.0 / 120 + d / 720)))) : e - d;
-        term += p.kl * k;
+        // exp(d) - 1 - d: by its series where that cancels (what is left out is below 2^-40 of it)
+        const double d = (double)i.ref - l, e = (double)expm1f((float)d);
+        const double series = d * d * (1.0 / 2 + d * (1.0 / 6 + d * (1.0 / 24 + d * (1.0 / 120 + d * (1.0 / 720 + d * (1.0 / 5040 + d * (1.0 / 40320 + d / 362880)))))));
+        term += p.kl * (fabs(d) < 0.25 ? series : e - d);
         by -= p.kl * e;
     }
     *slope = by;
     return term;
 }
 
-// The share of a row of sequence q in the policy loss.
-__device__ __forceinline__ double policy_weight(int kind, const int* counts, uint32_t sequences, int q) {
-    return kind == TS_REDUCE_TOKEN ? 1.0 / counts[sequences] : kind == TS_REDUCE_SEQUENCE ? 1.0 / ((double)counts[q] * sequences) : 1.0;
+// A row's results but its gradient, written where `write` is set; returns
+// what the gradient needs and adds to the loss.
+__device__ __forceinline__ Coef finish_row(const RowArgs& a, const RowInfo& i, long long row, const RowStats& s, bool write, double* loss) {
+    float g = i.a;
+    if (a.mode == LOGPROBS || a.mode == POLICY) {
+        const double l = logprob(i.zy, s);
+        if (write) {
+            if (a.o.logprobs) a.o.logprobs[row] = (float)l;
+            if (a.mode == LOGPROBS && a.w.stats) a.w.stats[row] = s, a.w.logs[row] = l;
+        }
+        if (a.mode == POLICY) {
+            double slope;
+            *loss += i.share * policy_term(a.p, i, l, &slope);
+            g = (float)(i.scaled * slope);
+        }
+    }
+    return {g, -__fdiv_rn(g, s.sum), i.zy, s.max};
+}
+
+// The same for a row that does not count.
+__device__ __forceinline__ void skip_row(const RowArgs& a, long long row) {
+    if ((a.mode == LOGPROBS || a.mode == POLICY) && a.o.logprobs) a.o.logprobs[row] = 0.f;
+}
+
+// The loss from its parts in the order of their numbers, by the last warp to
+// get here; the parts are there.
+__device__ __forceinline__ void total(const LossWork& w, int parts, double by, float* out) {
+    const int lane = (int)(threadIdx.x & 31);
+    unsigned before = 0;
+    __syncwarp();
+    if (lane == 0) {
+        __threadfence();
+        before = atomicAdd(w.ticket, 1u);
+    }
+    if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)parts - 1) return;
+    __threadfence();
+    double v = 0.0;
+    for (int i = lane; i < parts; i += 32) v += __ldcg(w.parts + i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) *out = (float)(v * by);
+}
+
+// The vector at p of a row (addressed as Span says) by its elements: -inf for
+// what lies outside of [head, last).  Out of line, and by values: rows have two of them.
+template <class T>
+__device__ __noinline__ uint4 load_edge(const T* x, uint32_t head, uint32_t last, uint32_t p) {
+    uint4 z = make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow);
+    T* e = reinterpret_cast<T*>(&z);
+#pragma unroll
+    for (uint32_t i = 0; i < Lane<T>::N; i++)
+        if (p + i >= head && p + i < last) e[i] = x[p + i - head];
+    return z;
+}
+template <class T>
+__device__ __noinline__ void store_edge(T* out, uint32_t head, uint32_t last, uint32_t p, uint4 z) {
+    const T* e = reinterpret_cast<const T*>(&z);
+#pragma unroll
+    for (uint32_t i = 0; i < Lane<T>::N; i++)
+        if (p + i >= head && p + i < last) out[p + i - head] = e[i];
 }
 
 // A CTA's part [first, last) of a row whose elements are addressed by
@@ -166,167 +324,409 @@ struct Span {
         const uint32_t end = head + vocab, span = ((end + cl - 1) / cl + 127) / 128 * 128;
         first = min(end, rank * span), last = min(end, first + span);
     }
-    // The vector at p < last; -inf for what lies outside.
-    __device__ __forceinline__ uint4 load(uint32_t p) const {
-        constexpr uint32_t N = Lane<T>::N;
-        if (p >= head && p + N <= last) return *reinterpret_cast<const uint4*>(x + p - head);
-        uint4 z = make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow);
-        T* e = reinterpret_cast<T*>(&z);
-#pragma unroll
-        for (uint32_t i = 0; i < N; i++)
-            if (p + i >= head && p + i < last) e[i] = x[p + i - head];
-        return z;
-    }
-    __device__ __forceinline__ void store(T* out, bool whole, uint32_t p, const uint4& z) const {
-        constexpr uint32_t N = Lane<T>::N;
-        if (whole && p >= head && p + N <= last) {
-            *reinterpret_cast<uint4*>(out + p - head) = z;
-            return;
-        }
-        const T* e = reinterpret_cast<const T*>(&z);
-#pragma unroll
-        for (uint32_t i = 0; i < N; i++)
-            if (p + i >= head && p + i < last) out[p + i - head] = e[i];
+    __device__ __forceinline__ bool whole(uint32_t p) const { return p >= head && p + Lane<T>::N <= last; }
+    __device__ __forceinline__ uint4 edge(uint32_t p) const { return load_edge(x, head, last, p); }
+    __device__ __forceinline__ void store(T* out, bool vec, uint32_t p, const uint4& z) const {
+        if (vec && whole(p)) *reinterpret_cast<uint4*>(out + p - head) = z;
+        else store_edge(out, head, last, p, z);
     }
 };
 
-template <class T>
-__device__ RowStats span_stats(const Span<T>& sp) {
-    constexpr uint32_t N = Lane<T>::N, kStep = kThreads * N;
-    RowStats t{-INFINITY, 0.f};
-    for (uint32_t p = sp.first + threadIdx.x * N; p < sp.last; p += 4 * kStep) {
-        uint4 z[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-            z[j] = p + j * kStep < sp.last ? sp.load(p + j * kStep) : make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow);
-        const float m = fmaxf(fmaxf(Lane<T>::top(z[0]), Lane<T>::top(z[1])), fmaxf(Lane<T>::top(z[2]), Lane<T>::top(z[3])));
-        if (m > t.max) t.sum *= weight(t.max, m), t.max = m;
-        const float from = t.max == -INFINITY ? 0.f : t.max;
-        float sum[4] = {};
+// The target of a row that counts, else -1.
+__device__ __forceinline__ int counted(const RowArgs& a, long long row, long long lo, long long hi) {
+    if (row < lo || row >= hi) return -1;
+    const int y = a.r.target(row);
+    return y >= 0 && a.mode == GIVEN && a.g[row] == 0.f ? -1 : y;
+}
+__device__ __forceinline__ long long rows_from(const LossRows& r) { return r.starts ? max(0ll, (long long)r.starts[0]) : 0ll; }
+__device__ __forceinline__ long long rows_to(const LossRows& r) { return r.starts ? min(r.n, (long long)r.starts[r.sequences]) : r.n; }
+
+// Rows that a CTA holds in registers, four vectors a thread.
+template <class T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
+    constexpr uint32_t N = Lane<T>::N, W = THREADS / 32;
+    __shared__ RowStats warp_stats[W];
+    __shared__ float shared_coef[sizeof(Coef) / 4];
+    const long long row = blockIdx.x;
+    const int y = counted(a, row, rows_from(a.r), rows_to(a.r)), lane = (int)(threadIdx.x & 31);
+    const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, 0, 1);
+    T* const out = a.o.grad ? static_cast<T*>(a.o.grad) + row * a.o.grad_stride : nullptr;
+    const bool vec = out && reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
+    uint4 z[4];
+    Coef c{0.f, 0.f, 0.f, 0.f};
+    if (y >= 0) {
+        const float zy = Lane<T>::one(sp.x[y]);  // before the row may be written
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-            float f[N];
-            Lane<T>::open(z[j], f);
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) sum[j] += exp2_fast((f[i] - from) * kLog2e);
+            const uint32_t p = (threadIdx.x + j * THREADS) * N;
+            z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
+                   : sp.whole(p) ? *reinterpret_cast<const uint4*>(sp.x + p - sp.head) : sp.edge(p);
         }
-        t.sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    }
-    return t;
-}
-
-template <class T, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) k_rows(const RowArgs a) {
-    constexpr uint32_t N = Lane<T>::N, kStep = kThreads * N;
-    __shared__ RowStats warp_stats[kThreads / 32], cta_stats[kCluster];
-    __shared__ float coef[2];  // g and -g / s
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster_arrive();
-    const int rank = (int)cluster.block_rank(), cl = (int)cluster.num_blocks();
-    const long long row = blockIdx.x / cl;
-    const T* x = static_cast<const T*>(a.r.logits) + row * a.r.stride;
-    const Span<T> sp(x, a.r.vocab, rank, cl);
-    T* out = a.o.grad ? static_cast<T*>(a.o.grad) + row * a.o.grad_stride : nullptr;
-    const bool out_vec = out && reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(x) % 16;
-
-    if (MODE == POLICY) grid_dependency_wait();
-    int y = a.r.target(row), q = -1;
-    if (MODE == POLICY) {
-        q = a.w.sequence[row];
-        if (q < 0) y = -1;
-    } else if (y >= 0 && (a.r.starts || MODE == KNOWN)) {
-        q = a.r.sequence(row);
-        if (q < 0) y = -1;
-    }
-    const float zy = y >= 0 ? Lane<T>::one(x[y]) : 0.f;
-    float g = 0.f;
-    RowStats s{0.f, 1.f};
-    if (MODE == GIVEN && y >= 0) g = a.g[row];
-    if (MODE == KNOWN) {
-        grid_dependency_wait();
-        if (y >= 0) g = a.w.slope[q], s = a.w.stats[row];
-    }
-    if (MODE != KNOWN && y >= 0 && (MODE != GIVEN || g != 0.f)) {
-        s = span_stats<T>(sp);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) s = join(s, {__shfl_xor_sync(0xffffffffu, s.max, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
-        if ((threadIdx.x & 31) == 0) warp_stats[threadIdx.x >> 5] = s;
+        RowStats s = nothing();
+        if (a.mode != KNOWN) {
+            see4<T>(s, z);
+            s = join_lanes(s);
+            if (lane == 0) warp_stats[threadIdx.x >> 5] = s;
+        }
         __syncthreads();
         if (threadIdx.x < 32) {
-            s = threadIdx.x < kThreads / 32 ? warp_stats[threadIdx.x] : RowStats{-INFINITY, 0.f};
-#pragma unroll
-            for (int o = kThreads / 64; o; o >>= 1) s = join(s, {__shfl_xor_sync(0xffffffffu, s.max, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
-            s = {__shfl_sync(0xffffffffu, s.max, 0), __shfl_sync(0xffffffffu, s.sum, 0)};  // the same bits for every CTA
-        }
-        cluster_wait();  // the other CTAs have started
-        if (threadIdx.x < cl) *cluster.map_shared_rank(&cta_stats[rank], (int)threadIdx.x) = s;
-        cluster.sync();
-        s = cta_stats[0];
-        for (int i = 1; i < cl; i++) s = join(s, cta_stats[i]);
-    } else {
-        cluster_wait();
-    }
-    if (MODE == LOGPROBS || MODE == POLICY) {
-        if (threadIdx.x == 0) {
-            const double l = y >= 0 ? logprob(zy, s) : 0.0;
-            double part = 0.0, slope = 0.0;
-            if (MODE == POLICY && y >= 0) {
-                const double wt = policy_weight(a.p.kind, a.w.counts, a.r.sequences, q);
-                part = wt * policy_term(a.p, row, l, a.p.advantages[a.p.advantage_rows ? row : q], &slope);
-                slope *= wt;
-            }
-            if (rank == 0) {
-                if (a.o.logprobs) a.o.logprobs[row] = (float)l;
-                if (MODE == LOGPROBS && a.w.stats) a.w.stats[row] = s;
-                if (MODE == POLICY) a.w.parts[row] = part;
-            }
-            if (MODE == POLICY && out) {
-                g = (float)(slope * (a.o.grad_scale ? *a.o.grad_scale : 1.f));
-                coef[0] = g;
+            if (a.wait) grid_dependency_wait();
+            const RowInfo i = row_info(a, row, zy);
+            s = a.mode == KNOWN ? i.s : join_lanes(lane < W ? warp_stats[lane] : nothing());
+            double loss = 0.0;
+            c = finish_row(a, i, row, s, lane == 0, &loss);
+            if (lane == 0) {
+                *reinterpret_cast<Coef*>(shared_coef) = c;
+                if (a.mode == POLICY) a.w.parts[row] = loss;
             }
         }
-        if (!out) return;
         __syncthreads();
-        g = coef[0];
-    }
-    if (MODE == LOGPROBS) return;
-    if (g == 0.f) {  // not for a NaN
-        for (uint32_t p = sp.first + threadIdx.x * N; p < sp.last; p += kStep) sp.store(out, out_vec, p, make_uint4(0, 0, 0, 0));
-        return;
-    }
-    const float c = -__fdiv_rn(g, s.sum), from = s.max == -INFINITY ? 0.f : s.max;
-    for (uint32_t p = sp.first + threadIdx.x * N; p < sp.last; p += 4 * kStep) {
-        uint4 z[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-            if (p + j * kStep < sp.last) z[j] = sp.load(p + j * kStep);
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            const uint32_t at = p + j * kStep;
-            if (at >= sp.last) break;
-            float f[N];
-            Lane<T>::open(z[j], f);
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) f[i] = c * exp2_fast((f[i] - from) * kLog2e);
-            const uint32_t k = (uint32_t)y + sp.head - at;
-            if (k < N) {
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++) f[i] += i == k ? g : 0.f;
-            }
-            sp.store(out, out_vec, at, Lane<T>::close(f));
+        c = *reinterpret_cast<const Coef*>(shared_coef);
+    } else if (threadIdx.x < 32) {
+        if (a.wait) grid_dependency_wait();
+        if (lane == 0) {
+            skip_row(a, row);
+            if (a.mode == POLICY) a.w.parts[row] = 0.0;
         }
+    }
+    if (a.mode == LOGPROBS && a.w.ticket && row == 0 && threadIdx.x == 0) *a.w.ticket = 0u;
+    if (a.mode == POLICY && threadIdx.x < 32) total(a.w, a.units, 1.0, a.o.loss);
+    if (!out) return;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t p = (threadIdx.x + j * THREADS) * N;
+        if (p >= sp.last) continue;
+        sp.store(out, vec, p, c.g == 0.f ? make_uint4(0u, 0u, 0u, 0u) : slope_of<T>(z[j], c));
+        if (c.g != 0.f && (uint32_t)y + sp.head - p < N) fix_target(out + y, c);
     }
 }
 
-// Rows that count: the sequence of each, how many each sequence has, and how
-// many there are.  One CTA.
+// Longer rows: persistent clusters, each with every so many-th row, a CTA with
+// its part of it in slots of a ring in shared memory.  Warps have roles:
+//   one starts the copies into the slots,
+//   S warps take the statistics of a part as it arrives,
+//   one joins them, exchanges them within the cluster and finishes the row,
+//   G warps write the part's gradient once that is known.
+// A part keeps `keep` slots until its gradient is written from them; what there is
+// more of it is copied once more (from L2) behind the rest and before the next
+// row, whose statistics are taken meanwhile.  So a row comes from memory once.
+constexpr uint32_t kSlot = 16384;
+constexpr uint32_t kZeros = 4096;
+constexpr int kTeam = 8;   // warps that take a slot together, four vectors a lane
+constexpr int kDepth = 4;  // rows between two roles
+// The teams of a role take the slots in turn, and every team always the same
+// ones: it has seen a slot's last load when it waits for the next, and a parity
+// wait tells the two apart.  Statistics alone: two CTAs on an SM (4096 rows of
+// 151936 in bf16: 197 us, with one of twice the slots 211).
+template <bool S, bool G>
+struct Roles {
+    static constexpr int TS = !S ? 0 : G ? 1 : 2, TG = G ? 2 : 0, CTAS = G ? 1 : 2, SLOTS = G ? 12 : 6;
+    static constexpr int KEEP = 8;  // of them; the rest is for the next row while one waits for its gradient
+    static constexpr int THREADS = 64 + (TS + TG) * kTeam * 32;
+    static constexpr size_t SMEM = SLOTS * kSlot + (G ? kZeros : 0);
+    static_assert((!S || SLOTS % TS == 0) && (!G || SLOTS % TG == 0), "a slot's team must not change");
+};
+
+struct RingShared {
+    uint64_t full[12], empty[12], stats_full[kDepth], stats_free[kDepth], joined[kDepth], coef_full[kDepth], coef_free[kDepth];
+    RowStats warp_stats[kDepth][2 * kTeam], cta_stats[kDepth][kCluster];
+    float coef[kDepth][sizeof(Coef) / 4];
+    uint32_t dead;
+};
+
+// mbar_wait with short sleeps between two looks: warps that wait would take
+// issue slots from those that compute (550 and 530 us for the gradient of 4096 rows of 151936).
+__device__ __forceinline__ bool sleep_wait(uint64_t* b, uint32_t parity, uint32_t* dead) {
+    if (mbar_try(b, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(b, parity)) {
+        __nanosleep(20);
+        if (*reinterpret_cast<volatile uint32_t*>(dead)) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            atomicAdd(&g_expired_waits, 1ull);
+            atomicExch(dead, 1u);
+            return false;
+        }
+    }
+    return true;
+}
+// A wait of a whole warp, whose lanes go on or give up together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* dead) {
+    return __all_sync(0xffffffffu, sleep_wait(bar, parity, dead));
+}
+
+// The next 32 of a cluster's rows, one a lane.
+struct Batch {
+    long long row;
+    int y;
+    uint32_t rows, counts;  // lanes that have a row; whose row counts
+    __device__ __forceinline__ Batch(const RowArgs& a, long long b, long long lo, long long hi, int cluster) {
+        const long long i = (b * 32 + (threadIdx.x & 31)) * a.units + cluster;
+        const bool there = i < a.r.n;
+        row = a.backwards ? a.r.n - 1 - i : i;
+        y = there ? counted(a, row, lo, hi) : -1;
+        rows = __ballot_sync(0xffffffffu, there), counts = __ballot_sync(0xffffffffu, y >= 0);
+    }
+    __device__ __forceinline__ long long row_of(int lane) const { return __shfl_sync(0xffffffffu, row, lane); }
+};
+
+template <class T, bool S, bool G>
+__global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_ring(const RowArgs a) {
+    constexpr uint32_t N = Lane<T>::N, SLOT = kSlot / sizeof(T);
+    constexpr int TS = Roles<S, G>::TS, TG = Roles<S, G>::TG, SLOTS = Roles<S, G>::SLOTS, KEEP = Roles<S, G>::KEEP;
+    constexpr uint32_t STEP = 32 * N, GROUPS = SLOT / (kTeam * 4 * STEP);  // a lane takes that often four vectors of a slot
+    extern __shared__ __align__(128) unsigned char slots[];
+    __shared__ RingShared sh;
+    const int rank = (int)cluster_rank(), warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
+    const int cl = (int)(gridDim.x / (unsigned)a.units), cluster = (int)(blockIdx.x / (unsigned)cl);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SLOTS; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kTeam);
+        for (int i = 0; i < kDepth; i++) {
+            mbar_init(&sh.stats_full[i], TS * kTeam), mbar_init(&sh.stats_free[i], 1), mbar_init(&sh.joined[i], 1);
+            mbar_init(&sh.coef_full[i], 1), mbar_init(&sh.coef_free[i], TG * kTeam);
+        }
+        sh.dead = 0;
+        mbar_init_fence();
+        if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) *a.w.ticket = 0u;
+    }
+    if (G && threadIdx.x < kZeros / 16) {
+        reinterpret_cast<uint4*>(slots + SLOTS * kSlot)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_shared();
+    }
+    __syncthreads();
+    cluster_arrive();  // waited for before the first access to another CTA's shared memory
+    const long long lo = rows_from(a.r), hi = rows_to(a.r);
+    const auto span_of = [&](long long row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, cl); };
+    const auto chunks_of = [](const Span<T>& sp) { return (int)((sp.last - sp.first + SLOT - 1) / SLOT); };
+    T* const data = reinterpret_cast<T*>(slots);
+    T* const zeros = data + SLOTS * SLOT;  // kZeros bytes of them
+    const auto again_of = [&](int n) { return S && G ? max(0, n - KEEP) : 0; };  // slots that are released after the statistics
+    bool ok = true;
+
+    if (warp == 0) {
+        Ring at(SLOTS, 1);
+        for (long long b = 0; ok; b++) {
+            const Batch rows(a, b, lo, hi, cluster);
+            if (!rows.rows) break;
+            for (uint32_t left = rows.counts; left && ok; left &= left - 1) {
+                const Span<T> sp = span_of(rows.row_of(__ffs(left) - 1));
+                const int n = chunks_of(sp), loads = n + again_of(n);
+                for (int c = 0; c < loads && ok; c++, at.next()) {
+                    if (lane) continue;
+                    const uint32_t p0 = sp.first + (c < n ? c : c - n) * SLOT, p1 = min(sp.last, p0 + SLOT);
+                    const uint32_t from = p0 < sp.head ? p0 + N : p0, to = p1 / N * N;
+                    const uint32_t bytes = to > from ? (to - from) * (uint32_t)sizeof(T) : 0u;
+                    ok = sleep_wait(&sh.empty[at.i], at.phase, &sh.dead);
+                    if (!ok) break;
+                    mbar_expect(&sh.full[at.i], bytes);
+                    if (bytes) bulk_copy(smem_u32(data + at.i * SLOT + (from - p0)), sp.x + from - sp.head, bytes, &sh.full[at.i]);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+        }
+        if (!ok) settle();
+    } else if (warp == 1) {
+        Ring k(kDepth, 0);
+        double loss = 0.0;
+        bool met = false;
+        if (a.wait) grid_dependency_wait();
+        for (long long b = 0; ok; b++) {
+            const Batch rows(a, b, lo, hi, cluster);
+            if (!rows.rows) break;
+            RowInfo mine{};
+            if (rows.y >= 0) mine = row_info(a, rows.row, Lane<T>::one((static_cast<const T*>(a.r.logits) + rows.row * a.r.stride)[rows.y]));
+            else if ((rows.rows >> lane & 1) && rank == 0) skip_row(a, rows.row);
+            for (uint32_t left = rows.counts; left && ok; left &= left - 1, k.next()) {
+                const int from = __ffs(left) - 1;
+                RowInfo i;
+                i.zy = __shfl_sync(0xffffffffu, mine.zy, from), i.old = __shfl_sync(0xffffffffu, mine.old, from);
+                i.ref = __shfl_sync(0xffffffffu, mine.ref, from), i.a = __shfl_sync(0xffffffffu, mine.a, from);
+                i.share = __shfl_sync(0xffffffffu, mine.share, from), i.scaled = __shfl_sync(0xffffffffu, mine.scaled, from);
+                RowStats s{__shfl_sync(0xffffffffu, mine.s.max, from), __shfl_sync(0xffffffffu, mine.s.sum, from)};
+                if (S) {
+                    ok = warp_wait(&sh.stats_full[k.i], k.phase, &sh.dead);
+                    if (!ok) break;
+                    s = join_lanes(lane < TS * kTeam ? sh.warp_stats[k.i][lane] : nothing());
+                    if (lane == 0) mbar_arrive(&sh.stats_free[k.i]);
+                    if (cl > 1) {
+                        if (!met) cluster_wait(), met = true;
+                        if (lane == 0) mbar_expect(&sh.joined[k.i], (uint32_t)cl * sizeof(RowStats));
+                        if (lane < cl)
+                            asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+                                             map_rank(&sh.cta_stats[k.i][rank], (uint32_t)lane)),
+                                         "f"(s.max), "f"(s.sum), "r"(map_rank(&sh.joined[k.i], (uint32_t)lane))
+                                         : "memory");
+                        ok = warp_wait(&sh.joined[k.i], k.phase, &sh.dead);
+                        if (!ok) break;
+                        s = join_lanes(lane < cl ? sh.cta_stats[k.i][lane] : nothing());
+                    }
+                }
+                const Coef c = finish_row(a, i, rows.row_of(from), s, rank == 0 && lane == 0, &loss);
+                if (G) {
+                    ok = warp_wait(&sh.coef_free[k.i], k.phase ^ 1, &sh.dead);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        *reinterpret_cast<Coef*>(sh.coef[k.i]) = c;
+                        mbar_arrive(&sh.coef_full[k.i]);
+                    }
+                }
+            }
+        }
+        if (a.mode == POLICY && rank == 0 && ok) {
+            if (lane == 0) a.w.parts[cluster] = loss;
+            total(a.w, a.units, 1.0, a.o.loss);
+        }
+        if (!met) cluster_wait();
+    } else if (S && (!G || warp < 2 + TS * kTeam)) {
+        const int w = (warp - 2) % kTeam, team = (warp - 2) / kTeam;
+        const uint32_t v0 = (uint32_t)w * GROUPS * 4 * STEP + lane * N;  // this lane's first vector of a slot
+        Ring at(SLOTS, 0), k(kDepth, 0);
+        for (long long b = 0; ok; b++) {
+            const Batch rows(a, b, lo, hi, cluster);
+            if (!rows.rows) break;
+            for (uint32_t left = rows.counts; left && ok; left &= left - 1, k.next()) {
+                const Span<T> sp = span_of(rows.row_of(__ffs(left) - 1));
+                const int n = chunks_of(sp), again = again_of(n);
+                RowStats t = nothing();
+                for (int c = 0; c < n; c++, at.next()) {
+                    if (at.i % TS != team) continue;
+                    ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
+                    if (!ok) break;
+                    const T* const from = data + at.i * SLOT + v0;
+                    const uint32_t p0 = sp.first + c * SLOT + v0;
+                    const bool inside = sp.first + c * SLOT >= sp.head && sp.first + (c + 1) * SLOT <= sp.last;
+#pragma unroll
+                    for (uint32_t q = 0; q < GROUPS; q++) {
+                        uint4 z[4];
+                        if (inside) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) z[j] = *reinterpret_cast<const uint4*>(from + (q * 4 + j) * STEP);
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) {
+                                const uint32_t p = p0 + (q * 4 + j) * STEP;
+                                z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
+                                       : sp.whole(p) ? *reinterpret_cast<const uint4*>(from + (q * 4 + j) * STEP) : sp.edge(p);
+                            }
+                        }
+                        if (q == GROUPS - 1 && (!G || c < again)) {
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh.empty[at.i]);
+                        }
+                        see4<T>(t, z);
+                    }
+                }
+                t = join_lanes(t);
+                ok = ok && warp_wait(&sh.stats_free[k.i], k.phase ^ 1, &sh.dead);
+                if (lane == 0 && ok) {
+                    sh.warp_stats[k.i][warp - 2] = t;
+                    mbar_arrive(&sh.stats_full[k.i]);
+                }
+                // what arrives once more is not for this role, but it has to be seen
+                for (int c = 0; c < again && ok; c++, at.next())
+                    if (at.i % TS == team) ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
+            }
+        }
+    } else {
+        constexpr int first = 2 + TS * kTeam;
+        constexpr uint32_t PIECE = GROUPS * 4 * STEP;  // elements of a slot that a warp takes
+        const int w = (warp - first) % kTeam, team = (warp - first) / kTeam;
+        Ring at(SLOTS, 0), k(kDepth, 0);
+        for (long long b = 0; ok; b++) {
+            const Batch rows(a, b, lo, hi, cluster);
+            if (!rows.rows) break;
+            for (uint32_t left = rows.rows; left && ok; left &= left - 1) {
+                const int of = __ffs(left) - 1;
+                const long long row = rows.row_of(of);
+                const Span<T> sp = span_of(row);
+                T* const out = static_cast<T*>(a.o.grad) + row * a.o.grad_stride;
+                const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
+                if (!(rows.counts >> of & 1)) {
+                    if (vec) {
+                        // whole vectors by bulk stores of zeros, the row's ends by elements
+                        const uint32_t from = sp.first < sp.head ? N : sp.first, to = sp.last / N * N;
+                        if (lane == 0) {
+                            for (uint32_t p = from + (uint32_t)(warp - first) * (kZeros / sizeof(T)); p < to; p += TG * kTeam * (kZeros / sizeof(T)))
+                                bulk_store(out + p - sp.head, smem_u32(zeros), min(to - p, (uint32_t)(kZeros / sizeof(T))) * sizeof(T));
+                            bulk_commit();
+                        }
+                        if (warp == first && sp.first < sp.last) {
+                            const uint32_t p = lane < (int)N ? sp.first + lane : max(to, from) + lane - N;
+                            if (lane < 2 * (int)N && p >= sp.head && p < sp.last && (lane < (int)N ? p < from : true)) out[p - sp.head] = Lane<T>::put(0.f);
+                        }
+                    } else {
+                        for (uint32_t p = sp.first + (uint32_t)(warp - first) * STEP + lane * N; p < sp.last; p += TG * kTeam * STEP)
+                            store_edge(out, sp.head, sp.last, p, make_uint4(0u, 0u, 0u, 0u));
+                    }
+                    continue;
+                }
+                const uint32_t y = (uint32_t)__shfl_sync(0xffffffffu, rows.y, of);
+                const int n = chunks_of(sp), again = again_of(n);
+                at.skip(again);
+                ok = warp_wait(&sh.coef_full[k.i], k.phase, &sh.dead);
+                if (!ok) break;
+                const Coef c = *reinterpret_cast<const Coef*>(sh.coef[k.i]);
+                const bool zero = c.g == 0.f;  // not for a NaN
+                for (int pos = again; pos < n + again; pos++, at.next()) {
+                    if (at.i % TG != team) continue;
+                    const int q = pos < n ? pos : pos - n;
+                    ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
+                    if (!ok) break;
+                    const T* const here = data + at.i * SLOT + w * PIECE + lane * N;  // this lane's first vector
+                    const uint32_t p0 = sp.first + q * SLOT + w * PIECE;
+                    const bool inside = vec && p0 >= sp.head && p0 + PIECE <= sp.last;
+                    T* const to = out + (p0 - sp.head) + lane * N;
+#pragma unroll
+                    for (uint32_t h = 0; h < GROUPS; h++) {
+                        uint4 z[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t v = (h * 4 + j) * STEP, p = p0 + v + lane * N;
+                            if (inside || sp.whole(p)) z[j] = *reinterpret_cast<const uint4*>(here + v);
+                            else if (p < sp.last) z[j] = sp.edge(p);
+                        }
+                        if (h == GROUPS - 1) {
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh.empty[at.i]);
+                        }
+                        if (!zero) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) z[j] = slope_of<T>(z[j], c);
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) z[j] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t v = (h * 4 + j) * STEP, p = p0 + v + lane * N;
+                            if (inside) *reinterpret_cast<uint4*>(to + v) = z[j];
+                            else if (p < sp.last) sp.store(out, vec, p, z[j]);
+                        }
+                    }
+                    // the target, by the lane that has its vector
+                    const uint32_t v = y + sp.head - p0;
+                    if (!zero && v < PIECE && v % STEP / N == (uint32_t)lane) fix_target(out + y, c);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.coef_free[k.i]);
+                k.next();
+            }
+        }
+        if (lane == 0) tma_store_wait_read<0>();
+    }
+    if (warp != 1) cluster_wait();
+    cluster_sync_all();  // no CTA ends while another may still write to its shared memory
+}
+
+// Rows that count, by sequence and all of them.  One CTA.
 __global__ void __launch_bounds__(1024) k_count(const LossRows r, const LossWork w) {
+    release_dependents();
     for (uint32_t i = threadIdx.x; i <= r.sequences; i += 1024) w.counts[i] = 0;
+    if (threadIdx.x == 0) *w.ticket = 0u;
     __syncthreads();
     for (long long at = 0; at < r.n; at += 1024) {
         const long long row = at + threadIdx.x;
         const int q = row < r.n && r.target(row) >= 0 ? r.sequence(row) : -1;
-        if (row < r.n) w.sequence[row] = q;
         const unsigned same = __match_any_sync(0xffffffffu, q), any = __ballot_sync(0xffffffffu, q >= 0);
         if (q >= 0 && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(w.counts + q, __popc(same));
         if ((threadIdx.x & 31) == 0 && any) atomicAdd(w.counts + r.sequences, __popc(any));
@@ -346,19 +746,10 @@ __device__ double block_sum(double v) {
     return v;
 }
 
-// The loss from its parts, always in the same order.  One CTA.
-__global__ void __launch_bounds__(1024) k_total(const double* parts, long long n, double by, float* out) {
-    grid_dependency_wait();
-    double v = 0.0;
-    for (long long i = threadIdx.x; i < n; i += 1024) v += parts[i];
-    v = block_sum<1024>(v);
-    if (threadIdx.x == 0) *out = (float)(v * by);
-}
-
 // A pair's lead over the reference, its loss and the slopes of its two
 // sequences.  One CTA for each pair.
-template <class T>
 __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTerms p, const LossWork w, const LossOut o) {
+    release_dependents();
     grid_dependency_wait();
     const uint32_t pairs = r.sequences / 2, pair = blockIdx.x;
     double lead[2];
@@ -369,17 +760,15 @@ __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTer
         const long long hi = r.starts ? min(r.n, (long long)r.starts[q + 1]) : lo + r.per;
         double v = 0.0, n = 0.0;
         for (long long row = lo + threadIdx.x; row < hi; row += 256) {
-            const int y = r.target(row);
-            if (y < 0) continue;
-            const float z = Lane<T>::one(static_cast<const T*>(r.logits)[row * r.stride + y]);
-            v += logprob(z, w.stats[row]) - (p.ref ? (double)p.ref[row] : 0.0);
+            if (r.target(row) < 0) continue;
+            v += w.logs[row] - (p.ref ? (double)p.ref[row] : 0.0);
             n += 1.0;
         }
         lead[side] = block_sum<256>(v);
         counted[side] = (long long)block_sum<256>(n);
         if (p.average && counted[side]) lead[side] /= (double)counted[side];
     }
-    if (threadIdx.x) return;
+    if (threadIdx.x >= 32) return;
     const double d = lead[0] - lead[1], h = p.beta * d, e = p.smoothing;
     double loss, slope;  // by d
     if (p.kind == TS_PREFER_SIGMOID) {
@@ -396,85 +785,128 @@ __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTer
         loss = off * off;
         slope = 2.0 * off;
     }
-    w.parts[pair] = loss;
-    if (o.margins) o.margins[pair] = (float)h;
-    slope *= (double)(o.grad_scale ? *o.grad_scale : 1.f) / pairs;
-    w.slope[pair] = (float)(p.average && counted[0] ? slope / counted[0] : slope);
-    w.slope[pair + pairs] = (float)-(p.average && counted[1] ? slope / counted[1] : slope);
+    if (threadIdx.x == 0) {
+        w.parts[pair] = loss;
+        if (o.margins) o.margins[pair] = (float)h;
+        slope *= (double)(o.grad_scale ? *o.grad_scale : 1.f) / pairs;
+        w.slope[pair] = (float)(p.average && counted[0] ? slope / counted[0] : slope);
+        w.slope[pair + pairs] = (float)-(p.average && counted[1] ? slope / counted[1] : slope);
+    }
+    total(w, (int)pairs, 1.0 / pairs, o.loss);
 }
 
-template <class T, int MODE>
-cudaError_t launch_rows(const RowArgs& a, bool dependent, cudaStream_t s) {
-    int dev = 0, sms = 1;
+// Clusters of `cl` CTAs of a k_ring that the current device runs at once.
+template <class T, bool S, bool G>
+cudaError_t clusters_at_once(int cl, int* out) {
+    using R = Roles<S, G>;
+    static std::atomic<int> known[64][kCluster + 1];  // by device
+    int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (*out = known[dev][cl].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    const Launch l(cl, 1, false, dim3((unsigned)cl), R::THREADS, R::SMEM, nullptr);
+    if (cl > 1) {
+        e = cudaOccupancyMaxActiveClusters(out, k_ring<T, S, G>, &l.cfg);
+    } else {
+        int sms = 0;
+        e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        *out = sms * R::CTAS;
+    }
+    if (e == cudaSuccess && *out < 1) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess && dev < 64) known[dev][cl].store(*out, std::memory_order_relaxed);
+    return e;
+}
+
+// CTAs to a row: rounds of the clusters that run at once, times what one of
+// them takes for a row, fixed and by the KiB of a CTA's part.  Measured, in us
+// for 1500 rows on 1, 2, 4 and 8 CTAs, statistics and gradient:
+//   16-bit, vocabulary  20000:  45  60  78 149      151936: 211 214 227 329
+//   f32,                20000:  52  63  95 131      151936: 428 343 364 374
+// (24 rows of 151936: 27 19 15 15 and 37 23 17 15; statistics alone are
+// fastest on one CTA from 300 rows on, on four for few.)  A part of more than
+// half of the slots overlaps less with the next row's, and rows that do not fit into
+// L2 together come from memory twice.
+template <class T, bool S, bool G>
+cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
+    using R = Roles<S, G>;
+    cudaError_t e = ensure_smem(k_ring<T, S, G>, R::SMEM);
     if (e != cudaSuccess) return e;
     int cl = 1;
     double least = 0;
     for (int c = 1; c <= kCluster; c *= 2) {
-        const double cost = (double)((a.r.n * c + 2 * sms - 1) / (2 * sms)) * (1.0 / c + 0.05);
-        if (c == 1 || cost < least) cl = c, least = cost;
+        if (c > 1 && a.r.vocab < 1024u * c) break;  // no part may be empty
+        int most = 1;
+        e = clusters_at_once<T, S, G>(c, &most);
+        if (e != cudaSuccess) return e;
+        const double kib = (double)a.r.vocab * sizeof(T) / c / 1024, l2 = most * kib * c / 1024;
+        double row = !G ? 1.2 + 0.042 * kib : !S ? 1.3 + 0.047 * kib : sizeof(T) == 2 ? 1.5 + 0.055 * kib : 1.1 + (kib > 96 ? 0.05 : 0.04) * kib;
+        if (S && G && kib > 128 && l2 > 64) row *= 1.3;
+        const double cost = (double)((a.r.n + most - 1) / most) * row;
+        if (c == 1 || cost < least) cl = c, least = cost, a.units = (int)(a.r.n < most ? a.r.n : most);
     }
-    const Launch l(cl, 1, dependent, dim3((unsigned)(a.r.n * cl)), kThreads, 0, s);
-    return cudaLaunchKernelEx(&l.cfg, k_rows<T, MODE>, a);
+    const Launch l(cl, 1, dependent, dim3((unsigned)(a.units * cl)), R::THREADS, R::SMEM, s);
+    return cudaLaunchKernelEx(&l.cfg, k_ring<T, S, G>, a);
 }
 
-template <int MODE>
-cudaError_t rows(const RowArgs& a, int dtype, bool dependent, cudaStream_t s) {
-    if (dtype == DT_F32) return launch_rows<float, MODE>(a, dependent, s);
-    return dtype == DT_BF16 ? launch_rows<__nv_bfloat16, MODE>(a, dependent, s) : launch_rows<__half, MODE>(a, dependent, s);
+template <class T, int THREADS>
+cudaError_t launch_short(RowArgs a, bool dependent, cudaStream_t s) {
+    a.units = (int)a.r.n;
+    const Launch l(1, 1, dependent, dim3((unsigned)a.r.n), THREADS, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS>, a);
 }
 
 template <class T>
-cudaError_t pairs(const LossRows& r, const PreferTerms& p, const LossWork& w, const LossOut& o, cudaStream_t s) {
-    return launch_dependent(1, k_pairs<T>, dim3(r.sequences / 2), 256, 0, s, r, p, w, o);
+cudaError_t rows_of(RowArgs a, bool dependent, cudaStream_t s) {
+    a.wait = dependent;
+    constexpr uint32_t per = 4 * Lane<T>::N, slack = Lane<T>::N;  // elements of a thread; a row's offset
+    if (a.r.vocab + slack <= 128 * per) return launch_short<T, 128>(a, dependent, s);
+    if (a.r.vocab + slack <= 512 * per) return launch_short<T, 512>(a, dependent, s);
+    if (!a.o.grad) return launch_ring<T, true, false>(a, dependent, s);
+    return a.mode == KNOWN ? launch_ring<T, false, true>(a, dependent, s) : launch_ring<T, true, true>(a, dependent, s);
+}
+
+cudaError_t rows(const RowArgs& a, int dtype, bool dependent, cudaStream_t s) {
+    return dtype == DT_F32 ? rows_of<float>(a, dependent, s) : dtype == DT_BF16 ? rows_of<__nv_bfloat16>(a, dependent, s) : rows_of<__half>(a, dependent, s);
 }
 
 }  // namespace
 
+cudaError_t expired_waits_loss(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
+
 cudaError_t launch_logprobs(const LossRows& r, float* logprobs, int dtype, cudaStream_t s) {
     RowArgs a{};
-    a.r = r;
+    a.r = r, a.mode = LOGPROBS;
     a.o.logprobs = logprobs;
     KScope ks("token_logprobs", s);
-    return rows<LOGPROBS>(a, dtype, false, s);
+    return rows(a, dtype, false, s);
 }
 
 cudaError_t launch_logprobs_backward(const LossRows& r, const float* g, const LossOut& o, int dtype, cudaStream_t s) {
     RowArgs a{};
-    a.r = r;
-    a.o = o;
-    a.g = g;
+    a.r = r, a.o = o, a.g = g, a.mode = GIVEN;
     KScope ks("token_logprobs_backward", s);
-    return rows<GIVEN>(a, dtype, false, s);
+    return rows(a, dtype, false, s);
 }
 
 cudaError_t launch_policy(const LossRows& r, const PolicyTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s) {
+    if (!r.n) return cudaMemsetAsync(o.loss, 0, sizeof(float), s);
     RowArgs a{};
-    a.r = r, a.p = p, a.w = w, a.o = o;
-    KScope ks("policy_loss", s, r.n ? 3 : 1);
-    cudaError_t e = cudaSuccess;
-    if (r.n) {
-        k_count<<<1, 1024, 0, s>>>(r, w);
-        e = cudaGetLastError();
-        if (e == cudaSuccess) e = rows<POLICY>(a, dtype, true, s);
-    }
-    if (e == cudaSuccess) e = launch_dependent(1, k_total, dim3(1), 1024, 0, s, (const double*)w.parts, r.n, 1.0, o.loss);
-    return e;
+    a.r = r, a.p = p, a.w = w, a.o = o, a.mode = POLICY;
+    KScope ks("policy_loss", s, 2);
+    k_count<<<1, 1024, 0, s>>>(r, w);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? rows(a, dtype, true, s) : e;
 }
 
 cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s) {
     RowArgs a{};
-    a.r = r, a.w = w, a.o = o;
+    a.r = r, a.w = w, a.o = o, a.mode = LOGPROBS;
     a.o.grad = nullptr;
-    const uint32_t n = r.sequences / 2;
-    KScope ks("preference_loss", s, 2 + (r.n > 0) + (r.n > 0 && o.grad));
-    cudaError_t e = r.n ? rows<LOGPROBS>(a, dtype, false, s) : cudaSuccess;
-    if (e == cudaSuccess)
-        e = dtype == DT_F32 ? pairs<float>(r, p, w, o, s) : dtype == DT_BF16 ? pairs<__nv_bfloat16>(r, p, w, o, s) : pairs<__half>(r, p, w, o, s);
-    if (e == cudaSuccess) e = launch_dependent(1, k_total, dim3(1), 1024, 0, s, (const double*)w.parts, (long long)n, 1.0 / n, o.loss);
-    a.o.grad = o.grad;
-    if (e == cudaSuccess && r.n && o.grad) e = rows<KNOWN>(a, dtype, true, s);
+    KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad));
+    cudaError_t e = r.n ? rows(a, dtype, false, s) : cudaMemsetAsync(w.ticket, 0, sizeof(unsigned), s);
+    if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 256, 0, s, r, p, w, o);
+    a.o.grad = o.grad, a.mode = KNOWN, a.backwards = 1;
+    if (e == cudaSuccess && r.n && o.grad) e = rows(a, dtype, true, s);
     return e;
 }
 

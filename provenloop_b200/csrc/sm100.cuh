@@ -171,6 +171,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// `bytes` from this CTA's shared to global memory, as bulk_copy; part of the
+// calling thread's bulk group.
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Until the stores have read their shared memory, but for the last N groups.
 template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {

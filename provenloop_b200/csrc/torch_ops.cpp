@@ -6,6 +6,7 @@
 // token is shorter on the GPU than its checks were in Python: this module is
 // those checks, compiled.  It does not link against the library: the entry
 // points' addresses come from the binding that loaded it (bind).
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
@@ -631,6 +632,11 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const bool each = args[2] != Py_None;
         const int groups = each ? whole_number(args[2]) : 1;
         if (groups < 1 || groups > TS_CLIP_MAX_GROUPS) bad("the number of adapters must be in 1 .. " + std::to_string(TS_CLIP_MAX_GROUPS));
+        // whether a tensor may have a forward-mode tangent at all: to ask each of hundreds takes as long as the call
+        const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
+        const auto history = [&](const at::Tensor& t) {
+            if (tangents || t.requires_grad()) no_history(&t);
+        };
         std::vector<ts_clip_tensor> list;
         list.reserve(grads.size());
         const at::Tensor* like = nullptr;
@@ -645,14 +651,14 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 bad(each ? "the gradients of stacked adapters must be contiguous" : "the gradients must be dense in memory");
             if (each && (t.dim() < 1 || t.size(0) != groups))
                 bad("the gradients of " + std::to_string(groups) + " stacked adapters must have that leading dimension, not " + shape_of(t.sizes()));
-            no_history(&t);
+            history(t);
             c.elements = (uint64_t)t.numel();
             if (apart) {
                 const at::Tensor& o = *tensor((*outs)[i], "every entry of out");
                 if (o.sizes() != t.sizes() || o.device() != t.device() || (o.scalar_type() != t.scalar_type() && o.scalar_type() != at::kFloat))
                     bad("an entry of out must be " + shape_of(t.sizes()) + " on " + t.device().str() + ", " + type_of(t.scalar_type()) + " or torch.float32");
                 if (o.strides() != t.strides() && !(o.is_contiguous() && t.is_contiguous())) bad("an entry of out must have its gradient's layout in memory");
-                no_history(&o);
+                history(o);
                 c.out_dtype = dtype_code(o.scalar_type());
                 c.out = o.mutable_data_ptr();
                 c.grad = t.const_data_ptr();

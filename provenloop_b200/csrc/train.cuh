@@ -57,11 +57,12 @@ struct PreferTerms {
 
 // What a loss's launches hand to one another, in the workspace.
 struct LossWork {
-    int* sequence;    // [n]: of a row that counts, else -1 (policy)
-    int* counts;      // [sequences + 1]: rows that count, and all of them (policy)
-    RowStats* stats;  // [n] (preference)
-    float* slope;     // [sequences]: d loss / d log-probability (preference)
-    double* parts;    // [n] (policy), [pairs] (preference): the loss is their sum
+    int* counts;       // [sequences + 1]: rows that count, and all of them (policy)
+    RowStats* stats;   // [n] (preference)
+    double* logs;      // [n]: log-probabilities (preference)
+    float* slope;      // [sequences]: d loss / d log-probability (preference)
+    double* parts;     // [n] (policy; by cluster or by row), [pairs] (preference): the loss is their sum
+    unsigned* ticket;  // parts that are there
 };
 
 struct LossOut {
@@ -75,6 +76,9 @@ cudaError_t launch_logprobs(const LossRows& r, float* logprobs, int dtype, cudaS
 cudaError_t launch_logprobs_backward(const LossRows& r, const float* g, const LossOut& o, int dtype, cudaStream_t s);
 cudaError_t launch_policy(const LossRows& r, const PolicyTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s);
 cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s);
+
+// waits of k_loss.cu that ran out on the current device so far
+cudaError_t expired_waits_loss(unsigned long long* out);
 
 // One group's part of one tensor.
 struct ClipTensor {
