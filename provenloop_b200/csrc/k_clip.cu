@@ -7,9 +7,12 @@
 // A group whose norm is not finite is left as it is.
 //
 // The bound is the tensors' traffic: each element is read for the norm, and
-// read and written for the clipping.  Three launches: the sums of squares of chunks
-// of parts, the norms, and the scaling, which goes backwards over the chunks,
-// since the latest are still in L2.
+// read and written for the clipping.  Two launches: the sums of squares of chunks of
+// parts, and the scaling, which goes backwards over the chunks, since the latest
+// are still in L2.  Every CTA of the second one adds up its group's sums by itself
+// where there are few; where there are many, a launch between the two does.
+// 295M elements in f32 (2.4 GB with the results, 3.5 GB with the second reading) take 576 us, 6.2 TB/s; the 112
+// gradients of 28 layers, 6.5M elements in bf16, 15 us.
 //
 // A chunk's sum of squares is a 64-bit value of its own, and a group's are
 // added in an order that depends on the sizes alone.
@@ -22,27 +25,31 @@ namespace tsg {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr uint32_t kChunkBytes = 32768;  // of a part that a CTA takes at a time
-constexpr int kMinTable = 16, kMaxTable = 448;  // tensors in a launch's arguments (14 KB of at most 32)
+// Bytes of a part that a CTA takes: as much as its threads load at a time, or
+// a quarter of that where this gives less than two CTAs to an SM (one layer's four gradients,
+// 0.9 MB: 6.5 us, in larger chunks 8.6).
+constexpr uint32_t kChunk = 32768, kSmallChunk = 8192;
+constexpr uint32_t kFold = 4096;  // sums of a group that every CTA of the scaling adds up: eight a thread
 
 struct ClipEntry {
     const void* grad;
     void* out;
     uint64_t part;
-    uint32_t chunk0;  // chunks of a group in the entries before
-    int16_t dtype, out_dtype;
+    int dtype, out_dtype;
 };
 template <int N>
 struct ClipTable {
     ClipEntry t[N];
+    uint32_t chunk0[N];  // chunks of a group in the entries before
     int count;
     uint32_t chunks;            // of a group in this launch
     uint32_t group_chunks, at;  // of a group in all launches, and in those before
+    uint32_t chunk;             // bytes
     double* partial;            // [groups][group_chunks]
-    float* factor;              // [groups]
+    float* factor;              // [groups], or null: the scaling finds it
 };
 
-__host__ __device__ __forceinline__ uint32_t chunk_elements(int dtype) { return kChunkBytes / (dtype == DT_F32 ? 4 : 2); }
+__host__ __device__ __forceinline__ uint32_t chunk_elements(int dtype, uint32_t bytes) { return bytes / (dtype == DT_F32 ? 4 : 2); }
 
 // Elements of one chunk.
 struct Piece {
@@ -55,12 +62,12 @@ __device__ __forceinline__ Piece piece_of(const ClipTable<N>& a, uint32_t group,
     int lo = 0, hi = a.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (chunk < a.t[mid].chunk0) hi = mid;
+        if (chunk < a.chunk0[mid]) hi = mid;
         else lo = mid;
     }
     const ClipEntry& t = a.t[lo];
-    const uint32_t most = chunk_elements(t.dtype);
-    const uint64_t at = (uint64_t)(chunk - t.chunk0) * most, left = t.part - at;
+    const uint32_t most = chunk_elements(t.dtype, a.chunk);
+    const uint64_t at = (uint64_t)(chunk - a.chunk0[lo]) * most, left = t.part - at;
     return {&t, group * t.part + at, left < most ? (uint32_t)left : most};
 }
 
@@ -194,42 +201,56 @@ __global__ void __launch_bounds__(1024) k_norms(const double* partial, uint32_t 
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ ClipTable<N> a) {
+__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ ClipTable<N> a, const Limit l, float* norms) {
     const uint32_t last = gridDim.x - 1 - blockIdx.x, group = last / a.chunks, chunk = last % a.chunks;
     const Piece p = piece_of(a, group, chunk);
     grid_dependency_wait();
-    const float by = a.factor[group];
+    float by;
+    if (a.factor) {
+        by = a.factor[group];
+    } else {
+        const double* sums = a.partial + (uint64_t)group * a.group_chunks;
+        double v = 0.0;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < a.group_chunks; i += kThreads) v += sums[i];
+        float norm;
+        by = l.factor(group, block_total<kThreads>(v), &norm);
+        if (chunk == 0 && a.at == 0 && threadIdx.x == 0) norms[group] = norm;
+    }
     if (by == 1.f && p.t->grad == p.t->out) return;
     if (p.t->dtype == DT_F32) piece_scaled<float>(p, by);
     else if (p.t->dtype == DT_BF16) piece_scaled<__nv_bfloat16>(p, by);
     else piece_scaled<__half>(p, by);
 }
 
-uint64_t chunks_of(const ClipTensor* t, uint64_t count) {
+uint64_t chunks_of(const ClipTensor* t, uint64_t count, uint32_t chunk) {
     uint64_t c = 0;
-    for (uint64_t i = 0; i < count; i++) c += (t[i].part + chunk_elements(t[i].dtype) - 1) / chunk_elements(t[i].dtype);
+    for (uint64_t i = 0; i < count; i++) c += (t[i].part + chunk_elements(t[i].dtype, chunk) - 1) / chunk_elements(t[i].dtype, chunk);
     return c;
+}
+
+uint32_t chunk_bytes(const ClipTensor* t, uint64_t count, uint32_t groups) {
+    return chunks_of(t, count, kChunk) * groups < 2 * kSms ? kSmallChunk : kChunk;
 }
 
 // The launches over the tensors, N to a launch: the squares, or the scaling.
 template <int N>
-cudaError_t passes(const ClipArgs& a, uint64_t chunks, float* factor, bool scale, KScope* ks, cudaStream_t s) {
+cudaError_t passes(const ClipArgs& a, uint32_t chunk, uint64_t chunks, float* factor, const Limit* scale, KScope* ks, cudaStream_t s) {
     uint64_t at = 0;
     cudaError_t e = cudaSuccess;
     for (uint64_t i = 0; i < a.count && e == cudaSuccess;) {
         ClipTable<N> t;
-        t.count = 0, t.chunks = 0, t.group_chunks = (uint32_t)chunks, t.at = (uint32_t)at, t.partial = a.partial, t.factor = factor;
+        t.count = 0, t.chunks = 0, t.group_chunks = (uint32_t)chunks, t.at = (uint32_t)at, t.chunk = chunk, t.partial = a.partial, t.factor = factor;
         for (; i < a.count && t.count < N; i++) {
             const ClipTensor& c = a.tensors[i];
-            if (!c.part) continue;
-            t.t[t.count++] = {c.grad, c.out, c.part, t.chunks, (int16_t)c.dtype, (int16_t)c.out_dtype};
-            t.chunks += (uint32_t)((c.part + chunk_elements(c.dtype) - 1) / chunk_elements(c.dtype));
+            t.chunk0[t.count] = t.chunks;
+            t.t[t.count++] = {c.grad, c.out, c.part, c.dtype, c.out_dtype};
+            t.chunks += (uint32_t)((c.part + chunk_elements(c.dtype, chunk) - 1) / chunk_elements(c.dtype, chunk));
         }
-        if (!t.count) break;
         at += t.chunks;
         const dim3 grid(t.chunks * a.groups);
         if (scale) {
-            e = launch_dependent(1, k_scale<N>, grid, kThreads, 0, s, t);
+            e = launch_dependent(1, k_scale<N>, grid, kThreads, 0, s, t, *scale, a.norms);
         } else {
             k_squares<N><<<grid, kThreads, 0, s>>>(t);
             e = cudaGetLastError();
@@ -239,21 +260,30 @@ cudaError_t passes(const ClipArgs& a, uint64_t chunks, float* factor, bool scale
     return e;
 }
 
+// N: the tensors in a launch's arguments, whose size the host pays for.
+template <int N>
+cudaError_t clip(const ClipArgs& a, cudaStream_t s) {
+    const uint32_t chunk = chunk_bytes(a.tensors, a.count, a.groups);
+    const uint64_t chunks = chunks_of(a.tensors, a.count, chunk);
+    const Limit l{a.max_norms, a.max_norm, a.one_max};
+    float* const factor = chunks <= kFold && chunks ? nullptr : reinterpret_cast<float*>(a.partial + chunks * a.groups);
+    KScope ks("clip_gradients", s, 0);
+    cudaError_t e = passes<N>(a, chunk, chunks, factor, nullptr, &ks, s);
+    if (e == cudaSuccess && factor) {
+        ks.kernels++;
+        e = launch_dependent(1, k_norms, dim3(a.groups), 1024, 0, s, (const double*)a.partial, (uint32_t)chunks, l, a.norms, factor);
+    }
+    return e == cudaSuccess ? passes<N>(a, chunk, chunks, factor, &l, &ks, s) : e;
+}
+
 }  // namespace
 
-uint64_t clip_partials(const ClipTensor* t, uint64_t count, uint32_t groups) { return chunks_of(t, count) * groups + (groups + 1) / 2; }
+uint64_t clip_partials(const ClipTensor* t, uint64_t count, uint32_t groups) {
+    return chunks_of(t, count, chunk_bytes(t, count, groups)) * groups + (groups + 1) / 2;
+}
 
 cudaError_t launch_clip(const ClipArgs& a, cudaStream_t s) {
-    const uint64_t chunks = chunks_of(a.tensors, a.count);
-    float* const factor = reinterpret_cast<float*>(a.partial + chunks * a.groups);
-    const Limit l{a.max_norms, a.max_norm, a.one_max};
-    KScope ks("clip_gradients", s, 1);
-    const bool few = a.count <= (uint64_t)kMinTable;
-    cudaError_t e = few ? passes<kMinTable>(a, chunks, factor, false, &ks, s) : passes<kMaxTable>(a, chunks, factor, false, &ks, s);
-    if (e == cudaSuccess)
-        e = launch_dependent(1, k_norms, dim3(a.groups), 1024, 0, s, (const double*)a.partial, (uint32_t)chunks, l, a.norms, factor);
-    if (e == cudaSuccess) e = few ? passes<kMinTable>(a, chunks, factor, true, &ks, s) : passes<kMaxTable>(a, chunks, factor, true, &ks, s);
-    return e;
+    return a.count <= 16 ? clip<16>(a, s) : a.count <= 128 ? clip<128>(a, s) : clip<448>(a, s);
 }
 
 }  // namespace tsg

@@ -619,6 +619,11 @@ struct Items {
     Items& operator=(const Items&) = delete;
     Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(o); }
     PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(o, i); }
+    // Entries some places on, whose parts lie far apart in memory.
+    void ahead(Py_ssize_t i) const {
+        if (i + 12 < size()) __builtin_prefetch((*this)[i + 12]);
+        if (i + 6 < size() && THPVariable_CheckExact((*this)[i + 6])) __builtin_prefetch(THPVariable_Unpack((*this)[i + 6]).unsafeGetTensorImpl());
+    }
 };
 
 // (grads, max_norm, adapters or None, out or None) -> norms
@@ -641,6 +646,8 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
         list.reserve(grads.size());
         const at::Tensor* like = nullptr;
         for (Py_ssize_t i = 0; i < grads.size(); i++) {
+            grads.ahead(i);
+            if (apart) outs->ahead(i);
             if (grads[i] == Py_None) continue;
             const at::Tensor& t = *tensor(grads[i], "every entry of grads");
             if (!like) like = &t;
