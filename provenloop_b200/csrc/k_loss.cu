@@ -157,21 +157,25 @@ __device__ __forceinline__ RowStats join_lanes(const RowStats& s) {
 // Of no elements, or of such as are -inf; differences of finite maxima are never NaN.
 __device__ __forceinline__ RowStats nothing() { return {-FLT_MAX, 0.f}; }
 
-// Adds four vectors to a thread's statistics.
-template <class T>
-__device__ __forceinline__ void see4(RowStats& t, const uint4 (&z)[4]) {
+// Adds V vectors to a thread's statistics.
+template <class T, int V>
+__device__ __forceinline__ void see(RowStats& t, const uint4 (&z)[V]) {
     constexpr int N = Lane<T>::N;
-    const float m = fmaxf(t.max, fmaxf(fmaxf(Lane<T>::top(z[0]), Lane<T>::top(z[1])), fmaxf(Lane<T>::top(z[2]), Lane<T>::top(z[3]))));
-    const float2 less = make_float2(-m, -m);
-    float2 sum[4] = {};
+    float m = t.max;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < V; j++) m = fmaxf(m, Lane<T>::top(z[j]));
+    const float2 less = make_float2(-m, -m);
+    float2 sum[V] = {};
+#pragma unroll
+    for (int j = 0; j < V; j++) {
         float f[N];
         Lane<T>::open(z[j], f);
 #pragma unroll
         for (int i = 0; i < N; i += 2) sum[j] = add2(sum[j], weight2(make_float2(f[i], f[i + 1]), less));
     }
-    const float2 all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+    float2 all = sum[0];
+#pragma unroll
+    for (int j = 1; j < V; j++) all = add2(all, sum[j]);
     t.sum = fmaf(t.sum, weight(t.max, m), all.x + all.y), t.max = m;
 }
 
@@ -341,60 +345,77 @@ __device__ __forceinline__ int counted(const RowArgs& a, long long row, long lon
 __device__ __forceinline__ long long rows_from(const LossRows& r) { return r.starts ? max(0ll, (long long)r.starts[0]) : 0ll; }
 __device__ __forceinline__ long long rows_to(const LossRows& r) { return r.starts ? min(r.n, (long long)r.starts[r.sequences]) : r.n; }
 
-// Rows that a CTA holds in registers, four vectors a thread.
-template <class T, int THREADS>
+// Rows that a CTA, or a cluster of them, holds in registers, V vectors a thread.
+template <class T, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
     constexpr uint32_t N = Lane<T>::N, W = THREADS / 32;
-    __shared__ RowStats warp_stats[W];
-    __shared__ float shared_coef[sizeof(Coef) / 4];
-    const long long row = blockIdx.x;
+    __shared__ RowStats warp_stats[W], cta_stats[kCluster];
+    __shared__ Coef shared_coef;
+    const int cl = (int)(gridDim.x / (unsigned)a.units), rank = (int)cluster_rank();
+    if (cl > 1) cluster_arrive();
+    const long long row = blockIdx.x / (unsigned)cl;
     const int y = counted(a, row, rows_from(a.r), rows_to(a.r)), lane = (int)(threadIdx.x & 31);
-    const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, 0, 1);
+    const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, cl);
     T* const out = a.o.grad ? static_cast<T*>(a.o.grad) + row * a.o.grad_stride : nullptr;
     const bool vec = out && reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
-    uint4 z[4];
+    uint4 z[V];
     Coef c{0.f, 0.f, 0.f, 0.f};
     if (y >= 0) {
         const float zy = Lane<T>::one(sp.x[y]);  // before the row may be written
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            const uint32_t p = (threadIdx.x + j * THREADS) * N;
+        for (uint32_t j = 0; j < V; j++) {
+            const uint32_t p = sp.first + (threadIdx.x + j * THREADS) * N;
             z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
                    : sp.whole(p) ? *reinterpret_cast<const uint4*>(sp.x + p - sp.head) : sp.edge(p);
         }
         RowStats s = nothing();
         if (a.mode != KNOWN) {
-            see4<T>(s, z);
+            see<T, V>(s, z);
             s = join_lanes(s);
             if (lane == 0) warp_stats[threadIdx.x >> 5] = s;
         }
         __syncthreads();
+        if (cl > 1 && a.mode != KNOWN) {
+            cluster_wait();  // the other CTAs have started
+            if (threadIdx.x < 32) {
+                s = join_lanes(lane < (int)W ? warp_stats[lane] : nothing());
+                if (lane < cl)
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(map_rank(&cta_stats[rank], (uint32_t)lane)), "f"(s.max), "f"(s.sum)
+                                 : "memory");
+            }
+            cluster_sync_all();
+        }
         if (threadIdx.x < 32) {
             if (a.wait) grid_dependency_wait();
             const RowInfo i = row_info(a, row, zy);
-            s = a.mode == KNOWN ? i.s : join_lanes(lane < W ? warp_stats[lane] : nothing());
+            const RowStats* const from = cl > 1 ? cta_stats : warp_stats;
+            s = a.mode == KNOWN ? i.s : join_lanes(lane < (cl > 1 ? cl : (int)W) ? from[lane] : nothing());
             double loss = 0.0;
-            c = finish_row(a, i, row, s, lane == 0, &loss);
+            c = finish_row(a, i, row, s, rank == 0 && lane == 0, &loss);
             if (lane == 0) {
-                *reinterpret_cast<Coef*>(shared_coef) = c;
-                if (a.mode == POLICY) a.w.parts[row] = loss;
+                shared_coef = c;
+                if (a.mode == POLICY && rank == 0) a.w.parts[row] = loss;
             }
         }
+        if (cl > 1 && a.mode == KNOWN) cluster_wait();
         __syncthreads();
-        c = *reinterpret_cast<const Coef*>(shared_coef);
-    } else if (threadIdx.x < 32) {
-        if (a.wait) grid_dependency_wait();
-        if (lane == 0) {
-            skip_row(a, row);
-            if (a.mode == POLICY) a.w.parts[row] = 0.0;
+        c = shared_coef;
+    } else {
+        if (cl > 1) cluster_wait();
+        if (threadIdx.x < 32) {
+            if (a.wait) grid_dependency_wait();
+            if (lane == 0 && rank == 0) {
+                skip_row(a, row);
+                if (a.mode == POLICY) a.w.parts[row] = 0.0;
+            }
         }
     }
-    if (a.mode == LOGPROBS && a.w.ticket && row == 0 && threadIdx.x == 0) *a.w.ticket = 0u;
-    if (a.mode == POLICY && threadIdx.x < 32) total(a.w, a.units, 1.0, a.o.loss);
+    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0 && threadIdx.x == 0) *a.w.ticket = 0u;
+    if (a.mode == POLICY && rank == 0 && threadIdx.x < 32) total(a.w, a.units, 1.0, a.o.loss);
     if (!out) return;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t p = (threadIdx.x + j * THREADS) * N;
+    for (uint32_t j = 0; j < V; j++) {
+        const uint32_t p = sp.first + (threadIdx.x + j * THREADS) * N;
         if (p >= sp.last) continue;
         sp.store(out, vec, p, c.g == 0.f ? make_uint4(0u, 0u, 0u, 0u) : slope_of<T>(z[j], c));
         if (c.g != 0.f && (uint32_t)y + sp.head - p < N) fix_target(out + y, c);
@@ -613,7 +634,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&sh.empty[at.i]);
                         }
-                        see4<T>(t, z);
+                        see<T, 4>(t, z);
                     }
                 }
                 t = join_lanes(t);
@@ -848,19 +869,35 @@ cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
     return cudaLaunchKernelEx(&l.cfg, k_ring<T, S, G>, a);
 }
 
-template <class T, int THREADS>
-cudaError_t launch_short(RowArgs a, bool dependent, cudaStream_t s) {
+template <class T, int THREADS, int V>
+cudaError_t launch_short(RowArgs a, int cl, bool dependent, cudaStream_t s) {
     a.units = (int)a.r.n;
-    const Launch l(1, 1, dependent, dim3((unsigned)a.r.n), THREADS, 0, s);
-    return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS>, a);
+    const Launch l(cl, 1, dependent, dim3((unsigned)(a.r.n * cl)), THREADS, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS, V>, a);
 }
 
 template <class T>
 cudaError_t rows_of(RowArgs a, bool dependent, cudaStream_t s) {
     a.wait = dependent;
-    constexpr uint32_t per = 4 * Lane<T>::N, slack = Lane<T>::N;  // elements of a thread; a row's offset
-    if (a.r.vocab + slack <= 128 * per) return launch_short<T, 128>(a, dependent, s);
-    if (a.r.vocab + slack <= 512 * per) return launch_short<T, 512>(a, dependent, s);
+    constexpr uint32_t N = Lane<T>::N;  // also what a row may be off its first vector
+    if (a.r.vocab + N <= 128 * 4 * N) return launch_short<T, 128, 4>(a, 1, dependent, s);
+    // Longer ones by a CTA or a cluster while these run at once, or (gradients of
+    // 16-bit types) in three rounds.  In us, so and by k_ring: 24 rows of 151936 in bf16 with
+    // gradients 9.5 and 15, 120 rows 27 and 28, 200 rows 50 and 42; 24 rows scored 8.7 and 9.9, 48 rows
+    // 13 and 11; 5000 rows of 8000 63 and 32.  12 rows in f32 8.6 and 13, with gradients of 24 rows 15 and 15.
+    const auto fits = [&](uint64_t elements, int cl) { return ((uint64_t)a.r.vocab + N + cl - 1) / cl + (cl > 1 ? 128 : 0) <= elements; };
+    const auto few = [&](int cl, int threads) {
+        const uint64_t at_once = kSms * 1024 / threads;
+        return (uint64_t)a.r.n * cl <= (a.o.grad && sizeof(T) == 2 ? 3 * at_once : at_once);
+    };
+    if (fits(512 * 4 * N, 1)) {
+        if (few(1, 512)) return launch_short<T, 512, 4>(a, 1, dependent, s);
+    } else {
+        constexpr int THREADS = sizeof(T) == 2 ? 512 : 1024;
+        int cl = 2;
+        while (cl < kCluster && !fits(THREADS * 5 * N, cl)) cl *= 2;
+        if (fits(THREADS * 5 * N, cl) && few(cl, THREADS)) return launch_short<T, THREADS, 5>(a, cl, dependent, s);
+    }
     if (!a.o.grad) return launch_ring<T, true, false>(a, dependent, s);
     return a.mode == KNOWN ? launch_ring<T, false, true>(a, dependent, s) : launch_ring<T, true, true>(a, dependent, s);
 }
