@@ -40,6 +40,7 @@ struct RowArgs {
     int backwards;   // the last rows first
     int wait;        // the launch before this one has to be waited for
     int units;       // clusters (k_ring) or rows (k_short)
+    int log;         // of the CTAs in a cluster
 };
 
 __device__ __forceinline__ float exp2_fast(float v) {
@@ -323,9 +324,10 @@ template <class T>
 struct Span {
     const T* x;
     uint32_t head, first, last;
-    __device__ __forceinline__ Span(const T* x_, uint32_t vocab, int rank, int cl) : x(x_) {
+    // the part `rank` of 2^log parts
+    __device__ __forceinline__ Span(const T* x_, uint32_t vocab, int rank, int log) : x(x_) {
         head = (uint32_t)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-        const uint32_t end = head + vocab, span = ((end + cl - 1) / cl + 127) / 128 * 128;
+        const uint32_t end = head + vocab, span = ((end + (1u << log) - 1 >> log) + 127) / 128 * 128;
         first = min(end, rank * span), last = min(end, first + span);
     }
     __device__ __forceinline__ bool whole(uint32_t p) const { return p >= head && p + Lane<T>::N <= last; }
@@ -351,11 +353,11 @@ __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
     constexpr uint32_t N = Lane<T>::N, W = THREADS / 32;
     __shared__ RowStats warp_stats[W], cta_stats[kCluster];
     __shared__ Coef shared_coef;
-    const int cl = (int)(gridDim.x / (unsigned)a.units), rank = (int)cluster_rank();
+    const int cl = 1 << a.log, rank = (int)cluster_rank();
     if (cl > 1) cluster_arrive();
-    const long long row = blockIdx.x / (unsigned)cl;
+    const long long row = blockIdx.x >> a.log;
     const int y = counted(a, row, rows_from(a.r), rows_to(a.r)), lane = (int)(threadIdx.x & 31);
-    const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, cl);
+    const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, a.log);
     T* const out = a.o.grad ? static_cast<T*>(a.o.grad) + row * a.o.grad_stride : nullptr;
     const bool vec = out && reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
     uint4 z[V];
@@ -435,6 +437,7 @@ constexpr uint32_t kSlot = 16384;
 constexpr uint32_t kZeros = 4096;
 constexpr int kTeam = 8;   // warps that take a slot together, four vectors a lane
 constexpr int kDepth = 4;  // rows between two roles
+constexpr int kStats = 2;  // rows whose lanes' statistics are waiting to be joined
 // The teams of a role take the slots in turn, and every team always the same
 // ones: it has seen a slot's last load when it waits for the next, and a parity
 // wait tells the two apart.  Statistics alone: two CTAs on an SM (4096 rows of
@@ -448,10 +451,11 @@ struct Roles {
     static_assert((!S || SLOTS % TS == 0) && (!G || SLOTS % TG == 0), "a slot's team must not change");
 };
 
+template <int S_THREADS>
 struct RingShared {
-    uint64_t full[12], empty[12], stats_full[kDepth], stats_free[kDepth], joined[kDepth], coef_full[kDepth], coef_free[kDepth];
-    RowStats warp_stats[kDepth][2 * kTeam], cta_stats[kDepth][kCluster];
-    float coef[kDepth][sizeof(Coef) / 4];
+    uint64_t full[12], empty[12], stats_full[kStats], stats_free[kStats], joined[kDepth], coef_full[kDepth], coef_free[kDepth];
+    RowStats lane_stats[kStats][S_THREADS ? S_THREADS : 1], cta_stats[kDepth][kCluster];
+    Coef coef[kDepth];
     uint32_t dead;
 };
 
@@ -497,13 +501,14 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     constexpr int TS = Roles<S, G>::TS, TG = Roles<S, G>::TG, SLOTS = Roles<S, G>::SLOTS, KEEP = Roles<S, G>::KEEP;
     constexpr uint32_t STEP = 32 * N, GROUPS = SLOT / (kTeam * 4 * STEP);  // a lane takes that often four vectors of a slot
     extern __shared__ __align__(128) unsigned char slots[];
-    __shared__ RingShared sh;
+    __shared__ RingShared<TS * kTeam * 32> sh;
     const int rank = (int)cluster_rank(), warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
-    const int cl = (int)(gridDim.x / (unsigned)a.units), cluster = (int)(blockIdx.x / (unsigned)cl);
+    const int cl = 1 << a.log, cluster = (int)(blockIdx.x >> a.log);
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLOTS; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kTeam);
+        for (int i = 0; i < kStats; i++) mbar_init(&sh.stats_full[i], TS * kTeam), mbar_init(&sh.stats_free[i], 1);
         for (int i = 0; i < kDepth; i++) {
-            mbar_init(&sh.stats_full[i], TS * kTeam), mbar_init(&sh.stats_free[i], 1), mbar_init(&sh.joined[i], 1);
+            mbar_init(&sh.joined[i], 1);
             mbar_init(&sh.coef_full[i], 1), mbar_init(&sh.coef_free[i], TG * kTeam);
         }
         sh.dead = 0;
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     __syncthreads();
     cluster_arrive();  // waited for before the first access to another CTA's shared memory
     const long long lo = rows_from(a.r), hi = rows_to(a.r);
-    const auto span_of = [&](long long row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, cl); };
+    const auto span_of = [&](long long row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, a.log); };
     const auto chunks_of = [](const Span<T>& sp) { return (int)((sp.last - sp.first + SLOT - 1) / SLOT); };
     T* const data = reinterpret_cast<T*>(slots);
     T* const zeros = data + SLOTS * SLOT;  // kZeros bytes of them
@@ -547,7 +552,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         }
         if (!ok) settle();
     } else if (warp == 1) {
-        Ring k(kDepth, 0);
+        Ring k(kDepth, 0), ks(kStats, 0);
         double loss = 0.0;
         bool met = false;
         if (a.wait) grid_dependency_wait();
@@ -565,10 +570,18 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                 i.share = __shfl_sync(0xffffffffu, mine.share, from), i.scaled = __shfl_sync(0xffffffffu, mine.scaled, from);
                 RowStats s{__shfl_sync(0xffffffffu, mine.s.max, from), __shfl_sync(0xffffffffu, mine.s.sum, from)};
                 if (S) {
-                    ok = warp_wait(&sh.stats_full[k.i], k.phase, &sh.dead);
+                    ok = warp_wait(&sh.stats_full[ks.i], ks.phase, &sh.dead);
                     if (!ok) break;
-                    s = join_lanes(lane < TS * kTeam ? sh.warp_stats[k.i][lane] : nothing());
-                    if (lane == 0) mbar_arrive(&sh.stats_free[k.i]);
+                    const RowStats* const t = sh.lane_stats[ks.i] + lane;
+                    s = nothing();
+#pragma unroll
+                    for (int j = 0; j < TS * kTeam; j++) s.max = fmaxf(s.max, t[j * 32].max);
+#pragma unroll 4
+                    for (int j = 0; j < TS * kTeam; j++) s.sum = fmaf(t[j * 32].sum, weight(t[j * 32].max, s.max), s.sum);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.stats_free[ks.i]);
+                    ks.next();
+                    s = join_lanes(s);
                     if (cl > 1) {
                         if (!met) cluster_wait(), met = true;
                         if (lane == 0) mbar_expect(&sh.joined[k.i], (uint32_t)cl * sizeof(RowStats));
@@ -587,7 +600,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                     ok = warp_wait(&sh.coef_free[k.i], k.phase ^ 1, &sh.dead);
                     if (!ok) break;
                     if (lane == 0) {
-                        *reinterpret_cast<Coef*>(sh.coef[k.i]) = c;
+                        sh.coef[k.i] = c;
                         mbar_arrive(&sh.coef_full[k.i]);
                     }
                 }
@@ -601,7 +614,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     } else if (S && (!G || warp < 2 + TS * kTeam)) {
         const int w = (warp - 2) % kTeam, team = (warp - 2) / kTeam;
         const uint32_t v0 = (uint32_t)w * GROUPS * 4 * STEP + lane * N;  // this lane's first vector of a slot
-        Ring at(SLOTS, 0), k(kDepth, 0);
+        Ring at(SLOTS, 0), k(kStats, 0);
         for (long long b = 0; ok; b++) {
             const Batch rows(a, b, lo, hi, cluster);
             if (!rows.rows) break;
@@ -637,12 +650,10 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                         see<T, 4>(t, z);
                     }
                 }
-                t = join_lanes(t);
                 ok = ok && warp_wait(&sh.stats_free[k.i], k.phase ^ 1, &sh.dead);
-                if (lane == 0 && ok) {
-                    sh.warp_stats[k.i][warp - 2] = t;
-                    mbar_arrive(&sh.stats_full[k.i]);
-                }
+                if (ok) sh.lane_stats[k.i][(warp - 2) * 32 + lane] = t;
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(&sh.stats_full[k.i]);
                 // what arrives once more is not for this role, but it has to be seen
                 for (int c = 0; c < again && ok; c++, at.next())
                     if (at.i % TS == team) ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
@@ -683,10 +694,10 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                 }
                 const uint32_t y = (uint32_t)__shfl_sync(0xffffffffu, rows.y, of);
                 const int n = chunks_of(sp), again = again_of(n);
-                at.skip(again);
+                if (again) at.skip(again);
                 ok = warp_wait(&sh.coef_full[k.i], k.phase, &sh.dead);
                 if (!ok) break;
-                const Coef c = *reinterpret_cast<const Coef*>(sh.coef[k.i]);
+                const Coef c = sh.coef[k.i];
                 const bool zero = c.g == 0.f;  // not for a NaN
                 for (int pos = again; pos < n + again; pos++, at.next()) {
                     if (at.i % TG != team) continue;
@@ -816,6 +827,8 @@ __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTer
     total(w, (int)pairs, 1.0 / pairs, o.loss);
 }
 
+int log2_of(int cl) { return cl == 8 ? 3 : cl / 2; }
+
 // Clusters of `cl` CTAs of a k_ring that the current device runs at once.
 template <class T, bool S, bool G>
 cudaError_t clusters_at_once(int cl, int* out) {
@@ -865,13 +878,14 @@ cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
         const double cost = (double)((a.r.n + most - 1) / most) * row;
         if (c == 1 || cost < least) cl = c, least = cost, a.units = (int)(a.r.n < most ? a.r.n : most);
     }
+    a.log = log2_of(cl);
     const Launch l(cl, 1, dependent, dim3((unsigned)(a.units * cl)), R::THREADS, R::SMEM, s);
     return cudaLaunchKernelEx(&l.cfg, k_ring<T, S, G>, a);
 }
 
 template <class T, int THREADS, int V>
 cudaError_t launch_short(RowArgs a, int cl, bool dependent, cudaStream_t s) {
-    a.units = (int)a.r.n;
+    a.units = (int)a.r.n, a.log = log2_of(cl);
     const Launch l(cl, 1, dependent, dim3((unsigned)(a.r.n * cl)), THREADS, 0, s);
     return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS, V>, a);
 }
