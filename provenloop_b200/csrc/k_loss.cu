@@ -480,16 +480,35 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
     return __all_sync(0xffffffffu, sleep_wait(bar, parity, dead));
 }
 
-// The next 32 of a cluster's rows, one a lane.
+// The next 32 of a cluster's rows, one a lane.  Of rows in order, every so
+// many-th that counts and every so many-th other one, evenly mixed: the others only
+// write, which costs next to nothing beside those that compute.
 struct Batch {
-    long long row;
-    int y;
+    long long row = 0;
+    int y = -1;
     uint32_t rows, counts;  // lanes that have a row; whose row counts
     __device__ __forceinline__ Batch(const RowArgs& a, long long b, long long lo, long long hi, int cluster) {
-        const long long i = (b * 32 + (threadIdx.x & 31)) * a.units + cluster;
-        const bool there = i < a.r.n;
-        row = a.backwards ? a.r.n - 1 - i : i;
-        y = there ? counted(a, row, lo, hi) : -1;
+        const long long t = b * 32 + (threadIdx.x & 31);
+        bool there;
+        if (a.w.order) {
+            const long long m = a.w.order[a.r.n], other = a.units - 1 - cluster;
+            const long long mine = m > cluster ? (m - cluster - 1) / a.units + 1 : 0, rest = a.r.n - m > other ? (a.r.n - m - other - 1) / a.units + 1 : 0;
+            there = t < mine + rest;
+            if (there) {
+                const long long before = t * mine / (mine + rest);
+                if ((t + 1) * mine / (mine + rest) > before) {
+                    row = a.w.order[cluster + (a.backwards ? mine - 1 - before : before) * a.units];
+                    y = a.r.target(row);
+                } else {
+                    row = a.w.order[a.r.n - 1 - (other + (t - before) * a.units)];
+                }
+            }
+        } else {
+            const long long i = t * a.units + cluster;
+            there = i < a.r.n;
+            row = a.backwards ? a.r.n - 1 - i : i;
+            if (there) y = counted(a, row, lo, hi);
+        }
         rows = __ballot_sync(0xffffffffu, there), counts = __ballot_sync(0xffffffffu, y >= 0);
     }
     __device__ __forceinline__ long long row_of(int lane) const { return __shfl_sync(0xffffffffu, row, lane); }
@@ -521,6 +540,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     }
     __syncthreads();
     cluster_arrive();  // waited for before the first access to another CTA's shared memory
+    if (a.w.order && a.wait) grid_dependency_wait();
     const long long lo = rows_from(a.r), hi = rows_to(a.r);
     const auto span_of = [&](long long row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, a.log); };
     const auto chunks_of = [](const Span<T>& sp) { return (int)((sp.last - sp.first + SLOT - 1) / SLOT); };
@@ -555,7 +575,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         Ring k(kDepth, 0), ks(kStats, 0);
         double loss = 0.0;
         bool met = false;
-        if (a.wait) grid_dependency_wait();
+        if (a.wait && !a.w.order) grid_dependency_wait();
         for (long long b = 0; ok; b++) {
             const Batch rows(a, b, lo, hi, cluster);
             if (!rows.rows) break;
@@ -750,18 +770,71 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     cluster_sync_all();  // no CTA ends while another may still write to its shared memory
 }
 
-// Rows that count, by sequence and all of them.  One CTA.
-__global__ void __launch_bounds__(1024) k_count(const LossRows r, const LossWork w) {
+// Before the rows: how many of them count (policy: by sequence, and all of
+// them), and their order (order[n]: how many count, which come first, the others from
+// the end), so that the clusters get as many.  By every so many-th of a padded batch's
+// rows some had a quarter more than the mean (6144 rows in 16 sequences, 2996 of
+// which count, on two CTAs each: 530 us, in order 506).  One CTA.
+__global__ void __launch_bounds__(1024) k_order(const RowArgs a) {
+    constexpr int EACH = 4;
+    __shared__ int before[32], found;
     release_dependents();
-    for (uint32_t i = threadIdx.x; i <= r.sequences; i += 1024) w.counts[i] = 0;
-    if (threadIdx.x == 0) *w.ticket = 0u;
+    const LossRows& r = a.r;
+    const bool policy = a.mode == POLICY;
+    const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
+    if (policy)
+        for (uint32_t i = threadIdx.x; i <= r.sequences; i += 1024) a.w.counts[i] = 0;
+    if (threadIdx.x == 0) {
+        found = 0;
+        if (a.w.ticket) *a.w.ticket = 0u;
+    }
     __syncthreads();
-    for (long long at = 0; at < r.n; at += 1024) {
-        const long long row = at + threadIdx.x;
-        const int q = row < r.n && r.target(row) >= 0 ? r.sequence(row) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, q), any = __ballot_sync(0xffffffffu, q >= 0);
-        if (q >= 0 && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(w.counts + q, __popc(same));
-        if ((threadIdx.x & 31) == 0 && any) atomicAdd(w.counts + r.sequences, __popc(any));
+    const long long lo = rows_from(r), hi = rows_to(r);
+    for (long long at = 0; at < r.n; at += 1024 * EACH) {
+        unsigned any[EACH];
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const long long row = at + (warp * EACH + j) * 32 + lane;
+            const bool is = row < r.n && counted(a, row, lo, hi) >= 0;
+            any[j] = __ballot_sync(0xffffffffu, is);
+            mine += __popc(any[j]);
+            if (policy) {
+                const int q = is ? r.sequence(row) : -1;
+                const unsigned same = __match_any_sync(0xffffffffu, q);
+                if (is && lane == __ffs(same) - 1) atomicAdd(a.w.counts + q, __popc(same));
+            }
+        }
+        if (lane == 0) before[warp] = mine;
+        __syncthreads();
+        if (warp == 0) {
+            const int v = before[lane];
+            int sum = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            before[lane] = found + sum - v;
+            __syncwarp();
+            if (lane == 31) found += sum;
+        }
+        __syncthreads();
+        if (a.w.order) {
+            int c = before[warp];  // rows that count in front of this warp's next 32
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                const long long row = at + (warp * EACH + j) * 32 + lane;
+                const int mine_before = c + __popc(any[j] & ((1u << lane) - 1));
+                if (row < r.n) a.w.order[any[j] >> lane & 1 ? mine_before : r.n - 1 - (row - mine_before)] = (int)row;
+                c += __popc(any[j]);
+            }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        if (policy) a.w.counts[r.sequences] = found;
+        if (a.w.order) a.w.order[r.n] = found;
     }
 }
 
@@ -858,8 +931,9 @@ cudaError_t clusters_at_once(int cl, int* out) {
 //   f32,                20000:  52  63  95 131      151936: 428 343 364 374
 // (24 rows of 151936: 27 19 15 15 and 37 23 17 15; statistics alone are
 // fastest on one CTA from 300 rows on, on four for few.)  A part of more than
-// half of the slots overlaps less with the next row's, and rows that do not fit into
-// L2 together come from memory twice.
+// half of the slots overlaps less with the next row's.  What a part has beyond the
+// slots that it keeps is read again, and not always found in L2: 6144 rows of 151936, half of which
+// are only written, take 600 us on one CTA each and 506 on two.
 template <class T, bool S, bool G>
 cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
     using R = Roles<S, G>;
@@ -874,7 +948,7 @@ cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         const double kib = (double)a.r.vocab * sizeof(T) / c / 1024, l2 = most * kib * c / 1024;
         double row = !G ? 1.2 + 0.042 * kib : !S ? 1.3 + 0.047 * kib : sizeof(T) == 2 ? 1.5 + 0.055 * kib : 1.1 + (kib > 96 ? 0.05 : 0.04) * kib;
-        if (S && G && kib > 128 && l2 > 64) row *= 1.3;
+        if (S && G && kib > 170) row *= sizeof(T) == 4 && l2 > 64 ? 1.3 : 1.15;
         const double cost = (double)((a.r.n + most - 1) / most) * row;
         if (c == 1 || cost < least) cl = c, least = cost, a.units = (int)(a.r.n < most ? a.r.n : most);
     }
@@ -890,28 +964,38 @@ cudaError_t launch_short(RowArgs a, int cl, bool dependent, cudaStream_t s) {
     return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS, V>, a);
 }
 
+// The kernel that a call's rows take: k_short with so many threads and CTAs
+// to a row, or (0 threads) k_ring.
+struct Path {
+    int threads, cl;
+};
+// Short rows in registers.  Longer ones too, by a CTA or a cluster, while these run at once, or
+// (gradients of 16-bit types) in three rounds.  In us, so and by k_ring: 24 rows of 151936 in bf16
+// with gradients 9.5 and 15, 120 rows 27 and 28, 200 rows 50 and 42; 24 rows scored 8.7 and 9.9, 48 rows
+// 13 and 11; 5000 rows of 8000 63 and 32.  12 rows in f32 8.6 and 13, with gradients of 24 rows 15 and 15.
+template <class T>
+Path path_of(uint64_t n, uint32_t vocab, bool grad) {
+    constexpr uint32_t N = Lane<T>::N;  // also what a row may be off its first vector
+    const auto fits = [&](uint64_t elements, int cl) { return ((uint64_t)vocab + N + cl - 1) / cl + (cl > 1 ? 128 : 0) <= elements; };
+    const auto few = [&](int cl, int threads) {
+        const uint64_t at_once = kSms * 1024 / threads;
+        return n * cl <= (grad && sizeof(T) == 2 ? 3 * at_once : at_once);
+    };
+    if (fits(128 * 4 * N, 1)) return {128, 1};
+    if (fits(512 * 4 * N, 1)) return {few(1, 512) ? 512 : 0, 1};
+    constexpr int THREADS = sizeof(T) == 2 ? 512 : 1024;
+    int cl = 2;
+    while (cl < kCluster && !fits(THREADS * 5 * N, cl)) cl *= 2;
+    return {fits(THREADS * 5 * N, cl) && few(cl, THREADS) ? THREADS : 0, cl};
+}
+
 template <class T>
 cudaError_t rows_of(RowArgs a, bool dependent, cudaStream_t s) {
     a.wait = dependent;
-    constexpr uint32_t N = Lane<T>::N;  // also what a row may be off its first vector
-    if (a.r.vocab + N <= 128 * 4 * N) return launch_short<T, 128, 4>(a, 1, dependent, s);
-    // Longer ones by a CTA or a cluster while these run at once, or (gradients of
-    // 16-bit types) in three rounds.  In us, so and by k_ring: 24 rows of 151936 in bf16 with
-    // gradients 9.5 and 15, 120 rows 27 and 28, 200 rows 50 and 42; 24 rows scored 8.7 and 9.9, 48 rows
-    // 13 and 11; 5000 rows of 8000 63 and 32.  12 rows in f32 8.6 and 13, with gradients of 24 rows 15 and 15.
-    const auto fits = [&](uint64_t elements, int cl) { return ((uint64_t)a.r.vocab + N + cl - 1) / cl + (cl > 1 ? 128 : 0) <= elements; };
-    const auto few = [&](int cl, int threads) {
-        const uint64_t at_once = kSms * 1024 / threads;
-        return (uint64_t)a.r.n * cl <= (a.o.grad && sizeof(T) == 2 ? 3 * at_once : at_once);
-    };
-    if (fits(512 * 4 * N, 1)) {
-        if (few(1, 512)) return launch_short<T, 512, 4>(a, 1, dependent, s);
-    } else {
-        constexpr int THREADS = sizeof(T) == 2 ? 512 : 1024;
-        int cl = 2;
-        while (cl < kCluster && !fits(THREADS * 5 * N, cl)) cl *= 2;
-        if (fits(THREADS * 5 * N, cl) && few(cl, THREADS)) return launch_short<T, THREADS, 5>(a, cl, dependent, s);
-    }
+    const Path p = path_of<T>((uint64_t)a.r.n, a.r.vocab, a.o.grad != nullptr);
+    if (p.threads == 128) return launch_short<T, 128, 4>(a, 1, dependent, s);
+    if (p.threads && p.cl == 1) return launch_short<T, 512, 4>(a, 1, dependent, s);
+    if (p.threads) return launch_short<T, sizeof(T) == 2 ? 512 : 1024, 5>(a, p.cl, dependent, s);
     if (!a.o.grad) return launch_ring<T, true, false>(a, dependent, s);
     return a.mode == KNOWN ? launch_ring<T, false, true>(a, dependent, s) : launch_ring<T, true, true>(a, dependent, s);
 }
@@ -920,23 +1004,38 @@ cudaError_t rows(const RowArgs& a, int dtype, bool dependent, cudaStream_t s) {
     return dtype == DT_F32 ? rows_of<float>(a, dependent, s) : dtype == DT_BF16 ? rows_of<__nv_bfloat16>(a, dependent, s) : rows_of<__half>(a, dependent, s);
 }
 
+// k_order, where the call needs it.
+cudaError_t order(const RowArgs& a, cudaStream_t s) {
+    if (!a.w.order && a.mode != POLICY) return cudaSuccess;
+    k_order<<<1, 1024, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
 }  // namespace
+
+bool loss_orders(uint64_t n, uint32_t vocab, int dtype, bool grad, bool both) {
+    if (n <= 8ull * kSms) return false;
+    const auto ring = [&](bool with) { return (dtype == DT_F32 ? path_of<float>(n, vocab, with) : path_of<__half>(n, vocab, with)).threads == 0; };
+    return ring(grad) || (both && ring(false));
+}
 
 cudaError_t expired_waits_loss(unsigned long long* out) { return cudaMemcpyFromSymbol(out, g_expired_waits, sizeof(*out)); }
 
-cudaError_t launch_logprobs(const LossRows& r, float* logprobs, int dtype, cudaStream_t s) {
+cudaError_t launch_logprobs(const LossRows& r, const LossWork& w, float* logprobs, int dtype, cudaStream_t s) {
     RowArgs a{};
-    a.r = r, a.mode = LOGPROBS;
+    a.r = r, a.w = w, a.mode = LOGPROBS;
     a.o.logprobs = logprobs;
-    KScope ks("token_logprobs", s);
-    return rows(a, dtype, false, s);
+    KScope ks("token_logprobs", s, 1 + !!w.order);
+    const cudaError_t e = order(a, s);
+    return e == cudaSuccess ? rows(a, dtype, w.order, s) : e;
 }
 
-cudaError_t launch_logprobs_backward(const LossRows& r, const float* g, const LossOut& o, int dtype, cudaStream_t s) {
+cudaError_t launch_logprobs_backward(const LossRows& r, const float* g, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s) {
     RowArgs a{};
-    a.r = r, a.o = o, a.g = g, a.mode = GIVEN;
-    KScope ks("token_logprobs_backward", s);
-    return rows(a, dtype, false, s);
+    a.r = r, a.w = w, a.o = o, a.g = g, a.mode = GIVEN;
+    KScope ks("token_logprobs_backward", s, 1 + !!w.order);
+    const cudaError_t e = order(a, s);
+    return e == cudaSuccess ? rows(a, dtype, w.order, s) : e;
 }
 
 cudaError_t launch_policy(const LossRows& r, const PolicyTerms& p, const LossWork& w, const LossOut& o, int dtype, cudaStream_t s) {
@@ -944,8 +1043,7 @@ cudaError_t launch_policy(const LossRows& r, const PolicyTerms& p, const LossWor
     RowArgs a{};
     a.r = r, a.p = p, a.w = w, a.o = o, a.mode = POLICY;
     KScope ks("policy_loss", s, 2);
-    k_count<<<1, 1024, 0, s>>>(r, w);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = order(a, s);
     return e == cudaSuccess ? rows(a, dtype, true, s) : e;
 }
 
@@ -953,8 +1051,9 @@ cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const Los
     RowArgs a{};
     a.r = r, a.w = w, a.o = o, a.mode = LOGPROBS;
     a.o.grad = nullptr;
-    KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad));
-    cudaError_t e = r.n ? rows(a, dtype, false, s) : cudaMemsetAsync(w.ticket, 0, sizeof(unsigned), s);
+    KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad) + !!w.order);
+    cudaError_t e = order(a, s);
+    if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, sizeof(unsigned), s);
     if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 256, 0, s, r, p, w, o);
     a.o.grad = o.grad, a.mode = KNOWN, a.backwards = 1;
     if (e == cudaSuccess && r.n && o.grad) e = rows(a, dtype, true, s);

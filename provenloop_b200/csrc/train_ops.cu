@@ -83,7 +83,8 @@ int check_loss(const ts_loss_args* a, int op) {
 }
 
 struct LossPlan {
-    uint64_t counts, stats, logs, slope, parts, ticket, bytes;
+    bool ordered;
+    uint64_t order, counts, stats, logs, slope, parts, ticket, bytes;
 };
 
 LossPlan plan_of(const ts_loss_args* a, int op) {
@@ -95,6 +96,8 @@ LossPlan plan_of(const ts_loss_args* a, int op) {
         return here;
     };
     const bool policy = op == TS_LOSS_POLICY, prefer = op == TS_LOSS_PREFERENCE;
+    p.ordered = loss_orders(a->n, a->vocab, a->dtype, a->grad, prefer);
+    p.order = take(p.ordered, (a->n + 1) * 4);
     p.counts = take(policy, ((uint64_t)a->sequences + 1) * 4);
     p.stats = take(prefer, a->n * sizeof(RowStats));
     p.logs = take(prefer, a->n * 8);
@@ -132,9 +135,10 @@ int run_loss(const ts_loss_args* a, int op) {
     const LossOut o{a->loss, a->margins, a->logprobs, a->grad, a->grad_stride, a->grad_scale};
     const auto at = [&](uint64_t off) { return static_cast<char*>(a->workspace) + off; };
     LossWork w{};
+    if (p.ordered) w.order = reinterpret_cast<int*>(at(p.order));
     switch (op) {
-        case TS_LOSS_LOGPROBS: return cuda_status(launch_logprobs(r, a->logprobs, a->dtype, s));
-        case TS_LOSS_LOGPROBS_BACKWARD: return cuda_status(launch_logprobs_backward(r, a->grad_logprobs, o, a->dtype, s));
+        case TS_LOSS_LOGPROBS: return cuda_status(launch_logprobs(r, w, a->logprobs, a->dtype, s));
+        case TS_LOSS_LOGPROBS_BACKWARD: return cuda_status(launch_logprobs_backward(r, a->grad_logprobs, w, o, a->dtype, s));
         case TS_LOSS_POLICY: {
             w.counts = reinterpret_cast<int*>(at(p.counts)), w.parts = reinterpret_cast<double*>(at(p.parts));
             w.ticket = reinterpret_cast<unsigned*>(at(p.ticket));
