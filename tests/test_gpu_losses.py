@@ -556,3 +556,74 @@ def test_gradients_against_differences(L):
         size = 1.0 + abs(out[0].item())
         tol = (2.0 ** -23 * size + grad.abs().sum().item() * (rel + 2.0 ** -22)) / h + 3 * size * h * h
         assert abs((up - down) / (2 * h) - (grad * u).sum()) <= tol and tol < 0.05 * (grad * u).sum().abs()
+
+
+# ---------------------------------------------------------------- rows by the hundred, which persistent clusters share
+
+
+def _padded(s, t, v, dt, seed=0):
+    """Sequences of ragged lengths behind prompts, padded: about half of the rows count."""
+    z, y = _rows(s * t, v, dt, seed=seed)
+    z, y = z.view(s, t, v), torch.randint(0, v, (s, t), generator=_gen(seed), device="cuda")
+    at = torch.arange(t, device="cuda")
+    ends = torch.randint(1, t + 1, (s, 1), generator=_gen(seed + 1), device="cuda")
+    prompts = (ends * torch.rand((s, 1), generator=_gen(seed + 2), device="cuda") * 0.6).long()
+    return z, torch.where((at >= prompts) & (at < ends), y, -100)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("s,t,v", [(6, 300, 5003), (40, 31, 9001), (3, 111, 33001), (2, 100, 151936)])
+def test_padded_batches(L, s, t, v, dt):
+    z, y = _padded(s, t, v, dt, seed=s)
+    old, adv, ref = _policy_inputs(z, y)
+    flat, yy = z.view(-1, v), y.view(-1)
+    _near_logprobs(L.token_logprobs(z, y), flat, yy)
+    g = torch.randn((s, t), generator=_gen(7), device="cuda")
+    g[0, :5] = 0.0
+    _near_gradient(L.token_logprobs_backward(g, z, y), flat, yy, g.double().view(-1), torch.zeros_like(g).double().view(-1))
+    out = torch.full_like(z, 7.0)
+    _check_policy(L, z, y, old, adv, ref, kl=0.04, kind="sequence", out=out)
+    if s % 2 == 0:
+        _check_preference(L, z, y, ref, average=True, out=out)
+        _check_preference(L, z, y, ref, kind="squared", beta=0.3, out=z)  # in place
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("count", ["none", "one", "all"])
+def test_batches_in_which_few_or_all_rows_count(L, count, dt):
+    n, v = 1300, 5000
+    z, y = _rows(n, v, dt, seed=3)
+    y = y.clamp_min(0)
+    if count != "all":
+        keep = y[777].item()
+        z[:777], z[778:] = math.nan, math.nan
+        y[:] = -1
+        if count == "one":
+            y[777] = keep
+    adv = torch.ones((n,), device="cuda")
+    loss, logp, grad = L.policy_loss(z, y, None, adv)
+    used = (y >= 0).nonzero()[:, 0]
+    assert loss == (-1 if len(used) else 0) and (logp[y < 0] == 0).all() and (grad[y < 0] == 0).all()
+    _near_logprobs(logp[used], z[used], y[used])
+    one = torch.full((len(used),), -1.0 / max(1, len(used)), dtype=torch.float64, device="cuda")
+    if len(used):
+        _near_gradient(grad[used], z[used], y[used], one, 2.0 ** -24 * one.abs())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 300, 700])
+@pytest.mark.parametrize("v", [2040, 2041, 4088, 4089, 8188, 8189, 16376, 16377, 20472, 20480, 40945, 81920, 163840])
+def test_where_the_kernels_change(L, v, n, dt):
+    """Vocabularies at the lengths that threads, CTAs and clusters can hold."""
+    if n * v > 60e6:
+        n = 150
+    z, y = _rows(n, v + 3, dt, seed=v)
+    z, y = z[:, 3:], y.clamp_max(v - 1)  # rows off 16-byte boundaries
+    g = torch.randn((n,), generator=_gen(8), device="cuda")
+    _near_logprobs(L.token_logprobs(z, y), z, y)
+    _near_gradient(L.token_logprobs_backward(g, z, y), z, y, g.double(), torch.zeros(n, device="cuda").double())
+
+
+def test_no_wait_ran_out():
+    from provenloop_b200 import adapters
+    assert adapters.expired_waits() == 0
