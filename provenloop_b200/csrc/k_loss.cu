@@ -9,7 +9,15 @@
 // row with g = 0 is read for its gradient.
 //
 // The bound is the logits' traffic: each is read once, and its gradient
-// written once.
+// written once.  Rows that fit are held in registers (k_short), of longer ones a
+// persistent cluster keeps what it can in shared memory (k_ring).  On one B200, in bf16
+// over 151936 tokens: 4096 rows' log-probabilities take 197 us (6.3 TB/s), with gradients for
+// given slopes 525 to 543 us (4.7 TB/s; 5.9 with known statistics).  The latter is
+// bound by the two exponentials and some twenty instructions that an element costs: without
+// them the same copies take 370 us.  Tried and slower: exponentials kept in
+// shared memory in 32 bits (570 us: a row's gradient then waits for the next one's
+// statistics), a part of them by polynomials on the FMA pipe (586 us), bulk stores of the
+// gradient (750 us), more statistics warps and fewer for the gradient (600 us and more).
 #include <atomic>
 #include <cfloat>
 
@@ -24,7 +32,6 @@ namespace {
 
 constexpr int kCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-
 
 // What is done with a row that counts: its log-probability; the gradient for
 // a given g; the policy loss; the gradient for known statistics and a g by sequence.
@@ -124,7 +131,7 @@ struct Lane<__half> {
     static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// Pairs of f32 in one instruction.
+// Pairs of f32 in one instruction: the issue slots bound what an element costs.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
     asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
@@ -139,7 +146,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-// exp(a - b) for a <= b, 1 where they are equal.
+// exp(a - b) for a <= b, 1 where they are equal, off by 2^-22 and 2^-22 |a - b|.
+// (a log2(e) - b log2(e) in one FMA would carry b's rounding, and not give 1.)
 __device__ __forceinline__ float weight(float a, float b) { return exp2_fast((a - b) * kLog2e); }
 __device__ __forceinline__ float2 weight2(float2 a, float2 less) {
     const float2 d = mul2(add2(a, less), make_float2(kLog2e, kLog2e));
@@ -180,9 +188,12 @@ __device__ __forceinline__ void see(RowStats& t, const uint4 (&z)[V]) {
     t.sum = fmaf(t.sum, weight(t.max, m), all.x + all.y), t.max = m;
 }
 
+// What the gradient of a row is made of: g, -g / s, the target's logit, m.
 struct Coef {
     float g, by, zy, max;
 };
+
+// -g p of one vector; the target's g is added by fix_target.
 template <class T>
 __device__ __forceinline__ uint4 slope_of(const uint4& z, const Coef& c) {
     constexpr int N = Lane<T>::N;
@@ -196,6 +207,7 @@ __device__ __forceinline__ uint4 slope_of(const uint4& z, const Coef& c) {
     }
     return Lane<T>::close(f);
 }
+// g (1 - p) for the target, by the thread that wrote -g p there.
 template <class T>
 __device__ __forceinline__ void fix_target(T* out, const Coef& c) {
     *out = Lane<T>::put(fmaf(c.by, weight(c.zy, c.max), c.g));
@@ -338,7 +350,7 @@ struct Span {
     }
 };
 
-// The target of a row that counts, else -1.
+// The target of a row that counts (for a given g of 0 it need not), else -1.
 __device__ __forceinline__ int counted(const RowArgs& a, long long row, long long lo, long long hi) {
     if (row < lo || row >= hi) return -1;
     const int y = a.r.target(row);
@@ -430,17 +442,20 @@ __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
 //   S warps take the statistics of a part as it arrives,
 //   one joins them, exchanges them within the cluster and finishes the row,
 //   G warps write the part's gradient once that is known.
-// A part keeps `keep` slots until its gradient is written from them; what there is
+// A part keeps KEEP slots until its gradient is written from them; what there is
 // more of it is copied once more (from L2) behind the rest and before the next
 // row, whose statistics are taken meanwhile.  So a row comes from memory once.
-constexpr uint32_t kSlot = 16384;
-constexpr uint32_t kZeros = 4096;
+// Every wait goes by one of these barriers, in the order of the rows; which it is
+// waiting for is never more than one phase away (test_loss_ring.py has a model).
+constexpr uint32_t kSlot = 16384;  // of half the size, the thread that starts the copies is the bound (4.0 TB/s)
+constexpr uint32_t kZeros = 4096;  // bytes that rows which do not count are written from
 constexpr int kTeam = 8;   // warps that take a slot together, four vectors a lane
 constexpr int kDepth = 4;  // rows between two roles
 constexpr int kStats = 2;  // rows whose lanes' statistics are waiting to be joined
 // The teams of a role take the slots in turn, and every team always the same
-// ones: it has seen a slot's last load when it waits for the next, and a parity
-// wait tells the two apart.  Statistics alone: two CTAs on an SM (4096 rows of
+// ones.  Where there are both roles, a slot is free again when a team of either has
+// arrived, whether the load was for it or not: so no team is more than one load behind, and a
+// parity wait tells the loads apart.  Statistics alone: two CTAs on an SM (4096 rows of
 // 151936 in bf16: 197 us, with one of twice the slots 211).
 template <bool S, bool G>
 struct Roles {
@@ -518,13 +533,14 @@ template <class T, bool S, bool G>
 __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_ring(const RowArgs a) {
     constexpr uint32_t N = Lane<T>::N, SLOT = kSlot / sizeof(T);
     constexpr int TS = Roles<S, G>::TS, TG = Roles<S, G>::TG, SLOTS = Roles<S, G>::SLOTS, KEEP = Roles<S, G>::KEEP;
-    constexpr uint32_t STEP = 32 * N, GROUPS = SLOT / (kTeam * 4 * STEP);  // a lane takes that often four vectors of a slot
+    constexpr uint32_t STEP = 32 * N, PIECE = 4 * STEP;  // elements of a slot that a warp takes
+    static_assert(PIECE * kTeam == SLOT, "a team takes a slot");
     extern __shared__ __align__(128) unsigned char slots[];
     __shared__ RingShared<TS * kTeam * 32> sh;
     const int rank = (int)cluster_rank(), warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
     const int cl = 1 << a.log, cluster = (int)(blockIdx.x >> a.log);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLOTS; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kTeam);
+        for (int i = 0; i < SLOTS; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], S && G ? 2 * kTeam : kTeam);
         for (int i = 0; i < kStats; i++) mbar_init(&sh.stats_full[i], TS * kTeam), mbar_init(&sh.stats_free[i], 1);
         for (int i = 0; i < kDepth; i++) {
             mbar_init(&sh.joined[i], 1);
@@ -633,7 +649,6 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         if (!met) cluster_wait();
     } else if (S && (!G || warp < 2 + TS * kTeam)) {
         const int w = (warp - 2) % kTeam, team = (warp - 2) / kTeam;
-        const uint32_t v0 = (uint32_t)w * GROUPS * 4 * STEP + lane * N;  // this lane's first vector of a slot
         Ring at(SLOTS, 0), k(kStats, 0);
         for (long long b = 0; ok; b++) {
             const Batch rows(a, b, lo, hi, cluster);
@@ -646,42 +661,39 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                     if (at.i % TS != team) continue;
                     ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
                     if (!ok) break;
-                    const T* const from = data + at.i * SLOT + v0;
-                    const uint32_t p0 = sp.first + c * SLOT + v0;
-                    const bool inside = sp.first + c * SLOT >= sp.head && sp.first + (c + 1) * SLOT <= sp.last;
+                    const T* const here = data + at.i * SLOT + w * PIECE + lane * N;  // this lane's first vector
+                    const uint32_t p0 = sp.first + c * SLOT + w * PIECE;
+                    uint4 z[4];
+                    if (p0 >= sp.head && p0 + PIECE <= sp.last) {
 #pragma unroll
-                    for (uint32_t q = 0; q < GROUPS; q++) {
-                        uint4 z[4];
-                        if (inside) {
+                        for (uint32_t j = 0; j < 4; j++) z[j] = *reinterpret_cast<const uint4*>(here + j * STEP);
+                    } else {
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; j++) z[j] = *reinterpret_cast<const uint4*>(from + (q * 4 + j) * STEP);
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; j++) {
-                                const uint32_t p = p0 + (q * 4 + j) * STEP;
-                                z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
-                                       : sp.whole(p) ? *reinterpret_cast<const uint4*>(from + (q * 4 + j) * STEP) : sp.edge(p);
-                            }
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t p = p0 + j * STEP + lane * N;
+                            z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
+                                   : sp.whole(p) ? *reinterpret_cast<const uint4*>(here + j * STEP) : sp.edge(p);
                         }
-                        if (q == GROUPS - 1 && (!G || c < again)) {
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sh.empty[at.i]);
-                        }
-                        see<T, 4>(t, z);
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.empty[at.i]);
+                    if (G && c < again && lane == 0) mbar_arrive(&sh.empty[at.i]);  // in the place of the other role
+                    see<T, 4>(t, z);
                 }
                 ok = ok && warp_wait(&sh.stats_free[k.i], k.phase ^ 1, &sh.dead);
                 if (ok) sh.lane_stats[k.i][(warp - 2) * 32 + lane] = t;
                 __syncwarp();
                 if (lane == 0 && ok) mbar_arrive(&sh.stats_full[k.i]);
-                // what arrives once more is not for this role, but it has to be seen
-                for (int c = 0; c < again && ok; c++, at.next())
-                    if (at.i % TS == team) ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
+                // what arrives once more is not for this role, but it has to be seen before the slot goes on
+                for (int c = 0; c < again && ok; c++, at.next()) {
+                    if (at.i % TS != team) continue;
+                    ok = warp_wait(&sh.full[at.i], at.phase, &sh.dead);
+                    if (lane == 0 && ok) mbar_arrive(&sh.empty[at.i]);
+                }
             }
         }
     } else {
         constexpr int first = 2 + TS * kTeam;
-        constexpr uint32_t PIECE = GROUPS * 4 * STEP;  // elements of a slot that a warp takes
         const int w = (warp - first) % kTeam, team = (warp - first) / kTeam;
         Ring at(SLOTS, 0), k(kDepth, 0);
         for (long long b = 0; ok; b++) {
@@ -728,32 +740,27 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                     const uint32_t p0 = sp.first + q * SLOT + w * PIECE;
                     const bool inside = vec && p0 >= sp.head && p0 + PIECE <= sp.last;
                     T* const to = out + (p0 - sp.head) + lane * N;
+                    uint4 z[4];
 #pragma unroll
-                    for (uint32_t h = 0; h < GROUPS; h++) {
-                        uint4 z[4];
+                    for (uint32_t j = 0; j < 4; j++) {
+                        const uint32_t p = p0 + j * STEP + lane * N;
+                        if (inside || sp.whole(p)) z[j] = *reinterpret_cast<const uint4*>(here + j * STEP);
+                        else if (p < sp.last) z[j] = sp.edge(p);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.empty[at.i]);
+                    if (!zero) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) {
-                            const uint32_t v = (h * 4 + j) * STEP, p = p0 + v + lane * N;
-                            if (inside || sp.whole(p)) z[j] = *reinterpret_cast<const uint4*>(here + v);
-                            else if (p < sp.last) z[j] = sp.edge(p);
-                        }
-                        if (h == GROUPS - 1) {
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sh.empty[at.i]);
-                        }
-                        if (!zero) {
+                        for (uint32_t j = 0; j < 4; j++) z[j] = slope_of<T>(z[j], c);
+                    } else {
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; j++) z[j] = slope_of<T>(z[j], c);
-                        } else {
+                        for (uint32_t j = 0; j < 4; j++) z[j] = make_uint4(0u, 0u, 0u, 0u);
+                    }
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; j++) z[j] = make_uint4(0u, 0u, 0u, 0u);
-                        }
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) {
-                            const uint32_t v = (h * 4 + j) * STEP, p = p0 + v + lane * N;
-                            if (inside) *reinterpret_cast<uint4*>(to + v) = z[j];
-                            else if (p < sp.last) sp.store(out, vec, p, z[j]);
-                        }
+                    for (uint32_t j = 0; j < 4; j++) {
+                        const uint32_t p = p0 + j * STEP + lane * N;
+                        if (inside) *reinterpret_cast<uint4*>(to + j * STEP) = z[j];
+                        else if (p < sp.last) sp.store(out, vec, p, z[j]);
                     }
                     // the target, by the lane that has its vector
                     const uint32_t v = y + sp.head - p0;
@@ -852,7 +859,7 @@ __device__ double block_sum(double v) {
 }
 
 // A pair's lead over the reference, its loss and the slopes of its two
-// sequences.  One CTA for each pair.
+// sequences, in 64 bits: differences of long sums.  One CTA for each pair.
 __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTerms p, const LossWork w, const LossOut o) {
     release_dependents();
     grid_dependency_wait();

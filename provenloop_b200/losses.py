@@ -67,7 +67,7 @@ def policy_loss(logits, targets, old_logprobs, advantages, ref_logprobs=None, st
     rows outside of them do not count.
     old_logprobs, ref_logprobs: float32 of targets' shape; old_logprobs None:
     rho is 1; ref_logprobs None: no KL term.  advantages: float32 of targets' shape or
-    [sequences].  reduction: "token", the mean over all rows that count;
+    [sequences] (where both are the same, by row).  reduction: "token", the mean over all rows that count;
     "sequence", the mean over the sequences of their means (0 where no row counts);
     "sum".  grad_scale: a float32 tensor with one value, which multiplies the
     gradient (not the loss).  out: where the gradient goes, ``logits``
