@@ -845,48 +845,40 @@ __global__ void __launch_bounds__(1024) k_order(const RowArgs a) {
     }
 }
 
-template <int N>
-__device__ double block_sum(double v) {
-    __shared__ double warp_sum[N / 32];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int i = 0; i < N / 32; i++) v += warp_sum[i];
-    return v;
-}
-
 // A pair's lead over the reference, its loss and the slopes of its two
-// sequences, in 64 bits: differences of long sums.  One CTA for each pair.
-__global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTerms p, const LossWork w, const LossOut o) {
+// sequences, in 64 bits: differences of long sums.  One CTA for each pair, half
+// of it for each sequence, so that nothing waits but the loads, once.
+__global__ void __launch_bounds__(512) k_pairs(const LossRows r, const PreferTerms p, const LossWork w, const LossOut o) {
+    constexpr int HALF = 256;
+    __shared__ double sums[16], numbers[16];
     release_dependents();
     grid_dependency_wait();
-    const uint32_t pairs = r.sequences / 2, pair = blockIdx.x;
-    double lead[2];
-    long long counted[2];
-    for (int side = 0; side < 2; side++) {
-        const uint32_t q = pair + side * pairs;
-        const long long lo = r.starts ? max(0ll, (long long)r.starts[q]) : q * r.per;
-        const long long hi = r.starts ? min(r.n, (long long)r.starts[q + 1]) : lo + r.per;
-        double v = 0.0, n = 0.0;
-        for (long long row = lo + threadIdx.x; row < hi; row += 256) {
-            if (r.target(row) < 0) continue;
-            v += w.logs[row] - (p.ref ? (double)p.ref[row] : 0.0);
-            n += 1.0;
-        }
-        lead[side] = block_sum<256>(v);
-        counted[side] = (long long)block_sum<256>(n);
-        if (p.average && counted[side]) lead[side] /= (double)counted[side];
+    const uint32_t pairs = r.sequences / 2, pair = blockIdx.x, q = pair + (threadIdx.x / HALF) * pairs;
+    const int lane = (int)(threadIdx.x & 31);
+    const long long lo = r.starts ? max(0ll, (long long)r.starts[q]) : q * r.per;
+    const long long hi = r.starts ? min(r.n, (long long)r.starts[q + 1]) : lo + r.per;
+    double v = 0.0, n = 0.0;
+#pragma unroll 2
+    for (long long row = lo + threadIdx.x % HALF; row < hi; row += HALF) {
+        const double l = w.logs[row];  // anything where the row does not count
+        const float ref = p.ref ? p.ref[row] : 0.f;
+        if (r.target(row) >= 0) v += l - (double)ref, n += 1.0;
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d), n += __shfl_xor_sync(0xffffffffu, n, d);
+    if (lane == 0) sums[threadIdx.x >> 5] = v, numbers[threadIdx.x >> 5] = n;
+    __syncthreads();
     if (threadIdx.x >= 32) return;
-    const double d = lead[0] - lead[1], h = p.beta * d, e = p.smoothing;
+    v = sums[lane & 15], n = numbers[lane & 15];
+#pragma unroll
+    for (int d = 4; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d), n += __shfl_xor_sync(0xffffffffu, n, d);
+    if (p.average && n > 0.0) v /= n;
+    const double d = __shfl_sync(0xffffffffu, v, 0) - __shfl_sync(0xffffffffu, v, 8), h = p.beta * d, e = p.smoothing;
     double loss, slope;  // by d
     if (p.kind == TS_PREFER_SIGMOID) {
-        // log sigmoid(h) = min(h, 0) - log1p(exp(-|h|)), sigmoid'(h) / sigmoid(h) = sigmoid(-h)
-        const double t = log1p(exp(-fabs(h))), up = 1.0 / (1.0 + exp(-h)), down = 1.0 / (1.0 + exp(h));
-        loss = (1.0 - e) * (t - fmin(h, 0.0)) + e * (t + fmax(h, 0.0));
+        // log sigmoid(h) = min(h, 0) - log(1 + t) and sigmoid(-|h|) = t / (1 + t) with t = exp(-|h|)
+        const double t = exp(-fabs(h)), rest = log1p(t), small = t / (1.0 + t), up = h < 0.0 ? small : 1.0 - small, down = h < 0.0 ? 1.0 - small : small;
+        loss = (1.0 - e) * (rest - fmin(h, 0.0)) + e * (rest + fmax(h, 0.0));
         if (h != h) loss = h;
         slope = p.beta * (e * up - (1.0 - e) * down);
     } else if (p.kind == TS_PREFER_HINGE) {
@@ -897,13 +889,12 @@ __global__ void __launch_bounds__(256) k_pairs(const LossRows r, const PreferTer
         loss = off * off;
         slope = 2.0 * off;
     }
-    if (threadIdx.x == 0) {
+    slope *= (double)(o.grad_scale ? *o.grad_scale : 1.f) / pairs;
+    if (lane == 0) {
         w.parts[pair] = loss;
         if (o.margins) o.margins[pair] = (float)h;
-        slope *= (double)(o.grad_scale ? *o.grad_scale : 1.f) / pairs;
-        w.slope[pair] = (float)(p.average && counted[0] ? slope / counted[0] : slope);
-        w.slope[pair + pairs] = (float)-(p.average && counted[1] ? slope / counted[1] : slope);
     }
+    if (lane == 0 || lane == 8) w.slope[q + (lane ? pairs : 0)] = (float)((lane ? -slope : slope) / (p.average && n > 0.0 ? n : 1.0));
     total(w, (int)pairs, 1.0 / pairs, o.loss);
 }
 
@@ -1061,7 +1052,7 @@ cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const Los
     KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad) + !!w.order);
     cudaError_t e = order(a, s);
     if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, sizeof(unsigned), s);
-    if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 256, 0, s, r, p, w, o);
+    if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 512, 0, s, r, p, w, o);
     a.o.grad = o.grad, a.mode = KNOWN, a.backwards = 1;
     if (e == cudaSuccess && r.n && o.grad) e = rows(a, dtype, true, s);
     return e;
