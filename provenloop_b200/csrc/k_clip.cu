@@ -90,12 +90,12 @@ __device__ __forceinline__ float value(T v) { return (float)v; }
 // overflow or lose what is small.
 template <class T>
 __device__ __forceinline__ double vector_squares(const uint4& z) {
-    constexpr uint32_t N = 16 / sizeof(T);
+    constexpr uint32_t N = 16 / sizeof(T), ABS = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
     const T* e = reinterpret_cast<const T*>(&z);
     float s = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) s = fmaf(value(e[i]), value(e[i]), s);
-    if ((s > 1e-30f && s < 1e37f) || ((z.x | z.y | z.z | z.w) & 0x7fff7fffu) == 0) return s;
+    if ((s > 1e-30f && s < 1e37f) || ((z.x | z.y | z.z | z.w) & ABS) == 0) return s;
     double d = 0.0;
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) d += (double)value(e[i]) * value(e[i]);

@@ -292,23 +292,40 @@ __device__ __forceinline__ void skip_row(const RowArgs& a, long long row) {
     if ((a.mode == LOGPROBS || a.mode == POLICY) && a.o.logprobs) a.o.logprobs[row] = 0.f;
 }
 
-// The loss from its parts in the order of their numbers, by the last warp to
-// get here; the parts are there.
-__device__ __forceinline__ void total(const LossWork& w, int parts, double by, float* out) {
+// The loss from its parts in an order that depends on their number alone: the
+// last warp to come to a group of them adds it up, the last of these the groups.  Part
+// `part` is there.
+__device__ __forceinline__ void total(const LossWork& w, uint32_t part, uint32_t parts, double by, float* out) {
     const int lane = (int)(threadIdx.x & 31);
-    unsigned before = 0;
-    __syncwarp();
-    if (lane == 0) {
+    double* from = w.parts;
+    unsigned* ticket = w.ticket;
+    for (;;) {
+        const uint32_t groups = (uint32_t)loss_groups(parts), group = part / kLossGroup, here = min(kLossGroup, parts - group * kLossGroup);
+        unsigned before = 0;
+        __syncwarp();
+        if (lane == 0) {
+            __threadfence();
+            before = atomicAdd(ticket + group, 1u);
+        }
+        if (__shfl_sync(0xffffffffu, before, 0) != here - 1) return;
         __threadfence();
-        before = atomicAdd(w.ticket, 1u);
-    }
-    if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)parts - 1) return;
-    __threadfence();
-    double v = 0.0;
-    for (int i = lane; i < parts; i += 32) v += __ldcg(w.parts + i);
+        double v = 0.0;
+#pragma unroll 8
+        for (uint32_t i = lane; i < here; i += 32) v += __ldcg(from + group * kLossGroup + i);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) *out = (float)(v * by);
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (groups == 1) {
+            if (lane == 0) *out = (float)(v * by);
+            return;
+        }
+        from += parts, ticket += groups;
+        if (lane == 0) from[group] = v;
+        part = group, parts = groups;
+    }
+}
+// Before any part: none has come yet.  By a whole CTA.
+__device__ __forceinline__ void clear_tickets(const LossWork& w, uint32_t parts) {
+    for (uint64_t i = threadIdx.x; i < loss_tickets(parts); i += blockDim.x) w.ticket[i] = 0u;
 }
 
 // The vector at p of a row (addressed as Span says) by its elements: -inf for
@@ -424,8 +441,8 @@ __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
             }
         }
     }
-    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0 && threadIdx.x == 0) *a.w.ticket = 0u;
-    if (a.mode == POLICY && rank == 0 && threadIdx.x < 32) total(a.w, a.units, 1.0, a.o.loss);
+    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) clear_tickets(a.w, a.r.sequences / 2);
+    if (a.mode == POLICY && rank == 0 && threadIdx.x < 32) total(a.w, (uint32_t)row, (uint32_t)a.units, 1.0, a.o.loss);
     if (!out) return;
 #pragma unroll
     for (uint32_t j = 0; j < V; j++) {
@@ -548,8 +565,8 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         }
         sh.dead = 0;
         mbar_init_fence();
-        if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) *a.w.ticket = 0u;
     }
+    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) clear_tickets(a.w, a.r.sequences / 2);
     if (G && threadIdx.x < kZeros / 16) {
         reinterpret_cast<uint4*>(slots + SLOTS * kSlot)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
         fence_async_shared();
@@ -644,7 +661,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         }
         if (a.mode == POLICY && rank == 0 && ok) {
             if (lane == 0) a.w.parts[cluster] = loss;
-            total(a.w, a.units, 1.0, a.o.loss);
+            total(a.w, (uint32_t)cluster, (uint32_t)a.units, 1.0, a.o.loss);
         }
         if (!met) cluster_wait();
     } else if (S && (!G || warp < 2 + TS * kTeam)) {
@@ -791,10 +808,8 @@ __global__ void __launch_bounds__(1024) k_order(const RowArgs a) {
     const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
     if (policy)
         for (uint32_t i = threadIdx.x; i <= r.sequences; i += 1024) a.w.counts[i] = 0;
-    if (threadIdx.x == 0) {
-        found = 0;
-        if (a.w.ticket) *a.w.ticket = 0u;
-    }
+    if (a.w.ticket) clear_tickets(a.w, policy ? (uint32_t)r.n : r.sequences / 2);
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
     const long long lo = rows_from(r), hi = rows_to(r);
     for (long long at = 0; at < r.n; at += 1024 * EACH) {
@@ -895,7 +910,7 @@ __global__ void __launch_bounds__(512) k_pairs(const LossRows r, const PreferTer
         if (o.margins) o.margins[pair] = (float)h;
     }
     if (lane == 0 || lane == 8) w.slope[q + (lane ? pairs : 0)] = (float)((lane ? -slope : slope) / (p.average && n > 0.0 ? n : 1.0));
-    total(w, (int)pairs, 1.0 / pairs, o.loss);
+    total(w, pair, pairs, 1.0 / pairs, o.loss);
 }
 
 int log2_of(int cl) { return cl == 8 ? 3 : cl / 2; }
@@ -1051,7 +1066,7 @@ cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const Los
     a.o.grad = nullptr;
     KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad) + !!w.order);
     cudaError_t e = order(a, s);
-    if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, sizeof(unsigned), s);
+    if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, loss_tickets(r.sequences / 2) * sizeof(unsigned), s);
     if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 512, 0, s, r, p, w, o);
     a.o.grad = o.grad, a.mode = KNOWN, a.backwards = 1;
     if (e == cudaSuccess && r.n && o.grad) e = rows(a, dtype, true, s);

@@ -55,6 +55,13 @@ struct PreferTerms {
     float beta, smoothing;
 };
 
+// A loss is the sum of its parts by groups of so many, and of the groups.
+constexpr uint32_t kLossGroup = 1024;
+__host__ __device__ constexpr uint64_t loss_groups(uint64_t parts) { return (parts + kLossGroup - 1) / kLossGroup; }
+// Sums for `parts`: those, and the groups' of each level above.
+__host__ __device__ constexpr uint64_t loss_sums(uint64_t parts) { return parts + (parts > kLossGroup ? loss_sums(loss_groups(parts)) : 0); }
+__host__ __device__ constexpr uint64_t loss_tickets(uint64_t parts) { return loss_groups(parts) + (parts > kLossGroup ? loss_tickets(loss_groups(parts)) : 0); }
+
 // What a loss's launches hand to one another, in the workspace.
 struct LossWork {
     int* order;        // [n + 1], or null: loss_orders
@@ -62,8 +69,8 @@ struct LossWork {
     RowStats* stats;   // [n] (preference)
     double* logs;      // [n]: log-probabilities (preference)
     float* slope;      // [sequences]: d loss / d log-probability (preference)
-    double* parts;     // [n] (policy; by cluster or by row), [pairs] (preference): the loss is their sum
-    unsigned* ticket;  // parts that are there
+    double* parts;     // loss_sums(n) (policy; by cluster or by row) or (pairs) (preference)
+    unsigned* ticket;  // loss_tickets(...): parts of each group that are there
 };
 
 struct LossOut {

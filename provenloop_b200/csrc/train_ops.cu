@@ -102,8 +102,9 @@ LossPlan plan_of(const ts_loss_args* a, int op) {
     p.stats = take(prefer, a->n * sizeof(RowStats));
     p.logs = take(prefer, a->n * 8);
     p.slope = take(prefer, (uint64_t)a->sequences * 4);
-    p.parts = take(policy || prefer, (policy ? a->n : a->sequences / 2) * 8);
-    p.ticket = take(policy || prefer, 4);
+    const uint64_t parts = policy ? a->n : a->sequences / 2;
+    p.parts = take(policy || prefer, loss_sums(parts) * 8);
+    p.ticket = take(policy || prefer, loss_tickets(parts) * 4);
     p.bytes = at;
     return p;
 }

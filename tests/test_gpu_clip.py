@@ -172,6 +172,15 @@ def test_norm_beyond_32_bits_is_not_finite(A):
     assert A.clip_gradients([x], 1.0).item() == math.inf and (x == 3e38).all()
 
 
+def test_least_values(A):
+    """Gradients of the types' least values have a norm, and are clipped by it."""
+    for dt, least in ((torch.float32, -149), (torch.float32, -134), (torch.bfloat16, -133), (torch.float16, -24)):
+        t = torch.full((16,), 2.0 ** least, dtype=dt, device="cuda")
+        want = t.double().norm()
+        norm = A.clip_gradients([t], 0.0)
+        assert abs(norm.item() - want.item()) <= 2.0 ** -24 * want.item() + 2.0 ** -150 and (t == 0).all()
+
+
 def test_large_stack(A):
     """A part of more than 2^31 bytes."""
     x = torch.empty((2, 1 << 30), dtype=torch.bfloat16, device="cuda")

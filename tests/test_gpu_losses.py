@@ -624,6 +624,25 @@ def test_where_the_kernels_change(L, v, n, dt):
     _near_gradient(L.token_logprobs_backward(g, z, y), z, y, g.double(), torch.zeros(n, device="cuda").double())
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 4097, 262147, 1050001])
+def test_losses_of_many_rows(L, n):
+    """Losses that are sums of sums: of groups of rows or pairs, and of groups of those."""
+    z, y = _rows(n, 8, "bf16", seed=n)
+    old, adv, ref = _policy_inputs(z, y, per_row=True)
+    for kind in ("token", "sum"):
+        _check_policy(L, z, y, old, adv, ref, kl=0.1, kind=kind)
+    starts = torch.cat([torch.arange(0, n, 7, device="cuda"), torch.tensor([n], device="cuda")]).int()
+    _check_policy(L, z, y, old, adv, None, starts=starts, kind="sequence")
+    # as pairs of single tokens: the loss is the margins' mean form
+    z, y = z[:n // 2 * 2], y[:n // 2 * 2]
+    loss, margins, logp, _ = L.preference_loss(z.view(-1, 1, 8), y.view(-1, 1), beta=0.5)
+    _near_logprobs(logp, z, y)
+    h = 0.5 * (logp[:n // 2].double() - logp[n // 2:].double()).view(-1)
+    _near(margins, h, 2.0 ** -24 * (logp[:n // 2].abs() + logp[n // 2:].abs()).view(-1).double() + 2.0 ** -24 * h.abs(), "margins")
+    want = torch.nn.functional.softplus(-margins.double()).mean()
+    _near(loss.view(1), want.view(1), 2.0 ** -24 * (want.item() + margins.double().abs().mean().item()), "loss")
+
+
 def test_no_wait_ran_out():
     from provenloop_b200 import adapters
     assert adapters.expired_waits() == 0
