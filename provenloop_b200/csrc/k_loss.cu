@@ -9,7 +9,7 @@
 // row with g = 0 is read for its gradient.
 //
 // The bound is the logits' traffic: each is read once, and its gradient
-// written once.  Rows that fit are held in registers (k_short), of longer ones a
+// written once.  Rows that fit are held in registers (k_rows, k_short), of longer ones a
 // persistent cluster keeps what it can in shared memory (k_ring).  On one B200, in bf16
 // over 151936 tokens: 4096 rows' log-probabilities take 197 us (6.3 TB/s), with gradients for
 // given slopes 525 to 543 us (4.7 TB/s; 5.9 with known statistics).  The latter is
@@ -18,6 +18,7 @@
 // shared memory in 32 bits (570 us: a row's gradient then waits for the next one's
 // statistics), a part of them by polynomials on the FMA pipe (586 us), bulk stores of the
 // gradient (750 us), more statistics warps and fewer for the gradient (600 us and more).
+#include <algorithm>
 #include <atomic>
 #include <cfloat>
 
@@ -31,6 +32,7 @@ namespace tsg {
 namespace {
 
 constexpr int kCluster = 8;
+constexpr int kRowWarps = 8;  // of a CTA of k_rows
 constexpr float kLog2e = 1.4426950408889634f;
 
 // What is done with a row that counts: its log-probability; the gradient for
@@ -324,8 +326,8 @@ __device__ __forceinline__ void total(const LossWork& w, uint32_t part, uint32_t
     }
 }
 // Before any part: none has come yet.  By a whole CTA.
-__device__ __forceinline__ void clear_tickets(const LossWork& w, uint32_t parts) {
-    for (uint64_t i = threadIdx.x; i < loss_tickets(parts); i += blockDim.x) w.ticket[i] = 0u;
+__device__ __forceinline__ void clear_tickets(const LossWork& w) {
+    for (uint32_t i = threadIdx.x; i < w.tickets; i += blockDim.x) w.ticket[i] = 0u;
 }
 
 // The vector at p of a row (addressed as Span says) by its elements: -inf for
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
             }
         }
     }
-    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) clear_tickets(a.w, a.r.sequences / 2);
+    if (a.mode == LOGPROBS && blockIdx.x == 0) clear_tickets(a.w);
     if (a.mode == POLICY && rank == 0 && threadIdx.x < 32) total(a.w, (uint32_t)row, (uint32_t)a.units, 1.0, a.o.loss);
     if (!out) return;
 #pragma unroll
@@ -450,6 +452,67 @@ __global__ void __launch_bounds__(THREADS) k_short(const RowArgs a) {
         if (p >= sp.last) continue;
         sp.store(out, vec, p, c.g == 0.f ? make_uint4(0u, 0u, 0u, 0u) : slope_of<T>(z[j], c));
         if (c.g != 0.f && (uint32_t)y + sp.head - p < N) fix_target(out + y, c);
+    }
+}
+
+// Many short rows: a warp to a row, V vectors a lane, and no barriers.
+template <class T, int V>
+__global__ void __launch_bounds__(kRowWarps * 32) k_rows(const RowArgs a) {
+    constexpr uint32_t N = Lane<T>::N;
+    const int lane = (int)(threadIdx.x & 31), unit = (int)(blockIdx.x * kRowWarps + (threadIdx.x >> 5));
+    if (a.mode == LOGPROBS && blockIdx.x == 0) clear_tickets(a.w);
+    const long long lo = rows_from(a.r), hi = rows_to(a.r);
+    const auto row_at = [&](long long i) { return a.backwards ? a.r.n - 1 - i : i; };
+    double loss = 0.0;
+    bool wait = a.wait;
+    int y = unit < a.r.n ? counted(a, row_at(unit), lo, hi) : -1;
+    for (long long i = unit; i < a.r.n; i += a.units) {
+        const long long row = row_at(i);
+        const Span<T> sp(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, 0, 0);
+        uint4 z[V];
+        float zy = 0.f;
+        if (y >= 0) {
+            zy = Lane<T>::one(sp.x[y]);
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) {
+                const uint32_t p = (lane + j * 32) * N;
+                z[j] = p >= sp.last ? make_uint4(Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow, Lane<T>::kLow)
+                       : sp.whole(p) ? *reinterpret_cast<const uint4*>(sp.x + p - sp.head) : sp.edge(p);
+            }
+        }
+        const int next = i + a.units < a.r.n ? counted(a, row_at(i + a.units), lo, hi) : -1;
+        if (wait) grid_dependency_wait(), wait = false;
+        Coef c{0.f, 0.f, 0.f, 0.f};
+        if (y >= 0) {
+            const RowInfo info = row_info(a, row, zy);
+            RowStats s = info.s;
+            if (a.mode != KNOWN) {
+                s = nothing();
+                see<T, V>(s, z);
+                s = join_lanes(s);
+            }
+            c = finish_row(a, info, row, s, lane == 0, &loss);
+        } else if (lane == 0) {
+            skip_row(a, row);
+        }
+        __syncwarp();  // the row may be written now
+        if (a.o.grad) {
+            T* const out = static_cast<T*>(a.o.grad) + row * a.o.grad_stride;
+            const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
+#pragma unroll
+            for (uint32_t j = 0; j < V; j++) {
+                const uint32_t p = (lane + j * 32) * N;
+                if (p >= sp.last) continue;
+                sp.store(out, vec, p, c.g == 0.f ? make_uint4(0u, 0u, 0u, 0u) : slope_of<T>(z[j], c));
+                if (c.g != 0.f && (uint32_t)y + sp.head - p < N) fix_target(out + y, c);
+            }
+        }
+        y = next;
+    }
+    if (a.mode == POLICY && unit < a.units) {
+        if (wait) grid_dependency_wait();
+        if (lane == 0) a.w.parts[unit] = loss;
+        total(a.w, (uint32_t)unit, (uint32_t)a.units, 1.0, a.o.loss);
     }
 }
 
@@ -566,7 +629,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         sh.dead = 0;
         mbar_init_fence();
     }
-    if (a.mode == LOGPROBS && a.w.ticket && blockIdx.x == 0) clear_tickets(a.w, a.r.sequences / 2);
+    if (a.mode == LOGPROBS && blockIdx.x == 0) clear_tickets(a.w);
     if (G && threadIdx.x < kZeros / 16) {
         reinterpret_cast<uint4*>(slots + SLOTS * kSlot)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
         fence_async_shared();
@@ -794,25 +857,27 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     cluster_sync_all();  // no CTA ends while another may still write to its shared memory
 }
 
+constexpr int kOrderRows = 4096;  // of a CTA of k_order at a time
 // Before the rows: how many of them count (policy: by sequence, and all of
 // them), and their order (order[n]: how many count, which come first, the others from
 // the end), so that the clusters get as many.  By every so many-th of a padded batch's
 // rows some had a quarter more than the mean (6144 rows in 16 sequences, 2996 of
-// which count, on two CTAs each: 530 us, in order 506).  One CTA.
+// which count, on two CTAs each: 530 us, in order 506).  One CTA, or without an order several,
+// whose counts then are zeros already.
 __global__ void __launch_bounds__(1024) k_order(const RowArgs a) {
-    constexpr int EACH = 4;
+    constexpr int EACH = kOrderRows / 1024;
     __shared__ int before[32], found;
     release_dependents();
     const LossRows& r = a.r;
-    const bool policy = a.mode == POLICY;
+    const bool policy = a.mode == POLICY, one = gridDim.x == 1;
     const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
-    if (policy)
+    if (policy && one)
         for (uint32_t i = threadIdx.x; i <= r.sequences; i += 1024) a.w.counts[i] = 0;
-    if (a.w.ticket) clear_tickets(a.w, policy ? (uint32_t)r.n : r.sequences / 2);
+    if (blockIdx.x == 0) clear_tickets(a.w);
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
     const long long lo = rows_from(r), hi = rows_to(r);
-    for (long long at = 0; at < r.n; at += 1024 * EACH) {
+    for (long long at = blockIdx.x * 1024ll * EACH; at < r.n; at += gridDim.x * 1024ll * EACH) {
         unsigned any[EACH];
         int mine = 0;
 #pragma unroll
@@ -855,7 +920,8 @@ __global__ void __launch_bounds__(1024) k_order(const RowArgs a) {
         __syncthreads();
     }
     if (threadIdx.x == 0) {
-        if (policy) a.w.counts[r.sequences] = found;
+        if (policy && one) a.w.counts[r.sequences] = found;
+        else if (policy) atomicAdd(a.w.counts + r.sequences, found);
         if (a.w.order) a.w.order[r.n] = found;
     }
 }
@@ -977,12 +1043,24 @@ cudaError_t launch_short(RowArgs a, int cl, bool dependent, cudaStream_t s) {
     return cudaLaunchKernelEx(&l.cfg, k_short<T, THREADS, V>, a);
 }
 
-// The kernel that a call's rows take: k_short with so many threads and CTAs
-// to a row, or (0 threads) k_ring.
+template <class T, int V>
+cudaError_t launch_rows(RowArgs a, bool dependent, cudaStream_t s) {
+    const long long most = (long long)kSms * 64;  // warps that an SM has room for
+    a.units = (int)(a.r.n < most ? a.r.n : most);
+    const Launch l(1, 1, dependent, dim3((unsigned)(a.units + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, k_rows<T, V>, a);
+}
+
+// The kernel that a call's rows take: k_rows (32 threads) with so many vectors a
+// lane, k_short with so many threads and CTAs to a row, or (0 threads) k_ring.
 struct Path {
-    int threads, cl;
+    int threads, cl, vectors;
 };
-// Short rows in registers.  Longer ones too, by a CTA or a cluster, while these run at once, or
+// Short rows in registers, by a warp each if they are many (a CTA to a row is bound by the CTAs' starts,
+// 2.6 ns a row): 262144 rows of 1000 in bf16 scored in 200 us and by a CTA each in 695, with gradients 299 and
+// 803; 100000 rows of 2040, 128 and 275, 213 and 348; 50000 rows of 4080, 101 and 148, 189 and 211.  500 rows
+// of 2040 take the same, 4800 rows of 4080 25 and 21; in f32 a lane holds no 16 vectors (50000 rows of 2040
+// with gradients 235 and 181).  Longer ones too, by a CTA or a cluster, while these run at once, or
 // (gradients of 16-bit types) in three rounds.  In us, so and by k_ring: 24 rows of 151936 in bf16
 // with gradients 9.5 and 15, 120 rows 27 and 28, 200 rows 50 and 42; 24 rows scored 8.7 and 9.9, 48 rows
 // 13 and 11; 5000 rows of 8000 63 and 32.  12 rows in f32 8.6 and 13, with gradients of 24 rows 15 and 15.
@@ -994,6 +1072,9 @@ Path path_of(uint64_t n, uint32_t vocab, bool grad) {
         const uint64_t at_once = kSms * 1024 / threads;
         return n * cl <= (grad && sizeof(T) == 2 ? 3 * at_once : at_once);
     };
+    if (fits(32 * 4 * N, 1)) return {32, 1, 4};
+    if (fits(32 * 8 * N, 1) && n > 8 * kSms) return {32, 1, 8};
+    if (sizeof(T) == 2 && fits(32 * 16 * N, 1) && n > 128 * kSms) return {32, 1, 16};
     if (fits(128 * 4 * N, 1)) return {128, 1};
     if (fits(512 * 4 * N, 1)) return {few(1, 512) ? 512 : 0, 1};
     constexpr int THREADS = sizeof(T) == 2 ? 512 : 1024;
@@ -1006,6 +1087,11 @@ template <class T>
 cudaError_t rows_of(RowArgs a, bool dependent, cudaStream_t s) {
     a.wait = dependent;
     const Path p = path_of<T>((uint64_t)a.r.n, a.r.vocab, a.o.grad != nullptr);
+    if (p.threads == 32) {
+        if (p.vectors == 4) return launch_rows<T, 4>(a, dependent, s);
+        if (sizeof(T) == 4 || p.vectors == 8) return launch_rows<T, 8>(a, dependent, s);
+        return launch_rows<T, sizeof(T) == 4 ? 8 : 16>(a, dependent, s);
+    }
     if (p.threads == 128) return launch_short<T, 128, 4>(a, 1, dependent, s);
     if (p.threads && p.cl == 1) return launch_short<T, 512, 4>(a, 1, dependent, s);
     if (p.threads) return launch_short<T, sizeof(T) == 2 ? 512 : 1024, 5>(a, p.cl, dependent, s);
@@ -1020,7 +1106,13 @@ cudaError_t rows(const RowArgs& a, int dtype, bool dependent, cudaStream_t s) {
 // k_order, where the call needs it.
 cudaError_t order(const RowArgs& a, cudaStream_t s) {
     if (!a.w.order && a.mode != POLICY) return cudaSuccess;
-    k_order<<<1, 1024, 0, s>>>(a);
+    unsigned ctas = 1;
+    if (!a.w.order && a.r.n > 2 * kOrderRows) {
+        ctas = (unsigned)std::min<long long>((a.r.n + kOrderRows - 1) / kOrderRows, kSms);
+        const cudaError_t e = cudaMemsetAsync(a.w.counts, 0, (a.r.sequences + 1ull) * sizeof(int), s);
+        if (e != cudaSuccess) return e;
+    }
+    k_order<<<ctas, 1024, 0, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -1066,7 +1158,7 @@ cudaError_t launch_preference(const LossRows& r, const PreferTerms& p, const Los
     a.o.grad = nullptr;
     KScope ks("preference_loss", s, 1 + (r.n > 0) + (r.n > 0 && o.grad) + !!w.order);
     cudaError_t e = order(a, s);
-    if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, loss_tickets(r.sequences / 2) * sizeof(unsigned), s);
+    if (e == cudaSuccess) e = r.n ? rows(a, dtype, w.order, s) : cudaMemsetAsync(w.ticket, 0, w.tickets * sizeof(unsigned), s);
     if (e == cudaSuccess) e = launch_dependent(1, k_pairs, dim3(r.sequences / 2), 512, 0, s, r, p, w, o);
     a.o.grad = o.grad, a.mode = KNOWN, a.backwards = 1;
     if (e == cudaSuccess && r.n && o.grad) e = rows(a, dtype, true, s);

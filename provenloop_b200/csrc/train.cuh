@@ -25,7 +25,7 @@ struct LossRows {
     }
     // The row's sequence, or -1: it is in none (with `starts` alone).
     __device__ __forceinline__ int sequence(long long row) const {
-        if (!starts) return (int)(row / per);
+        if (!starts) return (int)((uint32_t)row / (uint32_t)per);  // fewer than 2^32 rows
         if (row < starts[0] || row >= starts[sequences]) return -1;
         uint32_t lo = 0, hi = sequences;  // starts[lo] <= row < starts[hi]
         while (hi - lo > 1) {
@@ -59,8 +59,8 @@ struct PreferTerms {
 constexpr uint32_t kLossGroup = 1024;
 __host__ __device__ constexpr uint64_t loss_groups(uint64_t parts) { return (parts + kLossGroup - 1) / kLossGroup; }
 // Sums for `parts`: those, and the groups' of each level above.
-__host__ __device__ constexpr uint64_t loss_sums(uint64_t parts) { return parts + (parts > kLossGroup ? loss_sums(loss_groups(parts)) : 0); }
-__host__ __device__ constexpr uint64_t loss_tickets(uint64_t parts) { return loss_groups(parts) + (parts > kLossGroup ? loss_tickets(loss_groups(parts)) : 0); }
+constexpr uint64_t loss_sums(uint64_t parts) { return parts + (parts > kLossGroup ? loss_sums(loss_groups(parts)) : 0); }
+constexpr uint64_t loss_tickets(uint64_t parts) { return loss_groups(parts) + (parts > kLossGroup ? loss_tickets(loss_groups(parts)) : 0); }
 
 // What a loss's launches hand to one another, in the workspace.
 struct LossWork {
@@ -70,7 +70,8 @@ struct LossWork {
     double* logs;      // [n]: log-probabilities (preference)
     float* slope;      // [sequences]: d loss / d log-probability (preference)
     double* parts;     // loss_sums(n) (policy; by cluster or by row) or (pairs) (preference)
-    unsigned* ticket;  // loss_tickets(...): parts of each group that are there
+    unsigned* ticket;  // [tickets]: parts of each group that are there
+    uint32_t tickets;  // loss_tickets(n) or (pairs), 0 where there is no loss
 };
 
 struct LossOut {

@@ -84,6 +84,7 @@ int check_loss(const ts_loss_args* a, int op) {
 
 struct LossPlan {
     bool ordered;
+    uint32_t tickets;
     uint64_t order, counts, stats, logs, slope, parts, ticket, bytes;
 };
 
@@ -104,7 +105,8 @@ LossPlan plan_of(const ts_loss_args* a, int op) {
     p.slope = take(prefer, (uint64_t)a->sequences * 4);
     const uint64_t parts = policy ? a->n : a->sequences / 2;
     p.parts = take(policy || prefer, loss_sums(parts) * 8);
-    p.ticket = take(policy || prefer, loss_tickets(parts) * 4);
+    p.tickets = (uint32_t)loss_tickets(parts);
+    p.ticket = take(policy || prefer, p.tickets * 4ull);
     p.bytes = at;
     return p;
 }
@@ -142,7 +144,7 @@ int run_loss(const ts_loss_args* a, int op) {
         case TS_LOSS_LOGPROBS_BACKWARD: return cuda_status(launch_logprobs_backward(r, a->grad_logprobs, w, o, a->dtype, s));
         case TS_LOSS_POLICY: {
             w.counts = reinterpret_cast<int*>(at(p.counts)), w.parts = reinterpret_cast<double*>(at(p.parts));
-            w.ticket = reinterpret_cast<unsigned*>(at(p.ticket));
+            w.ticket = reinterpret_cast<unsigned*>(at(p.ticket)), w.tickets = p.tickets;
             const PolicyTerms t{a->old_logprobs, a->ref_logprobs, a->advantages, a->advantage_rows, a->kind, 1.f - a->clip_low, 1.f + a->clip_high, a->kl};
             return cuda_status(launch_policy(r, t, w, o, a->dtype, s));
         }
@@ -150,7 +152,7 @@ int run_loss(const ts_loss_args* a, int op) {
             if (!a->sequences) return cuda_status(cudaMemsetAsync(a->loss, 0, 4, s));
             w.stats = reinterpret_cast<RowStats*>(at(p.stats)), w.slope = reinterpret_cast<float*>(at(p.slope));
             w.logs = reinterpret_cast<double*>(at(p.logs)), w.parts = reinterpret_cast<double*>(at(p.parts));
-            w.ticket = reinterpret_cast<unsigned*>(at(p.ticket));
+            w.ticket = reinterpret_cast<unsigned*>(at(p.ticket)), w.tickets = p.tickets;
             const PreferTerms t{a->ref_logprobs, a->kind, a->average, a->beta, a->smoothing};
             return cuda_status(launch_preference(r, t, w, o, a->dtype, s));
         }

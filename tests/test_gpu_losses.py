@@ -643,6 +643,29 @@ def test_losses_of_many_rows(L, n):
     _near(loss.view(1), want.view(1), 2.0 ** -24 * (want.item() + margins.double().abs().mean().item()), "loss")
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,v", [(2, 5), (1185, 1017), (1185, 2041), (9001, 500), (19001, 1016), (19001, 2040), (18945, 4088)])
+def test_many_short_rows(L, n, v, dt):
+    """As many as a warp, or a CTA, takes each, and more of them than run at once; rows off 16-byte boundaries too."""
+    z, y = _rows(n, v + 3, dt, seed=v)
+    wide, y = torch.empty_like(z), y.clamp_max(v - 1)
+    z, out = z[:, 3:], wide[:, 1:v + 1]  # not the same offset
+    g = torch.randn((n,), generator=_gen(8), device="cuda")
+    g[n // 2] = 0.0
+    _near_logprobs(L.token_logprobs(z, y), z, y)
+    _near_gradient(L.token_logprobs_backward(g, z, y, out=out), z, y, g.double(), torch.zeros(n, device="cuda").double())
+    starts = torch.tensor(sorted([1, n // 3, n // 3, n // 2, n]), dtype=torch.int32, device="cuda")  # ascending with two rows too
+    adv = torch.randn((4,), generator=_gen(9), device="cuda")
+    old, _, ref = _policy_inputs(z, y)
+    for kind in ("token", "sequence"):
+        _check_policy(L, z, y, old, adv, ref, starts=starts, kl=0.1, kind=kind)
+    _check_preference(L, z, y, ref, starts=starts, average=True)
+    mine = z.contiguous()  # the sums' order goes by the rows' offsets from 16-byte boundaries: the same tensor twice
+    want = L.preference_loss(mine, y, ref, starts=starts, average=True)
+    loss, _, _, grad = L.preference_loss(mine, y, ref, starts=starts, average=True, out=mine)
+    assert grad is mine and torch.equal(loss, want[0]) and torch.equal(mine, want[3])
+
+
 def test_no_wait_ran_out():
     from provenloop_b200 import adapters
     assert adapters.expired_waits() == 0
