@@ -330,7 +330,7 @@ int ts_adapter_project(const ts_adapter_args* args);
  * (f16) or 2^-15 (bf16). */
 int ts_adapter_project_backward(const ts_adapter_args* args);
 
-/* Waits within a kernel of ts_adapter_* or ts_logit_rules that ran out (two seconds) on
+/* Waits within a kernel of ts_adapter_*, ts_logit_rules or the losses that ran out (two seconds) on
  * `device` since the library was loaded: 0, unless a kernel or the device is
  * broken; the results of such a call are not complete.  Waits for the device. */
 int ts_expired_waits(int device, uint64_t* out);

@@ -99,7 +99,7 @@ def clip_gradients(grads, max_norm, adapters=None, out=None):
 
 
 def expired_waits(device=None) -> int:
-    """How many waits inside kernels of this module and of ``logits`` have run
+    """How many waits inside kernels of this module, ``logits`` and ``losses`` have run
     out (after two seconds) on ``device`` (default: the current one) since the
     library was loaded.  Anything but 0 means that a kernel or the device is
     broken and that some call's results are incomplete: the calls themselves do
