@@ -50,6 +50,7 @@ struct RowArgs {
     int wait;        // the launch before this one has to be waited for
     int units;       // clusters (k_ring) or rows (k_short)
     int log;         // of the CTAs in a cluster
+    int own_order;   // the CTAs put the rows in order by themselves
 };
 
 __device__ __forceinline__ float exp2_fast(float v) {
@@ -373,7 +374,8 @@ struct Span {
 __device__ __forceinline__ int counted(const RowArgs& a, long long row, long long lo, long long hi) {
     if (row < lo || row >= hi) return -1;
     const int y = a.r.target(row);
-    return y >= 0 && a.mode == GIVEN && a.g[row] == 0.f ? -1 : y;
+    const float g = a.mode == GIVEN ? a.g[row] : 1.f;  // at once with the target
+    return g == 0.f ? -1 : y;
 }
 __device__ __forceinline__ long long rows_from(const LossRows& r) { return r.starts ? max(0ll, (long long)r.starts[0]) : 0ll; }
 __device__ __forceinline__ long long rows_to(const LossRows& r) { return r.starts ? min(r.n, (long long)r.starts[r.sequences]) : r.n; }
@@ -531,6 +533,7 @@ constexpr uint32_t kSlot = 16384;  // of half the size, the thread that starts t
 constexpr uint32_t kZeros = 4096;  // bytes that rows which do not count are written from
 constexpr int kTeam = 8;   // warps that take a slot together, four vectors a lane
 constexpr int kDepth = 4;  // rows between two roles
+constexpr int kOwnOrder = 2048;  // rows that the CTAs put in order by themselves
 constexpr int kStats = 2;  // rows whose lanes' statistics are waiting to be joined
 // The teams of a role take the slots in turn, and every team always the same
 // ones.  Where there are both roles, a slot is free again when a team of either has
@@ -575,38 +578,53 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
     return __all_sync(0xffffffffu, sleep_wait(bar, parity, dead));
 }
 
+// Before a thread says that it has read a slot: the next copy into it is of
+// another proxy, which the arrival at a barrier alone does not order with loads that have
+// not come back yet (they met the next row's elements in one row of 13000).
+__device__ __forceinline__ void reads_done() { fence_async_shared(); }
+
+// The rows that count, and behind them from the end the others: by k_order, by
+// the CTA itself, or as they come.
+struct Order {
+    uint16_t own[kOwnOrder];  // if a.own_order
+    int counts[32], count;
+    __device__ __forceinline__ int at(const RowArgs& a, int i) const { return a.own_order ? own[i] : a.w.order[i]; }
+};
+
 // The next 32 of a cluster's rows, one a lane.  Of rows in order, every so
 // many-th that counts and every so many-th other one, evenly mixed: the others only
 // write, which costs next to nothing beside those that compute.
 struct Batch {
-    long long row = 0;
-    int y = -1;
+    int row = 0, y = -1;
     uint32_t rows, counts;  // lanes that have a row; whose row counts
-    __device__ __forceinline__ Batch(const RowArgs& a, long long b, long long lo, long long hi, int cluster) {
-        const long long t = b * 32 + (threadIdx.x & 31);
+    __device__ __forceinline__ Batch(const RowArgs& a, const Order& o, int b, int lo, int hi, int cluster) {
+        const int t = b * 32 + (int)(threadIdx.x & 31), n = (int)a.r.n;
         bool there;
-        if (a.w.order) {
-            const long long m = a.w.order[a.r.n], other = a.units - 1 - cluster;
-            const long long mine = m > cluster ? (m - cluster - 1) / a.units + 1 : 0, rest = a.r.n - m > other ? (a.r.n - m - other - 1) / a.units + 1 : 0;
+        if (a.own_order || a.w.order) {
+            const int other = a.units - 1 - cluster;
+            const int mine = o.count > cluster ? (o.count - cluster - 1) / a.units + 1 : 0;
+            const int rest = n - o.count > other ? (n - o.count - other - 1) / a.units + 1 : 0;
             there = t < mine + rest;
             if (there) {
-                const long long before = t * mine / (mine + rest);
-                if ((t + 1) * mine / (mine + rest) > before) {
-                    row = a.w.order[cluster + (a.backwards ? mine - 1 - before : before) * a.units];
+                const int before = (int)((long long)t * mine / (mine + rest));
+                if ((int)((t + 1ll) * mine / (mine + rest)) > before) {
+                    row = o.at(a, cluster + (a.backwards ? mine - 1 - before : before) * a.units);
                     y = a.r.target(row);
                 } else {
-                    row = a.w.order[a.r.n - 1 - (other + (t - before) * a.units)];
+                    row = o.at(a, n - 1 - (other + (t - before) * a.units));
                 }
             }
         } else {
-            const long long i = t * a.units + cluster;
-            there = i < a.r.n;
-            row = a.backwards ? a.r.n - 1 - i : i;
-            if (there) y = counted(a, row, lo, hi);
+            const long long i = (long long)t * a.units + cluster;
+            there = i < n;
+            if (there) {
+                row = a.backwards ? n - 1 - (int)i : (int)i;
+                y = counted(a, row, lo, hi);
+            }
         }
         rows = __ballot_sync(0xffffffffu, there), counts = __ballot_sync(0xffffffffu, y >= 0);
     }
-    __device__ __forceinline__ long long row_of(int lane) const { return __shfl_sync(0xffffffffu, row, lane); }
+    __device__ __forceinline__ int row_of(int lane) const { return __shfl_sync(0xffffffffu, row, lane); }
 };
 
 template <class T, bool S, bool G>
@@ -617,6 +635,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     static_assert(PIECE * kTeam == SLOT, "a team takes a slot");
     extern __shared__ __align__(128) unsigned char slots[];
     __shared__ RingShared<TS * kTeam * 32> sh;
+    __shared__ Order order;
     const int rank = (int)cluster_rank(), warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
     const int cl = 1 << a.log, cluster = (int)(blockIdx.x >> a.log);
     if (threadIdx.x == 0) {
@@ -634,11 +653,40 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         reinterpret_cast<uint4*>(slots + SLOTS * kSlot)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
         fence_async_shared();
     }
+    const int lo = (int)rows_from(a.r), hi = (int)rows_to(a.r);
+    if (a.own_order) {
+        constexpr int W = Roles<S, G>::THREADS / 32, EACH = (kOwnOrder / 32 + W - 1) / W;
+        int y[EACH];
+        unsigned any[EACH];
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const int row = (warp * EACH + j) * 32 + lane;
+            y[j] = row < a.r.n ? counted(a, row, lo, hi) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < EACH; j++) any[j] = __ballot_sync(0xffffffffu, y[j] >= 0), mine += __popc(any[j]);
+        if (lane == 0) order.counts[warp] = mine;
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int w = 0; w < W; w++) {
+            if (w == warp) before = all;
+            all += order.counts[w];
+        }
+        if (threadIdx.x == 0) order.count = all;
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const int row = (warp * EACH + j) * 32 + lane, in_front = before + __popc(any[j] & ((1u << lane) - 1));
+            if (row < a.r.n) order.own[any[j] >> lane & 1 ? in_front : (int)a.r.n - 1 - (row - in_front)] = (uint16_t)row;
+            before += __popc(any[j]);
+        }
+    } else if (a.w.order) {
+        if (a.wait) grid_dependency_wait();
+        if (threadIdx.x == 0) order.count = a.w.order[a.r.n];
+    }
     __syncthreads();
     cluster_arrive();  // waited for before the first access to another CTA's shared memory
-    if (a.w.order && a.wait) grid_dependency_wait();
-    const long long lo = rows_from(a.r), hi = rows_to(a.r);
-    const auto span_of = [&](long long row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, a.log); };
+    const auto span_of = [&](int row) { return Span<T>(static_cast<const T*>(a.r.logits) + row * a.r.stride, a.r.vocab, rank, a.log); };
     const auto chunks_of = [](const Span<T>& sp) { return (int)((sp.last - sp.first + SLOT - 1) / SLOT); };
     T* const data = reinterpret_cast<T*>(slots);
     T* const zeros = data + SLOTS * SLOT;  // kZeros bytes of them
@@ -647,8 +695,8 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
 
     if (warp == 0) {
         Ring at(SLOTS, 1);
-        for (long long b = 0; ok; b++) {
-            const Batch rows(a, b, lo, hi, cluster);
+        for (int b = 0; ok; b++) {
+            const Batch rows(a, order, b, lo, hi, cluster);
             if (!rows.rows) break;
             for (uint32_t left = rows.counts; left && ok; left &= left - 1) {
                 const Span<T> sp = span_of(rows.row_of(__ffs(left) - 1));
@@ -672,8 +720,8 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         double loss = 0.0;
         bool met = false;
         if (a.wait && !a.w.order) grid_dependency_wait();
-        for (long long b = 0; ok; b++) {
-            const Batch rows(a, b, lo, hi, cluster);
+        for (int b = 0; ok; b++) {
+            const Batch rows(a, order, b, lo, hi, cluster);
             if (!rows.rows) break;
             RowInfo mine{};
             if (rows.y >= 0) mine = row_info(a, rows.row, Lane<T>::one((static_cast<const T*>(a.r.logits) + rows.row * a.r.stride)[rows.y]));
@@ -730,8 +778,8 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
     } else if (S && (!G || warp < 2 + TS * kTeam)) {
         const int w = (warp - 2) % kTeam, team = (warp - 2) / kTeam;
         Ring at(SLOTS, 0), k(kStats, 0);
-        for (long long b = 0; ok; b++) {
-            const Batch rows(a, b, lo, hi, cluster);
+        for (int b = 0; ok; b++) {
+            const Batch rows(a, order, b, lo, hi, cluster);
             if (!rows.rows) break;
             for (uint32_t left = rows.counts; left && ok; left &= left - 1, k.next()) {
                 const Span<T> sp = span_of(rows.row_of(__ffs(left) - 1));
@@ -755,6 +803,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                                    : sp.whole(p) ? *reinterpret_cast<const uint4*>(here + j * STEP) : sp.edge(p);
                         }
                     }
+                    reads_done();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.empty[at.i]);
                     if (G && c < again && lane == 0) mbar_arrive(&sh.empty[at.i]);  // in the place of the other role
@@ -776,12 +825,12 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
         constexpr int first = 2 + TS * kTeam;
         const int w = (warp - first) % kTeam, team = (warp - first) / kTeam;
         Ring at(SLOTS, 0), k(kDepth, 0);
-        for (long long b = 0; ok; b++) {
-            const Batch rows(a, b, lo, hi, cluster);
+        for (int b = 0; ok; b++) {
+            const Batch rows(a, order, b, lo, hi, cluster);
             if (!rows.rows) break;
             for (uint32_t left = rows.rows; left && ok; left &= left - 1) {
                 const int of = __ffs(left) - 1;
-                const long long row = rows.row_of(of);
+                const int row = rows.row_of(of);
                 const Span<T> sp = span_of(row);
                 T* const out = static_cast<T*>(a.o.grad) + row * a.o.grad_stride;
                 const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(sp.x) % 16;
@@ -827,6 +876,7 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                         if (inside || sp.whole(p)) z[j] = *reinterpret_cast<const uint4*>(here + j * STEP);
                         else if (p < sp.last) z[j] = sp.edge(p);
                     }
+                    reads_done();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.empty[at.i]);
                     if (!zero) {
@@ -1025,13 +1075,14 @@ cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
         int most = 1;
         e = clusters_at_once<T, S, G>(c, &most);
         if (e != cudaSuccess) return e;
-        const double kib = (double)a.r.vocab * sizeof(T) / c / 1024, l2 = most * kib * c / 1024;
+        const double kib = (double)a.r.vocab * sizeof(T) / c / 1024;
         double row = !G ? 1.2 + 0.042 * kib : !S ? 1.3 + 0.047 * kib : sizeof(T) == 2 ? 1.5 + 0.055 * kib : 1.1 + (kib > 96 ? 0.05 : 0.04) * kib;
-        if (S && G && kib > 170) row *= sizeof(T) == 4 && l2 > 64 ? 1.3 : 1.15;
+        if (S && G && kib > 170) row *= sizeof(T) == 4 ? 1.3 : 1.15;
         const double cost = (double)((a.r.n + most - 1) / most) * row;
         if (c == 1 || cost < least) cl = c, least = cost, a.units = (int)(a.r.n < most ? a.r.n : most);
     }
     a.log = log2_of(cl);
+    a.own_order = !a.w.order && a.r.n > a.units && a.r.n <= kOwnOrder;
     const Launch l(cl, 1, dependent, dim3((unsigned)(a.units * cl)), R::THREADS, R::SMEM, s);
     return cudaLaunchKernelEx(&l.cfg, k_ring<T, S, G>, a);
 }
@@ -1119,7 +1170,7 @@ cudaError_t order(const RowArgs& a, cudaStream_t s) {
 }  // namespace
 
 bool loss_orders(uint64_t n, uint32_t vocab, int dtype, bool grad, bool both) {
-    if (n <= 8ull * kSms) return false;
+    if (n <= (uint64_t)kOwnOrder) return false;
     const auto ring = [&](bool with) { return (dtype == DT_F32 ? path_of<float>(n, vocab, with) : path_of<__half>(n, vocab, with)).threads == 0; };
     return ring(grad) || (both && ring(false));
 }

@@ -666,6 +666,23 @@ def test_many_short_rows(L, n, v, dt):
     assert grad is mine and torch.equal(loss, want[0]) and torch.equal(mine, want[3])
 
 
+@pytest.mark.parametrize("n,v,dt", [(18945, 4088, "fp32"), (6000, 8000, "bf16"), (3000, 20000, "fp16"), (2000, 50257, "fp32"), (900, 151936, "bf16")])
+def test_same_bits_however_the_copies_arrive(L, n, v, dt):
+    """Many rows through the slots of a ring, many times: each load of a slot is done before the next copy into it."""
+    z, y = _rows(n, v, dt, seed=n)
+    adv = torch.randn((n,), generator=_gen(1), device="cuda")
+    starts = torch.tensor([1, n // 3, n // 3, n // 2, n], dtype=torch.int32, device="cuda")
+
+    def everything():
+        return (L.token_logprobs(z, y), L.token_logprobs_backward(adv, z, y), *L.policy_loss(z, y, None, adv),
+                *L.preference_loss(z, y, starts=starts, average=True))
+
+    want = everything()
+    _near_logprobs(want[0][:300], z[:300], y[:300])
+    bad = sum((~(a == b)).sum() for _ in range(20) for a, b in zip(everything(), want))
+    assert bad == 0
+
+
 def test_no_wait_ran_out():
     from provenloop_b200 import adapters
     assert adapters.expired_waits() == 0
