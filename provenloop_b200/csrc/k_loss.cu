@@ -533,7 +533,11 @@ constexpr uint32_t kSlot = 16384;  // of half the size, the thread that starts t
 constexpr uint32_t kZeros = 4096;  // bytes that rows which do not count are written from
 constexpr int kTeam = 8;   // warps that take a slot together, four vectors a lane
 constexpr int kDepth = 4;  // rows between two roles
-constexpr int kOwnOrder = 2048;  // rows that the CTAs put in order by themselves
+// Rows that the CTAs put in order by themselves, each for itself before its first copy, where
+// k_order would be another launch to wait for.  As they come, in order by k_order, and so (us, with gradients):
+// 1001 rows of 151936 in bf16, 615 of which count, 140, 119 and 118; 600, 296 of which, 83, 70 and 69; 1100 rows that
+// all count 160, 165 and 163; 909 rows of 50257 in f32, 391 of which, 63, 66 and 64.
+constexpr int kOwnOrder = 2048;
 constexpr int kStats = 2;  // rows whose lanes' statistics are waiting to be joined
 // The teams of a role take the slots in turn, and every team always the same
 // ones.  Where there are both roles, a slot is free again when a team of either has
@@ -1062,7 +1066,8 @@ cudaError_t clusters_at_once(int cl, int* out) {
 // fastest on one CTA from 300 rows on, on four for few.)  A part of more than
 // half of the slots overlaps less with the next row's.  What a part has beyond the
 // slots that it keeps is read again, and not always found in L2: 6144 rows of 151936, half of which
-// are only written, take 600 us on one CTA each and 506 on two.
+// are only written, take 600 us on one CTA each and 506 on two; 1001 rows in f32, 623 of which count, 233 on
+// one, 216 on two and 183 on four.
 template <class T, bool S, bool G>
 cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
     using R = Roles<S, G>;

@@ -81,8 +81,8 @@ struct LossOut {
     const float* grad_scale;
 };
 
-// Whether the rows are put in order first: those of persistent clusters, if each has many
-// (909 rows, 383 of which count: 81 us as they are, 90 in order).
+// Whether k_order puts the rows in order first: those of persistent clusters, if they are more
+// than the CTAs do by themselves.
 // both: a call that goes over them once without a gradient too.
 bool loss_orders(uint64_t n, uint32_t vocab, int dtype, bool grad, bool both);
 cudaError_t launch_logprobs(const LossRows& r, const LossWork& w, float* logprobs, int dtype, cudaStream_t s);
