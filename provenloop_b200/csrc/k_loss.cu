@@ -896,9 +896,10 @@ __global__ void __launch_bounds__(Roles<S, G>::THREADS, Roles<S, G>::CTAS) k_rin
                         if (inside) *reinterpret_cast<uint4*>(to + j * STEP) = z[j];
                         else if (p < sp.last) sp.store(out, vec, p, z[j]);
                     }
-                    // the target, by the lane that has its vector
+                    // the target, by the lane that has its vector; a last slot reaches into the next CTA's part, whose
+                    // target it must not touch: in place, that CTA may not have read the logit yet
                     const uint32_t v = y + sp.head - p0;
-                    if (!zero && v < PIECE && v % STEP / N == (uint32_t)lane) fix_target(out + y, c);
+                    if (!zero && v < PIECE && y + sp.head < sp.last && v % STEP / N == (uint32_t)lane) fix_target(out + y, c);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.coef_free[k.i]);
