@@ -1014,7 +1014,8 @@ __global__ void __launch_bounds__(512) k_pairs(const LossRows r, const PreferTer
     if (p.kind == TS_PREFER_SIGMOID) {
         // log sigmoid(h) = min(h, 0) - log(1 + t) and sigmoid(-|h|) = t / (1 + t) with t = exp(-|h|)
         const double t = exp(-fabs(h)), rest = log1p(t), small = t / (1.0 + t), up = h < 0.0 ? small : 1.0 - small, down = h < 0.0 ? 1.0 - small : small;
-        loss = (1.0 - e) * (rest - fmin(h, 0.0)) + e * (rest + fmax(h, 0.0));
+        loss = (1.0 - e) * (rest - fmin(h, 0.0));
+        if (e > 0.0) loss += e * (rest + fmax(h, 0.0));  // 0, and not 0 times infinity, where h is infinite
         if (h != h) loss = h;
         slope = p.beta * (e * up - (1.0 - e) * down);
     } else if (p.kind == TS_PREFER_HINGE) {
