@@ -149,12 +149,50 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-// exp(a - b) for a <= b, 1 where they are equal, off by 2^-22 and 2^-22 |a - b|.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+// The greater one, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// exp(a - b) for a <= b, 1 where they are equal, as 2^t with t = d log2(e), d = a - b.
 // (a log2(e) - b log2(e) in one FMA would carry b's rounding, and not give 1.)
+// t's rounding and constant make it off by 2^-22 + 2^-22 |d|.  In a row's sum that counts by the
+// weight itself, exp(d) |d| at most; results below 2^-126 are 0.
 __device__ __forceinline__ float weight(float a, float b) { return exp2_fast((a - b) * kLog2e); }
 __device__ __forceinline__ float2 weight2(float2 a, float2 less) {
     const float2 d = mul2(add2(a, less), make_float2(kLog2e, kLog2e));
     return make_float2(exp2_fast(d.x), exp2_fast(d.y));
+}
+// The same for an element of the gradient, which hangs on its own exponential.  In 16 bits the
+// error is lost in the result's rounding (at |d| = 30 a five hundredth of half a step of bf16, a
+// sixtieth of fp16's); in f32 it would be most of what the result is off (2^-19 at |d| = 40).
+// There 2^t is multiplied by exp(d - t ln 2), 1 + (d - t ln 2) in 32 bits since t's
+// rounding is all that is left, and found by one FMA: off by 2^-21 and 2^-28 |d|, beside d's own
+// 2^-24 |d|.  Gradients of 300 rows of 50257 (deviation 3) are so off by 3.5e-7 of themselves (root
+// of the mean square), without it 5.2e-7; it costs 3 % (1500 rows of 151936: 385 and 375 us).  The
+// rows' sums with it: log-probabilities no nearer (3.3e-7 and 3.2e-7), 2 to 5 % slower.
+constexpr float kLn2 = 0.69314718f, kLeastExp = -128.f;  // exp of the latter is 0 here; an infinite d would give NaN
+template <class T>
+__device__ __forceinline__ float grad_weight(float a, float b) {
+    if constexpr (sizeof(T) == 2) return weight(a, b);
+    const float d = max_nan(a - b, kLeastExp), t = __fmul_rn(d, kLog2e), e = exp2_fast(t);
+    return fmaf(e, fmaf(t, -kLn2, d), e);
+}
+template <class T>
+__device__ __forceinline__ float2 grad_weight2(float2 a, float2 less) {
+    if constexpr (sizeof(T) == 2) return weight2(a, less);
+    float2 d = add2(a, less);
+    d = make_float2(max_nan(d.x, kLeastExp), max_nan(d.y, kLeastExp));
+    const float2 t = mul2(d, make_float2(kLog2e, kLog2e)), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+    return fma2(e, fma2(t, make_float2(-kLn2, -kLn2), d), e);
 }
 
 // Of a warp's lanes, the same bits in all of them.
@@ -205,7 +243,7 @@ __device__ __forceinline__ uint4 slope_of(const uint4& z, const Coef& c) {
     Lane<T>::open(z, f);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float2 p = mul2(weight2(make_float2(f[i], f[i + 1]), less), by);
+        const float2 p = mul2(grad_weight2<T>(make_float2(f[i], f[i + 1]), less), by);
         f[i] = p.x, f[i + 1] = p.y;
     }
     return Lane<T>::close(f);
@@ -213,7 +251,7 @@ __device__ __forceinline__ uint4 slope_of(const uint4& z, const Coef& c) {
 // g (1 - p) for the target, by the thread that wrote -g p there.
 template <class T>
 __device__ __forceinline__ void fix_target(T* out, const Coef& c) {
-    *out = Lane<T>::put(fmaf(c.by, weight(c.zy, c.max), c.g));
+    *out = Lane<T>::put(fmaf(c.by, grad_weight<T>(c.zy, c.max), c.g));
 }
 
 // log s: the exponent's part in 64 bits, so that what is left has an error of 2^-24.

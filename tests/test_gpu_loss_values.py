@@ -48,3 +48,39 @@ def test_preference_loss_of_masked_targets(L, kind, smoothing, average, dt):  # 
         want = torch.stack([torch.full((t,), g), torch.full((t,), -g)]).to(p)[:, :, None] * (torch.nn.functional.one_hot(y[one], v) - p)
         # p by 2^-17 of itself (sums of a row and distances up to 20), the type's rounding, fp16's least values
         assert ((grad.double() - want).abs() <= torch.finfo(z.dtype).eps / 2 * want.abs() + 2.0 ** -17 * abs(g) * p + 2.0 ** -24 * abs(g) + 2.0 ** -25).all()
+
+
+# ---------------------------------------------------------------- f32: as near as 32 bits allow
+
+
+@pytest.mark.parametrize("n,v", [(1, 40), (3, 2041), (40, 9001), (3, 151936), (300, 20000), (40, 400003)])
+def test_exponentials_far_from_the_maximum(L, n, v):  # noqa: F811
+    """Gradients of f32 logits, which are multiples of 1/8 here, so that their differences are exact: warps,
+    CTAs and clusters to a row, and the ring.
+
+    -g p is an exp by ex2.approx (2^-22), corrected by a constant's 2^-28 |d| and rounded (2^-24), times -g / s,
+    rounded (2^-24).  The rest is s, which all of a row's elements share: their quotients by p lie within those
+    3 2^-23 + 80 2^-28 of one value.  s >= 1 is a sum of the maximum's 1 and of exps off by 2^-22 (1 + |d|) each, and
+    of additions that are off by half a step of s, 2^-24 of it, each.  Those that the 1 goes through: six in a
+    group of 16 elements, one for each later group of the thread (of 256 threads or more), and at most 42 for the
+    warps, lanes and CTAs.  -g / s is off by 2^-24 more."""
+    g = _gen(v)
+    z = -torch.randint(80, 640, (n, v), generator=g, device="cuda").float() / 8  # 10 to 80 below the maximum
+    y = torch.randint(0, v, (n,), generator=g, device="cuda")
+    top = torch.randint(0, v, (n,), generator=g, device="cuda")
+    z[torch.arange(n, device="cuda"), top] = 0.0
+    grad = L.token_logprobs_backward(torch.ones(n, device="cuda"), z, y)
+    logp = L.token_logprobs(z, y)
+    d = z.double()
+    s = torch.exp(d).sum(1, keepdim=True)
+    p = torch.exp(d) / s
+    exp_off = 3 * 2.0 ** -23 + 80 * 2.0 ** -28
+    s_off = (p * torch.where(d < 0, 1 - d, 0.0)).sum(1, keepdim=True) * 2.0 ** -22 + (v / 4096 + 48) * 2.0 ** -24
+    off = torch.arange(v, device="cuda") != y[:, None]
+    by = -grad.double() / p
+    assert ((by - 1).abs() <= s_off + 2.0 ** -24 + exp_off)[off].all()
+    high, low = torch.where(off, by, 0.0).amax(1), torch.where(off, by, 2.0).amin(1)
+    assert (high - low <= 2 * exp_off * high).all()
+    at = torch.arange(n, device="cuda")
+    want = d[at, y] - s.log()[:, 0]
+    assert ((logp.double() - want).abs() <= 2.0 ** -24 * want.abs() + s_off[:, 0] + 2.0 ** -24).all()
