@@ -84,3 +84,47 @@ def test_exponentials_far_from_the_maximum(L, n, v):  # noqa: F811
     at = torch.arange(n, device="cuda")
     want = d[at, y] - s.log()[:, 0]
     assert ((logp.double() - want).abs() <= 2.0 ** -24 * want.abs() + s_off[:, 0] + 2.0 ** -24).all()
+
+
+# ---------------------------------------------------------------- the policy loss's ratio and KL term: 64 bits
+
+
+def _two(n, dt="fp32"):
+    """Logits of two tokens that are alike: every log-probability is -log 2, every probability a half."""
+    z = torch.randn((n, 1), generator=_gen(5), device="cuda").to(TYPES[dt]).expand(n, 2).contiguous()
+    return z, torch.randint(0, 2, (n,), generator=_gen(6), device="cuda")
+
+
+def _row_by_row(L, n, one, want, slope):
+    """Each row's loss by a call of its own, and all gradients by one.  The loss and g are
+    rounded to 32 bits (2^-24), g p and g - g p too."""
+    z, y = _two(n)
+    for i in range(n):
+        assert abs(L.policy_loss(z[i:i + 1], y[i:i + 1], reduction="sum", need_grad=False, **one(slice(i, i + 1)))[0].double() - want[i]) <= 2.0 ** -23.99 * want[i].abs()
+    grad = L.policy_loss(z, y, reduction="sum", **one(slice(0, n)))[2].double()
+    sign = torch.where(torch.arange(2, device="cuda") == y[:, None], 0.5, -0.5)
+    assert ((grad - slope[:, None] * sign).abs() <= 2.0 ** -22.9 * 0.5 * slope[:, None].abs()).all()
+
+
+def test_policy_ratios_in_64_bits(L):  # noqa: F811
+    """Ratios between exp(-60) and exp(60) that nothing clips."""
+    n = 48
+    old = -math.log(2) - 60 * (2 * torch.rand((n,), generator=_gen(7), device="cuda") - 1)
+    rho = torch.exp(-math.log(2) - old.double())
+    adv = torch.where(rho > 1, -1.0, 1.0).float()  # a ratio above 1 counts whole where it harms, one below where it helps
+    _row_by_row(L, n, lambda at: dict(old_logprobs=old[at], advantages=adv[at]), -rho * adv, -rho * adv)
+
+
+def test_policy_divergence_in_64_bits(L):  # noqa: F811
+    """exp(d) - 1 - d on both sides of the place where its series takes over, and far off."""
+    d = torch.tensor([1e-6, -3e-4, 0.01, -0.1, 0.2, 0.249, 0.251, -0.249, -0.251, 0.26, 0.3, -0.3, 0.5, -0.7, 1.0, -2.0, 5.0, -9.0, 30.0, -50.0], device="cuda")
+    ref = -math.log(2) + d
+    d = ref.double() + math.log(2)
+    # exp(d) - 1 - d as a sum of its series' terms where it cancels
+    want, term = torch.zeros_like(d), d.clone()
+    for k in range(2, 60):
+        term = term * d / k
+        want += term
+    want = torch.where(d.abs() < 2, want, torch.expm1(d) - d)
+    zero = torch.zeros(len(d), device="cuda")
+    _row_by_row(L, len(d), lambda at: dict(old_logprobs=None, advantages=zero[at], ref_logprobs=ref[at], kl=0.5), 0.5 * want, -0.5 * torch.expm1(d))
