@@ -1,8 +1,13 @@
 """GPU checks of the losses on rows that clusters of CTAs share."""
+import os
+import re
+
 import pytest
 import torch
 
-from tests.test_gpu_losses import TYPES, L, _device, _gen  # noqa: F401
+from provenloop_b200 import build
+from tests.test_gpu_losses import (TYPES, L, _check_policy, _check_preference, _device, _gen, _near_gradient, _near_logprobs,  # noqa: F401
+                                   _padded, _policy_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +38,26 @@ def test_gradient_in_place_with_targets_behind_a_part(L, dt, n, v):  # noqa: F81
         mine = z.clone()
         again, _, _, grad = L.preference_loss(mine, y, beta=0.01, average=True, out=mine)
         assert grad is mine and torch.equal(again, loss) and torch.equal(mine, want)
+
+
+with open(os.path.join(build.CSRC, "k_loss.cu")) as _f:
+    OWN_ORDER = int(re.search(r"kOwnOrder = (\d+)", _f.read())[1])
+
+
+@pytest.mark.parametrize("s,t,v,dt", [(6, 350, 20000, "bf16"), (6, 350, 20000, "fp16"), (70, 31, 50257, "fp32"), (6, 350, 151936, "bf16"), (2, 1200, 9001, "fp32")])
+def test_padded_batches_that_a_launch_puts_in_order(L, s, t, v, dt):  # noqa: F811
+    """More rows than CTAs put in order by themselves; rows of a slot, of several, of parts that are copied again."""
+    assert s * t > OWN_ORDER
+    z, y = _padded(s, t, v, dt, seed=s)
+    old, adv, ref = _policy_inputs(z, y)
+    flat, yy = z.view(-1, v), y.view(-1)
+    _near_logprobs(L.token_logprobs(z, y), flat, yy)
+    g = torch.randn((s, t), generator=_gen(7), device="cuda")
+    g[0, :5] = 0.0
+    _near_gradient(L.token_logprobs_backward(g, z, y), flat, yy, g.double().view(-1), torch.zeros_like(g).double().view(-1))
+    out = torch.full_like(z, 7.0)
+    _check_policy(L, z, y, old, adv, ref, kl=0.04, kind="sequence", out=out)
+    _check_preference(L, z, y, ref, average=True, out=out)
+    mine = z.clone()
+    _check_policy(L, mine, y, old, adv, ref, kl=0.04, out=mine)
+    _check_preference(L, z, y, ref, kind="squared", beta=0.3, out=z)
