@@ -16,9 +16,11 @@ the gradient on to the adapters, ``adapters.clip_gradients`` clips theirs.
 
 Logits are [..., vocab] (float32, bfloat16 or float16; rows may be strided), targets
 their leading shape (int32 or int64): row i's target is the token that its
-log-probability is taken of (next-token targets are shifted by the caller).  A
+log-probability is taken of.  Next-token targets are shifted by the caller, with
+the logits left whole (rows of ``logits[:, :-1]`` do not have one stride):
+``targets = torch.nn.functional.pad(ids[:, 1:], (0, 1), value=-100)``.  A
 target outside the vocabulary, such as -100, means that the row does not count: its
-log-probability is 0 and its gradient zeros, whatever its logits are.
+log-probability is 0 and its gradient zeros, whatever its logits are; it is not read.
 Log-probabilities are float32.  Sums are held in 32 bits, what is computed
 from a row's log-probability and sums over rows in 64; gradients are rounded once.
 A target whose logit is -inf has the log-probability -inf; a row with a NaN

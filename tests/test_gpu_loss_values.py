@@ -128,3 +128,28 @@ def test_policy_divergence_in_64_bits(L):  # noqa: F811
     want = torch.where(d.abs() < 2, want, torch.expm1(d) - d)
     zero = torch.zeros(len(d), device="cuda")
     _row_by_row(L, len(d), lambda at: dict(old_logprobs=None, advantages=zero[at], ref_logprobs=ref[at], kl=0.5), 0.5 * want, -0.5 * torch.expm1(d))
+
+
+# ---------------------------------------------------------------- targets shifted in place of sliced logits
+
+
+def test_next_token_targets(L):  # noqa: F811
+    """All of the logits with targets that are shifted, the last of each sequence -100, as against slices."""
+    s, t, v = 5, 19, 1003
+    z = (torch.randn((s, t, v), generator=_gen(8), device="cuda") * 3).bfloat16()
+    ids = torch.randint(0, v, (s, t), generator=_gen(9), device="cuda")
+    targets = torch.nn.functional.pad(ids[:, 1:], (0, 1), value=-100)
+    logp = L.token_logprobs(z, targets)
+    want = torch.log_softmax(z[:, :-1].double(), 2).gather(2, ids[:, 1:, None])[:, :, 0]
+    assert (logp[:, -1] == 0).all() and ((logp[:, :-1] - want).abs() <= 2.0 ** -17 * want.abs().clamp_min(1)).all()
+    adv = torch.randn((s,), generator=_gen(10), device="cuda")
+    cut = z[:, :-1].contiguous()
+    for kind in ("token", "sequence"):
+        loss, _, grad = L.policy_loss(z, targets, None, adv, reduction=kind)
+        less, _, part = L.policy_loss(cut, ids[:, 1:].contiguous(), None, adv, reduction=kind)
+        # the rows' offsets from 16 bytes differ, and with them the order of their sums
+        assert abs(loss - less) <= 2.0 ** -20 * less.abs().clamp_min(1)
+        assert (grad[:, -1] == 0).all() and ((grad[:, :-1] - part).abs() <= 2.0 ** -7 * part.abs() + 2.0 ** -30).all()
+    for call in (lambda: L.token_logprobs(z[:, :-1], targets[:, :-1].contiguous()), lambda: L.token_logprobs(cut, ids[:, 1:])):
+        with pytest.raises(ValueError, match="one stride|contiguous"):
+            call()
