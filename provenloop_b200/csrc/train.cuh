@@ -81,7 +81,7 @@ struct LossOut {
     const float* grad_scale;
 };
 
-// Whether k_order puts the rows in order first: those of persistent clusters, if they are more
+// Whether k_order puts the rows in order first: long ones of persistent clusters, if they are more
 // than the CTAs do by themselves.
 // both: a call that goes over them once without a gradient too.
 bool loss_orders(uint64_t n, uint32_t vocab, int dtype, bool grad, bool both);

@@ -44,9 +44,11 @@ with open(os.path.join(build.CSRC, "k_loss.cu")) as _f:
     OWN_ORDER = int(re.search(r"kOwnOrder = (\d+)", _f.read())[1])
 
 
-@pytest.mark.parametrize("s,t,v,dt", [(6, 350, 20000, "bf16"), (6, 350, 20000, "fp16"), (70, 31, 50257, "fp32"), (6, 350, 151936, "bf16"), (2, 1200, 9001, "fp32")])
+@pytest.mark.parametrize("s,t,v,dt", [(6, 350, 20000, "bf16"), (6, 350, 20000, "fp16"), (70, 31, 50257, "fp32"), (6, 350, 60001, "fp16"),
+                                      (6, 350, 151936, "bf16"), (30, 71, 70001, "fp32"), (2, 1200, 9001, "fp32")])
 def test_padded_batches_that_a_launch_puts_in_order(L, s, t, v, dt):  # noqa: F811
-    """More rows than CTAs put in order by themselves; rows of a slot, of several, of parts that are copied again."""
+    """More rows than CTAs put in order by themselves; rows of a slot, of several, of parts that are copied
+    again; short ones as they come, longer ones in order for gradients, the longest for all."""
     assert s * t > OWN_ORDER
     z, y = _padded(s, t, v, dt, seed=s)
     old, adv, ref = _policy_inputs(z, y)
