@@ -307,7 +307,7 @@ __device__ __forceinline__ double policy_term(const PolicyTerms& p, const RowInf
         const double e = __shfl_sync(0xffffffffu, own, 1) - 1.0;
         const double series = d * d * (1.0 / 2 + d * (1.0 / 6 + d * (1.0 / 24 + d * (1.0 / 120 + d * (1.0 / 720 + d * (1.0 / 5040 + d * (1.0 / 40320 + d / 362880)))))));
         const bool near = fabs(d) < 0.25;
-        term += p.kl * (near ? series : e - d);
+        term += p.kl * (near ? series : e == INFINITY ? e : e - d);  // d may be infinite too
         by -= p.kl * (near ? d + series : e);
     }
     *slope = by;

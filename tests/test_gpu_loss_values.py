@@ -130,6 +130,24 @@ def test_policy_divergence_in_64_bits(L):  # noqa: F811
     _row_by_row(L, len(d), lambda at: dict(old_logprobs=None, advantages=zero[at], ref_logprobs=ref[at], kl=0.5), 0.5 * want, -0.5 * torch.expm1(d))
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_policy_loss_of_masked_targets(L, dt):  # noqa: F811
+    """A target masked by -inf: the ratio is 0, or 1 without old log-probabilities; the KL term is infinite for a finite
+    reference, as its limit is, and finite slopes give finite gradients."""
+    n, v = 4, 300
+    z = torch.randn((n, v), generator=_gen(11), device="cuda").to(TYPES[dt])
+    y = torch.randint(0, v, (n,), generator=_gen(12), device="cuda")
+    z[1, y[1]] = -math.inf
+    adv, ref = torch.ones(n, device="cuda"), torch.full((n,), -2.0, device="cuda")
+    for old in (None, torch.full((n,), -6.0, device="cuda")):
+        loss, logp, grad = L.policy_loss(z, y, old, adv)
+        assert torch.isfinite(loss) and logp[1] == -math.inf and torch.isfinite(grad).all()
+        if old is not None:
+            assert (grad[1] == 0).all()
+        loss, logp, grad = L.policy_loss(z, y, old, adv, ref, kl=0.1)
+        assert loss == math.inf and torch.isfinite(grad[[0, 2, 3]]).all()
+
+
 # ---------------------------------------------------------------- targets shifted in place of sliced logits
 
 
