@@ -11,10 +11,11 @@
 // The bound is the logits' traffic: each is read once, and its gradient
 // written once.  Rows that fit are held in registers (k_rows, k_short), of longer ones a
 // persistent cluster keeps what it can in shared memory (k_ring).  On one B200, in bf16
-// over 151936 tokens: 4096 rows' log-probabilities take 197 us (6.3 TB/s), with gradients for
-// given slopes 525 to 543 us (4.7 TB/s; 5.9 with known statistics).  The latter is
-// bound by the two exponentials and some twenty instructions that an element costs: without
-// them the same copies take 370 us.  Tried and slower: exponentials kept in
+// over 151936 tokens: 4096 rows' log-probabilities take 197 to 205 us (6.1 to 6.3 TB/s), gradients for
+// given slopes 525 to 563 us (4.4 to 4.7 TB/s; 5.9 with known statistics).  Without an element's two exponentials
+// and some twenty instructions the same copies take 370 us; with them neither the issue slots (54 to 56 %)
+// nor the unit of exponentials (51 %) is at its limit: the rest is roles that wait for one another,
+// a row's gradient for its statistics first of all.  Tried and slower: exponentials kept in
 // shared memory in 32 bits (570 us: a row's gradient then waits for the next one's
 // statistics), a part of them by polynomials on the FMA pipe (586 us), bulk stores of the
 // gradient (750 us), more statistics warps and fewer for the gradient (600 us and more).
@@ -1106,13 +1107,13 @@ cudaError_t clusters_at_once(int cl, int* out) {
 // them takes for a row, fixed and by the KiB of a CTA's part.  Measured, in us
 // for 1500 rows on 1, 2, 4 and 8 CTAs, statistics and gradient:
 //   16-bit, vocabulary  20000:  45  60  78 149      151936: 211 214 227 329
-//   f32,                20000:  52  63  95 131      151936: 428 343 364 374
-// (24 rows of 151936: 27 19 15 15 and 37 23 17 15; statistics alone are
+//   f32,                20000:  57  68  96 129      151936: 427 357 384 408
+// (24 rows of 151936: 27 19 15 15 and 37 23 17 17; statistics alone are
 // fastest on one CTA from 300 rows on, on four for few.)  A part of more than
 // half of the slots overlaps less with the next row's.  What a part has beyond the
 // slots that it keeps is read again, and not always found in L2: 6144 rows of 151936, half of which
-// are only written, take 600 us on one CTA each and 506 on two; 1001 rows in f32, 623 of which count, 233 on
-// one, 216 on two and 183 on four.
+// are only written, take 576 to 600 us on one CTA each and 507 on two; 1001 rows in f32, 623 of which count, 232 on
+// one, 216 on two and 187 on four.
 template <class T, bool S, bool G>
 cudaError_t launch_ring(RowArgs a, bool dependent, cudaStream_t s) {
     using R = Roles<S, G>;

@@ -22,7 +22,8 @@ the logits left whole (rows of ``logits[:, :-1]`` do not have one stride):
 target outside the vocabulary, such as -100, means that the row does not count: its
 log-probability is 0 and its gradient zeros, whatever its logits are; it is not read.
 Log-probabilities are float32.  Sums are held in 32 bits, what is computed
-from a row's log-probability and sums over rows in 64; gradients are rounded once.
+from a row's log-probability and sums over rows in 64; gradients are rounded once, and
+probabilities below 2^-126 count as 0 in them.
 A target whose logit is -inf has the log-probability -inf; a row with a NaN
 or +inf has NaN.
 """
